@@ -93,7 +93,8 @@ enum { MOE_ROUTE_TOPK_SOFTMAX = 0, MOE_ROUTE_SOFTMAX_TOPK_RENORM = 1 };
 enum { MOE_ROUTER_D_E = 0, MOE_ROUTER_E_D = 1 }; /* router weight layout */
 
 /* device status bits */
-enum { MOE_STATUS_BAD_EXPERT_ID = 1, MOE_STATUS_ROW_OVERFLOW = 2, MOE_STATUS_TIMEOUT = 4 };
+enum { MOE_STATUS_BAD_EXPERT_ID = 1, MOE_STATUS_ROW_OVERFLOW = 2, MOE_STATUS_TIMEOUT = 4,
+       MOE_STATUS_BAD_PAGE = 8 };
 
 /* ---- library ------------------------------------------------------------ */
 
@@ -120,7 +121,8 @@ int moe_read_status(const void* workspace, int* status_out, moe_stream_t stream)
 enum {
   MOE_K_ROUTER = 0, MOE_K_ROUTER_SELECT, MOE_K_DISPATCH, MOE_K_PLAN, MOE_K_XPREP,
   MOE_K_GATEUP, MOE_K_DOWN, MOE_K_COMBINE, MOE_K_RMS_NORM, MOE_K_PACK, MOE_K_DEQUANT,
-  MOE_K_AUX, MOE_K_EP_SEND, MOE_K_EP_RECV, MOE_K_EP_RETURN, MOE_K_EP_WAIT, MOE_K_COUNT
+  MOE_K_AUX, MOE_K_EP_SEND, MOE_K_EP_RECV, MOE_K_EP_RETURN, MOE_K_EP_WAIT, MOE_K_ROPE_APPEND,
+  MOE_K_ATTENTION, MOE_K_LINEAR, MOE_K_COUNT
 };
 int moe_profile_enable(int on);
 int moe_profile_collect(float* ms, int* launches, int n);
@@ -380,6 +382,100 @@ int moe_ep_forward_phases(const moe_layer_weights* w, int W, int rank, void* con
                           void* window, const float* x, int T, float* out, const float* residual,
                           int epoch, int phases, void* workspace, size_t workspace_bytes,
                           moe_stream_t stream);
+
+/* ---- attention half of a decode step (no counterpart among the MoE calls) ---------
+ * Position rotation and append to a paged key-value cache, attention of one
+ * new token per sequence over that cache, and matrix-vector products with
+ * block-quantised weights (the q/k/v, output and vocabulary projections).
+ * Rows are f32, as in the MoE layer.
+ *
+ * A paged cache: `pages` pages of `page_size` token slots, each slot holding
+ * kv_heads vectors of head_dim keys (k) and as many values (v).  Element
+ * (page, slot, head, i) of either is at page * page_stride + slot *
+ * token_stride + head * head_stride + i (strides in elements; the stride of an
+ * axis of extent 1 is ignored), so both the token-major and the head-major
+ * layout of a page fit.  Token position p of sequence s is in page
+ * block_table[s * table_stride + p / page_size], slot p % page_size; entries
+ * behind a sequence's last page are never read.  Bases and strides must be
+ * multiples of 16 bytes; head_dim a multiple of 8 (16 for MOE_CACHE_E4M3), at
+ * most 256.  MOE_CACHE_E4M3 holds value / scale, rounded to nearest even and
+ * saturated at +-448; the scales of the other types must be 1.
+ * A page id outside [0, pages) sets MOE_STATUS_BAD_PAGE; its slots are neither
+ * read nor written. */
+enum { MOE_CACHE_F16 = 0, MOE_CACHE_BF16 = 1, MOE_CACHE_E4M3 = 2 };
+
+typedef struct moe_paged_cache {
+  void* k;
+  void* v;
+  const int32_t* block_table; /* (seqs, table_width) */
+  int64_t page_stride, token_stride, head_stride;
+  int64_t table_stride;
+  int dtype; /* MOE_CACHE_* */
+  int pages, page_size, kv_heads, head_dim;
+  int seqs, table_width;
+  float k_scale, v_scale;
+} moe_paged_cache;
+
+/* Rotates q and k by their positions, writes the rotated q to q_out and the
+ * rotated k and the v of every token into the cache.
+ *   q (T, q_heads, head_dim), k, v (T, kv_heads, head_dim) f32; row t, head h
+ *          at t * tok_stride + h * head_stride.  q_heads 0: no q
+ *   positions (T,) int32; a token with a negative position is skipped (its
+ *          q_out row is left as it was).  No two tokens of a call may have
+ *          the same sequence and position
+ *   seq_ids (T,) int32, or NULL: token t belongs to sequence t
+ *   inv_freq (rot / 2,) f64: pair i turns by the angle position * inv_freq[i],
+ *          formed in 64 bits.  Pairs are (i, i + rot / 2), or (2i, 2i + 1)
+ *          with interleaved != 0; elements from rot on are copied.  rot 0: no
+ *          rotation (inv_freq unused)
+ *   q_out  same shape as q, may be q itself with the same strides; must not
+ *          overlap k or v
+ *   status int32 that receives MOE_STATUS_BAD_PAGE (also for a sequence id
+ *          outside [0, seqs)), or NULL */
+int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_stride,
+                    int64_t q_head_stride, const float* k, int64_t k_tok_stride,
+                    int64_t k_head_stride, const float* v, int64_t v_tok_stride,
+                    int64_t v_head_stride, int T, int q_heads, const int32_t* positions,
+                    const int32_t* seq_ids, const double* inv_freq, int rot, int interleaved,
+                    float* q_out, int64_t qo_tok_stride, int64_t qo_head_stride, int32_t* status,
+                    moe_stream_t stream);
+
+int moe_paged_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int head_dim,
+                                        size_t* bytes);
+
+/* Attention of one token per sequence over the cache:
+ *   s_j = scale * q . k_j for the keys j in [max(0, len - window), len)
+ *   (window 0 = all of them), softcap * tanh(s_j / softcap) if softcap > 0;
+ *   out = sum_j softmax(s)_j v_j, lse = ln sum_j exp(s_j).
+ * Query head h reads key head h / (q_heads / kv_heads).
+ *   q (seqs, q_heads, head_dim) f32, sequence s, head h at s * q_seq_stride +
+ *          h * q_head_stride
+ *   seq_lens (seqs,) int32, the new token included; 0 or less gives zeros in
+ *          out and -inf in lse.  More than table_width * page_size sets
+ *          MOE_STATUS_BAD_PAGE and counts as that many
+ *   max_len no sequence is longer (0 = table_width * page_size); it sizes the
+ *          launch, a longer sequence is still computed in full
+ *   out (seqs, q_heads, head_dim) f32 contiguous; lse (seqs, q_heads) or NULL
+ *   workspace: zeroed by the caller before its first use and then kept between
+ *          calls, which leave it ready for the next one (but for the status
+ *          word at its start); calls that may overlap need one each
+ * The split of a sequence over the GPU depends on the lengths and the device
+ * alone, and its parts are joined in a fixed order: equal calls give equal bits. */
+int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_seq_stride,
+                        int64_t q_head_stride, const int32_t* seq_lens, int q_heads, int max_len,
+                        int window, float scale, float softcap, float* out, float* lse,
+                        void* workspace, size_t workspace_bytes, moe_stream_t stream);
+
+/* y[t] = W x[t] (+ residual[t]) for T rows, f32 accumulate.
+ *   w: a Q4_0 or Q8_0 matrix of `rows` x `cols`, cols a multiple of 32, padded
+ *      with zero blocks to rows % 16 == 0 and cols % 64 == 0 and packed by
+ *      moe_pack_weights
+ *   x (T, cols), y (T, rows), residual (T, rows) or NULL: rows at the given
+ *      strides (elements); residual may be y itself with the same stride
+ * Made for a few rows: the weights are read once for every 16 of them. */
+int moe_linear(const uint8_t* w, int qtype, int rows, int cols, const float* x, int64_t x_stride,
+               int T, const float* residual, int64_t residual_stride, float* y, int64_t y_stride,
+               moe_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,10 @@ Modules:
   engine       the reference engines' MoE calls served by the layer
   ep           expert parallelism over NVLink peer memory (IPC exchange
                windows, device-side send / serve / combine)
-  stacked      stacked decode step (MoE layers + shared expert + RMSNorm)
+  attention    attention half of a decode step: paged key-value cache, rotary
+               append, single-token attention, Q4_0 / Q8_0 projections
+  stacked      stacked decode step (MoE layers + shared expert + RMSNorm,
+               with attention layers where given)
   synth        seeded synthetic workloads as raw GGUF block bytes
   build        nvcc build of the library
 """

@@ -36,6 +36,9 @@ MOE_ROUTER_E_D = 1
 MOE_STATUS_BAD_EXPERT_ID = 1
 MOE_STATUS_ROW_OVERFLOW = 2
 MOE_STATUS_TIMEOUT = 4
+MOE_STATUS_BAD_PAGE = 8
+
+MOE_CACHE_F16, MOE_CACHE_BF16, MOE_CACHE_E4M3 = 0, 1, 2
 
 vp = ctypes.c_void_p
 ci = ctypes.c_int
@@ -58,6 +61,17 @@ class MoELayerWeights(ctypes.Structure):
         ("router_layout", ci), ("qtype", ci), ("shared_qtype", ci),
         ("E", ci), ("k", ci), ("d", ci), ("F", ci), ("Fs", ci), ("mode", ci),
         ("opts", ctypes.POINTER(MoEExpertOpts)),
+    ]
+
+
+class MoEPagedCache(ctypes.Structure):
+    """Mirror of ``moe_paged_cache``."""
+    _fields_ = [
+        ("k", vp), ("v", vp), ("block_table", vp),
+        ("page_stride", ci64), ("token_stride", ci64), ("head_stride", ci64),
+        ("table_stride", ci64), ("dtype", ci), ("pages", ci), ("page_size", ci),
+        ("kv_heads", ci), ("head_dim", ci), ("seqs", ci), ("table_width", ci),
+        ("k_scale", cf), ("v_scale", cf),
     ]
 
 
@@ -101,12 +115,18 @@ SIGNATURES = {
     "moe_ep_forward_phases": [vp, ci, ci, vp, vp, vp, ci, vp, vp, ci, ci, vp, csz, vp],
     "moe_layer_workspace_bytes": [ctypes.POINTER(MoELayerWeights), ci, ctypes.POINTER(csz)],
     "moe_layer_forward": [ctypes.POINTER(MoELayerWeights), vp, ci, vp, vp, vp, vp, vp, csz, vp],
+    "moe_rope_append": [ctypes.POINTER(MoEPagedCache), vp, ci64, ci64, vp, ci64, ci64, vp, ci64,
+                        ci64, ci, ci, vp, vp, vp, ci, ci, vp, ci64, ci64, vp, vp],
+    "moe_paged_attention_workspace_bytes": [ci, ci, ci, ci, ctypes.POINTER(csz)],
+    "moe_paged_attention": [ctypes.POINTER(MoEPagedCache), vp, ci64, ci64, vp, ci, ci, ci, cf, cf,
+                            vp, vp, vp, csz, vp],
+    "moe_linear": [vp, ci, ci, ci, vp, ci64, ci, vp, ci64, vp, ci64, vp],
 }
 
 
 KERNEL_NAMES = ["router", "router_select", "dispatch", "plan", "xprep", "gateup", "down",
                 "combine", "rms_norm", "pack", "dequant", "aux", "ep_send", "ep_recv_plan",
-                "ep_return", "ep_wait"]
+                "ep_return", "ep_wait", "rope_append", "attention", "linear"]
 
 MOE_EP_PHASE_SEND = 1
 MOE_EP_PHASE_SERVE = 2

@@ -26,6 +26,7 @@ KERNELS_AUTO = _lib.MOE_KERNELS_AUTO
 KERNELS_GEMV = _lib.MOE_KERNELS_GEMV
 KERNELS_BLOCKSCALE = _lib.MOE_KERNELS_BLOCKSCALE
 KERNELS_SPLIT_GEMM = _lib.MOE_KERNELS_SPLIT_GEMM
+STATUS_BAD_PAGE = _lib.MOE_STATUS_BAD_PAGE
 # GGML type -> (weights per block, bytes per block), dequant_fast.py:723-754
 BLOCK_GEOMETRY = {QTYPE_F32: (1, 4), QTYPE_Q4_0: (32, 18), QTYPE_Q5_1: (32, 24),
                   QTYPE_Q8_0: (32, 34), QTYPE_Q4_K: (256, 144), QTYPE_Q6_K: (256, 210)}
@@ -255,6 +256,230 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
         out = torch.empty_like(x)
     call("moe_rms_norm_ex", _ptr(x), _ptr(weight), ctypes.c_float(eps), 1 if gemma_style else 0,
          T, d, _ptr(out), _stream())
+    return out
+
+
+# --------------------------------------------------------------------------- attention half
+
+CACHE_TYPES = {torch.float16: _lib.MOE_CACHE_F16, torch.bfloat16: _lib.MOE_CACHE_BF16,
+               torch.float8_e4m3fn: _lib.MOE_CACHE_E4M3}
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """The entry point on ``device`` and its current stream, whichever device
+    is current."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, _stream())
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, _stream())
+
+
+def _rows_f32(t: torch.Tensor, name: str, device, shape=None) -> torch.Tensor:
+    """A CUDA f32 tensor whose last axis is contiguous; other axes may stride."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} must be {torch.float32}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} is {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"the last axis of {name} must be contiguous")
+    return t
+
+
+def _i32(t: torch.Tensor, name: str, device, n: Optional[int] = None) -> torch.Tensor:
+    _need(t, torch.int32, name)
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if n is not None and (t.dim() != 1 or t.shape[0] != n):
+        raise ValueError(f"{name} is {tuple(t.shape)}, expected ({n},)")
+    return t
+
+
+def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                 k_scale: float, v_scale: float) -> _lib.MoEPagedCache:
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise TypeError(f"{n} must be a CUDA tensor")
+    dtype = CACHE_TYPES.get(k_cache.dtype)
+    if dtype is None or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"caches of {k_cache.dtype} and {v_cache.dtype}: both must be one of "
+                        f"{', '.join(str(t) for t in CACHE_TYPES)}")
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != strides:
+        raise ValueError("k_cache and v_cache must be (pages, page_size, kv_heads, head_dim) of "
+                         "the same shape and strides")
+    if strides[3] != 1 and shape[3] > 1:
+        raise ValueError("the last axis of the caches must be contiguous")
+    for t, n in ((v_cache, "v_cache"), (block_table, "block_table")):
+        if t.device != k_cache.device:
+            raise ValueError(f"{n} is on {t.device}, expected {k_cache.device}")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (
+            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be int32 (sequences, pages of a sequence) with "
+                         "contiguous rows")
+    return _lib.MoEPagedCache(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                              strides[0], strides[1], strides[2], block_table.stride(0), dtype,
+                              shape[0], shape[1], shape[2], shape[3], block_table.shape[0],
+                              block_table.shape[1], k_scale, v_scale)
+
+
+def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                positions: torch.Tensor, inv_freq: Optional[torch.Tensor] = None,
+                seq_ids: Optional[torch.Tensor] = None, interleaved: bool = False,
+                k_scale: float = 1.0, v_scale: float = 1.0, q_out: Optional[torch.Tensor] = None,
+                status: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Rotates q (T, q_heads, head_dim) and k (T, kv_heads, head_dim) by their
+    positions, writes k and v into the paged caches (pages, page_size,
+    kv_heads, head_dim; any page layout as a view) and returns the rotated q
+    (``q_out``, which may be q itself).
+
+    ``inv_freq`` (rot / 2,) f64 holds the angle of each pair per position
+    (``rope_inv_freq``); None rotates nothing.  Pairs are (i, i + rot / 2), or
+    adjacent with ``interleaved``.  ``seq_ids`` maps tokens to rows of
+    ``block_table`` (None: token t is sequence t); a negative position skips
+    its token, q row included; no two tokens may share sequence and position.
+    ``status`` (int32) receives STATUS_BAD_PAGE for a page or sequence that
+    does not exist; such a token's k and v are not stored."""
+    c = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
+    dev = k_cache.device
+    T = k.shape[0]
+    _rows_f32(k, "k", dev, (T, c.kv_heads, c.head_dim))
+    _rows_f32(v, "v", dev, (T, c.kv_heads, c.head_dim))
+    _i32(positions, "positions", dev, T)
+    if seq_ids is not None:
+        _i32(seq_ids, "seq_ids", dev, T)
+    if status is not None:
+        _i32(status, "status", dev)
+    rot = 0
+    if inv_freq is not None:
+        _need(inv_freq, torch.float64, "inv_freq")
+        if inv_freq.device != dev:
+            raise ValueError(f"inv_freq is on {inv_freq.device}, expected {dev}")
+        rot = 2 * inv_freq.numel()
+    hq, qs, os_ = 0, (0, 0), (0, 0)
+    if q is not None:
+        if q.dim() != 3:
+            raise ValueError("q must be (tokens, q_heads, head_dim)")
+        hq = q.shape[1]
+        _rows_f32(q, "q", dev, (T, hq, c.head_dim))
+        if q_out is None:
+            q_out = torch.empty((T, hq, c.head_dim), dtype=torch.float32, device=dev)
+        else:
+            _rows_f32(q_out, "q_out", dev, (T, hq, c.head_dim))
+        qs, os_ = q.stride(), q_out.stride()
+    _call_on(dev, "moe_rope_append", ctypes.byref(c), _ptr(q), qs[0], qs[1], _ptr(k), k.stride(0),
+             k.stride(1), _ptr(v), v.stride(0), v.stride(1), T, hq, _ptr(positions),
+             _ptr(seq_ids), _ptr(inv_freq), rot, 1 if interleaved else 0, _ptr(q_out), os_[0],
+             os_[1], _ptr(status))
+    return q_out
+
+
+def rope_inv_freq(rot: int, base: float = 10000.0, factors: Optional[torch.Tensor] = None,
+                  device=None) -> torch.Tensor:
+    """(rot / 2,) f64 angles per position, base ** (-2 i / rot), divided by
+    ``factors`` (a GGUF ``rope_freqs`` tensor) if given."""
+    if rot <= 0 or rot % 2:
+        raise ValueError(f"rot {rot} must be even and positive")
+    f = float(base) ** (-2.0 * torch.arange(rot // 2, dtype=torch.float64) / rot)
+    if factors is not None:
+        if factors.numel() != rot // 2:
+            raise ValueError(f"{factors.numel()} factors for {rot // 2} pairs")
+        f = f / factors.detach().to("cpu", torch.float64).reshape(-1)
+    return f.to(device if device is not None else torch.device("cuda"))
+
+
+def paged_attention_workspace(seqs: int, q_heads: int, kv_heads: int, head_dim: int,
+                              device) -> torch.Tensor:
+    """A workspace for ``paged_attention`` calls of these sizes that follow one
+    another (calls that may overlap need one each)."""
+    n = _size_out("moe_paged_attention_workspace_bytes", seqs, q_heads, kv_heads, head_dim)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_table: torch.Tensor, seq_lens: torch.Tensor,
+                    scale: Optional[float] = None, window: int = 0, softcap: float = 0.0,
+                    k_scale: float = 1.0, v_scale: float = 1.0, max_len: int = 0,
+                    out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                    ws: Optional[torch.Tensor] = None):
+    """Attention of one new token per sequence, q (seqs, q_heads, head_dim),
+    over the first ``seq_lens[s]`` tokens of its pages (the last ``window`` of
+    them if given): softmax(scale q.k, capped at ``softcap``) v, f32.  Returns
+    out, or (out, lse) with the natural log of the softmax sums; a sequence of
+    length 0 gives zeros and -inf.  ``scale`` defaults to 1 / sqrt(head_dim);
+    ``max_len`` (no sequence is longer; 0 = what the table holds) sizes the
+    launch.  ``ws`` comes from ``paged_attention_workspace``."""
+    c = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
+    dev = k_cache.device
+    if q.dim() != 3:
+        raise ValueError("q must be (sequences, q_heads, head_dim)")
+    hq = q.shape[1]
+    shape = (c.seqs, hq, c.head_dim)
+    _rows_f32(q, "q", dev, shape)
+    _i32(seq_lens, "seq_lens", dev, c.seqs)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=dev)
+    elif _need(out, torch.float32, "out").shape != shape or out.device != dev:
+        raise ValueError(f"out is {tuple(out.shape)} on {out.device}, expected {shape} on {dev}")
+    lse = torch.empty((c.seqs, hq), dtype=torch.float32, device=dev) if return_lse else None
+    if ws is None:
+        ws = paged_attention_workspace(c.seqs, hq, c.kv_heads, c.head_dim, dev)
+    elif _need(ws, torch.uint8, "ws").device != dev:
+        raise ValueError(f"ws is on {ws.device}, expected {dev}")
+    _call_on(dev, "moe_paged_attention", ctypes.byref(c), _ptr(q), q.stride(0), q.stride(1),
+             _ptr(seq_lens), hq, max_len, window,
+             c.head_dim ** -0.5 if scale is None else scale, softcap, _ptr(out), _ptr(lse),
+             _ptr(ws), ws.numel())
+    return (out, lse) if return_lse else out
+
+
+class LinearWeights:
+    """A Q4_0 or Q8_0 matrix (rows, cols) for ``linear``: raw GGUF blocks on
+    the device, padded to whole tiles and packed once."""
+
+    def __init__(self, raw: torch.Tensor, qtype: int, rows: int, cols: int):
+        if qtype not in PACKED_QTYPES:
+            raise ValueError(f"unsupported GGML type {qtype} (Q4_0 = 2, Q8_0 = 8)")
+        if rows <= 0 or cols <= 0:
+            raise ValueError(f"bad shape ({rows}, {cols})")
+        _need(raw, torch.uint8, "raw")
+        rb = row_bytes(qtype, cols)
+        if raw.numel() != rows * rb:
+            raise ValueError(f"raw blocks hold {raw.numel()} bytes, expected {rows * rb}")
+        self.qtype, self.rows, self.cols, self.device = qtype, rows, cols, raw.device
+        pr, pc = -rows % 16, -cols % 64
+        if pr or pc:
+            raw = torch.nn.functional.pad(raw.view(rows, rb), (0, pc // 32 * BLOCK_BYTES[qtype], 0,
+                                                               pr))
+        with torch.cuda.device(raw.device):
+            self.packed = pack_weights(raw, qtype, 1, rows + pr, cols + pc)
+
+
+def linear(x: torch.Tensor, w: LinearWeights, residual: Optional[torch.Tensor] = None,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x (T, cols) f32 -> (T, rows) f32: W x[t] (+ residual[t]) for a few rows.
+    Rows of x, residual and out may stride; out may be residual."""
+    dev = w.device
+    if x.dim() != 2:
+        raise ValueError("x must be (tokens, cols)")
+    T = x.shape[0]
+    _rows_f32(x, "x", dev, (T, w.cols))
+    if residual is not None:
+        _rows_f32(residual, "residual", dev, (T, w.rows))
+    if out is None:
+        out = torch.empty((T, w.rows), dtype=torch.float32, device=dev)
+    else:
+        _rows_f32(out, "out", dev, (T, w.rows))
+        if T > 1 and out.stride(0) < w.rows:
+            raise ValueError("rows of out overlap")
+    _call_on(dev, "moe_linear", _ptr(w.packed), w.qtype, w.rows, w.cols, _ptr(x), x.stride(0), T,
+             _ptr(residual), 0 if residual is None else residual.stride(0), _ptr(out),
+             out.stride(0))
     return out
 
 

@@ -1,6 +1,7 @@
 """Stacked decode step: L MoE layers, each with an always-on shared expert,
 with the residual and RMSNorm of MoETransformerModel._layer_forward
-(moe_forward.py:348-359): ``x = x + moe(rms_norm(x, w))``."""
+(moe_forward.py:348-359): ``x = x + moe(rms_norm(x, w))``, after ``x = x +
+attention(rms_norm(x, wa))`` where the stack has attention layers."""
 from __future__ import annotations
 
 from typing import List, Optional, Sequence
@@ -8,14 +9,28 @@ from typing import List, Optional, Sequence
 import torch
 
 from . import kernels as K
+from .attention import AttentionLayer, PagedKVCache
 from .moe_forward import MoELayer
 
 
 class StackedMoE:
-    def __init__(self, layers: Sequence[MoELayer], norms: Sequence[torch.Tensor], eps: float = 1e-6):
+    """``attention`` (an ``AttentionLayer`` per MoE layer) with
+    ``attention_norms`` makes whole decoder layers of the stack."""
+
+    def __init__(self, layers: Sequence[MoELayer], norms: Sequence[torch.Tensor], eps: float = 1e-6,
+                 attention: Optional[Sequence[AttentionLayer]] = None,
+                 attention_norms: Optional[Sequence[torch.Tensor]] = None):
         self.layers = list(layers)
         self.norms = list(norms)
         self.eps = eps
+        self.attention = list(attention) if attention is not None else None
+        self.attention_norms = list(attention_norms) if attention_norms is not None else None
+        if (self.attention is None) != (self.attention_norms is None):
+            raise ValueError("attention and attention_norms come together")
+        if self.attention is not None and not (
+                len(self.attention) == len(self.attention_norms) == len(self.layers)):
+            raise ValueError(f"{len(self.attention)} attention layers and "
+                             f"{len(self.attention_norms)} norms for {len(self.layers)} MoE layers")
         self._buf: Optional[torch.Tensor] = None
 
     @classmethod
@@ -36,17 +51,34 @@ class StackedMoE:
             norms.append(torch.from_numpy(data.norm_w).to(layer.router.device))
         return cls(layers, norms, eps)
 
-    def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None,
+                caches: Optional[Sequence[PagedKVCache]] = None,
+                positions: Optional[torch.Tensor] = None,
+                seq_lens: Optional[torch.Tensor] = None, max_len: int = 0) -> torch.Tensor:
         """x (T, d) f32 on the device -> (T, d).  The residual stream lives in
         ``out`` (allocated once if not given): the first layer adds x into it,
         later layers update it in place (the combine may write over its own
-        residual input), so a step allocates nothing after the first."""
+        residual input), so a step allocates nothing after the first.
+
+        With attention layers row t is the new token of sequence t:
+        ``caches`` (one per layer), ``positions`` and ``seq_lens`` as
+        ``AttentionLayer.forward`` takes them."""
         if self._buf is None or self._buf.shape != x.shape:
             self._buf = torch.empty_like(x)
+        if self.attention is not None:
+            if caches is None or positions is None or seq_lens is None:
+                raise ValueError("attention layers need caches, positions and seq_lens")
+            if len(caches) != len(self.layers):
+                raise ValueError(f"{len(caches)} caches for {len(self.layers)} layers")
         xn = self._buf
         res = out if out is not None else torch.empty_like(x)
         cur = x
-        for layer, nw in zip(self.layers, self.norms):
+        for i, (layer, nw) in enumerate(zip(self.layers, self.norms)):
+            if self.attention is not None:
+                K.rms_norm(cur, self.attention_norms[i], self.eps, out=xn)
+                self.attention[i].forward(xn, caches[i], positions, seq_lens, residual=cur,
+                                          out=res, max_len=max_len)
+                cur = res
             K.rms_norm(cur, nw, self.eps, out=xn)
             layer.forward_batch(xn, residual=cur, out=res)
             cur = res

@@ -1,0 +1,183 @@
+"""Host side of the attention half: refusals of the C entries before any
+device work, the ctypes mirror of the cache, the page bookkeeping."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+from linuxnightmaresuite_b200 import _lib, kernels as K
+from linuxnightmaresuite_b200.attention import PagedKVCache
+
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include",
+                      "moe_b200.h")
+P = ctypes.c_void_p(256)      # an aligned address that no refused call follows
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from linuxnightmaresuite_b200 import build
+    build.build()
+    return _lib.load()
+
+
+def cache(**kw):
+    a = dict(k=256, v=256, block_table=256, page_stride=16 * 2 * 64, token_stride=2 * 64,
+             head_stride=64, table_stride=8, dtype=0, pages=10, page_size=16, kv_heads=2,
+             head_dim=64, seqs=4, table_width=8, k_scale=1.0, v_scale=1.0)
+    a.update(kw)
+    return _lib.MoEPagedCache(**a)
+
+
+def test_cache_mirror_matches_header():
+    src = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    body = re.search(r"typedef struct moe_paged_cache \{(.*?)\} moe_paged_cache;", src, re.S)
+    fields = []
+    for line in body.group(1).split(";"):
+        names = re.sub(r"^\s*(const\s+)?(void|int32_t|int64_t|int|float)\b", "", line).strip()
+        fields += [n.strip(" *") for n in names.split(",") if n.strip()]
+    assert fields == [f[0] for f in _lib.MoEPagedCache._fields_]
+    enum = re.search(r"enum \{ (MOE_CACHE_F16[^}]*)\}", src, re.S).group(1)
+    for name, value in re.findall(r"(MOE_CACHE_\w+)\s*=\s*(\d+)", enum):
+        assert getattr(_lib, name) == int(value)
+    bits = re.search(r"enum \{ (MOE_STATUS_BAD_EXPERT_ID[^}]*)\}", src, re.S).group(1)
+    for name, value in re.findall(r"(MOE_STATUS_\w+)\s*=\s*(\d+)", bits):
+        assert getattr(_lib, name) == int(value)
+    kinds = re.search(r"enum \{\s*MOE_K_ROUTER(.*?)MOE_K_COUNT", src, re.S).group(0)
+    assert len(re.findall(r"MOE_K_\w+", kinds)) - 1 == len(_lib.KERNEL_NAMES)
+
+
+BAD_CACHES = [
+    (dict(dtype=3), "UNSUPPORTED", "cache type"),
+    (dict(k=0), "INVALID", "null"),
+    (dict(block_table=0), "INVALID", "null"),
+    (dict(pages=0), "INVALID", "shape"),
+    (dict(page_size=0), "INVALID", "shape"),
+    (dict(kv_heads=0), "INVALID", "shape"),
+    (dict(seqs=-1), "INVALID", "shape"),
+    (dict(table_width=0), "INVALID", "shape"),
+    (dict(table_width=1 << 28), "UNSUPPORTED", "longer than"),
+    (dict(head_dim=0), "UNSUPPORTED", "head_dim"),
+    (dict(head_dim=60), "UNSUPPORTED", "head_dim"),
+    (dict(head_dim=264), "UNSUPPORTED", "head_dim"),
+    (dict(dtype=2, head_dim=72), "UNSUPPORTED", "head_dim"),
+    (dict(k=264), "INVALID", "16 bytes"),
+    (dict(token_stride=132), "INVALID", "16 bytes"),
+    (dict(page_stride=-2048), "INVALID", "negative"),
+    (dict(k_scale=0.5), "INVALID", "scales"),
+    (dict(dtype=2, k_scale=0.0), "INVALID", "scales"),
+    (dict(dtype=2, v_scale=float("nan")), "INVALID", "scales"),
+]
+
+
+def attention(lib, c, q=P, lens=P, hq=4, max_len=0, window=0, scale=0.1, cap=0.0, out=P, ws=P,
+              nbytes=1 << 26):
+    return lib.moe_paged_attention(ctypes.byref(c), q, 256, 64, lens, hq, max_len, window, scale,
+                                   cap, out, None, ws, nbytes, None)
+
+
+def append(lib, c, q=P, k=P, v=P, T=2, hq=4, pos=P, seq=None, freq=P, rot=64, q_out=P):
+    return lib.moe_rope_append(ctypes.byref(c), q, 256, 64, k, 128, 64, v, 128, 64, T, hq, pos,
+                               seq, freq, rot, 0, q_out, 256, 64, None, None)
+
+
+@pytest.mark.parametrize("change,status,words", BAD_CACHES)
+def test_bad_caches_are_refused(lib, change, status, words):
+    c = cache(**change)
+    for call in (attention, append):
+        assert call(lib, c) == getattr(_lib, "MOE_ERR_" + status)
+        assert words in _lib.last_error()
+
+
+def test_bad_attention_arguments_are_refused(lib):
+    c = cache()
+    for kw, status in ((dict(hq=0), "INVALID"), (dict(hq=5), "INVALID"),
+                       (dict(max_len=-1), "INVALID"), (dict(window=-1), "INVALID"),
+                       (dict(cap=-1.0), "INVALID"), (dict(cap=float("inf")), "INVALID"),
+                       (dict(scale=float("nan")), "INVALID"), (dict(q=None), "INVALID"),
+                       (dict(lens=None), "INVALID"), (dict(out=None), "INVALID"),
+                       (dict(ws=None), "INVALID"), (dict(nbytes=16), "WORKSPACE")):
+        assert attention(lib, c, **kw) == getattr(_lib, "MOE_ERR_" + status), kw
+    assert attention(lib, cache(seqs=0), q=None) == _lib.MOE_OK       # nothing to do
+    assert lib.moe_paged_attention(None, P, 1, 1, P, 4, 0, 0, 0.1, 0.0, P, None, P, 1 << 26,
+                                   None) == _lib.MOE_ERR_INVALID
+    n = ctypes.c_size_t()
+    assert lib.moe_paged_attention_workspace_bytes(4, 4, 2, 64, ctypes.byref(n)) == _lib.MOE_OK
+    assert n.value >= 256
+    for bad in ((-1, 4, 2, 64), (4, 5, 2, 64), (4, 4, 0, 64), (4, 4, 2, 257)):
+        assert lib.moe_paged_attention_workspace_bytes(*bad, ctypes.byref(n)) == \
+            _lib.MOE_ERR_INVALID
+
+
+def test_bad_append_arguments_are_refused(lib):
+    c = cache()
+    for kw in (dict(T=-1), dict(hq=-1), dict(rot=3), dict(rot=66), dict(rot=-2), dict(k=None),
+               dict(v=None), dict(pos=None), dict(freq=None), dict(q=None), dict(q_out=None),
+               dict(T=5)):
+        assert append(lib, c, **kw) == _lib.MOE_ERR_INVALID, kw
+    assert append(lib, c, T=0, k=None) == _lib.MOE_OK
+    assert lib.moe_rope_append(None, P, 1, 1, P, 1, 1, P, 1, 1, 1, 1, P, None, P, 64, 0, P, 1, 1,
+                               None, None) == _lib.MOE_ERR_INVALID
+
+
+def test_bad_linear_arguments_are_refused(lib):
+    def lin(w=P, qt=2, rows=64, cols=64, x=P, T=1, y=P):
+        return lib.moe_linear(w, qt, rows, cols, x, 64, T, None, 0, y, 64, None)
+    for kw, status in ((dict(qt=12), "UNSUPPORTED"), (dict(cols=48), "UNSUPPORTED"),
+                       (dict(rows=0), "INVALID"), (dict(cols=0), "INVALID"),
+                       (dict(T=-1), "INVALID"), (dict(w=None), "INVALID"),
+                       (dict(x=None), "INVALID"), (dict(y=None), "INVALID"),
+                       (dict(w=ctypes.c_void_p(264)), "INVALID")):
+        assert lin(**kw) == getattr(_lib, "MOE_ERR_" + status), kw
+    assert lin(T=0, x=None) == _lib.MOE_OK
+
+
+def test_wrappers_refuse_host_tensors():
+    k = torch.zeros((2, 4, 1, 64), dtype=torch.float16)
+    t = torch.zeros((1, 2), dtype=torch.int32)
+    with pytest.raises(TypeError, match="CUDA"):
+        K.paged_attention(torch.zeros(1, 2, 64), k, k, t, t[0, :1])
+    with pytest.raises(TypeError, match="CUDA"):
+        K.rope_append(None, k[:, 0], k[:, 0], k, k, t, t[0, :1])
+    with pytest.raises(TypeError, match="CUDA"):
+        K.LinearWeights(torch.zeros(18, dtype=torch.uint8), 2, 1, 32)
+    with pytest.raises(ValueError):
+        K.rope_inv_freq(7)
+    f = K.rope_inv_freq(8, 10000.0, torch.tensor([1.0, 1.0, 2.0, 4.0]), device="cpu")
+    assert f.dtype == torch.float64
+    assert torch.allclose(f, torch.tensor([1.0, 0.1, 0.005, 0.00025], dtype=torch.float64))
+
+
+def test_pages_are_handed_out_and_come_back():
+    c = PagedKVCache(6, 4, 2, 16, max_seqs=3, max_pages_per_seq=4, device="cpu")
+    address = c.block_table.data_ptr()
+    c.reserve(0, 1)
+    c.reserve(0, 4)
+    assert c.free_pages == 5
+    c.reserve(0, 5)
+    c.reserve(2, 16)
+    assert c.free_pages == 0
+    held = c.block_table[0, :2].tolist() + c.block_table[2].tolist()
+    assert sorted(held) == list(range(6))
+    assert (c.block_table[1] == -1).all() and (c.block_table[0, 2:] == -1).all()
+    with pytest.raises(RuntimeError, match="full"):
+        c.reserve(1, 1)
+    with pytest.raises(ValueError, match="at most 4"):
+        c.reserve(2, 17)
+    with pytest.raises(IndexError):
+        c.reserve(3, 1)
+    c.release(2)
+    assert c.free_pages == 4 and (c.block_table[2] == -1).all()
+    c.reserve(1, 16)
+    assert c.free_pages == 0
+    assert sorted(c.block_table[0, :2].tolist() + c.block_table[1].tolist()) == list(range(6))
+    c.reserve(1, 0)
+    c.reserve(1, -3)
+    assert c.block_table.data_ptr() == address
+    with pytest.raises(TypeError):
+        PagedKVCache(1, 1, 1, 16, 1, dtype=torch.float32, device="cpu")
+    with pytest.raises(ValueError):
+        PagedKVCache(0, 1, 1, 16, 1, device="cpu")
+    e = PagedKVCache(2, 4, 1, 16, 1, dtype=torch.float8_e4m3fn, device="cpu")
+    assert e.k.view(torch.uint8).sum() == 0
