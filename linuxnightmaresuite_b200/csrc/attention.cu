@@ -1,14 +1,48 @@
-// Attention of one new token per sequence over a paged cache.
+// Attention of one new token per sequence over a paged cache, in one launch.
 //
-// First form: one CTA per (sequence, query head), four warps taking keys in
-// turn, each with its own running maximum and sum; joined in shared memory.
+//   s_j = scale q.k_j,  o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
+//
+// Keys and values are read once and each meets the 1..8 query heads that share
+// them, so the bound is memory; the arithmetic goes to mma.sync (m16n8k16): a
+// CUDA-core form needs 2 FMAs per head and element and would be issue-bound
+// from 4 heads on, and a tcgen05 tile (64 rows at least) would be mostly
+// padding.
+//
+// Work.  A unit is one (sequence, key head, group of up to 8 query heads); it
+// is cut into rounds of NW * KEYS keys, and the rounds of all units, in order,
+// are dealt out in equal contiguous runs to the CTAs of one resident grid,
+// whatever the lengths: every CTA streams the same number of keys.  Each CTA
+// finds its run by a scan of the lengths, so one captured launch serves every
+// later length.  A unit that ends up in several CTAs is joined by the last of
+// them to finish, from f32 partials in the workspace, in the order of its
+// keys; the arrival counters return to zero.
+//
+// A warp takes every NW-th tile of KEYS keys through a ring of its own
+// (cp.async, 16 bytes at a time, rows swizzled so that ldmatrix meets no bank
+// twice); the warps meet only at the end of a unit.  Page ids are fetched one
+// tile ahead of the rows they lead to.
+//
+// Precision.  q has f32 rows, so it enters the products in parts: hi + lo fp16
+// (22 bits) for fp16 and e4m3 caches, three bf16 parts for bf16 caches.  With
+// at most 8 heads per 16-row operand the rows below them are free: row g holds
+// the hi part of head g, row g + 8 the lo part, and the two results, which meet
+// in one thread, are added.  Probabilities are split the same way (times 2^14
+// first, which keeps the lo part of small ones above fp16's range end).  The
+// tensor core truncates where it adds, so no accumulator takes more than four
+// k16 steps; from there on sums are f32 adds.
 #include <math.h>
+
+#include <algorithm>
+#include <atomic>
 
 #include "paged_cache.cuh"
 
 namespace moe {
 
-constexpr int kAttWarps = 4;
+constexpr int kAttHeads = 8;          // query heads of a unit at most
+constexpr int kAttMaxCtasPerSm = 2;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 struct AttArgs {
   moe_paged_cache c;
@@ -17,76 +51,606 @@ struct AttArgs {
   const int32_t* seq_lens;
   float *out, *lse;
   int* status;
+  int* arrivals;                      // one per CTA
+  float2* part_ml;                    // [2 * grid][kAttHeads] (maximum, sum)
+  float* part_o;                      // [2 * grid][kAttHeads][DP]
   int hq, window;
   float scale, cap;
 };
 
-template <int DT>
-__global__ void __launch_bounds__(kAttWarps * 32) attention_kernel(const AttArgs A) {
-  using T = typename CacheType<DT>::T;
-  __shared__ float sm[kAttWarps], sl[kAttWarps], so[kAttWarps][kMaxHeadDim];
+// ---------------------------------------------------------------------------
+// fragments
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool BF>
+__device__ __forceinline__ void mma_acc(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// two adjacent values -> NP packed parts that add up to them (22 bits of fp16,
+// 24 of bf16); the lower value sits in the lower half
+template <bool BF, int NP>
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&r)[NP]) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    if (BF) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      r[i] = *reinterpret_cast<const uint32_t*>(&h);
+      x -= __low2float(h);
+      y -= __high2float(h);
+    } else {
+      const __half2 h = __floats2half2_rn(x, y);
+      r[i] = *reinterpret_cast<const uint32_t*>(&h);
+      x -= __low2float(h);
+      y -= __high2float(h);
+    }
+  }
+}
+
+// e4m3 pair (low 16 bits) -> fp16x2, exact
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t v) {
+  uint32_t r;
+  asm("{\n .reg .b16 l;\n cvt.u16.u32 l, %1;\n cvt.rn.f16x2.e4m3x2 %0, l;\n}" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// A operand of one k16 step: one 16-row tile of {hi rows, lo rows}; bf16 has a
+// second tile {third part, zero} that goes into the same accumulators.
+template <bool BF> struct AFrag {
+  static constexpr int kParts = BF ? 3 : 2;
+  uint32_t lo[kParts], hi[kParts];    // k columns 2t, 2t+1 and 2t+8, 2t+9
+  __device__ __forceinline__ void set(float x0, float x1, float x2, float x3) {
+    split2<BF, kParts>(x0, x1, lo);
+    split2<BF, kParts>(x2, x3, hi);
+  }
+  __device__ __forceinline__ void mul(float (&d)[4], uint32_t b0, uint32_t b1) const {
+    mma_acc<BF>(d, lo[0], lo[1], hi[0], hi[1], b0, b1);
+    if (BF) mma_acc<BF>(d, lo[kParts - 1], 0u, hi[kParts - 1], 0u, b0, b1);
+  }
+};
+
+// ---------------------------------------------------------------------------
+// shapes: DP = head_dim rounded up to 64, 128 or 256; the rings of a CTA take
+// about 96 KB, two CTAs per SM, but for 16-bit rows of 256, where one CTA's
+// take 192 KB
+// ---------------------------------------------------------------------------
+template <int DT, int DP> struct AttCfg {
+  static constexpr bool kBf = DT == MOE_CACHE_BF16;
+  static constexpr int kElem = DT == MOE_CACHE_E4M3 ? 1 : 2;
+  static constexpr int kRow = DP * kElem;                   // bytes of a row in the ring
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kWarps = 4;
+  static constexpr int kKeys = kRow <= 128 ? 32 : 16;       // keys of a warp's tile
+  static constexpr int kStage = 2 * kKeys * kRow;           // keys, then values
+  static constexpr int kStages = kStage <= 4096 ? 5 : 3;
+  static constexpr int kRound = kWarps * kKeys;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kCtasPerSm = kRing <= 100 * 1024 ? 2 : 1;
+  static constexpr int kMergeRow = DP + 8;                  // floats
+  static constexpr int kMerge = kWarps * kAttHeads * kMergeRow * 4;
+  static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+};
+
+// swizzled byte offset of 16-byte chunk c of ring row r
+template <int CHUNKS>
+__device__ __forceinline__ uint32_t ring_at(int r, int c) {
+  const int x = CHUNKS >= 8 ? (r & 7) : ((r >> 1) & 3);
+  return (uint32_t)(r * CHUNKS * 16 + ((c ^ x) << 4));
+}
+
+struct AttShared {
+  long long base, scan[32];
+  int seq, last;
+  uint32_t seen[4][8];               // valid keys of each warp's stages
+  float m[4][kAttHeads], l[4][kAttHeads];
+};
+
+template <int DT, int DP>
+__global__ void __launch_bounds__(AttCfg<DT, DP>::kWarps * 32, AttCfg<DT, DP>::kCtasPerSm)
+attention_kernel(const AttArgs A) {
+  using Cfg = AttCfg<DT, DP>;
+  constexpr bool BF = Cfg::kBf;
+  constexpr int NW = Cfg::kWarps, NT = NW * 32, KEYS = Cfg::kKeys, NST = Cfg::kStages;
+  constexpr int CH = Cfg::kChunks, RK = Cfg::kRound;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ AttShared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int S = A.c.seqs, D = A.c.head_dim, G = A.hq / A.c.kv_heads;
+  const int NHT = (G + kAttHeads - 1) / kAttHeads, HU = A.c.kv_heads * NHT;
+  const int most = A.c.table_width * A.c.page_size;
   pdl_trigger();
   pdl_wait();
-  const int s = blockIdx.y, h = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int D = A.c.head_dim, kvh = h / (A.hq / A.c.kv_heads);
-  int len = A.seq_lens[s];
-  const int most = A.c.table_width * A.c.page_size;
-  if (len > most) {
-    if (threadIdx.x == 0) set_status(A.status, MOE_STATUS_BAD_PAGE);
-    len = most;
+
+  // ---- this CTA's run of rounds
+  auto keys_of = [&](int s, int& first) {
+    const int n = min(max(A.seq_lens[s], 0), most);
+    first = A.window > 0 && n > A.window ? n - A.window : 0;
+    return n;
+  };
+  auto rounds_of = [&](int s) {
+    int first;
+    const int n = keys_of(s, first);
+    return max(1, (n - first + RK - 1) / RK);   // an empty sequence still writes its zeros
+  };
+  const int per = (S + NT - 1) / NT, s0 = min(S, tid * per), s1 = min(S, s0 + per);
+  long long mine = 0;
+  for (int s = s0; s < s1; ++s) {
+    mine += (long long)rounds_of(s) * HU;
+    if (blockIdx.x == 0 && A.seq_lens[s] > most) set_status(A.status, MOE_STATUS_BAD_PAGE);
   }
-  const int first = A.window > 0 && len > A.window ? len - A.window : 0;
-  float q[kMaxHeadDim / 32], o[kMaxHeadDim / 32];
+  long long incl = mine;
 #pragma unroll
-  for (int i = 0; i < kMaxHeadDim / 32; ++i) {
-    o[i] = 0.f;
-    q[i] = 32 * i + lane < D ? A.q[s * A.q_ss + h * A.q_hs + 32 * i + lane] : 0.f;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long n = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += n;
   }
-  float m = -INFINITY, l = 0.f;
-  for (int j = first + warp; j < len; j += kAttWarps) {
-    const int page = A.c.block_table[(int64_t)s * A.c.table_stride + j / A.c.page_size];
-    if (page < 0 || page >= A.c.pages) {
-      if (lane == 0) set_status(A.status, MOE_STATUS_BAD_PAGE);
-      continue;
-    }
-    const int64_t at = (int64_t)page * A.c.page_stride +
-                       (int64_t)(j % A.c.page_size) * A.c.token_stride +
-                       (int64_t)kvh * A.c.head_stride;
-    const T* k = static_cast<const T*>(A.c.k) + at;
-    const T* v = static_cast<const T*>(A.c.v) + at;
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < kMaxHeadDim / 32; ++i)
-      if (32 * i + lane < D) x = fmaf(q[i], (float)k[32 * i + lane], x);
-#pragma unroll
-    for (int b = 16; b > 0; b >>= 1) x += __shfl_xor_sync(0xffffffffu, x, b);
-    x *= A.scale * A.c.k_scale;
-    if (A.cap > 0.f) x = A.cap * tanhf(x / A.cap);
-    const float mn = fmaxf(m, x);
-    const float keep = m == -INFINITY ? 0.f : expf(m - mn), p = expf(x - mn);
-    m = mn;
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < kMaxHeadDim / 32; ++i)
-      if (32 * i + lane < D) o[i] = fmaf(p, (float)v[32 * i + lane], o[i] * keep);
-  }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-  for (int i = 0; i < kMaxHeadDim / 32; ++i) so[warp][32 * i + lane] = o[i];
+  if (lane == 31) sh.scan[warp] = incl;
   __syncthreads();
-  float M = -INFINITY;
-  for (int w = 0; w < kAttWarps; ++w) M = fmaxf(M, sm[w]);
-  float L = 0.f;
-  for (int w = 0; w < kAttWarps; ++w) L += M == -INFINITY ? 0.f : sl[w] * expf(sm[w] - M);
-  for (int i = threadIdx.x; i < D; i += blockDim.x) {
-    float y = 0.f;
-    for (int w = 0; w < kAttWarps; ++w)
-      y += M == -INFINITY ? 0.f : so[w][i] * expf(sm[w] - M);
-    A.out[((int64_t)s * A.hq + h) * D + i] = L > 0.f || L != L ? y / L * A.c.v_scale : 0.f;
+  long long total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < warp) before += sh.scan[w];
+    total += sh.scan[w];
   }
-  if (threadIdx.x == 0 && A.lse) A.lse[(int64_t)s * A.hq + h] = M + logf(L);
+  const long long quota = (total + gridDim.x - 1) / gridDim.x;
+  long long at = (long long)blockIdx.x * quota;
+  if (at >= total) return;
+  const long long end = min(total, at + quota);
+  if (mine > 0 && before <= at && at < before + mine) {
+    int s = s0;
+    for (;;) {
+      const long long n = (long long)rounds_of(s) * HU;
+      if (at < before + n) break;
+      before += n;
+      ++s;
+    }
+    sh.seq = s;
+    sh.base = before;
+  }
+  __syncthreads();
+  int seq = sh.seq;
+  long long base = sh.base;
+
+  uint8_t* const ring = smem + warp * NST * Cfg::kStage;
+  const uint32_t ring_a = smem_u32(ring);
+  const uint8_t* const kbase = static_cast<const uint8_t*>(A.c.k);
+  const uint8_t* const vbase = static_cast<const uint8_t*>(A.c.v);
+  const int chunks = (D * Cfg::kElem + 15) / 16;            // chunks of a row in memory
+  const int zchunks = ((D + 15) / 16 * 16) * Cfg::kElem / 16;  // with the zeros of a last half step
+
+  while (at < end) {
+    int first;
+    const int len = keys_of(seq, first);
+    const int R = max(1, (len - first + RK - 1) / RK);
+    const int u = (int)((at - base) / R);
+    const long long ustart = base + (long long)u * R;
+    const int r0 = (int)(at - ustart), r1 = (int)min((long long)R, r0 + (end - at));
+    const int kvh = u / NHT, head0 = kvh * G + (u - kvh * NHT) * kAttHeads;
+    const int nh = min(kAttHeads, kvh * G + G - head0);
+    const int klo = first + r0 * RK, khi = min(len, first + r1 * RK);
+    const int32_t* table = A.c.block_table + (int64_t)seq * A.c.table_stride;
+    const int64_t head_off = (int64_t)kvh * A.c.head_stride;
+
+    // ---- tiles of this warp: keys klo + (i * NW + warp) * KEYS ...
+    const int kw = klo + warp * KEYS;
+    const int ntile = khi > kw ? (khi - kw + RK - 1) / RK : 0;
+    int page = 0, slot = 0;
+    bool in = false;
+    auto fetch = [&](int i) {                    // page of this lane's key of tile i
+      const int key = kw + i * RK + (lane & (KEYS - 1));
+      in = i < ntile && key < khi;
+      if (in) {
+        const int p = (int)((unsigned)key / (unsigned)A.c.page_size);
+        slot = key - p * A.c.page_size;
+        page = table[p];
+      }
+    };
+    auto issue = [&](int i) {                    // rows of tile i, after fetch(i)
+      if (i < ntile) {
+        int64_t off = -1;
+        if (in) {
+          if (page >= 0 && page < A.c.pages)
+            off = ((int64_t)page * A.c.page_stride + (int64_t)slot * A.c.token_stride + head_off) *
+                  Cfg::kElem;
+          else
+            set_status(A.status, MOE_STATUS_BAD_PAGE);
+        }
+        const int st = i % NST;
+        const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
+        if (lane == 0) sh.seen[warp][st] = ok;
+        const uint32_t dst = ring_a + st * Cfg::kStage;
+        constexpr int LPR = CH < 32 ? CH : 32, RPI = 32 / LPR;   // lanes per row, rows at once
+#pragma unroll
+        for (int r = 0; r < KEYS; r += RPI) {
+          const int row = r + lane / LPR, c = lane % LPR;
+          const int64_t o = __shfl_sync(0xffffffffu, off, row);
+          if (c < zchunks) {
+            const uint32_t n = o >= 0 && c < chunks ? 16u : 0u;
+            const int64_t b = n ? o + c * 16 : 0;
+            const uint32_t to = dst + ring_at<CH>(row, c);
+            cp_async16(to, kbase + b, n);
+            cp_async16(to + KEYS * Cfg::kRow, vbase + b, n);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+    fetch(0);
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i) {
+      issue(i);
+      fetch(i + 1);
+    }
+
+    // ---- q of head g as A fragments, scaled by a power of two to [2^10, 2^11)
+    AFrag<BF> qf[DP / 16];
+    float qscale;                                // score = product * qscale
+    {
+      const float* q = A.q + (int64_t)seq * A.q_ss + (int64_t)(head0 + g) * A.q_hs;
+      float mx = 0.f;
+      float x[DP / 16][4];
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        // columns 2t, 2t+1, 2t+8, 2t+9 of the operand; e4m3 keys are read
+        // four bytes per lane, which makes them elements 4t .. 4t+3
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = 16 * kk + (Cfg::kElem == 1 ? 4 * t + j : 2 * t + (j & 1) + 8 * (j >> 1));
+          x[kk][j] = g < nh && e < D ? q[e] : 0.f;
+          mx = fmaxf(mx, fabsf(x[kk][j]));
+        }
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const int e = mx > 0.f && mx <= 3.4e38f ? 10 - ilogbf(mx) : 0;
+      qscale = ldexpf(A.scale * A.c.k_scale, -e);
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk)
+        qf[kk].set(ldexpf(x[kk][0], e), ldexpf(x[kk][1], e), ldexpf(x[kk][2], e),
+                   ldexpf(x[kk][3], e));
+    }
+    const float x2 = qscale * kLog2e;
+
+    float o[DP / 8][2];                          // head g, two columns of each 8-wide block
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) o[c][0] = o[c][1] = 0.f;
+    float m = -INFINITY, l = 0.f;                // l: this lane's keys only
+
+    for (int i = 0; i < ntile; ++i) {
+      cp_async_wait<NST - 2>();
+      __syncwarp();
+      issue(i + NST - 1);
+      fetch(i + NST);
+      const int st = i % NST;
+      const uint32_t ka = ring_a + st * Cfg::kStage, va = ka + KEYS * Cfg::kRow;
+      const uint32_t seen = sh.seen[warp][st];
+
+      // scores: keys 8b + 2t, 8b + 2t + 1 of head g in this lane
+      float x[KEYS / 8][2];
+#pragma unroll
+      for (int kb = 0; kb < KEYS / 16; ++kb) {
+        float s[2][2] = {};
+#pragma unroll
+        for (int k4 = 0; k4 < DP / 64; ++k4) {
+          float a[2][4] = {};
+          if (Cfg::kElem == 2) {
+#pragma unroll
+            for (int kk = 4 * k4; kk < 4 * k4 + 4; ++kk) {
+              if (16 * kk < D) {
+                uint32_t b[4];
+                const int row = 16 * kb + (lane >> 4) * 8 + (lane & 7);
+                ldsm4(b, ka + ring_at<CH>(row, 2 * kk + ((lane >> 3) & 1)));
+                qf[kk].mul(a[0], b[0], b[1]);
+                qf[kk].mul(a[1], b[2], b[3]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int kk = 4 * k4; kk < 4 * k4 + 4; kk += 2) {
+              if (16 * kk < D) {
+                uint32_t b[4];
+                const int row = 16 * kb + ((lane >> 3) & 1) * 8 + (lane & 7);
+                ldsm4(b, ka + ring_at<CH>(row, kk + (lane >> 4)));
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (16 * (kk + (j >> 1)) < D)
+                    qf[kk + (j >> 1)].mul(a[j & 1], e4m3x2_f16x2(b[j]), e4m3x2_f16x2(b[j] >> 16));
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[j][0] += a[j][0] + a[j][2];
+            s[j][1] += a[j][1] + a[j][3];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v = s[j][h];
+            v = A.cap > 0.f ? A.cap * tanhf(v * qscale / A.cap) * kLog2e : v * x2;
+            x[2 * kb + j][h] = (seen >> (16 * kb + 8 * j + 2 * t + h)) & 1u ? v : -INFINITY;
+          }
+      }
+
+      // running maximum and sum
+      float mx = m;
+#pragma unroll
+      for (int b = 0; b < KEYS / 8; ++b) mx = fmaxf(mx, fmaxf(x[b][0], x[b][1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float ms = mx == -INFINITY ? 0.f : mx;
+      const float keep = ex2(m - ms);
+      m = mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int b = 0; b < KEYS / 8; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          x[b][h] = ex2(x[b][h] - ms);
+          sum += x[b][h];
+        }
+      l = fmaf(l, keep, sum);
+      AFrag<BF> pf[KEYS / 16];
+#pragma unroll
+      for (int kb = 0; kb < KEYS / 16; ++kb)
+        pf[kb].set(x[2 * kb][0] * 16384.f, x[2 * kb][1] * 16384.f, x[2 * kb + 1][0] * 16384.f,
+                   x[2 * kb + 1][1] * 16384.f);
+
+      // o = o * keep + p v
+      if (Cfg::kElem == 2) {
+#pragma unroll
+        for (int c = 0; c < DP / 8; c += 2) {
+          if (8 * c < D) {
+            float a[2][4] = {};
+#pragma unroll
+            for (int kb = 0; kb < KEYS / 16; ++kb) {
+              uint32_t b[4];
+              const int row = 16 * kb + ((lane >> 3) & 1) * 8 + (lane & 7);
+              ldsm4_t(b, va + ring_at<CH>(row, c + (lane >> 4)));
+              pf[kb].mul(a[0], b[0], b[1]);
+              pf[kb].mul(a[1], b[2], b[3]);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              o[c + j][0] = fmaf(o[c + j][0], keep, a[j][0] + a[j][2]);
+              o[c + j][1] = fmaf(o[c + j][1], keep, a[j][1] + a[j][3]);
+            }
+          }
+        }
+      } else {
+        // a 16-byte chunk holds 16 columns; transposed in pairs of bytes, a
+        // register has columns (2g, 2g + 1) of two keys, which become the
+        // B registers of the even and of the odd columns
+#pragma unroll
+        for (int c = 0; c < DP / 16; c += 2) {
+          if (16 * c < D) {
+            float a[2][2][4] = {};
+#pragma unroll
+            for (int kb = 0; kb < KEYS / 16; ++kb) {
+              uint32_t b[4];
+              const int row = 16 * kb + ((lane >> 3) & 1) * 8 + (lane & 7);
+              ldsm4_t(b, va + ring_at<CH>(row, c + (lane >> 4)));
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                if (16 * (c + j) < D) {
+                  const uint32_t k0 = e4m3x2_f16x2(b[2 * j]), k1 = e4m3x2_f16x2(b[2 * j] >> 16);
+                  const uint32_t k8 = e4m3x2_f16x2(b[2 * j + 1]),
+                                 k9 = e4m3x2_f16x2(b[2 * j + 1] >> 16);
+                  pf[kb].mul(a[j][0], prmt(k0, k1, 0x5410u), prmt(k8, k9, 0x5410u));
+                  pf[kb].mul(a[j][1], prmt(k0, k1, 0x7632u), prmt(k8, k9, 0x7632u));
+                }
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int b = 2 * (c + j) + h;
+                o[b][0] = fmaf(o[b][0], keep, a[j][h][0] + a[j][h][2]);
+                o[b][1] = fmaf(o[b][1], keep, a[j][h][1] + a[j][h][3]);
+              }
+          }
+        }
+      }
+    }
+
+    // ---- the warps' parts meet in shared memory
+    cp_async_wait<0>();
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (t == 0) {
+      sh.m[warp][g] = m;
+      sh.l[warp][g] = l;
+    }
+    __syncthreads();                             // every ring is idle
+    float* const mo = reinterpret_cast<float*>(smem);
+    {
+      float* row = mo + (warp * kAttHeads + g) * Cfg::kMergeRow;
+#pragma unroll
+      for (int c = 0; c < DP / 8; ++c) {
+        if (Cfg::kElem == 2) {
+          *reinterpret_cast<float2*>(row + 8 * c + 2 * t) = make_float2(o[c][0], o[c][1]);
+        } else {                                 // block 2c: even columns 4t, 4t + 2; 2c + 1: odd
+          row[16 * (c >> 1) + 4 * t + (c & 1)] = o[c][0];
+          row[16 * (c >> 1) + 4 * t + 2 + (c & 1)] = o[c][1];
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = r0 == 0 && r1 == R;
+    const int my_slot = 2 * blockIdx.x + (r0 == 0 ? 1 : 0);
+    for (int e = tid; e < nh * D; e += NT) {
+      const int h = e / D, c = e - h * D;
+      float M = sh.m[0][h];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) M = fmaxf(M, sh.m[w][h]);
+      const float ms = M == -INFINITY ? 0.f : M;
+      float L = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = ex2(sh.m[w][h] - ms);
+        L = fmaf(sh.l[w][h], f, L);
+        y = fmaf(mo[(w * kAttHeads + h) * Cfg::kMergeRow + c], f, y);
+      }
+      if (whole) {
+        const int64_t row = (int64_t)seq * A.hq + head0 + h;
+        A.out[row * D + c] = L == 0.f ? 0.f : y * (1.f / 16384.f) * A.c.v_scale / L;
+        if (c == 0 && A.lse) A.lse[row] = (M + log2f(L)) * kLn2;
+      } else {
+        A.part_o[((int64_t)my_slot * kAttHeads + h) * DP + c] = y;
+        if (c == 0) A.part_ml[my_slot * kAttHeads + h] = make_float2(M, L);
+      }
+    }
+    if (!whole) {
+      // ---- the last CTA of a unit to arrive joins the unit's parts, in order
+      const int c0 = (int)(ustart / quota);
+      const int n = (int)((ustart + R - 1) / quota) - c0 + 1;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const int arrived = atomicAdd(A.arrivals + c0, 1);
+        sh.last = arrived == n - 1;
+        if (sh.last) A.arrivals[c0] = 0;
+      }
+      __syncthreads();
+      if (sh.last) {
+        __threadfence();
+        // weights of the parts, [head][part]; mo is free again
+        for (int h = warp; h < nh; h += NW) {
+          float M = -INFINITY;
+          for (int i = lane; i < n; i += 32)
+            M = fmaxf(M, __ldcg(A.part_ml + (2 * (c0 + i) + (i == 0)) * kAttHeads + h).x);
+#pragma unroll
+          for (int b = 16; b > 0; b >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, b));
+          const float ms = M == -INFINITY ? 0.f : M;
+          float L = 0.f;
+          for (int i = lane; i < n; i += 32) {
+            const float2 v = __ldcg(A.part_ml + (2 * (c0 + i) + (i == 0)) * kAttHeads + h);
+            const float f = ex2(v.x - ms);
+            mo[h * n + i] = f;
+            L = fmaf(v.y, f, L);
+          }
+#pragma unroll
+          for (int b = 16; b > 0; b >>= 1) L += __shfl_xor_sync(0xffffffffu, L, b);
+          if (lane == 0) {
+            sh.m[0][h] = M;
+            sh.l[0][h] = L;
+          }
+        }
+        __syncthreads();
+        for (int e = tid; e < nh * D; e += NT) {
+          const int h = e / D, c = e - h * D;
+          const float* po = A.part_o + ((int64_t)2 * c0 * kAttHeads + h) * DP + c;
+          float y = __ldcg(po + kAttHeads * DP) * mo[h * n];
+#pragma unroll 8
+          for (int i = 1; i < n; ++i) y = fmaf(__ldcg(po + (int64_t)2 * i * kAttHeads * DP), mo[h * n + i], y);
+          const float L = sh.l[0][h];
+          const int64_t row = (int64_t)seq * A.hq + head0 + h;
+          A.out[row * D + c] = L == 0.f ? 0.f : y * (1.f / 16384.f) * A.c.v_scale / L;
+          if (c == 0 && A.lse) A.lse[row] = (sh.m[0][h] + log2f(L)) * kLn2;
+        }
+      }
+    }
+    __syncthreads();                             // mo and sh are rings and stages again
+    at += r1 - r0;
+    if (at - base == (long long)R * HU) {
+      base = at;
+      ++seq;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+inline int padded_head_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+static int attention_workspace(int head_dim, AttArgs* a, void* ws, size_t* bytes) {
+  Carve cv = {static_cast<uint8_t*>(ws), 0, 0};
+  const int slots = kAttMaxCtasPerSm * sm_count();
+  cv.take<uint8_t>(256);
+  int* arrivals = cv.take<int>(slots);
+  float2* ml = cv.take<float2>((size_t)2 * slots * kAttHeads);
+  float* o = cv.take<float>((size_t)2 * slots * kAttHeads * padded_head_dim(head_dim));
+  if (a) {
+    a->arrivals = arrivals;
+    a->part_ml = ml;
+    a->part_o = o;
+  }
+  *bytes = align_up(cv.used, 256);
+  return MOE_OK;
+}
+
+template <int DT, int DP>
+static int launch_attention(const AttArgs& a, int max_len, cudaStream_t s) {
+  using Cfg = AttCfg<DT, DP>;
+  static_assert(Cfg::kStages >= 2 && Cfg::kStages <= 8 && Cfg::kCtasPerSm <= kAttMaxCtasPerSm, "");
+  static_assert(kAttHeads * kAttMaxCtasPerSm * 160 * 4 <= Cfg::kSmem, "weights of a unit's parts");
+  static std::atomic<uint64_t> ready{0};
+  auto kern = attention_kernel<DT, DP>;
+  int dev = 0;
+  MOE_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !((ready.load() >> dev) & 1)) {
+    MOE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  const int G = a.hq / a.c.kv_heads;
+  const int64_t units = (int64_t)a.c.seqs * a.c.kv_heads * ((G + kAttHeads - 1) / kAttHeads);
+  const int64_t keys = a.window > 0 ? std::min(a.window, max_len) : max_len;
+  const int64_t rounds = units * std::max<int64_t>(1, (keys + Cfg::kRound - 1) / Cfg::kRound);
+  const int grid = (int)std::min<int64_t>(rounds, (int64_t)Cfg::kCtasPerSm * sm_count());
+  MOE_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(Cfg::kWarps * 32), Cfg::kSmem, s, a));
+  return MOE_OK;
+}
+
+template <int DT>
+static int launch_attention_dt(const AttArgs& a, int max_len, cudaStream_t s) {
+  switch (padded_head_dim(a.c.head_dim)) {
+    case 64: return launch_attention<DT, 64>(a, max_len, s);
+    case 128: return launch_attention<DT, 128>(a, max_len, s);
+    default: return launch_attention<DT, 256>(a, max_len, s);
+  }
 }
 
 }  // namespace moe
@@ -100,8 +664,7 @@ int moe_paged_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int
               MOE_ERR_INVALID, "bad attention shape");
   MOE_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0, MOE_ERR_INVALID,
               "%d query heads for %d key heads", q_heads, kv_heads);
-  *bytes = 256;
-  return MOE_OK;
+  return moe::attention_workspace(head_dim, nullptr, nullptr, bytes);
 }
 
 int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_seq_stride,
@@ -117,22 +680,33 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
               "scale and softcap must be finite, softcap >= 0");
   if (cache->seqs == 0) return MOE_OK;
   MOE_REQUIRE(q && seq_lens && out && workspace, MOE_ERR_INVALID, "null pointer");
+  moe::AttArgs a = {};
+  a.c = *cache;
+  a.q = q;
+  a.q_ss = q_seq_stride;
+  a.q_hs = q_head_stride;
+  a.seq_lens = seq_lens;
+  a.out = out;
+  a.lse = lse;
+  a.status = static_cast<int*>(workspace);
+  a.hq = q_heads;
+  a.window = window;
+  a.scale = scale;
+  a.cap = softcap;
+  moe::normalise_strides(a.c);
   size_t need = 0;
-  MOE_CHECK(moe_paged_attention_workspace_bytes(cache->seqs, q_heads, cache->kv_heads,
-                                                cache->head_dim, &need));
+  MOE_CHECK(moe::attention_workspace(cache->head_dim, &a, workspace, &need));
   MOE_REQUIRE(workspace_bytes >= need, MOE_ERR_WORKSPACE, "workspace %zu < %zu bytes",
               workspace_bytes, need);
-  moe::AttArgs a = {*cache, q, q_seq_stride, q_head_stride, seq_lens, out, lse,
-                    static_cast<int*>(workspace), q_heads, window, scale, softcap};
-  moe::normalise_strides(a.c);
+  const int most = cache->table_width * cache->page_size;
+  const int longest = max_len > 0 && max_len < most ? max_len : most;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   {
     ::moe::ProfScope _prof(MOE_K_ATTENTION, s);
-    auto kern = cache->dtype == MOE_CACHE_F16    ? moe::attention_kernel<MOE_CACHE_F16>
-                : cache->dtype == MOE_CACHE_BF16 ? moe::attention_kernel<MOE_CACHE_BF16>
-                                                 : moe::attention_kernel<MOE_CACHE_E4M3>;
-    MOE_CUDA(moe::launch_pdl(kern, dim3((unsigned)q_heads, (unsigned)cache->seqs),
-                             dim3(moe::kAttWarps * 32), 0, s, a));
+    MOE_CHECK(cache->dtype == MOE_CACHE_F16 ? moe::launch_attention_dt<MOE_CACHE_F16>(a, longest, s)
+              : cache->dtype == MOE_CACHE_BF16
+                  ? moe::launch_attention_dt<MOE_CACHE_BF16>(a, longest, s)
+                  : moe::launch_attention_dt<MOE_CACHE_E4M3>(a, longest, s));
   }
   return moe::check_launch("paged_attention");
 }
