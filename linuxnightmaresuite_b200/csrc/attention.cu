@@ -43,6 +43,7 @@ constexpr int kAttHeads = 8;          // query heads of a unit at most
 constexpr int kAttMaxCtasPerSm = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kPScale = 128.f;      // probabilities enter the products times this
 
 struct AttArgs {
   moe_paged_cache c;
@@ -126,11 +127,12 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&r)[NP]) {
   }
 }
 
-// e4m3 pair (low 16 bits) -> fp16x2, exact
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t v) {
-  uint32_t r;
-  asm("{\n .reg .b16 l;\n cvt.u16.u32 l, %1;\n cvt.rn.f16x2.e4m3x2 %0, l;\n}" : "=r"(r) : "r"(v));
-  return r;
+// four e4m3 -> two fp16x2, exact
+__device__ __forceinline__ void e4m3x4_f16x2(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n"
+      " cvt.rn.f16x2.e4m3x2 %1, h;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(v));
 }
 
 // A operand of one k16 step: one 16-row tile of {hi rows, lo rows}; bf16 has a
@@ -146,12 +148,31 @@ template <bool BF> struct AFrag {
     mma_acc<BF>(d, lo[0], lo[1], hi[0], hi[1], b0, b1);
     if (BF) mma_acc<BF>(d, lo[kParts - 1], 0u, hi[kParts - 1], 0u, b0, b1);
   }
+  // in shared memory: 16 bytes per lane, then for bf16 8 more
+  static constexpr int kBytes = 32 * 8 * kParts;
+  __device__ __forceinline__ void store(uint8_t* at, int lane) const {
+    *reinterpret_cast<uint4*>(at + lane * 16) = make_uint4(lo[0], lo[1], hi[0], hi[1]);
+    if (BF) *reinterpret_cast<uint2*>(at + 512 + lane * 8) =
+        make_uint2(lo[kParts - 1], hi[kParts - 1]);
+  }
+  __device__ __forceinline__ void load(const uint8_t* at, int lane) {
+    const uint4 v = *reinterpret_cast<const uint4*>(at + lane * 16);
+    lo[0] = v.x;
+    lo[1] = v.y;
+    hi[0] = v.z;
+    hi[1] = v.w;
+    if (BF) {
+      const uint2 w = *reinterpret_cast<const uint2*>(at + 512 + lane * 8);
+      lo[kParts - 1] = w.x;
+      hi[kParts - 1] = w.y;
+    }
+  }
 };
 
 // ---------------------------------------------------------------------------
-// shapes: DP = head_dim rounded up to 64, 128 or 256; the rings of a CTA take
-// about 96 KB, two CTAs per SM, but for 16-bit rows of 256, where one CTA's
-// take 192 KB
+// shapes: DP = head_dim rounded up to 64, 128 or 256.  A ring slot holds the
+// keys or the values of a tile; an odd number of slots makes the slot freed
+// by keys the next one that keys go to.
 // ---------------------------------------------------------------------------
 template <int DT, int DP> struct AttCfg {
   static constexpr bool kBf = DT == MOE_CACHE_BF16;
@@ -160,14 +181,21 @@ template <int DT, int DP> struct AttCfg {
   static constexpr int kChunks = kRow / 16;
   static constexpr int kWarps = 4;
   static constexpr int kKeys = kRow <= 128 ? 32 : 16;       // keys of a warp's tile
-  static constexpr int kStage = 2 * kKeys * kRow;           // keys, then values
-  static constexpr int kStages = kStage <= 4096 ? 5 : 3;
+  static constexpr int kSlot = kKeys * kRow;
+  static constexpr int kSlots = kSlot <= 2048 ? 9 : 5;
   static constexpr int kRound = kWarps * kKeys;
-  static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kCtasPerSm = kRing <= 100 * 1024 ? 2 : 1;
+  static constexpr int kRing = kWarps * kSlots * kSlot;
   static constexpr int kMergeRow = DP + 8;                  // floats
-  static constexpr int kMerge = kWarps * kAttHeads * kMergeRow * 4;
-  static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+  // one row per warp and head; at least the weights of a unit split over 320 CTAs
+  static constexpr int kMerge = kAttHeads * 4 * (kWarps * kMergeRow > 320 ? kWarps * kMergeRow : 320);
+  static constexpr int kQ = DP / 16 * AFrag<kBf>::kBytes;
+  static constexpr int kSmem = kRing + kMerge + kQ;
+  static constexpr int kCtasPerSm = kSmem <= 112 * 1024 ? 2 : 1;
+  // Whether the products p v stay in MMA accumulators for kFold tiles (four
+  // k16 steps) before they are added up; at 256 columns the registers do not
+  // hold both, and every tile is added up.
+  static constexpr bool kHold = DP <= 128;
+  static constexpr int kFold = 64 / kKeys;
 };
 
 // swizzled byte offset of 16-byte chunk c of ring row r
@@ -178,10 +206,16 @@ __device__ __forceinline__ uint32_t ring_at(int r, int c) {
 }
 
 struct AttShared {
-  long long base, scan[32];
+  long long base, scan[4];
   int seq, last;
-  uint32_t seen[4][8];               // valid keys of each warp's stages
-  float m[4][kAttHeads], l[4][kAttHeads];
+  uint32_t seen[4][8];               // valid keys of the tiles in each warp's ring
+  float m[4][kAttHeads], l[4][kAttHeads], qmax[4][kAttHeads], qscale[kAttHeads];
+};
+
+// One CTA's part of a unit: rounds r0 .. r1 of R.
+struct Piece {
+  int ustart, R, r0, r1, head0, nh, kw, khi, ntile;
+  int64_t head_off;
 };
 
 template <int DT, int DP>
@@ -189,7 +223,7 @@ __global__ void __launch_bounds__(AttCfg<DT, DP>::kWarps * 32, AttCfg<DT, DP>::k
 attention_kernel(const AttArgs A) {
   using Cfg = AttCfg<DT, DP>;
   constexpr bool BF = Cfg::kBf;
-  constexpr int NW = Cfg::kWarps, NT = NW * 32, KEYS = Cfg::kKeys, NST = Cfg::kStages;
+  constexpr int NW = Cfg::kWarps, NT = NW * 32, KEYS = Cfg::kKeys, NS = Cfg::kSlots;
   constexpr int CH = Cfg::kChunks, RK = Cfg::kRound;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ AttShared sh;
@@ -231,15 +265,15 @@ attention_kernel(const AttArgs A) {
     if (w < warp) before += sh.scan[w];
     total += sh.scan[w];
   }
-  const long long quota = (total + gridDim.x - 1) / gridDim.x;
-  long long at = (long long)blockIdx.x * quota;
-  if (at >= total) return;
-  const long long end = min(total, at + quota);
-  if (mine > 0 && before <= at && at < before + mine) {
+  const int quota = (int)((total + gridDim.x - 1) / gridDim.x);
+  const long long start = (long long)blockIdx.x * quota;
+  if (start >= total) return;
+  const int end = (int)min(total - start, (long long)quota);   // rounds count from `start` on
+  if (mine > 0 && before <= start && start < before + mine) {
     int s = s0;
     for (;;) {
       const long long n = (long long)rounds_of(s) * HU;
-      if (at < before + n) break;
+      if (start < before + n) break;
       before += n;
       ++s;
     }
@@ -247,264 +281,366 @@ attention_kernel(const AttArgs A) {
     sh.base = before;
   }
   __syncthreads();
-  int seq = sh.seq;
-  long long base = sh.base;
+  const int seq0 = sh.seq, base0 = (int)(sh.base - start);
 
-  uint8_t* const ring = smem + warp * NST * Cfg::kStage;
-  const uint32_t ring_a = smem_u32(ring);
+  // part of a unit at round `at` of sequence s, whose first round is `base`
+  auto piece_at = [&](int s, int base, int at) {
+    Piece p;
+    int first;
+    const int len = keys_of(s, first);
+    p.R = max(1, (len - first + RK - 1) / RK);
+    const int u = (at - base) / p.R;
+    p.ustart = base + u * p.R;
+    p.r0 = at - p.ustart;
+    p.r1 = min(p.R, p.r0 + (end - at));
+    const int kvh = u / NHT;
+    p.head0 = kvh * G + (u - kvh * NHT) * kAttHeads;
+    p.nh = min(kAttHeads, kvh * G + G - p.head0);
+    p.kw = first + p.r0 * RK + warp * KEYS;     // tiles of this warp: kw + i * RK ...
+    p.khi = min(len, first + p.r1 * RK);
+    p.ntile = p.khi > p.kw ? (p.khi - p.kw + RK - 1) / RK : 0;
+    p.head_off = (int64_t)kvh * A.c.head_stride;
+    return p;
+  };
+
+  // ---- loads: a cursor of its own that runs ahead of the arithmetic, across
+  // the ends of units
+  const uint32_t ring_a = smem_u32(smem) + warp * NS * Cfg::kSlot;
   const uint8_t* const kbase = static_cast<const uint8_t*>(A.c.k);
   const uint8_t* const vbase = static_cast<const uint8_t*>(A.c.v);
-  const int chunks = (D * Cfg::kElem + 15) / 16;            // chunks of a row in memory
-  const int zchunks = ((D + 15) / 16 * 16) * Cfg::kElem / 16;  // with the zeros of a last half step
-
-  while (at < end) {
-    int first;
-    const int len = keys_of(seq, first);
-    const int R = max(1, (len - first + RK - 1) / RK);
-    const int u = (int)((at - base) / R);
-    const long long ustart = base + (long long)u * R;
-    const int r0 = (int)(at - ustart), r1 = (int)min((long long)R, r0 + (end - at));
-    const int kvh = u / NHT, head0 = kvh * G + (u - kvh * NHT) * kAttHeads;
-    const int nh = min(kAttHeads, kvh * G + G - head0);
-    const int klo = first + r0 * RK, khi = min(len, first + r1 * RK);
-    const int32_t* table = A.c.block_table + (int64_t)seq * A.c.table_stride;
-    const int64_t head_off = (int64_t)kvh * A.c.head_stride;
-
-    // ---- tiles of this warp: keys klo + (i * NW + warp) * KEYS ...
-    const int kw = klo + warp * KEYS;
-    const int ntile = khi > kw ? (khi - kw + RK - 1) / RK : 0;
-    int page = 0, slot = 0;
-    bool in = false;
-    auto fetch = [&](int i) {                    // page of this lane's key of tile i
-      const int key = kw + i * RK + (lane & (KEYS - 1));
-      in = i < ntile && key < khi;
-      if (in) {
-        const int p = (int)((unsigned)key / (unsigned)A.c.page_size);
-        slot = key - p * A.c.page_size;
-        page = table[p];
+  const int chunks = (D * Cfg::kElem + 15) / 16;               // chunks of a row in memory
+  const int zchunks = ((D + 15) / 16 * 16) * Cfg::kElem / 16;  // with the zeros of a half step
+  int lseq = seq0, lbase = base0, lat = 0, li = 0, lslot = 0;
+  uint32_t ltile = 0;
+  Piece lp = piece_at(lseq, lbase, lat);
+  int page = 0, slot = 0;
+  bool in = false;
+  int64_t off = -1;                              // this lane's row of the tile, bytes
+  auto settle = [&]() {                          // to the next piece that has a tile li
+    while (li >= lp.ntile) {
+      lat += lp.r1 - lp.r0;
+      if (lat >= end) {
+        lp.ntile = 0x7fffffff;                   // nothing left: tiles without rows
+        lp.khi = lp.kw = 0;
+        break;
       }
-    };
-    auto issue = [&](int i) {                    // rows of tile i, after fetch(i)
-      if (i < ntile) {
-        int64_t off = -1;
-        if (in) {
-          if (page >= 0 && page < A.c.pages)
-            off = ((int64_t)page * A.c.page_stride + (int64_t)slot * A.c.token_stride + head_off) *
-                  Cfg::kElem;
-          else
-            set_status(A.status, MOE_STATUS_BAD_PAGE);
-        }
-        const int st = i % NST;
-        const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
-        if (lane == 0) sh.seen[warp][st] = ok;
-        const uint32_t dst = ring_a + st * Cfg::kStage;
-        constexpr int LPR = CH < 32 ? CH : 32, RPI = 32 / LPR;   // lanes per row, rows at once
+      if (lat - lbase == lp.R * HU) {
+        lbase = lat;
+        ++lseq;
+      }
+      lp = piece_at(lseq, lbase, lat);
+      li = 0;
+    }
+  };
+  auto fetch = [&]() {                           // page of this lane's key of tile li
+    const int key = lp.kw + li * RK + (lane & (KEYS - 1));
+    in = lat < end && key < lp.khi;
+    if (in) {
+      const int p = (int)((unsigned)key / (unsigned)A.c.page_size);
+      slot = key - p * A.c.page_size;
+      page = A.c.block_table[(int64_t)lseq * A.c.table_stride + p];
+    }
+  };
+  auto copy = [&](const uint8_t* from) {
+    if (lat < end) {
+      const uint32_t dst = ring_a + lslot * Cfg::kSlot;
+      constexpr int LPR = CH < 32 ? CH : 32, RPI = 32 / LPR;   // lanes per row, rows at once
 #pragma unroll
-        for (int r = 0; r < KEYS; r += RPI) {
-          const int row = r + lane / LPR, c = lane % LPR;
-          const int64_t o = __shfl_sync(0xffffffffu, off, row);
-          if (c < zchunks) {
-            const uint32_t n = o >= 0 && c < chunks ? 16u : 0u;
-            const int64_t b = n ? o + c * 16 : 0;
-            const uint32_t to = dst + ring_at<CH>(row, c);
-            cp_async16(to, kbase + b, n);
-            cp_async16(to + KEYS * Cfg::kRow, vbase + b, n);
-          }
+      for (int r = 0; r < KEYS; r += RPI) {
+        const int row = r + lane / LPR, c = lane % LPR;
+        const int64_t o = __shfl_sync(0xffffffffu, off, row);
+        if (c < zchunks) {
+          const uint32_t n = o >= 0 && c < chunks ? 16u : 0u;
+          cp_async16(dst + ring_at<CH>(row, c), from + (n ? o + c * 16 : 0), n);
         }
       }
-      cp_async_commit();
-    };
-    fetch(0);
+    }
+    cp_async_commit();
+    lslot = lslot + 1 == NS ? 0 : lslot + 1;
+  };
+  auto issue_keys = [&]() {
+    off = -1;
+    if (in) {
+      if (page >= 0 && page < A.c.pages)
+        off = ((int64_t)page * A.c.page_stride + (int64_t)slot * A.c.token_stride + lp.head_off) *
+              Cfg::kElem;
+      else
+        set_status(A.status, MOE_STATUS_BAD_PAGE);
+    }
+    const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
+    if (lane == 0) sh.seen[warp][ltile & 7] = ok;
+    ++ltile;
+    copy(kbase);
+  };
+  auto issue_values = [&]() {
+    copy(vbase);
+    if (lat < end) {
+      ++li;
+      settle();
+      fetch();
+    }
+  };
+  settle();
+  fetch();
 #pragma unroll
-    for (int i = 0; i < NST - 1; ++i) {
-      issue(i);
-      fetch(i + 1);
+  for (int i = 0; i < (NS - 1) / 2; ++i) {
+    issue_keys();
+    issue_values();
+  }
+
+  // ---- q: this thread's values of the next piece's operand (k16 steps warp,
+  // warp + NW, ...), fetched a piece ahead; columns 2t, 2t+1, 2t+8, 2t+9 of a
+  // step, but for e4m3 keys, which are read four bytes per lane: 4t .. 4t+3
+  constexpr int QK = DP / 16 / NW;
+  uint8_t* const qs = smem + Cfg::kRing + Cfg::kMerge;
+  float* const mo = reinterpret_cast<float*>(smem + Cfg::kRing);
+  float qn[QK][4];
+  auto q_fetch = [&](int s, const Piece& p) {
+    const float* q = A.q + (int64_t)s * A.q_ss + (int64_t)(p.head0 + g) * A.q_hs;
+#pragma unroll
+    for (int i = 0; i < QK; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = 16 * (warp + i * NW) +
+                      (Cfg::kElem == 1 ? 4 * t + j : 2 * t + (j & 1) + 8 * (j >> 1));
+        qn[i][j] = g < p.nh && e < D ? q[e] : 0.f;
+      }
+  };
+  auto q_max = [&]() {
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < QK; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fabsf(qn[i][j]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    if (t == 0) sh.qmax[warp][g] = mx;
+  };
+  auto q_split = [&]() {                         // scaled by a power of two to [2^10, 2^11)
+    float mx = sh.qmax[0][g];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, sh.qmax[w][g]);
+    const int e = mx > 0.f && mx <= 3.4e38f ? 10 - ilogbf(mx) : 0;
+    if (warp == 0 && t == 0) sh.qscale[g] = ldexpf(A.scale * A.c.k_scale, -e);
+#pragma unroll
+    for (int i = 0; i < QK; ++i) {
+      AFrag<BF> f;
+      f.set(ldexpf(qn[i][0], e), ldexpf(qn[i][1], e), ldexpf(qn[i][2], e), ldexpf(qn[i][3], e));
+      f.store(qs + (warp + i * NW) * AFrag<BF>::kBytes, lane);
+    }
+  };
+
+  int seq = seq0, base = base0, at = 0, cslot = 0;
+  uint32_t ctile = 0;
+  Piece P = piece_at(seq, base, at);
+  q_fetch(seq, P);
+  q_max();
+  __syncthreads();
+  q_split();
+  __syncthreads();
+
+  // lane constants of the fragment addresses
+  const int krow = Cfg::kElem == 2 ? (lane >> 4) * 8 + (lane & 7) : ((lane >> 3) & 1) * 8 + (lane & 7);
+  const int kch = Cfg::kElem == 2 ? (lane >> 3) & 1 : lane >> 4;
+  const int vrow = ((lane >> 3) & 1) * 8 + (lane & 7), vch = lane >> 4;
+
+  for (;;) {
+    // the piece after this one, and its q
+    const int at2 = at + (P.r1 - P.r0);
+    int seq2 = seq, base2 = base;
+    if (at2 - base == P.R * HU) {
+      base2 = at2;
+      ++seq2;
+    }
+    const bool more = at2 < end;
+    Piece N = P;
+    if (more) {
+      N = piece_at(seq2, base2, at2);
+      q_fetch(seq2, N);
     }
 
-    // ---- q of head g as A fragments, scaled by a power of two to [2^10, 2^11)
-    AFrag<BF> qf[DP / 16];
-    float qscale;                                // score = product * qscale
-    {
-      const float* q = A.q + (int64_t)seq * A.q_ss + (int64_t)(head0 + g) * A.q_hs;
-      float mx = 0.f;
-      float x[DP / 16][4];
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        // columns 2t, 2t+1, 2t+8, 2t+9 of the operand; e4m3 keys are read
-        // four bytes per lane, which makes them elements 4t .. 4t+3
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int e = 16 * kk + (Cfg::kElem == 1 ? 4 * t + j : 2 * t + (j & 1) + 8 * (j >> 1));
-          x[kk][j] = g < nh && e < D ? q[e] : 0.f;
-          mx = fmaxf(mx, fabsf(x[kk][j]));
-        }
-      }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const int e = mx > 0.f && mx <= 3.4e38f ? 10 - ilogbf(mx) : 0;
-      qscale = ldexpf(A.scale * A.c.k_scale, -e);
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk)
-        qf[kk].set(ldexpf(x[kk][0], e), ldexpf(x[kk][1], e), ldexpf(x[kk][2], e),
-                   ldexpf(x[kk][3], e));
-    }
+    const float qscale = sh.qscale[g];           // score = product * qscale
     const float x2 = qscale * kLog2e;
-
     float o[DP / 8][2];                          // head g, two columns of each 8-wide block
+    float acc[Cfg::kHold ? DP / 8 : 1][4];
 #pragma unroll
     for (int c = 0; c < DP / 8; ++c) o[c][0] = o[c][1] = 0.f;
-    float m = -INFINITY, l = 0.f;                // l: this lane's keys only
+#pragma unroll
+    for (int c = 0; c < (Cfg::kHold ? DP / 8 : 1); ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[c][j] = 0.f;
+    // m: reference of the exponentials, 2^8 below the maximum at most; l: sum
+    // over this lane's keys
+    float m = -INFINITY, l = 0.f;
+    auto fold = [&](float f) {                   // o = (o + acc) * f
+      if (Cfg::kHold) {
+#pragma unroll
+        for (int c = 0; c < DP / 8; ++c) {
+          o[c][0] = (o[c][0] + (acc[c][0] + acc[c][2])) * f;
+          o[c][1] = (o[c][1] + (acc[c][1] + acc[c][3])) * f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[c][j] = 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < DP / 8; ++c) {
+          o[c][0] *= f;
+          o[c][1] *= f;
+        }
+      }
+    };
 
-    for (int i = 0; i < ntile; ++i) {
-      cp_async_wait<NST - 2>();
+    for (int i = 0; i < P.ntile; ++i) {
+      cp_async_wait<NS - 2>();
       __syncwarp();
-      issue(i + NST - 1);
-      fetch(i + NST);
-      const int st = i % NST;
-      const uint32_t ka = ring_a + st * Cfg::kStage, va = ka + KEYS * Cfg::kRow;
-      const uint32_t seen = sh.seen[warp][st];
+      issue_keys();
+      const uint32_t ka = ring_a + cslot * Cfg::kSlot;
+      cslot = cslot + 1 == NS ? 0 : cslot + 1;
+      const uint32_t seen = sh.seen[warp][ctile & 7];
+      ++ctile;
 
       // scores: keys 8b + 2t, 8b + 2t + 1 of head g in this lane
       float x[KEYS / 8][2];
 #pragma unroll
-      for (int kb = 0; kb < KEYS / 16; ++kb) {
-        float s[2][2] = {};
+      for (int b = 0; b < KEYS / 8; ++b) x[b][0] = x[b][1] = 0.f;
 #pragma unroll
-        for (int k4 = 0; k4 < DP / 64; ++k4) {
-          float a[2][4] = {};
-          if (Cfg::kElem == 2) {
+      for (int k4 = 0; k4 < DP / 64; ++k4) {
+        float a[KEYS / 8][4] = {};
 #pragma unroll
-            for (int kk = 4 * k4; kk < 4 * k4 + 4; ++kk) {
-              if (16 * kk < D) {
-                uint32_t b[4];
-                const int row = 16 * kb + (lane >> 4) * 8 + (lane & 7);
-                ldsm4(b, ka + ring_at<CH>(row, 2 * kk + ((lane >> 3) & 1)));
-                qf[kk].mul(a[0], b[0], b[1]);
-                qf[kk].mul(a[1], b[2], b[3]);
+        for (int kk = 4 * k4; kk < 4 * k4 + 4; kk += 3 - Cfg::kElem) {
+          if (16 * kk < D) {
+            AFrag<BF> q0, q1;
+            q0.load(qs + kk * AFrag<BF>::kBytes, lane);
+            if (Cfg::kElem == 1) q1.load(qs + (kk + 1) * AFrag<BF>::kBytes, lane);
+#pragma unroll
+            for (int kb = 0; kb < KEYS / 16; ++kb) {
+              uint32_t b[4];
+              if (Cfg::kElem == 2) {
+                ldsm4(b, ka + ring_at<CH>(16 * kb + krow, 2 * kk + kch));
+                q0.mul(a[2 * kb], b[0], b[1]);
+                q0.mul(a[2 * kb + 1], b[2], b[3]);
+              } else {
+                ldsm4(b, ka + ring_at<CH>(16 * kb + krow, kk + kch));
+                uint32_t f[4][2];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) e4m3x4_f16x2(b[j], f[j][0], f[j][1]);
+                q0.mul(a[2 * kb], f[0][0], f[0][1]);
+                q0.mul(a[2 * kb + 1], f[1][0], f[1][1]);
+                if (16 * (kk + 1) < D) {
+                  q1.mul(a[2 * kb], f[2][0], f[2][1]);
+                  q1.mul(a[2 * kb + 1], f[3][0], f[3][1]);
+                }
               }
             }
-          } else {
-#pragma unroll
-            for (int kk = 4 * k4; kk < 4 * k4 + 4; kk += 2) {
-              if (16 * kk < D) {
-                uint32_t b[4];
-                const int row = 16 * kb + ((lane >> 3) & 1) * 8 + (lane & 7);
-                ldsm4(b, ka + ring_at<CH>(row, kk + (lane >> 4)));
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (16 * (kk + (j >> 1)) < D)
-                    qf[kk + (j >> 1)].mul(a[j & 1], e4m3x2_f16x2(b[j]), e4m3x2_f16x2(b[j] >> 16));
-              }
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            s[j][0] += a[j][0] + a[j][2];
-            s[j][1] += a[j][1] + a[j][3];
           }
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int b = 0; b < KEYS / 8; ++b) {
+          x[b][0] += a[b][0] + a[b][2];
+          x[b][1] += a[b][1] + a[b][3];
+        }
+      }
+      if (A.cap > 0.f) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float v = s[j][h];
-            v = A.cap > 0.f ? A.cap * tanhf(v * qscale / A.cap) * kLog2e : v * x2;
-            x[2 * kb + j][h] = (seen >> (16 * kb + 8 * j + 2 * t + h)) & 1u ? v : -INFINITY;
-          }
+        for (int b = 0; b < KEYS / 8; ++b)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) x[b][h] = A.cap * tanhf(x[b][h] * qscale / A.cap) * kLog2e;
+      } else {
+#pragma unroll
+        for (int b = 0; b < KEYS / 8; ++b)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) x[b][h] *= x2;
+      }
+      if (seen != 0xffffffffu) {                 // lanes past KEYS repeat the first ones
+#pragma unroll
+        for (int b = 0; b < KEYS / 8; ++b)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (!((seen >> (8 * b + 2 * t + h)) & 1u)) x[b][h] = -INFINITY;
       }
 
-      // running maximum and sum
-      float mx = m;
+      // reference and sum
+      float mx = -INFINITY;
 #pragma unroll
       for (int b = 0; b < KEYS / 8; ++b) mx = fmaxf(mx, fmaxf(x[b][0], x[b][1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float ms = mx == -INFINITY ? 0.f : mx;
-      const float keep = ex2(m - ms);
-      m = mx;
-      float sum = 0.f;
+      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+        const float to = mx > m + 8.f ? mx : m;
+        const float f = to == -INFINITY ? 1.f : ex2(m - to);
+        fold(f);
+        l *= f;
+        m = to;
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int b = 0; b < KEYS / 8; ++b)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           x[b][h] = ex2(x[b][h] - ms);
-          sum += x[b][h];
+          l += x[b][h];
         }
-      l = fmaf(l, keep, sum);
       AFrag<BF> pf[KEYS / 16];
 #pragma unroll
       for (int kb = 0; kb < KEYS / 16; ++kb)
-        pf[kb].set(x[2 * kb][0] * 16384.f, x[2 * kb][1] * 16384.f, x[2 * kb + 1][0] * 16384.f,
-                   x[2 * kb + 1][1] * 16384.f);
+        pf[kb].set(x[2 * kb][0] * kPScale, x[2 * kb][1] * kPScale, x[2 * kb + 1][0] * kPScale,
+                   x[2 * kb + 1][1] * kPScale);
 
-      // o = o * keep + p v
-      if (Cfg::kElem == 2) {
+      cp_async_wait<NS - 2>();
+      __syncwarp();
+      issue_values();
+      const uint32_t va = ring_a + cslot * Cfg::kSlot;
+      cslot = cslot + 1 == NS ? 0 : cslot + 1;
+
+      // p v.  e4m3: a 16-byte chunk holds 16 columns; transposed in pairs of
+      // bytes, a register has columns (2g, 2g + 1) of two keys, which become
+      // the B registers of the even and of the odd columns
+      constexpr int CPB = Cfg::kElem == 2 ? 2 : 4;      // 8-wide blocks of two chunks
 #pragma unroll
-        for (int c = 0; c < DP / 8; c += 2) {
-          if (8 * c < D) {
-            float a[2][4] = {};
+      for (int c = 0; c < DP / 8; c += CPB) {
+        if (8 * c < D) {
+          float tmp[CPB][4] = {};
 #pragma unroll
-            for (int kb = 0; kb < KEYS / 16; ++kb) {
-              uint32_t b[4];
-              const int row = 16 * kb + ((lane >> 3) & 1) * 8 + (lane & 7);
-              ldsm4_t(b, va + ring_at<CH>(row, c + (lane >> 4)));
-              pf[kb].mul(a[0], b[0], b[1]);
-              pf[kb].mul(a[1], b[2], b[3]);
-            }
+          for (int kb = 0; kb < KEYS / 16; ++kb) {
+            uint32_t b[4];
+            ldsm4_t(b, va + ring_at<CH>(16 * kb + vrow, (Cfg::kElem == 2 ? c : c / 2) + vch));
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              o[c + j][0] = fmaf(o[c + j][0], keep, a[j][0] + a[j][2]);
-              o[c + j][1] = fmaf(o[c + j][1], keep, a[j][1] + a[j][3]);
+              if (Cfg::kElem == 2) {
+                pf[kb].mul(Cfg::kHold ? acc[(c + j) * Cfg::kHold] : tmp[j], b[2 * j], b[2 * j + 1]);
+              } else if (8 * c + 16 * j < D) {
+                uint32_t k0, k1, k8, k9;
+                e4m3x4_f16x2(b[2 * j], k0, k1);
+                e4m3x4_f16x2(b[2 * j + 1], k8, k9);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  pf[kb].mul(Cfg::kHold ? acc[(c + 2 * j + h) * Cfg::kHold]
+                                        : tmp[(2 * j + h) % CPB],
+                             prmt(k0, k1, h ? 0x7632u : 0x5410u),
+                             prmt(k8, k9, h ? 0x7632u : 0x5410u));
+              }
             }
           }
-        }
-      } else {
-        // a 16-byte chunk holds 16 columns; transposed in pairs of bytes, a
-        // register has columns (2g, 2g + 1) of two keys, which become the
-        // B registers of the even and of the odd columns
+          if (!Cfg::kHold) {
 #pragma unroll
-        for (int c = 0; c < DP / 16; c += 2) {
-          if (16 * c < D) {
-            float a[2][2][4] = {};
-#pragma unroll
-            for (int kb = 0; kb < KEYS / 16; ++kb) {
-              uint32_t b[4];
-              const int row = 16 * kb + ((lane >> 3) & 1) * 8 + (lane & 7);
-              ldsm4_t(b, va + ring_at<CH>(row, c + (lane >> 4)));
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                if (16 * (c + j) < D) {
-                  const uint32_t k0 = e4m3x2_f16x2(b[2 * j]), k1 = e4m3x2_f16x2(b[2 * j] >> 16);
-                  const uint32_t k8 = e4m3x2_f16x2(b[2 * j + 1]),
-                                 k9 = e4m3x2_f16x2(b[2 * j + 1] >> 16);
-                  pf[kb].mul(a[j][0], prmt(k0, k1, 0x5410u), prmt(k8, k9, 0x5410u));
-                  pf[kb].mul(a[j][1], prmt(k0, k1, 0x7632u), prmt(k8, k9, 0x7632u));
-                }
-              }
+            for (int j = 0; j < CPB; ++j) {
+              o[c + j][0] += tmp[j][0] + tmp[j][2];
+              o[c + j][1] += tmp[j][1] + tmp[j][3];
             }
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int b = 2 * (c + j) + h;
-                o[b][0] = fmaf(o[b][0], keep, a[j][h][0] + a[j][h][2]);
-                o[b][1] = fmaf(o[b][1], keep, a[j][h][1] + a[j][h][3]);
-              }
           }
         }
       }
+      if (Cfg::kHold && i % Cfg::kFold == Cfg::kFold - 1) fold(1.f);
     }
+    if (Cfg::kHold) fold(1.f);
 
     // ---- the warps' parts meet in shared memory
-    cp_async_wait<0>();
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (t == 0) {
       sh.m[warp][g] = m;
       sh.l[warp][g] = l;
     }
-    __syncthreads();                             // every ring is idle
-    float* const mo = reinterpret_cast<float*>(smem);
     {
       float* row = mo + (warp * kAttHeads + g) * Cfg::kMergeRow;
 #pragma unroll
@@ -517,35 +653,45 @@ attention_kernel(const AttArgs A) {
         }
       }
     }
+    if (more) q_max();
     __syncthreads();
-    const bool whole = r0 == 0 && r1 == R;
-    const int my_slot = 2 * blockIdx.x + (r0 == 0 ? 1 : 0);
-    for (int e = tid; e < nh * D; e += NT) {
-      const int h = e / D, c = e - h * D;
+    const bool whole = P.r0 == 0 && P.r1 == P.R;
+    const int my_slot = 2 * blockIdx.x + (P.r0 == 0 ? 1 : 0);
+    const float unit = A.c.v_scale / kPScale;
+    for (int h = warp; h < P.nh; h += NW) {
       float M = sh.m[0][h];
 #pragma unroll
       for (int w = 1; w < NW; ++w) M = fmaxf(M, sh.m[w][h]);
       const float ms = M == -INFINITY ? 0.f : M;
-      float L = 0.f, y = 0.f;
+      float L = 0.f, f[NW];
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float f = ex2(sh.m[w][h] - ms);
-        L = fmaf(sh.l[w][h], f, L);
-        y = fmaf(mo[(w * kAttHeads + h) * Cfg::kMergeRow + c], f, y);
+        f[w] = ex2(sh.m[w][h] - ms);
+        L = fmaf(sh.l[w][h], f[w], L);
       }
-      if (whole) {
-        const int64_t row = (int64_t)seq * A.hq + head0 + h;
-        A.out[row * D + c] = L == 0.f ? 0.f : y * (1.f / 16384.f) * A.c.v_scale / L;
-        if (c == 0 && A.lse) A.lse[row] = (M + log2f(L)) * kLn2;
-      } else {
-        A.part_o[((int64_t)my_slot * kAttHeads + h) * DP + c] = y;
-        if (c == 0) A.part_ml[my_slot * kAttHeads + h] = make_float2(M, L);
+      const int64_t row = (int64_t)seq * A.hq + P.head0 + h;
+      for (int c = lane; c < D; c += 32) {
+        float y = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w)
+          y = fmaf(mo[(w * kAttHeads + h) * Cfg::kMergeRow + c], f[w], y);
+        if (whole)
+          A.out[row * D + c] = L == 0.f ? 0.f : y * unit / L;
+        else
+          A.part_o[((int64_t)my_slot * kAttHeads + h) * DP + c] = y;
+      }
+      if (lane == 0) {
+        if (!whole)
+          A.part_ml[my_slot * kAttHeads + h] = make_float2(M, L);
+        else if (A.lse)
+          A.lse[row] = (M + log2f(L)) * kLn2;
       }
     }
+    if (more) q_split();
     if (!whole) {
       // ---- the last CTA of a unit to arrive joins the unit's parts, in order
-      const int c0 = (int)(ustart / quota);
-      const int n = (int)((ustart + R - 1) / quota) - c0 + 1;
+      const int c0 = (int)((start + P.ustart) / quota);
+      const int n = (int)((start + P.ustart + P.R - 1) / quota) - c0 + 1;
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -557,48 +703,45 @@ attention_kernel(const AttArgs A) {
       if (sh.last) {
         __threadfence();
         // weights of the parts, [head][part]; mo is free again
-        for (int h = warp; h < nh; h += NW) {
+        for (int h = warp; h < P.nh; h += NW) {
+          const float2* ml = A.part_ml + (int64_t)2 * c0 * kAttHeads + h;
           float M = -INFINITY;
           for (int i = lane; i < n; i += 32)
-            M = fmaxf(M, __ldcg(A.part_ml + (2 * (c0 + i) + (i == 0)) * kAttHeads + h).x);
+            M = fmaxf(M, __ldcg(ml + (2 * i + (i == 0)) * kAttHeads).x);
 #pragma unroll
           for (int b = 16; b > 0; b >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, b));
           const float ms = M == -INFINITY ? 0.f : M;
           float L = 0.f;
           for (int i = lane; i < n; i += 32) {
-            const float2 v = __ldcg(A.part_ml + (2 * (c0 + i) + (i == 0)) * kAttHeads + h);
+            const float2 v = __ldcg(ml + (2 * i + (i == 0)) * kAttHeads);
             const float f = ex2(v.x - ms);
             mo[h * n + i] = f;
             L = fmaf(v.y, f, L);
           }
 #pragma unroll
           for (int b = 16; b > 0; b >>= 1) L += __shfl_xor_sync(0xffffffffu, L, b);
-          if (lane == 0) {
-            sh.m[0][h] = M;
-            sh.l[0][h] = L;
-          }
-        }
-        __syncthreads();
-        for (int e = tid; e < nh * D; e += NT) {
-          const int h = e / D, c = e - h * D;
-          const float* po = A.part_o + ((int64_t)2 * c0 * kAttHeads + h) * DP + c;
-          float y = __ldcg(po + kAttHeads * DP) * mo[h * n];
+          __syncwarp();
+          const int64_t row = (int64_t)seq * A.hq + P.head0 + h;
+          for (int c = lane; c < D; c += 32) {
+            const float* po = A.part_o + ((int64_t)2 * c0 * kAttHeads + h) * DP + c;
+            float y = __ldcg(po + kAttHeads * DP) * mo[h * n];
 #pragma unroll 8
-          for (int i = 1; i < n; ++i) y = fmaf(__ldcg(po + (int64_t)2 * i * kAttHeads * DP), mo[h * n + i], y);
-          const float L = sh.l[0][h];
-          const int64_t row = (int64_t)seq * A.hq + head0 + h;
-          A.out[row * D + c] = L == 0.f ? 0.f : y * (1.f / 16384.f) * A.c.v_scale / L;
-          if (c == 0 && A.lse) A.lse[row] = (sh.m[0][h] + log2f(L)) * kLn2;
+            for (int i = 1; i < n; ++i)
+              y = fmaf(__ldcg(po + (int64_t)2 * i * kAttHeads * DP), mo[h * n + i], y);
+            A.out[row * D + c] = L == 0.f ? 0.f : y * unit / L;
+          }
+          if (lane == 0 && A.lse) A.lse[row] = (M + log2f(L)) * kLn2;
         }
       }
     }
-    __syncthreads();                             // mo and sh are rings and stages again
-    at += r1 - r0;
-    if (at - base == (long long)R * HU) {
-      base = at;
-      ++seq;
-    }
+    if (!more) break;
+    __syncthreads();                             // q of the next piece; mo and sh are free
+    at = at2;
+    seq = seq2;
+    base = base2;
+    P = N;
   }
+  cp_async_wait<0>();
 }
 
 // ---------------------------------------------------------------------------
@@ -625,8 +768,8 @@ static int attention_workspace(int head_dim, AttArgs* a, void* ws, size_t* bytes
 template <int DT, int DP>
 static int launch_attention(const AttArgs& a, int max_len, cudaStream_t s) {
   using Cfg = AttCfg<DT, DP>;
-  static_assert(Cfg::kStages >= 2 && Cfg::kStages <= 8 && Cfg::kCtasPerSm <= kAttMaxCtasPerSm, "");
-  static_assert(kAttHeads * kAttMaxCtasPerSm * 160 * 4 <= Cfg::kSmem, "weights of a unit's parts");
+  static_assert(Cfg::kSlots % 2 == 1 && (Cfg::kSlots + 1) / 2 <= 8 && Cfg::kWarps == 4, "");
+  static_assert(Cfg::kCtasPerSm <= kAttMaxCtasPerSm, "");
   static std::atomic<uint64_t> ready{0};
   auto kern = attention_kernel<DT, DP>;
   int dev = 0;
@@ -640,6 +783,14 @@ static int launch_attention(const AttArgs& a, int max_len, cudaStream_t s) {
   const int64_t keys = a.window > 0 ? std::min(a.window, max_len) : max_len;
   const int64_t rounds = units * std::max<int64_t>(1, (keys + Cfg::kRound - 1) / Cfg::kRound);
   const int grid = (int)std::min<int64_t>(rounds, (int64_t)Cfg::kCtasPerSm * sm_count());
+  // a CTA counts its rounds, and a sequence's, in 32 bits
+  const int64_t most = (int64_t)a.c.table_width * a.c.page_size / Cfg::kRound + 1;
+  MOE_REQUIRE(units / a.c.seqs * most < (1ll << 30) && units * most / grid < (1ll << 30),
+              MOE_ERR_UNSUPPORTED, "%d sequences of up to %d pages are too many", a.c.seqs,
+              a.c.table_width);
+  // the weights of a unit's parts fit into the merge rows
+  MOE_REQUIRE(kAttHeads * grid * 4 <= Cfg::kMerge, MOE_ERR_UNSUPPORTED, "%d CTAs are too many",
+              grid);
   MOE_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(Cfg::kWarps * 32), Cfg::kSmem, s, a));
   return MOE_OK;
 }
