@@ -17,10 +17,14 @@
 // them to finish, from f32 partials in the workspace, in the order of its
 // keys; the arrival counters return to zero.
 //
-// A warp takes every NW-th tile of KEYS keys through a ring of its own
-// (cp.async, 16 bytes at a time, rows swizzled so that ldmatrix meets no bank
-// twice); the warps meet only at the end of a unit.  Page ids are fetched one
-// tile ahead of the rows they lead to.
+// A warp takes every NW-th tile of KEYS keys through a ring of its own, keys
+// and values in slots of their own; the warps meet only at the end of a unit.
+// Slots are filled by TMA in boxes of as many rows as are sure to lie in one
+// page (the largest power of two up to KEYS that divides the page size) and 128
+// bytes, swizzled so that ldmatrix meets no bank twice: two instructions per
+// box instead of two per 16 bytes, without which a tile's copies cost more
+// instructions than its arithmetic.  The load cursor runs ahead across the ends
+// of units; page ids are fetched one tile ahead of the rows they lead to.
 //
 // Precision.  q has f32 rows, so it enters the products in parts: hi + lo fp16
 // (22 bits) for fp16 and e4m3 caches, three bf16 parts for bf16 caches.  With
@@ -34,8 +38,10 @@
 
 #include <algorithm>
 #include <atomic>
+#include <numeric>
 
 #include "paged_cache.cuh"
+#include "tc_common.cuh"
 
 namespace moe {
 
@@ -47,6 +53,8 @@ constexpr float kPScale = 128.f;      // probabilities enter the products times 
 
 struct AttArgs {
   moe_paged_cache c;
+  int page_units, head_units;         // strides in rows of the tensor maps
+  int box_shift;                      // log2 of the rows of a TMA box
   const float* q;
   int64_t q_ss, q_hs;
   const int32_t* seq_lens;
@@ -74,17 +82,23 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(bytes)
-               : "memory");
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                            int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -92,19 +106,22 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-template <bool BF>
+// d = a b (+ d unless FIRST)
+template <bool BF, bool FIRST>
 __device__ __forceinline__ void mma_acc(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  const float c0 = FIRST ? 0.f : d[0], c1 = FIRST ? 0.f : d[1], c2 = FIRST ? 0.f : d[2],
+              c3 = FIRST ? 0.f : d[3];
   if (BF)
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
-        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   else
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 // two adjacent values -> NP packed parts that add up to them (22 bits of fp16,
@@ -144,9 +161,10 @@ template <bool BF> struct AFrag {
     split2<BF, kParts>(x0, x1, lo);
     split2<BF, kParts>(x2, x3, hi);
   }
+  template <bool FIRST = false>
   __device__ __forceinline__ void mul(float (&d)[4], uint32_t b0, uint32_t b1) const {
-    mma_acc<BF>(d, lo[0], lo[1], hi[0], hi[1], b0, b1);
-    if (BF) mma_acc<BF>(d, lo[kParts - 1], 0u, hi[kParts - 1], 0u, b0, b1);
+    mma_acc<BF, FIRST>(d, lo[0], lo[1], hi[0], hi[1], b0, b1);
+    if (BF) mma_acc<BF, false>(d, lo[kParts - 1], 0u, hi[kParts - 1], 0u, b0, b1);
   }
   // in shared memory: 16 bytes per lane, then for bf16 8 more
   static constexpr int kBytes = 32 * 8 * kParts;
@@ -174,15 +192,15 @@ template <bool BF> struct AFrag {
 // keys or the values of a tile; an odd number of slots makes the slot freed
 // by keys the next one that keys go to.
 // ---------------------------------------------------------------------------
+constexpr int kLine = 128;             // bytes of a row in one box
 template <int DT, int DP> struct AttCfg {
   static constexpr bool kBf = DT == MOE_CACHE_BF16;
   static constexpr int kElem = DT == MOE_CACHE_E4M3 ? 1 : 2;
-  static constexpr int kRow = DP * kElem;                   // bytes of a row in the ring
-  static constexpr int kChunks = kRow / 16;
+  static constexpr int kRow = DP * kElem < kLine ? kLine : DP * kElem;   // bytes in the ring
   static constexpr int kWarps = 4;
   static constexpr int kKeys = kRow <= 128 ? 32 : 16;       // keys of a warp's tile
   static constexpr int kSlot = kKeys * kRow;
-  static constexpr int kSlots = kSlot <= 2048 ? 9 : 5;
+  static constexpr int kSlots = 5;
   static constexpr int kRound = kWarps * kKeys;
   static constexpr int kRing = kWarps * kSlots * kSlot;
   static constexpr int kMergeRow = DP + 8;                  // floats
@@ -198,39 +216,44 @@ template <int DT, int DP> struct AttCfg {
   static constexpr int kFold = 64 / kKeys;
 };
 
-// swizzled byte offset of 16-byte chunk c of ring row r
-template <int CHUNKS>
-__device__ __forceinline__ uint32_t ring_at(int r, int c) {
-  const int x = CHUNKS >= 8 ? (r & 7) : ((r >> 1) & 3);
-  return (uint32_t)(r * CHUNKS * 16 + ((c ^ x) << 4));
+// byte offset of 16-byte chunk c of row r in a slot: blocks of KEYS lines,
+// swizzled as TMA swizzles them
+template <int KEYS>
+__device__ __forceinline__ uint32_t slot_at(int r, int c) {
+  return (uint32_t)((c >> 3) * KEYS * kLine + r * kLine + (((c & 7) ^ (r & 7)) << 4));
 }
 
 struct AttShared {
   long long base, scan[4];
-  int seq, last;
+  int seq, last, dead;
+  uint64_t bars[4][5];               // a barrier per ring slot
   uint32_t seen[4][8];               // valid keys of the tiles in each warp's ring
   float m[4][kAttHeads], l[4][kAttHeads], qmax[4][kAttHeads], qscale[kAttHeads];
 };
 
 // One CTA's part of a unit: rounds r0 .. r1 of R.
 struct Piece {
-  int ustart, R, r0, r1, head0, nh, kw, khi, ntile;
-  int64_t head_off;
+  int ustart, R, r0, r1, head0, nh, head, first, kw, khi, ntile;
 };
 
 template <int DT, int DP>
 __global__ void __launch_bounds__(AttCfg<DT, DP>::kWarps * 32, AttCfg<DT, DP>::kCtasPerSm)
-attention_kernel(const AttArgs A) {
+attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                 const AttArgs A) {
   using Cfg = AttCfg<DT, DP>;
   constexpr bool BF = Cfg::kBf;
   constexpr int NW = Cfg::kWarps, NT = NW * 32, KEYS = Cfg::kKeys, NS = Cfg::kSlots;
-  constexpr int CH = Cfg::kChunks, RK = Cfg::kRound;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int LINE = kLine, RK = Cfg::kRound;
+  extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ AttShared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int S = A.c.seqs, D = A.c.head_dim, G = A.hq / A.c.kv_heads;
   const int NHT = (G + kAttHeads - 1) / kAttHeads, HU = A.c.kv_heads * NHT;
   const int most = A.c.table_width * A.c.page_size;
+  if (lane < NS) {
+    mbar_init(&sh.bars[warp][lane], 1);
+    fence_mbar_init();
+  }
   pdl_trigger();
   pdl_wait();
 
@@ -240,10 +263,12 @@ attention_kernel(const AttArgs A) {
     first = A.window > 0 && n > A.window ? n - A.window : 0;
     return n;
   };
+  // rounds start at a multiple of KEYS, so that no box crosses a page's end;
+  // an empty sequence has one too, which writes its zeros
   auto rounds_of = [&](int s) {
     int first;
     const int n = keys_of(s, first);
-    return max(1, (n - first + RK - 1) / RK);   // an empty sequence still writes its zeros
+    return max(1, (n - first / KEYS * KEYS + RK - 1) / RK);
   };
   const int per = (S + NT - 1) / NT, s0 = min(S, tid * per), s1 = min(S, s0 + per);
   long long mine = 0;
@@ -265,6 +290,7 @@ attention_kernel(const AttArgs A) {
     if (w < warp) before += sh.scan[w];
     total += sh.scan[w];
   }
+  if (tid == 0) sh.dead = 0;
   const int quota = (int)((total + gridDim.x - 1) / gridDim.x);
   const long long start = (long long)blockIdx.x * quota;
   if (start >= total) return;
@@ -288,7 +314,8 @@ attention_kernel(const AttArgs A) {
     Piece p;
     int first;
     const int len = keys_of(s, first);
-    p.R = max(1, (len - first + RK - 1) / RK);
+    const int from = first / KEYS * KEYS;
+    p.R = max(1, (len - from + RK - 1) / RK);
     const int u = (at - base) / p.R;
     p.ustart = base + u * p.R;
     p.r0 = at - p.ustart;
@@ -296,32 +323,38 @@ attention_kernel(const AttArgs A) {
     const int kvh = u / NHT;
     p.head0 = kvh * G + (u - kvh * NHT) * kAttHeads;
     p.nh = min(kAttHeads, kvh * G + G - p.head0);
-    p.kw = first + p.r0 * RK + warp * KEYS;     // tiles of this warp: kw + i * RK ...
-    p.khi = min(len, first + p.r1 * RK);
+    p.first = first;
+    p.kw = from + p.r0 * RK + warp * KEYS;      // tiles of this warp: kw + i * RK ...
+    p.khi = min(len, from + p.r1 * RK);
     p.ntile = p.khi > p.kw ? (p.khi - p.kw + RK - 1) / RK : 0;
-    p.head_off = (int64_t)kvh * A.c.head_stride;
+    p.head = kvh;
     return p;
   };
 
   // ---- loads: a cursor of its own that runs ahead of the arithmetic, across
   // the ends of units
   const uint32_t ring_a = smem_u32(smem) + warp * NS * Cfg::kSlot;
-  const uint8_t* const kbase = static_cast<const uint8_t*>(A.c.k);
-  const uint8_t* const vbase = static_cast<const uint8_t*>(A.c.v);
-  const int chunks = (D * Cfg::kElem + 15) / 16;               // chunks of a row in memory
-  const int zchunks = ((D + 15) / 16 * 16) * Cfg::kElem / 16;  // with the zeros of a half step
+  constexpr int BLOCKS = DP * Cfg::kElem < LINE ? 1 : DP * Cfg::kElem / LINE;
+  const int box = 1 << A.box_shift, boxes = KEYS >> A.box_shift, ps = A.c.page_size;
+  const int step_pages = RK / ps, step_slots = RK - step_pages * ps;   // from tile to tile
   int lseq = seq0, lbase = base0, lat = 0, li = 0, lslot = 0;
   uint32_t ltile = 0;
   Piece lp = piece_at(lseq, lbase, lat);
-  int page = 0, slot = 0;
+  // of this lane's box of tile li: number in the sequence's pages and slot,
+  // row of the tensor map
+  int pidx = 0, pslot = 0, row = 0, key = 0, page = 0;
   bool in = false;
-  int64_t off = -1;                              // this lane's row of the tile, bytes
+  auto enter = [&]() {                           // first tile of a piece
+    li = 0;
+    key = lp.kw + (lane << A.box_shift);
+    pidx = (int)((unsigned)key / (unsigned)ps);
+    pslot = key - pidx * ps;
+  };
   auto settle = [&]() {                          // to the next piece that has a tile li
     while (li >= lp.ntile) {
       lat += lp.r1 - lp.r0;
       if (lat >= end) {
-        lp.ntile = 0x7fffffff;                   // nothing left: tiles without rows
-        lp.khi = lp.kw = 0;
+        lp.ntile = 0x7fffffff;                   // nothing left
         break;
       }
       if (lat - lbase == lp.R * HU) {
@@ -329,57 +362,78 @@ attention_kernel(const AttArgs A) {
         ++lseq;
       }
       lp = piece_at(lseq, lbase, lat);
-      li = 0;
+      enter();
     }
   };
-  auto fetch = [&]() {                           // page of this lane's key of tile li
-    const int key = lp.kw + li * RK + (lane & (KEYS - 1));
-    in = lat < end && key < lp.khi;
+  auto fetch = [&]() {                           // page of this lane's box of tile li
+    in = lat < end && lane < boxes && key < lp.khi && key + box > lp.first;
+    if (in) page = A.c.block_table[(int64_t)lseq * A.c.table_stride + pidx];
+  };
+  auto copy = [&](const CUtensorMap* map, int n) {
+    uint64_t* bar = &sh.bars[warp][lslot];
+    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(n * BLOCKS * LINE) << A.box_shift);
+    __syncwarp();
     if (in) {
-      const int p = (int)((unsigned)key / (unsigned)A.c.page_size);
-      slot = key - p * A.c.page_size;
-      page = A.c.block_table[(int64_t)lseq * A.c.table_stride + p];
-    }
-  };
-  auto copy = [&](const uint8_t* from) {
-    if (lat < end) {
-      const uint32_t dst = ring_a + lslot * Cfg::kSlot;
-      constexpr int LPR = CH < 32 ? CH : 32, RPI = 32 / LPR;   // lanes per row, rows at once
+      const uint32_t dst = ring_a + lslot * Cfg::kSlot + (lane << A.box_shift) * LINE;
 #pragma unroll
-      for (int r = 0; r < KEYS; r += RPI) {
-        const int row = r + lane / LPR, c = lane % LPR;
-        const int64_t o = __shfl_sync(0xffffffffu, off, row);
-        if (c < zchunks) {
-          const uint32_t n = o >= 0 && c < chunks ? 16u : 0u;
-          cp_async16(dst + ring_at<CH>(row, c), from + (n ? o + c * 16 : 0), n);
-        }
-      }
+      for (int b = 0; b < BLOCKS; ++b)
+        tma_load_3d(dst + b * KEYS * LINE, map, b * (LINE / Cfg::kElem), row, pslot, bar);
     }
-    cp_async_commit();
     lslot = lslot + 1 == NS ? 0 : lslot + 1;
   };
+  uint32_t lok = 0;                              // boxes of the tile that exist
   auto issue_keys = [&]() {
-    off = -1;
-    if (in) {
-      if (page >= 0 && page < A.c.pages)
-        off = ((int64_t)page * A.c.page_stride + (int64_t)slot * A.c.token_stride + lp.head_off) *
-              Cfg::kElem;
-      else
-        set_status(A.status, MOE_STATUS_BAD_PAGE);
+    if (lat >= end) return;
+    if (in && (page < 0 || page >= A.c.pages)) {
+      set_status(A.status, MOE_STATUS_BAD_PAGE);
+      in = false;
     }
-    const uint32_t ok = __ballot_sync(0xffffffffu, off >= 0);
-    if (lane == 0) sh.seen[warp][ltile & 7] = ok;
+    row = page * A.page_units + lp.head * A.head_units;
+    lok = __ballot_sync(0xffffffffu, in);
+    const int k0 = lp.kw + li * RK;
+    uint32_t seen = 0xffffffffu;
+    if (__popc(lok) != boxes || k0 < lp.first || k0 + KEYS > lp.khi) {
+      const int r = lane & (KEYS - 1);
+      seen = __ballot_sync(0xffffffffu, k0 + r >= lp.first && k0 + r < lp.khi &&
+                                            ((lok >> (r >> A.box_shift)) & 1u));
+    }
+    if (lane == 0) sh.seen[warp][ltile & 7] = seen;
     ++ltile;
-    copy(kbase);
+    copy(&kmap, __popc(lok));
   };
   auto issue_values = [&]() {
-    copy(vbase);
-    if (lat < end) {
-      ++li;
-      settle();
-      fetch();
+    if (lat >= end) return;
+    copy(&vmap, __popc(lok));
+    ++li;
+    key += RK;
+    pidx += step_pages;
+    pslot += step_slots;
+    if (pslot >= ps) {
+      pslot -= ps;
+      ++pidx;
     }
+    settle();
+    fetch();
   };
+  // Waits for the slot that is due.  Bounded; after a timeout anywhere in the
+  // CTA no wait takes long any more, so that the kernel ends.
+  int cslot = 0;
+  uint32_t cphase = 0;
+  auto wait_slot = [&]() {
+    uint64_t* bar = &sh.bars[warp][cslot];
+    if (!mbar_test(bar, cphase) && !*(volatile int*)&sh.dead && !mbar_wait(bar, cphase)) {
+      sh.dead = 1;
+      set_status(A.status, MOE_STATUS_TIMEOUT);
+    }
+    __syncwarp();
+    const uint32_t a = ring_a + cslot * Cfg::kSlot;
+    if (++cslot == NS) {
+      cslot = 0;
+      cphase ^= 1u;
+    }
+    return a;
+  };
+  enter();
   settle();
   fetch();
 #pragma unroll
@@ -430,7 +484,7 @@ attention_kernel(const AttArgs A) {
     }
   };
 
-  int seq = seq0, base = base0, at = 0, cslot = 0;
+  int seq = seq0, base = base0, at = 0;
   uint32_t ctile = 0;
   Piece P = piece_at(seq, base, at);
   q_fetch(seq, P);
@@ -439,10 +493,21 @@ attention_kernel(const AttArgs A) {
   q_split();
   __syncthreads();
 
-  // lane constants of the fragment addresses
-  const int krow = Cfg::kElem == 2 ? (lane >> 4) * 8 + (lane & 7) : ((lane >> 3) & 1) * 8 + (lane & 7);
+  // lane constants of the fragment addresses: row, and for each of the four
+  // chunk pairs of a line the swizzled offset
+  const int krow = Cfg::kElem == 2 ? (lane >> 4) * 8 + (lane & 7)
+                                   : ((lane >> 3) & 1) * 8 + (lane & 7);
   const int kch = Cfg::kElem == 2 ? (lane >> 3) & 1 : lane >> 4;
   const int vrow = ((lane >> 3) & 1) * 8 + (lane & 7), vch = lane >> 4;
+  uint32_t kof[LINE / 32], vof[LINE / 32];
+#pragma unroll
+  for (int j = 0; j < LINE / 32; ++j) {
+    kof[j] = slot_at<KEYS>(krow, 2 * j + kch);
+    vof[j] = slot_at<KEYS>(vrow, 2 * j + vch);
+  }
+  // chunk pair j of a row block of 16: offset beyond kof / vof
+  constexpr int PPL = LINE / 32;                 // chunk pairs of a line
+  auto beyond = [](int j, int kb) { return (uint32_t)((j / PPL) * KEYS * LINE + kb * 16 * LINE); };
 
   for (;;) {
     // the piece after this one, and its q
@@ -491,53 +556,55 @@ attention_kernel(const AttArgs A) {
     };
 
     for (int i = 0; i < P.ntile; ++i) {
-      cp_async_wait<NS - 2>();
-      __syncwarp();
+      const uint32_t ka = wait_slot();
       issue_keys();
-      const uint32_t ka = ring_a + cslot * Cfg::kSlot;
-      cslot = cslot + 1 == NS ? 0 : cslot + 1;
       const uint32_t seen = sh.seen[warp][ctile & 7];
       ++ctile;
 
-      // scores: keys 8b + 2t, 8b + 2t + 1 of head g in this lane
+      // scores: keys 8b + 2t, 8b + 2t + 1 of head g in this lane.  Columns past
+      // head_dim are zeros in the ring and in q
       float x[KEYS / 8][2];
 #pragma unroll
-      for (int b = 0; b < KEYS / 8; ++b) x[b][0] = x[b][1] = 0.f;
-#pragma unroll
       for (int k4 = 0; k4 < DP / 64; ++k4) {
-        float a[KEYS / 8][4] = {};
+        float a[KEYS / 8][4];
 #pragma unroll
         for (int kk = 4 * k4; kk < 4 * k4 + 4; kk += 3 - Cfg::kElem) {
-          if (16 * kk < D) {
-            AFrag<BF> q0, q1;
-            q0.load(qs + kk * AFrag<BF>::kBytes, lane);
-            if (Cfg::kElem == 1) q1.load(qs + (kk + 1) * AFrag<BF>::kBytes, lane);
+          AFrag<BF> q0, q1;
+          q0.load(qs + kk * AFrag<BF>::kBytes, lane);
+          if (Cfg::kElem == 1) q1.load(qs + (kk + 1) * AFrag<BF>::kBytes, lane);
 #pragma unroll
-            for (int kb = 0; kb < KEYS / 16; ++kb) {
-              uint32_t b[4];
-              if (Cfg::kElem == 2) {
-                ldsm4(b, ka + ring_at<CH>(16 * kb + krow, 2 * kk + kch));
+          for (int kb = 0; kb < KEYS / 16; ++kb) {
+            uint32_t b[4];
+            const int j = Cfg::kElem == 2 ? kk : kk / 2;
+            ldsm4(b, ka + kof[j % PPL] + beyond(j, kb));
+            if (Cfg::kElem == 2) {
+              if (kk == 4 * k4) {
+                q0.template mul<true>(a[2 * kb], b[0], b[1]);
+                q0.template mul<true>(a[2 * kb + 1], b[2], b[3]);
+              } else {
                 q0.mul(a[2 * kb], b[0], b[1]);
                 q0.mul(a[2 * kb + 1], b[2], b[3]);
-              } else {
-                ldsm4(b, ka + ring_at<CH>(16 * kb + krow, kk + kch));
-                uint32_t f[4][2];
+              }
+            } else {
+              uint32_t f[4][2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) e4m3x4_f16x2(b[j], f[j][0], f[j][1]);
+              for (int i = 0; i < 4; ++i) e4m3x4_f16x2(b[i], f[i][0], f[i][1]);
+              if (kk == 4 * k4) {
+                q0.template mul<true>(a[2 * kb], f[0][0], f[0][1]);
+                q0.template mul<true>(a[2 * kb + 1], f[1][0], f[1][1]);
+              } else {
                 q0.mul(a[2 * kb], f[0][0], f[0][1]);
                 q0.mul(a[2 * kb + 1], f[1][0], f[1][1]);
-                if (16 * (kk + 1) < D) {
-                  q1.mul(a[2 * kb], f[2][0], f[2][1]);
-                  q1.mul(a[2 * kb + 1], f[3][0], f[3][1]);
-                }
               }
+              q1.mul(a[2 * kb], f[2][0], f[2][1]);
+              q1.mul(a[2 * kb + 1], f[3][0], f[3][1]);
             }
           }
         }
 #pragma unroll
         for (int b = 0; b < KEYS / 8; ++b) {
-          x[b][0] += a[b][0] + a[b][2];
-          x[b][1] += a[b][1] + a[b][3];
+          x[b][0] = (k4 ? x[b][0] : 0.f) + (a[b][0] + a[b][2]);
+          x[b][1] = (k4 ? x[b][1] : 0.f) + (a[b][1] + a[b][3]);
         }
       }
       if (A.cap > 0.f) {
@@ -586,11 +653,17 @@ attention_kernel(const AttArgs A) {
         pf[kb].set(x[2 * kb][0] * kPScale, x[2 * kb][1] * kPScale, x[2 * kb + 1][0] * kPScale,
                    x[2 * kb + 1][1] * kPScale);
 
-      cp_async_wait<NS - 2>();
-      __syncwarp();
+      const uint32_t va = wait_slot();
       issue_values();
-      const uint32_t va = ring_a + cslot * Cfg::kSlot;
-      cslot = cslot + 1 == NS ? 0 : cslot + 1;
+      if (seen != 0xffffffffu) {                 // nothing of a row that is not seen counts
+        for (int r = 0; r < KEYS; ++r)
+          if (!((seen >> r) & 1u) && lane < Cfg::kRow / 16) {
+            const uint32_t to = va + slot_at<KEYS>(r, lane);
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(to), "r"(0) : "memory");
+          }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
 
       // p v.  e4m3: a 16-byte chunk holds 16 columns; transposed in pairs of
       // bytes, a register has columns (2g, 2g + 1) of two keys, which become
@@ -598,35 +671,44 @@ attention_kernel(const AttArgs A) {
       constexpr int CPB = Cfg::kElem == 2 ? 2 : 4;      // 8-wide blocks of two chunks
 #pragma unroll
       for (int c = 0; c < DP / 8; c += CPB) {
-        if (8 * c < D) {
-          float tmp[CPB][4] = {};
+        float tmp[CPB][4];
 #pragma unroll
-          for (int kb = 0; kb < KEYS / 16; ++kb) {
-            uint32_t b[4];
-            ldsm4_t(b, va + ring_at<CH>(16 * kb + vrow, (Cfg::kElem == 2 ? c : c / 2) + vch));
+        for (int kb = 0; kb < KEYS / 16; ++kb) {
+          uint32_t b[4];
+          const int pair = Cfg::kElem == 2 ? c / 2 : c / 4;
+          ldsm4_t(b, va + vof[pair % PPL] + beyond(pair, kb));
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              if (Cfg::kElem == 2) {
-                pf[kb].mul(Cfg::kHold ? acc[(c + j) * Cfg::kHold] : tmp[j], b[2 * j], b[2 * j + 1]);
-              } else if (8 * c + 16 * j < D) {
-                uint32_t k0, k1, k8, k9;
-                e4m3x4_f16x2(b[2 * j], k0, k1);
-                e4m3x4_f16x2(b[2 * j + 1], k8, k9);
+          for (int j = 0; j < 2; ++j) {
+            if (Cfg::kElem == 2) {
+              if (Cfg::kHold)
+                pf[kb].mul(acc[(c + j) * Cfg::kHold], b[2 * j], b[2 * j + 1]);
+              else if (kb == 0)
+                pf[kb].template mul<true>(tmp[j], b[2 * j], b[2 * j + 1]);
+              else
+                pf[kb].mul(tmp[j], b[2 * j], b[2 * j + 1]);
+            } else {
+              uint32_t k0, k1, k8, k9;
+              e4m3x4_f16x2(b[2 * j], k0, k1);
+              e4m3x4_f16x2(b[2 * j + 1], k8, k9);
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                  pf[kb].mul(Cfg::kHold ? acc[(c + 2 * j + h) * Cfg::kHold]
-                                        : tmp[(2 * j + h) % CPB],
-                             prmt(k0, k1, h ? 0x7632u : 0x5410u),
-                             prmt(k8, k9, h ? 0x7632u : 0x5410u));
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t b0 = prmt(k0, k1, h ? 0x7632u : 0x5410u);
+                const uint32_t b1 = prmt(k8, k9, h ? 0x7632u : 0x5410u);
+                if (Cfg::kHold)
+                  pf[kb].mul(acc[(c + 2 * j + h) * Cfg::kHold], b0, b1);
+                else if (kb == 0)
+                  pf[kb].template mul<true>(tmp[(2 * j + h) % CPB], b0, b1);
+                else
+                  pf[kb].mul(tmp[(2 * j + h) % CPB], b0, b1);
               }
             }
           }
-          if (!Cfg::kHold) {
+        }
+        if (!Cfg::kHold) {
 #pragma unroll
-            for (int j = 0; j < CPB; ++j) {
-              o[c + j][0] += tmp[j][0] + tmp[j][2];
-              o[c + j][1] += tmp[j][1] + tmp[j][3];
-            }
+          for (int j = 0; j < CPB; ++j) {
+            o[c + j][0] += tmp[j][0] + tmp[j][2];
+            o[c + j][1] += tmp[j][1] + tmp[j][3];
           }
         }
       }
@@ -741,7 +823,12 @@ attention_kernel(const AttArgs A) {
     base = base2;
     P = N;
   }
-  cp_async_wait<0>();
+  // after a timeout copies may still be under way: give them time to land
+  if (*(volatile int*)&sh.dead)
+    for (int i = 0; i < NS; ++i) {
+      mbar_wait(&sh.bars[warp][i], 0);
+      mbar_wait(&sh.bars[warp][i], 1);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -765,10 +852,44 @@ static int attention_workspace(int head_dim, AttArgs* a, void* ws, size_t* bytes
   return MOE_OK;
 }
 
+// The cache as a 3-D tensor for TMA: elements of a row; rows one common unit of
+// the strides apart (a page and a head lead to a row number); tokens of a page.
+static int make_cache_map(CUtensorMap* map, AttArgs& a, void* base, int keys) {
+  const moe_paged_cache& c = a.c;
+  const int eb = cache_elem_bytes(c.dtype);
+  const int64_t row = (int64_t)c.head_dim;
+  int64_t unit = std::gcd(std::gcd(c.page_stride, c.token_stride), c.head_stride);
+  if (unit == 0) unit = row;
+  MOE_REQUIRE(unit >= row, MOE_ERR_UNSUPPORTED,
+              "cache strides (%lld, %lld, %lld) are not multiples of one row of at least head_dim "
+              "elements",
+              (long long)c.page_stride, (long long)c.token_stride, (long long)c.head_stride);
+  const int64_t rows = ((c.pages - 1) * c.page_stride + (c.kv_heads - 1) * c.head_stride) / unit + 1;
+  MOE_REQUIRE(rows <= 0x7fffffff && unit * eb < (1ll << 40) && c.token_stride * eb < (1ll << 40),
+              MOE_ERR_UNSUPPORTED, "cache of %lld rows is too large", (long long)rows);
+  a.page_units = (int)(c.page_stride / unit);
+  a.head_units = (int)(c.head_stride / unit);
+  const int rows_of_box = std::min(keys, c.page_size & -c.page_size);
+  a.box_shift = 31 - __builtin_clz((unsigned)rows_of_box);
+  const cuuint64_t dims[3] = {(cuuint64_t)row, (cuuint64_t)rows, (cuuint64_t)c.page_size};
+  const cuuint64_t strides[2] = {(cuuint64_t)(unit * eb),
+                                 (cuuint64_t)(std::max(c.token_stride, unit) * eb)};
+  const cuuint32_t box[3] = {(cuuint32_t)(kLine / eb), 1, (cuuint32_t)rows_of_box};
+  const cuuint32_t each[3] = {1, 1, 1};
+  EncodeTiledFn fn = encode_fn();
+  MOE_REQUIRE(fn, MOE_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const CUresult r =
+      fn(map, eb == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base,
+         dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  MOE_REQUIRE(r == CUDA_SUCCESS, MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return MOE_OK;
+}
+
 template <int DT, int DP>
-static int launch_attention(const AttArgs& a, int max_len, cudaStream_t s) {
+static int launch_attention(AttArgs& a, int max_len, cudaStream_t s) {
   using Cfg = AttCfg<DT, DP>;
-  static_assert(Cfg::kSlots % 2 == 1 && (Cfg::kSlots + 1) / 2 <= 8 && Cfg::kWarps == 4, "");
+  static_assert(Cfg::kSlots % 2 == 1 && Cfg::kSlots <= 5 && Cfg::kWarps == 4, "");
   static_assert(Cfg::kCtasPerSm <= kAttMaxCtasPerSm, "");
   static std::atomic<uint64_t> ready{0};
   auto kern = attention_kernel<DT, DP>;
@@ -778,6 +899,9 @@ static int launch_attention(const AttArgs& a, int max_len, cudaStream_t s) {
     MOE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
+  CUtensorMap kmap, vmap;
+  MOE_CHECK(make_cache_map(&kmap, a, a.c.k, Cfg::kKeys));
+  MOE_CHECK(make_cache_map(&vmap, a, a.c.v, Cfg::kKeys));
   const int G = a.hq / a.c.kv_heads;
   const int64_t units = (int64_t)a.c.seqs * a.c.kv_heads * ((G + kAttHeads - 1) / kAttHeads);
   const int64_t keys = a.window > 0 ? std::min(a.window, max_len) : max_len;
@@ -791,12 +915,13 @@ static int launch_attention(const AttArgs& a, int max_len, cudaStream_t s) {
   // the weights of a unit's parts fit into the merge rows
   MOE_REQUIRE(kAttHeads * grid * 4 <= Cfg::kMerge, MOE_ERR_UNSUPPORTED, "%d CTAs are too many",
               grid);
-  MOE_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(Cfg::kWarps * 32), Cfg::kSmem, s, a));
+  MOE_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(Cfg::kWarps * 32), Cfg::kSmem, s, kmap, vmap,
+                      a));
   return MOE_OK;
 }
 
 template <int DT>
-static int launch_attention_dt(const AttArgs& a, int max_len, cudaStream_t s) {
+static int launch_attention_dt(AttArgs& a, int max_len, cudaStream_t s) {
   switch (padded_head_dim(a.c.head_dim)) {
     case 64: return launch_attention<DT, 64>(a, max_len, s);
     case 128: return launch_attention<DT, 128>(a, max_len, s);
