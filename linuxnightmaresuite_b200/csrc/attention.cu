@@ -49,6 +49,7 @@ constexpr int kAttHeads = 8;          // query heads of a unit at most
 constexpr int kAttMaxCtasPerSm = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kAttParts = 320;        // CTAs that one unit may be split over
 constexpr float kPScale = 128.f;      // probabilities enter the products times this
 
 struct AttArgs {
@@ -204,8 +205,11 @@ template <int DT, int DP> struct AttCfg {
   static constexpr int kRound = kWarps * kKeys;
   static constexpr int kRing = kWarps * kSlots * kSlot;
   static constexpr int kMergeRow = DP + 8;                  // floats
-  // one row per warp and head; at least the weights of a unit split over 320 CTAs
-  static constexpr int kMerge = kAttHeads * 4 * (kWarps * kMergeRow > 320 ? kWarps * kMergeRow : 320);
+  // one row per warp and head; when a unit's parts are joined first a weight per
+  // part and head, then four floats per thread and head
+  static constexpr int kMerge =
+      4 * kAttHeads * (kWarps * kMergeRow > 4 * 32 * kWarps ? kWarps * kMergeRow : 4 * 32 * kWarps);
+  static_assert(kMerge >= kAttParts * kAttHeads * 4, "weights of the parts");
   static constexpr int kQ = DP / 16 * AFrag<kBf>::kBytes;
   static constexpr int kSmem = kRing + kMerge + kQ;
   static constexpr int kCtasPerSm = kSmem <= 112 * 1024 ? 2 : 1;
@@ -231,9 +235,11 @@ struct AttShared {
   float m[4][kAttHeads], l[4][kAttHeads], qmax[4][kAttHeads], qscale[kAttHeads];
 };
 
-// One CTA's part of a unit: rounds r0 .. r1 of R.
-struct Piece {
-  int ustart, R, r0, r1, head0, nh, head, first, kw, khi, ntile;
+// A cursor over a CTA's pieces: rounds r0 .. r1 of R of unit u of a sequence.
+struct Cursor {
+  int seq, u, head, group;           // unit: key head and group of query heads
+  int at, r0, r1, R;                 // `at`: rounds of this CTA before the piece
+  int len, first, from;              // the sequence's keys first .. len, rounds from `from` on
 };
 
 template <int DT, int DP>
@@ -309,26 +315,41 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   __syncthreads();
   const int seq0 = sh.seq, base0 = (int)(sh.base - start);
 
-  // part of a unit at round `at` of sequence s, whose first round is `base`
-  auto piece_at = [&](int s, int base, int at) {
-    Piece p;
-    int first;
-    const int len = keys_of(s, first);
-    const int from = first / KEYS * KEYS;
-    p.R = max(1, (len - from + RK - 1) / RK);
-    const int u = (at - base) / p.R;
-    p.ustart = base + u * p.R;
-    p.r0 = at - p.ustart;
-    p.r1 = min(p.R, p.r0 + (end - at));
-    const int kvh = u / NHT;
-    p.head0 = kvh * G + (u - kvh * NHT) * kAttHeads;
-    p.nh = min(kAttHeads, kvh * G + G - p.head0);
-    p.first = first;
-    p.kw = from + p.r0 * RK + warp * KEYS;      // tiles of this warp: kw + i * RK ...
-    p.khi = min(len, from + p.r1 * RK);
-    p.ntile = p.khi > p.kw ? (p.khi - p.kw + RK - 1) / RK : 0;
-    p.head = kvh;
-    return p;
+  auto open_seq = [&](Cursor& c) {
+    c.len = keys_of(c.seq, c.first);
+    c.from = c.first / KEYS * KEYS;
+    c.R = max(1, (c.len - c.from + RK - 1) / RK);
+  };
+  auto next_piece = [&](Cursor& c) {             // false: that was the CTA's last
+    c.at += c.r1 - c.r0;
+    if (c.at >= end) return false;
+    if (++c.u == HU) {
+      c.u = c.head = c.group = 0;
+      ++c.seq;
+      open_seq(c);
+    } else if (++c.group == NHT) {
+      c.group = 0;
+      ++c.head;
+    }
+    c.r0 = 0;
+    c.r1 = min(c.R, end - c.at);
+    return true;
+  };
+  Cursor C;                                      // of the arithmetic
+  C.seq = seq0;
+  open_seq(C);
+  C.u = -base0 / C.R;
+  C.head = C.u / NHT;
+  C.group = C.u - C.head * NHT;
+  C.at = 0;
+  C.r0 = -base0 - C.u * C.R;
+  C.r1 = min(C.R, C.r0 + end);
+  // tiles of this warp in a piece: first key, end of the keys, number
+  auto tile0 = [&](const Cursor& c) { return c.from + c.r0 * RK + warp * KEYS; };
+  auto keys_end = [&](const Cursor& c) { return min(c.len, c.from + c.r1 * RK); };
+  auto tiles = [&](const Cursor& c) {
+    const int n = keys_end(c) - tile0(c);
+    return n > 0 ? (n + RK - 1) / RK : 0;
   };
 
   // ---- loads: a cursor of its own that runs ahead of the arithmetic, across
@@ -337,37 +358,33 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   constexpr int BLOCKS = DP * Cfg::kElem < LINE ? 1 : DP * Cfg::kElem / LINE;
   const int box = 1 << A.box_shift, boxes = KEYS >> A.box_shift, ps = A.c.page_size;
   const int step_pages = RK / ps, step_slots = RK - step_pages * ps;   // from tile to tile
-  int lseq = seq0, lbase = base0, lat = 0, li = 0, lslot = 0;
+  Cursor W = C;                                  // of the loads
+  int wtiles = tiles(W), wend = keys_end(W), wkey = tile0(W), li = 0, lslot = 0;
   uint32_t ltile = 0;
-  Piece lp = piece_at(lseq, lbase, lat);
+  bool wmore = true;
   // of this lane's box of tile li: number in the sequence's pages and slot,
   // row of the tensor map
   int pidx = 0, pslot = 0, row = 0, key = 0, page = 0;
   bool in = false;
   auto enter = [&]() {                           // first tile of a piece
     li = 0;
-    key = lp.kw + (lane << A.box_shift);
+    wtiles = tiles(W);
+    wend = keys_end(W);
+    wkey = tile0(W);
+    key = wkey + (lane << A.box_shift);
     pidx = (int)((unsigned)key / (unsigned)ps);
     pslot = key - pidx * ps;
   };
   auto settle = [&]() {                          // to the next piece that has a tile li
-    while (li >= lp.ntile) {
-      lat += lp.r1 - lp.r0;
-      if (lat >= end) {
-        lp.ntile = 0x7fffffff;                   // nothing left
-        break;
-      }
-      if (lat - lbase == lp.R * HU) {
-        lbase = lat;
-        ++lseq;
-      }
-      lp = piece_at(lseq, lbase, lat);
+    while (li >= wtiles) {
+      wmore = next_piece(W);
+      if (!wmore) break;
       enter();
     }
   };
   auto fetch = [&]() {                           // page of this lane's box of tile li
-    in = lat < end && lane < boxes && key < lp.khi && key + box > lp.first;
-    if (in) page = A.c.block_table[(int64_t)lseq * A.c.table_stride + pidx];
+    in = wmore && lane < boxes && key < wend && key + box > W.first;
+    if (in) page = A.c.block_table[(int64_t)W.seq * A.c.table_stride + pidx];
   };
   auto copy = [&](const CUtensorMap* map, int n) {
     uint64_t* bar = &sh.bars[warp][lslot];
@@ -383,18 +400,17 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   };
   uint32_t lok = 0;                              // boxes of the tile that exist
   auto issue_keys = [&]() {
-    if (lat >= end) return;
+    if (!wmore) return;
     if (in && (page < 0 || page >= A.c.pages)) {
       set_status(A.status, MOE_STATUS_BAD_PAGE);
       in = false;
     }
-    row = page * A.page_units + lp.head * A.head_units;
+    row = page * A.page_units + W.head * A.head_units;
     lok = __ballot_sync(0xffffffffu, in);
-    const int k0 = lp.kw + li * RK;
     uint32_t seen = 0xffffffffu;
-    if (__popc(lok) != boxes || k0 < lp.first || k0 + KEYS > lp.khi) {
+    if (__popc(lok) != boxes || wkey < W.first || wkey + KEYS > wend) {
       const int r = lane & (KEYS - 1);
-      seen = __ballot_sync(0xffffffffu, k0 + r >= lp.first && k0 + r < lp.khi &&
+      seen = __ballot_sync(0xffffffffu, wkey + r >= W.first && wkey + r < wend &&
                                             ((lok >> (r >> A.box_shift)) & 1u));
     }
     if (lane == 0) sh.seen[warp][ltile & 7] = seen;
@@ -402,10 +418,11 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     copy(&kmap, __popc(lok));
   };
   auto issue_values = [&]() {
-    if (lat >= end) return;
+    if (!wmore) return;
     copy(&vmap, __popc(lok));
     ++li;
     key += RK;
+    wkey += RK;
     pidx += step_pages;
     pslot += step_slots;
     if (pslot >= ps) {
@@ -449,15 +466,18 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   uint8_t* const qs = smem + Cfg::kRing + Cfg::kMerge;
   float* const mo = reinterpret_cast<float*>(smem + Cfg::kRing);
   float qn[QK][4];
-  auto q_fetch = [&](int s, const Piece& p) {
-    const float* q = A.q + (int64_t)s * A.q_ss + (int64_t)(p.head0 + g) * A.q_hs;
+  auto first_head = [&](const Cursor& c) { return c.head * G + c.group * kAttHeads; };
+  auto heads = [&](const Cursor& c) { return min(kAttHeads, G - c.group * kAttHeads); };
+  auto q_fetch = [&](const Cursor& c) {
+    const float* q = A.q + (int64_t)c.seq * A.q_ss + (int64_t)(first_head(c) + g) * A.q_hs;
+    const int nh = heads(c);
 #pragma unroll
     for (int i = 0; i < QK; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int e = 16 * (warp + i * NW) +
                       (Cfg::kElem == 1 ? 4 * t + j : 2 * t + (j & 1) + 8 * (j >> 1));
-        qn[i][j] = g < p.nh && e < D ? q[e] : 0.f;
+        qn[i][j] = g < nh && e < D ? q[e] : 0.f;
       }
   };
   auto q_max = [&]() {
@@ -474,20 +494,23 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     float mx = sh.qmax[0][g];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mx = fmaxf(mx, sh.qmax[w][g]);
-    const int e = mx > 0.f && mx <= 3.4e38f ? 10 - ilogbf(mx) : 0;
+    // 2^e in two factors, since e may lie outside the exponents of a float
+    const int ex = (int)(__float_as_uint(mx) >> 23);           // 0 .. 255
+    const int e = mx > 0.f && ex < 255 ? 137 - max(ex, 1) : 0;
+    const int e1 = e / 2, e2 = e - e1;
+    const float f1 = __uint_as_float((uint32_t)(127 + e1) << 23);
+    const float f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
     if (warp == 0 && t == 0) sh.qscale[g] = ldexpf(A.scale * A.c.k_scale, -e);
 #pragma unroll
     for (int i = 0; i < QK; ++i) {
       AFrag<BF> f;
-      f.set(ldexpf(qn[i][0], e), ldexpf(qn[i][1], e), ldexpf(qn[i][2], e), ldexpf(qn[i][3], e));
+      f.set(qn[i][0] * f1 * f2, qn[i][1] * f1 * f2, qn[i][2] * f1 * f2, qn[i][3] * f1 * f2);
       f.store(qs + (warp + i * NW) * AFrag<BF>::kBytes, lane);
     }
   };
 
-  int seq = seq0, base = base0, at = 0;
   uint32_t ctile = 0;
-  Piece P = piece_at(seq, base, at);
-  q_fetch(seq, P);
+  q_fetch(C);
   q_max();
   __syncthreads();
   q_split();
@@ -511,18 +534,10 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 
   for (;;) {
     // the piece after this one, and its q
-    const int at2 = at + (P.r1 - P.r0);
-    int seq2 = seq, base2 = base;
-    if (at2 - base == P.R * HU) {
-      base2 = at2;
-      ++seq2;
-    }
-    const bool more = at2 < end;
-    Piece N = P;
-    if (more) {
-      N = piece_at(seq2, base2, at2);
-      q_fetch(seq2, N);
-    }
+    Cursor N = C;
+    const bool more = next_piece(N);
+    if (more) q_fetch(N);
+    const int ntile = tiles(C);
 
     const float qscale = sh.qscale[g];           // score = product * qscale
     const float x2 = qscale * kLog2e;
@@ -555,7 +570,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       }
     };
 
-    for (int i = 0; i < P.ntile; ++i) {
+    for (int i = 0; i < ntile; ++i) {
       const uint32_t ka = wait_slot();
       issue_keys();
       const uint32_t seen = sh.seen[warp][ctile & 7];
@@ -737,10 +752,12 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     }
     if (more) q_max();
     __syncthreads();
-    const bool whole = P.r0 == 0 && P.r1 == P.R;
-    const int my_slot = 2 * blockIdx.x + (P.r0 == 0 ? 1 : 0);
+    const bool whole = C.r0 == 0 && C.r1 == C.R;
+    const int my_slot = 2 * blockIdx.x + (C.r0 == 0 ? 1 : 0);
+    const int nh = heads(C);
+    const int64_t row0 = (int64_t)C.seq * A.hq + first_head(C);
     const float unit = A.c.v_scale / kPScale;
-    for (int h = warp; h < P.nh; h += NW) {
+    for (int h = warp; h < nh; h += NW) {
       float M = sh.m[0][h];
 #pragma unroll
       for (int w = 1; w < NW; ++w) M = fmaxf(M, sh.m[w][h]);
@@ -751,77 +768,106 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         f[w] = ex2(sh.m[w][h] - ms);
         L = fmaf(sh.l[w][h], f[w], L);
       }
-      const int64_t row = (int64_t)seq * A.hq + P.head0 + h;
+      if (whole) {
+        const float norm = L == 0.f ? 0.f : unit / L;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) f[w] *= norm;
+        if (lane == 0 && A.lse) A.lse[row0 + h] = (M + log2f(L)) * kLn2;
+      } else if (lane == 0) {
+        A.part_ml[my_slot * kAttHeads + h] = make_float2(M, L);
+      }
+      float* to = whole ? A.out + (row0 + h) * D : A.part_o + ((int64_t)my_slot * kAttHeads + h) * DP;
       for (int c = lane; c < D; c += 32) {
         float y = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w)
           y = fmaf(mo[(w * kAttHeads + h) * Cfg::kMergeRow + c], f[w], y);
-        if (whole)
-          A.out[row * D + c] = L == 0.f ? 0.f : y * unit / L;
-        else
-          A.part_o[((int64_t)my_slot * kAttHeads + h) * DP + c] = y;
-      }
-      if (lane == 0) {
-        if (!whole)
-          A.part_ml[my_slot * kAttHeads + h] = make_float2(M, L);
-        else if (A.lse)
-          A.lse[row] = (M + log2f(L)) * kLn2;
+        to[c] = y;
       }
     }
     if (more) q_split();
     if (!whole) {
       // ---- the last CTA of a unit to arrive joins the unit's parts, in order
-      const int c0 = (int)((start + P.ustart) / quota);
-      const int n = (int)((start + P.ustart + P.R - 1) / quota) - c0 + 1;
-      __threadfence();
+      const long long ustart = start + C.at - C.r0;
+      const int c0 = (int)(ustart / quota), n = (int)((ustart + C.R - 1) / quota) - c0 + 1;
       __syncthreads();
       if (tid == 0) {
+        __threadfence();
         const int arrived = atomicAdd(A.arrivals + c0, 1);
         sh.last = arrived == n - 1;
         if (sh.last) A.arrivals[c0] = 0;
+        __threadfence();
       }
       __syncthreads();
       if (sh.last) {
-        __threadfence();
-        // weights of the parts, [head][part]; mo is free again
-        for (int h = warp; h < P.nh; h += NW) {
-          const float2* ml = A.part_ml + (int64_t)2 * c0 * kAttHeads + h;
-          float M = -INFINITY;
-          for (int i = lane; i < n; i += 32)
-            M = fmaxf(M, __ldcg(ml + (2 * i + (i == 0)) * kAttHeads).x);
+        // weights of the parts, [part][head]; mo is free again
+        const int64_t slot0 = 2 * (int64_t)c0;   // part i: slot0 + 2 i, part 0: slot0 + 1
+        for (int h = warp; h < nh; h += NW) {
+          float2 v[kAttParts / 32];
+          float M = -INFINITY, L = 0.f;
+#pragma unroll
+          for (int k = 0; k < kAttParts / 32; ++k) {
+            const int i = lane + 32 * k;
+            v[k] = i < n ? __ldcg(A.part_ml + (slot0 + 2 * i + (i == 0)) * kAttHeads + h)
+                         : make_float2(-INFINITY, 0.f);
+          }
+#pragma unroll
+          for (int k = 0; k < kAttParts / 32; ++k) M = fmaxf(M, v[k].x);
 #pragma unroll
           for (int b = 16; b > 0; b >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, b));
           const float ms = M == -INFINITY ? 0.f : M;
-          float L = 0.f;
-          for (int i = lane; i < n; i += 32) {
-            const float2 v = __ldcg(ml + (2 * i + (i == 0)) * kAttHeads);
-            const float f = ex2(v.x - ms);
-            mo[h * n + i] = f;
-            L = fmaf(v.y, f, L);
+#pragma unroll
+          for (int k = 0; k < kAttParts / 32; ++k) {
+            v[k].x = ex2(v[k].x - ms);
+            L = fmaf(v[k].y, v[k].x, L);
           }
 #pragma unroll
           for (int b = 16; b > 0; b >>= 1) L += __shfl_xor_sync(0xffffffffu, L, b);
-          __syncwarp();
-          const int64_t row = (int64_t)seq * A.hq + P.head0 + h;
-          for (int c = lane; c < D; c += 32) {
-            const float* po = A.part_o + ((int64_t)2 * c0 * kAttHeads + h) * DP + c;
-            float y = __ldcg(po + kAttHeads * DP) * mo[h * n];
-#pragma unroll 8
-            for (int i = 1; i < n; ++i)
-              y = fmaf(__ldcg(po + (int64_t)2 * i * kAttHeads * DP), mo[h * n + i], y);
-            A.out[row * D + c] = L == 0.f ? 0.f : y * unit / L;
-          }
-          if (lane == 0 && A.lse) A.lse[row] = (M + log2f(L)) * kLn2;
+          const float norm = L == 0.f ? 0.f : unit / L;
+#pragma unroll
+          for (int k = 0; k < kAttParts / 32; ++k)
+            if (lane + 32 * k < n) mo[(lane + 32 * k) * kAttHeads + h] = v[k].x * norm;
+          if (lane == 0 && A.lse) A.lse[row0 + h] = (M + log2f(L)) * kLn2;
+        }
+        __syncthreads();
+        // thread: four columns of every PL-th part, all heads
+        constexpr int CT = DP / 4, PL = NT / CT;
+        const int col = tid % CT, pl = tid / CT;
+        float4 y[kAttHeads];
+#pragma unroll
+        for (int h = 0; h < kAttHeads; ++h) y[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (int i = pl; i < n; i += PL) {
+          const float4* po = reinterpret_cast<const float4*>(
+              A.part_o + (slot0 + 2 * i + (i == 0)) * kAttHeads * DP) + col;
+#pragma unroll
+          for (int h = 0; h < kAttHeads; ++h)
+            if (h < nh) {
+              const float4 v = __ldcg(po + h * CT);
+              const float w = mo[i * kAttHeads + h];
+              y[h].x = fmaf(v.x, w, y[h].x);
+              y[h].y = fmaf(v.y, w, y[h].y);
+              y[h].z = fmaf(v.z, w, y[h].z);
+              y[h].w = fmaf(v.w, w, y[h].w);
+            }
+        }
+        __syncthreads();                         // the weights are done with
+#pragma unroll
+        for (int h = 0; h < kAttHeads; ++h)
+          if (h < nh) reinterpret_cast<float4*>(mo)[(pl * kAttHeads + h) * CT + col] = y[h];
+        __syncthreads();
+        for (int e = tid; e < nh * DP; e += NT) {
+          const int h = e / DP, c = e % DP;
+          float v = mo[h * DP + c];
+#pragma unroll
+          for (int k = 1; k < PL; ++k) v += mo[(k * kAttHeads + h) * DP + c];
+          if (c < D) A.out[(row0 + h) * D + c] = v;
         }
       }
     }
     if (!more) break;
     __syncthreads();                             // q of the next piece; mo and sh are free
-    at = at2;
-    seq = seq2;
-    base = base2;
-    P = N;
+    C = N;
   }
   // after a timeout copies may still be under way: give them time to land
   if (*(volatile int*)&sh.dead)
@@ -912,9 +958,7 @@ static int launch_attention(AttArgs& a, int max_len, cudaStream_t s) {
   MOE_REQUIRE(units / a.c.seqs * most < (1ll << 30) && units * most / grid < (1ll << 30),
               MOE_ERR_UNSUPPORTED, "%d sequences of up to %d pages are too many", a.c.seqs,
               a.c.table_width);
-  // the weights of a unit's parts fit into the merge rows
-  MOE_REQUIRE(kAttHeads * grid * 4 <= Cfg::kMerge, MOE_ERR_UNSUPPORTED, "%d CTAs are too many",
-              grid);
+  MOE_REQUIRE(grid <= kAttParts, MOE_ERR_UNSUPPORTED, "%d CTAs are too many", grid);
   MOE_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(Cfg::kWarps * 32), Cfg::kSmem, s, kmap, vmap,
                       a));
   return MOE_OK;
