@@ -1,10 +1,31 @@
 // y = W x (+ residual) for a few rows, W in packed Q4_0 / Q8_0 tiles.
 //
-// First form: one warp per (row of W, row of x), decoding its weights from the
-// packed tiles.
-#include "moe_common.cuh"
+// Each weight is read once for up to 16 rows, so the bound is memory up to
+// about 8 rows, and mma.sync issue beyond.  As in the experts' gate/up kernel
+// the quants themselves are the (exact, subnormal fp16) A operand, x enters as
+// fp16 hi + lo columns (4 rows fill the 8 columns of an MMA), and every
+// 32-weight block has an accumulator of its own that is scaled in f32.
+//
+// One CTA of 16 warps per SM stays resident.  It turns its columns of x into
+// fragments in shared memory once, while the first weights are under way, and
+// then its warps stream W: a warp owns pairs of 16-row strips (two strips share
+// each fragment read) and 1 / ks of their columns, through a ring of bulk
+// copies.  Where x is too wide for one SM's shared memory (or W has few rows) a
+// cluster of cs CTAs splits the columns, so that each converts only its part of
+// x; their sums meet in distributed shared memory.  The split (cs, ks) is the
+// one with the least estimated time; sums are in a fixed order.
+#include <algorithm>
+#include <atomic>
+
+#include "packed_tiles.cuh"
 
 namespace moe {
+
+constexpr int kLinWarps = 16;
+constexpr int kLinU = 2;               // tiles of each strip per ring stage
+constexpr int kLinMaxStages = 4;
+constexpr int kLinHead = 2048;         // barriers, row maxima and scales
+constexpr int kLinSmem = 226 * 1024;
 
 struct LinArgs {
   const uint8_t* w;
@@ -12,36 +33,435 @@ struct LinArgs {
   float* y;
   int64_t xs, rs, ys;
   int rows, cols, T;
+  int kt;                              // tiles of a strip
+  int pairs;                           // pairs of strips
+  int cs, ks, nst, rounds, vec;
 };
 
-template <int QT>
-__global__ void __launch_bounds__(256) linear_kernel(const LinArgs A) {
+__device__ __forceinline__ float pow2f(int e) {   // -126 <= e <= 127
+  return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// x columns [64 t0, 64 t1) of n rows -> fragment records; returns the rows'
+// exponents in `ex` (a row times 2^ex has its largest |x| in [2^14, 2^15)).
+template <int QT, int G>
+__device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, int* ex,
+                                                uint32_t* smax, int row0, int n, int t0, int t1) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = lane & 3;
+  const int nb = 2 * (t1 - t0), real = min(nb, A.cols / 32 - 2 * t0);   // blocks, with columns
+  const int P = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : n <= 8 ? 8 : 16;
+  const int wpr = kLinWarps / P, row = warp / wpr, part = warp % wpr;   // warps of a row
+  const bool on = row < n;
+  const float* x = A.x + (int64_t)(row0 + (on ? row : 0)) * A.xs + (int64_t)t0 * 64;
+  auto values = [&](int b, float (&v)[8]) {
+    const int c0 = 32 * b + (QT == MOE_Q4_0 ? 4 * t : 8 * t), c1 = c0 + (QT == MOE_Q4_0 ? 16 : 4);
+    if (A.vec) {
+      const float4 a = *reinterpret_cast<const float4*>(x + c0);
+      const float4 c = *reinterpret_cast<const float4*>(x + c1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = c.x; v[5] = c.y; v[6] = c.z; v[7] = c.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = x[c0 + i];
+        v[4 + i] = x[c1 + i];
+      }
+    }
+  };
+  uint32_t mx = 0;
+  if (on)
+#pragma unroll 4
+    for (int b = part * 8 + (lane >> 2); b < real; b += wpr * 8) {
+      float v[8];
+      values(b, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(fabsf(v[i])));
+    }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  if (lane == 0) smax[warp] = mx;
+  if (tid < 4 * G) ex[tid] = 0;
+  __syncthreads();
+  mx = 0;
+  for (int i = 0; i < wpr; ++i) mx = max(mx, smax[row * wpr + i]);
+  const int eb = (int)(mx >> 23);                // biased exponent; 255: Inf or NaN
+  const int e = mx == 0 || eb == 255 ? 0 : 141 - max(eb, 1);
+  const float f1 = pow2f(e / 2), f2 = pow2f(e - e / 2);
+  if (part == 0 && lane == 0 && row < 4 * G) ex[row] = e;
+  const int cg = row >> 2, w = row & 3;
+  if (row < 4 * G)
+    for (int b = part * 8 + (lane >> 2); b < (nb + 7) / 8 * 8; b += wpr * 8) {
+      uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+      float sh = 0.f, sl = 0.f;
+      if (on && b < real) {
+        float v[8];
+        values(b, v);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          // register slots i, i + 1 hold elements 0, 2 | 1, 3 of each four (Q4_0)
+          const int p = QT == MOE_Q4_0 ? (i & 4) + ((i & 2) ? 1 : 0) : i;
+          const int q = QT == MOE_Q4_0 ? p + 2 : i + 1;
+          // high nibbles stay 16 times too large; their x is stored / 16
+          const float div = QT == MOE_Q4_0 && i >= 4 ? 0.0625f : 1.f;
+          const float mul = QT == MOE_Q4_0 && i >= 4 ? 16.f : 1.f;
+          const float a = v[p] * f1 * f2 * div, c = v[q] * f1 * f2 * div;
+          const __half2 h = __floats2half2_rn(a, c);
+          const float ha = __low2float(h), hc = __high2float(h);
+          const __half2 l = __floats2half2_rn(a - ha, c - hc);
+          sh += mul * (ha + hc);
+          sl += mul * (__low2float(l) + __high2float(l));
+          hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+          lo[i / 2] = *reinterpret_cast<const uint32_t*>(&l);
+        }
+      }
+      sh += __shfl_xor_sync(0xffffffffu, sh, 1);
+      sl += __shfl_xor_sync(0xffffffffu, sl, 1);
+      sh += __shfl_xor_sync(0xffffffffu, sh, 2);
+      sl += __shfl_xor_sync(0xffffffffu, sl, 2);
+      if (b < nb) {
+        uint8_t* r = rec + (size_t)(cg * nb + b) * kXRec;
+        *reinterpret_cast<uint4*>(r + w * 64 + t * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(r + 256 + w * 64 + t * 16) =
+            make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (t == 0) {
+          const float k = -quant_offset<QT>() / kSubUnit;
+          float* cor = reinterpret_cast<float*>(r + 512);
+          cor[4 * (w >> 1) + (w & 1)] = cor[4 * (w >> 1) + (w & 1) + 2] = k * sh;
+          cor[4 * (2 + (w >> 1)) + (w & 1)] = cor[4 * (2 + (w >> 1)) + (w & 1) + 2] = k * sl;
+        }
+      }
+    }
+  // rows of the column groups that no warp has
+  for (int i = tid; i < (4 * G - P) * nb; i += kLinWarps * 32) {
+    const int r = P + i / nb, b = i % nb, z = r & 3;
+    uint8_t* p = rec + (size_t)((r >> 2) * nb + b) * kXRec;
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<uint4*>(p + (q >> 2) * 256 + z * 64 + (q & 3) * 16) = make_uint4(0, 0, 0, 0);
+    float* cor = reinterpret_cast<float*>(p + 512);
+    cor[4 * (z >> 1) + (z & 1)] = cor[4 * (z >> 1) + (z & 1) + 2] = 0.f;
+    cor[4 * (2 + (z >> 1)) + (z & 1)] = cor[4 * (2 + (z >> 1)) + (z & 1) + 2] = 0.f;
+  }
+}
+
+template <int QT, int G>
+__global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs A) {
   using Tr = QTraits<QT>;
-  constexpr int SL = Tr::kLaneBytes / 4;
+  constexpr int U = kLinU, TB = Tr::kTileBytes, STAGE = 2 * U * TB;
+  constexpr int NRED = 2 * G * 4 * 16;           // floats of a pair: 32 rows x 4 G tokens
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint64_t* const bars_all = reinterpret_cast<uint64_t*>(smem);
+  uint32_t* const smax = reinterpret_cast<uint32_t*>(smem + 1024);
+  int* const ex = reinterpret_cast<int*>(smem + 1024 + 64);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int rank = blockIdx.x % A.cs, cluster = blockIdx.x / A.cs, nclusters = gridDim.x / A.cs;
+  const int groups = kLinWarps / A.ks, group = warp / A.ks, kq = warp % A.ks;
+  const int row0 = blockIdx.y * 4 * G, n = min(4 * G, A.T - row0);
+  // columns: this CTA's tiles, this warp's
+  const int tps = (A.kt + A.cs - 1) / A.cs, t0 = min(A.kt, rank * tps), t1 = min(A.kt, t0 + tps);
+  const int wps = (t1 - t0 + A.ks - 1) / A.ks;
+  const int wt0 = min(t1, t0 + kq * wps), wt1 = min(t1, wt0 + wps), nt = wt1 - wt0;
+  const int nb = 2 * (t1 - t0);
+  uint8_t* const rec = smem + kLinHead;
+  float* const red = reinterpret_cast<float*>(rec + (size_t)G * 2 * tps * kXRec);
+  float* const part = red + (A.ks > 1 ? kLinWarps * NRED : 0);
+  uint8_t* const ring =
+      reinterpret_cast<uint8_t*>(part + (A.cs > 1 ? 2 * groups * NRED : 0)) + warp * A.nst * STAGE;
+  uint64_t* const bars = bars_all + warp * kLinMaxStages;
+
+  if (lane < A.nst) {
+    mbar_init(&bars[lane], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
   pdl_trigger();
   pdl_wait();
-  const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (unit >= (int64_t)A.rows * A.T) return;
-  const int row = (int)(unit % A.rows), t = (int)(unit / A.rows);
-  const int kt = (A.cols + 63) / 64, g = row & 7, half = (row >> 3) & 1;
-  float acc = 0.f;
-  for (int b = 0; b < A.cols / 32; ++b) {
-    const uint8_t* tile = A.w + ((int64_t)(row >> 4) * kt + (b >> 1)) * Tr::kTileBytes;
-    const int sub = half * 2 + (b & 1);
-    const float d =
-        __half2float(*reinterpret_cast<const __half*>(tile + Tr::kTileQuant + 8 * g + 2 * sub));
-    const int i = QT == MOE_Q4_0 ? lane & 15 : lane;
-    const uint8_t byte = tile[(4 * g + i / SL) * Tr::kLaneBytes + sub * SL + i % SL];
-    const int v = QT == MOE_Q4_0 ? (lane < 16 ? byte & 15 : byte >> 4) - 8 : (int)(int8_t)byte;
-    acc = fmaf(d * (float)v, A.x[t * A.xs + 32 * b + lane], acc);
+
+  // ---- weights: stage q of this warp is tiles [wt0 + j U, ..) of pair `p`
+  const int nsr = (nt + U - 1) / U;              // stages of a pair
+  const int p0 = cluster * groups + group, pstep = nclusters * groups;
+  const int mine = p0 < A.pairs ? (A.pairs - p0 + pstep - 1) / pstep : 0;
+  const int total = mine * nsr;
+  const uint64_t pol = evict_first_policy();
+  const int strips = (A.rows + 15) / 16;
+  int ip = p0, ij = 0, islot = 0, issued = 0;
+  auto issue = [&]() {                           // lane 0
+    const uint32_t bytes = (uint32_t)(min(U, nt - ij * U) * TB);
+    const uint8_t* src = A.w + ((int64_t)2 * ip * A.kt + wt0 + ij * U) * TB;
+    const bool two = 2 * ip + 1 < strips;
+    uint8_t* dst = ring + islot * STAGE;
+    mbar_expect_tx(&bars[islot], two ? 2 * bytes : bytes);
+    bulk_g2s(dst, src, bytes, &bars[islot], pol);
+    if (two) bulk_g2s(dst + U * TB, src + (int64_t)A.kt * TB, bytes, &bars[islot], pol);
+  };
+  auto step = [&]() {
+    ++issued;
+    islot = islot + 1 == A.nst ? 0 : islot + 1;
+    if (++ij == nsr) {
+      ij = 0;
+      ip += pstep;
+    }
+  };
+  for (int q = 0; q < A.nst && q < total; ++q) {
+    if (lane == 0) issue();
+    step();
   }
+  build_fragments<QT, G>(A, rec, ex, smax, row0, n, t0, t1);
+  __syncthreads();
+
+  // ---- stream
+  bool ok = true;
+  int slot = 0;
+  uint32_t phase = 0;
+  const uint8_t* const xl = rec + lane * 16 + (size_t)2 * (wt0 - t0) * kXRec;
+  const uint8_t* const cl = rec + 512 + t * 16 + (size_t)2 * (wt0 - t0) * kXRec;
+  const int cstride = nb * kXRec;
+  for (int r = 0; r < A.rounds; ++r) {
+    const int p = p0 + r * pstep;
+    float2 acc[2][G][2];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  if (lane == 0) {
-    if (A.residual) acc += A.residual[t * A.rs + row];
-    A.y[t * A.ys + row] = acc;
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int cg = 0; cg < G; ++cg) acc[s][cg][0] = acc[s][cg][1] = make_float2(0.f, 0.f);
+    if (p < A.pairs) {
+      for (int j = 0; j < nsr; ++j) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bars[slot], phase));
+        const uint8_t* st = ring + slot * STAGE + 0;
+        TileRegs<QT> w[2][U];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int u = 0; u < U; ++u) lds_tile<QT>(w[s][u], st + (s * U + u) * TB, lane);
+        __syncwarp();
+        if (ok && issued < total) {
+          if (lane == 0) {
+            fence_proxy_async_smem();
+            issue();
+          }
+          step();
+        }
+        if (++slot == A.nst) {
+          slot = 0;
+          phase ^= 1u;
+        }
+        const int off = 2 * j * U * kXRec;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (j * U + u < nt) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              uint32_t a0[2][4], a1[2][4];
+              float2 d0[2], d8[2];
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+                tile_afrags<QT, true>(w[s][u], b, a0[s], a1[s], d0[s], d8[s]);
+#pragma unroll
+              for (int cg = 0; cg < G; ++cg) {
+                const int o = off + (2 * u + b) * kXRec + cg * cstride;
+                const uint4 xf = *reinterpret_cast<const uint4*>(xl + o);
+                const float4 c0 = *reinterpret_cast<const float4*>(cl + o);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+                  block_mma(acc[s][cg], a0[s], a1[s], xf, c0, d0[s], d8[s]);
+              }
+            }
+          }
+        }
+      }
+    }
+    // hi + lo: columns 2t, 2t + 1 and those 4 further on; lanes t < 2 keep
+    // rows g, g + 8 of tokens 4 cg + 2t, + 1
+    float v[2][G][4];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int cg = 0; cg < G; ++cg)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a = (i & 1) ? acc[s][cg][i >> 1].y : acc[s][cg][i >> 1].x;
+          v[s][cg][i] = ok ? a + __shfl_xor_sync(0xffffffffu, a, 2)
+                           : __uint_as_float(0x7fffffffu);   // a wait ran out: NaN
+        }
+    const int at = g * 2 + t;                    // lanes t < 2: 16 places
+    if (A.ks > 1) {
+      // the column parts of a pair meet in the group's first warp
+      if (r > 0) asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * A.ks) : "memory");
+      if (kq > 0 && t < 2)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int cg = 0; cg < G; ++cg)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              red[warp * NRED + ((s * G + cg) * 4 + i) * 16 + at] = v[s][cg][i];
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * A.ks) : "memory");
+      if (kq == 0 && t < 2)
+        for (int k = 1; k < A.ks; ++k)
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int cg = 0; cg < G; ++cg)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                v[s][cg][i] += red[(warp + k) * NRED + ((s * G + cg) * 4 + i) * 16 + at];
+    }
+    const bool lead = kq == 0 && t < 2 && p < A.pairs;
+    if (lead) {
+#pragma unroll
+      for (int cg = 0; cg < G; ++cg)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = ex[4 * cg + 2 * t + (i & 1)];
+          const float f1 = pow2f(-(e / 2)), f2 = pow2f(-(e - e / 2));
+#pragma unroll
+          for (int s = 0; s < 2; ++s) v[s][cg][i] = v[s][cg][i] * kSubUnit * f1 * f2;
+        }
+    }
+    bool write = lead;
+    if (A.cs > 1) {
+      // the CTAs' parts: CTA group % cs adds up the pair of group `group`
+      float* mine_p = part + ((r & 1) * groups + group) * NRED;
+      if (kq == 0 && t < 2)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int cg = 0; cg < G; ++cg)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine_p[((s * G + cg) * 4 + i) * 16 + at] = v[s][cg][i];
+      cluster_sync();
+      write = lead && group % A.cs == rank;
+      if (write) {
+        const uint32_t a = smem_u32(mine_p);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int cg = 0; cg < G; ++cg)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float y = 0.f;
+              for (int c = 0; c < A.cs; ++c)
+                y += ld_cluster(a + (((s * G + cg) * 4 + i) * 16 + at) * 4, c);
+              v[s][cg][i] = y;
+            }
+      }
+    }
+    if (write) {
+#pragma unroll
+      for (int cg = 0; cg < G; ++cg)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = 4 * cg + 2 * t + (i & 1);
+          if (tok < n)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const int row = 32 * p + 16 * s + g + 8 * (i >> 1);
+              if (row < A.rows) {
+                float y = v[s][cg][i];
+                if (A.residual) y += A.residual[(int64_t)(row0 + tok) * A.rs + row];
+                A.y[(int64_t)(row0 + tok) * A.ys + row] = y;
+              }
+            }
+        }
+    }
   }
+  // after a timeout the copies already issued are still waited for (bounded)
+  if (!ok)
+    for (int i = 0; i < A.nst; ++i) {
+      mbar_wait(&bars[i], 0);
+      mbar_wait(&bars[i], 1);
+    }
+  if (A.cs > 1) cluster_sync();                  // nobody reads this CTA's parts any more
+}
+
+// Shared memory of a split; nst ring stages take what is left.
+template <int QT, int G>
+static size_t linear_smem(int kt, int cs, int ks, int nst) {
+  const size_t nred = (size_t)2 * G * 4 * 16 * 4;
+  const int tps = (kt + cs - 1) / cs;
+  return kLinHead + (size_t)G * 2 * tps * kXRec + (ks > 1 ? kLinWarps * nred : 0) +
+         (cs > 1 ? 2 * (kLinWarps / ks) * nred : 0) +
+         (size_t)kLinWarps * nst * 2 * kLinU * QTraits<QT>::kTileBytes;
+}
+
+template <int QT, int G>
+static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
+  // Estimated time of a split, in the time all warps of an SM take for one tile
+  // pair each (about 800 cycles of HBM): rounds x (tiles of a warp, and the
+  // meetings of warps, 3, and of a cluster, 8), and the fragments, 4 G rows of
+  // the CTA's columns (28 cycles per group and tile).
+  const int sms = sm_count();
+  double best = 0;
+  a.cs = 0;
+  for (int cs = 1; cs <= 8; cs *= 2)
+    for (int ks = 1; ks <= kLinWarps; ks *= 2) {
+      if (linear_smem<QT, G>(a.kt, cs, ks, 2) > kLinSmem) continue;
+      const int tps = (a.kt + cs - 1) / cs, wt = (tps + ks - 1) / ks;
+      const int slots = sms / cs * (kLinWarps / ks);
+      const int rounds = (a.pairs + slots - 1) / slots;
+      const double t = rounds * (wt * (1 + 0.25 * (G - 1)) + (ks > 1 ? 3 : 0) + (cs > 1 ? 8 : 0)) +
+                       0.035 * G * tps;
+      if (a.cs == 0 || t < best) {
+        best = t;
+        a.cs = cs;
+        a.ks = ks;
+      }
+    }
+  fits = a.cs > 0;
+  if (!fits) return MOE_OK;
+  a.nst = 2;
+  while (a.nst < kLinMaxStages && linear_smem<QT, G>(a.kt, a.cs, a.ks, a.nst + 1) <= kLinSmem)
+    ++a.nst;
+  const int per = kLinWarps / a.ks;                  // pairs of a cluster's round
+  const int clusters = std::min(sms / a.cs, (a.pairs + per - 1) / per);
+  a.rounds = (a.pairs + clusters * per - 1) / (clusters * per);
+  const size_t smem = linear_smem<QT, G>(a.kt, a.cs, a.ks, a.nst);
+  auto kern = linear_kernel<QT, G>;
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  MOE_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !((ready.load() >> dev) & 1)) {
+    MOE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem));
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(clusters * a.cs), (unsigned)((a.T + 4 * G - 1) / (4 * G)));
+  cfg.blockDim = dim3(kLinWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)a.cs;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.cs > 1 ? 2 : 1;
+  MOE_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+  return MOE_OK;
+}
+
+// Column groups of 4 rows: as many as T needs, fewer where x is so wide that
+// more do not fit.
+template <int QT>
+static int launch_linear_qt(LinArgs& a, cudaStream_t s) {
+  bool fits = false;
+  if (a.T > 8) MOE_CHECK((launch_linear<QT, 4>(a, s, fits)));
+  if (!fits && a.T > 4) MOE_CHECK((launch_linear<QT, 2>(a, s, fits)));
+  if (!fits) MOE_CHECK((launch_linear<QT, 1>(a, s, fits)));
+  MOE_REQUIRE(fits, MOE_ERR_UNSUPPORTED, "cols %d: rows of x this wide do not fit", a.cols);
+  return MOE_OK;
 }
 
 }  // namespace moe
@@ -52,16 +472,30 @@ extern "C" int moe_linear(const uint8_t* w, int qtype, int rows, int cols, const
   MOE_REQUIRE(moe::qtype_ok(qtype), MOE_ERR_UNSUPPORTED, "quant type %d not supported", qtype);
   MOE_REQUIRE(rows > 0 && cols > 0 && T >= 0, MOE_ERR_INVALID, "bad shape");
   MOE_REQUIRE(cols % 32 == 0, MOE_ERR_UNSUPPORTED, "cols %d is not a multiple of 32", cols);
+  MOE_REQUIRE(rows <= 0x7ffffff0 - 32, MOE_ERR_UNSUPPORTED, "%d rows are too many", rows);
   if (T == 0) return MOE_OK;
   MOE_REQUIRE(w && x && y, MOE_ERR_INVALID, "null pointer");
   MOE_REQUIRE((uintptr_t)w % 16 == 0, MOE_ERR_INVALID, "w must be 16-byte aligned");
-  moe::LinArgs a = {w, x, residual, y, x_stride, residual_stride, y_stride, rows, cols, T};
+  MOE_REQUIRE(T <= 65535 * 4, MOE_ERR_UNSUPPORTED, "%d rows of x are too many", T);
+  moe::LinArgs a = {};
+  a.w = w;
+  a.x = x;
+  a.residual = residual;
+  a.y = y;
+  a.xs = x_stride;
+  a.rs = residual_stride;
+  a.ys = y_stride;
+  a.rows = rows;
+  a.cols = cols;
+  a.T = T;
+  a.kt = (cols + 63) / 64;
+  a.pairs = ((rows + 15) / 16 + 1) / 2;
+  a.vec = (uintptr_t)x % 16 == 0 && (T == 1 || x_stride % 4 == 0);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int64_t units = (int64_t)rows * T;
   {
     ::moe::ProfScope _prof(MOE_K_LINEAR, s);
-    auto kern = qtype == MOE_Q4_0 ? moe::linear_kernel<MOE_Q4_0> : moe::linear_kernel<MOE_Q8_0>;
-    MOE_CUDA(moe::launch_pdl(kern, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, s, a));
+    MOE_CHECK(qtype == MOE_Q4_0 ? moe::launch_linear_qt<MOE_Q4_0>(a, s)
+                                : moe::launch_linear_qt<MOE_Q8_0>(a, s));
   }
   return moe::check_launch("linear");
 }
