@@ -227,6 +227,14 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
   const uint8_t* const xl = rec + lane * 16 + (size_t)2 * (wt0 - t0) * kXRec;
   const uint8_t* const cl = rec + 512 + t * 16 + (size_t)2 * (wt0 - t0) * kXRec;
   const int cstride = nb * kXRec;
+  // place `at` = 2 g + t of strip s, column group cg, value i of an MMA result
+  auto put = [&](int p, int s, int cg, int i, int at, float y) {
+    const int tok = 4 * cg + 2 * (at & 1) + (i & 1), row = 32 * p + 16 * s + (at >> 1) + 8 * (i >> 1);
+    if (tok < n && row < A.rows) {
+      if (A.residual) y += A.residual[(int64_t)(row0 + tok) * A.rs + row];
+      A.y[(int64_t)(row0 + tok) * A.ys + row] = y;
+    }
+  };
   for (int r = 0; r < A.rounds; ++r) {
     const int p = p0 + r * pstep;
     float2 acc[2][G][2];
@@ -328,51 +336,39 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
           for (int s = 0; s < 2; ++s) v[s][cg][i] = v[s][cg][i] * kSubUnit * f1 * f2;
         }
     }
-    bool write = lead;
-    if (A.cs > 1) {
-      // the CTAs' parts: CTA group % cs adds up the pair of group `group`
-      float* mine_p = part + ((r & 1) * groups + group) * NRED;
+    if (A.cs == 1) {
+      if (lead) {
+#pragma unroll
+        for (int cg = 0; cg < G; ++cg)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+              put(p, s, cg, i, at, v[s][cg][i]);
+      }
+    } else {
+      // the CTAs' parts: every thread of the cluster adds up its places
+      float* mine_p = part + (size_t)(r & 1) * groups * NRED;
       if (kq == 0 && t < 2)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
           for (int cg = 0; cg < G; ++cg)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mine_p[((s * G + cg) * 4 + i) * 16 + at] = v[s][cg][i];
+            for (int i = 0; i < 4; ++i)
+              mine_p[group * NRED + ((s * G + cg) * 4 + i) * 16 + at] = v[s][cg][i];
       cluster_sync();
-      write = lead && group % A.cs == rank;
-      if (write) {
-        const uint32_t a = smem_u32(mine_p);
+      for (int e = rank * kLinWarps * 32 + tid; e < groups * NRED; e += A.cs * kLinWarps * 32) {
+        const int pe = cluster * groups + e / NRED + r * pstep, k = e % NRED / 16;
+        const uint32_t a = smem_u32(mine_p + e);
+        float f[8];
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int c = 0; c < 8; ++c) f[c] = c < A.cs ? ld_cluster(a, c) : 0.f;
+        float y = f[0];
 #pragma unroll
-          for (int cg = 0; cg < G; ++cg)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float y = 0.f;
-              for (int c = 0; c < A.cs; ++c)
-                y += ld_cluster(a + (((s * G + cg) * 4 + i) * 16 + at) * 4, c);
-              v[s][cg][i] = y;
-            }
+        for (int c = 1; c < 8; ++c) y += f[c];
+        if (pe < A.pairs) put(pe, k / (4 * G), k / 4 % G, k % 4, e % 16, y);
       }
-    }
-    if (write) {
-#pragma unroll
-      for (int cg = 0; cg < G; ++cg)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tok = 4 * cg + 2 * t + (i & 1);
-          if (tok < n)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              const int row = 32 * p + 16 * s + g + 8 * (i >> 1);
-              if (row < A.rows) {
-                float y = v[s][cg][i];
-                if (A.residual) y += A.residual[(int64_t)(row0 + tok) * A.rs + row];
-                A.y[(int64_t)(row0 + tok) * A.ys + row] = y;
-              }
-            }
-        }
     }
   }
   // after a timeout the copies already issued are still waited for (bounded)
