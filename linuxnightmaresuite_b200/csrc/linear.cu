@@ -35,7 +35,7 @@ struct LinArgs {
   int rows, cols, T;
   int kt;                              // tiles of a strip
   int pairs;                           // pairs of strips
-  int cs, ks, nst, rounds, vec;
+  int cs, ks, tps, nst, rounds, vec;   // tps: tiles of a CTA's columns
 };
 
 __device__ __forceinline__ float pow2f(int e) {   // -126 <= e <= 127
@@ -54,11 +54,27 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
   return v;
 }
 
-// x columns [64 t0, 64 t1) of n rows -> fragment records; returns the rows'
-// exponents in `ex` (a row times 2^ex has its largest |x| in [2^14, 2^15)).
-template <int QT, int G>
-__device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, int* ex,
-                                                uint32_t* smax, int row0, int n, int t0, int t1) {
+// The eight columns of an MMA are four pairs (hi part, lo part).  With 3 rows of
+// x or more a pair is a row, and G column groups hold up to 4 G rows.  With one
+// or two rows the pairs are NBG = 4 or 2 consecutive 32-weight blocks of a row
+// (the fragment of a block is zero in the other blocks' columns): one
+// accumulator then serves NBG blocks, and a lane scales its own block only.
+template <int NBG, int G> struct LinCfg {
+  static constexpr int kTok = 4 / NBG;           // rows of a column group
+  static constexpr int kRows = kTok * G;         // rows of a pass
+  static constexpr int kRed = 2 * G * 2 * 32;    // floats of a pair of strips
+  // fragments of a tile's two blocks, and their offset corrections (hi, lo)
+  static constexpr int kTileBytes = G * (2 * 512 + (NBG == 4 ? 1 : NBG == 2 ? 1 : 2) * 32);
+};
+
+// x columns [64 t0, 64 t1) of n rows -> fragments `rec` ([block][column group] of
+// 512 bytes) and corrections `cor` ([blocks / NBG][column group][pair]); a row
+// times 2^ex has its largest |x| in [2^14, 2^15).
+template <int QT, int NBG, int G>
+__device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, float2* cor,
+                                                int rec_blocks, int* ex, uint32_t* smax, int row0,
+                                                int n, int t0, int t1) {
+  constexpr int TOK = LinCfg<NBG, G>::kTok, ROWS = LinCfg<NBG, G>::kRows;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = lane & 3;
   const int nb = 2 * (t1 - t0), real = min(nb, A.cols / 32 - 2 * t0);   // blocks, with columns
   const int P = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : n <= 8 ? 8 : 16;
@@ -91,75 +107,66 @@ __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, 
     }
   mx = __reduce_max_sync(0xffffffffu, mx);
   if (lane == 0) smax[warp] = mx;
-  if (tid < 4 * G) ex[tid] = 0;
+  if (tid < ROWS) ex[tid] = 0;
+  for (int i = tid; i < G * rec_blocks * 32; i += kLinWarps * 32)
+    reinterpret_cast<uint4*>(rec)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = tid; i < G * (rec_blocks / NBG) * 4; i += kLinWarps * 32)
+    cor[i] = make_float2(0.f, 0.f);
   __syncthreads();
+  if (!on) return;
   mx = 0;
   for (int i = 0; i < wpr; ++i) mx = max(mx, smax[row * wpr + i]);
   const int eb = (int)(mx >> 23);                // biased exponent; 255: Inf or NaN
   const int e = mx == 0 || eb == 255 ? 0 : 141 - max(eb, 1);
   const float f1 = pow2f(e / 2), f2 = pow2f(e - e / 2);
-  if (part == 0 && lane == 0 && row < 4 * G) ex[row] = e;
-  const int cg = row >> 2, w = row & 3;
-  if (row < 4 * G)
-    for (int b = part * 8 + (lane >> 2); b < (nb + 7) / 8 * 8; b += wpr * 8) {
-      uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-      float sh = 0.f, sl = 0.f;
-      if (on && b < real) {
-        float v[8];
-        values(b, v);
+  if (part == 0 && lane == 0) ex[row] = e;
+  const int cg = row / TOK;
+  for (int b = part * 8 + (lane >> 2); b < (real + 7) / 8 * 8; b += wpr * 8) {
+    uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+    float sh = 0.f, sl = 0.f;
+    if (b < real) {
+      float v[8];
+      values(b, v);
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          // register slots i, i + 1 hold elements 0, 2 | 1, 3 of each four (Q4_0)
-          const int p = QT == MOE_Q4_0 ? (i & 4) + ((i & 2) ? 1 : 0) : i;
-          const int q = QT == MOE_Q4_0 ? p + 2 : i + 1;
-          // high nibbles stay 16 times too large; their x is stored / 16
-          const float div = QT == MOE_Q4_0 && i >= 4 ? 0.0625f : 1.f;
-          const float mul = QT == MOE_Q4_0 && i >= 4 ? 16.f : 1.f;
-          const float a = v[p] * f1 * f2 * div, c = v[q] * f1 * f2 * div;
-          const __half2 h = __floats2half2_rn(a, c);
-          const float ha = __low2float(h), hc = __high2float(h);
-          const __half2 l = __floats2half2_rn(a - ha, c - hc);
-          sh += mul * (ha + hc);
-          sl += mul * (__low2float(l) + __high2float(l));
-          hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-          lo[i / 2] = *reinterpret_cast<const uint32_t*>(&l);
-        }
-      }
-      sh += __shfl_xor_sync(0xffffffffu, sh, 1);
-      sl += __shfl_xor_sync(0xffffffffu, sl, 1);
-      sh += __shfl_xor_sync(0xffffffffu, sh, 2);
-      sl += __shfl_xor_sync(0xffffffffu, sl, 2);
-      if (b < nb) {
-        uint8_t* r = rec + (size_t)(cg * nb + b) * kXRec;
-        *reinterpret_cast<uint4*>(r + w * 64 + t * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(r + 256 + w * 64 + t * 16) =
-            make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if (t == 0) {
-          const float k = -quant_offset<QT>() / kSubUnit;
-          float* cor = reinterpret_cast<float*>(r + 512);
-          cor[4 * (w >> 1) + (w & 1)] = cor[4 * (w >> 1) + (w & 1) + 2] = k * sh;
-          cor[4 * (2 + (w >> 1)) + (w & 1)] = cor[4 * (2 + (w >> 1)) + (w & 1) + 2] = k * sl;
-        }
+      for (int i = 0; i < 8; i += 2) {
+        // register slots i, i + 1 hold elements 0, 2 | 1, 3 of each four (Q4_0)
+        const int p = QT == MOE_Q4_0 ? (i & 4) + ((i & 2) ? 1 : 0) : i;
+        const int q = QT == MOE_Q4_0 ? p + 2 : i + 1;
+        // high nibbles stay 16 times too large; their x is stored / 16
+        const float div = QT == MOE_Q4_0 && i >= 4 ? 0.0625f : 1.f;
+        const float mul = QT == MOE_Q4_0 && i >= 4 ? 16.f : 1.f;
+        const float a = v[p] * f1 * f2 * div, c = v[q] * f1 * f2 * div;
+        const __half2 h = __floats2half2_rn(a, c);
+        const float ha = __low2float(h), hc = __high2float(h);
+        const __half2 l = __floats2half2_rn(a - ha, c - hc);
+        sh += mul * (ha + hc);
+        sl += mul * (__low2float(l) + __high2float(l));
+        hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+        lo[i / 2] = *reinterpret_cast<const uint32_t*>(&l);
       }
     }
-  // rows of the column groups that no warp has
-  for (int i = tid; i < (4 * G - P) * nb; i += kLinWarps * 32) {
-    const int r = P + i / nb, b = i % nb, z = r & 3;
-    uint8_t* p = rec + (size_t)((r >> 2) * nb + b) * kXRec;
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      *reinterpret_cast<uint4*>(p + (q >> 2) * 256 + z * 64 + (q & 3) * 16) = make_uint4(0, 0, 0, 0);
-    float* cor = reinterpret_cast<float*>(p + 512);
-    cor[4 * (z >> 1) + (z & 1)] = cor[4 * (z >> 1) + (z & 1) + 2] = 0.f;
-    cor[4 * (2 + (z >> 1)) + (z & 1)] = cor[4 * (2 + (z >> 1)) + (z & 1) + 2] = 0.f;
+    sh += __shfl_xor_sync(0xffffffffu, sh, 1);
+    sl += __shfl_xor_sync(0xffffffffu, sl, 1);
+    sh += __shfl_xor_sync(0xffffffffu, sh, 2);
+    sl += __shfl_xor_sync(0xffffffffu, sl, 2);
+    if (b < real) {
+      const int pair = (b % NBG) * TOK + row % TOK;
+      uint8_t* r = rec + (size_t)(b * G + cg) * 512 + pair * 128 + t * 16;
+      *reinterpret_cast<uint4*>(r) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(r + 64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      const float k = -quant_offset<QT>() / kSubUnit;
+      if (t == 0)
+        cor[(b / NBG * G + cg) * 4 + pair] = make_float2(k * sh, k * sl);
+    }
   }
 }
 
-template <int QT, int G>
+template <int QT, int NBG, int G>
 __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs A) {
   using Tr = QTraits<QT>;
-  constexpr int U = kLinU, TB = Tr::kTileBytes, STAGE = 2 * U * TB;
-  constexpr int NRED = 2 * G * 4 * 16;           // floats of a pair: 32 rows x 4 G tokens
+  using Cfg = LinCfg<NBG, G>;
+  constexpr int U = kLinU, TB = Tr::kTileBytes, STAGE = 2 * U * TB, NRED = Cfg::kRed;
+  constexpr int TOK = Cfg::kTok;
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* const bars_all = reinterpret_cast<uint64_t*>(smem);
   uint32_t* const smax = reinterpret_cast<uint32_t*>(smem + 1024);
@@ -167,14 +174,15 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % A.cs, cluster = blockIdx.x / A.cs, nclusters = gridDim.x / A.cs;
   const int groups = kLinWarps / A.ks, group = warp / A.ks, kq = warp % A.ks;
-  const int row0 = blockIdx.y * 4 * G, n = min(4 * G, A.T - row0);
-  // columns: this CTA's tiles, this warp's
-  const int tps = (A.kt + A.cs - 1) / A.cs, t0 = min(A.kt, rank * tps), t1 = min(A.kt, t0 + tps);
-  const int wps = (t1 - t0 + A.ks - 1) / A.ks;
+  const int row0 = blockIdx.y * Cfg::kRows, n = min(Cfg::kRows, A.T - row0);
+  // columns: this CTA's tiles, this warp's (an even number: whole stages)
+  const int tps = A.tps, t0 = min(A.kt, rank * tps), t1 = min(A.kt, t0 + tps);
+  const int wps = ((t1 - t0 + A.ks - 1) / A.ks + 1) / 2 * 2;
   const int wt0 = min(t1, t0 + kq * wps), wt1 = min(t1, wt0 + wps), nt = wt1 - wt0;
-  const int nb = 2 * (t1 - t0);
+  const int rec_blocks = 2 * tps;                // tps is even
   uint8_t* const rec = smem + kLinHead;
-  float* const red = reinterpret_cast<float*>(rec + (size_t)G * 2 * tps * kXRec);
+  float2* const cor = reinterpret_cast<float2*>(rec + (size_t)G * rec_blocks * 512);
+  float* const red = reinterpret_cast<float*>(rec + (size_t)tps * Cfg::kTileBytes);
   float* const part = red + (A.ks > 1 ? kLinWarps * NRED : 0);
   uint8_t* const ring =
       reinterpret_cast<uint8_t*>(part + (A.cs > 1 ? 2 * groups * NRED : 0)) + warp * A.nst * STAGE;
@@ -196,170 +204,192 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
   const uint64_t pol = evict_first_policy();
   const int strips = (A.rows + 15) / 16;
   int ip = p0, ij = 0, islot = 0, issued = 0;
-  auto issue = [&]() {                           // lane 0
-    const uint32_t bytes = (uint32_t)(min(U, nt - ij * U) * TB);
-    const uint8_t* src = A.w + ((int64_t)2 * ip * A.kt + wt0 + ij * U) * TB;
-    const bool two = 2 * ip + 1 < strips;
-    uint8_t* dst = ring + islot * STAGE;
-    mbar_expect_tx(&bars[islot], two ? 2 * bytes : bytes);
-    bulk_g2s(dst, src, bytes, &bars[islot], pol);
-    if (two) bulk_g2s(dst + U * TB, src + (int64_t)A.kt * TB, bytes, &bars[islot], pol);
-  };
-  auto step = [&]() {
+  const int64_t strip = (int64_t)A.kt * TB;      // bytes from strip to strip
+  const uint8_t* src = A.w + 2 * ip * strip + (int64_t)wt0 * TB;
+  const int last = (nt - (nsr - 1) * U) * TB;    // bytes of a pair's last stage
+  auto issue = [&]() {                           // stage `issued`
+    if (lane == 0) {
+      const uint32_t bytes = ij == nsr - 1 ? last : U * TB;
+      const bool two = 2 * ip + 1 < strips;
+      uint8_t* dst = ring + islot * STAGE;
+      mbar_expect_tx(&bars[islot], two ? 2 * bytes : bytes);
+      bulk_g2s(dst, src, bytes, &bars[islot], pol);
+      if (two) bulk_g2s(dst + U * TB, src + strip, bytes, &bars[islot], pol);
+    }
     ++issued;
+    src += U * TB;
     islot = islot + 1 == A.nst ? 0 : islot + 1;
     if (++ij == nsr) {
       ij = 0;
       ip += pstep;
+      src += 2 * pstep * strip - (int64_t)nsr * U * TB;
     }
   };
-  for (int q = 0; q < A.nst && q < total; ++q) {
-    if (lane == 0) issue();
-    step();
-  }
-  build_fragments<QT, G>(A, rec, ex, smax, row0, n, t0, t1);
+  for (int q = 0; q < A.nst && q < total; ++q) issue();
+  build_fragments<QT, NBG, G>(A, rec, cor, rec_blocks, ex, smax, row0, n, t0, t1);
   __syncthreads();
 
   // ---- stream
   bool ok = true;
   int slot = 0;
   uint32_t phase = 0;
-  const uint8_t* const xl = rec + lane * 16 + (size_t)2 * (wt0 - t0) * kXRec;
-  const uint8_t* const cl = rec + 512 + t * 16 + (size_t)2 * (wt0 - t0) * kXRec;
-  const int cstride = nb * kXRec;
-  // place `at` = 2 g + t of strip s, column group cg, value i of an MMA result
-  auto put = [&](int p, int s, int cg, int i, int at, float y) {
-    const int tok = 4 * cg + 2 * (at & 1) + (i & 1), row = 32 * p + 16 * s + (at >> 1) + 8 * (i >> 1);
-    if (tok < n && row < A.rows) {
+  // fragments and corrections of this warp's columns
+  const uint8_t* const xl = rec + lane * 16 + (size_t)2 * (wt0 - t0) * G * 512;
+  const float2* const cl = cor + t + 2 * (wt0 - t0) / NBG * G * 4;
+  // value i (row g + 8 i) of strip s, column group cg in lane l
+  auto put = [&](int p, int s, int cg, int i, int l, float y) {
+    const int tok = TOK * cg + (l & 3), row = 32 * p + 16 * s + (l >> 2) + 8 * i;
+    if ((l & 3) < TOK && tok < n && row < A.rows) {
       if (A.residual) y += A.residual[(int64_t)(row0 + tok) * A.rs + row];
       A.y[(int64_t)(row0 + tok) * A.ys + row] = y;
     }
   };
   for (int r = 0; r < A.rounds; ++r) {
     const int p = p0 + r * pstep;
-    float2 acc[2][G][2];
+    float v[2][G][2];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int cg = 0; cg < G; ++cg) acc[s][cg][0] = acc[s][cg][1] = make_float2(0.f, 0.f);
+      for (int cg = 0; cg < G; ++cg) v[s][cg][0] = v[s][cg][1] = 0.f;
     if (p < A.pairs) {
       for (int j = 0; j < nsr; ++j) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bars[slot], phase));
-        const uint8_t* st = ring + slot * STAGE + 0;
-        TileRegs<QT> w[2][U];
+        if (ok && !mbar_wait(&bars[slot], phase)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        const uint8_t* st = ring + slot * STAGE;
+        const uint8_t* xq = xl + j * (U * 2 * G * 512);
+        const float2* cq = cl + j * (U * 2 / NBG * G * 4);
+        const int left = nt - j * U;             // tiles of the stage, 2 or more: both
+        float c[2][G][4];
+        auto begin = [&](int grp) {              // offset corrections of a group of blocks
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+          for (int cg = 0; cg < G; ++cg) {
+            const float2 z = cq[(grp * G + cg) * 4];
 #pragma unroll
-          for (int u = 0; u < U; ++u) lds_tile<QT>(w[s][u], st + (s * U + u) * TB, lane);
-        __syncwarp();
-        if (ok && issued < total) {
-          if (lane == 0) {
-            fence_proxy_async_smem();
-            issue();
+            for (int s = 0; s < 2; ++s) {
+              c[s][cg][0] = c[s][cg][2] = z.x;
+              c[s][cg][1] = c[s][cg][3] = z.y;
+            }
           }
-          step();
+        };
+        auto finish = [&](int tile, int half, bool valid) {   // scales of this lane's block
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const __half* d = reinterpret_cast<const __half*>(st + (s * U + tile) * TB +
+                                                              Tr::kTileQuant + g * 8) + half;
+            const float d0 = valid ? __half2float(d[0]) : 0.f;
+            const float d8 = valid ? __half2float(d[2]) : 0.f;
+#pragma unroll
+            for (int cg = 0; cg < G; ++cg) {
+              v[s][cg][0] = fmaf(d0, c[s][cg][0] + c[s][cg][1], v[s][cg][0]);
+              v[s][cg][1] = fmaf(d8, c[s][cg][2] + c[s][cg][3], v[s][cg][1]);
+            }
+          }
+        };
+        if (NBG == 4) begin(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (u == 0 || u < left) {
+            TileRegs<QT> w[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) lds_quants<QT>(w[s], st + (s * U + u) * TB, lane);
+            if (NBG == 2) begin(u);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              if (NBG == 1) begin(2 * u + b);
+              uint32_t a0[2][4], a1[2][4];
+#pragma unroll
+              for (int s = 0; s < 2; ++s) tile_quants<QT, true>(w[s], b, a0[s], a1[s]);
+#pragma unroll
+              for (int cg = 0; cg < G; ++cg) {
+                const uint4 xf =
+                    *reinterpret_cast<const uint4*>(xq + ((2 * u + b) * G + cg) * 512);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                  mma_16816(c[s][cg], a0[s][0], a0[s][1], a0[s][2], a0[s][3], xf.x, xf.y, c[s][cg]);
+                  mma_16816(c[s][cg], a1[s][0], a1[s][1], a1[s][2], a1[s][3], xf.z, xf.w, c[s][cg]);
+                }
+              }
+              if (NBG == 1) finish(u, b, true);
+            }
+            if (NBG == 2) finish(u, t >> 1, true);
+          }
         }
+        if (NBG == 4) finish(t >> 1, t & 1, (t >> 1) < left);
+        __syncwarp();                            // the stage has been read
+        if (ok && issued < total) issue();
         if (++slot == A.nst) {
           slot = 0;
           phase ^= 1u;
         }
-        const int off = 2 * j * U * kXRec;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (j * U + u < nt) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              uint32_t a0[2][4], a1[2][4];
-              float2 d0[2], d8[2];
-#pragma unroll
-              for (int s = 0; s < 2; ++s)
-                tile_afrags<QT, true>(w[s][u], b, a0[s], a1[s], d0[s], d8[s]);
-#pragma unroll
-              for (int cg = 0; cg < G; ++cg) {
-                const int o = off + (2 * u + b) * kXRec + cg * cstride;
-                const uint4 xf = *reinterpret_cast<const uint4*>(xl + o);
-                const float4 c0 = *reinterpret_cast<const float4*>(cl + o);
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-                  block_mma(acc[s][cg], a0[s], a1[s], xf, c0, d0[s], d8[s]);
-              }
-            }
-          }
-        }
       }
     }
-    // hi + lo: columns 2t, 2t + 1 and those 4 further on; lanes t < 2 keep
-    // rows g, g + 8 of tokens 4 cg + 2t, + 1
-    float v[2][G][4];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int cg = 0; cg < G; ++cg)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = (i & 1) ? acc[s][cg][i >> 1].y : acc[s][cg][i >> 1].x;
-          v[s][cg][i] = ok ? a + __shfl_xor_sync(0xffffffffu, a, 2)
-                           : __uint_as_float(0x7fffffffu);   // a wait ran out: NaN
+        for (int i = 0; i < 2; ++i) {
+          if (NBG >= 2) v[s][cg][i] += __shfl_xor_sync(0xffffffffu, v[s][cg][i], 2);
+          if (NBG == 4) v[s][cg][i] += __shfl_xor_sync(0xffffffffu, v[s][cg][i], 1);
+          if (!ok) v[s][cg][i] = __uint_as_float(0x7fffffffu);   // a wait ran out: NaN
         }
-    const int at = g * 2 + t;                    // lanes t < 2: 16 places
     if (A.ks > 1) {
       // the column parts of a pair meet in the group's first warp
       if (r > 0) asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * A.ks) : "memory");
-      if (kq > 0 && t < 2)
+      if (kq > 0)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
           for (int cg = 0; cg < G; ++cg)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              red[warp * NRED + ((s * G + cg) * 4 + i) * 16 + at] = v[s][cg][i];
+            for (int i = 0; i < 2; ++i)
+              red[warp * NRED + ((s * G + cg) * 2 + i) * 32 + lane] = v[s][cg][i];
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * A.ks) : "memory");
-      if (kq == 0 && t < 2)
+      if (kq == 0)
         for (int k = 1; k < A.ks; ++k)
 #pragma unroll
           for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int cg = 0; cg < G; ++cg)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                v[s][cg][i] += red[(warp + k) * NRED + ((s * G + cg) * 4 + i) * 16 + at];
+              for (int i = 0; i < 2; ++i)
+                v[s][cg][i] += red[(warp + k) * NRED + ((s * G + cg) * 2 + i) * 32 + lane];
     }
-    const bool lead = kq == 0 && t < 2 && p < A.pairs;
+    const bool lead = kq == 0 && p < A.pairs;
     if (lead) {
 #pragma unroll
-      for (int cg = 0; cg < G; ++cg)
+      for (int cg = 0; cg < G; ++cg) {
+        const int e = ex[TOK * cg + (t < TOK ? t : 0)];
+        const float f1 = pow2f(-(e / 2)), f2 = pow2f(-(e - e / 2));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = ex[4 * cg + 2 * t + (i & 1)];
-          const float f1 = pow2f(-(e / 2)), f2 = pow2f(-(e - e / 2));
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int s = 0; s < 2; ++s) v[s][cg][i] = v[s][cg][i] * kSubUnit * f1 * f2;
-        }
+          for (int i = 0; i < 2; ++i) v[s][cg][i] = v[s][cg][i] * kSubUnit * f1 * f2;
+      }
     }
     if (A.cs == 1) {
       if (lead) {
-#pragma unroll
-        for (int cg = 0; cg < G; ++cg)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-              put(p, s, cg, i, at, v[s][cg][i]);
-      }
-    } else {
-      // the CTAs' parts: every thread of the cluster adds up its places
-      float* mine_p = part + (size_t)(r & 1) * groups * NRED;
-      if (kq == 0 && t < 2)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
           for (int cg = 0; cg < G; ++cg)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              mine_p[group * NRED + ((s * G + cg) * 4 + i) * 16 + at] = v[s][cg][i];
+            for (int i = 0; i < 2; ++i) put(p, s, cg, i, lane, v[s][cg][i]);
+      }
+    } else {
+      // the CTAs' parts: every thread of the cluster adds up its places
+      float* mine_p = part + (size_t)(r & 1) * groups * NRED;
+      if (kq == 0)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int cg = 0; cg < G; ++cg)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              mine_p[group * NRED + ((s * G + cg) * 2 + i) * 32 + lane] = v[s][cg][i];
       cluster_sync();
       for (int e = rank * kLinWarps * 32 + tid; e < groups * NRED; e += A.cs * kLinWarps * 32) {
-        const int pe = cluster * groups + e / NRED + r * pstep, k = e % NRED / 16;
+        const int pe = cluster * groups + e / NRED + r * pstep, k = e % NRED / 32;
         const uint32_t a = smem_u32(mine_p + e);
         float f[8];
 #pragma unroll
@@ -367,7 +397,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
         float y = f[0];
 #pragma unroll
         for (int c = 1; c < 8; ++c) y += f[c];
-        if (pe < A.pairs) put(pe, k / (4 * G), k / 4 % G, k % 4, e % 16, y);
+        if (pe < A.pairs) put(pe, k / (2 * G), k / 2 % G, k % 2, e % 32, y);
       }
     }
   }
@@ -380,49 +410,51 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
   if (A.cs > 1) cluster_sync();                  // nobody reads this CTA's parts any more
 }
 
+// Tiles of a CTA's columns: an even number, so that a stage is two of them.
+inline int linear_tps(int kt, int cs) { return ((kt + cs - 1) / cs + 1) / 2 * 2; }
+
 // Shared memory of a split; nst ring stages take what is left.
-template <int QT, int G>
+template <int QT, int NBG, int G>
 static size_t linear_smem(int kt, int cs, int ks, int nst) {
-  const size_t nred = (size_t)2 * G * 4 * 16 * 4;
-  const int tps = (kt + cs - 1) / cs;
-  return kLinHead + (size_t)G * 2 * tps * kXRec + (ks > 1 ? kLinWarps * nred : 0) +
+  using Cfg = LinCfg<NBG, G>;
+  const size_t nred = (size_t)Cfg::kRed * 4;
+  return kLinHead + (size_t)linear_tps(kt, cs) * Cfg::kTileBytes + (ks > 1 ? kLinWarps * nred : 0) +
          (cs > 1 ? 2 * (kLinWarps / ks) * nred : 0) +
          (size_t)kLinWarps * nst * 2 * kLinU * QTraits<QT>::kTileBytes;
 }
 
-template <int QT, int G>
-static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
-  // Estimated time of a split, in the time all warps of an SM take for one tile
-  // pair each (about 800 cycles of HBM): rounds x (tiles of a warp, and the
-  // meetings of warps, 3, and of a cluster, 8), and the fragments, 4 G rows of
-  // the CTA's columns (28 cycles per group and tile).
-  const int sms = sm_count();
-  double best = 0;
-  a.cs = 0;
-  for (int cs = 1; cs <= 8; cs *= 2)
-    for (int ks = 1; ks <= kLinWarps; ks *= 2) {
-      if (linear_smem<QT, G>(a.kt, cs, ks, 2) > kLinSmem) continue;
-      const int tps = (a.kt + cs - 1) / cs, wt = (tps + ks - 1) / ks;
-      const int slots = sms / cs * (kLinWarps / ks);
-      const int rounds = (a.pairs + slots - 1) / slots;
-      const double t = rounds * (wt * (1 + 0.25 * (G - 1)) + (ks > 1 ? 3 : 0) + (cs > 1 ? 8 : 0)) +
-                       0.035 * G * tps;
-      if (a.cs == 0 || t < best) {
-        best = t;
-        a.cs = cs;
-        a.ks = ks;
-      }
+// Clusters of cs CTAs that are resident at once (a cluster stays inside one GPC:
+// 148 SMs hold 74, 33 and 15 clusters of 2, 4 and 8).
+static int resident_clusters(const void* kern, int cs, int dev) {
+  static std::atomic<int> known[64][4];
+  const int k = cs == 2 ? 1 : cs == 4 ? 2 : 3;
+  if (cs == 1) return sm_count();
+  int n = dev < 64 ? known[dev][k].load() : 0;
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(cs * 148));
+    cfg.blockDim = dim3(kLinWarps * 32);
+    cfg.dynamicSmemBytes = kLinSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cs;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = std::max(1, sm_count() / (2 * cs));
     }
-  fits = a.cs > 0;
-  if (!fits) return MOE_OK;
-  a.nst = 2;
-  while (a.nst < kLinMaxStages && linear_smem<QT, G>(a.kt, a.cs, a.ks, a.nst + 1) <= kLinSmem)
-    ++a.nst;
-  const int per = kLinWarps / a.ks;                  // pairs of a cluster's round
-  const int clusters = std::min(sms / a.cs, (a.pairs + per - 1) / per);
-  a.rounds = (a.pairs + clusters * per - 1) / (clusters * per);
-  const size_t smem = linear_smem<QT, G>(a.kt, a.cs, a.ks, a.nst);
-  auto kern = linear_kernel<QT, G>;
+    if (dev < 64) known[dev][k].store(n);
+  }
+  return n;
+}
+
+template <int QT, int NBG, int G>
+static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
+  using Cfg = LinCfg<NBG, G>;
+  auto kern = linear_kernel<QT, NBG, G>;
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
   MOE_CUDA(cudaGetDevice(&dev));
@@ -430,10 +462,44 @@ static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
     MOE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem));
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
+  // Estimated time of a split, in the time all warps of an SM take for one tile
+  // of two strips each (about 800 cycles of HBM): rounds x (tiles of a warp, and
+  // the meetings of warps, 3, and of a cluster, 8), and the fragments of the
+  // CTA's columns (28 cycles per group and tile).
+  double best = 0;
+  int clusters = 0;
+  a.cs = 0;
+  for (int cs = 1; cs <= 8; cs *= 2) {
+    if (linear_smem<QT, NBG, G>(a.kt, cs, kLinWarps, 2) > kLinSmem) continue;
+    const int resident = resident_clusters((const void*)kern, cs, dev);
+    for (int ks = 1; ks <= kLinWarps; ks *= 2) {
+      if (linear_smem<QT, NBG, G>(a.kt, cs, ks, 2) > kLinSmem) continue;
+      const int tps = linear_tps(a.kt, cs), wt = ((tps + ks - 1) / ks + 1) / 2 * 2;
+      const int slots = resident * (kLinWarps / ks);
+      const int rounds = (a.pairs + slots - 1) / slots;
+      const double t = rounds * (wt * (1 + 0.25 * (G - 1)) + (ks > 1 ? 3 : 0) + (cs > 1 ? 8 : 0)) +
+                       0.035 * G * tps;
+      if (a.cs == 0 || t < best) {
+        best = t;
+        a.cs = cs;
+        a.ks = ks;
+        clusters = resident;
+      }
+    }
+  }
+  fits = a.cs > 0;
+  if (!fits) return MOE_OK;
+  a.tps = linear_tps(a.kt, a.cs);
+  a.nst = 2;
+  while (a.nst < kLinMaxStages && linear_smem<QT, NBG, G>(a.kt, a.cs, a.ks, a.nst + 1) <= kLinSmem)
+    ++a.nst;
+  const int per = kLinWarps / a.ks;                  // pairs of a cluster's round
+  clusters = std::min(clusters, (a.pairs + per - 1) / per);
+  a.rounds = (a.pairs + clusters * per - 1) / (clusters * per);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(clusters * a.cs), (unsigned)((a.T + 4 * G - 1) / (4 * G)));
+  cfg.gridDim = dim3((unsigned)(clusters * a.cs), (unsigned)((a.T + Cfg::kRows - 1) / Cfg::kRows));
   cfg.blockDim = dim3(kLinWarps * 32);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = linear_smem<QT, NBG, G>(a.kt, a.cs, a.ks, a.nst);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -448,14 +514,16 @@ static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
   return MOE_OK;
 }
 
-// Column groups of 4 rows: as many as T needs, fewer where x is so wide that
-// more do not fit.
+// Rows of a pass: as many as T needs (1, 2, 4, 8 or 16), fewer where x is so wide
+// that their fragments do not fit.
 template <int QT>
 static int launch_linear_qt(LinArgs& a, cudaStream_t s) {
   bool fits = false;
-  if (a.T > 8) MOE_CHECK((launch_linear<QT, 4>(a, s, fits)));
-  if (!fits && a.T > 4) MOE_CHECK((launch_linear<QT, 2>(a, s, fits)));
-  if (!fits) MOE_CHECK((launch_linear<QT, 1>(a, s, fits)));
+  if (a.T > 8) MOE_CHECK((launch_linear<QT, 1, 4>(a, s, fits)));
+  if (!fits && a.T > 4) MOE_CHECK((launch_linear<QT, 1, 2>(a, s, fits)));
+  if (!fits && a.T > 2) MOE_CHECK((launch_linear<QT, 1, 1>(a, s, fits)));
+  if (!fits && a.T == 2) MOE_CHECK((launch_linear<QT, 2, 1>(a, s, fits)));
+  if (!fits && a.T == 1) MOE_CHECK((launch_linear<QT, 4, 1>(a, s, fits)));
   MOE_REQUIRE(fits, MOE_ERR_UNSUPPORTED, "cols %d: rows of x this wide do not fit", a.cols);
   return MOE_OK;
 }

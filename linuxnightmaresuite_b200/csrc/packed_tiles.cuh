@@ -56,11 +56,15 @@ struct TileRegs {
 
 // fragment registers of one staged tile (shared memory, lane-contiguous)
 template <int QT>
-__device__ __forceinline__ void lds_tile(TileRegs<QT>& r, const uint8_t* tile, int lane) {
-  using Tr = QTraits<QT>;
-  const uint8_t* qp = tile + lane * Tr::kLaneBytes;
+__device__ __forceinline__ void lds_quants(TileRegs<QT>& r, const uint8_t* tile, int lane) {
+  const uint8_t* qp = tile + lane * QTraits<QT>::kLaneBytes;
   r.q[0] = *reinterpret_cast<const uint4*>(qp);
   if (QT == MOE_Q8_0) r.q[QT == MOE_Q4_0 ? 0 : 1] = *reinterpret_cast<const uint4*>(qp + 16);
+}
+template <int QT>
+__device__ __forceinline__ void lds_tile(TileRegs<QT>& r, const uint8_t* tile, int lane) {
+  using Tr = QTraits<QT>;
+  lds_quants<QT>(r, tile, lane);
   r.sc = *reinterpret_cast<const uint2*>(tile + Tr::kTileQuant + (lane >> 2) * 8);
 }
 
@@ -82,12 +86,12 @@ __device__ __forceinline__ void dequant_q8_sub(uint32_t w, uint32_t& h01, uint32
   h23 = prmt(u, 0u, 0x4342u);
 }
 
-// A fragments of both k16 steps for block b (rows g and g+8), block scales.
+// A fragments of both k16 steps for block b (rows g and g+8).
 // SUB: subnormal quants (offset handled by the accumulator's initial value);
 // otherwise exact signed fp16 integers.
 template <int QT, bool SUB>
-__device__ __forceinline__ void tile_afrags(const TileRegs<QT>& r, int b, uint32_t (&a0)[4],
-                                            uint32_t (&a1)[4], float2& dg, float2& dg8) {
+__device__ __forceinline__ void tile_quants(const TileRegs<QT>& r, int b, uint32_t (&a0)[4],
+                                            uint32_t (&a1)[4]) {
   if (QT == MOE_Q4_0) {
     uint32_t wg = b ? r.q[0].y : r.q[0].x;
     uint32_t w8 = b ? r.q[0].w : r.q[0].z;
@@ -124,6 +128,13 @@ __device__ __forceinline__ void tile_afrags(const TileRegs<QT>& r, int b, uint32
     }
     a1[0] = x01; a1[1] = y01; a1[2] = x23; a1[3] = y23;
   }
+}
+
+// The same with the block's scales.
+template <int QT, bool SUB>
+__device__ __forceinline__ void tile_afrags(const TileRegs<QT>& r, int b, uint32_t (&a0)[4],
+                                            uint32_t (&a1)[4], float2& dg, float2& dg8) {
+  tile_quants<QT, SUB>(r, b, a0, a1);
   const float s0 = b ? half_hi(r.sc.x) : half_lo(r.sc.x);
   const float s8 = b ? half_hi(r.sc.y) : half_lo(r.sc.y);
   dg = make_float2(s0, s0);
