@@ -115,10 +115,10 @@ SIGNATURES = {
     "moe_ep_forward_phases": [vp, ci, ci, vp, vp, vp, ci, vp, vp, ci, ci, vp, csz, vp],
     "moe_layer_workspace_bytes": [ctypes.POINTER(MoELayerWeights), ci, ctypes.POINTER(csz)],
     "moe_layer_forward": [ctypes.POINTER(MoELayerWeights), vp, ci, vp, vp, vp, vp, vp, csz, vp],
-    "moe_rope_append": [ctypes.POINTER(MoEPagedCache), vp, ci64, ci64, vp, ci64, ci64, vp, ci64,
+    "moe_rope_append": [vp, vp, ci64, ci64, vp, ci64, ci64, vp, ci64,
                         ci64, ci, ci, vp, vp, vp, ci, ci, vp, ci64, ci64, vp, vp],
     "moe_paged_attention_workspace_bytes": [ci, ci, ci, ci, ctypes.POINTER(csz)],
-    "moe_paged_attention": [ctypes.POINTER(MoEPagedCache), vp, ci64, ci64, vp, ci, ci, ci, cf, cf,
+    "moe_paged_attention": [vp, vp, ci64, ci64, vp, ci, ci, ci, cf, cf,
                             vp, vp, vp, csz, vp],
     "moe_linear": [vp, ci, ci, ci, vp, ci64, ci, vp, ci64, vp, ci64, vp],
 }
@@ -186,5 +186,13 @@ def check(status: int) -> None:
         raise MoEError(status, last_error())
 
 
+_entries = {}
+
+
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args))
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(load(), name)
+    status = fn(*args)
+    if status != MOE_OK:
+        check(status)

@@ -7,6 +7,7 @@ are not contiguous CUDA tensors of the right dtype are rejected.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -265,66 +266,85 @@ CACHE_TYPES = {torch.float16: _lib.MOE_CACHE_F16, torch.bfloat16: _lib.MOE_CACHE
                torch.float8_e4m3fn: _lib.MOE_CACHE_E4M3}
 
 
-def _call_on(device: torch.device, name: str, *args) -> None:
-    """The entry point on ``device`` and its current stream, whichever device
-    is current."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, _stream())
+# A cache as the entry points read it (moe_paged_cache), packed in one step.
+_CACHE_STRUCT = struct.Struct("@3P4q7i2f0q")
+assert _CACHE_STRUCT.size == ctypes.sizeof(_lib.MoEPagedCache)
+
+
+def _call_on(index: int, name: str, *args) -> None:
+    """The entry point on device ``index`` and its current stream, whichever
+    device is current."""
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            call(name, *args, _stream())
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _rows_f32(t: torch.Tensor, name: str, device, shape=None) -> torch.Tensor:
-    """A CUDA f32 tensor whose last axis is contiguous; other axes may stride."""
+# These wrappers are called once per layer and token, on kernels of a few
+# microseconds, so each check of an argument is one expression; what it refuses
+# is told apart here.
+def _refuse(t, name: str, dtype, index: int, shape=None) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
-    if t.dtype != torch.float32:
-        raise TypeError(f"{name} must be {torch.float32}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} is {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    raise ValueError(f"{name} must be contiguous")
+
+
+_F32, _I32 = torch.float32, torch.int32
+
+
+def _rows_f32(t: torch.Tensor, name: str, index: int, shape) -> Tuple[int, ...]:
+    """Strides of a CUDA f32 tensor of the shape whose last axis is contiguous;
+    the other axes may stride."""
+    if t.dtype is not _F32 or t.get_device() != index or t.shape != shape:
+        _refuse(t, name, _F32, index, shape)
+    strides = t.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"the last axis of {name} must be contiguous")
-    return t
+    return strides
 
 
-def _i32(t: torch.Tensor, name: str, device, n: Optional[int] = None) -> torch.Tensor:
-    _need(t, torch.int32, name)
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if n is not None and (t.dim() != 1 or t.shape[0] != n):
-        raise ValueError(f"{name} is {tuple(t.shape)}, expected ({n},)")
-    return t
+def _vector(t: torch.Tensor, dtype, name: str, index: int, n: int) -> int:
+    """Address of a contiguous CUDA vector of n elements."""
+    if t.dtype is not dtype or t.get_device() != index or t.shape != (n,) or \
+            not t.is_contiguous():
+        _refuse(t, name, dtype, index, (n,))
+    return t.data_ptr()
 
 
 def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
-                 k_scale: float, v_scale: float) -> _lib.MoEPagedCache:
-    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise TypeError(f"{n} must be a CUDA tensor")
-    dtype = CACHE_TYPES.get(k_cache.dtype)
-    if dtype is None or v_cache.dtype != k_cache.dtype:
-        raise TypeError(f"caches of {k_cache.dtype} and {v_cache.dtype}: both must be one of "
-                        f"{', '.join(str(t) for t in CACHE_TYPES)}")
+                 k_scale: float, v_scale: float):
+    """(packed moe_paged_cache, device index, sequences, kv_heads, head_dim)."""
+    index, dtype = k_cache.get_device(), k_cache.dtype
+    if index < 0:
+        raise TypeError("k_cache must be a CUDA tensor")
+    kind = CACHE_TYPES.get(dtype)
+    if kind is None:
+        raise TypeError(f"caches of {dtype}: one of "
+                        f"{', '.join(str(t) for t in CACHE_TYPES)} is needed")
     shape, strides = k_cache.shape, k_cache.stride()
+    if v_cache.dtype is not dtype or v_cache.get_device() != index:
+        _refuse(v_cache, "v_cache", dtype, index)
     if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != strides:
         raise ValueError("k_cache and v_cache must be (pages, page_size, kv_heads, head_dim) of "
                          "the same shape and strides")
     if strides[3] != 1 and shape[3] > 1:
         raise ValueError("the last axis of the caches must be contiguous")
-    for t, n in ((v_cache, "v_cache"), (block_table, "block_table")):
-        if t.device != k_cache.device:
-            raise ValueError(f"{n} is on {t.device}, expected {k_cache.device}")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be int32 (sequences, pages of a sequence) with "
-                         "contiguous rows")
-    return _lib.MoEPagedCache(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-                              strides[0], strides[1], strides[2], block_table.stride(0), dtype,
-                              shape[0], shape[1], shape[2], shape[3], block_table.shape[0],
-                              block_table.shape[1], k_scale, v_scale)
+    if block_table.dtype is not _I32 or block_table.get_device() != index:
+        _refuse(block_table, "block_table", _I32, index)
+    table, trow = block_table.shape, block_table.stride()
+    if len(table) != 2 or (trow[1] != 1 and table[1] > 1):
+        raise ValueError("block_table must be (sequences, pages of a sequence) with contiguous "
+                         "rows")
+    return _CACHE_STRUCT.pack(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                              strides[0], strides[1], strides[2], trow[0], kind, *shape, *table,
+                              k_scale, v_scale), index, table[0], shape[2], shape[3]
 
 
 def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
@@ -345,37 +365,31 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     its token, q row included; no two tokens may share sequence and position.
     ``status`` (int32) receives STATUS_BAD_PAGE for a page or sequence that
     does not exist; such a token's k and v are not stored."""
-    c = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
-    dev = k_cache.device
+    c, dev, _, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
     T = k.shape[0]
-    _rows_f32(k, "k", dev, (T, c.kv_heads, c.head_dim))
-    _rows_f32(v, "v", dev, (T, c.kv_heads, c.head_dim))
-    _i32(positions, "positions", dev, T)
-    if seq_ids is not None:
-        _i32(seq_ids, "seq_ids", dev, T)
-    if status is not None:
-        _i32(status, "status", dev)
-    rot = 0
+    ks = _rows_f32(k, "k", dev, (T, hk, d))
+    vs = _rows_f32(v, "v", dev, (T, hk, d))
+    rot, freq = 0, None
     if inv_freq is not None:
-        _need(inv_freq, torch.float64, "inv_freq")
-        if inv_freq.device != dev:
-            raise ValueError(f"inv_freq is on {inv_freq.device}, expected {dev}")
         rot = 2 * inv_freq.numel()
-    hq, qs, os_ = 0, (0, 0), (0, 0)
+        freq = _vector(inv_freq, torch.float64, "inv_freq", dev, inv_freq.numel())
+    hq, qs, os_, q_ptr, o_ptr = 0, (0, 0), (0, 0), None, None
     if q is not None:
         if q.dim() != 3:
             raise ValueError("q must be (tokens, q_heads, head_dim)")
         hq = q.shape[1]
-        _rows_f32(q, "q", dev, (T, hq, c.head_dim))
+        qs = _rows_f32(q, "q", dev, (T, hq, d))
         if q_out is None:
-            q_out = torch.empty((T, hq, c.head_dim), dtype=torch.float32, device=dev)
+            q_out = q.new_empty((T, hq, d))
+            os_ = (hq * d, d)
         else:
-            _rows_f32(q_out, "q_out", dev, (T, hq, c.head_dim))
-        qs, os_ = q.stride(), q_out.stride()
-    _call_on(dev, "moe_rope_append", ctypes.byref(c), _ptr(q), qs[0], qs[1], _ptr(k), k.stride(0),
-             k.stride(1), _ptr(v), v.stride(0), v.stride(1), T, hq, _ptr(positions),
-             _ptr(seq_ids), _ptr(inv_freq), rot, 1 if interleaved else 0, _ptr(q_out), os_[0],
-             os_[1], _ptr(status))
+            os_ = _rows_f32(q_out, "q_out", dev, (T, hq, d))
+        q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
+    _call_on(dev, "moe_rope_append", c, q_ptr, qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+             v.data_ptr(), vs[0], vs[1], T, hq, _vector(positions, _I32, "positions", dev, T),
+             None if seq_ids is None else _vector(seq_ids, _I32, "seq_ids", dev, T), freq,
+             rot, 1 if interleaved else 0, o_ptr, os_[0], os_[1],
+             None if status is None else _vector(status, _I32, "status", dev, 1))
     return q_out
 
 
@@ -414,27 +428,25 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     length 0 gives zeros and -inf.  ``scale`` defaults to 1 / sqrt(head_dim);
     ``max_len`` (no sequence is longer; 0 = what the table holds) sizes the
     launch.  ``ws`` comes from ``paged_attention_workspace``."""
-    c = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
-    dev = k_cache.device
+    c, dev, seqs, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
     if q.dim() != 3:
         raise ValueError("q must be (sequences, q_heads, head_dim)")
     hq = q.shape[1]
-    shape = (c.seqs, hq, c.head_dim)
-    _rows_f32(q, "q", dev, shape)
-    _i32(seq_lens, "seq_lens", dev, c.seqs)
+    qs = _rows_f32(q, "q", dev, (seqs, hq, d))
     if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=dev)
-    elif _need(out, torch.float32, "out").shape != shape or out.device != dev:
-        raise ValueError(f"out is {tuple(out.shape)} on {out.device}, expected {shape} on {dev}")
-    lse = torch.empty((c.seqs, hq), dtype=torch.float32, device=dev) if return_lse else None
+        out = q.new_empty((seqs, hq, d))
+    elif out.dtype is not _F32 or out.get_device() != dev or out.shape != (seqs, hq, d) or \
+            not out.is_contiguous():
+        _refuse(out, "out", _F32, dev, (seqs, hq, d))
+    lse = q.new_empty((seqs, hq)) if return_lse else None
     if ws is None:
-        ws = paged_attention_workspace(c.seqs, hq, c.kv_heads, c.head_dim, dev)
-    elif _need(ws, torch.uint8, "ws").device != dev:
-        raise ValueError(f"ws is on {ws.device}, expected {dev}")
-    _call_on(dev, "moe_paged_attention", ctypes.byref(c), _ptr(q), q.stride(0), q.stride(1),
-             _ptr(seq_lens), hq, max_len, window,
-             c.head_dim ** -0.5 if scale is None else scale, softcap, _ptr(out), _ptr(lse),
-             _ptr(ws), ws.numel())
+        ws = paged_attention_workspace(seqs, hq, hk, d, q.device)
+    elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
+        _refuse(ws, "ws", torch.uint8, dev)
+    _call_on(dev, "moe_paged_attention", c, q.data_ptr(), qs[0], qs[1],
+             _vector(seq_lens, _I32, "seq_lens", dev, seqs), hq, max_len, window,
+             d ** -0.5 if scale is None else scale, softcap, out.data_ptr(),
+             None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel())
     return (out, lse) if return_lse else out
 
 
@@ -458,28 +470,28 @@ class LinearWeights:
                                                                pr))
         with torch.cuda.device(raw.device):
             self.packed = pack_weights(raw, qtype, 1, rows + pr, cols + pc)
+        self.index, self.address = raw.get_device(), self.packed.data_ptr()
 
 
 def linear(x: torch.Tensor, w: LinearWeights, residual: Optional[torch.Tensor] = None,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x (T, cols) f32 -> (T, rows) f32: W x[t] (+ residual[t]) for a few rows.
     Rows of x, residual and out may stride; out may be residual."""
-    dev = w.device
     if x.dim() != 2:
         raise ValueError("x must be (tokens, cols)")
-    T = x.shape[0]
-    _rows_f32(x, "x", dev, (T, w.cols))
+    dev, T = w.index, x.shape[0]
+    xs = _rows_f32(x, "x", dev, (T, w.cols))[0]
+    rs, res = 0, None
     if residual is not None:
-        _rows_f32(residual, "residual", dev, (T, w.rows))
+        rs, res = _rows_f32(residual, "residual", dev, (T, w.rows))[0], residual.data_ptr()
     if out is None:
-        out = torch.empty((T, w.rows), dtype=torch.float32, device=dev)
+        out, ys = x.new_empty((T, w.rows)), w.rows
     else:
-        _rows_f32(out, "out", dev, (T, w.rows))
-        if T > 1 and out.stride(0) < w.rows:
+        ys = _rows_f32(out, "out", dev, (T, w.rows))[0]
+        if ys < w.rows and T > 1:
             raise ValueError("rows of out overlap")
-    _call_on(dev, "moe_linear", _ptr(w.packed), w.qtype, w.rows, w.cols, _ptr(x), x.stride(0), T,
-             _ptr(residual), 0 if residual is None else residual.stride(0), _ptr(out),
-             out.stride(0))
+    _call_on(dev, "moe_linear", w.address, w.qtype, w.rows, w.cols, x.data_ptr(), xs, T, res, rs,
+             out.data_ptr(), ys)
     return out
 
 
