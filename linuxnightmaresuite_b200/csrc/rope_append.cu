@@ -10,6 +10,8 @@
 // its heads.  Bound by memory for prompts, by latency for single tokens.
 #include <math.h>
 
+#include <algorithm>
+
 #include "paged_cache.cuh"
 
 namespace moe {
@@ -46,7 +48,41 @@ __device__ __forceinline__ void cache_put(__nv_fp8_e4m3* p, float x, float scale
   p->__x = __nv_cvt_float_to_fp8(__fdiv_rn(x, scale), __NV_SATFINITE, __NV_E4M3);
 }
 
-template <int DT>
+// Four elements at a time; VEC 1 takes them one by one (rows that are not
+// aligned to 16 bytes, rotations that end inside four elements).
+template <int VEC> struct Elems { float v[VEC]; };
+
+template <int VEC>
+__device__ __forceinline__ Elems<VEC> load_elems(const float* p) {
+  Elems<VEC> e;
+  if (VEC == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    e.v[0] = f.x;
+    e.v[1 % VEC] = f.y;
+    e.v[2 % VEC] = f.z;
+    e.v[3 % VEC] = f.w;
+  } else {
+    e.v[0] = *p;
+  }
+  return e;
+}
+template <int VEC>
+__device__ __forceinline__ void store_f32(float* p, const Elems<VEC>& e) {
+  if (VEC == 4)
+    *reinterpret_cast<float4*>(p) = make_float4(e.v[0], e.v[1 % VEC], e.v[2 % VEC], e.v[3 % VEC]);
+  else
+    *p = e.v[0];
+}
+template <int VEC, typename T>
+__device__ __forceinline__ void store_cache(T* p, const Elems<VEC>& e, float scale) {
+  struct alignas(VEC * sizeof(T)) Pack { T v[VEC]; } out;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) cache_put(&out.v[i], e.v[i], scale);
+  *reinterpret_cast<Pack*>(p) = out;
+}
+
+// An item is one load, or for a pair half a head apart two.
+template <int DT, int VEC>
 __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeArgs A) {
   using T = typename CacheType<DT>::T;
   __shared__ float2 cs[kMaxHeadDim / 2];
@@ -66,44 +102,74 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeArg
   const int h = A.rot / 2;
   for (int i = threadIdx.x; i < h; i += blockDim.x) cs[i] = rope_cos_sin(pos, A.inv_freq[i]);
   __syncthreads();
-  const int half = A.c.head_dim / 2;                 // pairs per head
-  const int heads = A.hq + 2 * A.c.kv_heads;
-  for (int it = blockIdx.y * blockDim.x + threadIdx.x; it < heads * half;
-       it += gridDim.y * blockDim.x) {
-    int j = it / half;
-    const int i = it - j * half;
-    const bool turn = j < A.hq + A.c.kv_heads && i < h;
-    const int e0 = turn && !A.interleaved ? i : 2 * i;
-    const int e1 = turn && !A.interleaved ? i + h : 2 * i + 1;
-    const float* src;
-    if (j < A.hq) {
-      src = A.q + t * A.q_ts + j * A.q_hs;
-    } else if (j < A.hq + A.c.kv_heads) {
-      src = A.k + t * A.k_ts + (j - A.hq) * A.k_hs;
-    } else {
-      src = A.v + t * A.v_ts + (j - A.hq - A.c.kv_heads) * A.v_hs;
+  // items of a head: of the rotated half (h / VEC), or of all rotated elements
+  // where pairs are adjacent, then of the rest
+  const int D = A.c.head_dim, hk = A.c.kv_heads;
+  const int nr = A.interleaved ? A.rot / VEC : h / VEC, ni = nr + (D - A.rot) / VEC, nv = D / VEC;
+  const int turned = (A.hq + hk) * ni, total = turned + hk * nv;
+  for (int it = blockIdx.y * blockDim.x + threadIdx.x; it < total; it += gridDim.y * blockDim.x) {
+    if (it >= turned) {                        // a value: copied
+      const int k = it - turned, j = k / nv, e = (k - j * nv) * VEC;
+      if (slot >= 0)
+        store_cache<VEC>(static_cast<T*>(A.c.v) + slot + (int64_t)j * A.c.head_stride + e,
+                         load_elems<VEC>(A.v + t * A.v_ts + j * A.v_hs + e), A.c.v_scale);
+      continue;
     }
-    float x0 = src[e0], x1 = src[e1];
-    if (turn) {
-      const float2 w = cs[i];
-      const float y0 = fmaf(x0, w.x, -x1 * w.y);
-      x1 = fmaf(x1, w.x, x0 * w.y);
-      x0 = y0;
+    const int j = it / ni, i = it - j * ni;
+    const bool is_q = j < A.hq;
+    const float* src = is_q ? A.q + t * A.q_ts + j * A.q_hs : A.k + t * A.k_ts + (j - A.hq) * A.k_hs;
+    const int e0 = i < nr ? i * VEC : A.rot + (i - nr) * VEC;
+    const bool two = i < nr && (!A.interleaved || VEC == 1);
+    const int e1 = A.interleaved ? e0 + 1 : e0 + h;   // partner, in another load
+    Elems<VEC> a, b;
+    if (VEC == 1 && A.interleaved && i < nr) {
+      if (i & 1) continue;                     // its pair's first element does both
     }
-    if (j < A.hq) {
+    a = load_elems<VEC>(src + e0);
+    if (two) {
+      b = load_elems<VEC>(src + e1);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float2 w = cs[A.interleaved ? e0 / 2 : e0 + k];
+        const float x0 = a.v[k], x1 = b.v[k];
+        a.v[k] = fmaf(x0, w.x, -x1 * w.y);
+        b.v[k] = fmaf(x1, w.x, x0 * w.y);
+      }
+    } else if (i < nr) {
+#pragma unroll
+      for (int k = 0; k + 1 < VEC; k += 2) {
+        const float2 w = cs[(e0 + k) / 2];
+        const float x0 = a.v[k], x1 = a.v[k + 1];
+        a.v[k] = fmaf(x0, w.x, -x1 * w.y);
+        a.v[k + 1] = fmaf(x1, w.x, x0 * w.y);
+      }
+    }
+    if (is_q) {
       float* dst = A.q_out + t * A.qo_ts + j * A.qo_hs;
-      dst[e0] = x0;
-      dst[e1] = x1;
+      store_f32<VEC>(dst + e0, a);
+      if (two) store_f32<VEC>(dst + e1, b);
     } else if (slot >= 0) {
-      j -= A.hq;
-      const bool is_k = j < A.c.kv_heads;
-      T* dst = static_cast<T*>(is_k ? A.c.k : A.c.v) + slot +
-               (int64_t)(is_k ? j : j - A.c.kv_heads) * A.c.head_stride;
-      const float scale = is_k ? A.c.k_scale : A.c.v_scale;
-      cache_put(dst + e0, x0, scale);
-      cache_put(dst + e1, x1, scale);
+      T* dst = static_cast<T*>(A.c.k) + slot + (int64_t)(j - A.hq) * A.c.head_stride;
+      store_cache<VEC>(dst + e0, a, A.c.k_scale);
+      if (two) store_cache<VEC>(dst + e1, b, A.c.k_scale);
     }
   }
+}
+
+template <int DT>
+static int launch_rope(const RopeArgs& a, int T, cudaStream_t s) {
+  auto aligned = [](const void* p, int64_t ts, int64_t hs) {
+    return (uintptr_t)p % 16 == 0 && ts % 4 == 0 && hs % 4 == 0;
+  };
+  const bool vec = a.rot % (a.interleaved ? 4 : 8) == 0 && aligned(a.k, a.k_ts, a.k_hs) &&
+                   aligned(a.v, a.v_ts, a.v_hs) &&
+                   (a.hq == 0 || (aligned(a.q, a.q_ts, a.q_hs) && aligned(a.q_out, a.qo_ts, a.qo_hs)));
+  // a token's heads over several CTAs while there are fewer tokens than SMs
+  const int items = (a.hq + 2 * a.c.kv_heads) * a.c.head_dim / (vec ? 4 : 1);
+  const int parts = std::max(1, std::min(sm_count() / T, items / kRopeThreads));
+  auto kern = vec ? rope_append_kernel<DT, 4> : rope_append_kernel<DT, 1>;
+  MOE_CUDA(launch_pdl(kern, dim3((unsigned)T, (unsigned)parts), dim3(kRopeThreads), 0, s, a));
+  return MOE_OK;
 }
 
 }  // namespace moe
@@ -132,13 +198,11 @@ int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_
                      seq_ids, inv_freq, status, q_heads, rot, interleaved};
   moe::normalise_strides(a.c);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  dim3 grid((unsigned)T, 1);
   {
     ::moe::ProfScope _prof(MOE_K_ROPE_APPEND, s);
-    auto kern = cache->dtype == MOE_CACHE_F16    ? moe::rope_append_kernel<MOE_CACHE_F16>
-                : cache->dtype == MOE_CACHE_BF16 ? moe::rope_append_kernel<MOE_CACHE_BF16>
-                                                 : moe::rope_append_kernel<MOE_CACHE_E4M3>;
-    MOE_CUDA(moe::launch_pdl(kern, grid, dim3(moe::kRopeThreads), 0, s, a));
+    MOE_CHECK(cache->dtype == MOE_CACHE_F16    ? moe::launch_rope<MOE_CACHE_F16>(a, T, s)
+              : cache->dtype == MOE_CACHE_BF16 ? moe::launch_rope<MOE_CACHE_BF16>(a, T, s)
+                                               : moe::launch_rope<MOE_CACHE_E4M3>(a, T, s));
   }
   return moe::check_launch("rope_append");
 }
