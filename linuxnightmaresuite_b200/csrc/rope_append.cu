@@ -27,7 +27,9 @@ struct RopeArgs {
   const double* inv_freq;
   int* status;
   int hq, rot, interleaved;
-};
+  int nr, ni, nv;                      // items: rotated and all of a turned head, of a value head
+  uint32_t mi, mv;                     // 2^32 / ni, 2^32 / nv rounded up: it / ni = hi(it * mi),
+};                                     // exact for it < 2^24 since ni, nv <= 256
 
 __device__ __forceinline__ float2 rope_cos_sin(int pos, double freq) {
   const double kTwoPi = 6.283185307179586476925;
@@ -86,36 +88,42 @@ template <int DT, int VEC>
 __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeArgs A) {
   using T = typename CacheType<DT>::T;
   __shared__ float2 cs[kMaxHeadDim / 2];
+  __shared__ int64_t sh_slot;
   pdl_trigger();
   pdl_wait();
   const int t = blockIdx.x;
   const int pos = A.positions[t];
   if (pos < 0) return;
-  const int seq = A.seq_ids ? A.seq_ids[t] : t;
-  int64_t slot = -1;   // the token's slot in both caches, -1: none
-  if (seq >= 0 && seq < A.c.seqs && pos / A.c.page_size < A.c.table_width) {
-    const int page = A.c.block_table[(int64_t)seq * A.c.table_stride + pos / A.c.page_size];
-    if (page >= 0 && page < A.c.pages)
-      slot = (int64_t)page * A.c.page_stride + (int64_t)(pos % A.c.page_size) * A.c.token_stride;
+  if (threadIdx.x == blockDim.x - 1) {           // the token's slot in both caches, -1: none
+    const int seq = A.seq_ids ? A.seq_ids[t] : t, n = pos / A.c.page_size;
+    int64_t slot = -1;
+    if (seq >= 0 && seq < A.c.seqs && n < A.c.table_width) {
+      const int page = A.c.block_table[(int64_t)seq * A.c.table_stride + n];
+      if (page >= 0 && page < A.c.pages)
+        slot = (int64_t)page * A.c.page_stride +
+               (int64_t)(pos - n * A.c.page_size) * A.c.token_stride;
+    }
+    if (slot < 0) set_status(A.status, MOE_STATUS_BAD_PAGE);
+    sh_slot = slot;
   }
-  if (slot < 0 && threadIdx.x == 0) set_status(A.status, MOE_STATUS_BAD_PAGE);
   const int h = A.rot / 2;
   for (int i = threadIdx.x; i < h; i += blockDim.x) cs[i] = rope_cos_sin(pos, A.inv_freq[i]);
   __syncthreads();
+  const int64_t slot = sh_slot;
   // items of a head: of the rotated half (h / VEC), or of all rotated elements
   // where pairs are adjacent, then of the rest
-  const int D = A.c.head_dim, hk = A.c.kv_heads;
-  const int nr = A.interleaved ? A.rot / VEC : h / VEC, ni = nr + (D - A.rot) / VEC, nv = D / VEC;
+  const int hk = A.c.kv_heads, nr = A.nr, ni = A.ni, nv = A.nv;
   const int turned = (A.hq + hk) * ni, total = turned + hk * nv;
   for (int it = blockIdx.y * blockDim.x + threadIdx.x; it < total; it += gridDim.y * blockDim.x) {
     if (it >= turned) {                        // a value: copied
-      const int k = it - turned, j = k / nv, e = (k - j * nv) * VEC;
+      const int k = it - turned, j = nv == 1 ? k : (int)__umulhi((uint32_t)k, A.mv);
+      const int e = (k - j * nv) * VEC;
       if (slot >= 0)
         store_cache<VEC>(static_cast<T*>(A.c.v) + slot + (int64_t)j * A.c.head_stride + e,
                          load_elems<VEC>(A.v + t * A.v_ts + j * A.v_hs + e), A.c.v_scale);
       continue;
     }
-    const int j = it / ni, i = it - j * ni;
+    const int j = ni == 1 ? it : (int)__umulhi((uint32_t)it, A.mi), i = it - j * ni;
     const bool is_q = j < A.hq;
     const float* src = is_q ? A.q + t * A.q_ts + j * A.q_hs : A.k + t * A.k_ts + (j - A.hq) * A.k_hs;
     const int e0 = i < nr ? i * VEC : A.rot + (i - nr) * VEC;
@@ -157,13 +165,19 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeArg
 }
 
 template <int DT>
-static int launch_rope(const RopeArgs& a, int T, cudaStream_t s) {
+static int launch_rope(RopeArgs& a, int T, cudaStream_t s) {
   auto aligned = [](const void* p, int64_t ts, int64_t hs) {
     return (uintptr_t)p % 16 == 0 && ts % 4 == 0 && hs % 4 == 0;
   };
   const bool vec = a.rot % (a.interleaved ? 4 : 8) == 0 && aligned(a.k, a.k_ts, a.k_hs) &&
                    aligned(a.v, a.v_ts, a.v_hs) &&
                    (a.hq == 0 || (aligned(a.q, a.q_ts, a.q_hs) && aligned(a.q_out, a.qo_ts, a.qo_hs)));
+  const int V = vec ? 4 : 1;
+  a.nr = a.interleaved ? a.rot / V : a.rot / 2 / V;
+  a.ni = a.nr + (a.c.head_dim - a.rot) / V;
+  a.nv = a.c.head_dim / V;
+  a.mi = 0xffffffffu / (uint32_t)a.ni + 1;
+  a.mv = 0xffffffffu / (uint32_t)a.nv + 1;
   // a token's heads over several CTAs while there are fewer tokens than SMs
   const int items = (a.hq + 2 * a.c.kv_heads) * a.c.head_dim / (vec ? 4 : 1);
   const int parts = std::max(1, std::min(sm_count() / T, items / kRopeThreads));
@@ -186,6 +200,7 @@ int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_
   MOE_REQUIRE(cache, MOE_ERR_INVALID, "null cache");
   MOE_CHECK(moe::check_cache(*cache));
   MOE_REQUIRE(T >= 0 && q_heads >= 0, MOE_ERR_INVALID, "negative size");
+  MOE_REQUIRE(q_heads <= 32767 && cache->kv_heads <= 16383, MOE_ERR_UNSUPPORTED, "too many heads");
   MOE_REQUIRE(rot >= 0 && rot % 2 == 0 && rot <= cache->head_dim, MOE_ERR_INVALID,
               "rot %d: an even number up to head_dim %d is needed", rot, cache->head_dim);
   if (T == 0) return MOE_OK;
