@@ -46,11 +46,11 @@
 namespace moe {
 
 constexpr int kAttHeads = 8;          // query heads of a unit at most
-constexpr int kAttMaxCtasPerSm = 2;
+constexpr int kAttCtasPerSm = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kAttParts = 320;        // CTAs that one unit may be split over
-constexpr float kPScale = 128.f;      // probabilities enter the products times this
+constexpr float kPShift = 7.f;        // probabilities enter sums and products times 2^7
 
 struct AttArgs {
   moe_paged_cache c;
@@ -191,32 +191,34 @@ template <bool BF> struct AFrag {
 // ---------------------------------------------------------------------------
 // shapes: DP = head_dim rounded up to 64, 128 or 256.  A ring slot holds the
 // keys or the values of a tile; an odd number of slots makes the slot freed
-// by keys the next one that keys go to.
+// by keys the next one that keys go to.  At 256 columns two warps share a tile,
+// half of the columns each, and add their halves of the scores: the registers
+// of one warp do not hold the accumulators of 256 columns, and without them
+// every tile would be folded.
 // ---------------------------------------------------------------------------
 constexpr int kLine = 128;             // bytes of a row in one box
 template <int DT, int DP> struct AttCfg {
   static constexpr bool kBf = DT == MOE_CACHE_BF16;
   static constexpr int kElem = DT == MOE_CACHE_E4M3 ? 1 : 2;
-  static constexpr int kRow = DP * kElem < kLine ? kLine : DP * kElem;   // bytes in the ring
+  static constexpr int kSplit = DP > 128 ? 2 : 1;           // warps of a tile
+  static constexpr int kDh = DP / kSplit;                   // columns of a warp
+  static constexpr int kRow = kDh * kElem < kLine ? kLine : kDh * kElem;   // bytes in the ring
   static constexpr int kWarps = 4;
-  static constexpr int kKeys = kRow <= 128 ? 32 : 16;       // keys of a warp's tile
+  static constexpr int kTiles = kWarps / kSplit;            // tiles of a round
+  static constexpr int kKeys = kRow <= 128 ? 32 : 16;       // keys of a tile
   static constexpr int kSlot = kKeys * kRow;
   static constexpr int kSlots = 5;
-  static constexpr int kRound = kWarps * kKeys;
+  static constexpr int kRound = kTiles * kKeys;
   static constexpr int kRing = kWarps * kSlots * kSlot;
   static constexpr int kMergeRow = DP + 8;                  // floats
-  // one row per warp and head; when a unit's parts are joined first a weight per
+  // one row per tile and head; when a unit's parts are joined first a weight per
   // part and head, then four floats per thread and head
   static constexpr int kMerge =
-      4 * kAttHeads * (kWarps * kMergeRow > 4 * 32 * kWarps ? kWarps * kMergeRow : 4 * 32 * kWarps);
+      4 * kAttHeads * (kTiles * kMergeRow > 4 * 32 * kWarps ? kTiles * kMergeRow : 4 * 32 * kWarps);
   static_assert(kMerge >= kAttParts * kAttHeads * 4, "weights of the parts");
   static constexpr int kQ = DP / 16 * AFrag<kBf>::kBytes;
-  static constexpr int kSmem = kRing + kMerge + kQ;
-  static constexpr int kCtasPerSm = kSmem <= 112 * 1024 ? 2 : 1;
-  // Whether the products p v stay in MMA accumulators for kFold tiles (four
-  // k16 steps) before they are added up; at 256 columns the registers do not
-  // hold both, and every tile is added up.
-  static constexpr bool kHold = DP <= 128;
+  static constexpr int kX = kSplit > 1 ? kWarps * 32 * (kKeys / 4) * 4 : 0;   // halves of scores
+  static constexpr int kSmem = kRing + kMerge + kQ + kX;
   static constexpr int kFold = 64 / kKeys;
 };
 
@@ -248,13 +250,13 @@ struct Cursor {
 };
 
 template <int DT, int DP>
-__global__ void __launch_bounds__(AttCfg<DT, DP>::kWarps * 32, AttCfg<DT, DP>::kCtasPerSm)
+__global__ void __launch_bounds__(AttCfg<DT, DP>::kWarps * 32, kAttCtasPerSm)
 attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                  const AttArgs A) {
   using Cfg = AttCfg<DT, DP>;
   constexpr bool BF = Cfg::kBf;
   constexpr int NW = Cfg::kWarps, NT = NW * 32, KEYS = Cfg::kKeys, NS = Cfg::kSlots;
-  constexpr int LINE = kLine, RK = Cfg::kRound;
+  constexpr int LINE = kLine, RK = Cfg::kRound, SP = Cfg::kSplit, DH = Cfg::kDh, NG = Cfg::kTiles;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ AttShared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -351,7 +353,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   C.r0 = max(0, -C.at);
   C.r1 = min(C.R, end - C.at);
   // tiles of this warp in a piece: first key, end of the keys, number
-  auto tile0 = [&](const Cursor& c) { return c.from + c.r0 * RK + warp * KEYS; };
+  auto tile0 = [&](const Cursor& c) { return c.from + c.r0 * RK + warp / SP * KEYS; };
   auto keys_end = [&](const Cursor& c) { return min(c.len, c.from + c.r1 * RK); };
   auto tiles = [&](const Cursor& c) {
     const int n = keys_end(c) - tile0(c);
@@ -361,7 +363,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   // ---- loads: a cursor of its own that runs ahead of the arithmetic, across
   // the ends of units
   const uint32_t ring_a = smem_u32(smem) + warp * NS * Cfg::kSlot;
-  constexpr int BLOCKS = DP * Cfg::kElem < LINE ? 1 : DP * Cfg::kElem / LINE;
+  constexpr int BLOCKS = Cfg::kRow / LINE;
   const int box = 1 << A.box_shift, boxes = KEYS >> A.box_shift, ps = A.c.page_size;
   const int step_pages = RK / ps, step_slots = RK - step_pages * ps;   // from tile to tile
   Cursor W = C;                                  // of the loads
@@ -400,7 +402,8 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       const uint32_t dst = ring_a + lslot * Cfg::kSlot + (lane << A.box_shift) * LINE;
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b)
-        tma_load_3d(dst + b * KEYS * LINE, map, b * (LINE / Cfg::kElem), row, pslot, bar);
+        tma_load_3d(dst + b * KEYS * LINE, map, warp % SP * DH + b * (LINE / Cfg::kElem), row, pslot,
+                    bar);
     }
     lslot = lslot + 1 == NS ? 0 : lslot + 1;
   };
@@ -471,6 +474,8 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   constexpr int QK = DP / 16 / NW;
   uint8_t* const qs = smem + Cfg::kRing + Cfg::kMerge;
   float* const mo = reinterpret_cast<float*>(smem + Cfg::kRing);
+  const uint8_t* const qw = qs + warp % SP * (DH / 16) * AFrag<BF>::kBytes;   // this warp's columns
+  float4* const xs = reinterpret_cast<float4*>(smem + Cfg::kRing + Cfg::kMerge + Cfg::kQ);
   float qn[QK][4];
   auto first_head = [&](const Cursor& c) { return c.head * G + c.group * kAttHeads; };
   auto heads = [&](const Cursor& c) { return min(kAttHeads, G - c.group * kAttHeads); };
@@ -506,11 +511,16 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     const int e1 = e / 2, e2 = e - e1;
     const float f1 = __uint_as_float((uint32_t)(127 + e1) << 23);
     const float f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
-    if (warp == 0 && t == 0) sh.qscale[g] = ldexpf(A.scale * A.c.k_scale, -e);
+    // a negative scale turns q; one that vanishes stays above zero, so that it
+    // leaves the minus infinity of a key that is not seen what it is
+    const float sign = A.scale < 0.f ? -1.f : 1.f;
+    if (warp == 0 && t == 0)
+      sh.qscale[g] = fmaxf(ldexpf(fabsf(A.scale) * A.c.k_scale, -e), 1e-30f);
 #pragma unroll
     for (int i = 0; i < QK; ++i) {
       AFrag<BF> f;
-      f.set(qn[i][0] * f1 * f2, qn[i][1] * f1 * f2, qn[i][2] * f1 * f2, qn[i][3] * f1 * f2);
+      const float f0 = f1 * sign;
+      f.set(qn[i][0] * f0 * f2, qn[i][1] * f0 * f2, qn[i][2] * f0 * f2, qn[i][3] * f0 * f2);
       f.store(qs + (warp + i * NW) * AFrag<BF>::kBytes, lane);
     }
   };
@@ -546,33 +556,23 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     const int ntile = tiles(C);
 
     const float qscale = sh.qscale[g];           // score = product * qscale
-    const float x2 = qscale * kLog2e;
-    float o[DP / 8][2];                          // head g, two columns of each 8-wide block
-    float acc[Cfg::kHold ? DP / 8 : 1][4];
+    const float x2 = A.cap > 0.f ? 1.f : qscale * kLog2e;
+    float o[DH / 8][2];                          // head g, two columns of each 8-wide block
+    float acc[DH / 8][4];
 #pragma unroll
-    for (int c = 0; c < DP / 8; ++c) o[c][0] = o[c][1] = 0.f;
-#pragma unroll
-    for (int c = 0; c < (Cfg::kHold ? DP / 8 : 1); ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[c][j] = 0.f;
+    for (int c = 0; c < DH / 8; ++c) {
+      o[c][0] = o[c][1] = 0.f;
+      acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
+    }
     // m: reference of the exponentials, 2^8 below the maximum at most; l: sum
     // over this lane's keys
     float m = -INFINITY, l = 0.f;
     auto fold = [&](float f) {                   // o = (o + acc) * f
-      if (Cfg::kHold) {
 #pragma unroll
-        for (int c = 0; c < DP / 8; ++c) {
-          o[c][0] = (o[c][0] + (acc[c][0] + acc[c][2])) * f;
-          o[c][1] = (o[c][1] + (acc[c][1] + acc[c][3])) * f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[c][j] = 0.f;
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < DP / 8; ++c) {
-          o[c][0] *= f;
-          o[c][1] *= f;
-        }
+      for (int c = 0; c < DH / 8; ++c) {
+        o[c][0] = (o[c][0] + (acc[c][0] + acc[c][2])) * f;
+        o[c][1] = (o[c][1] + (acc[c][1] + acc[c][3])) * f;
+        acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
       }
     };
 
@@ -586,13 +586,13 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       // head_dim are zeros in the ring and in q
       float x[KEYS / 8][2];
 #pragma unroll
-      for (int k4 = 0; k4 < DP / 64; ++k4) {
+      for (int k4 = 0; k4 < DH / 64; ++k4) {
         float a[KEYS / 8][4];
 #pragma unroll
         for (int kk = 4 * k4; kk < 4 * k4 + 4; kk += 3 - Cfg::kElem) {
           AFrag<BF> q0, q1;
-          q0.load(qs + kk * AFrag<BF>::kBytes, lane);
-          if (Cfg::kElem == 1) q1.load(qs + (kk + 1) * AFrag<BF>::kBytes, lane);
+          q0.load(qw + kk * AFrag<BF>::kBytes, lane);
+          if (Cfg::kElem == 1) q1.load(qw + (kk + 1) * AFrag<BF>::kBytes, lane);
 #pragma unroll
           for (int kb = 0; kb < KEYS / 16; ++kb) {
             uint32_t b[4];
@@ -628,16 +628,30 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
           x[b][1] = (k4 ? x[b][1] : 0.f) + (a[b][1] + a[b][3]);
         }
       }
+      if (SP > 1) {
+        // the other half of the columns: both warps get the same sums
+        constexpr int V = KEYS / 16;
+        float4* mine = xs + warp * 32 * V + lane;
+        const float4* other = xs + (warp ^ 1) * 32 * V + lane;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          mine[v * 32] = make_float4(x[2 * v][0], x[2 * v][1], x[2 * v + 1][0], x[2 * v + 1][1]);
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + warp / SP) : "memory");
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float4 y = other[v * 32];
+          x[2 * v][0] += y.x;
+          x[2 * v][1] += y.y;
+          x[2 * v + 1][0] += y.z;
+          x[2 * v + 1][1] += y.w;
+        }
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + warp / SP) : "memory");
+      }
       if (A.cap > 0.f) {
 #pragma unroll
         for (int b = 0; b < KEYS / 8; ++b)
 #pragma unroll
           for (int h = 0; h < 2; ++h) x[b][h] = A.cap * tanhf(x[b][h] * qscale / A.cap) * kLog2e;
-      } else {
-#pragma unroll
-        for (int b = 0; b < KEYS / 8; ++b)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) x[b][h] *= x2;
       }
       if (seen != 0xffffffffu) {                 // lanes past KEYS repeat the first ones
 #pragma unroll
@@ -652,7 +666,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 #pragma unroll
       for (int b = 0; b < KEYS / 8; ++b) mx = fmaxf(mx, fmaxf(x[b][0], x[b][1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * x2;
       if (__any_sync(0xffffffffu, mx > m + 8.f)) {
         const float to = mx > m + 8.f ? mx : m;
         const float f = to == -INFINITY ? 1.f : ex2(m - to);
@@ -660,19 +674,18 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         l *= f;
         m = to;
       }
-      const float ms = m == -INFINITY ? 0.f : m;
+      const float shift = kPShift - (m == -INFINITY ? 0.f : m);
 #pragma unroll
       for (int b = 0; b < KEYS / 8; ++b)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          x[b][h] = ex2(x[b][h] - ms);
+          x[b][h] = ex2(fmaf(x[b][h], x2, shift));
           l += x[b][h];
         }
       AFrag<BF> pf[KEYS / 16];
 #pragma unroll
       for (int kb = 0; kb < KEYS / 16; ++kb)
-        pf[kb].set(x[2 * kb][0] * kPScale, x[2 * kb][1] * kPScale, x[2 * kb + 1][0] * kPScale,
-                   x[2 * kb + 1][1] * kPScale);
+        pf[kb].set(x[2 * kb][0], x[2 * kb][1], x[2 * kb + 1][0], x[2 * kb + 1][1]);
 
       const uint32_t va = wait_slot();
       issue_values();
@@ -688,11 +701,11 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 
       // p v.  e4m3: a 16-byte chunk holds 16 columns; transposed in pairs of
       // bytes, a register has columns (2g, 2g + 1) of two keys, which become
-      // the B registers of the even and of the odd columns
+      // the B registers of the even and of the odd columns.  The accumulators
+      // take kFold tiles (four k16 steps) before they are added up
       constexpr int CPB = Cfg::kElem == 2 ? 2 : 4;      // 8-wide blocks of two chunks
 #pragma unroll
-      for (int c = 0; c < DP / 8; c += CPB) {
-        float tmp[CPB][4];
+      for (int c = 0; c < DH / 8; c += CPB) {
 #pragma unroll
         for (int kb = 0; kb < KEYS / 16; ++kb) {
           uint32_t b[4];
@@ -701,53 +714,32 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             if (Cfg::kElem == 2) {
-              if (Cfg::kHold)
-                pf[kb].mul(acc[(c + j) * Cfg::kHold], b[2 * j], b[2 * j + 1]);
-              else if (kb == 0)
-                pf[kb].template mul<true>(tmp[j], b[2 * j], b[2 * j + 1]);
-              else
-                pf[kb].mul(tmp[j], b[2 * j], b[2 * j + 1]);
+              pf[kb].mul(acc[c + j], b[2 * j], b[2 * j + 1]);
             } else {
-              uint32_t k0, k1, k8, k9;
-              e4m3x4_f16x2(b[2 * j], k0, k1);
-              e4m3x4_f16x2(b[2 * j + 1], k8, k9);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t b0 = prmt(k0, k1, h ? 0x7632u : 0x5410u);
-                const uint32_t b1 = prmt(k8, k9, h ? 0x7632u : 0x5410u);
-                if (Cfg::kHold)
-                  pf[kb].mul(acc[(c + 2 * j + h) * Cfg::kHold], b0, b1);
-                else if (kb == 0)
-                  pf[kb].template mul<true>(tmp[(2 * j + h) % CPB], b0, b1);
-                else
-                  pf[kb].mul(tmp[(2 * j + h) % CPB], b0, b1);
-              }
+              uint32_t e0, o0, e1, o1;           // even and odd columns, keys 0-7 and 8-15
+              e4m3x4_f16x2(prmt(b[2 * j], 0u, 0x3120u), e0, o0);
+              e4m3x4_f16x2(prmt(b[2 * j + 1], 0u, 0x3120u), e1, o1);
+              pf[kb].mul(acc[c + 2 * j], e0, e1);
+              pf[kb].mul(acc[c + 2 * j + 1], o0, o1);
             }
           }
         }
-        if (!Cfg::kHold) {
-#pragma unroll
-          for (int j = 0; j < CPB; ++j) {
-            o[c + j][0] += tmp[j][0] + tmp[j][2];
-            o[c + j][1] += tmp[j][1] + tmp[j][3];
-          }
-        }
       }
-      if (Cfg::kHold && i % Cfg::kFold == Cfg::kFold - 1) fold(1.f);
+      if (i % Cfg::kFold == Cfg::kFold - 1) fold(1.f);
     }
-    if (Cfg::kHold) fold(1.f);
+    fold(1.f);
 
     // ---- the warps' parts meet in shared memory
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (t == 0) {
-      sh.m[warp][g] = m;
-      sh.l[warp][g] = l;
+    if (t == 0 && warp % SP == 0) {
+      sh.m[warp / SP][g] = m;
+      sh.l[warp / SP][g] = l;
     }
     {
-      float* row = mo + (warp * kAttHeads + g) * Cfg::kMergeRow;
+      float* row = mo + (warp / SP * kAttHeads + g) * Cfg::kMergeRow + warp % SP * DH;
 #pragma unroll
-      for (int c = 0; c < DP / 8; ++c) {
+      for (int c = 0; c < DH / 8; ++c) {
         if (Cfg::kElem == 2) {
           *reinterpret_cast<float2*>(row + 8 * c + 2 * t) = make_float2(o[c][0], o[c][1]);
         } else {                                 // block 2c: even columns 4t, 4t + 2; 2c + 1: odd
@@ -762,23 +754,23 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     const int my_slot = 2 * blockIdx.x + (C.r0 == 0 ? 1 : 0);
     const int nh = heads(C);
     const int64_t row0 = (int64_t)C.seq * A.hq + first_head(C);
-    const float unit = A.c.v_scale / kPScale;
+    const float unit = A.c.v_scale;
     for (int h = warp; h < nh; h += NW) {
       float M = sh.m[0][h];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) M = fmaxf(M, sh.m[w][h]);
+      for (int w = 1; w < NG; ++w) M = fmaxf(M, sh.m[w][h]);
       const float ms = M == -INFINITY ? 0.f : M;
-      float L = 0.f, f[NW];
+      float L = 0.f, f[NG];
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
+      for (int w = 0; w < NG; ++w) {
         f[w] = ex2(sh.m[w][h] - ms);
         L = fmaf(sh.l[w][h], f[w], L);
       }
       if (whole) {
         const float norm = L == 0.f ? 0.f : unit / L;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) f[w] *= norm;
-        if (lane == 0 && A.lse) A.lse[row0 + h] = (M + log2f(L)) * kLn2;
+        for (int w = 0; w < NG; ++w) f[w] *= norm;
+        if (lane == 0 && A.lse) A.lse[row0 + h] = (M + (log2f(L) - kPShift)) * kLn2;
       } else if (lane == 0) {
         A.part_ml[my_slot * kAttHeads + h] = make_float2(M, L);
       }
@@ -786,7 +778,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       for (int c = lane; c < D; c += 32) {
         float y = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w)
+        for (int w = 0; w < NG; ++w)
           y = fmaf(mo[(w * kAttHeads + h) * Cfg::kMergeRow + c], f[w], y);
         to[c] = y;
       }
@@ -833,7 +825,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 #pragma unroll
           for (int k = 0; k < kAttParts / 32; ++k)
             if (lane + 32 * k < n) mo[(lane + 32 * k) * kAttHeads + h] = v[k].x * norm;
-          if (lane == 0 && A.lse) A.lse[row0 + h] = (M + log2f(L)) * kLn2;
+          if (lane == 0 && A.lse) A.lse[row0 + h] = (M + (log2f(L) - kPShift)) * kLn2;
         }
         __syncthreads();
         // thread: four columns of every PL-th part, all heads
@@ -890,7 +882,7 @@ inline int padded_head_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; 
 
 static int attention_workspace(int head_dim, AttArgs* a, void* ws, size_t* bytes) {
   Carve cv = {static_cast<uint8_t*>(ws), 0, 0};
-  const int slots = kAttMaxCtasPerSm * sm_count();
+  const int slots = kAttCtasPerSm * sm_count();
   cv.take<uint8_t>(256);
   int* arrivals = cv.take<int>(slots);
   float2* ml = cv.take<float2>((size_t)2 * slots * kAttHeads);
@@ -942,7 +934,6 @@ template <int DT, int DP>
 static int launch_attention(AttArgs& a, int max_len, cudaStream_t s) {
   using Cfg = AttCfg<DT, DP>;
   static_assert(Cfg::kSlots % 2 == 1 && Cfg::kSlots <= 5 && Cfg::kWarps == 4, "");
-  static_assert(Cfg::kCtasPerSm <= kAttMaxCtasPerSm, "");
   static std::atomic<uint64_t> ready{0};
   auto kern = attention_kernel<DT, DP>;
   int dev = 0;
@@ -959,7 +950,7 @@ static int launch_attention(AttArgs& a, int max_len, cudaStream_t s) {
   const int64_t keys = a.window > 0 ? std::min(a.window, max_len) : max_len;
   const int64_t cost =
       units * (std::max<int64_t>(1, (keys + Cfg::kRound - 1) / Cfg::kRound) + kUnitCost);
-  const int grid = (int)std::min<int64_t>(cost, (int64_t)Cfg::kCtasPerSm * sm_count());
+  const int grid = (int)std::min<int64_t>(cost, (int64_t)kAttCtasPerSm * sm_count());
   // a CTA counts its costs, and a sequence's, in 32 bits
   const int64_t most = (int64_t)a.c.table_width * a.c.page_size / Cfg::kRound + 2 + kUnitCost;
   MOE_REQUIRE(units / a.c.seqs * most < (1ll << 30) && units * most / grid < (1ll << 30),

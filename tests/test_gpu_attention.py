@@ -178,7 +178,8 @@ def test_attention(dtype, layout, hq, hkv, d, page):
 
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
 @pytest.mark.parametrize("window,cap,scale", [(1, 0.0, None), (16, 0.0, 0.3), (100, 30.0, None),
-                                              (5000, 5.0, 1.0), (0, 50.0, 0.0)])
+                                              (5000, 5.0, 1.0), (0, 50.0, 0.0), (0, 0.0, -0.2),
+                                              (0, 0.0, 0.0), (64, 8.0, -1.0)])
 def test_attention_window_cap_scale(dtype, window, cap, scale):
     hq, hkv, d, page = 6, 2, 128, 16
     lens = [1, 0, 99, 100, 101, 400, 1500]
