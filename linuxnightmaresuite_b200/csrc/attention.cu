@@ -33,7 +33,7 @@
 // in one thread, are added.  Probabilities are split the same way (times 2^14
 // first, which keeps the lo part of small ones above fp16's range end).  The
 // tensor core truncates where it adds, so no accumulator takes more than four
-// k16 steps; from there on sums are f32 adds.
+// (scores) or eight (values) k16 steps; from there on sums are f32 adds.
 #include <math.h>
 
 #include <algorithm>
@@ -153,26 +153,40 @@ __device__ __forceinline__ void e4m3x4_f16x2(uint32_t v, uint32_t& lo, uint32_t&
       : "r"(v));
 }
 
-// A operand of one k16 step: one 16-row tile of {hi rows, lo rows}; bf16 has a
-// second tile {third part, zero} that goes into the same accumulators.
-template <bool BF> struct AFrag {
+// A operand of one k16 step: one 16-row tile of {hi rows, lo rows}.  bf16 has a
+// second tile {third part, zero} that goes into the same accumulators, unless a
+// unit has at most four heads (PACK): then rows 4 to 7 hold the third parts, and
+// lanes g and g + 4 add up their results.
+template <bool BF, bool PACK> struct AFrag {
   static constexpr int kParts = BF ? 3 : 2;
-  uint32_t lo[kParts], hi[kParts];    // k columns 2t, 2t+1 and 2t+8, 2t+9
-  __device__ __forceinline__ void set(float x0, float x1, float x2, float x3) {
-    split2<BF, kParts>(x0, x1, lo);
-    split2<BF, kParts>(x2, x3, hi);
+  static constexpr bool kTwo = BF && !PACK;      // a second tile
+  static constexpr int kRegs = kTwo ? 3 : 2;
+  uint32_t lo[kRegs], hi[kRegs];      // k columns 2t, 2t+1 and 2t+8, 2t+9
+  __device__ __forceinline__ static void parts(float x, float y, int g, uint32_t (&r)[kRegs]) {
+    if (BF && PACK) {
+      uint32_t all[3];
+      split2<true, 3>(x, y, all);
+      r[0] = g < 4 ? all[0] : all[2];
+      r[1] = g < 4 ? all[1] : 0u;
+    } else {
+      split2<BF, kRegs>(x, y, r);
+    }
+  }
+  __device__ __forceinline__ void set(float x0, float x1, float x2, float x3, int g) {
+    parts(x0, x1, g, lo);
+    parts(x2, x3, g, hi);
   }
   template <bool FIRST = false>
   __device__ __forceinline__ void mul(float (&d)[4], uint32_t b0, uint32_t b1) const {
     mma_acc<BF, FIRST>(d, lo[0], lo[1], hi[0], hi[1], b0, b1);
-    if (BF) mma_acc<BF, false>(d, lo[kParts - 1], 0u, hi[kParts - 1], 0u, b0, b1);
+    if (kTwo) mma_acc<BF, false>(d, lo[kRegs - 1], 0u, hi[kRegs - 1], 0u, b0, b1);
   }
-  // in shared memory: 16 bytes per lane, then for bf16 8 more
-  static constexpr int kBytes = 32 * 8 * kParts;
+  // in shared memory: 16 bytes per lane, then for a second tile 8 more
+  static constexpr int kBytes = 32 * 8 * kRegs;
   __device__ __forceinline__ void store(uint8_t* at, int lane) const {
     *reinterpret_cast<uint4*>(at + lane * 16) = make_uint4(lo[0], lo[1], hi[0], hi[1]);
-    if (BF) *reinterpret_cast<uint2*>(at + 512 + lane * 8) =
-        make_uint2(lo[kParts - 1], hi[kParts - 1]);
+    if (kTwo) *reinterpret_cast<uint2*>(at + 512 + lane * 8) =
+        make_uint2(lo[kRegs - 1], hi[kRegs - 1]);
   }
   __device__ __forceinline__ void load(const uint8_t* at, int lane) {
     const uint4 v = *reinterpret_cast<const uint4*>(at + lane * 16);
@@ -180,10 +194,10 @@ template <bool BF> struct AFrag {
     lo[1] = v.y;
     hi[0] = v.z;
     hi[1] = v.w;
-    if (BF) {
+    if (kTwo) {
       const uint2 w = *reinterpret_cast<const uint2*>(at + 512 + lane * 8);
-      lo[kParts - 1] = w.x;
-      hi[kParts - 1] = w.y;
+      lo[kRegs - 1] = w.x;
+      hi[kRegs - 1] = w.y;
     }
   }
 };
@@ -197,8 +211,9 @@ template <bool BF> struct AFrag {
 // every tile would be folded.
 // ---------------------------------------------------------------------------
 constexpr int kLine = 128;             // bytes of a row in one box
-template <int DT, int DP> struct AttCfg {
+template <int DT, int DP, bool PACK> struct AttCfg {
   static constexpr bool kBf = DT == MOE_CACHE_BF16;
+  using Frag = AFrag<kBf, PACK>;
   static constexpr int kElem = DT == MOE_CACHE_E4M3 ? 1 : 2;
   static constexpr int kSplit = DP > 128 ? 2 : 1;           // warps of a tile
   static constexpr int kDh = DP / kSplit;                   // columns of a warp
@@ -216,10 +231,10 @@ template <int DT, int DP> struct AttCfg {
   static constexpr int kMerge =
       4 * kAttHeads * (kTiles * kMergeRow > 4 * 32 * kWarps ? kTiles * kMergeRow : 4 * 32 * kWarps);
   static_assert(kMerge >= kAttParts * kAttHeads * 4, "weights of the parts");
-  static constexpr int kQ = DP / 16 * AFrag<kBf>::kBytes;
+  static constexpr int kQ = DP / 16 * Frag::kBytes;
   static constexpr int kX = kSplit > 1 ? kWarps * 32 * (kKeys / 4) * 4 : 0;   // halves of scores
   static constexpr int kSmem = kRing + kMerge + kQ + kX;
-  static constexpr int kFold = 64 / kKeys;
+  static constexpr int kFold = 128 / kKeys;                 // tiles between folds
 };
 
 // What the start and the end of a unit cost, in rounds (measured: about 2 us at
@@ -249,12 +264,12 @@ struct Cursor {
   int len, first, from;              // the sequence's keys first .. len, rounds from `from` on
 };
 
-template <int DT, int DP>
-__global__ void __launch_bounds__(AttCfg<DT, DP>::kWarps * 32, kAttCtasPerSm)
+template <int DT, int DP, bool PACK>
+__global__ void __launch_bounds__(AttCfg<DT, DP, PACK>::kWarps * 32, kAttCtasPerSm)
 attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                  const AttArgs A) {
-  using Cfg = AttCfg<DT, DP>;
-  constexpr bool BF = Cfg::kBf;
+  using Cfg = AttCfg<DT, DP, PACK>;
+  using Frag = typename Cfg::Frag;
   constexpr int NW = Cfg::kWarps, NT = NW * 32, KEYS = Cfg::kKeys, NS = Cfg::kSlots;
   constexpr int LINE = kLine, RK = Cfg::kRound, SP = Cfg::kSplit, DH = Cfg::kDh, NG = Cfg::kTiles;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -474,21 +489,21 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   constexpr int QK = DP / 16 / NW;
   uint8_t* const qs = smem + Cfg::kRing + Cfg::kMerge;
   float* const mo = reinterpret_cast<float*>(smem + Cfg::kRing);
-  const uint8_t* const qw = qs + warp % SP * (DH / 16) * AFrag<BF>::kBytes;   // this warp's columns
+  const uint8_t* const qw = qs + warp % SP * (DH / 16) * Frag::kBytes;   // this warp's columns
   float4* const xs = reinterpret_cast<float4*>(smem + Cfg::kRing + Cfg::kMerge + Cfg::kQ);
   float qn[QK][4];
   auto first_head = [&](const Cursor& c) { return c.head * G + c.group * kAttHeads; };
   auto heads = [&](const Cursor& c) { return min(kAttHeads, G - c.group * kAttHeads); };
   auto q_fetch = [&](const Cursor& c) {
-    const float* q = A.q + (int64_t)c.seq * A.q_ss + (int64_t)(first_head(c) + g) * A.q_hs;
-    const int nh = heads(c);
+    const int head = PACK ? g & 3 : g, nh = heads(c);
+    const float* q = A.q + (int64_t)c.seq * A.q_ss + (int64_t)(first_head(c) + head) * A.q_hs;
 #pragma unroll
     for (int i = 0; i < QK; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int e = 16 * (warp + i * NW) +
                       (Cfg::kElem == 1 ? 4 * t + j : 2 * t + (j & 1) + 8 * (j >> 1));
-        qn[i][j] = g < nh && e < D ? q[e] : 0.f;
+        qn[i][j] = head < nh && e < D ? q[e] : 0.f;
       }
   };
   auto q_max = [&]() {
@@ -518,10 +533,11 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       sh.qscale[g] = fmaxf(ldexpf(fabsf(A.scale) * A.c.k_scale, -e), 1e-30f);
 #pragma unroll
     for (int i = 0; i < QK; ++i) {
-      AFrag<BF> f;
+      Frag f;
       const float f0 = f1 * sign;
-      f.set(qn[i][0] * f0 * f2, qn[i][1] * f0 * f2, qn[i][2] * f0 * f2, qn[i][3] * f0 * f2);
-      f.store(qs + (warp + i * NW) * AFrag<BF>::kBytes, lane);
+      f.set(qn[i][0] * f0 * f2, qn[i][1] * f0 * f2, qn[i][2] * f0 * f2, qn[i][3] * f0 * f2,
+            g);
+      f.store(qs + (warp + i * NW) * Frag::kBytes, lane);
     }
   };
 
@@ -556,6 +572,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     const int ntile = tiles(C);
 
     const float qscale = sh.qscale[g];           // score = product * qscale
+    const float to_cap = qscale / A.cap, from_cap = A.cap * kLog2e;   // with a cap only
     const float x2 = A.cap > 0.f ? 1.f : qscale * kLog2e;
     float o[DH / 8][2];                          // head g, two columns of each 8-wide block
     float acc[DH / 8][4];
@@ -590,9 +607,9 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         float a[KEYS / 8][4];
 #pragma unroll
         for (int kk = 4 * k4; kk < 4 * k4 + 4; kk += 3 - Cfg::kElem) {
-          AFrag<BF> q0, q1;
-          q0.load(qw + kk * AFrag<BF>::kBytes, lane);
-          if (Cfg::kElem == 1) q1.load(qw + (kk + 1) * AFrag<BF>::kBytes, lane);
+          Frag q0, q1;
+          q0.load(qw + kk * Frag::kBytes, lane);
+          if (Cfg::kElem == 1) q1.load(qw + (kk + 1) * Frag::kBytes, lane);
 #pragma unroll
           for (int kb = 0; kb < KEYS / 16; ++kb) {
             uint32_t b[4];
@@ -628,6 +645,12 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
           x[b][1] = (k4 ? x[b][1] : 0.f) + (a[b][1] + a[b][3]);
         }
       }
+      if (PACK) {                                // the third part of q, in the other lanes
+#pragma unroll
+        for (int b = 0; b < KEYS / 8; ++b)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) x[b][h] += __shfl_xor_sync(0xffffffffu, x[b][h], 16);
+      }
       if (SP > 1) {
         // the other half of the columns: both warps get the same sums
         constexpr int V = KEYS / 16;
@@ -647,11 +670,32 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         }
         asm volatile("bar.sync %0, 64;" ::"r"(1 + warp / SP) : "memory");
       }
-      if (A.cap > 0.f) {
+      if (A.cap > 0.f) {                         // x = cap tanh(score / cap) log2 e
+        float big = 0.f;
 #pragma unroll
         for (int b = 0; b < KEYS / 8; ++b)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) x[b][h] = A.cap * tanhf(x[b][h] * qscale / A.cap) * kLog2e;
+          for (int h = 0; h < 2; ++h) {
+            x[b][h] *= to_cap;
+            big = fmaxf(big, fabsf(x[b][h]));
+          }
+        if (__any_sync(0xffffffffu, !(big < 0.5f))) {
+#pragma unroll
+          for (int b = 0; b < KEYS / 8; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[b][h] = from_cap * tanhf(x[b][h]);
+        } else {
+          // Lambert's continued fraction y / (1 + y^2 / (3 + y^2 / (5 + y^2 / (7 + y^2 / 9)))),
+          // off by less than 2^-29 of tanh y for |y| < 1/2
+#pragma unroll
+          for (int b = 0; b < KEYS / 8; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float y = x[b][h], z = y * y;
+              const float num = fmaf(z, z + 105.f, 945.f), den = fmaf(z, fmaf(15.f, z, 420.f), 945.f);
+              x[b][h] = from_cap * __fdividef(y * num, den);
+            }
+        }
       }
       if (seen != 0xffffffffu) {                 // lanes past KEYS repeat the first ones
 #pragma unroll
@@ -682,10 +726,10 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
           x[b][h] = ex2(fmaf(x[b][h], x2, shift));
           l += x[b][h];
         }
-      AFrag<BF> pf[KEYS / 16];
+      Frag pf[KEYS / 16];
 #pragma unroll
       for (int kb = 0; kb < KEYS / 16; ++kb)
-        pf[kb].set(x[2 * kb][0], x[2 * kb][1], x[2 * kb + 1][0], x[2 * kb + 1][1]);
+        pf[kb].set(x[2 * kb][0], x[2 * kb][1], x[2 * kb + 1][0], x[2 * kb + 1][1], g);
 
       const uint32_t va = wait_slot();
       issue_values();
@@ -702,7 +746,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       // p v.  e4m3: a 16-byte chunk holds 16 columns; transposed in pairs of
       // bytes, a register has columns (2g, 2g + 1) of two keys, which become
       // the B registers of the even and of the odd columns.  The accumulators
-      // take kFold tiles (four k16 steps) before they are added up
+      // take kFold tiles (eight k16 steps) before they are added up
       constexpr int CPB = Cfg::kElem == 2 ? 2 : 4;      // 8-wide blocks of two chunks
 #pragma unroll
       for (int c = 0; c < DH / 8; c += CPB) {
@@ -728,6 +772,12 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       if (i % Cfg::kFold == Cfg::kFold - 1) fold(1.f);
     }
     fold(1.f);
+    if (PACK) {
+#pragma unroll
+      for (int c = 0; c < DH / 8; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) o[c][h] += __shfl_xor_sync(0xffffffffu, o[c][h], 16);
+    }
 
     // ---- the warps' parts meet in shared memory
     l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -930,12 +980,12 @@ static int make_cache_map(CUtensorMap* map, AttArgs& a, void* base, int keys) {
   return MOE_OK;
 }
 
-template <int DT, int DP>
+template <int DT, int DP, bool PACK>
 static int launch_attention(AttArgs& a, int max_len, cudaStream_t s) {
-  using Cfg = AttCfg<DT, DP>;
+  using Cfg = AttCfg<DT, DP, PACK>;
   static_assert(Cfg::kSlots % 2 == 1 && Cfg::kSlots <= 5 && Cfg::kWarps == 4, "");
   static std::atomic<uint64_t> ready{0};
-  auto kern = attention_kernel<DT, DP>;
+  auto kern = attention_kernel<DT, DP, PACK>;
   int dev = 0;
   MOE_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !((ready.load() >> dev) & 1)) {
@@ -962,12 +1012,12 @@ static int launch_attention(AttArgs& a, int max_len, cudaStream_t s) {
   return MOE_OK;
 }
 
-template <int DT>
+template <int DT, bool PACK>
 static int launch_attention_dt(AttArgs& a, int max_len, cudaStream_t s) {
   switch (padded_head_dim(a.c.head_dim)) {
-    case 64: return launch_attention<DT, 64>(a, max_len, s);
-    case 128: return launch_attention<DT, 128>(a, max_len, s);
-    default: return launch_attention<DT, 256>(a, max_len, s);
+    case 64: return launch_attention<DT, 64, PACK>(a, max_len, s);
+    case 128: return launch_attention<DT, 128, PACK>(a, max_len, s);
+    default: return launch_attention<DT, 256, PACK>(a, max_len, s);
   }
 }
 
@@ -1021,10 +1071,14 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   {
     ::moe::ProfScope _prof(MOE_K_ATTENTION, s);
-    MOE_CHECK(cache->dtype == MOE_CACHE_F16 ? moe::launch_attention_dt<MOE_CACHE_F16>(a, longest, s)
-              : cache->dtype == MOE_CACHE_BF16
-                  ? moe::launch_attention_dt<MOE_CACHE_BF16>(a, longest, s)
-                  : moe::launch_attention_dt<MOE_CACHE_E4M3>(a, longest, s));
+    if (cache->dtype == MOE_CACHE_F16)
+      MOE_CHECK((moe::launch_attention_dt<MOE_CACHE_F16, false>(a, longest, s)));
+    else if (cache->dtype == MOE_CACHE_E4M3)
+      MOE_CHECK((moe::launch_attention_dt<MOE_CACHE_E4M3, false>(a, longest, s)));
+    else if (q_heads / cache->kv_heads <= 4)
+      MOE_CHECK((moe::launch_attention_dt<MOE_CACHE_BF16, true>(a, longest, s)));
+    else
+      MOE_CHECK((moe::launch_attention_dt<MOE_CACHE_BF16, false>(a, longest, s)));
   }
   return moe::check_launch("paged_attention");
 }
