@@ -1,10 +1,14 @@
 // y = W x (+ residual) for a few rows, W in packed Q4_0 / Q8_0 tiles.
 //
 // Each weight is read once for up to 16 rows, so the bound is memory up to
-// about 8 rows, and mma.sync issue beyond.  As in the experts' gate/up kernel
-// the quants themselves are the (exact, subnormal fp16) A operand, x enters as
-// fp16 hi + lo columns (4 rows fill the 8 columns of an MMA), and every
-// 32-weight block has an accumulator of its own that is scaled in f32.
+// about 8 rows, and mma.sync issue beyond.  As in the experts' GEMVs the quants
+// themselves are the (exact fp16) A operand, x enters as fp16 hi + lo columns (4
+// rows fill the 8 columns of an MMA), and a 32-weight block is scaled in f32 after
+// its sum.  The quants are made signed: as subnormals with their offset in the
+// accumulator, the experts' form, they take 8 half-precision operations per
+// 512 weights less (262144 x 2816 for one row 75 us instead of 83), but the
+// tensor core aligns the subnormals' products to exponents 7 bits too large, and
+// the result was off by up to 1.1e-6 of its norm instead of 1e-7.
 //
 // One CTA of 16 warps per SM stays resident.  It turns its columns of x into
 // fragments in shared memory once, while the first weights are under way, and
@@ -63,17 +67,15 @@ template <int NBG, int G> struct LinCfg {
   static constexpr int kTok = 4 / NBG;           // rows of a column group
   static constexpr int kRows = kTok * G;         // rows of a pass
   static constexpr int kRed = 2 * G * 2 * 32;    // floats of a pair of strips
-  // fragments of a tile's two blocks, and their offset corrections (hi, lo)
-  static constexpr int kTileBytes = G * (2 * 512 + (NBG == 4 ? 1 : NBG == 2 ? 1 : 2) * 32);
+  static constexpr int kTileBytes = G * 2 * 512; // fragments of a tile's two blocks
 };
 
 // x columns [64 t0, 64 t1) of n rows -> fragments `rec` ([block][column group] of
-// 512 bytes) and corrections `cor` ([blocks / NBG][column group][pair]); a row
-// times 2^ex has its largest |x| in [2^14, 2^15).
+// 512 bytes); a row times 2^ex has its largest |x| in [2^14, 2^15).
 template <int QT, int NBG, int G>
-__device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, float2* cor,
-                                                int rec_blocks, int* ex, uint32_t* smax, int row0,
-                                                int n, int t0, int t1) {
+__device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, int rec_blocks,
+                                                int* ex, uint32_t* smax, int row0, int n, int t0,
+                                                int t1) {
   constexpr int TOK = LinCfg<NBG, G>::kTok, ROWS = LinCfg<NBG, G>::kRows;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = lane & 3;
   const int nb = 2 * (t1 - t0), real = min(nb, A.cols / 32 - 2 * t0);   // blocks, with columns
@@ -110,8 +112,6 @@ __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, 
   if (tid < ROWS) ex[tid] = 0;
   for (int i = tid; i < G * rec_blocks * 32; i += kLinWarps * 32)
     reinterpret_cast<uint4*>(rec)[i] = make_uint4(0, 0, 0, 0);
-  for (int i = tid; i < G * (rec_blocks / NBG) * 4; i += kLinWarps * 32)
-    cor[i] = make_float2(0.f, 0.f);
   __syncthreads();
   if (!on) return;
   mx = 0;
@@ -121,43 +121,25 @@ __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, 
   const float f1 = pow2f(e / 2), f2 = pow2f(e - e / 2);
   if (part == 0 && lane == 0) ex[row] = e;
   const int cg = row / TOK;
-  for (int b = part * 8 + (lane >> 2); b < (real + 7) / 8 * 8; b += wpr * 8) {
-    uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-    float sh = 0.f, sl = 0.f;
-    if (b < real) {
-      float v[8];
-      values(b, v);
+  for (int b = part * 8 + (lane >> 2); b < real; b += wpr * 8) {
+    uint32_t hi[4], lo[4];
+    float v[8];
+    values(b, v);
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        // register slots i, i + 1 hold elements 0, 2 | 1, 3 of each four (Q4_0)
-        const int p = QT == MOE_Q4_0 ? (i & 4) + ((i & 2) ? 1 : 0) : i;
-        const int q = QT == MOE_Q4_0 ? p + 2 : i + 1;
-        // high nibbles stay 16 times too large; their x is stored / 16
-        const float div = QT == MOE_Q4_0 && i >= 4 ? 0.0625f : 1.f;
-        const float mul = QT == MOE_Q4_0 && i >= 4 ? 16.f : 1.f;
-        const float a = v[p] * f1 * f2 * div, c = v[q] * f1 * f2 * div;
-        const __half2 h = __floats2half2_rn(a, c);
-        const float ha = __low2float(h), hc = __high2float(h);
-        const __half2 l = __floats2half2_rn(a - ha, c - hc);
-        sh += mul * (ha + hc);
-        sl += mul * (__low2float(l) + __high2float(l));
-        hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-        lo[i / 2] = *reinterpret_cast<const uint32_t*>(&l);
-      }
+    for (int i = 0; i < 8; i += 2) {
+      // register slots i, i + 1 hold elements 0, 2 | 1, 3 of each four (Q4_0)
+      const int p = QT == MOE_Q4_0 ? (i & 4) + ((i & 2) ? 1 : 0) : i;
+      const int q = QT == MOE_Q4_0 ? p + 2 : i + 1;
+      const float a = v[p] * f1 * f2, c = v[q] * f1 * f2;
+      const __half2 h = __floats2half2_rn(a, c);
+      const __half2 l = __floats2half2_rn(a - __low2float(h), c - __high2float(h));
+      hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+      lo[i / 2] = *reinterpret_cast<const uint32_t*>(&l);
     }
-    sh += __shfl_xor_sync(0xffffffffu, sh, 1);
-    sl += __shfl_xor_sync(0xffffffffu, sl, 1);
-    sh += __shfl_xor_sync(0xffffffffu, sh, 2);
-    sl += __shfl_xor_sync(0xffffffffu, sl, 2);
-    if (b < real) {
-      const int pair = (b % NBG) * TOK + row % TOK;
-      uint8_t* r = rec + (size_t)(b * G + cg) * 512 + pair * 128 + t * 16;
-      *reinterpret_cast<uint4*>(r) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(r + 64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      const float k = -quant_offset<QT>() / kSubUnit;
-      if (t == 0)
-        cor[(b / NBG * G + cg) * 4 + pair] = make_float2(k * sh, k * sl);
-    }
+    const int pair = (b % NBG) * TOK + row % TOK;
+    uint8_t* r = rec + (size_t)(b * G + cg) * 512 + pair * 128 + t * 16;
+    *reinterpret_cast<uint4*>(r) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(r + 64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
 }
 
@@ -171,6 +153,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
   uint64_t* const bars_all = reinterpret_cast<uint64_t*>(smem);
   uint32_t* const smax = reinterpret_cast<uint32_t*>(smem + 1024);
   int* const ex = reinterpret_cast<int*>(smem + 1024 + 64);
+  volatile int* const dead = reinterpret_cast<volatile int*>(smem + 1024 + 128);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % A.cs, cluster = blockIdx.x / A.cs, nclusters = gridDim.x / A.cs;
   const int groups = kLinWarps / A.ks, group = warp / A.ks, kq = warp % A.ks;
@@ -181,7 +164,6 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
   const int wt0 = min(t1, t0 + kq * wps), wt1 = min(t1, wt0 + wps), nt = wt1 - wt0;
   const int rec_blocks = 2 * tps;                // tps is even
   uint8_t* const rec = smem + kLinHead;
-  float2* const cor = reinterpret_cast<float2*>(rec + (size_t)G * rec_blocks * 512);
   float* const red = reinterpret_cast<float*>(rec + (size_t)tps * Cfg::kTileBytes);
   float* const part = red + (A.ks > 1 ? kLinWarps * NRED : 0);
   uint8_t* const ring =
@@ -192,6 +174,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
     mbar_init(&bars[lane], 1);
     fence_mbar_init();
   }
+  if (tid == 0) *dead = 0;                       // seen by all after build_fragments
   __syncwarp();
   pdl_trigger();
   pdl_wait();
@@ -205,17 +188,14 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
   const int strips = (A.rows + 15) / 16;
   int ip = p0, ij = 0, islot = 0, issued = 0;
   const int64_t strip = (int64_t)A.kt * TB;      // bytes from strip to strip
-  const uint8_t* src = A.w + 2 * ip * strip + (int64_t)wt0 * TB;
+  // lanes 0 and 1 copy a strip each
+  const uint8_t* src = A.w + (2 * ip + (lane & 1)) * strip + (int64_t)wt0 * TB;
   const int last = (nt - (nsr - 1) * U) * TB;    // bytes of a pair's last stage
   auto issue = [&]() {                           // stage `issued`
-    if (lane == 0) {
-      const uint32_t bytes = ij == nsr - 1 ? last : U * TB;
-      const bool two = 2 * ip + 1 < strips;
-      uint8_t* dst = ring + islot * STAGE;
-      mbar_expect_tx(&bars[islot], two ? 2 * bytes : bytes);
-      bulk_g2s(dst, src, bytes, &bars[islot], pol);
-      if (two) bulk_g2s(dst + U * TB, src + strip, bytes, &bars[islot], pol);
-    }
+    const uint32_t bytes = ij == nsr - 1 ? last : U * TB;
+    const int n = 2 * ip + 1 < strips ? 2 : 1;
+    if (lane == 0) mbar_expect_tx(&bars[islot], n * bytes);
+    if (lane < n) bulk_g2s(ring + islot * STAGE + lane * U * TB, src, bytes, &bars[islot], pol);
     ++issued;
     src += U * TB;
     islot = islot + 1 == A.nst ? 0 : islot + 1;
@@ -226,16 +206,14 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
     }
   };
   for (int q = 0; q < A.nst && q < total; ++q) issue();
-  build_fragments<QT, NBG, G>(A, rec, cor, rec_blocks, ex, smax, row0, n, t0, t1);
+  build_fragments<QT, NBG, G>(A, rec, rec_blocks, ex, smax, row0, n, t0, t1);
   __syncthreads();
 
   // ---- stream
-  bool ok = true;
   int slot = 0;
   uint32_t phase = 0;
-  // fragments and corrections of this warp's columns
+  // fragments of this warp's columns
   const uint8_t* const xl = rec + lane * 16 + (size_t)2 * (wt0 - t0) * G * 512;
-  const float2* const cl = cor + t + 2 * (wt0 - t0) / NBG * G * 4;
   // value i (row g + 8 i) of strip s, column group cg in lane l
   auto put = [&](int p, int s, int cg, int i, int l, float y) {
     const int tok = TOK * cg + (l & 3), row = 32 * p + 16 * s + (l >> 2) + 8 * i;
@@ -253,23 +231,18 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
       for (int cg = 0; cg < G; ++cg) v[s][cg][0] = v[s][cg][1] = 0.f;
     if (p < A.pairs) {
       for (int j = 0; j < nsr; ++j) {
-        if (ok && !mbar_wait(&bars[slot], phase)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
+        // bounded; after a timeout anywhere in the CTA no wait takes long any more
+        if (!mbar_test(&bars[slot], phase) && !*dead && !mbar_wait(&bars[slot], phase)) *dead = 1;
+        __syncwarp();
         const uint8_t* st = ring + slot * STAGE;
         const uint8_t* xq = xl + j * (U * 2 * G * 512);
-        const float2* cq = cl + j * (U * 2 / NBG * G * 4);
         const int left = nt - j * U;             // tiles of the stage, 2 or more: both
         float c[2][G][4];
-        auto begin = [&](int grp) {              // offset corrections of a group of blocks
+        auto begin = [&]() {                     // of a group of blocks
 #pragma unroll
-          for (int cg = 0; cg < G; ++cg) {
-            const float2 z = cq[(grp * G + cg) * 4];
+          for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              c[s][cg][0] = c[s][cg][2] = z.x;
-              c[s][cg][1] = c[s][cg][3] = z.y;
-            }
-          }
+            for (int cg = 0; cg < G; ++cg) c[s][cg][0] = c[s][cg][1] = c[s][cg][2] = c[s][cg][3] = 0.f;
         };
         auto finish = [&](int tile, int half, bool valid) {   // scales of this lane's block
 #pragma unroll
@@ -285,20 +258,20 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
             }
           }
         };
-        if (NBG == 4) begin(0);
+        if (NBG == 4) begin();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (u == 0 || u < left) {
             TileRegs<QT> w[2];
 #pragma unroll
             for (int s = 0; s < 2; ++s) lds_quants<QT>(w[s], st + (s * U + u) * TB, lane);
-            if (NBG == 2) begin(u);
+            if (NBG == 2) begin();
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-              if (NBG == 1) begin(2 * u + b);
+              if (NBG == 1) begin();
               uint32_t a0[2][4], a1[2][4];
 #pragma unroll
-              for (int s = 0; s < 2; ++s) tile_quants<QT, true>(w[s], b, a0[s], a1[s]);
+              for (int s = 0; s < 2; ++s) tile_quants<QT, false>(w[s], b, a0[s], a1[s]);
 #pragma unroll
               for (int cg = 0; cg < G; ++cg) {
                 const uint4 xf =
@@ -316,7 +289,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
         }
         if (NBG == 4) finish(t >> 1, t & 1, (t >> 1) < left);
         __syncwarp();                            // the stage has been read
-        if (ok && issued < total) issue();
+        if (issued < total && !*dead) issue();
         if (++slot == A.nst) {
           slot = 0;
           phase ^= 1u;
@@ -331,7 +304,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
         for (int i = 0; i < 2; ++i) {
           if (NBG >= 2) v[s][cg][i] += __shfl_xor_sync(0xffffffffu, v[s][cg][i], 2);
           if (NBG == 4) v[s][cg][i] += __shfl_xor_sync(0xffffffffu, v[s][cg][i], 1);
-          if (!ok) v[s][cg][i] = __uint_as_float(0x7fffffffu);   // a wait ran out: NaN
+          if (*dead) v[s][cg][i] = __uint_as_float(0x7fffffffu);   // a wait ran out: NaN
         }
     if (A.ks > 1) {
       // the column parts of a pair meet in the group's first warp
@@ -364,7 +337,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) v[s][cg][i] = v[s][cg][i] * kSubUnit * f1 * f2;
+          for (int i = 0; i < 2; ++i) v[s][cg][i] = v[s][cg][i] * f1 * f2;
       }
     }
     if (A.cs == 1) {
@@ -402,7 +375,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
     }
   }
   // after a timeout the copies already issued are still waited for (bounded)
-  if (!ok)
+  if (*dead)
     for (int i = 0; i < A.nst; ++i) {
       mbar_wait(&bars[i], 0);
       mbar_wait(&bars[i], 1);

@@ -359,6 +359,18 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
   return t;
 }
 
+// Whether an mbarrier phase is complete.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
 // Bounded wait for an mbarrier phase.  Gives up (returns false; the caller
 // flags MOE_STATUS_TIMEOUT) after ~0.2 s of wall time or 2^24 polls.  Each
 // poll may suspend the thread in hardware for up to that many ns while the
