@@ -396,8 +396,8 @@ int moe_ep_forward_phases(const moe_layer_weights* w, int W, int rank, void* con
  * axis of extent 1 is ignored), so both the token-major and the head-major
  * layout of a page fit.  Token position p of sequence s is in page
  * block_table[s * table_stride + p / page_size], slot p % page_size; entries
- * behind a sequence's last page are never read.  Bases and strides must be
- * multiples of 16 bytes; head_dim a multiple of 8 (16 for MOE_CACHE_E4M3), at
+ * behind a sequence's last page are never read, and a page may belong to
+ * several sequences.  Bases and strides must be multiples of 16 bytes; head_dim a multiple of 8 (16 for MOE_CACHE_E4M3), at
  * most 256.  MOE_CACHE_E4M3 holds value / scale, rounded to nearest even and
  * saturated at +-448; the scales of the other types must be 1.
  * A page id outside [0, pages) sets MOE_STATUS_BAD_PAGE; its slots are neither
@@ -456,6 +456,8 @@ int moe_paged_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int
  *   max_len no sequence is longer (0 = table_width * page_size); it sizes the
  *          launch, a longer sequence is still computed in full
  *   out (seqs, q_heads, head_dim) f32 contiguous; lse (seqs, q_heads) or NULL
+ *   the cache's strides must be multiples of a common row of head_dim elements
+ *          or more (every dense layout, also with padded rows or pages)
  *   workspace: zeroed by the caller before its first use and then kept between
  *          calls, which leave it ready for the next one (but for the status
  *          word at its start); calls that may overlap need one each
@@ -471,8 +473,10 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
  *      with zero blocks to rows % 16 == 0 and cols % 64 == 0 and packed by
  *      moe_pack_weights
  *   x (T, cols), y (T, rows), residual (T, rows) or NULL: rows at the given
- *      strides (elements); residual may be y itself with the same stride
- * Made for a few rows: the weights are read once for every 16 of them. */
+ *      strides (elements); residual may be y itself with the same stride;
+ *      y must not overlap x or w
+ * Made for a few rows: the weights are read once for every 16 of them (8 or 4
+ * where x is so wide that 16 do not fit).  Should a copy never arrive, y is NaN. */
 int moe_linear(const uint8_t* w, int qtype, int rows, int cols, const float* x, int64_t x_stride,
                int T, const float* residual, int64_t residual_stride, float* y, int64_t y_stride,
                moe_stream_t stream);

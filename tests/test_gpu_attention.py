@@ -316,6 +316,84 @@ def test_attention_offsets_past_32_bits():
         check_stored(v[at, p % page], vn[s].double(), 0 * vn[s].double(), E4M3, c.v_scale)
 
 
+@pytest.mark.parametrize("dtype", [F16, E4M3])
+def test_other_cache_layouts(dtype):
+    """Keys and values side by side in one pool, rows with padding behind them,
+    a pool of one page, one slot per page, one key head."""
+    hq, hkv, d = 4, 2, 64
+    c = Cache([70, 33], 16, hkv, d, dtype, seed=20)
+    q = randn(2, hq, d, seed=20)
+    want = K.paged_attention(q, *c.args, c.lens, **c.scales)
+    check_attention(c, q, want, None, d ** -0.5)
+    bits = torch.uint8
+    pool = torch.zeros((c.k.shape[0], 2) + c.k.shape[1:], dtype=dtype, device="cuda")
+    pool.view(bits)[:, 0], pool.view(bits)[:, 1] = c.k.view(bits), c.v.view(bits)
+    got = K.paged_attention(q, pool[:, 0], pool[:, 1], c.table_d, c.lens, **c.scales)
+    assert torch.equal(got, want)
+    wide = [torch.zeros(c.k.shape[:3] + (d + 16,), dtype=dtype, device="cuda") for _ in range(2)]
+    for w, x in zip(wide, (c.k, c.v)):
+        w.view(bits)[..., :x.view(bits).shape[-1]] = x.view(bits)
+    got = K.paged_attention(q, wide[0][..., :d], wide[1][..., :d], c.table_d, c.lens, **c.scales)
+    assert torch.equal(got, want)
+    kn, vn, pos = randn(2, hkv, d, seed=21), randn(2, hkv, d, seed=22), c.lens - 1
+    K.rope_append(None, kn, vn, *c.args, pos, **c.scales)
+    for k, v in ((pool[:, 0], pool[:, 1]), (wide[0][..., :d], wide[1][..., :d])):
+        K.rope_append(None, kn, vn, k, v, c.table_d, pos, **c.scales)
+        assert torch.equal(k.contiguous().view(bits), c.k.view(bits))
+        assert torch.equal(v.contiguous().view(bits), c.v.view(bits))
+    one = Cache([5], 8, 1, d, dtype, seed=23, spare=0)
+    out = K.paged_attention(q[:1], *one.args, one.lens, **one.scales)
+    check_attention(one, q[:1], out, None, d ** -0.5)
+    single = Cache([1], 1, 1, d, dtype, seed=24, spare=0)
+    out = K.paged_attention(q[:1], *single.args, single.lens, **single.scales)
+    check_attention(single, q[:1], out, None, d ** -0.5)
+    odd = torch.zeros((3, 16 * (2 * d + 16)), dtype=dtype, device="cuda").as_strided(
+        (3, 16, 2, d), (16 * (2 * d + 16), 2 * d + 16, d, 1))
+    with pytest.raises(_lib.MoEError, match="strides"):
+        K.paged_attention(q, odd, odd, c.table_d, c.lens, **c.scales)
+
+
+def test_pages_shared_by_sequences():
+    """A common prefix is held once; two sequences list its pages."""
+    hq, hkv, d, page = 8, 2, 128, 16
+    c = Cache([64, 30], page, hkv, d, BF16, seed=25)
+    table = c.table_d.clone()
+    table[1, 2] = table[1, 0]
+    table[1, 3] = table[1, 1]
+    table[1, 0], table[1, 1] = table[0, 0], table[0, 1]
+    lens = torch.tensor([64, 62], dtype=torch.int32).cuda()
+    q = randn(2, hq, d, seed=26)
+    out = K.paged_attention(q, c.k, c.v, table, lens, max_len=1)   # too small a hint: still whole
+    both = type("C", (), dict(kd=[c.kd[0], torch.cat([c.kd[0][:32], c.kd[1]])],
+                              vd=[c.vd[0], torch.cat([c.vd[0][:32], c.vd[1]])]))
+    check_attention(both, q, out, None, d ** -0.5)
+
+
+def test_two_calls_at_once():
+    """Two streams, a workspace each, many calls under way together."""
+    hq, hkv, d = 8, 2, 128
+    caches = [Cache([6000, 10], 16, hkv, d, F16, seed=30 + i) for i in range(2)]
+    qs = [randn(2, hq, d, seed=32 + i) for i in range(2)]
+    ws = [K.paged_attention_workspace(2, hq, hkv, d, "cuda") for _ in range(2)]
+    want = [K.paged_attention(q, *c.args, c.lens, ws=w) for q, c, w in zip(qs, caches, ws)]
+    rng = np.random.default_rng(3)
+    raw, w, big = matrix(rng, 2, 512, 4096)
+    lw = K.LinearWeights(torch.from_numpy(raw.reshape(-1)).cuda(), 2, 512, 4096)
+    xs = [randn(3 + 8 * i, 4096, seed=34 + i) for i in range(2)]
+    want_y = [K.linear(x, lw) for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((K.paged_attention(qs[i], *caches[i].args, caches[i].lens, ws=ws[i]),
+                               K.linear(xs[i], lw)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, y in got[i]:
+            assert torch.equal(o, want[i]) and torch.equal(y, want_y[i])
+
+
 def test_attention_many_sequences():
     """More sequences than a CTA has threads, most of them empty."""
     hq, hkv, d = 4, 2, 64
@@ -399,6 +477,37 @@ def test_linear_wide(qtype, T, rows, cols):
     res = rng.standard_normal((T, rows), dtype=np.float32)
     y = K.linear(torch.from_numpy(x).cuda(), lw, residual=torch.from_numpy(res).cuda())
     check_linear(y.cpu().numpy(), x, w, big, res)
+
+
+def test_linear_many_rows():
+    """More rows than one pass, the last pass with one of them."""
+    rng = np.random.default_rng(5)
+    raw, w, big = matrix(rng, 2, 80, 224)
+    lw = K.LinearWeights(torch.from_numpy(raw.reshape(-1)).cuda(), 2, 80, 224)
+    x = rng.standard_normal((321, 224), dtype=np.float32)
+    y = K.linear(torch.from_numpy(x).cuda(), lw).cpu().numpy()
+    check_linear(y, x, w, big)
+    # parts of the batch by themselves
+    for t in (0, 15, 16, 320):
+        one = K.linear(torch.from_numpy(x[t:t + 16]).cuda(), lw).cpu().numpy()
+        check_linear(one, x[t:t + 16], w, big)
+
+
+def test_linear_captured():
+    rng = np.random.default_rng(6)
+    raw, w, big = matrix(rng, 2, 256, 8192)
+    lw = K.LinearWeights(torch.from_numpy(raw.reshape(-1)).cuda(), 2, 256, 8192)
+    for T in (1, 2, 16):
+        x = torch.zeros((T, 8192), device="cuda")
+        y = torch.empty((T, 256), device="cuda")
+        K.linear(x, lw, out=y)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            K.linear(x, lw, out=y)
+        for seed in range(3):
+            x.copy_(randn(T, 8192, seed=seed))
+            g.replay()
+            check_linear(y.cpu().numpy(), x.cpu().numpy(), w, big)
 
 
 def test_linear_strides_residual_in_place_and_no_rows():
