@@ -189,10 +189,15 @@ def check(status: int) -> None:
 _entries = {}
 
 
-def call(name: str, *args) -> None:
+def entry(name: str):
+    """An entry point, looked up once."""
     fn = _entries.get(name)
     if fn is None:
         fn = _entries[name] = getattr(load(), name)
-    status = fn(*args)
+    return fn
+
+
+def call(name: str, *args) -> None:
+    status = entry(name)(*args)
     if status != MOE_OK:
         check(status)

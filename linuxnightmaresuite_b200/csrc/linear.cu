@@ -435,39 +435,48 @@ static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
     MOE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem));
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
-  // Estimated time of a split, in the time all warps of an SM take for one tile
-  // of two strips each (about 800 cycles of HBM): rounds x (tiles of a warp, and
-  // the meetings of warps, 3, and of a cluster, 8), and the fragments of the
-  // CTA's columns (28 cycles per group and tile).
-  double best = 0;
-  int clusters = 0;
-  a.cs = 0;
-  for (int cs = 1; cs <= 8; cs *= 2) {
-    if (linear_smem<QT, NBG, G>(a.kt, cs, kLinWarps, 2) > kLinSmem) continue;
-    const int resident = resident_clusters((const void*)kern, cs, dev);
-    for (int ks = 1; ks <= kLinWarps; ks *= 2) {
-      if (linear_smem<QT, NBG, G>(a.kt, cs, ks, 2) > kLinSmem) continue;
-      const int tps = linear_tps(a.kt, cs), wt = ((tps + ks - 1) / ks + 1) / 2 * 2;
-      const int slots = resident * (kLinWarps / ks);
-      const int rounds = (a.pairs + slots - 1) / slots;
-      const double t = rounds * (wt * (1 + 0.25 * (G - 1)) + (ks > 1 ? 3 : 0) + (cs > 1 ? 8 : 0)) +
-                       0.035 * G * tps;
-      if (a.cs == 0 || t < best) {
-        best = t;
-        a.cs = cs;
-        a.ks = ks;
-        clusters = resident;
+  // The splits of a few sizes are remembered, for calls that repeat them.
+  struct Plan { int dev = -1, kt, pairs, cs, ks, nst, clusters; };
+  static thread_local Plan plans[16];
+  Plan& plan = plans[(a.kt * 31 + a.pairs) & 15];
+  if (plan.dev != dev || plan.kt != a.kt || plan.pairs != a.pairs)
+    plan = {dev, a.kt, a.pairs, 0, 0, 0, 0};
+  if (plan.nst == 0) {
+    // Estimated time of a split, in the time all warps of an SM take for one tile
+    // of two strips each (about 800 cycles of HBM): rounds x (tiles of a warp, and
+    // the meetings of warps, 3, and of a cluster, 8), and the fragments of the
+    // CTA's columns (28 cycles per group and tile).
+    double best = 0;
+    for (int cs = 1; cs <= 8; cs *= 2) {
+      const int resident = resident_clusters((const void*)kern, cs, dev);
+      for (int ks = 1; ks <= kLinWarps; ks *= 2) {
+        if (linear_smem<QT, NBG, G>(a.kt, cs, ks, 2) > kLinSmem) continue;
+        const int tps = linear_tps(a.kt, cs), wt = ((tps + ks - 1) / ks + 1) / 2 * 2;
+        const int slots = resident * (kLinWarps / ks);
+        const int rounds = (a.pairs + slots - 1) / slots;
+        const double t = rounds * (wt * (1 + 0.25 * (G - 1)) + (ks > 1 ? 3 : 0) + (cs > 1 ? 8 : 0)) +
+                         0.035 * G * tps;
+        if (plan.cs == 0 || t < best) {
+          best = t;
+          plan.cs = cs;
+          plan.ks = ks;
+          plan.clusters = resident;
+        }
       }
     }
+    plan.nst = 2;
+    while (plan.cs > 0 && plan.nst < kLinMaxStages &&
+           linear_smem<QT, NBG, G>(a.kt, plan.cs, plan.ks, plan.nst + 1) <= kLinSmem)
+      ++plan.nst;
   }
-  fits = a.cs > 0;
+  fits = plan.cs > 0;
   if (!fits) return MOE_OK;
+  a.cs = plan.cs;
+  a.ks = plan.ks;
+  a.nst = plan.nst;
   a.tps = linear_tps(a.kt, a.cs);
-  a.nst = 2;
-  while (a.nst < kLinMaxStages && linear_smem<QT, NBG, G>(a.kt, a.cs, a.ks, a.nst + 1) <= kLinSmem)
-    ++a.nst;
   const int per = kLinWarps / a.ks;                  // pairs of a cluster's round
-  clusters = std::min(clusters, (a.pairs + per - 1) / per);
+  const int clusters = std::min(plan.clusters, (a.pairs + per - 1) / per);
   a.rounds = (a.pairs + clusters * per - 1) / (clusters * per);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * a.cs), (unsigned)((a.T + Cfg::kRows - 1) / Cfg::kRows));

@@ -13,7 +13,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import call
+from ._lib import call, entry
 
 QTYPE_F32 = _lib.MOE_F32
 QTYPE_Q4_0 = _lib.MOE_Q4_0
@@ -271,14 +271,10 @@ _CACHE_STRUCT = struct.Struct("@3P4q7i2f0q")
 assert _CACHE_STRUCT.size == ctypes.sizeof(_lib.MoEPagedCache)
 
 
-def _call_on(index: int, name: str, *args) -> None:
-    """The entry point on device ``index`` and its current stream, whichever
-    device is current."""
-    if index == torch._C._cuda_getDevice():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+def _elsewhere(index: int, fn, args) -> int:
+    """The entry point with device ``index`` made current."""
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
 
 
 # These wrappers are called once per layer and token, on kernels of a few
@@ -297,6 +293,8 @@ def _refuse(t, name: str, dtype, index: int, shape=None) -> None:
 
 
 _F32, _I32 = torch.float32, torch.int32
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _rows_f32(t: torch.Tensor, name: str, index: int, shape) -> Tuple[int, ...]:
@@ -380,16 +378,20 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         hq = q.shape[1]
         qs = _rows_f32(q, "q", dev, (T, hq, d))
         if q_out is None:
-            q_out = q.new_empty((T, hq, d))
-            os_ = (hq * d, d)
+            q_out = torch.empty_like(q)          # dense, whatever q's strides
+            os_ = q_out.stride()
         else:
             os_ = _rows_f32(q_out, "q_out", dev, (T, hq, d))
         q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
-    _call_on(dev, "moe_rope_append", c, q_ptr, qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
-             v.data_ptr(), vs[0], vs[1], T, hq, _vector(positions, _I32, "positions", dev, T),
-             None if seq_ids is None else _vector(seq_ids, _I32, "seq_ids", dev, T), freq,
-             rot, 1 if interleaved else 0, o_ptr, os_[0], os_[1],
-             None if status is None else _vector(status, _I32, "status", dev, 1))
+    args = (c, q_ptr, qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], T, hq,
+            _vector(positions, _I32, "positions", dev, T),
+            None if seq_ids is None else _vector(seq_ids, _I32, "seq_ids", dev, T), freq, rot,
+            1 if interleaved else 0, o_ptr, os_[0], os_[1],
+            None if status is None else _vector(status, _I32, "status", dev, 1))
+    fn = entry("moe_rope_append")
+    rc = fn(*args, _raw_stream(dev)) if dev == _current_device() else _elsewhere(dev, fn, args)
+    if rc:
+        _lib.check(rc)
     return q_out
 
 
@@ -434,7 +436,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     hq = q.shape[1]
     qs = _rows_f32(q, "q", dev, (seqs, hq, d))
     if out is None:
-        out = q.new_empty((seqs, hq, d))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype is not _F32 or out.get_device() != dev or out.shape != (seqs, hq, d) or \
             not out.is_contiguous():
         _refuse(out, "out", _F32, dev, (seqs, hq, d))
@@ -443,10 +445,13 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         ws = paged_attention_workspace(seqs, hq, hk, d, q.device)
     elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
         _refuse(ws, "ws", torch.uint8, dev)
-    _call_on(dev, "moe_paged_attention", c, q.data_ptr(), qs[0], qs[1],
-             _vector(seq_lens, _I32, "seq_lens", dev, seqs), hq, max_len, window,
-             d ** -0.5 if scale is None else scale, softcap, out.data_ptr(),
-             None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel())
+    args = (c, q.data_ptr(), qs[0], qs[1], _vector(seq_lens, _I32, "seq_lens", dev, seqs), hq,
+            max_len, window, d ** -0.5 if scale is None else scale, softcap, out.data_ptr(),
+            None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel())
+    fn = entry("moe_paged_attention")
+    rc = fn(*args, _raw_stream(dev)) if dev == _current_device() else _elsewhere(dev, fn, args)
+    if rc:
+        _lib.check(rc)
     return (out, lse) if return_lse else out
 
 
@@ -490,8 +495,11 @@ def linear(x: torch.Tensor, w: LinearWeights, residual: Optional[torch.Tensor] =
         ys = _rows_f32(out, "out", dev, (T, w.rows))[0]
         if ys < w.rows and T > 1:
             raise ValueError("rows of out overlap")
-    _call_on(dev, "moe_linear", w.address, w.qtype, w.rows, w.cols, x.data_ptr(), xs, T, res, rs,
-             out.data_ptr(), ys)
+    args = (w.address, w.qtype, w.rows, w.cols, x.data_ptr(), xs, T, res, rs, out.data_ptr(), ys)
+    fn = entry("moe_linear")
+    rc = fn(*args, _raw_stream(dev)) if dev == _current_device() else _elsewhere(dev, fn, args)
+    if rc:
+        _lib.check(rc)
     return out
 
 
