@@ -26,7 +26,6 @@
 namespace moe {
 
 constexpr int kLinWarps = 16;
-constexpr int kLinU = 2;               // tiles of each strip per ring stage
 constexpr int kLinMaxStages = 4;
 constexpr int kLinHead = 2048;         // barriers, row maxima and scales
 constexpr int kLinSmem = 226 * 1024;
@@ -143,11 +142,11 @@ __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, 
   }
 }
 
-template <int QT, int NBG, int G>
+template <int QT, int NBG, int G, int U>
 __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs A) {
   using Tr = QTraits<QT>;
   using Cfg = LinCfg<NBG, G>;
-  constexpr int U = kLinU, TB = Tr::kTileBytes, STAGE = 2 * U * TB, NRED = Cfg::kRed;
+  constexpr int TB = Tr::kTileBytes, STAGE = 2 * U * TB, NRED = Cfg::kRed;
   constexpr int TOK = Cfg::kTok;
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* const bars_all = reinterpret_cast<uint64_t*>(smem);
@@ -236,7 +235,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
         __syncwarp();
         const uint8_t* st = ring + slot * STAGE;
         const uint8_t* xq = xl + j * (U * 2 * G * 512);
-        const int left = nt - j * U;             // tiles of the stage, 2 or more: both
+        const int left = nt - j * U;             // tiles of the stage, U or more: all
         float c[2][G][4];
         auto begin = [&]() {                     // of a group of blocks
 #pragma unroll
@@ -258,10 +257,10 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
             }
           }
         };
-        if (NBG == 4) begin();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (u == 0 || u < left) {
+            if (NBG == 4 && u % 2 == 0) begin();
             TileRegs<QT> w[2];
 #pragma unroll
             for (int s = 0; s < 2; ++s) lds_quants<QT>(w[s], st + (s * U + u) * TB, lane);
@@ -286,8 +285,10 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
             }
             if (NBG == 2) finish(u, t >> 1, true);
           }
+          // four blocks: the lane's is in tile t / 2 of the two
+          if (NBG == 4 && u % 2 == 1 && u - 1 < left)
+            finish(u - 1 + (t >> 1), t & 1, u - 1 + (t >> 1) < left);
         }
-        if (NBG == 4) finish(t >> 1, t & 1, (t >> 1) < left);
         __syncwarp();                            // the stage has been read
         if (issued < total && !*dead) issue();
         if (++slot == A.nst) {
@@ -387,13 +388,13 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
 inline int linear_tps(int kt, int cs) { return ((kt + cs - 1) / cs + 1) / 2 * 2; }
 
 // Shared memory of a split; nst ring stages take what is left.
-template <int QT, int NBG, int G>
+template <int QT, int NBG, int G, int U>
 static size_t linear_smem(int kt, int cs, int ks, int nst) {
   using Cfg = LinCfg<NBG, G>;
   const size_t nred = (size_t)Cfg::kRed * 4;
   return kLinHead + (size_t)linear_tps(kt, cs) * Cfg::kTileBytes + (ks > 1 ? kLinWarps * nred : 0) +
          (cs > 1 ? 2 * (kLinWarps / ks) * nred : 0) +
-         (size_t)kLinWarps * nst * 2 * kLinU * QTraits<QT>::kTileBytes;
+         (size_t)kLinWarps * nst * 2 * U * QTraits<QT>::kTileBytes;
 }
 
 // Clusters of cs CTAs that are resident at once (a cluster stays inside one GPC:
@@ -424,10 +425,10 @@ static int resident_clusters(const void* kern, int cs, int dev) {
   return n;
 }
 
-template <int QT, int NBG, int G>
+template <int QT, int NBG, int G, int U>
 static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
   using Cfg = LinCfg<NBG, G>;
-  auto kern = linear_kernel<QT, NBG, G>;
+  auto kern = linear_kernel<QT, NBG, G, U>;
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
   MOE_CUDA(cudaGetDevice(&dev));
@@ -450,7 +451,7 @@ static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
     for (int cs = 1; cs <= 8; cs *= 2) {
       const int resident = resident_clusters((const void*)kern, cs, dev);
       for (int ks = 1; ks <= kLinWarps; ks *= 2) {
-        if (linear_smem<QT, NBG, G>(a.kt, cs, ks, 2) > kLinSmem) continue;
+        if (linear_smem<QT, NBG, G, U>(a.kt, cs, ks, 2) > kLinSmem) continue;
         const int tps = linear_tps(a.kt, cs), wt = ((tps + ks - 1) / ks + 1) / 2 * 2;
         const int slots = resident * (kLinWarps / ks);
         const int rounds = (a.pairs + slots - 1) / slots;
@@ -466,7 +467,7 @@ static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
     }
     plan.nst = 2;
     while (plan.cs > 0 && plan.nst < kLinMaxStages &&
-           linear_smem<QT, NBG, G>(a.kt, plan.cs, plan.ks, plan.nst + 1) <= kLinSmem)
+           linear_smem<QT, NBG, G, U>(a.kt, plan.cs, plan.ks, plan.nst + 1) <= kLinSmem)
       ++plan.nst;
   }
   fits = plan.cs > 0;
@@ -481,7 +482,7 @@ static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * a.cs), (unsigned)((a.T + Cfg::kRows - 1) / Cfg::kRows));
   cfg.blockDim = dim3(kLinWarps * 32);
-  cfg.dynamicSmemBytes = linear_smem<QT, NBG, G>(a.kt, a.cs, a.ks, a.nst);
+  cfg.dynamicSmemBytes = linear_smem<QT, NBG, G, U>(a.kt, a.cs, a.ks, a.nst);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -501,11 +502,14 @@ static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
 template <int QT>
 static int launch_linear_qt(LinArgs& a, cudaStream_t s) {
   bool fits = false;
-  if (a.T > 8) MOE_CHECK((launch_linear<QT, 1, 4>(a, s, fits)));
-  if (!fits && a.T > 4) MOE_CHECK((launch_linear<QT, 1, 2>(a, s, fits)));
-  if (!fits && a.T > 2) MOE_CHECK((launch_linear<QT, 1, 1>(a, s, fits)));
-  if (!fits && a.T == 2) MOE_CHECK((launch_linear<QT, 2, 1>(a, s, fits)));
-  if (!fits && a.T == 1) MOE_CHECK((launch_linear<QT, 4, 1>(a, s, fits)));
+  if (a.T > 8) MOE_CHECK((launch_linear<QT, 1, 4, 2>(a, s, fits)));
+  if (!fits && a.T > 4) MOE_CHECK((launch_linear<QT, 1, 2, 2>(a, s, fits)));
+  if (!fits && a.T > 2) MOE_CHECK((launch_linear<QT, 1, 1, 2>(a, s, fits)));
+  if (!fits && a.T == 2) MOE_CHECK((launch_linear<QT, 2, 1, 2>(a, s, fits)));
+  // one row of 4-bit weights is bound by instructions: twice the tiles per wait
+  if (QT == MOE_Q4_0 && a.T == 1 && a.pairs >= 2048)
+    MOE_CHECK((launch_linear<QT, 4, 1, 4>(a, s, fits)));
+  if (!fits && a.T == 1) MOE_CHECK((launch_linear<QT, 4, 1, 2>(a, s, fits)));
   MOE_REQUIRE(fits, MOE_ERR_UNSUPPORTED, "cols %d: rows of x this wide do not fit", a.cols);
   return MOE_OK;
 }
