@@ -476,7 +476,8 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
  *      strides (elements); residual may be y itself with the same stride;
  *      y must not overlap x or w
  * Made for a few rows: the weights are read once for every 16 of them (8 or 4
- * where x is so wide that 16 do not fit).  Should a copy never arrive, y is NaN. */
+ * where x is so wide that 16 do not fit).  32768 columns always fit; much wider
+ * ones are MOE_ERR_UNSUPPORTED.  Should a copy never arrive, y is NaN. */
 int moe_linear(const uint8_t* w, int qtype, int rows, int cols, const float* x, int64_t x_stride,
                int T, const float* residual, int64_t residual_stride, float* y, int64_t y_stride,
                moe_stream_t stream);

@@ -243,7 +243,6 @@ struct AttShared {
   long long base, scan[4];
   int seq, last, dead;
   uint64_t bars[4][5];               // a barrier per ring slot
-  uint32_t seen[4][8];               // valid keys of the tiles in each warp's ring
   float m[4][kAttHeads], l[4][kAttHeads], qmax[4][kAttHeads], qscale[kAttHeads];
 };
 
@@ -373,7 +372,6 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   const int step_pages = RK / ps, step_slots = RK - step_pages * ps;   // from tile to tile
   Cursor W = C;                                  // of the loads
   int wtiles = tiles(W), wend = keys_end(W), wkey = tile0(W), li = 0, lslot = 0;
-  uint32_t ltile = 0;
   bool wmore = true;
   // of this lane's box of tile li: number in the sequence's pages and slot,
   // row of the tensor map
@@ -399,9 +397,10 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     in = wmore && lane < boxes && key < wend && key + box > W.first;
     if (in) page = A.c.block_table[(int64_t)W.seq * A.c.table_stride + pidx];
   };
-  auto copy = [&](const CUtensorMap* map, int n) {
+  uint32_t bytes = 0;                            // of the tile's boxes that exist
+  auto copy = [&](const CUtensorMap* map) {
     uint64_t* bar = &sh.bars[warp][lslot];
-    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(n * BLOCKS * LINE) << A.box_shift);
+    if (lane == 0) mbar_expect_tx(bar, bytes);
     __syncwarp();
     if (in) {
       const uint32_t dst = ring_a + lslot * Cfg::kSlot + (lane << A.box_shift) * LINE;
@@ -412,28 +411,28 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     }
     lslot = lslot + 1 == NS ? 0 : lslot + 1;
   };
-  uint32_t lok = 0;                              // boxes of the tile that exist
-  auto issue_keys = [&]() {
-    if (!wmore) return;
+  auto issue_keys = [&]() -> uint32_t {          // which keys of the tile are valid
+    if (!wmore) return 0u;
     if (in && (page < 0 || page >= A.c.pages)) {
       set_status(A.status, MOE_STATUS_BAD_PAGE);
       in = false;
     }
     row = page * A.page_units + W.head * A.head_units;
-    lok = __ballot_sync(0xffffffffu, in);
+    const uint32_t ok = __ballot_sync(0xffffffffu, in);
+    const int n = __popc(ok);
     uint32_t seen = 0xffffffffu;
-    if (__popc(lok) != boxes || wkey < W.first || wkey + KEYS > wend) {
+    if (n != boxes || wkey < W.first || wkey + KEYS > wend) {
       const int r = lane & (KEYS - 1);
       seen = __ballot_sync(0xffffffffu, wkey + r >= W.first && wkey + r < wend &&
-                                            ((lok >> (r >> A.box_shift)) & 1u));
+                                            ((ok >> (r >> A.box_shift)) & 1u));
     }
-    if (lane == 0) sh.seen[warp][ltile & 7] = seen;
-    ++ltile;
-    copy(&kmap, __popc(lok));
+    bytes = (uint32_t)(n * BLOCKS * LINE) << A.box_shift;
+    copy(&kmap);
+    return seen;
   };
   auto issue_values = [&]() {
     if (!wmore) return;
-    copy(&vmap, __popc(lok));
+    copy(&vmap);
     ++li;
     key += RK;
     wkey += RK;
@@ -467,9 +466,11 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   enter();
   settle();
   fetch();
+  constexpr int AHEAD = (NS - 1) / 2;            // tiles under way
+  uint32_t seen_of[AHEAD];
 #pragma unroll
-  for (int i = 0; i < (NS - 1) / 2; ++i) {
-    issue_keys();
+  for (int i = 0; i < AHEAD; ++i) {
+    seen_of[i] = issue_keys();
     issue_values();
   }
 
@@ -531,7 +532,6 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     }
   };
 
-  uint32_t ctile = 0;
   q_fetch(C);
   q_max();
   __syncthreads();
@@ -571,8 +571,9 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       o[c][0] = o[c][1] = 0.f;
       acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
     }
-    // m: reference of the exponentials, 2^8 below the maximum at most; l: sum
-    // over this lane's keys
+    // m: reference of the exponentials, 2^8 below the maximum at most (it moves
+    // up seldom, so a tile's maximum is not shared between lanes until it has to);
+    // l: sum over this lane's keys
     float m = -INFINITY, l = 0.f;
     auto fold = [&](float f) {                   // o = (o + acc) * f
 #pragma unroll
@@ -585,9 +586,10 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 
     for (int i = 0; i < ntile; ++i) {
       const uint32_t ka = wait_slot();
-      issue_keys();
-      const uint32_t seen = sh.seen[warp][ctile & 7];
-      ++ctile;
+      const uint32_t seen = seen_of[0];
+#pragma unroll
+      for (int k = 0; k + 1 < AHEAD; ++k) seen_of[k] = seen_of[k + 1];
+      seen_of[AHEAD - 1] = issue_keys();
 
       // scores: keys 8b + 2t, 8b + 2t + 1 of head g in this lane.  Columns past
       // head_dim are zeros in the ring and in q
@@ -699,9 +701,9 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       float mx = -INFINITY;
 #pragma unroll
       for (int b = 0; b < KEYS / 8; ++b) mx = fmaxf(mx, fmaxf(x[b][0], x[b][1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * x2;
-      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+      if (__any_sync(0xffffffffu, mx * x2 > m + 8.f)) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * x2;
         const float to = mx > m + 8.f ? mx : m;
         const float f = to == -INFINITY ? 1.f : ex2(m - to);
         fold(f);

@@ -498,18 +498,22 @@ static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
 }
 
 // Rows of a pass: as many as T needs (1, 2, 4, 8 or 16), fewer where x is so wide
-// that their fragments do not fit.
+// that their fragments do not fit.  Up to 4 rows of 4-bit weights are bound by
+// instructions, so four tiles are taken per wait where the ring fits (65536 x
+// 2816: 1 row 25.7 -> 22.9 us, 4 rows 28.1 -> 24.9 us; 8 rows, nearer the MMAs'
+// bound, 36.5 -> 37.4 us).
 template <int QT>
 static int launch_linear_qt(LinArgs& a, cudaStream_t s) {
+  constexpr int U = QT == MOE_Q4_0 ? 4 : 2;
   bool fits = false;
   if (a.T > 8) MOE_CHECK((launch_linear<QT, 1, 4, 2>(a, s, fits)));
   if (!fits && a.T > 4) MOE_CHECK((launch_linear<QT, 1, 2, 2>(a, s, fits)));
-  if (!fits && a.T > 2) MOE_CHECK((launch_linear<QT, 1, 1, 2>(a, s, fits)));
-  if (!fits && a.T == 2) MOE_CHECK((launch_linear<QT, 2, 1, 2>(a, s, fits)));
-  // one row of 4-bit weights is bound by instructions: twice the tiles per wait
-  if (QT == MOE_Q4_0 && a.T == 1 && a.pairs >= 2048)
-    MOE_CHECK((launch_linear<QT, 4, 1, 4>(a, s, fits)));
-  if (!fits && a.T == 1) MOE_CHECK((launch_linear<QT, 4, 1, 2>(a, s, fits)));
+  if (!fits && a.T > 2) MOE_CHECK((launch_linear<QT, 1, 1, U>(a, s, fits)));
+  if (!fits && a.T > 2 && U > 2) MOE_CHECK((launch_linear<QT, 1, 1, 2>(a, s, fits)));
+  if (!fits && a.T == 2) MOE_CHECK((launch_linear<QT, 2, 1, U>(a, s, fits)));
+  if (!fits && a.T == 2 && U > 2) MOE_CHECK((launch_linear<QT, 2, 1, 2>(a, s, fits)));
+  if (!fits && a.T == 1) MOE_CHECK((launch_linear<QT, 4, 1, U>(a, s, fits)));
+  if (!fits && a.T == 1 && U > 2) MOE_CHECK((launch_linear<QT, 4, 1, 2>(a, s, fits)));
   MOE_REQUIRE(fits, MOE_ERR_UNSUPPORTED, "cols %d: rows of x this wide do not fit", a.cols);
   return MOE_OK;
 }

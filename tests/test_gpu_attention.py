@@ -468,7 +468,8 @@ def test_linear(qtype, T, rows, cols):
 @pytest.mark.parametrize("qtype", [2, 8])
 @pytest.mark.parametrize("T,rows,cols", [(1, 6144, 2816), (1, 20011, 1024), (4, 2816, 8192),
                                          (16, 4096, 8192), (9, 513, 12288), (1, 64, 32768),
-                                         (16, 64, 32768), (33, 1024, 2816), (6, 40000, 512)])
+                                         (16, 64, 32768), (33, 1024, 2816), (6, 40000, 512), (3, 40, 32768),
+                                         (7, 33, 32768)])
 def test_linear_wide(qtype, T, rows, cols):
     rng = np.random.default_rng(cols)
     raw, w, big = matrix(rng, qtype, rows, cols)
@@ -477,6 +478,22 @@ def test_linear_wide(qtype, T, rows, cols):
     res = rng.standard_normal((T, rows), dtype=np.float32)
     y = K.linear(torch.from_numpy(x).cuda(), lw, residual=torch.from_numpy(res).cuda())
     check_linear(y.cpu().numpy(), x, w, big, res)
+
+
+@pytest.mark.parametrize("T", [1, 2, 7])
+def test_linear_widest(T):
+    """Columns that leave room for fewer rows and tiles at a time, and more
+    than fit at all."""
+    rng = np.random.default_rng(7)
+    raw, w, big = matrix(rng, 2, 40, 65536)
+    lw = K.LinearWeights(torch.from_numpy(raw.reshape(-1)).cuda(), 2, 40, 65536)
+    x = rng.standard_normal((T, 65536), dtype=np.float32)
+    check_linear(K.linear(torch.from_numpy(x).cuda(), lw).cpu().numpy(), x, w, big)
+    for qtype in (2, 8):
+        wide = K.LinearWeights(torch.zeros(16 * (1 << 20) // 32 * synth.block_bytes(qtype),
+                                           dtype=torch.uint8, device="cuda"), qtype, 16, 1 << 20)
+        with pytest.raises(_lib.MoEError, match="do not fit"):
+            K.linear(torch.zeros((T, 1 << 20), device="cuda"), wide)
 
 
 def test_linear_many_rows():
