@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
 
   // ---- weights: stage q of this warp is tiles [wt0 + j U, ..) of pair `p`
   const int nsr = (nt + U - 1) / U;              // stages of a pair
-  const int p0 = cluster * groups + group, pstep = nclusters * groups;
+  // pairs go round the clusters, so that few of them still use every SM
+  const int p0 = group * nclusters + cluster, pstep = nclusters * groups;
   const int mine = p0 < A.pairs ? (A.pairs - p0 + pstep - 1) / pstep : 0;
   const int total = mine * nsr;
   const uint64_t pol = evict_first_policy();
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
               mine_p[group * NRED + ((s * G + cg) * 2 + i) * 32 + lane] = v[s][cg][i];
       cluster_sync();
       for (int e = rank * kLinWarps * 32 + tid; e < groups * NRED; e += A.cs * kLinWarps * 32) {
-        const int pe = cluster * groups + e / NRED + r * pstep, k = e % NRED / 32;
+        const int pe = e / NRED * nclusters + cluster + r * pstep, k = e % NRED / 32;
         const uint32_t a = smem_u32(mine_p + e);
         float f[8];
 #pragma unroll
@@ -477,7 +478,7 @@ static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
   a.nst = plan.nst;
   a.tps = linear_tps(a.kt, a.cs);
   const int per = kLinWarps / a.ks;                  // pairs of a cluster's round
-  const int clusters = std::min(plan.clusters, (a.pairs + per - 1) / per);
+  const int clusters = std::min(plan.clusters, a.pairs);
   a.rounds = (a.pairs + clusters * per - 1) / (clusters * per);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * a.cs), (unsigned)((a.T + Cfg::kRows - 1) / Cfg::kRows));
