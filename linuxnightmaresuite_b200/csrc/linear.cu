@@ -18,6 +18,11 @@
 // cluster of cs CTAs splits the columns, so that each converts only its part of
 // x; their sums meet in distributed shared memory.  The split (cs, ks) is the
 // one with the least estimated time; sums are in a fixed order.
+//
+// Measured on a B200 (copy bandwidth 6.55 TB/s): 262144 x 2816 Q4_0 for one row 72
+// us (416 MB, 88 %), 65536 x 2816 for 1, 4, 8, 16 rows 22.6, 24.8, 35, 54 us (floor
+// 15.9), 6144 x 2816 for one row 6.3 us, of which 4 are launch, fragments and the
+// meeting of the warps.
 #include <algorithm>
 #include <atomic>
 
