@@ -98,6 +98,9 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -223,11 +226,11 @@ template <int DT, int DP, bool PACK> struct AttCfg {
   static constexpr int kRound = kTiles * kKeys;
   static constexpr int kRing = kWarps * kSlots * kSlot;
   static constexpr int kMergeRow = DP + 8;                  // floats
-  // one row per tile and head; when a unit's parts are joined first a weight per
-  // part and head, then four floats per thread and head
-  static constexpr int kMerge =
-      4 * kAttHeads * (kTiles * kMergeRow > 4 * 32 * kWarps ? kTiles * kMergeRow : 4 * 32 * kWarps);
-  static_assert(kMerge >= kAttParts * kAttHeads * 4, "weights of the parts");
+  // one row per tile and head; when a unit's parts are joined a weight per part
+  // and head, and four floats per thread
+  static constexpr int kRows = 4 * kAttHeads * kTiles * kMergeRow;
+  static constexpr int kJoin = 4 * kAttHeads * kAttParts + 16 * 32 * kWarps;
+  static constexpr int kMerge = kRows > kJoin ? kRows : kJoin;
   static constexpr int kQ = DP / 16 * Frag::kBytes;
   static constexpr int kX = kSplit > 1 ? kWarps * 32 * (kKeys / 4) * 4 : 0;   // halves of scores
   static constexpr int kSmem = kRing + kMerge + kQ + kX;
@@ -247,18 +250,19 @@ __device__ __forceinline__ uint32_t slot_at(int r, int c) {
   return (uint32_t)((c >> 3) * KEYS * kLine + r * kLine + (((c & 7) ^ (r & 7)) << 4));
 }
 
-struct AttShared {
-  long long base, scan[4];
-  int seq, last, dead;
-  uint64_t bars[4][5];               // a barrier per ring slot
-  float m[4][kAttHeads], l[4][kAttHeads], qmax[4][kAttHeads], qscale[kAttHeads];
-};
-
 // A cursor over a CTA's pieces: rounds r0 .. r1 of R of unit u of a sequence.
 struct Cursor {
   int seq, u, head, group;           // unit: key head and group of query heads
   int at, r0, r1, R;                 // `at`: cost at which the unit's rounds begin
   int len, first, from;              // the sequence's keys first .. len, rounds from `from` on
+};
+
+struct AttShared {
+  Cursor first;                      // a piece that waits for its join
+  long long base, scan[4];
+  int seq, dead, join[2];            // join: of the last piece, of the first
+  uint64_t bars[4][5];               // a barrier per ring slot
+  float m[4][kAttHeads], l[4][kAttHeads], qmax[4][kAttHeads], qscale[kAttHeads];
 };
 
 template <int DT, int DP, bool PACK>
@@ -278,6 +282,10 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   if (lane < NS) {
     mbar_init(&sh.bars[warp][lane], 1);
     fence_mbar_init();
+  }
+  if (tid == 0) {
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
   }
   pdl_trigger();
   pdl_wait();
@@ -315,7 +323,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     if (w < warp) before += sh.scan[w];
     total += sh.scan[w];
   }
-  if (tid == 0) sh.dead = 0;
+  if (tid == 0) sh.dead = sh.join[0] = sh.join[1] = 0;
   const int quota = (int)((total + gridDim.x - 1) / gridDim.x);
   const long long start = (long long)blockIdx.x * quota;
   if (start >= total) return;
@@ -371,6 +379,67 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     const int n = keys_end(c) - tile0(c);
     return n > 0 ? (n + RK - 1) / RK : 0;
   };
+
+  // ---- q: this thread's values of the next piece's operand (k16 steps warp,
+  // warp + NW, ...), fetched a piece ahead; columns 2t, 2t+1, 2t+8, 2t+9 of a
+  // step, but for e4m3 keys, which are read four bytes per lane: 4t .. 4t+3
+  constexpr int QK = DP / 16 / NW;
+  uint8_t* const qs = smem + Cfg::kRing + Cfg::kMerge;
+  float* const mo = reinterpret_cast<float*>(smem + Cfg::kRing);
+  const uint8_t* const qw = qs + warp % SP * (DH / 16) * Frag::kBytes;   // this warp's columns
+  float4* const xs = reinterpret_cast<float4*>(smem + Cfg::kRing + Cfg::kMerge + Cfg::kQ);
+  float qn[QK][4];
+  auto first_head = [&](const Cursor& c) { return c.head * G + c.group * kAttHeads; };
+  auto heads = [&](const Cursor& c) { return min(kAttHeads, G - c.group * kAttHeads); };
+  auto q_fetch = [&](const Cursor& c) {
+    const int head = PACK ? g & 3 : g, nh = heads(c);
+    const float* q = A.q + (int64_t)c.seq * A.q_ss + (int64_t)(first_head(c) + head) * A.q_hs;
+#pragma unroll
+    for (int i = 0; i < QK; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = 16 * (warp + i * NW) +
+                      (Cfg::kElem == 1 ? 4 * t + j : 2 * t + (j & 1) + 8 * (j >> 1));
+        qn[i][j] = head < nh && e < D ? q[e] : 0.f;
+      }
+  };
+  auto q_max = [&]() {
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < QK; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fabsf(qn[i][j]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    if (t == 0) sh.qmax[warp][g] = mx;
+  };
+  auto q_split = [&]() {                         // scaled by a power of two to [2^10, 2^11)
+    float mx = sh.qmax[0][g];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, sh.qmax[w][g]);
+    // 2^e in two factors, since e may lie outside the exponents of a float
+    const int ex = (int)(__float_as_uint(mx) >> 23);           // 0 .. 255
+    const int e = mx > 0.f && ex < 255 ? 137 - max(ex, 1) : 0;
+    const int e1 = e / 2, e2 = e - e1;
+    const float f1 = __uint_as_float((uint32_t)(127 + e1) << 23);
+    const float f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
+    // a negative scale turns q; one that vanishes stays above zero, so that it
+    // leaves the minus infinity of a key that is not seen what it is
+    const float sign = A.scale < 0.f ? -1.f : 1.f;
+    if (warp == 0 && t == 0)
+      sh.qscale[g] = fmaxf(ldexpf(fabsf(A.scale) * A.c.k_scale, -e), 1e-30f);
+#pragma unroll
+    for (int i = 0; i < QK; ++i) {
+      Frag f;
+      const float f0 = f1 * sign;
+      f.set(qn[i][0] * f0 * f2, qn[i][1] * f0 * f2, qn[i][2] * f0 * f2, qn[i][3] * f0 * f2,
+            g);
+      f.store(qs + (warp + i * NW) * Frag::kBytes, lane);
+    }
+  };
+
+  // the first q before the ring's copies: behind them it would arrive last
+  q_fetch(C);
 
   // ---- loads: a cursor of its own that runs ahead of the arithmetic, across
   // the ends of units
@@ -482,65 +551,6 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     issue_values();
   }
 
-  // ---- q: this thread's values of the next piece's operand (k16 steps warp,
-  // warp + NW, ...), fetched a piece ahead; columns 2t, 2t+1, 2t+8, 2t+9 of a
-  // step, but for e4m3 keys, which are read four bytes per lane: 4t .. 4t+3
-  constexpr int QK = DP / 16 / NW;
-  uint8_t* const qs = smem + Cfg::kRing + Cfg::kMerge;
-  float* const mo = reinterpret_cast<float*>(smem + Cfg::kRing);
-  const uint8_t* const qw = qs + warp % SP * (DH / 16) * Frag::kBytes;   // this warp's columns
-  float4* const xs = reinterpret_cast<float4*>(smem + Cfg::kRing + Cfg::kMerge + Cfg::kQ);
-  float qn[QK][4];
-  auto first_head = [&](const Cursor& c) { return c.head * G + c.group * kAttHeads; };
-  auto heads = [&](const Cursor& c) { return min(kAttHeads, G - c.group * kAttHeads); };
-  auto q_fetch = [&](const Cursor& c) {
-    const int head = PACK ? g & 3 : g, nh = heads(c);
-    const float* q = A.q + (int64_t)c.seq * A.q_ss + (int64_t)(first_head(c) + head) * A.q_hs;
-#pragma unroll
-    for (int i = 0; i < QK; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = 16 * (warp + i * NW) +
-                      (Cfg::kElem == 1 ? 4 * t + j : 2 * t + (j & 1) + 8 * (j >> 1));
-        qn[i][j] = head < nh && e < D ? q[e] : 0.f;
-      }
-  };
-  auto q_max = [&]() {
-    float mx = 0.f;
-#pragma unroll
-    for (int i = 0; i < QK; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fabsf(qn[i][j]));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    if (t == 0) sh.qmax[warp][g] = mx;
-  };
-  auto q_split = [&]() {                         // scaled by a power of two to [2^10, 2^11)
-    float mx = sh.qmax[0][g];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, sh.qmax[w][g]);
-    // 2^e in two factors, since e may lie outside the exponents of a float
-    const int ex = (int)(__float_as_uint(mx) >> 23);           // 0 .. 255
-    const int e = mx > 0.f && ex < 255 ? 137 - max(ex, 1) : 0;
-    const int e1 = e / 2, e2 = e - e1;
-    const float f1 = __uint_as_float((uint32_t)(127 + e1) << 23);
-    const float f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
-    // a negative scale turns q; one that vanishes stays above zero, so that it
-    // leaves the minus infinity of a key that is not seen what it is
-    const float sign = A.scale < 0.f ? -1.f : 1.f;
-    if (warp == 0 && t == 0)
-      sh.qscale[g] = fmaxf(ldexpf(fabsf(A.scale) * A.c.k_scale, -e), 1e-30f);
-#pragma unroll
-    for (int i = 0; i < QK; ++i) {
-      Frag f;
-      const float f0 = f1 * sign;
-      f.set(qn[i][0] * f0 * f2, qn[i][1] * f0 * f2, qn[i][2] * f0 * f2, qn[i][3] * f0 * f2,
-            g);
-      f.store(qs + (warp + i * NW) * Frag::kBytes, lane);
-    }
-  };
-
-  q_fetch(C);
   q_max();
   __syncthreads();
   q_split();
@@ -562,6 +572,25 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   constexpr int PPL = LINE / 32;                 // chunk pairs of a line
   auto beyond = [](int j, int kb) { return (uint32_t)((j / PPL) * KEYS * LINE + kb * 16 * LINE); };
 
+  // The piece's unit: its rounds begin in CTA c0 and go on in n - 1 more
+  auto spread = [&](const Cursor& c, int& c0) {
+    const int back = c.at < 0 ? (quota - 1 - c.at) / quota : 0;
+    c0 = blockIdx.x - back;
+    return (c.at + back * quota + c.R - 1) / quota + 1;
+  };
+  auto arrive = [&](const Cursor& c) {           // true: the last of its unit
+    int c0, arrived;
+    const int n = spread(c, c0);
+    // releases this CTA's partials, acquires those of the others
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;"
+                 : "=r"(arrived)
+                 : "l"(A.arrivals + c0)
+                 : "memory");
+    if (arrived != n - 1) return false;
+    A.arrivals[c0] = 0;
+    return true;
+  };
+
   for (;;) {
     // the piece after this one, and its q
     Cursor N = C;
@@ -570,7 +599,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     const int ntile = tiles(C);
 
     const float qscale = sh.qscale[g];           // score = product * qscale
-    const float to_cap = qscale / A.cap, from_cap = A.cap * kLog2e;   // with a cap only
+    const float to_cap = A.cap > 0.f ? qscale / A.cap : 0.f, from_cap = A.cap * kLog2e;
     const float x2 = A.cap > 0.f ? 1.f : qscale * kLog2e;
     float o[DH / 8][2];                          // head g, two columns of each 8-wide block
     float acc[DH / 8][4];
@@ -789,13 +818,12 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     {
       float* row = mo + (warp / SP * kAttHeads + g) * Cfg::kMergeRow + warp % SP * DH;
 #pragma unroll
-      for (int c = 0; c < DH / 8; ++c) {
-        if (Cfg::kElem == 2) {
+      for (int c = 0; c < DH / 8; c += 3 - Cfg::kElem) {
+        if (Cfg::kElem == 2)
           *reinterpret_cast<float2*>(row + 8 * c + 2 * t) = make_float2(o[c][0], o[c][1]);
-        } else {                                 // block 2c: even columns 4t, 4t + 2; 2c + 1: odd
-          row[16 * (c >> 1) + 4 * t + (c & 1)] = o[c][0];
-          row[16 * (c >> 1) + 4 * t + 2 + (c & 1)] = o[c][1];
-        }
+        else                                     // block c: even columns 4t, 4t + 2; c + 1: odd
+          *reinterpret_cast<float4*>(row + 8 * c + 4 * t) =
+              make_float4(o[c][0], o[c + 1][0], o[c][1], o[c + 1][1]);
       }
     }
     if (more) q_max();
@@ -825,97 +853,118 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         A.part_ml[my_slot * kAttHeads + h] = make_float2(M, L);
       }
       float* to = whole ? A.out + (row0 + h) * D : A.part_o + ((int64_t)my_slot * kAttHeads + h) * DP;
-      for (int c = lane; c < D; c += 32) {
+#pragma unroll
+      for (int c = lane; c < DP; c += 32) {
         float y = 0.f;
 #pragma unroll
         for (int w = 0; w < NG; ++w)
           y = fmaf(mo[(w * kAttHeads + h) * Cfg::kMergeRow + c], f[w], y);
-        to[c] = y;
+        if (c < D) to[c] = y;
       }
     }
     if (more) q_split();
-    if (!whole) {
-      // ---- the last CTA of a unit to arrive joins the unit's parts, in order
-      const long long ustart = start + C.at;
-      const int c0 = (int)(ustart / quota), n = (int)((ustart + C.R - 1) / quota) - c0 + 1;
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();
-        const int arrived = atomicAdd(A.arrivals + c0, 1);
-        sh.last = arrived == n - 1;
-        if (sh.last) A.arrivals[c0] = 0;
-        __threadfence();
-      }
-      __syncthreads();
-      if (sh.last) {
-        // weights of the parts, [part][head]; mo is free again
-        const int64_t slot0 = 2 * (int64_t)c0;   // part i: slot0 + 2 i, part 0: slot0 + 1
-        for (int h = warp; h < nh; h += NW) {
-          float2 v[kAttParts / 32];
-          float M = -INFINITY, L = 0.f;
-#pragma unroll
-          for (int k = 0; k < kAttParts / 32; ++k) {
-            const int i = lane + 32 * k;
-            v[k] = i < n ? __ldcg(A.part_ml + (slot0 + 2 * i + (i == 0)) * kAttHeads + h)
-                         : make_float2(-INFINITY, 0.f);
-          }
-#pragma unroll
-          for (int k = 0; k < kAttParts / 32; ++k) M = fmaxf(M, v[k].x);
-#pragma unroll
-          for (int b = 16; b > 0; b >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, b));
-          const float ms = M == -INFINITY ? 0.f : M;
-#pragma unroll
-          for (int k = 0; k < kAttParts / 32; ++k) {
-            v[k].x = ex2(v[k].x - ms);
-            L = fmaf(v[k].y, v[k].x, L);
-          }
-#pragma unroll
-          for (int b = 16; b > 0; b >>= 1) L += __shfl_xor_sync(0xffffffffu, L, b);
-          const float norm = L == 0.f ? 0.f : unit / L;
-#pragma unroll
-          for (int k = 0; k < kAttParts / 32; ++k)
-            if (lane + 32 * k < n) mo[(lane + 32 * k) * kAttHeads + h] = v[k].x * norm;
-          if (lane == 0 && A.lse) A.lse[row0 + h] = (M + (log2f(L) - kPShift)) * kLn2;
-        }
-        __syncthreads();
-        // thread: four columns of every PL-th part, all heads
-        constexpr int CT = DP / 4, PL = NT / CT;
-        const int col = tid % CT, pl = tid / CT;
-        float4 y[kAttHeads];
-#pragma unroll
-        for (int h = 0; h < kAttHeads; ++h) y[h] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-        for (int i = pl; i < n; i += PL) {
-          const float4* po = reinterpret_cast<const float4*>(
-              A.part_o + (slot0 + 2 * i + (i == 0)) * kAttHeads * DP) + col;
-#pragma unroll
-          for (int h = 0; h < kAttHeads; ++h)
-            if (h < nh) {
-              const float4 v = __ldcg(po + h * CT);
-              const float w = mo[i * kAttHeads + h];
-              y[h].x = fmaf(v.x, w, y[h].x);
-              y[h].y = fmaf(v.y, w, y[h].y);
-              y[h].z = fmaf(v.z, w, y[h].z);
-              y[h].w = fmaf(v.w, w, y[h].w);
-            }
-        }
-        __syncthreads();                         // the weights are done with
-#pragma unroll
-        for (int h = 0; h < kAttHeads; ++h)
-          if (h < nh) reinterpret_cast<float4*>(mo)[(pl * kAttHeads + h) * CT + col] = y[h];
-        __syncthreads();
-        for (int e = tid; e < nh * DP; e += NT) {
-          const int h = e / DP, c = e % DP;
-          float v = mo[h * DP + c];
-#pragma unroll
-          for (int k = 1; k < PL; ++k) v += mo[(k * kAttHeads + h) * DP + c];
-          if (c < D) A.out[(row0 + h) * D + c] = v;
-        }
-      }
+    __syncthreads();                             // q of the next piece; mo and sh are free
+    // Parts of units are announced as they are written; units that turn out to
+    // be complete are joined behind the loop.  Only a CTA's first piece and its
+    // last can be parts.
+    if (!whole && tid == 0) {
+      const bool last = arrive(C);
+      if (last && more) sh.first = C;
+      sh.join[more] = last;
     }
     if (!more) break;
-    __syncthreads();                             // q of the next piece; mo and sh are free
     C = N;
+  }
+  __syncthreads();
+  for (int k = 0; k < 2; ++k) {
+    if (!sh.join[k]) continue;
+    if (k) {
+      __syncthreads();                           // mo is free again
+      C = sh.first;
+    }
+    int c0;
+    const int n = spread(C, c0), nh = heads(C);
+    const int64_t row0 = (int64_t)C.seq * A.hq + first_head(C);
+    // thread: four columns of a head, of every PL-th part; the first loads
+    // go out before the weights are known
+    constexpr int CT = DP / 4, U = 16;
+    const int HW = min(nh <= 1 ? 1 : nh <= 2 ? 2 : nh <= 4 ? 4 : 8, NT / CT);
+    const int PL = NT / (CT * HW);
+    const int col = tid % CT, hw = tid / CT % HW, pl = tid / (CT * HW);
+    const int64_t slot0 = 2 * (int64_t)c0;   // part i: slot0 + 2 i, part 0: slot0 + 1
+    float4 v4[U];
+    auto load = [&](int h, int i0) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + k * PL;
+        if (i < n)
+          v4[k] = __ldcg(reinterpret_cast<const float4*>(
+                             A.part_o + ((slot0 + 2 * i + (i == 0)) * kAttHeads + h) * DP) + col);
+      }
+    };
+    if (hw < nh) load(hw, pl);
+    // weights of the parts, [part][head]; mo is free again
+    for (int h = warp; h < nh; h += NW) {
+      float2 v[kAttParts / 32];
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int k = 0; k < kAttParts / 32; ++k) {
+        const int i = lane + 32 * k;
+        v[k] = i < n ? __ldcg(A.part_ml + (slot0 + 2 * i + (i == 0)) * kAttHeads + h)
+                     : make_float2(-INFINITY, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < kAttParts / 32; ++k) M = fmaxf(M, v[k].x);
+#pragma unroll
+      for (int b = 16; b > 0; b >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, b));
+      const float ms = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int k = 0; k < kAttParts / 32; ++k) {
+        v[k].x = ex2(v[k].x - ms);
+        L = fmaf(v[k].y, v[k].x, L);
+      }
+#pragma unroll
+      for (int b = 16; b > 0; b >>= 1) L += __shfl_xor_sync(0xffffffffu, L, b);
+      const float norm = L == 0.f ? 0.f : A.c.v_scale / L;
+#pragma unroll
+      for (int k = 0; k < kAttParts / 32; ++k)
+        if (lane + 32 * k < n) mo[(lane + 32 * k) * kAttHeads + h] = v[k].x * norm;
+      if (lane == 0 && A.lse) A.lse[row0 + h] = (M + (log2f(L) - kPShift)) * kLn2;
+    }
+    __syncthreads();
+    float* const sums = mo + kAttParts * kAttHeads;   // [pl][head][DP]
+    for (int h = hw; h < nh; h += HW) {
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i0 = pl; i0 < n; i0 += U * PL) {
+        if (h != hw || i0 != pl) load(h, i0);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const int i = i0 + k * PL;
+          if (i < n) {
+            const float w = mo[i * kAttHeads + h];
+            y.x = fmaf(v4[k].x, w, y.x);
+            y.y = fmaf(v4[k].y, w, y.y);
+            y.z = fmaf(v4[k].z, w, y.z);
+            y.w = fmaf(v4[k].w, w, y.w);
+          }
+        }
+      }
+      if (PL > 1) {
+        reinterpret_cast<float4*>(sums)[(pl * nh + h) * CT + col] = y;
+      } else {
+        float* to = A.out + (row0 + h) * D + 4 * col;
+        if (4 * col < D) to[0] = y.x, to[1] = y.y, to[2] = y.z, to[3] = y.w;
+      }
+    }
+    if (PL > 1) {
+      __syncthreads();
+      for (int e = tid; e < nh * DP; e += NT) {
+        const int h = e / DP, c = e % DP;
+        float v = sums[e];
+        for (int k = 1; k < PL; ++k) v += sums[(k * nh) * DP + e];
+        if (c < D) A.out[(row0 + h) * D + c] = v;
+      }
+    }
   }
   // after a timeout copies may still be under way: give them time to land
   if (*(volatile int*)&sh.dead)
