@@ -397,8 +397,8 @@ int moe_ep_forward_phases(const moe_layer_weights* w, int W, int rank, void* con
  * layout of a page fit.  Token position p of sequence s is in page
  * block_table[s * table_stride + p / page_size], slot p % page_size; entries
  * behind a sequence's last page are never read, and a page may belong to
- * several sequences.  Bases and strides must be multiples of 16 bytes; head_dim a multiple of 8 (16 for MOE_CACHE_E4M3), at
- * most 256.  MOE_CACHE_E4M3 holds value / scale, rounded to nearest even and
+ * several sequences.  Bases and strides must be multiples of 16 bytes; head_dim
+ * a multiple of 8 (16 for MOE_CACHE_E4M3), at most 256.  MOE_CACHE_E4M3 holds value / scale, rounded to nearest even and
  * saturated at +-448; the scales of the other types must be 1.
  * A page id outside [0, pages) sets MOE_STATUS_BAD_PAGE; its slots are neither
  * read nor written. */
@@ -481,6 +481,51 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
 int moe_linear(const uint8_t* w, int qtype, int rows, int cols, const float* x, int64_t x_stride,
                int T, const float* residual, int64_t residual_stride, float* y, int64_t y_stride,
                moe_stream_t stream);
+
+/* The same three calls with their arguments in one record, for callers to whom
+ * each argument of a foreign call costs time (0.1 us in Python, of a call of a
+ * few microseconds). */
+typedef struct moe_rope_append_args {
+  moe_paged_cache cache;
+  const float *q, *k, *v;
+  int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+  const int32_t *positions, *seq_ids;
+  const double* inv_freq;
+  float* q_out;
+  int64_t qo_tok_stride, qo_head_stride;
+  int32_t* status;
+  moe_stream_t stream;
+  int T, q_heads, rot, interleaved;
+} moe_rope_append_args;
+
+typedef struct moe_paged_attention_args {
+  moe_paged_cache cache;
+  const float* q;
+  int64_t q_seq_stride, q_head_stride;
+  const int32_t* seq_lens;
+  float *out, *lse;
+  void* workspace;
+  size_t workspace_bytes;
+  moe_stream_t stream;
+  int q_heads, max_len, window;
+  float scale, softcap;
+} moe_paged_attention_args;
+
+typedef struct moe_linear_args {
+  const uint8_t* w;
+  const float* x;
+  int64_t x_stride;
+  const float* residual;
+  int64_t residual_stride;
+  float* y;
+  int64_t y_stride;
+  moe_stream_t stream;
+  int qtype, rows, cols, T;
+} moe_linear_args;
+
+int moe_rope_append_record(const moe_rope_append_args* args);
+int moe_paged_attention_record(const moe_paged_attention_args* args);
+int moe_linear_record(const moe_linear_args* args);
 
 #ifdef __cplusplus
 }

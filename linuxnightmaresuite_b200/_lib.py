@@ -75,6 +75,37 @@ class MoEPagedCache(ctypes.Structure):
     ]
 
 
+class MoERopeAppendArgs(ctypes.Structure):
+    """Mirror of ``moe_rope_append_args``."""
+    _fields_ = [
+        ("cache", MoEPagedCache), ("q", vp), ("k", vp), ("v", vp), ("q_tok_stride", ci64),
+        ("q_head_stride", ci64), ("k_tok_stride", ci64), ("k_head_stride", ci64),
+        ("v_tok_stride", ci64), ("v_head_stride", ci64), ("positions", vp), ("seq_ids", vp),
+        ("inv_freq", vp), ("q_out", vp), ("qo_tok_stride", ci64), ("qo_head_stride", ci64),
+        ("status", vp), ("stream", vp), ("T", ci), ("q_heads", ci), ("rot", ci),
+        ("interleaved", ci),
+    ]
+
+
+class MoEPagedAttentionArgs(ctypes.Structure):
+    """Mirror of ``moe_paged_attention_args``."""
+    _fields_ = [
+        ("cache", MoEPagedCache), ("q", vp), ("q_seq_stride", ci64), ("q_head_stride", ci64),
+        ("seq_lens", vp), ("out", vp), ("lse", vp), ("workspace", vp), ("workspace_bytes", csz),
+        ("stream", vp), ("q_heads", ci), ("max_len", ci), ("window", ci), ("scale", cf),
+        ("softcap", cf),
+    ]
+
+
+class MoELinearArgs(ctypes.Structure):
+    """Mirror of ``moe_linear_args``."""
+    _fields_ = [
+        ("w", vp), ("x", vp), ("x_stride", ci64), ("residual", vp), ("residual_stride", ci64),
+        ("y", vp), ("y_stride", ci64), ("stream", vp), ("qtype", ci), ("rows", ci), ("cols", ci),
+        ("T", ci),
+    ]
+
+
 # name -> (argtypes) ; every function returns int
 SIGNATURES = {
     "moe_version": [],
@@ -121,6 +152,9 @@ SIGNATURES = {
     "moe_paged_attention": [vp, vp, ci64, ci64, vp, ci, ci, ci, cf, cf,
                             vp, vp, vp, csz, vp],
     "moe_linear": [vp, ci, ci, ci, vp, ci64, ci, vp, ci64, vp, ci64, vp],
+    "moe_rope_append_record": [vp],
+    "moe_paged_attention_record": [vp],
+    "moe_linear_record": [vp],
 }
 
 

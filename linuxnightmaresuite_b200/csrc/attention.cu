@@ -1133,4 +1133,11 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
   return moe::check_launch("paged_attention");
 }
 
+int moe_paged_attention_record(const moe_paged_attention_args* a) {
+  MOE_REQUIRE(a, MOE_ERR_INVALID, "null arguments");
+  return moe_paged_attention(&a->cache, a->q, a->q_seq_stride, a->q_head_stride, a->seq_lens,
+                             a->q_heads, a->max_len, a->window, a->scale, a->softcap, a->out,
+                             a->lse, a->workspace, a->workspace_bytes, a->stream);
+}
+
 }  // extern "C"

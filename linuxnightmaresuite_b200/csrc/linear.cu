@@ -559,3 +559,9 @@ extern "C" int moe_linear(const uint8_t* w, int qtype, int rows, int cols, const
   }
   return moe::check_launch("linear");
 }
+
+extern "C" int moe_linear_record(const moe_linear_args* a) {
+  MOE_REQUIRE(a, MOE_ERR_INVALID, "null arguments");
+  return moe_linear(a->w, a->qtype, a->rows, a->cols, a->x, a->x_stride, a->T, a->residual,
+                    a->residual_stride, a->y, a->y_stride, a->stream);
+}

@@ -226,4 +226,12 @@ int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_
   return moe::check_launch("rope_append");
 }
 
+int moe_rope_append_record(const moe_rope_append_args* a) {
+  MOE_REQUIRE(a, MOE_ERR_INVALID, "null arguments");
+  return moe_rope_append(&a->cache, a->q, a->q_tok_stride, a->q_head_stride, a->k, a->k_tok_stride,
+                         a->k_head_stride, a->v, a->v_tok_stride, a->v_head_stride, a->T,
+                         a->q_heads, a->positions, a->seq_ids, a->inv_freq, a->rot, a->interleaved,
+                         a->q_out, a->qo_tok_stride, a->qo_head_stride, a->status, a->stream);
+}
+
 }  // extern "C"

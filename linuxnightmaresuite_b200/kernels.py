@@ -266,15 +266,27 @@ CACHE_TYPES = {torch.float16: _lib.MOE_CACHE_F16, torch.bfloat16: _lib.MOE_CACHE
                torch.float8_e4m3fn: _lib.MOE_CACHE_E4M3}
 
 
-# A cache as the entry points read it (moe_paged_cache), packed in one step.
-_CACHE_STRUCT = struct.Struct("@3P4q7i2f0q")
-assert _CACHE_STRUCT.size == ctypes.sizeof(_lib.MoEPagedCache)
+# The arguments as the entry points read them (moe_*_args), packed in one step:
+# a ctypes call converts each argument at the price of packing five.
+_CACHE = "3P4q7i2f"
+_APPEND_ARGS = struct.Struct("@" + _CACHE + "3P6q4P2q2P4i0q")
+_ATTENTION_ARGS = struct.Struct("@" + _CACHE + "P2q4PNP3i2f0q")
+_LINEAR_ARGS = struct.Struct("@2PqPqPqP4i")
+assert _APPEND_ARGS.size == ctypes.sizeof(_lib.MoERopeAppendArgs)
+assert _ATTENTION_ARGS.size == ctypes.sizeof(_lib.MoEPagedAttentionArgs)
+assert _LINEAR_ARGS.size == ctypes.sizeof(_lib.MoELinearArgs)
 
 
-def _elsewhere(index: int, fn, args) -> int:
-    """The entry point with device ``index`` made current."""
-    with torch.cuda.device(index):
-        return fn(*args, _raw_stream(index))
+def _enqueue(name: str, index: int, args: bytes) -> None:
+    """The entry point, with device ``index`` current."""
+    fn = entry(name)
+    if index == _current_device():
+        rc = fn(args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(args)
+    if rc:
+        _lib.check(rc)
 
 
 # These wrappers are called once per layer and token, on kernels of a few
@@ -318,7 +330,7 @@ def _vector(t: torch.Tensor, dtype, name: str, index: int, n: int) -> int:
 
 def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                  k_scale: float, v_scale: float):
-    """(packed moe_paged_cache, device index, sequences, kv_heads, head_dim)."""
+    """(fields of a moe_paged_cache, device index, sequences, kv_heads, head_dim)."""
     index, dtype = k_cache.get_device(), k_cache.dtype
     if index < 0:
         raise TypeError("k_cache must be a CUDA tensor")
@@ -340,9 +352,9 @@ def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torc
     if len(table) != 2 or (trow[1] != 1 and table[1] > 1):
         raise ValueError("block_table must be (sequences, pages of a sequence) with contiguous "
                          "rows")
-    return _CACHE_STRUCT.pack(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-                              strides[0], strides[1], strides[2], trow[0], kind, *shape, *table,
-                              k_scale, v_scale), index, table[0], shape[2], shape[3]
+    return ((k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), strides[0],
+             strides[1], strides[2], trow[0], kind, *shape, *table, k_scale, v_scale),
+            index, table[0], shape[2], shape[3])
 
 
 def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
@@ -367,15 +379,16 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     T = k.shape[0]
     ks = _rows_f32(k, "k", dev, (T, hk, d))
     vs = _rows_f32(v, "v", dev, (T, hk, d))
-    rot, freq = 0, None
+    rot = freq = 0
     if inv_freq is not None:
         rot = 2 * inv_freq.numel()
         freq = _vector(inv_freq, torch.float64, "inv_freq", dev, inv_freq.numel())
-    hq, qs, os_, q_ptr, o_ptr = 0, (0, 0), (0, 0), None, None
+    hq, qs, os_, q_ptr, o_ptr = 0, (0, 0), (0, 0), 0, 0
     if q is not None:
-        if q.dim() != 3:
+        shape = q.shape
+        if len(shape) != 3:
             raise ValueError("q must be (tokens, q_heads, head_dim)")
-        hq = q.shape[1]
+        hq = shape[1]
         qs = _rows_f32(q, "q", dev, (T, hq, d))
         if q_out is None:
             q_out = torch.empty_like(q)          # dense, whatever q's strides
@@ -383,15 +396,12 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         else:
             os_ = _rows_f32(q_out, "q_out", dev, (T, hq, d))
         q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
-    args = (c, q_ptr, qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], T, hq,
-            _vector(positions, _I32, "positions", dev, T),
-            None if seq_ids is None else _vector(seq_ids, _I32, "seq_ids", dev, T), freq, rot,
-            1 if interleaved else 0, o_ptr, os_[0], os_[1],
-            None if status is None else _vector(status, _I32, "status", dev, 1))
-    fn = entry("moe_rope_append")
-    rc = fn(*args, _raw_stream(dev)) if dev == _current_device() else _elsewhere(dev, fn, args)
-    if rc:
-        _lib.check(rc)
+    _enqueue("moe_rope_append_record", dev, _APPEND_ARGS.pack(
+        *c, q_ptr, k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+        _vector(positions, _I32, "positions", dev, T),
+        0 if seq_ids is None else _vector(seq_ids, _I32, "seq_ids", dev, T), freq, o_ptr, os_[0],
+        os_[1], 0 if status is None else _vector(status, _I32, "status", dev, 1),
+        _raw_stream(dev), T, hq, rot, 1 if interleaved else 0))
     return q_out
 
 
@@ -431,9 +441,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``max_len`` (no sequence is longer; 0 = what the table holds) sizes the
     launch.  ``ws`` comes from ``paged_attention_workspace``."""
     c, dev, seqs, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
-    if q.dim() != 3:
+    shape = q.shape
+    if len(shape) != 3:
         raise ValueError("q must be (sequences, q_heads, head_dim)")
-    hq = q.shape[1]
+    hq = shape[1]
     qs = _rows_f32(q, "q", dev, (seqs, hq, d))
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -445,13 +456,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         ws = paged_attention_workspace(seqs, hq, hk, d, q.device)
     elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
         _refuse(ws, "ws", torch.uint8, dev)
-    args = (c, q.data_ptr(), qs[0], qs[1], _vector(seq_lens, _I32, "seq_lens", dev, seqs), hq,
-            max_len, window, d ** -0.5 if scale is None else scale, softcap, out.data_ptr(),
-            None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel())
-    fn = entry("moe_paged_attention")
-    rc = fn(*args, _raw_stream(dev)) if dev == _current_device() else _elsewhere(dev, fn, args)
-    if rc:
-        _lib.check(rc)
+    _enqueue("moe_paged_attention_record", dev, _ATTENTION_ARGS.pack(
+        *c, q.data_ptr(), qs[0], qs[1], _vector(seq_lens, _I32, "seq_lens", dev, seqs),
+        out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
+        _raw_stream(dev), hq, max_len, window, d ** -0.5 if scale is None else scale, softcap))
     return (out, lse) if return_lse else out
 
 
@@ -482,11 +490,12 @@ def linear(x: torch.Tensor, w: LinearWeights, residual: Optional[torch.Tensor] =
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x (T, cols) f32 -> (T, rows) f32: W x[t] (+ residual[t]) for a few rows.
     Rows of x, residual and out may stride; out may be residual."""
-    if x.dim() != 2:
+    shape = x.shape
+    if len(shape) != 2:
         raise ValueError("x must be (tokens, cols)")
-    dev, T = w.index, x.shape[0]
+    dev, T = w.index, shape[0]
     xs = _rows_f32(x, "x", dev, (T, w.cols))[0]
-    rs, res = 0, None
+    rs = res = 0
     if residual is not None:
         rs, res = _rows_f32(residual, "residual", dev, (T, w.rows))[0], residual.data_ptr()
     if out is None:
@@ -495,11 +504,9 @@ def linear(x: torch.Tensor, w: LinearWeights, residual: Optional[torch.Tensor] =
         ys = _rows_f32(out, "out", dev, (T, w.rows))[0]
         if ys < w.rows and T > 1:
             raise ValueError("rows of out overlap")
-    args = (w.address, w.qtype, w.rows, w.cols, x.data_ptr(), xs, T, res, rs, out.data_ptr(), ys)
-    fn = entry("moe_linear")
-    rc = fn(*args, _raw_stream(dev)) if dev == _current_device() else _elsewhere(dev, fn, args)
-    if rc:
-        _lib.check(rc)
+    _enqueue("moe_linear_record", dev, _LINEAR_ARGS.pack(
+        w.address, x.data_ptr(), xs, res, rs, out.data_ptr(), ys, _raw_stream(dev), w.qtype,
+        w.rows, w.cols, T))
     return out
 
 

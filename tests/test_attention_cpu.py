@@ -181,3 +181,50 @@ def test_pages_are_handed_out_and_come_back():
         PagedKVCache(0, 1, 1, 16, 1, device="cpu")
     e = PagedKVCache(2, 4, 1, 16, 1, dtype=torch.float8_e4m3fn, device="cpu")
     assert e.k.view(torch.uint8).sum() == 0
+
+
+@pytest.mark.parametrize("name, mirror", [
+    ("moe_rope_append_args", _lib.MoERopeAppendArgs),
+    ("moe_paged_attention_args", _lib.MoEPagedAttentionArgs),
+    ("moe_linear_args", _lib.MoELinearArgs)])
+def test_argument_record_matches_header(name, mirror):
+    src = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), src, re.S).group(1)
+    size = {"int": 4, "float": 4}
+    fields = []
+    for line in body.split(";"):
+        m = re.match(r"\s*(?:const\s+)?(\w+)\s*(\*?)(.*)", line, re.S)
+        if m is None:
+            continue
+        for n in m.group(3).split(","):
+            star = bool(m.group(2)) or "*" in n
+            fields.append((n.strip(" *\n"), None if m.group(1) == "moe_paged_cache" else
+                           8 if star else size.get(m.group(1), 8)))
+    import ctypes
+    assert [f for f, _ in fields] == [f[0] for f in mirror._fields_]
+    assert all(b is None or b == ctypes.sizeof(f[1]) for (_, b), f in zip(fields, mirror._fields_))
+
+
+def test_records_reach_the_same_checks(lib):
+    """The record forms refuse and accept what the calls do."""
+    import ctypes
+    for n in ("moe_rope_append_record", "moe_paged_attention_record", "moe_linear_record"):
+        assert getattr(lib, n)(None) == _lib.MOE_ERR_INVALID
+        assert "null arguments" in _lib.last_error()
+    a = _lib.MoEPagedAttentionArgs(cache=cache(), q=256, q_seq_stride=256, q_head_stride=64,
+                                   seq_lens=256, out=256, lse=0, workspace=256,
+                                   workspace_bytes=1, stream=0, q_heads=4, max_len=0, window=0,
+                                   scale=0.1, softcap=0.0)
+    assert lib.moe_paged_attention_record(ctypes.byref(a)) == _lib.MOE_ERR_WORKSPACE
+    a.q_heads = 3
+    assert lib.moe_paged_attention_record(ctypes.byref(a)) == _lib.MOE_ERR_INVALID
+    a.cache.seqs, a.q_heads = 0, 4
+    assert lib.moe_paged_attention_record(ctypes.byref(a)) == _lib.MOE_OK
+    r = _lib.MoERopeAppendArgs(cache=cache(), T=0, q_heads=4, rot=64)
+    assert lib.moe_rope_append_record(ctypes.byref(r)) == _lib.MOE_OK
+    r.rot = 63
+    assert lib.moe_rope_append_record(ctypes.byref(r)) == _lib.MOE_ERR_INVALID
+    w = _lib.MoELinearArgs(qtype=_lib.MOE_Q4_0, rows=16, cols=64, T=0)
+    assert lib.moe_linear_record(ctypes.byref(w)) == _lib.MOE_OK
+    w.cols = 65
+    assert lib.moe_linear_record(ctypes.byref(w)) == _lib.MOE_ERR_UNSUPPORTED
