@@ -31,7 +31,7 @@
 namespace moe {
 
 constexpr int kLinWarps = 16;
-constexpr int kLinMaxStages = 4;
+constexpr int kLinMaxStages = 8;      // barriers of a warp
 constexpr int kLinHead = 2048;         // barriers, row maxima and scales
 constexpr int kLinSmem = 226 * 1024;
 
@@ -54,12 +54,18 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, int rank, float v) {
   uint32_t a;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
 
 // The eight columns of an MMA are four pairs (hi part, lo part).  With 3 rows of
@@ -102,20 +108,35 @@ __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, 
       }
     }
   };
+  if (tid < ROWS) ex[tid] = 0;
+  if (NBG > 1 || n < ROWS || real < rec_blocks)  // else every place is written below
+    for (int i = tid; i < G * rec_blocks * 32; i += kLinWarps * 32)
+      reinterpret_cast<uint4*>(rec)[i] = make_uint4(0, 0, 0, 0);
+  // with 16 rows the first loads of a lane stay in registers for the second pass;
+  // with fewer the code costs more than the second load (first use of an
+  // instruction line: 4096 columns of one row 4.8 -> 5.3 us)
+  constexpr int KEEP = G == 4 ? 8 : 0;
+  const int b0 = part * 8 + (lane >> 2), step = wpr * 8;
+  float kept[KEEP + 1][8];
   uint32_t mx = 0;
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i)
+    if (on && b0 + i * step < real) values(b0 + i * step, kept[i]);
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i)
+    if (on && b0 + i * step < real)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mx = max(mx, __float_as_uint(fabsf(kept[i][k])));
   if (on)
 #pragma unroll 4
-    for (int b = part * 8 + (lane >> 2); b < real; b += wpr * 8) {
+    for (int b = b0 + KEEP * step; b < real; b += step) {
       float v[8];
       values(b, v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(fabsf(v[i])));
+      for (int k = 0; k < 8; ++k) mx = max(mx, __float_as_uint(fabsf(v[k])));
     }
   mx = __reduce_max_sync(0xffffffffu, mx);
   if (lane == 0) smax[warp] = mx;
-  if (tid < ROWS) ex[tid] = 0;
-  for (int i = tid; i < G * rec_blocks * 32; i += kLinWarps * 32)
-    reinterpret_cast<uint4*>(rec)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   if (!on) return;
   mx = 0;
@@ -125,10 +146,8 @@ __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, 
   const float f1 = pow2f(e / 2), f2 = pow2f(e - e / 2);
   if (part == 0 && lane == 0) ex[row] = e;
   const int cg = row / TOK;
-  for (int b = part * 8 + (lane >> 2); b < real; b += wpr * 8) {
+  auto put = [&](int b, const float (&v)[8]) {
     uint32_t hi[4], lo[4];
-    float v[8];
-    values(b, v);
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       // register slots i, i + 1 hold elements 0, 2 | 1, 3 of each four (Q4_0)
@@ -142,8 +161,21 @@ __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, 
     }
     const int pair = (b % NBG) * TOK + row % TOK;
     uint8_t* r = rec + (size_t)(b * G + cg) * 512 + pair * 128 + t * 16;
-    *reinterpret_cast<uint4*>(r) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(r + 64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    // blocks lie on the same banks: the odd ones write their lo half first
+    const bool odd = b & 1;
+    *reinterpret_cast<uint4*>(r + (odd ? 64 : 0)) =
+        odd ? make_uint4(lo[0], lo[1], lo[2], lo[3]) : make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(r + (odd ? 0 : 64)) =
+        odd ? make_uint4(hi[0], hi[1], hi[2], hi[3]) : make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  };
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i)
+    if (b0 + i * step < real) put(b0 + i * step, kept[i]);
+#pragma unroll 2
+  for (int b = b0 + KEEP * step; b < real; b += step) {
+    float v[8];
+    values(b, v);
+    put(b, v);
   }
 }
 
@@ -168,10 +200,18 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
   const int wt0 = min(t1, t0 + kq * wps), wt1 = min(t1, wt0 + wps), nt = wt1 - wt0;
   const int rec_blocks = 2 * tps;                // tps is even
   uint8_t* const rec = smem + kLinHead;
-  float* const red = reinterpret_cast<float*>(rec + (size_t)tps * Cfg::kTileBytes);
-  float* const part = red + (A.ks > 1 ? kLinWarps * NRED : 0);
-  uint8_t* const ring =
-      reinterpret_cast<uint8_t*>(part + (A.cs > 1 ? 2 * groups * NRED : 0)) + warp * A.nst * STAGE;
+  // Sums of the warps: in their rings, which are read out when the only round
+  // ends, or in places of their own
+  const bool own_red = A.ks > 1 && A.rounds > 1;
+  float* const red0 = reinterpret_cast<float*>(rec + (size_t)tps * Cfg::kTileBytes);
+  float* const part = red0 + (own_red ? kLinWarps * NRED : 0);
+  // sums of a round in rows of 32, dealt out to the CTAs of the cluster
+  const int red_rows = groups * (NRED / 32), own_rows = (red_rows + A.cs - 1) / A.cs;
+  uint8_t* const rings = reinterpret_cast<uint8_t*>(
+      part + (A.cs > 1 ? (A.rounds > 1 ? 2 : 1) * A.cs * own_rows * 32 : 0));
+  uint8_t* const ring = rings + warp * A.nst * STAGE;
+  float* const red = own_red ? red0 : reinterpret_cast<float*>(rings);
+  const int red_step = own_red ? NRED : A.nst * STAGE / 4;   // floats from warp to warp
   uint64_t* const bars = bars_all + warp * kLinMaxStages;
 
   if (lane < A.nst) {
@@ -179,9 +219,9 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
     fence_mbar_init();
   }
   if (tid == 0) *dead = 0;                       // seen by all after build_fragments
+  if (A.cs > 1) cluster_arrive();                // waited for before the first store to another CTA
   __syncwarp();
   pdl_trigger();
-  pdl_wait();
 
   // ---- weights: stage q of this warp is tiles [wt0 + j U, ..) of pair `p`
   const int nsr = (nt + U - 1) / U;              // stages of a pair
@@ -210,6 +250,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
       src += 2 * pstep * strip - (int64_t)nsr * U * TB;
     }
   };
+  pdl_wait();
   for (int q = 0; q < A.nst && q < total; ++q) issue();
   build_fragments<QT, NBG, G>(A, rec, rec_blocks, ex, smax, row0, n, t0, t1);
   __syncthreads();
@@ -219,14 +260,17 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
   uint32_t phase = 0;
   // fragments of this warp's columns
   const uint8_t* const xl = rec + lane * 16 + (size_t)2 * (wt0 - t0) * G * 512;
-  // value i (row g + 8 i) of strip s, column group cg in lane l
-  auto put = [&](int p, int s, int cg, int i, int l, float y) {
-    const int tok = TOK * cg + (l & 3), row = 32 * p + 16 * s + (l >> 2) + 8 * i;
-    if ((l & 3) < TOK && tok < n && row < A.rows) {
-      if (A.residual) y += A.residual[(int64_t)(row0 + tok) * A.rs + row];
-      A.y[(int64_t)(row0 + tok) * A.ys + row] = y;
-    }
+  // value k = 2 (s G + cg) + i of lane l: row g + 8 i of strip s of pair p, row of x
+  // of column group cg
+  auto place = [&](int p, int k, int l, int& tok, int& row) {
+    tok = TOK * (k / 2 % G) + (l & 3);
+    row = 32 * p + 16 * (k / (2 * G)) + (l >> 2) + 8 * (k % 2);
+    return (l & 3) < TOK && tok < n && row < A.rows;
   };
+  auto residual_at = [&](int tok, int row) {
+    return A.residual ? A.residual[(int64_t)(row0 + tok) * A.rs + row] : 0.f;
+  };
+  auto store = [&](int tok, int row, float y) { A.y[(int64_t)(row0 + tok) * A.ys + row] = y; };
   for (int r = 0; r < A.rounds; ++r) {
     const int p = p0 + r * pstep;
     float v[2][G][2];
@@ -311,8 +355,19 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
         for (int i = 0; i < 2; ++i) {
           if (NBG >= 2) v[s][cg][i] += __shfl_xor_sync(0xffffffffu, v[s][cg][i], 2);
           if (NBG == 4) v[s][cg][i] += __shfl_xor_sync(0xffffffffu, v[s][cg][i], 1);
-          if (*dead) v[s][cg][i] = __uint_as_float(0x7fffffffu);   // a wait ran out: NaN
         }
+    float rv[2][G][2];                           // residuals, on the way while the warps meet
+    if (A.cs == 1 && kq == 0)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int cg = 0; cg < G; ++cg)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            int tok, row;
+            const bool here = place(p, (s * G + cg) * 2 + i, lane, tok, row);
+            rv[s][cg][i] = here ? residual_at(tok, row) : 0.f;
+          }
     if (A.ks > 1) {
       // the column parts of a pair meet in the group's first warp
       if (r > 0) asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * A.ks) : "memory");
@@ -323,7 +378,7 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
           for (int cg = 0; cg < G; ++cg)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              red[warp * NRED + ((s * G + cg) * 2 + i) * 32 + lane] = v[s][cg][i];
+              red[warp * red_step + ((s * G + cg) * 2 + i) * 32 + lane] = v[s][cg][i];
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * A.ks) : "memory");
       if (kq == 0)
         for (int k = 1; k < A.ks; ++k)
@@ -333,8 +388,13 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
             for (int cg = 0; cg < G; ++cg)
 #pragma unroll
               for (int i = 0; i < 2; ++i)
-                v[s][cg][i] += red[(warp + k) * NRED + ((s * G + cg) * 2 + i) * 32 + lane];
+                v[s][cg][i] += red[(warp + k) * red_step + ((s * G + cg) * 2 + i) * 32 + lane];
     }
+    if (*dead)                                   // a wait ran out: NaN
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int cg = 0; cg < G; ++cg) v[s][cg][0] = v[s][cg][1] = __uint_as_float(0x7fffffffu);
     const bool lead = kq == 0 && p < A.pairs;
     if (lead) {
 #pragma unroll
@@ -354,30 +414,44 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
 #pragma unroll
           for (int cg = 0; cg < G; ++cg)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) put(p, s, cg, i, lane, v[s][cg][i]);
+            for (int i = 0; i < 2; ++i) {
+              int tok, row;
+              if (place(p, (s * G + cg) * 2 + i, lane, tok, row))
+                store(tok, row, v[s][cg][i] + rv[s][cg][i]);
+            }
       }
     } else {
-      // the CTAs' parts: every thread of the cluster adds up its places
-      float* mine_p = part + (size_t)(r & 1) * groups * NRED;
+      // The CTAs' parts: row c goes to CTA c % cs, which adds up the rows that
+      // it gets.  A buffer is used again two rounds later, behind the barrier of
+      // the round between.
+      float* mine_p = part + (size_t)(r & 1) * A.cs * own_rows * 32;
+      const uint32_t to = smem_u32(mine_p);
+      if (r == 0) cluster_wait();
       if (kq == 0)
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int cg = 0; cg < G; ++cg)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              mine_p[group * NRED + ((s * G + cg) * 2 + i) * 32 + lane] = v[s][cg][i];
+        for (int k = 0; k < NRED / 32; ++k) {
+          const int c = group * (NRED / 32) + k, own = c / A.cs;
+          st_cluster(to + ((rank * own_rows + own) * 32 + lane) * 4, c - own * A.cs,
+                     v[k / (2 * G)][k / 2 % G][k % 2]);
+        }
+      // this warp's first row, and its residual on the way meanwhile
+      int tok = 0, row = 0;
+      auto find = [&](int own) {
+        const int c = own * A.cs + rank, gr = c / (NRED / 32);
+        const int pe = gr * nclusters + cluster + r * pstep;
+        return c < red_rows && pe < A.pairs && place(pe, c - gr * (NRED / 32), lane, tok, row);
+      };
+      bool here = warp < own_rows && find(warp);
+      float y = here ? residual_at(tok, row) : 0.f;
       cluster_sync();
-      for (int e = rank * kLinWarps * 32 + tid; e < groups * NRED; e += A.cs * kLinWarps * 32) {
-        const int pe = e / NRED * nclusters + cluster + r * pstep, k = e % NRED / 32;
-        const uint32_t a = smem_u32(mine_p + e);
-        float f[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) f[c] = c < A.cs ? ld_cluster(a, c) : 0.f;
-        float y = f[0];
-#pragma unroll
-        for (int c = 1; c < 8; ++c) y += f[c];
-        if (pe < A.pairs) put(pe, k / (2 * G), k / 2 % G, k % 2, e % 32, y);
+      for (int own = warp; own < own_rows; own += kLinWarps) {
+        if (own != warp) {
+          here = find(own);
+          y = here ? residual_at(tok, row) : 0.f;
+        }
+        float sum = 0.f;
+        for (int c = 0; c < A.cs; ++c) sum += mine_p[(c * own_rows + own) * 32 + lane];
+        if (here) store(tok, row, sum + y);
       }
     }
   }
@@ -387,19 +461,20 @@ __global__ void __launch_bounds__(kLinWarps * 32, 1) linear_kernel(const LinArgs
       mbar_wait(&bars[i], 0);
       mbar_wait(&bars[i], 1);
     }
-  if (A.cs > 1) cluster_sync();                  // nobody reads this CTA's parts any more
 }
 
 // Tiles of a CTA's columns: an even number, so that a stage is two of them.
 inline int linear_tps(int kt, int cs) { return ((kt + cs - 1) / cs + 1) / 2 * 2; }
 
-// Shared memory of a split; nst ring stages take what is left.
+// Shared memory of a split in so many rounds with nst ring stages.
 template <int QT, int NBG, int G, int U>
-static size_t linear_smem(int kt, int cs, int ks, int nst) {
+static size_t linear_smem(int kt, int cs, int ks, int rounds, int nst) {
   using Cfg = LinCfg<NBG, G>;
-  const size_t nred = (size_t)Cfg::kRed * 4;
-  return kLinHead + (size_t)linear_tps(kt, cs) * Cfg::kTileBytes + (ks > 1 ? kLinWarps * nred : 0) +
-         (cs > 1 ? 2 * (kLinWarps / ks) * nred : 0) +
+  const size_t own_rows = (kLinWarps / ks * (Cfg::kRed / 32) + cs - 1) / cs;
+  static_assert(Cfg::kRed * 4 <= 2 * 2 * U * QTraits<QT>::kTileBytes, "sums in a ring");
+  return kLinHead + (size_t)linear_tps(kt, cs) * Cfg::kTileBytes +
+         (ks > 1 && rounds > 1 ? kLinWarps * Cfg::kRed * 4 : 0) +
+         (cs > 1 ? (rounds > 1 ? 2 : 1) * 128 * cs * own_rows : 0) +
          (size_t)kLinWarps * nst * 2 * U * QTraits<QT>::kTileBytes;
 }
 
@@ -432,63 +507,82 @@ static int resident_clusters(const void* kern, int cs, int dev) {
 }
 
 template <int QT, int NBG, int G, int U>
-static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
-  using Cfg = LinCfg<NBG, G>;
-  auto kern = linear_kernel<QT, NBG, G, U>;
+static int linear_ready(int& dev) {
   static std::atomic<uint64_t> ready{0};
-  int dev = 0;
   MOE_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !((ready.load() >> dev) & 1)) {
-    MOE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem));
+    MOE_CUDA(cudaFuncSetAttribute(linear_kernel<QT, NBG, G, U>,
+                                  cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem));
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
-  // The splits of a few sizes are remembered, for calls that repeat them.
-  struct Plan { int dev = -1, kt, pairs, cs, ks, nst, clusters; };
-  static thread_local Plan plans[16];
-  Plan& plan = plans[(a.kt * 31 + a.pairs) & 15];
-  if (plan.dev != dev || plan.kt != a.kt || plan.pairs != a.pairs)
-    plan = {dev, a.kt, a.pairs, 0, 0, 0, 0};
-  if (plan.nst == 0) {
-    // Estimated time of a split, in the time all warps of an SM take for one tile
-    // of two strips each (about 800 cycles of HBM): rounds x (tiles of a warp, and
-    // the meetings of warps, 3, and of a cluster, 8), and the fragments of the
-    // CTA's columns (28 cycles per group and tile).
-    double best = 0;
-    for (int cs = 1; cs <= 8; cs *= 2) {
-      const int resident = resident_clusters((const void*)kern, cs, dev);
-      for (int ks = 1; ks <= kLinWarps; ks *= 2) {
-        if (linear_smem<QT, NBG, G, U>(a.kt, cs, ks, 2) > kLinSmem) continue;
-        const int tps = linear_tps(a.kt, cs), wt = ((tps + ks - 1) / ks + 1) / 2 * 2;
-        const int slots = resident * (kLinWarps / ks);
-        const int rounds = (a.pairs + slots - 1) / slots;
-        const double t = rounds * (wt * (1 + 0.25 * (G - 1)) + (ks > 1 ? 3 : 0) + (cs > 1 ? 8 : 0)) +
-                         0.035 * G * tps;
-        if (plan.cs == 0 || t < best) {
-          best = t;
-          plan.cs = cs;
-          plan.ks = ks;
-          plan.clusters = resident;
-        }
+  return MOE_OK;
+}
+
+// The split (cs, ks) of a size with the least estimated time.
+struct LinPlan {
+  int dev = -1, kt, pairs, cs, ks, nst, clusters, rounds;
+  double time;
+};
+template <int QT, int NBG, int G, int U>
+static const LinPlan& linear_plan(const LinArgs& a, int dev) {
+  using Cfg = LinCfg<NBG, G>;
+  // the plans of a few sizes are remembered, for calls that repeat them
+  static thread_local LinPlan plans[16];
+  LinPlan& plan = plans[(a.kt * 31 + a.pairs) & 15];
+  if (plan.dev == dev && plan.kt == a.kt && plan.pairs == a.pairs) return plan;
+  plan = {dev, a.kt, a.pairs, 0, 0, 2, 0, 0, 0};
+  // Microseconds: rounds x (tiles of a warp, the meetings of warps and of a
+  // cluster), the tiles again by the share of the warps that have work, and the
+  // fragments of the CTA's columns.  Fitted to all splits of 15 sizes with 1, 4, 8
+  // and 16 rows; the split that it takes is 0.6 % slower than the best one on
+  // average (8 % at worst).
+  const double g = G - 1;
+  const double tile = 0.13 + 0.06 * g + (QT == MOE_Q8_0 ? 0.18 : 0) + (U == 1 ? 0.06 : 0);
+  const double share = 0.1 + 0.05 * g, frag = 0.018 * G + 0.003 * Cfg::kRows;
+  const double warps_meet = 0.46 + 0.04 * g, ctas_meet = 1.36 + 0.56 * g;
+  for (int cs = 1; cs <= 8; cs *= 2) {
+    const int resident =
+        resident_clusters((const void*)linear_kernel<QT, NBG, G, U>, cs, dev);
+    for (int ks = 1; ks <= kLinWarps; ks *= 2) {
+      const int tps = linear_tps(a.kt, cs), wt = ((tps + ks - 1) / ks + 1) / 2 * 2;
+      const int slots = resident * (kLinWarps / ks);   // pairs of a round
+      const int rounds = (a.pairs + slots - 1) / slots;
+      if (linear_smem<QT, NBG, G, U>(a.kt, cs, ks, rounds, 2) > kLinSmem) continue;
+      const double t =
+          rounds * (wt * tile + (ks > 1 ? warps_meet : 0) + (cs > 1 ? ctas_meet : 0)) +
+          (double)a.pairs / slots * wt * share + tps * frag;
+      if (plan.cs == 0 || t < plan.time) {
+        plan.time = t;
+        plan.cs = cs;
+        plan.ks = ks;
+        plan.clusters = std::min(resident, a.pairs);
+        plan.rounds = rounds;
       }
     }
-    plan.nst = 2;
-    while (plan.cs > 0 && plan.nst < kLinMaxStages &&
-           linear_smem<QT, NBG, G, U>(a.kt, plan.cs, plan.ks, plan.nst + 1) <= kLinSmem)
-      ++plan.nst;
   }
+  while (plan.cs > 0 && plan.nst < (U > 1 ? 4 : kLinMaxStages) &&
+         linear_smem<QT, NBG, G, U>(a.kt, plan.cs, plan.ks, plan.rounds, plan.nst + 1) <= kLinSmem)
+    ++plan.nst;
+  return plan;
+}
+
+template <int QT, int NBG, int G, int U>
+static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
+  using Cfg = LinCfg<NBG, G>;
+  int dev = 0;
+  MOE_CHECK((linear_ready<QT, NBG, G, U>(dev)));
+  const LinPlan& plan = linear_plan<QT, NBG, G, U>(a, dev);
   fits = plan.cs > 0;
   if (!fits) return MOE_OK;
   a.cs = plan.cs;
   a.ks = plan.ks;
   a.nst = plan.nst;
   a.tps = linear_tps(a.kt, a.cs);
-  const int per = kLinWarps / a.ks;                  // pairs of a cluster's round
-  const int clusters = std::min(plan.clusters, a.pairs);
-  a.rounds = (a.pairs + clusters * per - 1) / (clusters * per);
+  a.rounds = plan.rounds;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(clusters * a.cs), (unsigned)((a.T + Cfg::kRows - 1) / Cfg::kRows));
+  cfg.gridDim = dim3((unsigned)(plan.clusters * a.cs), (unsigned)((a.T + Cfg::kRows - 1) / Cfg::kRows));
   cfg.blockDim = dim3(kLinWarps * 32);
-  cfg.dynamicSmemBytes = linear_smem<QT, NBG, G, U>(a.kt, a.cs, a.ks, a.nst);
+  cfg.dynamicSmemBytes = linear_smem<QT, NBG, G, U>(a.kt, a.cs, a.ks, a.rounds, a.nst);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -499,8 +593,22 @@ static int launch_linear(LinArgs& a, cudaStream_t s, bool& fits) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = a.cs > 1 ? 2 : 1;
-  MOE_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+  MOE_CUDA(cudaLaunchKernelEx(&cfg, linear_kernel<QT, NBG, G, U>, a));
   return MOE_OK;
+}
+
+// 16 rows, whose fragments take most of the shared memory: one tile per wait needs
+// half the ring, which lets splits over fewer CTAs fit (Q8_0 4096 x 8192 18.6 us
+// instead of 21.9).
+template <int QT>
+static int launch_linear_16(LinArgs& a, cudaStream_t s, bool& fits) {
+  int dev = 0;
+  MOE_CHECK((linear_ready<QT, 1, 4, 2>(dev)));
+  MOE_CHECK((linear_ready<QT, 1, 4, 1>(dev)));
+  const LinPlan &two = linear_plan<QT, 1, 4, 2>(a, dev), &one = linear_plan<QT, 1, 4, 1>(a, dev);
+  if (one.cs > 0 && (two.cs == 0 || one.time < two.time))
+    return launch_linear<QT, 1, 4, 1>(a, s, fits);
+  return launch_linear<QT, 1, 4, 2>(a, s, fits);
 }
 
 // Rows of a pass: as many as T needs (1, 2, 4, 8 or 16), fewer where x is so wide
@@ -512,7 +620,7 @@ template <int QT>
 static int launch_linear_qt(LinArgs& a, cudaStream_t s) {
   constexpr int U = QT == MOE_Q4_0 ? 4 : 2;
   bool fits = false;
-  if (a.T > 8) MOE_CHECK((launch_linear<QT, 1, 4, 2>(a, s, fits)));
+  if (a.T > 8) MOE_CHECK((launch_linear_16<QT>(a, s, fits)));
   if (!fits && a.T > 4) MOE_CHECK((launch_linear<QT, 1, 2, 2>(a, s, fits)));
   if (!fits && a.T > 2) MOE_CHECK((launch_linear<QT, 1, 1, U>(a, s, fits)));
   if (!fits && a.T > 2 && U > 2) MOE_CHECK((launch_linear<QT, 1, 1, 2>(a, s, fits)));
