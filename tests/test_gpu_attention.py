@@ -404,6 +404,23 @@ def test_attention_many_sequences():
     check_attention(c, q, out, lse, d ** -0.5)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("hq,hkv,d", [(5, 1, 128), (8, 8, 64), (6, 3, 256), (24, 2, 96)])
+def test_attention_parts_of_two_units(dtype, hq, hkv, d):
+    """Runs that begin in one unit and end in another, each joined by whichever
+    CTA comes last: the same bits every time."""
+    lens = [4001, 4733, 0, 1, 5099, 3777, 4510]
+    c = Cache(lens, 16, hkv, d, dtype, seed=d)
+    q = randn(len(lens), hq, d, seed=3)
+    ws = K.paged_attention_workspace(len(lens), hq, hkv, d, "cuda")
+    out, lse = K.paged_attention(q, *c.args, c.lens, return_lse=True, ws=ws,
+                                 **c.scales)
+    check_attention(c, q, out, lse, d ** -0.5)
+    for _ in range(50):
+        again, l2 = K.paged_attention(q, *c.args, c.lens, return_lse=True, ws=ws, **c.scales)
+        assert torch.equal(again, out) and torch.equal(l2, lse)
+
+
 def test_attention_captured_and_replayed_with_other_lengths():
     """One captured launch serves every later length; two captured graphs
     that share a workspace replay in turn."""
@@ -478,6 +495,23 @@ def test_linear_wide(qtype, T, rows, cols):
     res = rng.standard_normal((T, rows), dtype=np.float32)
     y = K.linear(torch.from_numpy(x).cuda(), lw, residual=torch.from_numpy(res).cuda())
     check_linear(y.cpu().numpy(), x, w, big, res)
+
+
+@pytest.mark.parametrize("qtype", [2, 8])
+@pytest.mark.parametrize("T,rows,cols", [(16, 20011, 4096), (8, 20011, 4096), (1, 20011, 4096),
+                                         (13, 65541, 512), (3, 9003, 2848)])
+def test_linear_several_rounds(qtype, T, rows, cols):
+    """More rows than the GPU takes at a time, alone and in clusters, in place."""
+    rng = np.random.default_rng(rows + cols)
+    raw, w, big = matrix(rng, qtype, rows, cols)
+    lw = K.LinearWeights(torch.from_numpy(raw.reshape(-1)).cuda(), qtype, rows, cols)
+    x = rng.standard_normal((T, cols), dtype=np.float32)
+    res = rng.standard_normal((T, rows), dtype=np.float32)
+    y, xd = torch.from_numpy(res).cuda(), torch.from_numpy(x).cuda()
+    K.linear(xd, lw, residual=y, out=y)
+    check_linear(y.cpu().numpy(), x, w, big, res)
+    for _ in range(20):
+        assert torch.equal(K.linear(xd, lw, residual=torch.from_numpy(res).cuda()), y)
 
 
 @pytest.mark.parametrize("T", [1, 2, 7])
