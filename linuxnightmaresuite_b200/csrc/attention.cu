@@ -53,10 +53,9 @@
 namespace moe {
 
 constexpr int kAttHeads = 8;          // query heads of a unit at most
-constexpr int kAttCtasPerSm = 2;
+constexpr int kAttCtasMost = 3;       // CTAs of an SM
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kAttParts = 320;        // CTAs that one unit may be split over
 constexpr float kPShift = 7.f;        // probabilities enter sums and products times 2^7
 
 struct AttArgs {
@@ -100,6 +99,9 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async() {
+  asm volatile("fence.proxy.async;" ::: "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -222,15 +224,15 @@ template <int DT, int DP, bool PACK> struct AttCfg {
   static constexpr int kTiles = kWarps / kSplit;            // tiles of a round
   static constexpr int kKeys = kRow <= 128 ? 32 : 16;       // keys of a tile
   static constexpr int kSlot = kKeys * kRow;
-  static constexpr int kSlots = 5;
+  // heads of 64 leave registers for a third CTA, in exchange for the fourth and
+  // fifth slot (256 sequences of up to 1024 keys, 8 heads, fp16 60 -> 56 us, e4m3
+  // 59 -> 49 us); 128 columns of e4m3 would spill (111 -> 136 us)
+  static constexpr int kCtas = DP == 64 ? 3 : 2;
+  static constexpr int kSlots = kCtas == 3 ? 3 : 5;
   static constexpr int kRound = kTiles * kKeys;
   static constexpr int kRing = kWarps * kSlots * kSlot;
   static constexpr int kMergeRow = DP + 8;                  // floats
-  // one row per tile and head; when a unit's parts are joined a weight per part
-  // and head, and four floats per thread
-  static constexpr int kRows = 4 * kAttHeads * kTiles * kMergeRow;
-  static constexpr int kJoin = 4 * kAttHeads * kAttParts + 16 * 32 * kWarps;
-  static constexpr int kMerge = kRows > kJoin ? kRows : kJoin;
+  static constexpr int kMerge = 4 * kAttHeads * kTiles * kMergeRow;   // a row per tile and head
   static constexpr int kQ = DP / 16 * Frag::kBytes;
   static constexpr int kX = kSplit > 1 ? kWarps * 32 * (kKeys / 4) * 4 : 0;   // halves of scores
   static constexpr int kSmem = kRing + kMerge + kQ + kX;
@@ -242,6 +244,7 @@ template <int DT, int DP, bool PACK> struct AttCfg {
 // 48 sequences of 1 .. 2500 keys, 16 heads of 64, 82 us instead of 58 (one round
 // 63 us, three 59 us).
 constexpr int kUnitCost = 2;
+constexpr int kWholeRounds = 2;        // units of so many rounds are not split if they need not be
 
 // byte offset of 16-byte chunk c of row r in a slot: blocks of KEYS lines,
 // swizzled as TMA swizzles them
@@ -262,11 +265,12 @@ struct AttShared {
   long long base, scan[4];
   int seq, dead, join[2];            // join: of the last piece, of the first
   uint64_t bars[4][5];               // a barrier per ring slot
+  uint64_t joined;                   // of the copies of other CTAs' parts
   float m[4][kAttHeads], l[4][kAttHeads], qmax[4][kAttHeads], qscale[kAttHeads];
 };
 
 template <int DT, int DP, bool PACK>
-__global__ void __launch_bounds__(AttCfg<DT, DP, PACK>::kWarps * 32, kAttCtasPerSm)
+__global__ void __launch_bounds__(AttCfg<DT, DP, PACK>::kWarps * 32, (AttCfg<DT, DP, PACK>::kCtas))
 attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                  const AttArgs A) {
   using Cfg = AttCfg<DT, DP, PACK>;
@@ -284,6 +288,8 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     fence_mbar_init();
   }
   if (tid == 0) {
+    mbar_init(&sh.joined, 1);
+    fence_mbar_init();
     prefetch_map(&kmap);
     prefetch_map(&vmap);
   }
@@ -862,6 +868,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         if (c < D) to[c] = y;
       }
     }
+    if (!whole) fence_proxy_async();             // a part may be fetched by a bulk copy
     if (more) q_split();
     __syncthreads();                             // q of the next piece; mo and sh are free
     // Parts of units are announced as they are written; units that turn out to
@@ -875,95 +882,85 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     if (!more) break;
     C = N;
   }
+  // Joins: the parts come into the ring, which has been read out, by one bulk copy
+  // for each part's sums and one for its values, and are added in order.  The
+  // loops are short because this code runs once: unrolled over 16 loads to
+  // registers it took 11600 cycles for 37 parts, most of them instruction fetches.
   __syncthreads();
+  uint32_t jphase = 0;
   for (int k = 0; k < 2; ++k) {
     if (!sh.join[k]) continue;
-    if (k) {
-      __syncthreads();                           // mo is free again
-      C = sh.first;
-    }
+    if (k) C = sh.first;
     int c0;
     const int n = spread(C, c0), nh = heads(C);
     const int64_t row0 = (int64_t)C.seq * A.hq + first_head(C);
-    // thread: four columns of a head, of every PL-th part; the first loads
-    // go out before the weights are known
-    constexpr int CT = DP / 4, U = 16;
-    const int HW = min(nh <= 1 ? 1 : nh <= 2 ? 2 : nh <= 4 ? 4 : 8, NT / CT);
-    const int PL = NT / (CT * HW);
-    const int col = tid % CT, hw = tid / CT % HW, pl = tid / (CT * HW);
-    const int64_t slot0 = 2 * (int64_t)c0;   // part i: slot0 + 2 i, part 0: slot0 + 1
-    float4 v4[U];
-    auto load = [&](int h, int i0) {
+    constexpr int ML = kAttHeads * 8, CT = DP / 4;
+    const int OB = nh * DP * 4;
+    const int most_parts = Cfg::kRing / (ML + OB);         // in the ring at a time
+    const float2* ml = reinterpret_cast<const float2*>(smem);
+    const float4* po = reinterpret_cast<const float4*>(smem + most_parts * ML);
+    // items: four columns of a head; M, L, y: maximum, sum and values so far
+    constexpr int ITEMS = kAttHeads * CT / NT > 0 ? kAttHeads * CT / NT : 1;
+    float M[ITEMS], L[ITEMS];
+    float4 y[ITEMS];
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int i = i0 + k * PL;
-        if (i < n)
-          v4[k] = __ldcg(reinterpret_cast<const float4*>(
-                             A.part_o + ((slot0 + 2 * i + (i == 0)) * kAttHeads + h) * DP) + col);
-      }
-    };
-    if (hw < nh) load(hw, pl);
-    // weights of the parts, [part][head]; mo is free again
-    for (int h = warp; h < nh; h += NW) {
-      float2 v[kAttParts / 32];
-      float M = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int k = 0; k < kAttParts / 32; ++k) {
-        const int i = lane + 32 * k;
-        v[k] = i < n ? __ldcg(A.part_ml + (slot0 + 2 * i + (i == 0)) * kAttHeads + h)
-                     : make_float2(-INFINITY, 0.f);
-      }
-#pragma unroll
-      for (int k = 0; k < kAttParts / 32; ++k) M = fmaxf(M, v[k].x);
-#pragma unroll
-      for (int b = 16; b > 0; b >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, b));
-      const float ms = M == -INFINITY ? 0.f : M;
-#pragma unroll
-      for (int k = 0; k < kAttParts / 32; ++k) {
-        v[k].x = ex2(v[k].x - ms);
-        L = fmaf(v[k].y, v[k].x, L);
-      }
-#pragma unroll
-      for (int b = 16; b > 0; b >>= 1) L += __shfl_xor_sync(0xffffffffu, L, b);
-      const float norm = L == 0.f ? 0.f : A.c.v_scale / L;
-#pragma unroll
-      for (int k = 0; k < kAttParts / 32; ++k)
-        if (lane + 32 * k < n) mo[(lane + 32 * k) * kAttHeads + h] = v[k].x * norm;
-      if (lane == 0 && A.lse) A.lse[row0 + h] = (M + (log2f(L) - kPShift)) * kLn2;
+    for (int j = 0; j < ITEMS; ++j) {
+      M[j] = -INFINITY;
+      L[j] = 0.f;
+      y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    __syncthreads();
-    float* const sums = mo + kAttParts * kAttHeads;   // [pl][head][DP]
-    for (int h = hw; h < nh; h += HW) {
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i0 = pl; i0 < n; i0 += U * PL) {
-        if (h != hw || i0 != pl) load(h, i0);
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const int i = i0 + k * PL;
-          if (i < n) {
-            const float w = mo[i * kAttHeads + h];
-            y.x = fmaf(v4[k].x, w, y.x);
-            y.y = fmaf(v4[k].y, w, y.y);
-            y.z = fmaf(v4[k].z, w, y.z);
-            y.w = fmaf(v4[k].w, w, y.w);
-          }
+    for (int i0 = 0; i0 < n; i0 += most_parts) {
+      const int cnt = min(most_parts, n - i0);
+      if (k || i0) __syncthreads();              // the parts before have been added
+      if (warp == 0) {
+        fence_proxy_async();
+        if (lane == 0) mbar_expect_tx(&sh.joined, cnt * (ML + OB));
+        __syncwarp();
+        for (int i = lane; i < cnt; i += 32) {
+          const int64_t slot = 2 * (int64_t)(c0 + i0 + i) + (i0 + i == 0);
+          bulk_g2s_plain(smem + i * ML, A.part_ml + slot * kAttHeads, ML, &sh.joined);
+          bulk_g2s_plain(smem + most_parts * ML + i * OB, A.part_o + slot * kAttHeads * DP, OB,
+                         &sh.joined);
         }
       }
-      if (PL > 1) {
-        reinterpret_cast<float4*>(sums)[(pl * nh + h) * CT + col] = y;
-      } else {
-        float* to = A.out + (row0 + h) * D + 4 * col;
-        if (4 * col < D) to[0] = y.x, to[1] = y.y, to[2] = y.z, to[3] = y.w;
+      if (!mbar_wait(&sh.joined, jphase)) {
+        sh.dead = 1;
+        set_status(A.status, MOE_STATUS_TIMEOUT);
+      }
+      jphase ^= 1u;
+#pragma unroll
+      for (int j = 0; j < ITEMS; ++j) {
+        const int e = tid + j * NT, h = e / CT, col = e % CT;
+        if (h >= nh) break;
+        float m = M[j];
+#pragma unroll 4
+        for (int i = 0; i < cnt; ++i) m = fmaxf(m, ml[i * kAttHeads + h].x);
+        const float ms = m == -INFINITY ? 0.f : m, f = ex2(M[j] - ms);
+        M[j] = m;
+        L[j] *= f;
+        y[j] = make_float4(y[j].x * f, y[j].y * f, y[j].z * f, y[j].w * f);
+#pragma unroll 4
+        for (int i = 0; i < cnt; ++i) {
+          const float2 p = ml[i * kAttHeads + h];
+          const float4 v = po[(i * nh + h) * CT + col];
+          const float w = ex2(p.x - ms);
+          L[j] = fmaf(p.y, w, L[j]);
+          y[j].x = fmaf(v.x, w, y[j].x);
+          y[j].y = fmaf(v.y, w, y[j].y);
+          y[j].z = fmaf(v.z, w, y[j].z);
+          y[j].w = fmaf(v.w, w, y[j].w);
+        }
       }
     }
-    if (PL > 1) {
-      __syncthreads();
-      for (int e = tid; e < nh * DP; e += NT) {
-        const int h = e / DP, c = e % DP;
-        float v = sums[e];
-        for (int k = 1; k < PL; ++k) v += sums[(k * nh) * DP + e];
-        if (c < D) A.out[(row0 + h) * D + c] = v;
-      }
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const int e = tid + j * NT, h = e / CT, col = e % CT;
+      if (h >= nh) break;
+      const float norm = L[j] == 0.f ? 0.f : A.c.v_scale / L[j];
+      float* to = A.out + (row0 + h) * D + 4 * col;
+      if (4 * col < D)
+        to[0] = y[j].x * norm, to[1] = y[j].y * norm, to[2] = y[j].z * norm, to[3] = y[j].w * norm;
+      if (col == 0 && A.lse) A.lse[row0 + h] = (M[j] + (log2f(L[j]) - kPShift)) * kLn2;
     }
   }
   // after a timeout copies may still be under way: give them time to land
@@ -981,7 +978,7 @@ inline int padded_head_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; 
 
 static int attention_workspace(int head_dim, AttArgs* a, void* ws, size_t* bytes) {
   Carve cv = {static_cast<uint8_t*>(ws), 0, 0};
-  const int slots = kAttCtasPerSm * sm_count();
+  const int slots = kAttCtasMost * sm_count();
   cv.take<uint8_t>(256);
   int* arrivals = cv.take<int>(slots);
   float2* ml = cv.take<float2>((size_t)2 * slots * kAttHeads);
@@ -1033,7 +1030,9 @@ static int make_cache_map(CUtensorMap* map, AttArgs& a, void* base, int keys) {
 template <int DT, int DP, bool PACK>
 static int launch_attention(AttArgs& a, int max_len, cudaStream_t s) {
   using Cfg = AttCfg<DT, DP, PACK>;
-  static_assert(Cfg::kSlots % 2 == 1 && Cfg::kSlots <= 5 && Cfg::kWarps == 4, "");
+  static_assert(Cfg::kSlots % 2 == 1 && Cfg::kSlots <= 5 && Cfg::kWarps == 4 &&
+                    Cfg::kCtas <= kAttCtasMost,
+                "");
   static std::atomic<uint64_t> ready{0};
   auto kern = attention_kernel<DT, DP, PACK>;
   int dev = 0;
@@ -1048,15 +1047,17 @@ static int launch_attention(AttArgs& a, int max_len, cudaStream_t s) {
   const int G = a.hq / a.c.kv_heads;
   const int64_t units = (int64_t)a.c.seqs * a.c.kv_heads * ((G + kAttHeads - 1) / kAttHeads);
   const int64_t keys = a.window > 0 ? std::min(a.window, max_len) : max_len;
-  const int64_t cost =
-      units * (std::max<int64_t>(1, (keys + Cfg::kRound - 1) / Cfg::kRound) + kUnitCost);
-  const int grid = (int)std::min<int64_t>(cost, (int64_t)kAttCtasPerSm * sm_count());
+  // A round costs about 1 us, a unit in parts about 3 us for their joining: short
+  // sequences get a CTA per unit (one of 100 keys 6.3 us instead of 8.0; with three
+  // rounds ragged batches lose more than that: their units are split all the same)
+  const int64_t rounds = std::max<int64_t>(1, (keys + Cfg::kRound - 1) / Cfg::kRound);
+  const int64_t ctas = rounds <= kWholeRounds ? units : units * (rounds + kUnitCost);
+  const int grid = (int)std::min<int64_t>(ctas, (int64_t)Cfg::kCtas * sm_count());
   // a CTA counts its costs, and a sequence's, in 32 bits
   const int64_t most = (int64_t)a.c.table_width * a.c.page_size / Cfg::kRound + 2 + kUnitCost;
   MOE_REQUIRE(units / a.c.seqs * most < (1ll << 30) && units * most / grid < (1ll << 30),
               MOE_ERR_UNSUPPORTED, "%d sequences of up to %d pages are too many", a.c.seqs,
               a.c.table_width);
-  MOE_REQUIRE(grid <= kAttParts, MOE_ERR_UNSUPPORTED, "%d CTAs are too many", grid);
   MOE_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(Cfg::kWarps * 32), Cfg::kSmem, s, kmap, vmap,
                       a));
   return MOE_OK;
