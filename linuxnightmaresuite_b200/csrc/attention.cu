@@ -9,13 +9,15 @@
 // padding.
 //
 // Work.  A unit is one (sequence, key head, group of up to 8 query heads); it
-// is cut into rounds of one tile of KEYS keys per warp.  All units in order, each at the cost of
-// its rounds and kUnitCost more for its start and end, are dealt out in equal
+// is cut into rounds of one tile of KEYS keys per warp.  All units in order, each at the
+// cost of its rounds and kUnitCost more for its start and end, are dealt out in equal
 // contiguous runs to the CTAs of one resident grid, whatever the lengths.  Each
 // CTA finds its run by a scan of the lengths, so one captured launch serves
 // every later length.  A unit that ends up in several CTAs is joined by the last of
 // them to finish, from f32 partials in the workspace, in the order of its
-// keys; the arrival counters return to zero.
+// keys; the arrival counters return to zero.  The join comes behind the loop over
+// the pieces, and the first piece's arrival does not stop the other warps: in the
+// loop both cost registers and time (ragged e4m3 batch 119 instead of 111 us).
 //
 // A warp takes every NW-th tile of KEYS keys through a ring of its own, keys
 // and values in slots of their own; the warps meet only at the end of a unit.
@@ -37,10 +39,11 @@
 // (values) k16 steps; from there on sums are f32 adds.
 //
 // Measured on a B200 (copy bandwidth 6.55 TB/s): 592 sequences of 1024 keys, 8 key
-// heads of 128, fp16 382 us (2.5 GB, 100 %); one of 131071 keys 95 us (0.54 GB,
-// 86 %: about 10 us are start, first misses and joining 37 parts); e4m3 256 x 2048
-// keys 194 us (1.1 GB, 85 %: bound by instructions, half of them the conversion
-// to fp16); one sequence of 37 keys 5.4 us, of 512 keys 9 us.
+// heads of 128, fp16 382 us (2.5 GB, 100 %); one of 131071 keys 93 us (0.54 GB,
+// 88 %: 4 us until the first tile, then CTAs that end between 74 and 86 us after the
+// start with equal work, then the join of 37 parts); e4m3 256 x 2048 keys 184 us
+// (1.1 GB, 90 %: bound by the latency of conversion, product and exponentials in
+// eight warps); one sequence of 37 keys 5.1 us, of 512 keys 8.7 us.
 #include <math.h>
 
 #include <algorithm>
@@ -239,10 +242,10 @@ template <int DT, int DP, bool PACK> struct AttCfg {
   static constexpr int kFold = 128 / kKeys;                 // tiles between folds
 };
 
-// What the start and the end of a unit cost, in rounds (measured: about 2 us at
-// 1.3 us a round).  Without it a CTA with many short sequences takes longest:
-// 48 sequences of 1 .. 2500 keys, 16 heads of 64, 82 us instead of 58 (one round
-// 63 us, three 59 us).
+// What the start and the end of a unit cost, in rounds.  Without it a CTA with many
+// short sequences takes longest: 48 sequences of 1 .. 2500 keys, 16 heads of 64, two
+// CTAs of an SM, 60 us with one round, 56 us with two, 58 us with three; 256
+// sequences of up to 2048 e4m3 keys 121, 111 and 114 us.
 constexpr int kUnitCost = 2;
 constexpr int kWholeRounds = 2;        // units of so many rounds are not split if they need not be
 

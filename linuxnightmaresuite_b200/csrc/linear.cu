@@ -6,7 +6,7 @@
 // rows fill the 8 columns of an MMA), and a 32-weight block is scaled in f32 after
 // its sum.  The quants are made signed: as subnormals with their offset in the
 // accumulator, the experts' form, they take 8 half-precision operations per
-// 512 weights less (262144 x 2816 for one row 75 us instead of 83), but the
+// 512 weights less (262144 x 2816 for one row 75 us instead of 83 then), but the
 // tensor core aligns the subnormals' products to exponents 7 bits too large, and
 // the result was off by up to 1.1e-6 of its norm instead of 1e-7.
 //
@@ -16,13 +16,16 @@
 // each fragment read) and 1 / ks of their columns, through a ring of bulk
 // copies.  Where x is too wide for one SM's shared memory (or W has few rows) a
 // cluster of cs CTAs splits the columns, so that each converts only its part of
-// x; their sums meet in distributed shared memory.  The split (cs, ks) is the
-// one with the least estimated time; sums are in a fixed order.
+// x; each CTA then stores its sums in the shared memory of the one that adds them.
+// The split (cs, ks) is the one with the least estimated time; sums are in a fixed
+// order.
 //
-// Measured on a B200 (copy bandwidth 6.55 TB/s): 262144 x 2816 Q4_0 for one row 72
-// us (416 MB, 88 %), 65536 x 2816 for 1, 4, 8, 16 rows 22.6, 24.8, 35, 54 us (floor
-// 15.9), 6144 x 2816 for one row 6.3 us, of which 4 are launch, fragments and the
-// meeting of the warps.
+// Measured on a B200 (copy bandwidth 6.55 TB/s): 262144 x 2816 Q4_0 for one row 70
+// us (416 MB, 90 %; 80 us and more once sustained load has lowered the clock, since
+// instructions come next), 65536 x 2816 for 1, 4, 8, 16 rows 22.4, 24.5, 35.6, 53 us
+// (floor 15.9), 6144 x 2816 for one row 6.0 us, of which 4 are launch, fragments and
+// the meeting of the warps, 4096 x 8192 for 16 rows 17.1 us (fragments 4.4, weights
+// 8.5 where the MMAs alone take 4.3, meetings 3.3).
 #include <algorithm>
 #include <atomic>
 
@@ -614,8 +617,8 @@ static int launch_linear_16(LinArgs& a, cudaStream_t s, bool& fits) {
 // Rows of a pass: as many as T needs (1, 2, 4, 8 or 16), fewer where x is so wide
 // that their fragments do not fit.  Up to 4 rows of 4-bit weights are bound by
 // instructions, so four tiles are taken per wait where the ring fits (65536 x
-// 2816: 1 row 25.7 -> 22.9 us, 4 rows 28.1 -> 24.9 us; 8 rows, nearer the MMAs'
-// bound, 36.5 -> 37.4 us).
+// 2816: 1 row 25.7 -> 22.9 us, 4 rows 28.1 -> 24.9 us when it was done; 8 rows,
+// nearer the MMAs' bound, 36.5 -> 37.4 us).
 template <int QT>
 static int launch_linear_qt(LinArgs& a, cudaStream_t s) {
   constexpr int U = QT == MOE_Q4_0 ? 4 : 2;

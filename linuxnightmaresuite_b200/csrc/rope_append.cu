@@ -8,9 +8,9 @@
 // One CTA per (token, part of its heads): the CTA computes the token's rot / 2
 // (cos, sin) pairs once into shared memory, one thread follows the page table to
 // the token's slot, then all walk the heads four elements at a time.  Bound by
-// memory for prompts (8191 tokens, 32 + 2 x 8 heads of 128: 68 us for 0.37 GB, 83 %
+// memory for prompts (8191 tokens, 32 + 2 x 8 heads of 128: 65.5 us for 0.37 GB, 86 %
 // of the copy bandwidth; the rest is the latency of position, page and slot,
-// which 7 resident CTAs per SM do not hide altogether), by latency for single
+// which the resident CTAs of an SM do not hide altogether), by latency for single
 // tokens (2.0 us).
 #include <math.h>
 
