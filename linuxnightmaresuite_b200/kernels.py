@@ -447,11 +447,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     hq = shape[1]
     qs = _rows_f32(q, "q", dev, (seqs, hq, d))
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = q.new_empty(seqs, hq, d)
     elif out.dtype is not _F32 or out.get_device() != dev or out.shape != (seqs, hq, d) or \
             not out.is_contiguous():
         _refuse(out, "out", _F32, dev, (seqs, hq, d))
-    lse = q.new_empty((seqs, hq)) if return_lse else None
+    lse = q.new_empty(seqs, hq) if return_lse else None
     if ws is None:
         ws = paged_attention_workspace(seqs, hq, hk, d, q.device)
     elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
@@ -499,7 +499,7 @@ def linear(x: torch.Tensor, w: LinearWeights, residual: Optional[torch.Tensor] =
     if residual is not None:
         rs, res = _rows_f32(residual, "residual", dev, (T, w.rows))[0], residual.data_ptr()
     if out is None:
-        out, ys = x.new_empty((T, w.rows)), w.rows
+        out, ys = x.new_empty(T, w.rows), w.rows
     else:
         ys = _rows_f32(out, "out", dev, (T, w.rows))[0]
         if ys < w.rows and T > 1:
