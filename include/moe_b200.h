@@ -440,6 +440,7 @@ int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_
                     float* q_out, int64_t qo_tok_stride, int64_t qo_head_stride, int32_t* status,
                     moe_stream_t stream);
 
+/* The size does not depend on seqs: a workspace serves any number of them. */
 int moe_paged_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int head_dim,
                                         size_t* bytes);
 

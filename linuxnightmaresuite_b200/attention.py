@@ -124,7 +124,9 @@ class AttentionLayer:
         self.inv_freq, self.interleaved = inv_freq, interleaved
         self.window, self.softcap, self.scale = window, softcap, scale
         self.device = w_qkv.device
-        self._buf = None
+        # one workspace for all sizes, cleared here and not in a call that a graph captures
+        self._ws = K.paged_attention_workspace(1, q_heads, kv_heads, head_dim, self.device)
+        self._qkv, self._att = K.RowBuffers(), K.RowBuffers()
 
     @classmethod
     def from_blocks(cls, w_q: Array, w_k: Array, w_v: Array, w_o: Array, qtype: int, dim: int,
@@ -144,13 +146,9 @@ class AttentionLayer:
                    q_heads, kv_heads, head_dim, freq, interleaved, window, softcap, scale)
 
     def _buffers(self, T: int):
-        if self._buf is None or self._buf[0].shape[0] != T:
-            hq, hk, d = self.q_heads, self.kv_heads, self.head_dim
-            qkv = torch.empty((T, (hq + 2 * hk) * d), dtype=torch.float32, device=self.device)
-            att = torch.empty((T, hq, d), dtype=torch.float32, device=self.device)
-            ws = K.paged_attention_workspace(T, hq, hk, d, self.device)
-            self._buf = (qkv, att, ws)
-        return self._buf
+        hq, hk, d = self.q_heads, self.kv_heads, self.head_dim
+        return (self._qkv.rows(T, (hq + 2 * hk) * d, self.device),
+                self._att.rows(T, hq * d, self.device).view(T, hq, d), self._ws)
 
     def forward(self, xn: torch.Tensor, cache: PagedKVCache, positions: torch.Tensor,
                 seq_lens: torch.Tensor, residual: Optional[torch.Tensor] = None,
@@ -160,7 +158,8 @@ class AttentionLayer:
         for a plain decode step; position -1 with length 0 is a padding row).
         Returns Wo attention (+ residual); ``out`` may be ``residual``.
         Allocates nothing after the first call of a size (but ``out`` when not
-        given)."""
+        given), and the buffers stay where they are, so captured steps of
+        several sizes can be replayed in any order, one after the other."""
         T = xn.shape[0]
         hq, hk, d = self.q_heads, self.kv_heads, self.head_dim
         qkv, att, ws = self._buffers(T)
@@ -174,4 +173,4 @@ class AttentionLayer:
 
     def device_status(self) -> int:
         """Reads and clears the attention's device status bits (synchronises)."""
-        return 0 if self._buf is None else K.read_status(self._buf[2])
+        return K.read_status(self._ws)

@@ -97,6 +97,30 @@ def workspace(nbytes: int, device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
 
 
+class RowBuffers:
+    """f32 scratch rows of an object that is called with any number of rows.  A
+    captured CUDA graph holds the addresses that its calls used, so no buffer is
+    ever replaced: there is one for each power of two of rows (at most twice the
+    largest in all), and a call uses the first rows of the one that fits."""
+
+    def __init__(self):
+        self._buffers = {}
+        self._rows = {}
+
+    def rows(self, T: int, width: int, device) -> torch.Tensor:
+        """(T, width), the same memory at every call."""
+        key = (T, width, device)
+        t = self._rows.get(key)
+        if t is None:
+            whole = (1 << max(T - 1, 0).bit_length(), width, device)
+            buf = self._buffers.get(whole)
+            if buf is None:
+                buf = self._buffers[whole] = torch.empty(whole[:2], dtype=torch.float32,
+                                                         device=device)
+            t = self._rows[key] = buf[:T]
+        return t
+
+
 def block_geometry(qtype: int) -> Tuple[int, int]:
     e, b = ctypes.c_int(0), ctypes.c_int(0)
     call("moe_block_geometry", qtype, ctypes.byref(e), ctypes.byref(b))
@@ -421,8 +445,8 @@ def rope_inv_freq(rot: int, base: float = 10000.0, factors: Optional[torch.Tenso
 
 def paged_attention_workspace(seqs: int, q_heads: int, kv_heads: int, head_dim: int,
                               device) -> torch.Tensor:
-    """A workspace for ``paged_attention`` calls of these sizes that follow one
-    another (calls that may overlap need one each)."""
+    """A workspace for ``paged_attention`` calls of these heads, with any number
+    of sequences, that follow one another (calls that may overlap need one each)."""
     n = _size_out("moe_paged_attention_workspace_bytes", seqs, q_heads, kv_heads, head_dim)
     return torch.zeros(n, dtype=torch.uint8, device=device)
 
