@@ -31,7 +31,7 @@ class StackedMoE:
                 len(self.attention) == len(self.attention_norms) == len(self.layers)):
             raise ValueError(f"{len(self.attention)} attention layers and "
                              f"{len(self.attention_norms)} norms for {len(self.layers)} MoE layers")
-        self._buf: Optional[torch.Tensor] = None
+        self._xn = K.RowBuffers()
 
     @classmethod
     def from_layers(cls, datas, device=None, eps: float = 1e-6) -> "StackedMoE":
@@ -58,19 +58,18 @@ class StackedMoE:
         """x (T, d) f32 on the device -> (T, d).  The residual stream lives in
         ``out`` (allocated once if not given): the first layer adds x into it,
         later layers update it in place (the combine may write over its own
-        residual input), so a step allocates nothing after the first.
+        residual input), so a step allocates nothing after the first of its
+        size.
 
         With attention layers row t is the new token of sequence t:
         ``caches`` (one per layer), ``positions`` and ``seq_lens`` as
         ``AttentionLayer.forward`` takes them."""
-        if self._buf is None or self._buf.shape != x.shape:
-            self._buf = torch.empty_like(x)
         if self.attention is not None:
             if caches is None or positions is None or seq_lens is None:
                 raise ValueError("attention layers need caches, positions and seq_lens")
             if len(caches) != len(self.layers):
                 raise ValueError(f"{len(caches)} caches for {len(self.layers)} layers")
-        xn = self._buf
+        xn = self._xn.rows(*x.shape, x.device)
         res = out if out is not None else torch.empty_like(x)
         cur = x
         for i, (layer, nw) in enumerate(zip(self.layers, self.norms)):
@@ -93,7 +92,7 @@ class StackedEP:
         self.layers = list(layers)
         self.norms = list(norms)
         self.eps = eps
-        self._buf: Optional[torch.Tensor] = None
+        self._xn = K.RowBuffers()
 
     @classmethod
     def build(cls, cfg, seed: int, tokens: int, group=None, device=None, eps: float = 1e-6,
@@ -143,9 +142,7 @@ class StackedEP:
 
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """As ``StackedMoE.forward``, every layer expert-parallel."""
-        if self._buf is None or self._buf.shape != x.shape:
-            self._buf = torch.empty_like(x)
-        xn = self._buf
+        xn = self._xn.rows(*x.shape, x.device)
         res = out if out is not None else torch.empty_like(x)
         cur = x
         for layer, nw in zip(self.layers, self.norms):

@@ -4,10 +4,12 @@ import gc
 import types
 import weakref
 
+import pytest
 import torch
 
-from linuxnightmaresuite_b200 import build
+from linuxnightmaresuite_b200 import build, kernels as K
 from linuxnightmaresuite_b200.attention import AttentionLayer
+from linuxnightmaresuite_b200.stacked import StackedEP, StackedMoE
 
 
 def _attention(hq=4, hk=2, d=64, dim=128):
@@ -38,3 +40,33 @@ def test_attention_has_one_workspace():
     a, b = layer._buffers(2)[2], layer._buffers(3)[2]
     assert a.data_ptr() == b.data_ptr() and a.numel() == b.numel()
     assert not a.any()
+
+
+class _Step:
+    """Stands for a layer on the host; notes the rows that it is given."""
+
+    def __init__(self, seen):
+        self.seen = seen
+
+    def forward_batch(self, xn, residual=None, out=None):
+        self.seen.append(xn)
+
+    def forward(self, xn, out=None, residual=None):
+        self.seen.append(xn)
+
+
+@pytest.mark.parametrize("kind", [StackedMoE, StackedEP])
+def test_stacked_buffer_of_a_size_stays(kind, monkeypatch):
+    monkeypatch.setattr(K, "rms_norm", lambda x, w, eps, out: out)
+    seen, at, held = [], {}, []
+    stack = kind([_Step(seen)], [None])
+    for T in (2, 3, 2, 1, 64, 7, 2, 3, 1):
+        x = torch.zeros(T, 32)
+        stack.forward(x)
+        xn = seen.pop()
+        assert xn.shape == x.shape
+        assert at.setdefault(T, xn.data_ptr()) == xn.data_ptr()
+        held.append(weakref.ref(xn.untyped_storage()))
+        del xn
+    gc.collect()
+    assert all(r() is not None for r in held)
