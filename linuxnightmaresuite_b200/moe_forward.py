@@ -215,6 +215,7 @@ class MoELayer:
                                       router.top_k, d, F, router.mode, router.bias,
                                       router.layout, sh, sq, Fs, opts)
         self._ws = None
+        self._held: List[torch.Tensor] = []   # workspaces that only captured graphs may still use
 
     @classmethod
     def from_blocks(cls, gate_weight: Array, w_gate: Array, w_up: Array, w_down: Array,
@@ -276,9 +277,19 @@ class MoELayer:
 
     def _workspace(self, T: int) -> torch.Tensor:
         need = self.weights.workspace_bytes(T)
-        if self._ws is None or self._ws.numel() < need:
-            self._ws = torch.zeros(need, dtype=torch.uint8, device=self.router.device)
-        return self._ws
+        if self._ws is not None and self._ws.numel() >= need:
+            return self._ws
+        # Captured graphs hold the addresses of earlier workspaces, so these are
+        # kept; growth by half or more keeps all of them within three times the last
+        size = max(need, 0 if self._ws is None else self._ws.numel() * 3 // 2)
+        ws = torch.zeros(size, dtype=torch.uint8, device=self.router.device)
+        if ws.is_cuda and torch.cuda.is_current_stream_capturing():
+            self._held.append(ws)            # cleared by the graph's replays alone: not for others
+            return ws
+        if self._ws is not None:
+            self._held.append(self._ws)
+        self._ws = ws
+        return ws
 
     def forward_batch(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
                       out: Optional[torch.Tensor] = None, return_routing: bool = False,
@@ -300,7 +311,10 @@ class MoELayer:
 
     def device_status(self) -> int:
         """Reads and clears the device status bits (synchronises)."""
-        return 0 if self._ws is None else K.read_status(self._ws)
+        bits = 0
+        for ws in self._held + ([] if self._ws is None else [self._ws]):
+            bits |= K.read_status(ws)
+        return bits
 
     def forward(self, x: Array):
         xt = _to_dev_f32(x, self.router.device)

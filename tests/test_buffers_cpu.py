@@ -9,6 +9,7 @@ import torch
 
 from linuxnightmaresuite_b200 import build, kernels as K
 from linuxnightmaresuite_b200.attention import AttentionLayer
+from linuxnightmaresuite_b200.moe_forward import MoELayer
 from linuxnightmaresuite_b200.stacked import StackedEP, StackedMoE
 
 
@@ -70,3 +71,37 @@ def test_stacked_buffer_of_a_size_stays(kind, monkeypatch):
         del xn
     gc.collect()
     assert all(r() is not None for r in held)
+
+
+def _moe(monkeypatch):
+    status = {}                                     # by address, as the device would set it
+    layer = MoELayer.__new__(MoELayer)
+    layer.router = types.SimpleNamespace(device=torch.device("cpu"))
+    layer._ws, layer._held = None, []
+    layer.weights = types.SimpleNamespace(workspace_bytes=lambda T: 256 + 100 * T)
+    monkeypatch.setattr(K, "read_status", lambda ws: status.pop(ws.data_ptr(), 0))
+    return layer, status
+
+
+def test_moe_workspace_that_a_graph_may_hold_stays(monkeypatch):
+    """A larger batch brings a larger workspace; the one before is kept, and what
+    a replayed graph reports into it is read."""
+    layer, status = _moe(monkeypatch)
+    assert layer.device_status() == 0
+    held, total = [], 0
+    for T in list(range(1, 200)) + [5, 1]:
+        ws = layer._workspace(T)
+        assert ws.numel() >= 256 + 100 * T and ws.dtype == torch.uint8 and not ws[:256].any()
+        if not any(r() is ws.untyped_storage() for r in held):
+            held.append(weakref.ref(ws.untyped_storage()))
+            total += ws.numel()
+        first = ws if T == 1 and len(held) == 1 else first
+        last = ws
+        del ws
+    gc.collect()
+    assert all(r() is not None for r in held)
+    assert last.numel() >= 256 + 100 * 199 and total <= 4 * last.numel()   # growth by halves
+    status[first.data_ptr()] = 1
+    status[last.data_ptr()] = 4
+    assert layer.device_status() == 5
+    assert layer.device_status() == 0

@@ -6,7 +6,6 @@ import math
 import pytest
 import torch
 
-from linuxnightmaresuite_b200 import kernels as K
 from linuxnightmaresuite_b200.attention import PagedKVCache
 
 from ._attention import F16
@@ -75,3 +74,41 @@ def test_attention_layer_two_sizes_captured():
         return lambda x, out, c, pos, lens: layer.forward(x, c[0], pos, lens, residual=x, out=out)
     _two_sizes(run(one), run(two), _caches(1, 8), _caches(1, 8))
     assert one.device_status() == 0 and two.device_status() == 0
+
+
+def _step(stack):
+    return lambda x, out, c, pos, lens: stack.forward(x, out=out, caches=c, positions=pos,
+                                                      seq_lens=lens)
+
+
+def test_decoder_two_sizes_captured():
+    one, two = (_decoder(F16, 2)[0] for _ in range(2))
+    _two_sizes(_step(one), _step(two), _caches(2, 8), _caches(2, 8))
+    for layer in one.attention + two.attention + one.layers + two.layers:
+        assert layer.device_status() == 0
+
+
+def test_first_call_captured():
+    """Layers whose first call is captured: what the graph's replays clear is not
+    there for calls before the first of them."""
+    warm, stack = (_decoder(F16, 2)[0] for _ in range(2))
+    caches, alone = _caches(2, 3), _caches(2, 3)
+    x, out = randn(3, 512, seed=1), torch.empty((3, 512), device="cuda")
+    pos = torch.zeros(3, dtype=torch.int32, device="cuda")
+    lens = pos + 1
+    want = torch.empty_like(out)
+    _step(warm)(x, want, alone, pos, lens)          # what the library loads at its first calls
+    others = _others(math.nan)
+    del others
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        _step(stack)(x, out, caches, pos, lens)
+    eager = torch.empty_like(out)
+    _step(stack)(x, eager, caches, pos, lens)
+    assert torch.equal(eager, want)
+    assert all(layer.device_status() == 0 for layer in stack.attention)
+    for _ in range(3):
+        out.fill_(math.nan)
+        g.replay()
+        assert torch.equal(out, want)
+    assert all(layer.device_status() == 0 for layer in stack.layers)
