@@ -398,7 +398,9 @@ int moe_ep_forward_phases(const moe_layer_weights* w, int W, int rank, void* con
  * block_table[s * table_stride + p / page_size], slot p % page_size; entries
  * behind a sequence's last page are never read, and a page may belong to
  * several sequences.  Bases and strides must be multiples of 16 bytes; head_dim
- * a multiple of 8 (16 for MOE_CACHE_E4M3), at most 256.  MOE_CACHE_E4M3 holds value / scale, rounded to nearest even and
+ * a multiple of 8 (16 for MOE_CACHE_E4M3), at most 256.  The slots of a page
+ * have memory of their own (no token stride of 0); for the append so have pages
+ * and heads.  MOE_CACHE_E4M3 holds value / scale, rounded to nearest even and
  * saturated at +-448; the scales of the other types must be 1.
  * A page id outside [0, pages) sets MOE_STATUS_BAD_PAGE; its slots are neither
  * read nor written. */

@@ -44,11 +44,24 @@ inline int check_cache(const moe_paged_cache& c) {
               MOE_ERR_INVALID, "cache bases and strides must be multiples of 16 bytes");
   MOE_REQUIRE(c.page_stride >= 0 && c.token_stride >= 0 && c.head_stride >= 0, MOE_ERR_INVALID,
               "negative cache stride");
+  // a tensor map holds no stride of 0 (pages and heads are counted in rows)
+  MOE_REQUIRE(c.page_size == 1 || c.token_stride > 0, MOE_ERR_INVALID,
+              "slots of a page share memory (token stride 0)");
   if (c.dtype == MOE_CACHE_E4M3)
     MOE_REQUIRE(c.k_scale > 0.f && c.v_scale > 0.f, MOE_ERR_INVALID, "cache scales must be > 0");
   else
     MOE_REQUIRE(c.k_scale == 1.f && c.v_scale == 1.f, MOE_ERR_INVALID,
                 "only an e4m3 cache has scales");
+  return MOE_OK;
+}
+
+// An append writes each row of head_dim elements by itself.
+inline int check_cache_rows_apart(const moe_paged_cache& c) {
+  const int64_t d = c.head_dim;
+  MOE_REQUIRE((c.pages == 1 || c.page_stride >= d) && (c.page_size == 1 || c.token_stride >= d) &&
+                  (c.kv_heads == 1 || c.head_stride >= d),
+              MOE_ERR_INVALID, "rows of the cache share memory: strides (%lld, %lld, %lld)",
+              (long long)c.page_stride, (long long)c.token_stride, (long long)c.head_stride);
   return MOE_OK;
 }
 

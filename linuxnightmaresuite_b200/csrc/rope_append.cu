@@ -207,6 +207,7 @@ int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_
                     moe_stream_t stream) {
   MOE_REQUIRE(cache, MOE_ERR_INVALID, "null cache");
   MOE_CHECK(moe::check_cache(*cache));
+  MOE_CHECK(moe::check_cache_rows_apart(*cache));
   MOE_REQUIRE(T >= 0 && q_heads >= 0, MOE_ERR_INVALID, "negative size");
   MOE_REQUIRE(q_heads <= 32767 && cache->kv_heads <= 16383, MOE_ERR_UNSUPPORTED, "too many heads");
   MOE_REQUIRE(rot >= 0 && rot % 2 == 0 && rot <= cache->head_dim, MOE_ERR_INVALID,

@@ -228,3 +228,25 @@ def test_records_reach_the_same_checks(lib):
     assert lib.moe_linear_record(ctypes.byref(w)) == _lib.MOE_OK
     w.cols = 65
     assert lib.moe_linear_record(ctypes.byref(w)) == _lib.MOE_ERR_UNSUPPORTED
+
+
+def test_slots_that_share_memory_are_refused(lib):
+    """A token stride of 0 with several slots per page: the tensor map of the
+    attention cannot hold it, an append would write its slots over one another.
+    Rows closer than head_dim are nothing to append to either."""
+    for kw in (dict(token_stride=0), dict(token_stride=0, page_stride=128, pages=2)):
+        for call in (attention, append):
+            assert call(lib, cache(**kw)) == _lib.MOE_ERR_INVALID, kw
+            assert "share memory" in _lib.last_error()
+    for kw in (dict(page_stride=0), dict(head_stride=0), dict(head_stride=56), dict(token_stride=8),
+               dict(page_stride=32)):
+        assert append(lib, cache(**kw)) == _lib.MOE_ERR_INVALID, kw
+        assert "share memory" in _lib.last_error()
+    # one slot, one head, one page: no stride that counts; T = 0 stops behind the checks
+    assert append(lib, cache(page_size=1, token_stride=0), T=0) == _lib.MOE_OK
+    assert append(lib, cache(kv_heads=1, head_stride=0), T=0) == _lib.MOE_OK
+    assert append(lib, cache(pages=1, page_stride=0), T=0) == _lib.MOE_OK
+    # the attention only reads: one head for all, one page for all
+    for kw in (dict(page_stride=0), dict(head_stride=0)):
+        assert attention(lib, cache(**kw), ws=None) == _lib.MOE_ERR_INVALID
+        assert "null pointer" in _lib.last_error()
