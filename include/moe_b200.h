@@ -461,7 +461,7 @@ int moe_paged_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int
  *   out (seqs, q_heads, head_dim) f32 contiguous; lse (seqs, q_heads) or NULL
  *   the cache's strides must be multiples of a common row of head_dim elements
  *          or more (every dense layout, also with padded rows or pages)
- *   workspace: zeroed by the caller before its first use and then kept between
+ *   workspace: 16-byte aligned, zeroed by the caller before its first use and then kept between
  *          calls, which leave it ready for the next one (but for the status
  *          word at its start); calls that may overlap need one each
  * The split of a sequence over the GPU depends on the lengths and the device

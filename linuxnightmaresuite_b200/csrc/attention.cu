@@ -1102,6 +1102,8 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
               "scale and softcap must be finite, softcap >= 0");
   if (cache->seqs == 0) return MOE_OK;
   MOE_REQUIRE(q && seq_lens && out && workspace, MOE_ERR_INVALID, "null pointer");
+  // parts in it are fetched by bulk copies
+  MOE_REQUIRE((uintptr_t)workspace % 16 == 0, MOE_ERR_INVALID, "workspace must be 16-byte aligned");
   moe::AttArgs a = {};
   a.c = *cache;
   a.q = q;

@@ -250,3 +250,11 @@ def test_slots_that_share_memory_are_refused(lib):
     for kw in (dict(page_stride=0), dict(head_stride=0)):
         assert attention(lib, cache(**kw), ws=None) == _lib.MOE_ERR_INVALID
         assert "null pointer" in _lib.last_error()
+
+
+def test_workspace_off_its_alignment_is_refused(lib):
+    """Parts of units are fetched from the workspace by bulk copies, whose source
+    must lie on 16 bytes."""
+    for at in (257, 260, 264):
+        assert attention(lib, cache(), ws=ctypes.c_void_p(at)) == _lib.MOE_ERR_INVALID
+        assert "16-byte" in _lib.last_error()
