@@ -1093,8 +1093,8 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
                         int64_t q_head_stride, const int32_t* seq_lens, int q_heads, int max_len,
                         int window, float scale, float softcap, float* out, float* lse,
                         void* workspace, size_t workspace_bytes, moe_stream_t stream) {
-  MOE_REQUIRE(cache, MOE_ERR_INVALID, "null cache");
-  MOE_CHECK(moe::check_cache(*cache));
+  moe::AttArgs a = {};
+  MOE_CHECK(moe::take_cache(cache, a.c));
   MOE_REQUIRE(q_heads > 0 && q_heads % cache->kv_heads == 0, MOE_ERR_INVALID,
               "%d query heads for %d key heads", q_heads, cache->kv_heads);
   MOE_REQUIRE(max_len >= 0 && window >= 0, MOE_ERR_INVALID, "negative length or window");
@@ -1104,8 +1104,6 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
   MOE_REQUIRE(q && seq_lens && out && workspace, MOE_ERR_INVALID, "null pointer");
   // parts in it are fetched by bulk copies
   MOE_REQUIRE((uintptr_t)workspace % 16 == 0, MOE_ERR_INVALID, "workspace must be 16-byte aligned");
-  moe::AttArgs a = {};
-  a.c = *cache;
   a.q = q;
   a.q_ss = q_seq_stride;
   a.q_hs = q_head_stride;
@@ -1117,7 +1115,6 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
   a.window = window;
   a.scale = scale;
   a.cap = softcap;
-  moe::normalise_strides(a.c);
   size_t need = 0;
   MOE_CHECK(moe::attention_workspace(cache->head_dim, &a, workspace, &need));
   MOE_REQUIRE(workspace_bytes >= need, MOE_ERR_WORKSPACE, "workspace %zu < %zu bytes",

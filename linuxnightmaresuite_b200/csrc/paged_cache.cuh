@@ -25,7 +25,11 @@ inline void normalise_strides(moe_paged_cache& c) {
   if (c.kv_heads == 1) c.head_stride = 0;
 }
 
-inline int check_cache(const moe_paged_cache& c) {
+// The cache as the kernels take it, or an error.
+inline int take_cache(const moe_paged_cache* cache, moe_paged_cache& c) {
+  MOE_REQUIRE(cache, MOE_ERR_INVALID, "null cache");
+  c = *cache;
+  normalise_strides(c);
   MOE_REQUIRE(c.dtype >= MOE_CACHE_F16 && c.dtype <= MOE_CACHE_E4M3, MOE_ERR_UNSUPPORTED,
               "cache type %d not supported", c.dtype);
   MOE_REQUIRE(c.k && c.v && c.block_table, MOE_ERR_INVALID, "null cache pointer");

@@ -205,9 +205,9 @@ int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_
                     const int32_t* seq_ids, const double* inv_freq, int rot, int interleaved,
                     float* q_out, int64_t qo_tok_stride, int64_t qo_head_stride, int32_t* status,
                     moe_stream_t stream) {
-  MOE_REQUIRE(cache, MOE_ERR_INVALID, "null cache");
-  MOE_CHECK(moe::check_cache(*cache));
-  MOE_CHECK(moe::check_cache_rows_apart(*cache));
+  moe_paged_cache c;
+  MOE_CHECK(moe::take_cache(cache, c));
+  MOE_CHECK(moe::check_cache_rows_apart(c));
   MOE_REQUIRE(T >= 0 && q_heads >= 0, MOE_ERR_INVALID, "negative size");
   MOE_REQUIRE(q_heads <= 32767 && cache->kv_heads <= 16383, MOE_ERR_UNSUPPORTED, "too many heads");
   MOE_REQUIRE(rot >= 0 && rot % 2 == 0 && rot <= cache->head_dim, MOE_ERR_INVALID,
@@ -217,10 +217,9 @@ int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_
   MOE_REQUIRE(q_heads == 0 || (q && q_out), MOE_ERR_INVALID, "null q or q_out");
   MOE_REQUIRE(seq_ids || T <= cache->seqs, MOE_ERR_INVALID,
               "%d tokens for %d sequences need seq_ids", T, cache->seqs);
-  moe::RopeArgs a = {*cache, q, k, v, q_tok_stride, q_head_stride, k_tok_stride, k_head_stride,
+  moe::RopeArgs a = {c, q, k, v, q_tok_stride, q_head_stride, k_tok_stride, k_head_stride,
                      v_tok_stride, v_head_stride, qo_tok_stride, qo_head_stride, q_out, positions,
                      seq_ids, inv_freq, status, q_heads, rot, interleaved};
-  moe::normalise_strides(a.c);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   {
     ::moe::ProfScope _prof(MOE_K_ROPE_APPEND, s);

@@ -365,7 +365,8 @@ def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torc
     shape, strides = k_cache.shape, k_cache.stride()
     if v_cache.dtype is not dtype or v_cache.get_device() != index:
         _refuse(v_cache, "v_cache", dtype, index)
-    if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != strides:
+    if len(shape) != 4 or v_cache.shape != shape or (v_cache.stride() != strides and any(
+            a != b and n > 1 for a, b, n in zip(strides, v_cache.stride(), shape))):
         raise ValueError("k_cache and v_cache must be (pages, page_size, kv_heads, head_dim) of "
                          "the same shape and strides")
     if strides[3] != 1 and shape[3] > 1:

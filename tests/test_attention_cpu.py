@@ -258,3 +258,14 @@ def test_workspace_off_its_alignment_is_refused(lib):
     for at in (257, 260, 264):
         assert attention(lib, cache(), ws=ctypes.c_void_p(at)) == _lib.MOE_ERR_INVALID
         assert "16-byte" in _lib.last_error()
+
+
+@pytest.mark.parametrize("axis", [dict(pages=1, page_stride=3), dict(page_size=1, token_stride=-5),
+                                  dict(kv_heads=1, head_stride=7),
+                                  dict(pages=1, page_stride=1, page_size=1, token_stride=-1,
+                                       kv_heads=1, head_stride=0)])
+def test_strides_of_single_axes_are_ignored(lib, axis):
+    c = cache(**axis)
+    assert append(lib, c, T=0) == _lib.MOE_OK
+    assert attention(lib, c, ws=None) == _lib.MOE_ERR_INVALID    # behind the cache's checks
+    assert "null pointer" in _lib.last_error()

@@ -1,0 +1,66 @@
+"""Forms of the attention half's arguments that the documentation allows: odd
+strides of single axes, heads and pages that share memory, status without a
+workspace, infinities."""
+import pytest
+import torch
+
+from linuxnightmaresuite_b200 import _lib, kernels as K
+
+from ._attention import BF16, E4M3, F16, Cache, check_attention
+from .test_gpu_attention import randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [F16, E4M3])
+def test_strides_of_single_axes(dtype):
+    """One key head, one slot per page, one page: their strides count for nothing,
+    in either cache."""
+    d = 64
+    for page, lens in ((16, [40, 3]), (1, [5, 2]), (64, [50])):
+        c = Cache(lens, page, 1, d, dtype, seed=page, spare=0)
+        q = randn(len(lens), 4, d, seed=page)
+        want = K.paged_attention(q, *c.args, c.lens, **c.scales)
+        check_attention(c, q, want, None, d ** -0.5)
+
+        def odd(t, at):
+            s = [t.stride(0), t.stride(1), at, 1]
+            for i in (0, 1):
+                if t.shape[i] == 1:
+                    s[i] = at + i
+            return t.as_strided(t.shape, s)
+        k, v = odd(c.k, 3), odd(c.v, 5)
+        assert torch.equal(K.paged_attention(q, k, v, c.table_d, c.lens, **c.scales), want)
+        kn, pos = randn(len(lens), 1, d, seed=1), c.lens - 1
+        K.rope_append(None, kn, kn, k, v, c.table_d, pos, **c.scales)
+        got = c.k.view(torch.uint8).clone()
+        K.rope_append(None, kn, kn, *c.args, pos, **c.scales)
+        assert torch.equal(got, c.k.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_heads_and_pages_that_share_memory(dtype):
+    """The attention only reads: one head stands for all key heads, one page for all."""
+    hkv, d, page = 4, 128, 16
+    c = Cache([70, 33, 0], page, 1, d, dtype, seed=2)
+    q = randn(3, 8, d, seed=2)
+    k, v = (t.expand(-1, -1, hkv, -1) for t in (c.k, c.v))
+    wide = type("C", (), dict(kd=[x.expand(-1, hkv, -1) for x in c.kd],
+                              vd=[x.expand(-1, hkv, -1) for x in c.vd]))
+    out, lse = K.paged_attention(q, k, v, c.table_d, c.lens, return_lse=True)
+    check_attention(wide, q, out, lse, d ** -0.5)
+    one = Cache([page], page, 1, d, dtype, seed=3, spare=0)
+    k, v = (t.expand(5, -1, -1, -1) for t in (one.k, one.v))
+    table = torch.tensor([[4, 0, 3, 1]], dtype=torch.int32).cuda()
+    lens = torch.tensor([3 * page + 5], dtype=torch.int32).cuda()
+    many = type("C", (), dict(kd=[one.kd[0].repeat(4, 1, 1)[:lens.item()]],
+                              vd=[one.vd[0].repeat(4, 1, 1)[:lens.item()]]))
+    out = K.paged_attention(q[:1], k, v, table, lens)
+    check_attention(many, q[:1], out, None, d ** -0.5)
+    for k, v in ((c.k.expand(-1, -1, hkv, -1),) * 2, (one.k.expand(5, -1, -1, -1),) * 2):
+        new = torch.zeros((1, k.shape[2], d), device="cuda")
+        with pytest.raises(_lib.MoEError, match="share memory"):
+            K.rope_append(None, new, new, k, v, table, table[0, :1])
+    with pytest.raises(_lib.MoEError, match="share memory"):
+        t = c.k[:, :1].expand(-1, page, -1, -1)
+        K.paged_attention(q, t, t, c.table_d, c.lens)
