@@ -92,13 +92,15 @@ class PagedKVCache:
                out: Optional[torch.Tensor] = None, return_lse: bool = False,
                ws: Optional[torch.Tensor] = None):
         """``kernels.paged_attention`` over this cache; q has a row for each
-        of the first ``q.shape[0]`` sequences."""
+        of the first ``q.shape[0]`` sequences.  Without ``ws`` one is made for
+        the call, and its status bits go where the append's do."""
         return K.paged_attention(q, self.k, self.v, self.block_table[:q.shape[0]], seq_lens, scale,
                                  window, softcap, self.k_scale, self.v_scale, max_len, out,
-                                 return_lse, ws)
+                                 return_lse, ws, self.status if ws is None else None)
 
     def device_status(self) -> int:
-        """Reads and clears the append's device status bits (synchronises)."""
+        """Reads and clears the device status bits of the appends and of the
+        attention calls without a workspace (synchronises)."""
         st = int(self.status.item())
         self.status.zero_()
         return st

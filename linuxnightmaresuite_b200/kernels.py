@@ -457,14 +457,17 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     scale: Optional[float] = None, window: int = 0, softcap: float = 0.0,
                     k_scale: float = 1.0, v_scale: float = 1.0, max_len: int = 0,
                     out: Optional[torch.Tensor] = None, return_lse: bool = False,
-                    ws: Optional[torch.Tensor] = None):
+                    ws: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None):
     """Attention of one new token per sequence, q (seqs, q_heads, head_dim),
     over the first ``seq_lens[s]`` tokens of its pages (the last ``window`` of
     them if given): softmax(scale q.k, capped at ``softcap``) v, f32.  Returns
     out, or (out, lse) with the natural log of the softmax sums; a sequence of
     length 0 gives zeros and -inf.  ``scale`` defaults to 1 / sqrt(head_dim);
     ``max_len`` (no sequence is longer; 0 = what the table holds) sizes the
-    launch.  ``ws`` comes from ``paged_attention_workspace``."""
+    launch.  ``ws`` comes from ``paged_attention_workspace``.  Its first word
+    gathers status bits (``read_status``: STATUS_BAD_PAGE for a page that does
+    not exist or a length that the table does not hold); ``status`` (int32)
+    receives them too, by a small launch of its own, for calls without ``ws``."""
     c, dev, seqs, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
     shape = q.shape
     if len(shape) != 3:
@@ -481,10 +484,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         ws = paged_attention_workspace(seqs, hq, hk, d, q.device)
     elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
         _refuse(ws, "ws", torch.uint8, dev)
+    if status is not None:
+        _vector(status, _I32, "status", dev, 1)
     _enqueue("moe_paged_attention_record", dev, _ATTENTION_ARGS.pack(
         *c, q.data_ptr(), qs[0], qs[1], _vector(seq_lens, _I32, "seq_lens", dev, seqs),
         out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
         _raw_stream(dev), hq, max_len, window, d ** -0.5 if scale is None else scale, softcap))
+    if status is not None and seqs:
+        status |= ws[:4].view(_I32)
     return (out, lse) if return_lse else out
 
 

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from linuxnightmaresuite_b200 import _lib, kernels as K
+from linuxnightmaresuite_b200.attention import PagedKVCache
 
 from ._attention import BF16, E4M3, F16, Cache, check_attention
 from .test_gpu_attention import randn
@@ -64,3 +65,25 @@ def test_heads_and_pages_that_share_memory(dtype):
     with pytest.raises(_lib.MoEError, match="share memory"):
         t = c.k[:, :1].expand(-1, page, -1, -1)
         K.paged_attention(q, t, t, c.table_d, c.lens)
+
+
+def test_status_without_a_workspace():
+    """A page that does not exist is reported also where no workspace is kept."""
+    cache = PagedKVCache(8, 4, 2, 64, max_seqs=2, dtype=F16)
+    cache.reserve(0, 8)
+    q, lens = randn(2, 4, 64), torch.tensor([8, 0], dtype=torch.int32).cuda()
+    cache.attend(q, lens)
+    assert cache.device_status() == 0
+    lens[1] = 3                                     # no page was reserved
+    cache.attend(q, lens)
+    assert cache.device_status() == K.STATUS_BAD_PAGE
+    assert cache.device_status() == 0
+    ws = K.paged_attention_workspace(2, 4, 2, 64, "cuda")
+    cache.attend(q, lens, ws=ws)                    # in the workspace, where one is given
+    assert cache.device_status() == 0 and K.read_status(ws) == K.STATUS_BAD_PAGE
+    for w in (None, ws):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        K.paged_attention(q, cache.k, cache.v, cache.block_table, lens, ws=w, status=status)
+        assert status.item() == K.STATUS_BAD_PAGE
+    with pytest.raises(TypeError):
+        K.paged_attention(q, cache.k, cache.v, cache.block_table, lens, status=status.float())
