@@ -635,6 +635,36 @@ static int launch_linear_qt(LinArgs& a, cudaStream_t s) {
   return MOE_OK;
 }
 
+// n rows of f32 at a pointer, `width` elements each, `stride` apart.
+struct Rows {
+  const float* p;
+  int64_t stride, width, n;
+};
+
+// Whether a row of a shares memory with a row of b.  Side by side in one buffer
+// their spans may meet although no rows do, so rows are compared then.
+static bool rows_overlap(Rows a, Rows b) {
+  auto upward = [](Rows& r) {                    // the same rows in rising order
+    if (r.stride < 0) {
+      r.p += (r.n - 1) * r.stride;
+      r.stride = -r.stride;
+    }
+  };
+  upward(a);
+  upward(b);
+  const int64_t d = (int64_t)((uintptr_t)b.p - (uintptr_t)a.p);   // bytes, as all from here on
+  const int64_t as = 4 * a.stride, aw = 4 * a.width, bs = 4 * b.stride, bw = 4 * b.width;
+  if (d >= (a.n - 1) * as + aw || d + (b.n - 1) * bs + bw <= 0) return false;
+  for (int64_t i = 0; i < a.n; ++i) {
+    const int64_t lo = i * as - bw - d, hi = i * as + aw - d;      // lo < offset of b's row < hi
+    if (bs == 0 ? lo < 0 && 0 < hi
+                : std::max<int64_t>(0, lo < 0 ? 0 : lo / bs + 1) <=
+                      std::min(b.n - 1, hi <= 0 ? -1 : (hi - 1) / bs))
+      return true;
+  }
+  return false;
+}
+
 }  // namespace moe
 
 extern "C" int moe_linear(const uint8_t* w, int qtype, int rows, int cols, const float* x,
@@ -648,6 +678,13 @@ extern "C" int moe_linear(const uint8_t* w, int qtype, int rows, int cols, const
   MOE_REQUIRE(w && x && y, MOE_ERR_INVALID, "null pointer");
   MOE_REQUIRE((uintptr_t)w % 16 == 0, MOE_ERR_INVALID, "w must be 16-byte aligned");
   MOE_REQUIRE(T <= 65535 * 4, MOE_ERR_UNSUPPORTED, "%d rows of x are too many", T);
+  MOE_REQUIRE(T == 1 || y_stride >= rows || -y_stride >= rows, MOE_ERR_INVALID,
+              "rows of y overlap");
+  const moe::Rows yr = {y, y_stride, rows, T};
+  MOE_REQUIRE(!moe::rows_overlap({x, x_stride, cols, T}, yr), MOE_ERR_INVALID, "x and y overlap");
+  MOE_REQUIRE(!residual || (residual == y && (T == 1 || residual_stride == y_stride)) ||
+                  !moe::rows_overlap({residual, residual_stride, rows, T}, yr),
+              MOE_ERR_INVALID, "residual and y overlap, and are not the same rows");
   moe::LinArgs a = {};
   a.w = w;
   a.x = x;

@@ -215,6 +215,15 @@ int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_
   if (T == 0) return MOE_OK;
   MOE_REQUIRE(k && v && positions && (rot == 0 || inv_freq), MOE_ERR_INVALID, "null pointer");
   MOE_REQUIRE(q_heads == 0 || (q && q_out), MOE_ERR_INVALID, "null q or q_out");
+  if (q_heads > 0) {
+    MOE_REQUIRE((T == 1 || qo_tok_stride >= c.head_dim || -qo_tok_stride >= c.head_dim) &&
+                    (q_heads == 1 || qo_head_stride >= c.head_dim || -qo_head_stride >= c.head_dim),
+                MOE_ERR_INVALID, "rows of q_out overlap");
+    MOE_REQUIRE(q_out != q || ((T == 1 || qo_tok_stride == q_tok_stride) &&
+                               (q_heads == 1 || qo_head_stride == q_head_stride)),
+                MOE_ERR_INVALID, "q_out is q with other strides");
+    MOE_REQUIRE(q_out != k && q_out != v, MOE_ERR_INVALID, "q_out overlaps k or v");
+  }
   MOE_REQUIRE(seq_ids || T <= cache->seqs, MOE_ERR_INVALID,
               "%d tokens for %d sequences need seq_ids", T, cache->seqs);
   moe::RopeArgs a = {c, q, k, v, q_tok_stride, q_head_stride, k_tok_stride, k_head_stride,

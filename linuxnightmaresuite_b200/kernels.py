@@ -391,7 +391,7 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     """Rotates q (T, q_heads, head_dim) and k (T, kv_heads, head_dim) by their
     positions, writes k and v into the paged caches (pages, page_size,
     kv_heads, head_dim; any page layout as a view) and returns the rotated q
-    (``q_out``, which may be q itself).
+    (``q_out``, which may be q itself but may not share memory with k or v).
 
     ``inv_freq`` (rot / 2,) f64 holds the angle of each pair per position
     (``rope_inv_freq``); None rotates nothing.  Pairs are (i, i + rot / 2), or
@@ -521,7 +521,8 @@ class LinearWeights:
 def linear(x: torch.Tensor, w: LinearWeights, residual: Optional[torch.Tensor] = None,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x (T, cols) f32 -> (T, rows) f32: W x[t] (+ residual[t]) for a few rows.
-    Rows of x, residual and out may stride; out may be residual."""
+    Rows of x, residual and out may stride; out may be residual, but may not
+    share memory with x."""
     shape = x.shape
     if len(shape) != 2:
         raise ValueError("x must be (tokens, cols)")

@@ -269,3 +269,40 @@ def test_strides_of_single_axes_are_ignored(lib, axis):
     assert append(lib, c, T=0) == _lib.MOE_OK
     assert attention(lib, c, ws=None) == _lib.MOE_ERR_INVALID    # behind the cache's checks
     assert "null pointer" in _lib.last_error()
+
+
+def test_linear_rows_that_overlap_are_refused(lib):
+    """y is written while x is still read.  The calls that pass the check are too
+    wide for any kernel, so nothing is launched."""
+    cols, rows, base = 1 << 21, 1 << 20, 1 << 40
+
+    def lin(x=0, xs=cols, y=1 << 30, ys=rows, T=1, res=None, rs=0):
+        at = [None if e is None else ctypes.c_void_p(base + 4 * e) for e in (x, y, res)]
+        return lib.moe_linear(P, 2, rows, cols, at[0], xs, T, at[2], rs, at[1], ys, None)
+    both = cols + rows                              # x and y side by side in one buffer
+    for kw in (dict(y=0), dict(y=cols - 1), dict(y=1 - rows), dict(y=0, T=3, ys=both, xs=both),
+               dict(y=3 * cols, T=4), dict(y=cols - 1, T=3, ys=both, xs=both),
+               dict(T=2, ys=rows - 1), dict(T=2, ys=0),                       # rows of y
+               dict(res=(1 << 30) + 1), dict(res=(1 << 30) - rows + 1),       # residual
+               dict(res=1 << 30, rs=rows + 8, T=2), dict(res=(1 << 30) + rows, rs=rows, T=2)):
+        assert lin(**kw) == _lib.MOE_ERR_INVALID, kw
+        assert "overlap" in _lib.last_error()
+    for kw in (dict(), dict(y=cols), dict(y=-rows), dict(y=cols, T=3, xs=both, ys=both),
+               dict(y=-rows, T=3, xs=both, ys=both), dict(xs=0, T=5), dict(T=1, ys=0),
+               dict(y=cols, T=2, xs=2 * both, ys=2 * both),
+               dict(res=1 << 30, rs=rows, T=2), dict(res=1 << 30, rs=7), dict(res=0, rs=rows, T=2),
+               dict(res=(1 << 30) + rows), dict(res=(1 << 30) + rows, rs=2 * rows, T=2, ys=2 * rows)):
+        assert lin(**kw) not in (_lib.MOE_ERR_INVALID, _lib.MOE_OK), (kw, _lib.last_error())
+        assert "overlap" not in _lib.last_error()
+
+
+def test_rotated_q_that_overlaps_is_refused(lib):
+    def rope(q=1024, k=4096, v=8192, out=1024, qs=(256, 64), os=(256, 64), T=2, hq=4):
+        at = [ctypes.c_void_p(a) for a in (q, k, v, out)]
+        return lib.moe_rope_append(ctypes.byref(cache()), at[0], *qs, at[1], 128, 64, at[2], 128,
+                                   64, T, hq, P, None, P, 64, 0, at[3], *os, None, None)
+    for kw in (dict(out=4096), dict(out=8192), dict(out=2048, os=(0, 64)),
+               dict(out=2048, os=(256, 0)), dict(out=2048, os=(256, 60)), dict(os=(512, 64)),
+               dict(os=(256, 128)), dict(qs=(0, 64))):
+        assert rope(**kw) == _lib.MOE_ERR_INVALID, kw
+        assert "q_out" in _lib.last_error()

@@ -87,3 +87,25 @@ def test_status_without_a_workspace():
         assert status.item() == K.STATUS_BAD_PAGE
     with pytest.raises(TypeError):
         K.paged_attention(q, cache.k, cache.v, cache.block_table, lens, status=status.float())
+
+
+def test_outputs_over_inputs():
+    """x and the output side by side in one buffer; an output over its own input
+    is refused before anything is written."""
+    lw = K.LinearWeights(torch.randint(0, 255, (64 * 2 * 18,), dtype=torch.uint8).cuda(), 2, 64, 64)
+    buf = randn(3, 128)
+    keep = buf.clone()
+    want = K.linear(keep[:, :64].contiguous(), lw)
+    got = K.linear(buf[:, :64], lw, out=buf[:, 64:])
+    assert torch.equal(got.view(torch.int32), want.view(torch.int32))    # NaN among the scales
+    assert torch.equal(buf[:, :64], keep[:, :64])
+    x = keep[:, :64].contiguous()
+    for out in (x, buf.view(-1)[1:].as_strided((3, 64), (128, 1))):
+        with pytest.raises(_lib.MoEError, match="overlap"):
+            K.linear(x if out is x else buf[:, :64], lw, out=out)
+    assert torch.equal(x, keep[:, :64])
+    c = Cache([8, 8], 4, 2, 64, F16)
+    q, k, pos = randn(2, 2, 64), randn(2, 2, 64, seed=1), c.lens - 1
+    for out in (k, q.transpose(0, 1), q[:1].expand(2, 2, 64)):
+        with pytest.raises(_lib.MoEError, match="q_out"):
+            K.rope_append(q, k, k.clone(), *c.args, pos, K.rope_inv_freq(64), q_out=out)
