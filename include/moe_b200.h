@@ -477,7 +477,8 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
  *      moe_pack_weights
  *   x (T, cols), y (T, rows), residual (T, rows) or NULL: rows at the given
  *      strides (elements); residual may be y itself with the same stride;
- *      y must not overlap x or w
+ *      y must not overlap x or w.  An infinity or NaN in x gives what the sum
+ *      of the products gives, in its own row
  * Made for a few rows: the weights are read once for every 16 of them (8 or 4
  * where x is so wide that 16 do not fit).  32768 columns always fit; much wider
  * ones are MOE_ERR_UNSUPPORTED.  Should a copy never arrive, y is NaN. */

@@ -28,6 +28,7 @@
 // 8.5 where the MMAs alone take 4.3, meetings 3.3).
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "packed_tiles.cuh"
 
@@ -84,7 +85,7 @@ template <int NBG, int G> struct LinCfg {
 };
 
 // x columns [64 t0, 64 t1) of n rows -> fragments `rec` ([block][column group] of
-// 512 bytes); a row times 2^ex has its largest |x| in [2^14, 2^15).
+// 512 bytes); a row times 2^ex has its largest finite |x| in [2^14, 2^15).
 template <int QT, int NBG, int G>
 __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, int rec_blocks,
                                                 int* ex, uint32_t* smax, int row0, int n, int t0,
@@ -144,12 +145,26 @@ __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, 
   if (!on) return;
   mx = 0;
   for (int i = 0; i < wpr; ++i) mx = max(mx, smax[row * wpr + i]);
-  const int eb = (int)(mx >> 23);                // biased exponent; 255: Inf or NaN
-  const int e = mx == 0 || eb == 255 ? 0 : 141 - max(eb, 1);
+  const bool special = mx >= 0x7f800000u;        // Inf or NaN: the scale goes by the others,
+  if (special) {                                 // which each warp of the row looks up for itself
+    mx = 0;
+    for (int b = lane >> 2; b < real; b += 8) {
+      float v[8];
+      values(b, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t u = __float_as_uint(fabsf(v[k]));
+        if (u < 0x7f800000u) mx = max(mx, u);
+      }
+    }
+    mx = __reduce_max_sync(0xffffffffu, mx);
+  }
+  const int eb = (int)(mx >> 23);                // biased exponent
+  const int e = mx == 0 ? 0 : 141 - max(eb, 1);
   const float f1 = pow2f(e / 2), f2 = pow2f(e - e / 2);
   if (part == 0 && lane == 0) ex[row] = e;
   const int cg = row / TOK;
-  auto put = [&](int b, const float (&v)[8]) {
+  auto put = [&](int b, const float (&v)[8], auto inf) {
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
@@ -158,7 +173,12 @@ __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, 
       const int q = QT == MOE_Q4_0 ? p + 2 : i + 1;
       const float a = v[p] * f1 * f2, c = v[q] * f1 * f2;
       const __half2 h = __floats2half2_rn(a, c);
-      const __half2 l = __floats2half2_rn(a - __low2float(h), c - __high2float(h));
+      float al = a - __low2float(h), cl = c - __high2float(h);
+      if (inf.value) {                           // an infinity is its hi part alone
+        if (isinf(a)) al = 0.f;
+        if (isinf(c)) cl = 0.f;
+      }
+      const __half2 l = __floats2half2_rn(al, cl);
       hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
       lo[i / 2] = *reinterpret_cast<const uint32_t*>(&l);
     }
@@ -171,14 +191,22 @@ __device__ __forceinline__ void build_fragments(const LinArgs& A, uint8_t* rec, 
     *reinterpret_cast<uint4*>(r + (odd ? 0 : 64)) =
         odd ? make_uint4(hi[0], hi[1], hi[2], hi[3]) : make_uint4(lo[0], lo[1], lo[2], lo[3]);
   };
+  if (special) {
+    for (int b = b0; b < real; b += step) {
+      float v[8];
+      values(b, v);
+      put(b, v, std::true_type());
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < KEEP; ++i)
-    if (b0 + i * step < real) put(b0 + i * step, kept[i]);
+    if (b0 + i * step < real) put(b0 + i * step, kept[i], std::false_type());
 #pragma unroll 2
   for (int b = b0 + KEEP * step; b < real; b += step) {
     float v[8];
     values(b, v);
-    put(b, v);
+    put(b, v, std::false_type());
   }
 }
 

@@ -1,13 +1,14 @@
 """Forms of the attention half's arguments that the documentation allows: odd
 strides of single axes, heads and pages that share memory, status without a
 workspace, infinities."""
+import numpy as np
 import pytest
 import torch
 
 from linuxnightmaresuite_b200 import _lib, kernels as K
 from linuxnightmaresuite_b200.attention import PagedKVCache
 
-from ._attention import BF16, E4M3, F16, Cache, check_attention
+from ._attention import BF16, E4M3, F16, Cache, check_attention, check_linear, matrix
 from .test_gpu_attention import randn
 
 pytestmark = pytest.mark.gpu
@@ -109,3 +110,41 @@ def test_outputs_over_inputs():
     for out in (k, q.transpose(0, 1), q[:1].expand(2, 2, 64)):
         with pytest.raises(_lib.MoEError, match="q_out"):
             K.rope_append(q, k, k.clone(), *c.args, pos, K.rope_inv_freq(64), q_out=out)
+
+
+@pytest.mark.parametrize("T", [1, 2, 4, 7, 16, 18])
+@pytest.mark.parametrize("qtype,rows,cols", [(2, 40, 8192), (8, 67, 256)])
+def test_linear_infinities(qtype, T, rows, cols):
+    """Infinities and NaN give what the sum of the products gives, whatever the
+    size of the row's other elements, and stay in their row."""
+    rng = np.random.default_rng(T + cols)
+    raw, w, big = matrix(rng, qtype, rows, cols)
+    lw = K.LinearWeights(torch.from_numpy(raw.reshape(-1)).cuda(), qtype, rows, cols)
+    for shift in range(6):
+        x = rng.standard_normal((T, cols), dtype=np.float32)
+        special = np.zeros(T, dtype=bool)
+        for t in range(T):
+            kind = (t + shift) % 6
+            special[t] = kind != 0
+            at = rng.integers(0, cols, 3)
+            if kind == 1:
+                x[t, at[0]] = np.inf
+            elif kind == 2:
+                x[t] *= np.float32(1e30)
+                x[t, at[0]] = -np.inf
+            elif kind == 3:
+                x[t, at[:2]] = np.inf, -np.inf
+            elif kind == 4:
+                x[t] *= np.float32(1e-30)
+                x[t, at] = np.inf
+            elif kind == 5:
+                x[t, at[:2]] = np.nan, np.inf
+        y = K.linear(torch.from_numpy(x).cuda(), lw).cpu().numpy()
+        with np.errstate(invalid="ignore"):
+            want = (x.astype(np.float64)[:, None] * w[None]).sum(-1)[special]
+        assert not np.isfinite(want).any()
+        assert np.array_equal(np.isnan(y[special]), np.isnan(want))
+        seen = ~np.isnan(want)
+        assert np.array_equal(y[special][seen], want[seen])
+        if not special.all():
+            check_linear(y[~special], x[~special], w, big)
