@@ -32,7 +32,7 @@ inline int take_cache(const moe_paged_cache* cache, moe_paged_cache& c) {
   normalise_strides(c);
   MOE_REQUIRE(c.dtype >= MOE_CACHE_F16 && c.dtype <= MOE_CACHE_E4M3, MOE_ERR_UNSUPPORTED,
               "cache type %d not supported", c.dtype);
-  MOE_REQUIRE(c.k && c.v && c.block_table, MOE_ERR_INVALID, "null cache pointer");
+  MOE_REQUIRE(c.k && c.v && (c.block_table || c.seqs == 0), MOE_ERR_INVALID, "null cache pointer");
   MOE_REQUIRE(c.pages > 0 && c.page_size > 0 && c.kv_heads > 0 && c.seqs >= 0 &&
                   c.table_width > 0 && c.table_stride >= 0,
               MOE_ERR_INVALID, "bad cache shape");

@@ -306,3 +306,11 @@ def test_rotated_q_that_overlaps_is_refused(lib):
                dict(os=(256, 128)), dict(qs=(0, 64))):
         assert rope(**kw) == _lib.MOE_ERR_INVALID, kw
         assert "q_out" in _lib.last_error()
+
+
+def test_no_sequences_need_no_table(lib):
+    """An empty tensor has no address."""
+    empty = cache(seqs=0, block_table=0)
+    assert attention(lib, empty, q=None) == _lib.MOE_OK
+    assert append(lib, empty, T=0) == _lib.MOE_OK
+    assert attention(lib, cache(block_table=0)) == _lib.MOE_ERR_INVALID

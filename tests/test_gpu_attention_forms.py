@@ -9,7 +9,7 @@ from linuxnightmaresuite_b200 import _lib, kernels as K
 from linuxnightmaresuite_b200.attention import PagedKVCache
 
 from ._attention import BF16, E4M3, F16, Cache, check_attention, check_linear, matrix
-from .test_gpu_attention import randn
+from .test_gpu_attention import _decoder, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -88,6 +88,17 @@ def test_status_without_a_workspace():
         assert status.item() == K.STATUS_BAD_PAGE
     with pytest.raises(TypeError):
         K.paged_attention(q, cache.k, cache.v, cache.block_table, lens, status=status.float())
+
+
+def test_no_sequences():
+    """A batch without rows: nothing to do, and nothing wrong."""
+    cache = PagedKVCache(4, 4, 2, 64, max_seqs=3, dtype=BF16)
+    q, none = randn(0, 4, 64), torch.zeros(0, dtype=torch.int32, device="cuda")
+    out, lse = cache.attend(q, none, return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    layer = _decoder(F16, 2, layers=1)[0].attention[0]
+    y = layer.forward(randn(0, 512), PagedKVCache(4, 4, 2, 64, max_seqs=3), none, none)
+    assert y.shape == (0, 512) and cache.device_status() == 0
 
 
 def test_outputs_over_inputs():
