@@ -204,8 +204,11 @@ def dispatch(ids: torch.Tensor, n_experts: int, ws: Optional[torch.Tensor] = Non
 
 
 def read_status(ws: torch.Tensor) -> int:
+    """Reads and clears a workspace's status bits, behind what its device's
+    current stream holds (synchronises)."""
     st = ctypes.c_int(0)
-    rc = _lib.load().moe_read_status(_ptr(ws), ctypes.byref(st), _stream())
+    with torch.cuda.device(ws.device):
+        rc = _lib.load().moe_read_status(_ptr(ws), ctypes.byref(st), _stream())
     if rc not in (_lib.MOE_OK, _lib.MOE_ERR_DEVICE):
         _lib.check(rc)
     return st.value

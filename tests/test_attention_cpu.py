@@ -314,3 +314,29 @@ def test_no_sequences_need_no_table(lib):
     assert attention(lib, empty, q=None) == _lib.MOE_OK
     assert append(lib, empty, T=0) == _lib.MOE_OK
     assert attention(lib, cache(block_table=0)) == _lib.MOE_ERR_INVALID
+
+
+def test_status_is_read_on_its_own_device(monkeypatch):
+    """The copy of a status word goes behind the kernels of the device that it is on."""
+    current, seen = [0], []
+
+    class On:
+        def __init__(self, device):
+            self.device = torch.device(device).index
+
+        def __enter__(self):
+            current.append(self.device)
+
+        def __exit__(self, *_):
+            current.pop()
+
+    class Lib:
+        @staticmethod
+        def moe_read_status(ws, out, stream):
+            seen.append(current[-1])
+            return _lib.MOE_OK
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(_lib, "load", lambda: Lib)
+    monkeypatch.setattr(K, "_stream", lambda: None)
+    ws = type("T", (), dict(device=torch.device("cuda", 3), data_ptr=lambda self: 256))()
+    assert K.read_status(ws) == 0 and seen == [3]
