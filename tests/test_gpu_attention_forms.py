@@ -90,6 +90,20 @@ def test_status_without_a_workspace():
         K.paged_attention(q, cache.k, cache.v, cache.block_table, lens, status=status.float())
 
 
+@pytest.mark.parametrize("cap", [1e-44, 1e-38, 1e-30])
+def test_smallest_cap(cap):
+    """Scores capped to next to nothing, exact zeros among them: every key weighs
+    the same."""
+    c = Cache([50], 16, 2, 64, F16, seed=4)
+    pages, slots = c.where(0, range(20, 30))
+    c.k[pages, slots] = 0
+    q = randn(1, 4, 64, seed=4)
+    for size in (1.0, 1e30):
+        out = K.paged_attention(size * q, *c.args, c.lens, softcap=cap)
+        want = c.vd[0].mean(0).repeat_interleave(2, 0)
+        assert (out[0].double() - want).abs().max() <= 2.0 ** -19 * c.vd[0].abs().max()
+
+
 def test_no_sequences():
     """A batch without rows: nothing to do, and nothing wrong."""
     cache = PagedKVCache(4, 4, 2, 64, max_seqs=3, dtype=BF16)
