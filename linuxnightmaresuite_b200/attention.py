@@ -128,7 +128,7 @@ class AttentionLayer:
         self.device = w_qkv.device
         # one workspace for all sizes, cleared here and not in a call that a graph captures
         self._ws = K.paged_attention_workspace(1, q_heads, kv_heads, head_dim, self.device)
-        self._qkv, self._att = K.RowBuffers(), K.RowBuffers()
+        self._qkv, self._att, self._parts = K.RowBuffers(), K.RowBuffers(), {}
 
     @classmethod
     def from_blocks(cls, w_q: Array, w_k: Array, w_v: Array, w_o: Array, qtype: int, dim: int,
@@ -148,9 +148,13 @@ class AttentionLayer:
                    q_heads, kv_heads, head_dim, freq, interleaved, window, softcap, scale)
 
     def _buffers(self, T: int):
-        hq, hk, d = self.q_heads, self.kv_heads, self.head_dim
-        return (self._qkv.rows(T, (hq + 2 * hk) * d, self.device),
+        parts = self._parts.get(T)
+        if parts is None:
+            hq, hk, d = self.q_heads, self.kv_heads, self.head_dim
+            parts = self._parts[T] = (
+                self._qkv.rows(T, (hq + 2 * hk) * d, self.device),
                 self._att.rows(T, hq * d, self.device).view(T, hq, d), self._ws)
+        return parts
 
     def forward(self, xn: torch.Tensor, cache: PagedKVCache, positions: torch.Tensor,
                 seq_lens: torch.Tensor, residual: Optional[torch.Tensor] = None,
