@@ -400,8 +400,9 @@ int moe_ep_forward_phases(const moe_layer_weights* w, int W, int rank, void* con
  * several sequences.  Bases and strides must be multiples of 16 bytes; head_dim
  * a multiple of 8 (16 for MOE_CACHE_E4M3), at most 256.  The slots of a page
  * have memory of their own (no token stride of 0); for the append so have pages
- * and heads.  MOE_CACHE_E4M3 holds value / scale, rounded to nearest even and
- * saturated at +-448; the scales of the other types must be 1.
+ * and heads.  Values are rounded to nearest even; MOE_CACHE_E4M3 holds value /
+ * scale, saturated at +-448, the other types an infinity beyond their range, and
+ * their scales must be 1.
  * A page id outside [0, pages) sets MOE_STATUS_BAD_PAGE; its slots are neither
  * read nor written. */
 enum { MOE_CACHE_F16 = 0, MOE_CACHE_BF16 = 1, MOE_CACHE_E4M3 = 2 };
@@ -457,15 +458,24 @@ int moe_paged_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int
  *          out and -inf in lse.  More than table_width * page_size sets
  *          MOE_STATUS_BAD_PAGE and counts as that many
  *   max_len no sequence is longer (0 = table_width * page_size); it sizes the
- *          launch, a longer sequence is still computed in full
- *   out (seqs, q_heads, head_dim) f32 contiguous; lse (seqs, q_heads) or NULL
+ *          launch (short sequences are not split where it is small), a longer
+ *          sequence is still computed in full
+ *   out (seqs, q_heads, head_dim) f32 contiguous, sharing no memory with q or
+ *          the cache; lse (seqs, q_heads) or NULL
  *   the cache's strides must be multiples of a common row of head_dim elements
  *          or more (every dense layout, also with padded rows or pages)
- *   workspace: 16-byte aligned, zeroed by the caller before its first use and then kept between
- *          calls, which leave it ready for the next one (but for the status
- *          word at its start); calls that may overlap need one each
- * The split of a sequence over the GPU depends on the lengths and the device
- * alone, and its parts are joined in a fixed order: equal calls give equal bits. */
+ *   workspace: 16-byte aligned, zeroed by the caller before its first use and
+ *          then kept between calls, which leave it ready for the next one (but for
+ *          the status word at its start); calls that may overlap need one each
+ * The split of a sequence over the GPU depends on the batch's lengths, on max_len
+ * and window (which size the launch), on the heads, the cache type and the device;
+ * its parts are joined in a fixed order.  Equal calls give equal bits; the same
+ * lengths under another max_len can differ in the last ones.
+ * The status word at the start of the workspace gathers MOE_STATUS_BAD_PAGE and
+ * MOE_STATUS_TIMEOUT (a copy never arrived; the outputs are not to be used).
+ * Infinities enter the products in parts, so one in q or in a key gives NaN or an
+ * infinity in the rows that meet it, one in a value in its column, whatever their
+ * sum would be; so does a NaN.  In slots that no row sees they count for nothing. */
 int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_seq_stride,
                         int64_t q_head_stride, const int32_t* seq_lens, int q_heads, int max_len,
                         int window, float scale, float softcap, float* out, float* lse,

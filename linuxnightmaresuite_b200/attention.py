@@ -162,6 +162,8 @@ class AttentionLayer:
         """xn (T, dim): the normalised row of the new token of sequences 0 ..
         T - 1, at ``positions`` (int32); ``seq_lens`` counts it (positions + 1
         for a plain decode step; position -1 with length 0 is a padding row).
+        ``max_len``: as in ``kernels.paged_attention``; with 0 the launch is sized
+        for the longest sequence that the table holds.
         Returns Wo attention (+ residual); ``out`` may be ``residual``.
         Allocates nothing after the first call of a size (but ``out`` when not
         given), and the buffers stay where they are, so captured steps of

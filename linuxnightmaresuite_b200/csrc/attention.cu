@@ -2,11 +2,12 @@
 //
 //   s_j = scale q.k_j,  o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
 //
-// Keys and values are read once and each meets the 1..8 query heads that share
-// them, so the bound is memory; the arithmetic goes to mma.sync (m16n8k16): a
-// CUDA-core form needs 2 FMAs per head and element and would be issue-bound
-// from 4 heads on, and a tcgen05 tile (64 rows at least) would be mostly
-// padding.
+// Up to 8 query heads that share a key head meet each of its keys and values at
+// one reading (more heads are groups of 8, each of which reads them again), so the
+// bound is memory; the arithmetic goes to mma.sync (m16n8k16), of which the heads
+// fill the M side in two parts each: a CUDA-core form needs 2 FMAs per head and
+// element and would be issue-bound from 4 heads on.  (A tcgen05 form would take
+// keys as M and q as N; its products would come back through tensor memory.)
 //
 // Work.  A unit is one (sequence, key head, group of up to 8 query heads); it
 // is cut into rounds of one tile of KEYS keys per warp.  All units in order, each at the

@@ -400,7 +400,7 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     (``rope_inv_freq``); None rotates nothing.  Pairs are (i, i + rot / 2), or
     adjacent with ``interleaved``.  ``seq_ids`` maps tokens to rows of
     ``block_table`` (None: token t is sequence t); a negative position skips
-    its token, q row included; no two tokens may share sequence and position.
+    its token, q row included (without ``q_out`` that row is not set); no two tokens may share sequence and position.
     ``status`` (int32) receives STATUS_BAD_PAGE for a page or sequence that
     does not exist; such a token's k and v are not stored."""
     c, dev, _, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
@@ -467,7 +467,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     out, or (out, lse) with the natural log of the softmax sums; a sequence of
     length 0 gives zeros and -inf.  ``scale`` defaults to 1 / sqrt(head_dim);
     ``max_len`` (no sequence is longer; 0 = what the table holds) sizes the
-    launch.  ``ws`` comes from ``paged_attention_workspace``.  Its first word
+    launch and with it the split of the sequences, so equal calls give equal
+    bits, but another ``max_len`` may change the last ones.  ``ws`` comes from ``paged_attention_workspace``.  Its first word
     gathers status bits (``read_status``: STATUS_BAD_PAGE for a page that does
     not exist or a length that the table does not hold); ``status`` (int32)
     receives them too, by a small launch of its own, for calls without ``ws``."""

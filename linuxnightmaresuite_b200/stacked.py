@@ -56,10 +56,10 @@ class StackedMoE:
                 positions: Optional[torch.Tensor] = None,
                 seq_lens: Optional[torch.Tensor] = None, max_len: int = 0) -> torch.Tensor:
         """x (T, d) f32 on the device -> (T, d).  The residual stream lives in
-        ``out`` (allocated once if not given): the first layer adds x into it,
+        ``out`` (allocated if not given): the first layer adds x into it,
         later layers update it in place (the combine may write over its own
-        residual input), so a step allocates nothing after the first of its
-        size.
+        residual input), so a step with ``out`` allocates nothing after
+        the first of its size.
 
         With attention layers row t is the new token of sequence t:
         ``caches`` (one per layer), ``positions`` and ``seq_lens`` as
