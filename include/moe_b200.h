@@ -460,8 +460,9 @@ int moe_paged_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int
  *   max_len no sequence is longer (0 = table_width * page_size); it sizes the
  *          launch (short sequences are not split where it is small), a longer
  *          sequence is still computed in full
- *   out (seqs, q_heads, head_dim) f32 contiguous, sharing no memory with q or
- *          the cache; lse (seqs, q_heads) or NULL
+ *   out (seqs, q_heads, head_dim) f32 contiguous; may be q itself where that is
+ *          contiguous, but must not lie between its rows or over the cache.
+ *          lse (seqs, q_heads) or NULL
  *   the cache's strides must be multiples of a common row of head_dim elements
  *          or more (every dense layout, also with padded rows or pages)
  *   workspace: 16-byte aligned, zeroed by the caller before its first use and

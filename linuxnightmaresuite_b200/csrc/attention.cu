@@ -1105,6 +1105,19 @@ int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_
   MOE_REQUIRE(q && seq_lens && out && workspace, MOE_ERR_INVALID, "null pointer");
   // parts in it are fetched by bulk copies
   MOE_REQUIRE((uintptr_t)workspace % 16 == 0, MOE_ERR_INVALID, "workspace must be 16-byte aligned");
+  {
+    // A unit's rows of out are written behind the last read of its rows of q, so out
+    // may be q itself, but over other rows it would be read when it is written already.
+    const int64_t S = a.c.seqs, d = a.c.head_dim, n = S * q_heads * d;
+    const bool same = (uintptr_t)out == (uintptr_t)q && (S == 1 || q_seq_stride == q_heads * d) &&
+                      (q_heads == 1 || q_head_stride == d);
+    const int64_t ss = (S - 1) * q_seq_stride, hs = (q_heads - 1) * q_head_stride;
+    const int64_t from = std::min<int64_t>(ss, 0) + std::min<int64_t>(hs, 0);
+    const int64_t to = std::max<int64_t>(ss, 0) + std::max<int64_t>(hs, 0) + d;
+    const int64_t at = (int64_t)((uintptr_t)out - (uintptr_t)q);         // bytes
+    MOE_REQUIRE(same || at >= 4 * to || at + 4 * n <= 4 * from, MOE_ERR_INVALID,
+                "q and out overlap, and are not the same rows");
+  }
   a.q = q;
   a.q_ss = q_seq_stride;
   a.q_hs = q_head_stride;

@@ -465,7 +465,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     over the first ``seq_lens[s]`` tokens of its pages (the last ``window`` of
     them if given): softmax(scale q.k, capped at ``softcap``) v, f32.  Returns
     out, or (out, lse) with the natural log of the softmax sums; a sequence of
-    length 0 gives zeros and -inf.  ``scale`` defaults to 1 / sqrt(head_dim);
+    length 0 gives zeros and -inf.  ``out`` may be q where q is contiguous.
+    ``scale`` defaults to 1 / sqrt(head_dim);
     ``max_len`` (no sequence is longer; 0 = what the table holds) sizes the
     launch and with it the split of the sequences, so equal calls give equal
     bits, but another ``max_len`` may change the last ones.  ``ws`` comes from ``paged_attention_workspace``.  Its first word

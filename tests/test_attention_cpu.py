@@ -340,3 +340,20 @@ def test_status_is_read_on_its_own_device(monkeypatch):
     monkeypatch.setattr(K, "_stream", lambda: None)
     ws = type("T", (), dict(device=torch.device("cuda", 3), data_ptr=lambda self: 256))()
     assert K.read_status(ws) == 0 and seen == [3]
+
+
+def test_attention_output_over_part_of_q_is_refused(lib):
+    c = cache()                                     # 4 sequences of 4 heads of 64: 4096 bytes
+
+    def att(q, out, ss=256, hs=64):
+        return lib.moe_paged_attention(ctypes.byref(c), ctypes.c_void_p(q), ss, hs, P, 4, 0, 0, 0.1,
+                                       0.0, ctypes.c_void_p(out), None, P, 16, None)
+    q = 1 << 20
+    for out, strides in ((q + 4, {}), (q - 4, {}), (q + 4092, {}), (q - 4092, {}), (q + 1024, {}),
+                         (q, dict(ss=512)), (q, dict(hs=128)), (q + 1024, dict(ss=512)),
+                         (q, dict(ss=0))):
+        assert att(q, out, **strides) == _lib.MOE_ERR_INVALID, (out - q, strides)
+        assert "overlap" in _lib.last_error()
+    for out, strides in ((q, {}), (q + 4096, {}), (q - 4096, {}), (q - 4096, dict(ss=512)),
+                         (q + 4 * (3 * 512 + 256), dict(ss=512))):
+        assert att(q, out, **strides) == _lib.MOE_ERR_WORKSPACE, (out - q, strides)

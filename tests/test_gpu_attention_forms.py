@@ -173,3 +173,24 @@ def test_linear_infinities(qtype, T, rows, cols):
         assert np.array_equal(y[special][seen], want[seen])
         if not special.all():
             check_linear(y[~special], x[~special], w, big)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+def test_attention_over_q(dtype):
+    """The output may be q itself: units split over CTAs, short ones, empty ones."""
+    hq, hkv, d = 16, 2, 128
+    for lens in ([20011], [4001, 0, 37, 1, 5099, 3777], [50] * 200):
+        c = Cache(lens, 16, hkv, d, dtype, seed=len(lens))
+        q = randn(len(lens), hq, d, seed=6)
+        want = K.paged_attention(q, *c.args, c.lens, **c.scales)
+        check_attention(c, q, want, None, d ** -0.5)
+        ws = K.paged_attention_workspace(len(lens), hq, hkv, d, "cuda")
+        for _ in range(10):
+            over = q.clone()
+            got = K.paged_attention(over, *c.args, c.lens, out=over, ws=ws, **c.scales)
+            assert got is over and torch.equal(got, want)
+    both = randn(3, hq, d, seed=7)
+    with pytest.raises(_lib.MoEError, match="overlap"):
+        K.paged_attention(both[:2], *Cache([9, 9], 16, hkv, d, dtype).args,
+                          torch.tensor([9, 9], dtype=torch.int32).cuda(), out=both[1:],
+                          **c.scales)
