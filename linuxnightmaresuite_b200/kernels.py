@@ -466,13 +466,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     them if given): softmax(scale q.k, capped at ``softcap``) v, f32.  Returns
     out, or (out, lse) with the natural log of the softmax sums; a sequence of
     length 0 gives zeros and -inf.  ``out`` may be q where q is contiguous.
-    ``scale`` defaults to 1 / sqrt(head_dim);
-    ``max_len`` (no sequence is longer; 0 = what the table holds) sizes the
-    launch and with it the split of the sequences, so equal calls give equal
-    bits, but another ``max_len`` may change the last ones.  ``ws`` comes from ``paged_attention_workspace``.  Its first word
-    gathers status bits (``read_status``: STATUS_BAD_PAGE for a page that does
-    not exist or a length that the table does not hold); ``status`` (int32)
-    receives them too, by a small launch of its own, for calls without ``ws``."""
+    ``scale`` defaults to 1 / sqrt(head_dim); ``max_len`` (no sequence is
+    longer; 0 = what the table holds) sizes the launch and with it the split of
+    the sequences, so equal calls give equal bits, but another ``max_len`` may
+    change the last ones.  ``ws`` comes from ``paged_attention_workspace``; its
+    first word gathers status bits (``read_status``: STATUS_BAD_PAGE for a page
+    that does not exist or a length that the table does not hold).  ``status``
+    (int32) receives them too, by a small launch of its own, for calls without
+    ``ws``."""
     c, dev, seqs, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
     shape = q.shape
     if len(shape) != 3:

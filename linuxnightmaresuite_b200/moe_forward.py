@@ -310,7 +310,9 @@ class MoELayer:
         return (out, ids, weights) if return_routing else out
 
     def device_status(self) -> int:
-        """Reads and clears the device status bits (synchronises)."""
+        """Reads and clears the device status bits (synchronises).  Those of a
+        graph that captured the layer's first call mean something once it has
+        been replayed."""
         bits = 0
         for ws in self._held + ([] if self._ws is None else [self._ws]):
             bits |= K.read_status(ws)
