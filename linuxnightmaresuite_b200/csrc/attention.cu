@@ -609,7 +609,8 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     const int ntile = tiles(C);
 
     const float qscale = sh.qscale[g];           // score = product * qscale
-    const float to_cap = A.cap > 0.f ? fminf(qscale / A.cap, 3e38f) : 0.f, from_cap = A.cap * kLog2e;
+    const float to_cap = A.cap > 0.f ? fminf(qscale / A.cap, 3e38f) : 0.f;
+    const float from_cap = A.cap * kLog2e;
     const float x2 = A.cap > 0.f ? 1.f : qscale * kLog2e;
     float o[DH / 8][2];                          // head g, two columns of each 8-wide block
     float acc[DH / 8][4];

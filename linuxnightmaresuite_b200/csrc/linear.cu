@@ -22,8 +22,8 @@
 //
 // Measured on a B200 (copy bandwidth 6.55 TB/s): 262144 x 2816 Q4_0 for one row 70
 // us in a short run (416 MB, 90 %), 77 to 83 us in calls that go on and on (77 to 82
-// %: the load lowers the clock, and instructions come next), 65536 x 2816 for 1, 4, 8, 16 rows 22.4, 24.5, 35.6, 53 us
-// (floor 15.9), 6144 x 2816 for one row 6.0 us, of which 4 are launch, fragments and
+// %: the load lowers the clock, and instructions come next), 65536 x 2816 for 1, 4,
+// 8, 16 rows 22.4, 24.5, 35.6, 53 us (floor 15.9), 6144 x 2816 for one row 6.0 us, of which 4 are launch, fragments and
 // the meeting of the warps, 4096 x 8192 for 16 rows 17.1 us (fragments 4.4, weights
 // 8.5 where the MMAs alone take 4.3, meetings 3.3).
 #include <algorithm>

@@ -400,7 +400,8 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     (``rope_inv_freq``); None rotates nothing.  Pairs are (i, i + rot / 2), or
     adjacent with ``interleaved``.  ``seq_ids`` maps tokens to rows of
     ``block_table`` (None: token t is sequence t); a negative position skips
-    its token, q row included (without ``q_out`` that row is not set); no two tokens may share sequence and position.
+    its token, q row included (without ``q_out`` that row is not set); no two
+    tokens may share sequence and position.
     ``status`` (int32) receives STATUS_BAD_PAGE for a page or sequence that
     does not exist; such a token's k and v are not stored."""
     c, dev, _, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)

@@ -194,3 +194,26 @@ def test_attention_over_q(dtype):
         K.paged_attention(both[:2], *Cache([9, 9], 16, hkv, d, dtype).args,
                           torch.tensor([9, 9], dtype=torch.int32).cuda(), out=both[1:],
                           **c.scales)
+
+
+def test_broadcast_rows():
+    """One bias for every row, one key and value for every token, one q for every
+    sequence (strides of 0)."""
+    rng = np.random.default_rng(8)
+    raw, w, big = matrix(rng, 2, 100, 160)
+    lw = K.LinearWeights(torch.from_numpy(raw.reshape(-1)).cuda(), 2, 100, 160)
+    for T in (2, 9):
+        x, bias = randn(T, 160, seed=T), randn(1, 100, seed=T + 1)
+        y = K.linear(x, lw, residual=bias.expand(T, 100))
+        check_linear(y.cpu().numpy(), x.cpu().numpy(), w, big, bias.cpu().numpy())
+    hkv, d = 2, 64
+    one, many = (Cache([9, 30, 17], 8, hkv, d, BF16, seed=9) for _ in range(2))
+    q, kv, pos = randn(1, 4, d, seed=9), randn(1, hkv, d, seed=10), one.lens - 1
+    freq = K.rope_inv_freq(d)
+    turned = []
+    for c, wide in ((one, lambda t: t.expand(3, -1, -1)), (many, lambda t: t.repeat(3, 1, 1))):
+        turned.append(K.rope_append(wide(q), wide(kv), wide(kv), *c.args, pos, freq))
+        turned.append(K.paged_attention(wide(q), *c.args, c.lens))
+    assert torch.equal(turned[0], turned[2]) and torch.equal(turned[1], turned[3])
+    assert torch.equal(one.k.view(torch.int16), many.k.view(torch.int16))
+    assert torch.equal(one.v.view(torch.int16), many.v.view(torch.int16))
