@@ -710,7 +710,16 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         }
         asm volatile("bar.sync %0, 64;" ::"r"(1 + warp / SP) : "memory");
       }
+      auto hide = [&](float value) {             // lanes past KEYS repeat the first ones
+        if (seen != 0xffffffffu)
+#pragma unroll
+          for (int b = 0; b < KEYS / 8; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (!((seen >> (8 * b + 2 * t + h)) & 1u)) x[b][h] = value;
+      };
       if (A.cap > 0.f) {                         // x = cap tanh(score / cap) log2 e
+        hide(0.f);                               // what the ring holds there picks no form of tanh
         float big = 0.f;
 #pragma unroll
         for (int b = 0; b < KEYS / 8; ++b)
@@ -737,13 +746,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             }
         }
       }
-      if (seen != 0xffffffffu) {                 // lanes past KEYS repeat the first ones
-#pragma unroll
-        for (int b = 0; b < KEYS / 8; ++b)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (!((seen >> (8 * b + 2 * t + h)) & 1u)) x[b][h] = -INFINITY;
-      }
+      hide(-INFINITY);
 
       // reference and sum
       float mx = -INFINITY;

@@ -217,3 +217,28 @@ def test_broadcast_rows():
     assert torch.equal(turned[0], turned[2]) and torch.equal(turned[1], turned[3])
     assert torch.equal(one.k.view(torch.int16), many.k.view(torch.int16))
     assert torch.equal(one.v.view(torch.int16), many.v.view(torch.int16))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("hq,hkv,d,window", [(12, 4, 64, 0), (8, 2, 128, 33), (6, 2, 256, 0)])
+def test_equal_calls_whatever_ran_before(dtype, hq, hkv, d, window):
+    """Slots that no row sees hold what earlier kernels left in shared memory; with
+    and without a cap they count for nothing, not even in the last bit."""
+    lens = [1, 20, 43, 7, 0, 65] * 40
+    c = Cache(lens, 4, hkv, d, dtype, seed=d)
+    q = 0.3 * randn(len(lens), hq, d, seed=d)
+    ws = K.paged_attention_workspace(1, hq, hkv, d, "cuda")
+    before = [Cache([200] * 150, 16, hkv, d, dtype, seed=1) for _ in range(2)]
+    for t in (before[1].k, before[1].v):
+        t.copy_(torch.full(t.shape, 3.0 if dtype == E4M3 else torch.inf, device="cuda").to(dtype))
+    qb = 8 * randn(150, hq, d, seed=2)
+    for cap in (0.0, 5.0, 30.0):
+        want = None
+        for b in before * 3:
+            K.paged_attention(qb, *b.args, b.lens, ws=ws, **b.scales)
+            got = K.paged_attention(q, *c.args, c.lens, window=window, softcap=cap, ws=ws,
+                                    return_lse=True, **c.scales)
+            if want is None:
+                want = got
+                check_attention(c, q, *got, d ** -0.5, window, cap)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), cap
