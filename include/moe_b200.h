@@ -122,7 +122,7 @@ enum {
   MOE_K_ROUTER = 0, MOE_K_ROUTER_SELECT, MOE_K_DISPATCH, MOE_K_PLAN, MOE_K_XPREP,
   MOE_K_GATEUP, MOE_K_DOWN, MOE_K_COMBINE, MOE_K_RMS_NORM, MOE_K_PACK, MOE_K_DEQUANT,
   MOE_K_AUX, MOE_K_EP_SEND, MOE_K_EP_RECV, MOE_K_EP_RETURN, MOE_K_EP_WAIT, MOE_K_ROPE_APPEND,
-  MOE_K_ATTENTION, MOE_K_LINEAR, MOE_K_COUNT
+  MOE_K_ATTENTION, MOE_K_LINEAR, MOE_K_ATTENTION_MASS, MOE_K_CACHE_EVICT, MOE_K_COUNT
 };
 int moe_profile_enable(int on);
 int moe_profile_collect(float* ms, int* launches, int n);
@@ -541,6 +541,95 @@ typedef struct moe_linear_args {
 int moe_rope_append_record(const moe_rope_append_args* args);
 int moe_paged_attention_record(const moe_paged_attention_args* args);
 int moe_linear_record(const moe_linear_args* args);
+
+/* ---- a cache that shrinks -------------------------------------------------------------
+ * The calls below take their arguments in one record only.
+ *
+ * A ledger says of each slot what it holds: `mass` (f32), the attention weight that the
+ * slot has received so far, and `held` (int32), the position of its token.  Both are
+ * (seqs, kv_heads, ledger_slots) contiguous, sequence s as in the block table; slot j of a
+ * (sequence, head) is entry j.  After an eviction the heads of a sequence hold different
+ * tokens in a slot, and slots no longer follow the positions. */
+
+/* moe_rope_append with, for each query and key head in front of the rotation,
+ *   x / sqrt(mean(x^2) + eps) * w        (1 + w with gemma_style)
+ *   q_norm, k_norm (head_dim,) f32, or NULL: heads of that kind are taken as they are
+ *   slots (T,) int32: where k and v of a token go, as moe_rope_append takes positions
+ *          for it (a negative one skips the token); NULL: the positions
+ *   mass, held: ledgers, or both NULL.  The new slots' entries become 0 and the token's
+ *          position.  A slot behind ledger_slots sets MOE_STATUS_BAD_PAGE; such a token's k
+ *          and v are not stored
+ * Sums of squares are f32.  All else as in moe_rope_append; no two tokens of a call may have
+ * the same sequence and slot. */
+typedef struct moe_norm_append_args {
+  moe_rope_append_args append;
+  const float *q_norm, *k_norm;
+  const int32_t* slots;
+  float* mass;
+  int32_t* held;
+  int64_t ledger_slots;
+  float eps;
+  int gemma_style;
+} moe_norm_append_args;
+int moe_norm_append_record(const moe_norm_append_args* args);
+
+/* The weight that each slot receives from the new tokens' queries, added up:
+ *   out[s, h, j] = mass[s, h, j] + sum over the query heads g of key head h of
+ *                  exp(s_gj - lse_g),   s_gj as in moe_paged_attention
+ * for the slots j < seq_lens[s] (with a window the last `window` of them; of those before it
+ * mass is copied).  Slots behind a sequence's length are left as they were.
+ *   q, seq_lens, window, scale, softcap, max_len: as moe_paged_attention takes them
+ *   lse   (seqs, q_heads) f32, what moe_paged_attention returned for this q; a head whose lse is
+ *         infinite gives nothing
+ *   mass, out (seqs, kv_heads, ledger_slots) f32; out may be mass itself
+ *   status int32 that receives MOE_STATUS_BAD_PAGE (a page that does not exist, whose slots get
+ *         no weight; a length that the table or the ledger does not hold, which counts as what
+ *         they hold), or NULL
+ * cache.v is not read (any non-null pointer). */
+typedef struct moe_attention_mass_args {
+  moe_paged_cache cache;
+  const float* q;
+  int64_t q_seq_stride, q_head_stride;
+  const int32_t* seq_lens;
+  const float *lse, *mass;
+  float* out;
+  int64_t ledger_slots;
+  int32_t* status;
+  moe_stream_t stream;
+  int q_heads, max_len, window;
+  float scale, softcap;
+} moe_attention_mass_args;
+int moe_attention_mass_record(const moe_attention_mass_args* args);
+
+/* Cuts every (sequence, key head) with more than `keep` slots down to `keep`: the tokens
+ * held at the last `recent` positions (above the largest position held less `recent`) stay,
+ * then those of the largest mass; of equal masses the lowest slot stays, a NaN goes first.
+ * Survivors in slots from `keep` on, in order, move to the slots below `keep` that are given
+ * up, in order: k, v and the ledger's entries.  All other slots keep what they hold, and
+ * the pages behind `keep` may be given back.
+ *   seq_lens (seqs,) int32, lens_out: min(seq_lens, keep); may be seq_lens itself
+ *   mass, held with ledger_slots; mass_out, held_out with out_slots >= keep (or max_len) slots: each may
+ *         be its input itself.  Otherwise the entries that stay are copied.  Entries from
+ *         `keep` on, or behind a shorter sequence's length, are left as they were
+ *   max_len no sequence is longer (0 = what table and ledger hold; at most 163840): it sizes the
+ *         launch.  A longer one sets MOE_STATUS_BAD_PAGE and is left as it is
+ *   status int32 that receives MOE_STATUS_BAD_PAGE (also for a page that does not exist,
+ *         whose slots' k and v are not moved), or NULL
+ * A page that several sequences share is changed for all of them: give up no shared pages.
+ * The rows of the cache must have memory of their own. */
+typedef struct moe_cache_evict_args {
+  moe_paged_cache cache;
+  const int32_t* seq_lens;
+  const float* mass;
+  const int32_t* held;
+  float* mass_out;
+  int32_t *held_out, *lens_out;
+  int64_t ledger_slots, out_slots;
+  int32_t* status;
+  moe_stream_t stream;
+  int keep, recent, max_len;
+} moe_cache_evict_args;
+int moe_cache_evict_record(const moe_cache_evict_args* args);
 
 #ifdef __cplusplus
 }

@@ -106,6 +106,33 @@ class MoELinearArgs(ctypes.Structure):
     ]
 
 
+class MoENormAppendArgs(ctypes.Structure):
+    """Mirror of ``moe_norm_append_args``."""
+    _fields_ = [
+        ("append", MoERopeAppendArgs), ("q_norm", vp), ("k_norm", vp), ("slots", vp),
+        ("mass", vp), ("held", vp), ("ledger_slots", ci64), ("eps", cf), ("gemma_style", ci),
+    ]
+
+
+class MoEAttentionMassArgs(ctypes.Structure):
+    """Mirror of ``moe_attention_mass_args``."""
+    _fields_ = [
+        ("cache", MoEPagedCache), ("q", vp), ("q_seq_stride", ci64), ("q_head_stride", ci64),
+        ("seq_lens", vp), ("lse", vp), ("mass", vp), ("out", vp), ("ledger_slots", ci64),
+        ("status", vp), ("stream", vp), ("q_heads", ci), ("max_len", ci), ("window", ci),
+        ("scale", cf), ("softcap", cf),
+    ]
+
+
+class MoECacheEvictArgs(ctypes.Structure):
+    """Mirror of ``moe_cache_evict_args``."""
+    _fields_ = [
+        ("cache", MoEPagedCache), ("seq_lens", vp), ("mass", vp), ("held", vp), ("mass_out", vp),
+        ("held_out", vp), ("lens_out", vp), ("ledger_slots", ci64), ("out_slots", ci64),
+        ("status", vp), ("stream", vp), ("keep", ci), ("recent", ci), ("max_len", ci),
+    ]
+
+
 # name -> (argtypes) ; every function returns int
 SIGNATURES = {
     "moe_version": [],
@@ -155,12 +182,16 @@ SIGNATURES = {
     "moe_rope_append_record": [vp],
     "moe_paged_attention_record": [vp],
     "moe_linear_record": [vp],
+    "moe_norm_append_record": [vp],
+    "moe_attention_mass_record": [vp],
+    "moe_cache_evict_record": [vp],
 }
 
 
 KERNEL_NAMES = ["router", "router_select", "dispatch", "plan", "xprep", "gateup", "down",
                 "combine", "rms_norm", "pack", "dequant", "aux", "ep_send", "ep_recv_plan",
-                "ep_return", "ep_wait", "rope_append", "attention", "linear"]
+                "ep_return", "ep_wait", "rope_append", "attention", "linear", "attention_mass",
+                "cache_evict"]
 
 MOE_EP_PHASE_SEND = 1
 MOE_EP_PHASE_SERVE = 2

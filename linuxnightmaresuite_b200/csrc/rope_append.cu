@@ -15,6 +15,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "paged_cache.cuh"
 
@@ -168,14 +169,19 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeArg
   }
 }
 
-template <int DT>
-static int launch_rope(RopeArgs& a, int T, cudaStream_t s) {
+// Whether all rows can be taken four elements at a time.
+static bool four_at_a_time(const RopeArgs& a) {
   auto aligned = [](const void* p, int64_t ts, int64_t hs) {
     return (uintptr_t)p % 16 == 0 && ts % 4 == 0 && hs % 4 == 0;
   };
-  const bool vec = a.rot % (a.interleaved ? 4 : 8) == 0 && aligned(a.k, a.k_ts, a.k_hs) &&
-                   aligned(a.v, a.v_ts, a.v_hs) &&
-                   (a.hq == 0 || (aligned(a.q, a.q_ts, a.q_hs) && aligned(a.q_out, a.qo_ts, a.qo_hs)));
+  return a.rot % (a.interleaved ? 4 : 8) == 0 && aligned(a.k, a.k_ts, a.k_hs) &&
+         aligned(a.v, a.v_ts, a.v_hs) &&
+         (a.hq == 0 || (aligned(a.q, a.q_ts, a.q_hs) && aligned(a.q_out, a.qo_ts, a.qo_hs)));
+}
+
+template <int DT>
+static int launch_rope(RopeArgs& a, int T, cudaStream_t s) {
+  const bool vec = four_at_a_time(a);
   const int V = vec ? 4 : 1;
   a.nr = a.interleaved ? a.rot / V : a.rot / 2 / V;
   a.ni = a.nr + (a.c.head_dim - a.rot) / V;
@@ -194,9 +200,271 @@ static int launch_rope(RopeArgs& a, int T, cudaStream_t s) {
   return MOE_OK;
 }
 
+// ---------------------------------------------------------------------------
+// The append with a norm of each query and key head in front of the rotation,
+//
+//   y = x / sqrt(mean(x^2) + eps) * w      (or 1 + w),
+//
+// cache slots apart from the positions, and the slots' ledger (accumulated
+// attention weight, position held).
+//
+// A norm needs its whole head before any element turns, so here a group of GL lanes
+// owns a row: it loads the row once, in the items of the rotation (both halves of a
+// pair meet in one lane), sums the squares by shuffles and turns what it holds.  Rows
+// of a token go to the groups of its CTA; each group has the loads of kRowsAhead rows
+// under way before it waits for the angles and the slot.  Bound by memory for
+// prompts, by latency for single tokens, like the form without norms.
+// ---------------------------------------------------------------------------
+struct NormArgs {
+  const float *q_norm, *k_norm;        // null: that head is not normed
+  const int32_t* slots;                // null: the positions
+  float* mass;                         // ledgers, null: none
+  int32_t* held;
+  int64_t ledger_row;                  // slots of a (sequence, head) in them
+  float eps, plus;                     // weights are plus + w
+};
+
+constexpr int kRowsAhead = 3;
+
+template <int VEC, int M>
+struct NormRow {
+  Elems<VEC> a[M], b[M];
+};
+
+template <int DT, int VEC, int GL>
+__global__ void __launch_bounds__(kRopeThreads) norm_append_kernel(const RopeArgs A, const NormArgs N) {
+  using T = typename CacheType<DT>::T;
+  constexpr int M = VEC == 4 ? 2 : 8;  // items of a lane
+  __shared__ float2 cs[kMaxHeadDim / 2];
+  __shared__ float ws[2][kMaxHeadDim];
+  __shared__ int64_t sh_slot;
+  pdl_trigger();
+  pdl_wait();
+  const int t = blockIdx.x;
+  const int pos = A.positions[t];
+  const int at = N.slots ? N.slots[t] : pos;
+  if (pos < 0 || at < 0) return;
+  const int hk = A.c.kv_heads, d = A.c.head_dim, nr = A.nr, ni = A.ni, nv = A.nv;
+  const int h = A.rot / 2, rows = A.hq + 2 * hk;
+  const int gl = threadIdx.x % GL, groups = blockDim.x / GL;
+  const int g0 = blockIdx.y * groups + threadIdx.x / GL, step = gridDim.y * groups;
+
+  auto first_of = [&](int i) { return i < nr ? i * VEC * (VEC == 1 && A.interleaved ? 2 : 1)
+                                              : A.rot + (i - nr) * VEC; };
+  const bool pairs = !A.interleaved || VEC == 1;       // an item of the rotation is two loads
+  const int apart = A.interleaved ? 1 : h;
+  auto fetch = [&](int row, NormRow<VEC, M>& r) {
+    if (row >= rows) return;
+    const bool value = row >= A.hq + hk;
+    const float* src = row < A.hq ? A.q + t * A.q_ts + row * A.q_hs
+                       : value    ? A.v + t * A.v_ts + (row - A.hq - hk) * A.v_hs
+                                  : A.k + t * A.k_ts + (row - A.hq) * A.k_hs;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int i = gl + m * GL;
+      if (value) {
+        if (i < nv) r.a[m] = load_elems<VEC>(src + i * VEC);
+      } else if (i < ni) {
+        const int e = first_of(i);
+        r.a[m] = load_elems<VEC>(src + e);
+        if (i < nr && pairs) r.b[m] = load_elems<VEC>(src + e + apart);
+      }
+    }
+  };
+  NormRow<VEC, M> ahead[kRowsAhead];
+#pragma unroll
+  for (int k = 0; k < kRowsAhead; ++k) fetch(g0 + k * step, ahead[k]);
+
+  if (threadIdx.x == blockDim.x - 1) {           // the token's slot in both caches, -1: none
+    const int seq = A.seq_ids ? A.seq_ids[t] : t, n = at / A.c.page_size;
+    int64_t slot = -1;
+    if (seq >= 0 && seq < A.c.seqs && n < A.c.table_width && (!N.mass || at < N.ledger_row)) {
+      const int page = A.c.block_table[(int64_t)seq * A.c.table_stride + n];
+      if (page >= 0 && page < A.c.pages)
+        slot = (int64_t)page * A.c.page_stride +
+               (int64_t)(at - n * A.c.page_size) * A.c.token_stride;
+    }
+    if (slot < 0) set_status(A.status, MOE_STATUS_BAD_PAGE);
+    sh_slot = slot;
+    if (slot >= 0 && N.mass && blockIdx.y == 0)
+      for (int j = 0; j < hk; ++j) {
+        const int64_t e = ((int64_t)seq * hk + j) * N.ledger_row + at;
+        N.mass[e] = 0.f;
+        N.held[e] = pos;
+      }
+  }
+  for (int i = threadIdx.x; i < h; i += blockDim.x) cs[i] = rope_cos_sin(pos, A.inv_freq[i]);
+  for (int i = threadIdx.x; i < d; i += blockDim.x) {
+    if (N.q_norm) ws[0][i] = N.plus + N.q_norm[i];
+    if (N.k_norm) ws[1][i] = N.plus + N.k_norm[i];
+  }
+  __syncthreads();
+  const int64_t slot = sh_slot;
+
+  auto finish = [&](int row, NormRow<VEC, M>& r) {
+    const bool is_q = row < A.hq, value = row >= A.hq + hk;
+    const float* w = is_q ? (N.q_norm ? ws[0] : nullptr) : (!value && N.k_norm ? ws[1] : nullptr);
+    float inv = 1.f;
+    if (w) {                                     // the same for all lanes of a group
+      float ss = 0.f;
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const int i = gl + m * GL;
+        if (i < ni) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) ss = fmaf(r.a[m].v[k], r.a[m].v[k], ss);
+          if (i < nr && pairs)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) ss = fmaf(r.b[m].v[k], r.b[m].v[k], ss);
+        }
+      }
+      const uint32_t mask = GL == 32 ? 0xffffffffu
+                                     : ((1u << GL % 32) - 1u) << (threadIdx.x % 32 / GL * GL);
+#pragma unroll
+      for (int o = GL / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+      inv = 1.f / sqrtf(ss / (float)d + N.eps);
+    }
+    const int j = is_q ? row : value ? row - A.hq - hk : row - A.hq;
+    float* qo = is_q ? A.q_out + t * A.qo_ts + j * A.qo_hs : nullptr;
+    T* co = is_q ? nullptr
+                 : static_cast<T*>(value ? A.c.v : A.c.k) + slot + (int64_t)j * A.c.head_stride;
+    if (!is_q && slot < 0) return;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int i = gl + m * GL;
+      if (i >= (value ? nv : ni)) continue;
+      if (value) {
+        store_cache<VEC>(co + i * VEC, r.a[m], A.c.v_scale);
+        continue;
+      }
+      const int e0 = first_of(i);
+      const bool two = i < nr && pairs;
+      Elems<VEC> a = r.a[m], b = r.b[m];
+      if (w) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) a.v[k] = a.v[k] * inv * w[e0 + k];
+        if (two)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) b.v[k] = b.v[k] * inv * w[e0 + apart + k];
+      }
+      if (two) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const float2 c = cs[A.interleaved ? e0 / 2 : e0 + k];
+          const float x0 = a.v[k], x1 = b.v[k];
+          a.v[k] = fmaf(x0, c.x, -x1 * c.y);
+          b.v[k] = fmaf(x1, c.x, x0 * c.y);
+        }
+      } else if (i < nr) {
+#pragma unroll
+        for (int k = 0; k + 1 < VEC; k += 2) {
+          const float2 c = cs[(e0 + k) / 2];
+          const float x0 = a.v[k], x1 = a.v[k + 1];
+          a.v[k] = fmaf(x0, c.x, -x1 * c.y);
+          a.v[k + 1] = fmaf(x1, c.x, x0 * c.y);
+        }
+      }
+      if (is_q) {
+        store_f32<VEC>(qo + e0, a);
+        if (two) store_f32<VEC>(qo + e0 + apart, b);
+      } else {
+        store_cache<VEC>(co + e0, a, A.c.k_scale);
+        if (two) store_cache<VEC>(co + e0 + apart, b, A.c.k_scale);
+      }
+    }
+  };
+  for (int row = g0; row < rows; row += kRowsAhead * step) {
+#pragma unroll
+    for (int k = 0; k < kRowsAhead; ++k) {
+      if (row + k * step < rows) finish(row + k * step, ahead[k]);
+      fetch(row + (k + kRowsAhead) * step, ahead[k]);
+    }
+  }
+}
+
+template <int DT>
+static int launch_norm_append(RopeArgs& a, const NormArgs& n, int T, cudaStream_t s) {
+  const bool vec = four_at_a_time(a);
+  const int d = a.c.head_dim;
+  if (vec) {
+    a.nr = a.interleaved ? a.rot / 4 : a.rot / 8;
+    a.ni = a.nr + (d - a.rot) / 4;
+    a.nv = d / 4;
+  } else {                             // items are pairs, then single elements
+    a.nr = a.rot / 2;
+    a.ni = a.nr + (d - a.rot);
+    a.nv = d;
+  }
+  // lanes of a row: two items each at most (eight single elements)
+  const int gl = !vec || d > 128 ? 32 : d > 64 ? 16 : 8;
+  auto kern = !vec       ? norm_append_kernel<DT, 1, 32>
+              : gl == 32 ? norm_append_kernel<DT, 4, 32>
+              : gl == 16 ? norm_append_kernel<DT, 4, 16>
+                         : norm_append_kernel<DT, 4, 8>;
+  const int rows = a.hq + 2 * a.c.kv_heads;
+  const int threads = T > 8 * sm_count() ? 128 : kRopeThreads;
+  const int parts = std::max(1, std::min(sm_count() / T, rows * gl / threads));
+  MOE_CUDA(launch_pdl(kern, dim3((unsigned)T, (unsigned)parts), dim3((unsigned)threads), 0, s, a, n));
+  return MOE_OK;
+}
+
+}  // namespace moe
+
+namespace moe {
+
+// The arguments that both forms of the append share.
+static int take_append(const moe_rope_append_args* r, RopeArgs& a) {
+  const moe_paged_cache* cache = &r->cache;
+  moe_paged_cache c;
+  MOE_CHECK(take_cache(cache, c));
+  MOE_CHECK(check_cache_rows_apart(c));
+  const int T = r->T, q_heads = r->q_heads, rot = r->rot;
+  const float *q = r->q, *k = r->k, *v = r->v;
+  float* q_out = r->q_out;
+  MOE_REQUIRE(T >= 0 && q_heads >= 0, MOE_ERR_INVALID, "negative size");
+  MOE_REQUIRE(q_heads <= 32767 && cache->kv_heads <= 16383, MOE_ERR_UNSUPPORTED, "too many heads");
+  MOE_REQUIRE(rot >= 0 && rot % 2 == 0 && rot <= cache->head_dim, MOE_ERR_INVALID,
+              "rot %d: an even number up to head_dim %d is needed", rot, cache->head_dim);
+  if (T == 0) return MOE_OK;
+  MOE_REQUIRE(k && v && r->positions && (rot == 0 || r->inv_freq), MOE_ERR_INVALID, "null pointer");
+  MOE_REQUIRE(q_heads == 0 || (q && q_out), MOE_ERR_INVALID, "null q or q_out");
+  if (q_heads > 0) {
+    MOE_REQUIRE((T == 1 || r->qo_tok_stride >= c.head_dim || -r->qo_tok_stride >= c.head_dim) &&
+                    (q_heads == 1 || r->qo_head_stride >= c.head_dim ||
+                     -r->qo_head_stride >= c.head_dim),
+                MOE_ERR_INVALID, "rows of q_out overlap");
+    MOE_REQUIRE(q_out != q || ((T == 1 || r->qo_tok_stride == r->q_tok_stride) &&
+                               (q_heads == 1 || r->qo_head_stride == r->q_head_stride)),
+                MOE_ERR_INVALID, "q_out is q with other strides");
+    MOE_REQUIRE(q_out != k && q_out != v, MOE_ERR_INVALID, "q_out overlaps k or v");
+  }
+  MOE_REQUIRE(r->seq_ids || T <= cache->seqs, MOE_ERR_INVALID,
+              "%d tokens for %d sequences need seq_ids", T, cache->seqs);
+  a = {c, q, k, v, r->q_tok_stride, r->q_head_stride, r->k_tok_stride, r->k_head_stride,
+       r->v_tok_stride, r->v_head_stride, r->qo_tok_stride, r->qo_head_stride, q_out, r->positions,
+       r->seq_ids, r->inv_freq, r->status, q_heads, rot, r->interleaved};
+  return MOE_OK;
+}
+
 }  // namespace moe
 
 extern "C" {
+
+int moe_rope_append_record(const moe_rope_append_args* r) {
+  MOE_REQUIRE(r, MOE_ERR_INVALID, "null arguments");
+  moe::RopeArgs a = {};
+  MOE_CHECK(moe::take_append(r, a));
+  if (r->T == 0) return MOE_OK;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(r->stream);
+  {
+    ::moe::ProfScope _prof(MOE_K_ROPE_APPEND, s);
+    const int dt = a.c.dtype;
+    MOE_CHECK(dt == MOE_CACHE_F16    ? moe::launch_rope<MOE_CACHE_F16>(a, r->T, s)
+              : dt == MOE_CACHE_BF16 ? moe::launch_rope<MOE_CACHE_BF16>(a, r->T, s)
+                                     : moe::launch_rope<MOE_CACHE_E4M3>(a, r->T, s));
+  }
+  return moe::check_launch("rope_append");
+}
 
 int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_stride,
                     int64_t q_head_stride, const float* k, int64_t k_tok_stride,
@@ -205,46 +473,34 @@ int moe_rope_append(const moe_paged_cache* cache, const float* q, int64_t q_tok_
                     const int32_t* seq_ids, const double* inv_freq, int rot, int interleaved,
                     float* q_out, int64_t qo_tok_stride, int64_t qo_head_stride, int32_t* status,
                     moe_stream_t stream) {
-  moe_paged_cache c;
-  MOE_CHECK(moe::take_cache(cache, c));
-  MOE_CHECK(moe::check_cache_rows_apart(c));
-  MOE_REQUIRE(T >= 0 && q_heads >= 0, MOE_ERR_INVALID, "negative size");
-  MOE_REQUIRE(q_heads <= 32767 && cache->kv_heads <= 16383, MOE_ERR_UNSUPPORTED, "too many heads");
-  MOE_REQUIRE(rot >= 0 && rot % 2 == 0 && rot <= cache->head_dim, MOE_ERR_INVALID,
-              "rot %d: an even number up to head_dim %d is needed", rot, cache->head_dim);
-  if (T == 0) return MOE_OK;
-  MOE_REQUIRE(k && v && positions && (rot == 0 || inv_freq), MOE_ERR_INVALID, "null pointer");
-  MOE_REQUIRE(q_heads == 0 || (q && q_out), MOE_ERR_INVALID, "null q or q_out");
-  if (q_heads > 0) {
-    MOE_REQUIRE((T == 1 || qo_tok_stride >= c.head_dim || -qo_tok_stride >= c.head_dim) &&
-                    (q_heads == 1 || qo_head_stride >= c.head_dim || -qo_head_stride >= c.head_dim),
-                MOE_ERR_INVALID, "rows of q_out overlap");
-    MOE_REQUIRE(q_out != q || ((T == 1 || qo_tok_stride == q_tok_stride) &&
-                               (q_heads == 1 || qo_head_stride == q_head_stride)),
-                MOE_ERR_INVALID, "q_out is q with other strides");
-    MOE_REQUIRE(q_out != k && q_out != v, MOE_ERR_INVALID, "q_out overlaps k or v");
-  }
-  MOE_REQUIRE(seq_ids || T <= cache->seqs, MOE_ERR_INVALID,
-              "%d tokens for %d sequences need seq_ids", T, cache->seqs);
-  moe::RopeArgs a = {c, q, k, v, q_tok_stride, q_head_stride, k_tok_stride, k_head_stride,
-                     v_tok_stride, v_head_stride, qo_tok_stride, qo_head_stride, q_out, positions,
-                     seq_ids, inv_freq, status, q_heads, rot, interleaved};
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  {
-    ::moe::ProfScope _prof(MOE_K_ROPE_APPEND, s);
-    MOE_CHECK(cache->dtype == MOE_CACHE_F16    ? moe::launch_rope<MOE_CACHE_F16>(a, T, s)
-              : cache->dtype == MOE_CACHE_BF16 ? moe::launch_rope<MOE_CACHE_BF16>(a, T, s)
-                                               : moe::launch_rope<MOE_CACHE_E4M3>(a, T, s));
-  }
-  return moe::check_launch("rope_append");
+  MOE_REQUIRE(cache, MOE_ERR_INVALID, "null cache");
+  const moe_rope_append_args a = {*cache, q, k, v, q_tok_stride, q_head_stride, k_tok_stride,
+                                  k_head_stride, v_tok_stride, v_head_stride, positions, seq_ids,
+                                  inv_freq, q_out, qo_tok_stride, qo_head_stride, status, stream, T,
+                                  q_heads, rot, interleaved};
+  return moe_rope_append_record(&a);
 }
 
-int moe_rope_append_record(const moe_rope_append_args* a) {
-  MOE_REQUIRE(a, MOE_ERR_INVALID, "null arguments");
-  return moe_rope_append(&a->cache, a->q, a->q_tok_stride, a->q_head_stride, a->k, a->k_tok_stride,
-                         a->k_head_stride, a->v, a->v_tok_stride, a->v_head_stride, a->T,
-                         a->q_heads, a->positions, a->seq_ids, a->inv_freq, a->rot, a->interleaved,
-                         a->q_out, a->qo_tok_stride, a->qo_head_stride, a->status, a->stream);
+int moe_norm_append_record(const moe_norm_append_args* r) {
+  MOE_REQUIRE(r, MOE_ERR_INVALID, "null arguments");
+  moe::RopeArgs a = {};
+  MOE_CHECK(moe::take_append(&r->append, a));
+  const int T = r->append.T;
+  MOE_REQUIRE(std::isfinite(r->eps) && r->eps >= 0.f, MOE_ERR_INVALID, "eps must be finite, >= 0");
+  MOE_REQUIRE(!r->mass == !r->held, MOE_ERR_INVALID, "mass and held come together");
+  MOE_REQUIRE(!r->mass || r->ledger_slots > 0, MOE_ERR_INVALID, "bad ledger");
+  if (T == 0) return MOE_OK;
+  const moe::NormArgs n = {r->q_norm, r->k_norm, r->slots, r->mass, r->held, r->ledger_slots, r->eps,
+                           r->gemma_style ? 1.f : 0.f};
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(r->append.stream);
+  {
+    ::moe::ProfScope _prof(MOE_K_ROPE_APPEND, s);
+    const int dt = a.c.dtype;
+    MOE_CHECK(dt == MOE_CACHE_F16    ? moe::launch_norm_append<MOE_CACHE_F16>(a, n, T, s)
+              : dt == MOE_CACHE_BF16 ? moe::launch_norm_append<MOE_CACHE_BF16>(a, n, T, s)
+                                     : moe::launch_norm_append<MOE_CACHE_E4M3>(a, n, T, s));
+  }
+  return moe::check_launch("norm_append");
 }
 
 }  // extern "C"

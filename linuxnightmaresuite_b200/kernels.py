@@ -299,6 +299,12 @@ _CACHE = "3P4q7i2f"
 _APPEND_ARGS = struct.Struct("@" + _CACHE + "3P6q4P2q2P4i0q")
 _ATTENTION_ARGS = struct.Struct("@" + _CACHE + "P2q4PNP3i2f0q")
 _LINEAR_ARGS = struct.Struct("@2PqPqPqP4i")
+_NORM_APPEND_ARGS = struct.Struct("@" + _CACHE + "3P6q4P2q2P4i5Pqfi0q")
+_MASS_ARGS = struct.Struct("@" + _CACHE + "P2q4Pq2P3i2f0q")
+_EVICT_ARGS = struct.Struct("@" + _CACHE + "6P2q2P3i0q")
+assert _NORM_APPEND_ARGS.size == ctypes.sizeof(_lib.MoENormAppendArgs)
+assert _MASS_ARGS.size == ctypes.sizeof(_lib.MoEAttentionMassArgs)
+assert _EVICT_ARGS.size == ctypes.sizeof(_lib.MoECacheEvictArgs)
 assert _APPEND_ARGS.size == ctypes.sizeof(_lib.MoERopeAppendArgs)
 assert _ATTENTION_ARGS.size == ctypes.sizeof(_lib.MoEPagedAttentionArgs)
 assert _LINEAR_ARGS.size == ctypes.sizeof(_lib.MoELinearArgs)
@@ -385,12 +391,26 @@ def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torc
             index, table[0], shape[2], shape[3])
 
 
+def _ledger(t: torch.Tensor, dtype, name: str, index: int, seqs: int,
+            kv_heads: int) -> Tuple[int, int]:
+    """(address, slots) of a contiguous CUDA tensor (sequences, kv_heads, slots)."""
+    shape = t.shape
+    if t.dtype is not dtype or t.get_device() != index or len(shape) != 3 or \
+            shape[0] != seqs or shape[1] != kv_heads or not t.is_contiguous():
+        _refuse(t, name, dtype, index, (seqs, kv_heads, shape[2] if len(shape) == 3 else 0))
+    return t.data_ptr(), shape[2]
+
+
 def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
                 k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                 positions: torch.Tensor, inv_freq: Optional[torch.Tensor] = None,
                 seq_ids: Optional[torch.Tensor] = None, interleaved: bool = False,
                 k_scale: float = 1.0, v_scale: float = 1.0, q_out: Optional[torch.Tensor] = None,
-                status: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                status: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
+                k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                gemma_style: bool = False, slots: Optional[torch.Tensor] = None,
+                mass: Optional[torch.Tensor] = None,
+                held: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Rotates q (T, q_heads, head_dim) and k (T, kv_heads, head_dim) by their
     positions, writes k and v into the paged caches (pages, page_size,
     kv_heads, head_dim; any page layout as a view) and returns the rotated q
@@ -403,8 +423,16 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     its token, q row included (without ``q_out`` that row is not set); no two
     tokens may share sequence and position.
     ``status`` (int32) receives STATUS_BAD_PAGE for a page or sequence that
-    does not exist; such a token's k and v are not stored."""
-    c, dev, _, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
+    does not exist; such a token's k and v are not stored.
+
+    ``q_norm``, ``k_norm`` (head_dim,) f32 norm each head of q and of k in
+    front of its rotation: x / sqrt(mean(x^2) + eps) * w, or * (1 + w) with
+    ``gemma_style``.  ``slots`` (T,) int32 says where in its sequence's pages a
+    token goes when that is not its position (a cache that ``cache_evict`` has
+    cut); a negative one skips the token.  ``mass`` f32 and ``held`` int32
+    (sequences, kv_heads, slots) get 0 and the token's position in the new
+    slots."""
+    c, dev, seqs, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
     T = k.shape[0]
     ks = _rows_f32(k, "k", dev, (T, hk, d))
     vs = _rows_f32(v, "v", dev, (T, hk, d))
@@ -425,12 +453,27 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         else:
             os_ = _rows_f32(q_out, "q_out", dev, (T, hq, d))
         q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
-    _enqueue("moe_rope_append_record", dev, _APPEND_ARGS.pack(
-        *c, q_ptr, k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
-        _vector(positions, _I32, "positions", dev, T),
-        0 if seq_ids is None else _vector(seq_ids, _I32, "seq_ids", dev, T), freq, o_ptr, os_[0],
-        os_[1], 0 if status is None else _vector(status, _I32, "status", dev, 1),
-        _raw_stream(dev), T, hq, rot, 1 if interleaved else 0))
+    args = (*c, q_ptr, k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+            _vector(positions, _I32, "positions", dev, T),
+            0 if seq_ids is None else _vector(seq_ids, _I32, "seq_ids", dev, T), freq, o_ptr,
+            os_[0], os_[1], 0 if status is None else _vector(status, _I32, "status", dev, 1),
+            _raw_stream(dev), T, hq, rot, 1 if interleaved else 0)
+    if q_norm is None and k_norm is None and slots is None and mass is None and held is None:
+        _enqueue("moe_rope_append_record", dev, _APPEND_ARGS.pack(*args))
+        return q_out
+    if (mass is None) != (held is None):
+        raise ValueError("mass and held come together")
+    m = h = width = 0
+    if mass is not None:
+        m, width = _ledger(mass, _F32, "mass", dev, seqs, hk)
+        h, width_h = _ledger(held, _I32, "held", dev, seqs, hk)
+        if width_h != width:
+            raise ValueError(f"mass has {width} slots, held {width_h}")
+    _enqueue("moe_norm_append_record", dev, _NORM_APPEND_ARGS.pack(
+        *args, 0 if q_norm is None else _vector(q_norm, _F32, "q_norm", dev, d),
+        0 if k_norm is None else _vector(k_norm, _F32, "k_norm", dev, d),
+        0 if slots is None else _vector(slots, _I32, "slots", dev, T), m, h, width, eps,
+        1 if gemma_style else 0))
     return q_out
 
 
@@ -500,6 +543,80 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if status is not None and seqs:
         status |= ws[:4].view(_I32)
     return (out, lse) if return_lse else out
+
+
+def attention_mass(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor,
+                   seq_lens: torch.Tensor, lse: torch.Tensor, mass: torch.Tensor,
+                   scale: Optional[float] = None, window: int = 0, softcap: float = 0.0,
+                   k_scale: float = 1.0, max_len: int = 0, out: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Adds to ``mass`` (sequences, kv_heads, slots) f32 the attention weight
+    that each of the first ``seq_lens[s]`` slots receives from q (sequences,
+    q_heads, head_dim): the sum of exp(scale q.k - lse) over the query heads of
+    a key head, with the ``lse`` (sequences, q_heads) that ``paged_attention``
+    returned for q and equal ``scale``, ``window`` and ``softcap``.  The sums go
+    to ``out`` (default: mass itself); slots behind a sequence are left as they
+    were.  ``max_len`` (no sequence is longer; 0 = what table and ledger hold)
+    sizes the launch.  ``status`` (int32) receives STATUS_BAD_PAGE for a page
+    that does not exist or a length that table or ledger do not hold."""
+    c, dev, seqs, hk, d = _paged_cache(k_cache, k_cache, block_table, k_scale, k_scale)
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError("q must be (sequences, q_heads, head_dim)")
+    hq = shape[1]
+    qs = _rows_f32(q, "q", dev, (seqs, hq, d))
+    if lse.dtype is not _F32 or lse.get_device() != dev or lse.shape != (seqs, hq) or \
+            not lse.is_contiguous():
+        _refuse(lse, "lse", _F32, dev, (seqs, hq))
+    m, width = _ledger(mass, _F32, "mass", dev, seqs, hk)
+    if out is None:
+        out, o = mass, m
+    else:
+        o, width_o = _ledger(out, _F32, "out", dev, seqs, hk)
+        if width_o != width:
+            raise ValueError(f"mass has {width} slots, out {width_o}")
+    _enqueue("moe_attention_mass_record", dev, _MASS_ARGS.pack(
+        *c, q.data_ptr(), qs[0], qs[1], _vector(seq_lens, _I32, "seq_lens", dev, seqs),
+        lse.data_ptr(), m, o, width, 0 if status is None else _vector(status, _I32, "status", dev, 1),
+        _raw_stream(dev), hq, max_len, window, d ** -0.5 if scale is None else scale, softcap))
+    return out
+
+
+def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                seq_lens: torch.Tensor, mass: torch.Tensor, held: torch.Tensor, keep: int,
+                recent: int = 0, mass_out: Optional[torch.Tensor] = None,
+                held_out: Optional[torch.Tensor] = None, lens_out: Optional[torch.Tensor] = None,
+                max_len: int = 0, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Cuts each (sequence, key head) that holds more than ``keep`` slots down to
+    ``keep``: the tokens held at the last ``recent`` positions stay, then those
+    of the largest ``mass`` (of equals the lowest slot).  Survivors in slots from
+    ``keep`` on move, in order, into the slots below that are given up: rows of
+    both caches and the entries of ``mass`` f32 and ``held`` int32 (sequences,
+    kv_heads, slots), in place unless ``mass_out`` or ``held_out`` (at least
+    ``keep`` slots) is given.  Returns ``lens_out`` (default: seq_lens itself),
+    min(seq_lens, keep).
+
+    ``max_len`` (no sequence is longer, 0 = what table and ledger hold; at most
+    163840) sizes the launch; a longer one is left as it is and reported.  No
+    page of a shortened sequence may belong to another sequence too.
+    ``status`` (int32) receives STATUS_BAD_PAGE."""
+    c, dev, seqs, hk, _ = _paged_cache(k_cache, v_cache, block_table, 1.0, 1.0)
+    m, width = _ledger(mass, _F32, "mass", dev, seqs, hk)
+    h, width_h = _ledger(held, _I32, "held", dev, seqs, hk)
+    mo, wide = (m, width) if mass_out is None else _ledger(mass_out, _F32, "mass_out", dev, seqs, hk)
+    ho, wide_h = (h, width) if held_out is None else _ledger(held_out, _I32, "held_out", dev, seqs,
+                                                             hk)
+    if width_h != width or wide_h != wide:
+        raise ValueError(f"mass has {width} slots, held {width_h}; mass_out {wide}, held_out "
+                         f"{wide_h}")
+    lens = _vector(seq_lens, _I32, "seq_lens", dev, seqs)
+    if lens_out is None:
+        lens_out = seq_lens
+    _enqueue("moe_cache_evict_record", dev, _EVICT_ARGS.pack(
+        *c, lens, m, h, mo, ho, _vector(lens_out, _I32, "lens_out", dev, seqs), width, wide,
+        0 if status is None else _vector(status, _I32, "status", dev, 1), _raw_stream(dev), keep,
+        recent, max_len))
+    return lens_out
 
 
 class LinearWeights:
