@@ -122,7 +122,8 @@ enum {
   MOE_K_ROUTER = 0, MOE_K_ROUTER_SELECT, MOE_K_DISPATCH, MOE_K_PLAN, MOE_K_XPREP,
   MOE_K_GATEUP, MOE_K_DOWN, MOE_K_COMBINE, MOE_K_RMS_NORM, MOE_K_PACK, MOE_K_DEQUANT,
   MOE_K_AUX, MOE_K_EP_SEND, MOE_K_EP_RECV, MOE_K_EP_RETURN, MOE_K_EP_WAIT, MOE_K_ROPE_APPEND,
-  MOE_K_ATTENTION, MOE_K_LINEAR, MOE_K_ATTENTION_MASS, MOE_K_CACHE_EVICT, MOE_K_COUNT
+  MOE_K_ATTENTION, MOE_K_LINEAR, MOE_K_ATTENTION_MASS, MOE_K_CACHE_EVICT,
+  MOE_K_PREFIX, MOE_K_COUNT
 };
 int moe_profile_enable(int on);
 int moe_profile_collect(float* ms, int* launches, int n);
@@ -541,6 +542,28 @@ typedef struct moe_linear_args {
 int moe_rope_append_record(const moe_rope_append_args* args);
 int moe_paged_attention_record(const moe_paged_attention_args* args);
 int moe_linear_record(const moe_linear_args* args);
+
+/* ---- a prefix that a batch shares -------------------------------------------------------
+ * moe_paged_attention for sequences that all begin with the same `prefix_pages` whole pages
+ * (a system prompt, a document): their keys are read and multiplied once, for the rows of all
+ * sequences together.
+ *   attention: as moe_paged_attention takes them, but for window, which must be 0, and workspace,
+ *          whose size is moe_prefix_attention_workspace_bytes.  out 16-byte aligned
+ *   prefix (prefix_pages,) int32: the pages.  Entries of the block table for the same tokens
+ *          are not read: keys and values of a sequence from prefix_pages * page_size on come
+ *          from its row
+ *   seq_lens: the prefix included.  0 or less gives zeros in out and -inf in lse.  So does a length
+ *          between, which sets MOE_STATUS_BAD_PAGE: every other sequence holds the whole prefix
+ * prefix_pages 0 is moe_paged_attention.  The split over the GPU depends on sizes alone; equal
+ * calls give equal bits. */
+typedef struct moe_prefix_attention_args {
+  moe_paged_attention_args attention;
+  const int32_t* prefix;
+  int prefix_pages;
+} moe_prefix_attention_args;
+int moe_prefix_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int head_dim,
+                                         size_t* bytes);
+int moe_prefix_attention_record(const moe_prefix_attention_args* args);
 
 /* ---- a cache that shrinks -------------------------------------------------------------
  * The calls below take their arguments in one record only.

@@ -106,6 +106,11 @@ class MoELinearArgs(ctypes.Structure):
     ]
 
 
+class MoEPrefixAttentionArgs(ctypes.Structure):
+    """Mirror of ``moe_prefix_attention_args``."""
+    _fields_ = [("attention", MoEPagedAttentionArgs), ("prefix", vp), ("prefix_pages", ci)]
+
+
 class MoENormAppendArgs(ctypes.Structure):
     """Mirror of ``moe_norm_append_args``."""
     _fields_ = [
@@ -182,6 +187,8 @@ SIGNATURES = {
     "moe_rope_append_record": [vp],
     "moe_paged_attention_record": [vp],
     "moe_linear_record": [vp],
+    "moe_prefix_attention_workspace_bytes": [ci, ci, ci, ci, ctypes.POINTER(csz)],
+    "moe_prefix_attention_record": [vp],
     "moe_norm_append_record": [vp],
     "moe_attention_mass_record": [vp],
     "moe_cache_evict_record": [vp],
@@ -191,7 +198,7 @@ SIGNATURES = {
 KERNEL_NAMES = ["router", "router_select", "dispatch", "plan", "xprep", "gateup", "down",
                 "combine", "rms_norm", "pack", "dequant", "aux", "ep_send", "ep_recv_plan",
                 "ep_return", "ep_wait", "rope_append", "attention", "linear", "attention_mass",
-                "cache_evict"]
+                "cache_evict", "prefix"]
 
 MOE_EP_PHASE_SEND = 1
 MOE_EP_PHASE_SERVE = 2

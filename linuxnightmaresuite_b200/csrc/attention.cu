@@ -57,12 +57,10 @@
 namespace moe {
 
 constexpr int kAttCtasMost = 3;       // CTAs of an SM
-constexpr float kPShift = 7.f;        // probabilities enter sums and products times 2^7
 
 struct AttArgs {
   moe_paged_cache c;
-  int page_units, head_units;         // strides in rows of the tensor maps
-  int box_shift;                      // log2 of the rows of a TMA box
+  CacheMap map;
   const float* q;
   int64_t q_ss, q_hs;
   const int32_t* seq_lens;
@@ -71,7 +69,7 @@ struct AttArgs {
   int* arrivals;                      // one per CTA
   float2* part_ml;                    // [2 * grid][kAttHeads] (maximum, sum)
   float* part_o;                      // [2 * grid][kAttHeads][DP]
-  int hq, window;
+  int hq, window, from;               // from: keys before it are not seen
   float scale, cap;
 };
 
@@ -83,7 +81,6 @@ struct AttArgs {
 // of one warp do not hold the accumulators of 256 columns, and without them
 // every tile would be folded.
 // ---------------------------------------------------------------------------
-constexpr int kLine = 128;             // bytes of a row in one box
 template <int DT, int DP, bool PACK> struct AttCfg {
   static constexpr bool kBf = DT == MOE_CACHE_BF16;
   using Frag = AFrag<kBf, PACK>;
@@ -170,7 +167,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   // ---- this CTA's run of rounds
   auto keys_of = [&](int s, int& first) {
     const int n = min(max(A.seq_lens[s], 0), most);
-    first = A.window > 0 && n > A.window ? n - A.window : 0;
+    first = A.window > 0 && n > A.window ? n - A.window : A.from;
     return n;
   };
   // rounds start at a multiple of KEYS, so that no box crosses a page's end;
@@ -322,7 +319,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   // the ends of units
   const uint32_t ring_a = smem_u32(smem) + warp * NS * Cfg::kSlot;
   constexpr int BLOCKS = Cfg::kRow / LINE;
-  const int box = 1 << A.box_shift, boxes = KEYS >> A.box_shift, ps = A.c.page_size;
+  const int box = 1 << A.map.box_shift, boxes = KEYS >> A.map.box_shift, ps = A.c.page_size;
   const int step_pages = RK / ps, step_slots = RK - step_pages * ps;   // from tile to tile
   Cursor W = C;                                  // of the loads
   int wtiles = tiles(W), wend = keys_end(W), wkey = tile0(W), li = 0, lslot = 0;
@@ -336,7 +333,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     wtiles = tiles(W);
     wend = keys_end(W);
     wkey = tile0(W);
-    key = wkey + (lane << A.box_shift);
+    key = wkey + (lane << A.map.box_shift);
     pidx = (int)((unsigned)key / (unsigned)ps);
     pslot = key - pidx * ps;
   };
@@ -357,7 +354,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     if (lane == 0) mbar_expect_tx(bar, bytes);
     __syncwarp();
     if (in) {
-      const uint32_t dst = ring_a + lslot * Cfg::kSlot + (lane << A.box_shift) * LINE;
+      const uint32_t dst = ring_a + lslot * Cfg::kSlot + (lane << A.map.box_shift) * LINE;
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b)
         tma_load_3d(dst + b * KEYS * LINE, map, warp % SP * DH + b * (LINE / Cfg::kElem), row, pslot,
@@ -371,16 +368,16 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       set_status(A.status, MOE_STATUS_BAD_PAGE);
       in = false;
     }
-    row = page * A.page_units + W.head * A.head_units;
+    row = page * A.map.page_units + W.head * A.map.head_units;
     const uint32_t ok = __ballot_sync(0xffffffffu, in);
     const int n = __popc(ok);
     uint32_t seen = 0xffffffffu;
     if (n != boxes || wkey < W.first || wkey + KEYS > wend) {
       const int r = lane & (KEYS - 1);
       seen = __ballot_sync(0xffffffffu, wkey + r >= W.first && wkey + r < wend &&
-                                            ((ok >> (r >> A.box_shift)) & 1u));
+                                            ((ok >> (r >> A.map.box_shift)) & 1u));
     }
-    bytes = (uint32_t)(n * BLOCKS * LINE) << A.box_shift;
+    bytes = (uint32_t)(n * BLOCKS * LINE) << A.map.box_shift;
     copy(&kmap);
     return seen;
   };
@@ -849,6 +846,41 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+// The cache as a 3-D tensor for TMA: elements of a row; rows one common unit of
+// the strides apart (a page and a head lead to a row number); tokens of a page.
+int make_cache_map(CUtensorMap* map, const moe_paged_cache& c, void* base, int keys,
+                   CacheMap* at) {
+  const int eb = cache_elem_bytes(c.dtype);
+  const int64_t row = (int64_t)c.head_dim;
+  int64_t unit = std::gcd(std::gcd(c.page_stride, c.token_stride), c.head_stride);
+  if (unit == 0) unit = row;
+  MOE_REQUIRE(unit >= row, MOE_ERR_UNSUPPORTED,
+              "cache strides (%lld, %lld, %lld) are not multiples of one row of at least head_dim "
+              "elements",
+              (long long)c.page_stride, (long long)c.token_stride, (long long)c.head_stride);
+  const int64_t rows = ((c.pages - 1) * c.page_stride + (c.kv_heads - 1) * c.head_stride) / unit + 1;
+  MOE_REQUIRE(rows <= 0x7fffffff && unit * eb < (1ll << 40) && c.token_stride * eb < (1ll << 40),
+              MOE_ERR_UNSUPPORTED, "cache of %lld rows is too large", (long long)rows);
+  at->page_units = (int)(c.page_stride / unit);
+  at->head_units = (int)(c.head_stride / unit);
+  const int rows_of_box = std::min(keys, c.page_size & -c.page_size);
+  at->box_shift = 31 - __builtin_clz((unsigned)rows_of_box);
+  const cuuint64_t dims[3] = {(cuuint64_t)row, (cuuint64_t)rows, (cuuint64_t)c.page_size};
+  const cuuint64_t strides[2] = {(cuuint64_t)(unit * eb),
+                                 (cuuint64_t)(std::max(c.token_stride, unit) * eb)};
+  const cuuint32_t box[3] = {(cuuint32_t)(kLine / eb), 1, (cuuint32_t)rows_of_box};
+  const cuuint32_t each[3] = {1, 1, 1};
+  EncodeTiledFn fn = encode_fn();
+  MOE_REQUIRE(fn, MOE_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const CUresult r =
+      fn(map, eb == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base,
+         dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  MOE_REQUIRE(r == CUDA_SUCCESS, MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return MOE_OK;
+}
+
 inline int padded_head_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 static int attention_workspace(int head_dim, AttArgs* a, void* ws, size_t* bytes) {
@@ -867,41 +899,6 @@ static int attention_workspace(int head_dim, AttArgs* a, void* ws, size_t* bytes
   return MOE_OK;
 }
 
-// The cache as a 3-D tensor for TMA: elements of a row; rows one common unit of
-// the strides apart (a page and a head lead to a row number); tokens of a page.
-static int make_cache_map(CUtensorMap* map, AttArgs& a, void* base, int keys) {
-  const moe_paged_cache& c = a.c;
-  const int eb = cache_elem_bytes(c.dtype);
-  const int64_t row = (int64_t)c.head_dim;
-  int64_t unit = std::gcd(std::gcd(c.page_stride, c.token_stride), c.head_stride);
-  if (unit == 0) unit = row;
-  MOE_REQUIRE(unit >= row, MOE_ERR_UNSUPPORTED,
-              "cache strides (%lld, %lld, %lld) are not multiples of one row of at least head_dim "
-              "elements",
-              (long long)c.page_stride, (long long)c.token_stride, (long long)c.head_stride);
-  const int64_t rows = ((c.pages - 1) * c.page_stride + (c.kv_heads - 1) * c.head_stride) / unit + 1;
-  MOE_REQUIRE(rows <= 0x7fffffff && unit * eb < (1ll << 40) && c.token_stride * eb < (1ll << 40),
-              MOE_ERR_UNSUPPORTED, "cache of %lld rows is too large", (long long)rows);
-  a.page_units = (int)(c.page_stride / unit);
-  a.head_units = (int)(c.head_stride / unit);
-  const int rows_of_box = std::min(keys, c.page_size & -c.page_size);
-  a.box_shift = 31 - __builtin_clz((unsigned)rows_of_box);
-  const cuuint64_t dims[3] = {(cuuint64_t)row, (cuuint64_t)rows, (cuuint64_t)c.page_size};
-  const cuuint64_t strides[2] = {(cuuint64_t)(unit * eb),
-                                 (cuuint64_t)(std::max(c.token_stride, unit) * eb)};
-  const cuuint32_t box[3] = {(cuuint32_t)(kLine / eb), 1, (cuuint32_t)rows_of_box};
-  const cuuint32_t each[3] = {1, 1, 1};
-  EncodeTiledFn fn = encode_fn();
-  MOE_REQUIRE(fn, MOE_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  const CUresult r =
-      fn(map, eb == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base,
-         dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  MOE_REQUIRE(r == CUDA_SUCCESS, MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return MOE_OK;
-}
-
 template <int DT, int DP, bool PACK>
 static int launch_attention(AttArgs& a, int max_len, cudaStream_t s) {
   using Cfg = AttCfg<DT, DP, PACK>;
@@ -917,11 +914,11 @@ static int launch_attention(AttArgs& a, int max_len, cudaStream_t s) {
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   CUtensorMap kmap, vmap;
-  MOE_CHECK(make_cache_map(&kmap, a, a.c.k, Cfg::kKeys));
-  MOE_CHECK(make_cache_map(&vmap, a, a.c.v, Cfg::kKeys));
+  MOE_CHECK(make_cache_map(&kmap, a.c, a.c.k, Cfg::kKeys, &a.map));
+  MOE_CHECK(make_cache_map(&vmap, a.c, a.c.v, Cfg::kKeys, &a.map));
   const int G = a.hq / a.c.kv_heads;
   const int64_t units = (int64_t)a.c.seqs * a.c.kv_heads * ((G + kAttHeads - 1) / kAttHeads);
-  const int64_t keys = a.window > 0 ? std::min(a.window, max_len) : max_len;
+  const int64_t keys = a.window > 0 ? std::min(a.window, max_len) : std::max(0, max_len - a.from);
   // A round costs about 1 us, a unit in parts about 3 us for their joining: short
   // sequences get a CTA per unit (one of 100 keys 6.3 us instead of 8.0; with three
   // rounds ragged batches lose more than that: their units are split all the same)
@@ -947,6 +944,74 @@ static int launch_attention_dt(AttArgs& a, int max_len, cudaStream_t s) {
   }
 }
 
+// Refuses what the attention cannot take; c: the cache as the kernels take it.
+int check_attention(const moe_paged_attention_args& r, moe_paged_cache& c) {
+  const float* q = r.q;
+  float* out = r.out;
+  MOE_CHECK(take_cache(&r.cache, c));
+  MOE_REQUIRE(r.q_heads > 0 && r.q_heads % c.kv_heads == 0, MOE_ERR_INVALID,
+              "%d query heads for %d key heads", r.q_heads, c.kv_heads);
+  MOE_REQUIRE(r.max_len >= 0 && r.window >= 0, MOE_ERR_INVALID, "negative length or window");
+  MOE_REQUIRE(isfinite(r.scale) && isfinite(r.softcap) && r.softcap >= 0.f, MOE_ERR_INVALID,
+              "scale and softcap must be finite, softcap >= 0");
+  if (c.seqs == 0) return MOE_OK;
+  MOE_REQUIRE(q && r.seq_lens && out && r.workspace, MOE_ERR_INVALID, "null pointer");
+  // parts in it are fetched by bulk copies
+  MOE_REQUIRE((uintptr_t)r.workspace % 16 == 0, MOE_ERR_INVALID, "workspace must be 16-byte aligned");
+  {
+    // A unit's rows of out are written behind the last read of its rows of q, so out
+    // may be q itself, but over other rows it would be read when it is written already.
+    const int64_t S = c.seqs, d = c.head_dim, n = S * r.q_heads * d;
+    const bool same = (uintptr_t)out == (uintptr_t)q && (S == 1 || r.q_seq_stride == r.q_heads * d) &&
+                      (r.q_heads == 1 || r.q_head_stride == d);
+    const int64_t ss = (S - 1) * r.q_seq_stride, hs = (r.q_heads - 1) * r.q_head_stride;
+    const int64_t lo = std::min<int64_t>(ss, 0) + std::min<int64_t>(hs, 0);
+    const int64_t hi = std::max<int64_t>(ss, 0) + std::max<int64_t>(hs, 0) + d;
+    const int64_t at = (int64_t)((uintptr_t)out - (uintptr_t)q);         // bytes
+    MOE_REQUIRE(same || at >= 4 * hi || at + 4 * n <= 4 * lo, MOE_ERR_INVALID,
+                "q and out overlap, and are not the same rows");
+  }
+  return MOE_OK;
+}
+
+// The attention over the keys from `from` on.
+int attention_from(const moe_paged_attention_args& r, int from) {
+  AttArgs a = {};
+  MOE_CHECK(check_attention(r, a.c));
+  if (a.c.seqs == 0) return MOE_OK;
+  a.q = r.q;
+  a.q_ss = r.q_seq_stride;
+  a.q_hs = r.q_head_stride;
+  a.seq_lens = r.seq_lens;
+  a.out = r.out;
+  a.lse = r.lse;
+  a.status = static_cast<int*>(r.workspace);
+  a.hq = r.q_heads;
+  a.window = r.window;
+  a.scale = r.scale;
+  a.cap = r.softcap;
+  a.from = from;
+  size_t need = 0;
+  MOE_CHECK(attention_workspace(a.c.head_dim, &a, r.workspace, &need));
+  MOE_REQUIRE(r.workspace_bytes >= need, MOE_ERR_WORKSPACE, "workspace %zu < %zu bytes",
+              r.workspace_bytes, need);
+  const int most = a.c.table_width * a.c.page_size;
+  const int longest = r.max_len > 0 && r.max_len < most ? r.max_len : most;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(r.stream);
+  {
+    ProfScope _prof(MOE_K_ATTENTION, s);
+    if (a.c.dtype == MOE_CACHE_F16)
+      MOE_CHECK((launch_attention_dt<MOE_CACHE_F16, false>(a, longest, s)));
+    else if (a.c.dtype == MOE_CACHE_E4M3)
+      MOE_CHECK((launch_attention_dt<MOE_CACHE_E4M3, false>(a, longest, s)));
+    else if (r.q_heads / a.c.kv_heads <= 4)
+      MOE_CHECK((launch_attention_dt<MOE_CACHE_BF16, true>(a, longest, s)));
+    else
+      MOE_CHECK((launch_attention_dt<MOE_CACHE_BF16, false>(a, longest, s)));
+  }
+  return check_launch("paged_attention");
+}
+
 }  // namespace moe
 
 extern "C" {
@@ -961,71 +1026,20 @@ int moe_paged_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int
   return moe::attention_workspace(head_dim, nullptr, nullptr, bytes);
 }
 
+int moe_paged_attention_record(const moe_paged_attention_args* a) {
+  MOE_REQUIRE(a, MOE_ERR_INVALID, "null arguments");
+  return moe::attention_from(*a, 0);
+}
+
 int moe_paged_attention(const moe_paged_cache* cache, const float* q, int64_t q_seq_stride,
                         int64_t q_head_stride, const int32_t* seq_lens, int q_heads, int max_len,
                         int window, float scale, float softcap, float* out, float* lse,
                         void* workspace, size_t workspace_bytes, moe_stream_t stream) {
-  moe::AttArgs a = {};
-  MOE_CHECK(moe::take_cache(cache, a.c));
-  MOE_REQUIRE(q_heads > 0 && q_heads % cache->kv_heads == 0, MOE_ERR_INVALID,
-              "%d query heads for %d key heads", q_heads, cache->kv_heads);
-  MOE_REQUIRE(max_len >= 0 && window >= 0, MOE_ERR_INVALID, "negative length or window");
-  MOE_REQUIRE(isfinite(scale) && isfinite(softcap) && softcap >= 0.f, MOE_ERR_INVALID,
-              "scale and softcap must be finite, softcap >= 0");
-  if (cache->seqs == 0) return MOE_OK;
-  MOE_REQUIRE(q && seq_lens && out && workspace, MOE_ERR_INVALID, "null pointer");
-  // parts in it are fetched by bulk copies
-  MOE_REQUIRE((uintptr_t)workspace % 16 == 0, MOE_ERR_INVALID, "workspace must be 16-byte aligned");
-  {
-    // A unit's rows of out are written behind the last read of its rows of q, so out
-    // may be q itself, but over other rows it would be read when it is written already.
-    const int64_t S = a.c.seqs, d = a.c.head_dim, n = S * q_heads * d;
-    const bool same = (uintptr_t)out == (uintptr_t)q && (S == 1 || q_seq_stride == q_heads * d) &&
-                      (q_heads == 1 || q_head_stride == d);
-    const int64_t ss = (S - 1) * q_seq_stride, hs = (q_heads - 1) * q_head_stride;
-    const int64_t from = std::min<int64_t>(ss, 0) + std::min<int64_t>(hs, 0);
-    const int64_t to = std::max<int64_t>(ss, 0) + std::max<int64_t>(hs, 0) + d;
-    const int64_t at = (int64_t)((uintptr_t)out - (uintptr_t)q);         // bytes
-    MOE_REQUIRE(same || at >= 4 * to || at + 4 * n <= 4 * from, MOE_ERR_INVALID,
-                "q and out overlap, and are not the same rows");
-  }
-  a.q = q;
-  a.q_ss = q_seq_stride;
-  a.q_hs = q_head_stride;
-  a.seq_lens = seq_lens;
-  a.out = out;
-  a.lse = lse;
-  a.status = static_cast<int*>(workspace);
-  a.hq = q_heads;
-  a.window = window;
-  a.scale = scale;
-  a.cap = softcap;
-  size_t need = 0;
-  MOE_CHECK(moe::attention_workspace(cache->head_dim, &a, workspace, &need));
-  MOE_REQUIRE(workspace_bytes >= need, MOE_ERR_WORKSPACE, "workspace %zu < %zu bytes",
-              workspace_bytes, need);
-  const int most = cache->table_width * cache->page_size;
-  const int longest = max_len > 0 && max_len < most ? max_len : most;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  {
-    ::moe::ProfScope _prof(MOE_K_ATTENTION, s);
-    if (cache->dtype == MOE_CACHE_F16)
-      MOE_CHECK((moe::launch_attention_dt<MOE_CACHE_F16, false>(a, longest, s)));
-    else if (cache->dtype == MOE_CACHE_E4M3)
-      MOE_CHECK((moe::launch_attention_dt<MOE_CACHE_E4M3, false>(a, longest, s)));
-    else if (q_heads / cache->kv_heads <= 4)
-      MOE_CHECK((moe::launch_attention_dt<MOE_CACHE_BF16, true>(a, longest, s)));
-    else
-      MOE_CHECK((moe::launch_attention_dt<MOE_CACHE_BF16, false>(a, longest, s)));
-  }
-  return moe::check_launch("paged_attention");
-}
-
-int moe_paged_attention_record(const moe_paged_attention_args* a) {
-  MOE_REQUIRE(a, MOE_ERR_INVALID, "null arguments");
-  return moe_paged_attention(&a->cache, a->q, a->q_seq_stride, a->q_head_stride, a->seq_lens,
-                             a->q_heads, a->max_len, a->window, a->scale, a->softcap, a->out,
-                             a->lse, a->workspace, a->workspace_bytes, a->stream);
+  MOE_REQUIRE(cache, MOE_ERR_INVALID, "null cache");
+  const moe_paged_attention_args a = {*cache, q, q_seq_stride, q_head_stride, seq_lens, out, lse,
+                                      workspace, workspace_bytes, stream, q_heads, max_len, window,
+                                      scale, softcap};
+  return moe::attention_from(a, 0);
 }
 
 }  // extern "C"

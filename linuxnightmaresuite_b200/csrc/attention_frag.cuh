@@ -1,6 +1,8 @@
-// Operands of the mma.sync products that the attention kernels share: query heads
-// as the 16 rows of M, split into 16-bit parts, keys as N.
+// What the attention kernels share: the cache as a tensor for TMA, operands split into
+// 16-bit parts, and the mma.sync products with query heads as the 16 rows of M and keys as N.
 #pragma once
+
+#include <cuda.h>
 
 #include "paged_cache.cuh"
 
@@ -9,6 +11,17 @@ namespace moe {
 constexpr int kAttHeads = 8;          // query heads of a unit at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kPShift = 7.f;        // probabilities enter sums and products times 2^7
+constexpr int kLine = 128;            // bytes of a row in one TMA box
+
+// A cache as the rows of a tensor map: row page * page_units + head * head_units, boxes of
+// 2^box_shift tokens.
+struct CacheMap {
+  int page_units, head_units, box_shift;
+};
+int make_cache_map(CUtensorMap* map, const moe_paged_cache& c, void* base, int keys, CacheMap* at);
+int check_attention(const moe_paged_attention_args& r, moe_paged_cache& c);
+int attention_from(const moe_paged_attention_args& r, int from);
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"

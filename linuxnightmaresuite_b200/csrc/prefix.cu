@@ -1,0 +1,936 @@
+// Attention of one new token per sequence where all sequences begin with the same pages.
+//
+//   out_s = (sum_{j < P} e^{s_j} v_j + sum_{P <= j < len} e^{s_j} v_j) / (sum of the e^{s_j})
+//
+// The first sums are over the same keys for every sequence: R = seqs x (query heads of a
+// key head) rows meet each key at one reading, which makes them matrix products for the
+// 5th-generation tensor cores.  The second ones are the paged attention's (attention.cu) from key P
+// on.  A last kernel joins both: every part is (maximum, sum, values) of a softmax.
+//
+// The prefix kernel.  M = 128 rows of one key head, N = KT keys:
+//   S = Q K^T   tcgen05.mma, Q and K in shared memory (K-major), S in tensor memory
+//   P = exp(S - m), split in two 16-bit parts, written over S
+//   O = P V     tcgen05.mma, P from tensor memory, V in shared memory as TMA left it (MN-major)
+// q's rows are f32.  They enter as hi + lo fp16 (22 bits; 24 in three bf16 parts for bf16 caches,
+// since a score's error is multiplied by its exponential), P as two parts (22 bits; 16 for bf16,
+// where V has 8, which is an error of 2^-17 of a probability whatever its size).  The tensor
+// core truncates where it adds, so the low parts go first, an O takes one tile of
+// keys, and sums over tiles are f32 adds in registers.
+//
+// Roles: two warpgroups take every other tile each, with a maximum, sum and O of their own
+// (they meet at the end of a piece): while one is at its exponentials the tensor cores
+// serve the other.  One thread issues the products, in the order S(i), O(i - 1), so that a
+// tile's exponentials have the time of a whole tile's products; one warp loads pages by TMA, two
+// tiles ahead.  e4m3 keys and values are widened to fp16 (exact) by four more warps.  At
+// 256 columns a CTA makes 128 columns of O: two CTAs form the same scores.
+//
+// Work.  A key head has RU row units (128 rows, or half of their columns).  m of them
+// (all, up to 16) are a team: CTAs that take the same keys at the same time, so that the
+// pages come from memory once, for one CTA of a team, and from L2 for the others.  Teams get equal
+// runs of tiles, across heads; a run that crosses into the next head writes two parts.
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+#include "attention_frag.cuh"
+#include "tc_common.cuh"
+
+namespace moe {
+
+constexpr int kPrefixRows = 128;
+constexpr int kTeamMost = 16;
+
+struct PrefixArgs {
+  moe_paged_cache c;                   // its block table is not used here
+  CacheMap map;
+  const float* q;
+  int64_t q_ss, q_hs;
+  const int32_t* pages;
+  int* status;
+  float2* part_ml;                     // [slot][row] (maximum in powers of two, sum)
+  float* part_o;                       // [slot][row][column of the unit]
+  int hq, G, rows, keys;               // rows of a key head, keys of the prefix
+  int RU, m, RG, tiles, quota, parts;  // row units, team, row groups; tiles of a head; parts of a unit
+  long long total;                     // tiles of all teams
+  float scale, cap;
+  int vec;                             // rows of q by 16 bytes
+};
+
+template <int DT, int DQ> struct PrefixCfg {
+  static constexpr bool kBf = DT == MOE_CACHE_BF16, kE4 = DT == MOE_CACHE_E4M3;
+  static constexpr int kParts = kBf ? 3 : 2;
+  // bf16 rows of 256: the third part is an operand in tensor memory, there is no room for
+  // it beside the others
+  static constexpr bool kTmemQ = kBf && DQ == 256;
+  static constexpr int kSmemParts = kTmemQ ? 2 : kParts;
+  static constexpr int kDV = DQ < 128 ? DQ : 128;
+  static constexpr int kHalves = DQ / kDV;
+  static constexpr int kKT = DQ == 256 ? 64 : 128;
+  static constexpr int kQPart = DQ / 64 * kPrefixRows * 128;
+  static constexpr int kQ = kSmemParts * kQPart;
+  static constexpr int kK = kKT * DQ * 2, kV = kKT * kDV * 2;
+  static constexpr int kStages = kE4 && DQ == 256 ? 1 : DQ == 64 ? 3 : 2;
+  static constexpr int kRawK = kE4 ? kKT * (DQ < 128 ? 128 : DQ) : 0, kRawV = kE4 ? kKT * 128 : 0;
+  static constexpr int kRawStages = kE4 ? (DQ == 128 ? 1 : 2) : 0;
+  static constexpr int kSmem = 1024 + kQ + kStages * (kK + kV) + kRawStages * (kRawK + kRawV);
+  static constexpr int kThreads = kE4 ? 512 : 384;
+  // registers of a thread by warpgroup: what the block was launched with, dealt out again
+  static constexpr int kRegsSoft = kE4 ? 192 : 224, kRegsIssue = kE4 ? 48 : 56, kRegsWiden = 80;
+  static_assert(2 * kRegsSoft + kRegsIssue + (kE4 ? kRegsWiden : 0) <=
+                    65536 / kThreads / 8 * 8 * (kThreads / 128),
+                "");
+  // tensor memory: S (P over it) and O of each warpgroup, then q's third part
+  static constexpr int kSlab = kKT + kDV;
+  static constexpr int kQCol = 2 * kSlab;
+  static_assert(kQCol + (kTmemQ ? DQ / 2 : 0) <= kTmemCols, "");
+  static constexpr uint32_t kIdesc16 = (kBf ? (1u << 7) | (1u << 10) : 0u);
+};
+
+struct PrefixShared {
+  uint64_t q_full, k_full[3], k_empty[3], v_full[3], v_empty[3];
+  uint64_t rk_full[2], rk_empty[2], rv_full[2], rv_empty[2];
+  uint64_t s_full[2], p_full[2], o_full[2], drain;
+  uint32_t tmem;
+  int dead;
+  uint32_t raw_seen[2][4], seen[3][4], soft_seen[2][4];
+  float qscale[kPrefixRows];
+  int qexp[kPrefixRows];
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st2(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(a), "r"(b)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld2(uint32_t addr, float& a, float& b) {
+  uint32_t r0, r1;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];"
+               : "=r"(r0), "=r"(r1)
+               : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  a = __uint_as_float(r0);
+  b = __uint_as_float(r1);
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// D (tensor memory) += A (tensor memory) B (shared memory)
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %5, 0;\n mov.b64 db, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// A CTA's pieces: tiles t0 .. t0 + n of row unit `unit` of a head, part j of its parts.
+struct PrefixPiece {
+  int head, ru, t0, n, slot;
+};
+struct PrefixRun {
+  const PrefixArgs& A;
+  long long at, end;
+  int team, member;
+  __device__ explicit PrefixRun(const PrefixArgs& a) : A(a) {
+    team = blockIdx.x / A.m;
+    member = blockIdx.x - team * A.m;
+    at = (long long)team * A.quota;
+    end = min(A.total, at + A.quota);
+  }
+  __device__ bool next(PrefixPiece& p) {
+    while (at < end) {
+      const int unit = (int)(at / A.tiles);            // head and row group
+      p.t0 = (int)(at - (long long)unit * A.tiles);
+      p.n = (int)min((long long)(A.tiles - p.t0), end - at);
+      at += p.n;
+      p.head = unit / A.RG;
+      p.ru = (unit - p.head * A.RG) * A.m + member;
+      const int first = (int)((long long)unit * A.tiles / A.quota);
+      p.slot = (unit * A.m + member) * A.parts + team - first;
+      if (p.ru < A.RU) return true;
+    }
+    return false;
+  }
+};
+
+template <int DT, int DQ>
+__global__ void __launch_bounds__(PrefixCfg<DT, DQ>::kThreads, 1)
+prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+              const PrefixArgs A) {
+  using Cfg = PrefixCfg<DT, DQ>;
+  constexpr bool BF = Cfg::kBf, E4 = Cfg::kE4;
+  constexpr int KT = Cfg::kKT, DV = Cfg::kDV, NS = Cfg::kStages, RS = Cfg::kRawStages;
+  constexpr int BLK = KT * 128;        // a block of 64 columns of a key or value tile
+  extern __shared__ uint8_t prefix_smem[];
+  __shared__ PrefixShared sh;
+  uint8_t* const smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(prefix_smem) + 1023) & ~(uintptr_t)1023);
+  uint8_t* const ks = smem + Cfg::kQ;
+  uint8_t* const vs = ks + NS * Cfg::kK;
+  uint8_t* const rk = vs + NS * Cfg::kV;
+  uint8_t* const rv = rk + RS * Cfg::kRawK;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(&sh.q_full, 8);
+    mbar_init(&sh.drain, 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&sh.k_full[i], E4 ? 4 : 1);
+      mbar_init(&sh.v_full[i], E4 ? 4 : 1);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.rk_full[i], 1);
+      mbar_init(&sh.rv_full[i], 1);
+      mbar_init(&sh.rk_empty[i], 4);
+      mbar_init(&sh.rv_empty[i], 4);
+      mbar_init(&sh.s_full[i], 2);
+      mbar_init(&sh.p_full[i], 128);
+      mbar_init(&sh.o_full[i], 1);
+    }
+    sh.dead = 0;
+    fence_mbar_init();
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
+  }
+  const uint32_t tmem = tc_alloc_all(&sh.tmem, warp);
+  pdl_trigger();
+  pdl_wait();
+
+  // Bounded; after a timeout anywhere in the CTA no wait takes long any more, nothing more
+  // is issued, and the kernel ends.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!mbar_test(bar, parity) && !*(volatile int*)&sh.dead && !mbar_wait(bar, parity)) {
+      *(volatile int*)&sh.dead = 1;
+      set_status(A.status, MOE_STATUS_TIMEOUT);
+    }
+    __syncwarp();
+  };
+  PrefixRun run(A);
+  PrefixPiece p;
+  int n = 0;                           // tiles so far: warpgroup n & 1, its use n >> 1
+
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSoft));
+    const int w = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t S = tmem + lanes + (uint32_t)(w * Cfg::kSlab), O = S + KT;
+    const uint32_t other = tmem + lanes + (uint32_t)((w ^ 1) * Cfg::kSlab) + KT;
+    while (run.next(p)) {
+      const int r0 = p.ru / Cfg::kHalves * kPrefixRows;
+      // ---- q: a warp takes 16 rows, each scaled by a power of two to [2^10, 2^11)
+      constexpr int PER = DQ / 32;     // values of a lane: 4 lane + 128 i .. (2 lane + for 64)
+      constexpr int VW = PER < 4 ? PER : 4;
+#pragma unroll 1
+      for (int b = 0; b < 16; b += 8) {
+        float v[8][PER];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = warp * 16 + b + j, at = r0 + r, s = at / A.G;
+          const float* q = A.q + s * A.q_ss + (p.head * A.G + at - s * A.G) * A.q_hs;
+          const bool in = at < A.rows;
+#pragma unroll
+          for (int i = 0; i < PER; i += VW) {
+            const int e = VW * lane + 32 * i;
+            if (VW == 4 && A.vec) {
+              const float4 f = in && e < A.c.head_dim ? *reinterpret_cast<const float4*>(q + e)
+                                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+              v[j][i] = f.x;
+              v[j][i + 1] = f.y;
+              v[j][i + 2 < PER ? i + 2 : 0] = f.z;
+              v[j][i + 3 < PER ? i + 3 : 0] = f.w;
+            } else {
+#pragma unroll
+              for (int k = 0; k < VW; ++k)
+                v[j][i + k] = in && e + k < A.c.head_dim ? q[e + k] : 0.f;
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = warp * 16 + b + j;
+          float mx = 0.f;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) mx = fmaxf(mx, fabsf(v[j][i]));
+          mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+          const int ex = (int)(__float_as_uint(mx) >> 23);
+          const int e = mx > 0.f && ex < 255 ? 137 - max(ex, 1) : 0;
+          const int e1 = e / 2, e2 = e - e1;     // 2^e may lie outside the exponents of a float
+          const float f1 = copysignf(__uint_as_float((uint32_t)(127 + e1) << 23), A.scale);
+          const float f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
+          if (lane == 0) {
+            sh.qscale[r] = fmaxf(ldexpf(fabsf(A.scale) * A.c.k_scale, -e), 1e-30f);
+            sh.qexp[r] = e;
+          }
+#pragma unroll
+          for (int i = 0; i < PER; i += VW) {
+            const int c = VW * lane + 32 * i;
+            uint8_t* to = smem + (c >> 6) * (kPrefixRows * 128) + r * 128 +
+                          ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2;
+            uint32_t lo[Cfg::kParts], hi[Cfg::kParts];
+            split2<BF, Cfg::kParts>(v[j][i] * f1 * f2, v[j][i + 1] * f1 * f2, lo);
+            if (VW == 4)
+              split2<BF, Cfg::kParts>(v[j][i + 2 < PER ? i + 2 : 0] * f1 * f2,
+                                      v[j][i + 3 < PER ? i + 3 : 0] * f1 * f2, hi);
+#pragma unroll
+            for (int k = 0; k < Cfg::kSmemParts; ++k) {
+              if (VW == 4)
+                *reinterpret_cast<uint2*>(to + k * Cfg::kQPart) = make_uint2(lo[k], hi[k]);
+              else
+                *reinterpret_cast<uint32_t*>(to + k * Cfg::kQPart) = lo[k];
+            }
+          }
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");       // qscale
+      if (Cfg::kTmemQ) {               // third parts: this thread's row, half of its columns
+        const int at = r0 + row, s = at / A.G;
+        const float* q = A.q + s * A.q_ss + (p.head * A.G + at - s * A.G) * A.q_hs;
+        const int e1 = sh.qexp[row] / 2, e2 = sh.qexp[row] - e1;
+        const float f1 = copysignf(__uint_as_float((uint32_t)(127 + e1) << 23), A.scale);
+        const float f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
+#pragma unroll 1
+        for (int c = 0; c < DQ / 2; c += 64) {
+          uint32_t x[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int e = w * (DQ / 2) + c + 2 * i;
+            uint32_t part[3];
+            const bool in = at < A.rows && e < A.c.head_dim;
+            split2<true, 3>(in ? q[e] * f1 * f2 : 0.f, in ? q[e + 1] * f1 * f2 : 0.f, part);
+            x[i] = part[2];
+          }
+          tmem_st32(tmem + lanes + Cfg::kQCol + (w * (DQ / 2) + c) / 2, x);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full);
+
+      const float qscale = sh.qscale[row];
+      const float to_cap = A.cap > 0.f ? fminf(qscale / A.cap, 3e38f) : 0.f;
+      const float from_cap = A.cap * kLog2e;
+      const float x2 = A.cap > 0.f ? 1.f : qscale * kLog2e;
+      float o[DV], m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int c = 0; c < DV; ++c) o[c] = 0.f;
+      for (int i = 0; i < p.n; ++i, ++n) {
+        if ((n & 1) != w) continue;
+        const uint32_t phase = (n >> 1) & 1;
+        wait(&sh.s_full[w], phase);
+        tc_fence_after();
+        uint32_t seen[KT / 32], all = 0xffffffffu;
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) {
+          seen[c] = sh.soft_seen[w][c];
+          all &= seen[c];
+        }
+        // ---- the largest score
+        float mx = -INFINITY, mn = INFINITY;
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) {
+          float v[32];
+          tmem_ld32(S + 32 * c, v);
+          if (all != 0xffffffffu)
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!((seen[c] >> k) & 1u)) v[k] = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) mx = fmaxf(mx, v[k]);
+          if (A.cap > 0.f)
+#pragma unroll
+            for (int k = 0; k < 32; ++k) mn = fminf(mn, (seen[c] >> k) & 1u ? v[k] : 0.f);
+        }
+        bool steep = false;            // some score is not small against the cap
+        if (A.cap > 0.f) {
+          steep = __any_sync(0xffffffffu, !(fmaxf(mx, -mn) * to_cap < 0.5f));
+          mx = mx == -INFINITY ? mx : from_cap * tanhf(mx * to_cap);
+        } else {
+          mx *= x2;
+        }
+        if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+          const float to = mx > m + 8.f ? mx : m;
+          const float f = to == -INFINITY ? 1.f : ex2(m - to);
+#pragma unroll
+          for (int c = 0; c < DV; ++c) o[c] *= f;
+          l *= f;
+          m = to;
+        }
+        const float shift = kPShift - (m == -INFINITY ? 0.f : m);
+        // ---- probabilities: 32 keys' hi parts in 16 columns, then their lo parts
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) {
+          float v[32];
+          uint32_t x[32];
+          tmem_ld32(S + 32 * c, v);
+          if (A.cap > 0.f) {
+            if (steep) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] = from_cap * tanhf(v[k] * to_cap);
+            } else {
+              // Lambert's continued fraction, off by less than 2^-29 of tanh y for |y| < 1/2
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const float y = v[k] * to_cap, z = y * y;
+                const float num = fmaf(z, z + 105.f, 945.f);
+                const float den = fmaf(z, fmaf(15.f, z, 420.f), 945.f);
+                v[k] = from_cap * __fdividef(y * num, den);
+              }
+            }
+          }
+          if (all != 0xffffffffu)
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!((seen[c] >> k) & 1u)) v[k] = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const float a = ex2(fmaf(v[k], x2, shift)), b = ex2(fmaf(v[k + 1], x2, shift));
+            sum[k & 2] += a;
+            sum[(k & 2) + 1] += b;
+            uint32_t part[2];
+            split2<BF, 2>(a, b, part);
+            x[k / 2] = part[0];
+            x[16 + k / 2] = part[1];
+          }
+          tmem_st32(S + 32 * c, x);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&sh.p_full[w]);
+        // ---- this tile's O
+        wait(&sh.o_full[w], phase);
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < DV / 32; ++c) {
+          float v[32];
+          tmem_ld32(O + 32 * c, v);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[32 * c + k] += v[k];
+        }
+        tc_fence_before();
+      }
+      // ---- both warpgroups' parts: each hands over half of its columns through its O
+      constexpr int H = DV / 2;
+      tmem_st2(O + H, __float_as_uint(m), __float_as_uint(l));
+#pragma unroll
+      for (int c = 0; c < H; c += 32) {
+        uint32_t x[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(w ? o[c + k] : o[H + c + k]);
+        tmem_st32(O + c, x);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      tc_fence_after();
+      float m1, l1;
+      tmem_ld2(other + H, m1, l1);
+      const float M = fmaxf(m, m1), ms = M == -INFINITY ? 0.f : M;
+      const float f0 = ex2(m - ms), f1 = ex2(m1 - ms);
+      const bool in = r0 + row < A.rows;
+      if (in && w == 0)
+        A.part_ml[(int64_t)p.slot * kPrefixRows + row] =
+            make_float2(M, l * f0 + l1 * f1);
+      float* to = A.part_o + ((int64_t)p.slot * kPrefixRows + row) * DV + w * H;
+#pragma unroll
+      for (int c = 0; c < H; c += 32) {
+        float v[32];
+        tmem_ld32(other + c, v);
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          float4 y;
+          y.x = (w ? o[H + c + k] : o[c + k]) * f0 + v[k] * f1;
+          y.y = (w ? o[H + c + k + 1] : o[c + k + 1]) * f0 + v[k + 1] * f1;
+          y.z = (w ? o[H + c + k + 2] : o[c + k + 2]) * f0 + v[k + 2] * f1;
+          y.w = (w ? o[H + c + k + 3] : o[c + k + 3]) * f0 + v[k + 3] * f1;
+          if (in) *reinterpret_cast<float4*>(to + c + k) = y;
+        }
+      }
+      tc_fence_before();
+      asm volatile("bar.sync 1, 256;" ::: "memory");       // O, m, l and q are free
+      tc_fence_after();
+    }
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsIssue));
+    if (warp == 8) {
+      // ---- products
+      const uint64_t dk = sw128_desc(ks), dq = sw128_desc(smem);
+      const uint32_t desc_hi = (uint32_t)(dk >> 32), q_lo = (uint32_t)dq, k_lo = (uint32_t)dk;
+      // V: 64 columns in a line of 128 bytes, 8 keys 1024 bytes on, 64 columns BLK on
+      const uint32_t v_lo = ((smem_u32(vs) >> 4) & 0x3FFF) | (uint32_t)(BLK >> 4) << 16;
+      const uint32_t is = tc_idesc(128, KT) | Cfg::kIdesc16;
+      const uint32_t io = tc_idesc(128, DV) | Cfg::kIdesc16 | (1u << 16);
+      uint32_t pieces = 0;
+      while (run.next(p)) {
+        wait(&sh.q_full, pieces & 1);
+        ++pieces;
+        tc_fence_after();
+        for (int i = 0; i <= p.n; ++i) {
+          if (i < p.n) {               // S of tile n + i
+            const int t = n + i, st = t % NS, w = t & 1;
+            wait(&sh.k_full[st], (t / NS) & 1);
+            if (lane < 4) sh.soft_seen[w][lane] = sh.seen[st][lane];
+            __syncwarp();
+            if (lane == 0 && !*(volatile int*)&sh.dead) {
+              tc_fence_after();
+              const uint32_t d = tmem + (uint32_t)(w * Cfg::kSlab);
+              const uint32_t kb = k_lo + (uint32_t)(st * Cfg::kK >> 4);
+              bool first = true;
+              for (int k = Cfg::kParts - 1; k >= 0; --k) {
+#pragma unroll
+                for (int c = 0; c < DQ / 16; ++c) {
+                  const uint32_t b = kb + (uint32_t)(((c >> 2) * BLK + (c & 3) * 32) >> 4);
+                  if (Cfg::kTmemQ && k == 2) {
+                    tc_mma_ts(d, tmem + Cfg::kQCol + 8 * c, b, desc_hi, is, first ? 0u : 1u);
+                  } else {
+                    const uint32_t a = q_lo + (uint32_t)((k * Cfg::kQPart + (c >> 2) * kPrefixRows * 128 +
+                                                          (c & 3) * 32) >> 4);
+                    tc_mma_lo(d, a, b, desc_hi, is, first ? 0u : 1u);
+                  }
+                  first = false;
+                }
+              }
+              tc_commit(&sh.k_empty[st]);
+              mbar_arrive(&sh.s_full[w]);
+              tc_commit(&sh.s_full[w]);
+            }
+            __syncwarp();
+          }
+          if (i > 0) {                 // O of the tile before
+            const int t = n + i - 1, st = t % NS, w = t & 1;
+            wait(&sh.v_full[st], (t / NS) & 1);
+            uint32_t all = 0xffffffffu;
+#pragma unroll
+            for (int c = 0; c < KT / 32; ++c) all &= sh.soft_seen[w][c];
+            if (all != 0xffffffffu) {  // nothing of a row that is not seen counts
+              for (int r = lane; r < KT; r += 32)
+                if (!((sh.soft_seen[w][r >> 5] >> (r & 31)) & 1u))
+                  for (int c = 0; c < DV / 64 * 8; ++c)
+                    *reinterpret_cast<uint4*>(vs + st * Cfg::kV + (c >> 3) * BLK + r * 128 +
+                                              (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
+            }
+            wait(&sh.p_full[w], (t >> 1) & 1);
+            __syncwarp();
+            if (lane == 0 && !*(volatile int*)&sh.dead) {
+              tc_fence_after();
+              const uint32_t a = tmem + (uint32_t)(w * Cfg::kSlab), d = a + KT;
+              const uint32_t vb = v_lo + (uint32_t)(st * Cfg::kV >> 4);
+#pragma unroll
+              for (int k = 1; k >= 0; --k)
+#pragma unroll
+                for (int c = 0; c < KT / 16; ++c)
+                  tc_mma_ts(d, a + 32 * (c >> 1) + 16 * k + 8 * (c & 1), vb + (uint32_t)(c * 2048 >> 4),
+                            desc_hi, io, k == 1 && c == 0 ? 0u : 1u);
+              tc_commit(&sh.v_empty[st]);
+              tc_commit(&sh.o_full[w]);
+            }
+            __syncwarp();
+          }
+        }
+        n += p.n;
+      }
+      if (lane == 0) {                 // nothing is in flight when the tensor memory goes
+        tc_commit(&sh.drain);
+        mbar_wait(&sh.drain, 0);
+      }
+    } else if (warp == 9) {
+      // ---- loads
+      constexpr int EB = E4 ? 1 : 2, LINE = 128 / EB;          // elements of a line
+      constexpr int RING = E4 ? (RS ? RS : 1) : NS;
+      uint64_t* kf = E4 ? sh.rk_full : sh.k_full;
+      uint64_t* vf = E4 ? sh.rv_full : sh.v_full;
+      uint64_t* ke = E4 ? sh.rk_empty : sh.k_empty;
+      uint64_t* ve = E4 ? sh.rv_empty : sh.v_empty;
+      uint8_t* kt = E4 ? rk : ks;
+      uint8_t* vt = E4 ? rv : vs;
+      constexpr int KB = E4 ? Cfg::kRawK : Cfg::kK, VB = E4 ? Cfg::kRawV : Cfg::kV;
+      const int ps = A.c.page_size, shift = A.map.box_shift, boxes = KT >> shift;
+      while (run.next(p)) {
+        const int x0 = p.ru % Cfg::kHalves * 128;              // this unit's columns of V
+        for (int i = 0; i < p.n; ++i, ++n) {
+          const int st = n % RING;
+          const uint32_t round = n / RING, key0 = (uint32_t)(p.t0 + i) * KT;
+          // this lane's boxes: lane, lane + 32, ...
+          int row[4], slot[4];
+          uint32_t ok[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int box = lane + 32 * b;
+            const uint32_t key = key0 + ((uint32_t)box << shift);
+            row[b] = -1;
+            slot[b] = 0;
+            if (box < boxes && key < (uint32_t)A.keys) {
+              const uint32_t pg = key / (uint32_t)ps;
+              const int page = A.pages[pg];
+              if (page >= 0 && page < A.c.pages) {
+                row[b] = page * A.map.page_units + p.head * A.map.head_units;
+                slot[b] = (int)(key - pg * ps);
+              } else {
+                set_status(A.status, MOE_STATUS_BAD_PAGE);
+              }
+            }
+            ok[b] = __ballot_sync(0xffffffffu, row[b] >= 0);
+          }
+          // keys of the tile that are there
+          uint32_t* seen = E4 ? sh.raw_seen[st] : sh.seen[st];
+          const uint32_t count = __popc(ok[0]) + __popc(ok[1]) + __popc(ok[2]) + __popc(ok[3]);
+          if (round > 0) wait(&ke[st], (round - 1) & 1);
+          if (lane < 4) {
+            uint32_t bits = 0;
+            for (int k = 0; k < 32; ++k) {
+              const int box = (32 * lane + k) >> shift;
+              const uint32_t word = box < 32 ? ok[0] : box < 64 ? ok[1] : box < 96 ? ok[2] : ok[3];
+              bits |= ((word >> (box & 31)) & 1u) << k;
+            }
+            seen[lane] = 32 * lane < KT ? bits : 0xffffffffu;
+          }
+          __syncwarp();
+          const bool go = !*(volatile int*)&sh.dead;
+          auto copy = [&](const CUtensorMap* map, uint8_t* to, uint64_t* bar, int bytes, int x) {
+            const int lines = bytes / BLK;
+            if (lane == 0) mbar_expect_tx(bar, (count << shift) * 128u * (uint32_t)lines);
+            __syncwarp();
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              if (row[b] >= 0)
+                for (int c = 0; c < lines; ++c)
+                  tma_load_3d(smem_u32(to) + c * BLK + ((lane + 32 * b) << shift) * 128, map,
+                              x + c * LINE, row[b], slot[b], bar);
+          };
+          if (__any_sync(0xffffffffu, !go)) break;
+          copy(&kmap, kt + st * KB, &kf[st], KB, 0);
+          if (round > 0) wait(&ve[st], (round - 1) & 1);
+          if (__any_sync(0xffffffffu, *(volatile int*)&sh.dead)) break;
+          copy(&vmap, vt + st * VB, &vf[st], VB, x0);
+        }
+      }
+      // after a timeout copies may still be under way: give them time to land
+      if (*(volatile int*)&sh.dead)
+        for (int s = 0; s < RING; ++s)
+          for (int k = 0; k < 2; ++k) {
+            mbar_wait(&kf[s], k);
+            mbar_wait(&vf[s], k);
+          }
+    }
+  } else if (E4) {
+    // ---- e4m3 -> fp16, rows of 128 bytes swizzled on both sides
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsWiden));
+    constexpr int R = RS ? RS : 1;
+    const int id = tid - 384;
+    auto widen = [&](const uint8_t* from, uint8_t* to, int columns) {
+      constexpr int SHARE = 128 / KT;  // threads of a row
+      const int r = id % KT, c0 = id / KT;
+      for (int c = c0; c < columns / 16; c += SHARE) {
+        const uint4 v = *reinterpret_cast<const uint4*>(from + (c >> 3) * BLK + r * 128 +
+                                                        (((c & 7) ^ (r & 7)) << 4));
+        uint4 a, b;
+        e4m3x4_f16x2(v.x, a.x, a.y);
+        e4m3x4_f16x2(v.y, a.z, a.w);
+        e4m3x4_f16x2(v.z, b.x, b.y);
+        e4m3x4_f16x2(v.w, b.z, b.w);
+        uint8_t* row = to + (c >> 2) * BLK + r * 128;
+        const int ch = 2 * (c & 3);
+        *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) = a;
+        *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = b;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    while (run.next(p)) {
+      for (int i = 0; i < p.n; ++i, ++n) {
+        const int rs = n % R, st = n % NS;
+        const uint32_t rr = (n / R) & 1, round = n / NS;
+        wait(&sh.rk_full[rs], rr);
+        if (round > 0) wait(&sh.k_empty[st], (round - 1) & 1);
+        widen(rk + rs * Cfg::kRawK, ks + st * Cfg::kK, DQ);
+        if (id < 4) sh.seen[st][id] = sh.raw_seen[rs][id];
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sh.k_full[st]);
+          mbar_arrive(&sh.rk_empty[rs]);
+        }
+        wait(&sh.rv_full[rs], rr);
+        if (round > 0) wait(&sh.v_empty[st], (round - 1) & 1);
+        widen(rv + rs * Cfg::kRawV, vs + st * Cfg::kV, DV);
+        if (lane == 0) {
+          mbar_arrive(&sh.v_full[st]);
+          mbar_arrive(&sh.rv_empty[rs]);
+        }
+        if (*(volatile int*)&sh.dead) break;
+      }
+    }
+  }
+  tc_dealloc_all(tmem, warp);
+}
+
+// ---------------------------------------------------------------------------
+// The join: a warp per row of the output.
+// ---------------------------------------------------------------------------
+struct PrefixJoinArgs {
+  const float2* part_ml;
+  const float* part_o;
+  const int32_t* seq_lens;
+  const float* own_lse;                // null: no key behind any prefix
+  float *out, *lse;
+  int* status;
+  int seqs, hq, G, d, DV, halves, keys;
+  int RU, m, RG, tiles, quota, parts;
+  float v_scale;
+};
+
+__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixJoinArgs A) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (id >= (int64_t)A.seqs * A.hq) return;
+  const int s = (int)(id / A.hq), h = (int)(id - (int64_t)s * A.hq), head = h / A.G;
+  const int len = A.seq_lens[s];
+  float* out = A.out + id * A.d;
+  if (len < A.keys) {                  // padding, or not behind this prefix
+    if (len > 0 && lane == 0) set_status(A.status, MOE_STATUS_BAD_PAGE);
+    for (int c = lane; c < A.d; c += 32) out[c] = 0.f;
+    if (lane == 0 && A.lse) A.lse[id] = -INFINITY;
+    return;
+  }
+  const int r = s * A.G + h - head * A.G;
+  const float own = A.own_lse[id] * kLog2e;
+  for (int half = 0; half < A.halves; ++half) {
+    const int ru = r / kPrefixRows * A.halves + half, row = r % kPrefixRows;
+    const int rg = ru / A.m, unit = head * A.RG + rg;
+    const int first = (int)((long long)unit * A.tiles / A.quota);
+    const int n = (int)(((long long)(unit + 1) * A.tiles - 1) / A.quota) - first + 1;
+    const int64_t slot = (int64_t)(unit * A.m + ru - rg * A.m) * A.parts;
+    const float2* ml = A.part_ml + slot * kPrefixRows + row;
+    const float* po = A.part_o + (slot * kPrefixRows + row) * A.DV;
+    float M = own;
+    for (int j = lane; j < n; j += 32) M = fmaxf(M, ml[(int64_t)j * kPrefixRows].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float ms = M == -INFINITY ? 0.f : M;
+    const float wo = ex2(own - ms);
+    const int c = 4 * lane, col = half * A.DV + c;
+    const bool mine = c < A.DV && col < A.d;
+    float L = wo;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (mine) {
+      const float4 v = *reinterpret_cast<const float4*>(out + col);
+      y = make_float4(v.x * wo, v.y * wo, v.z * wo, v.w * wo);
+    }
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const float2 p = ml[(int64_t)j * kPrefixRows];
+      const float w = ex2(p.x - ms - kPShift), wv = w * A.v_scale;
+      L = fmaf(p.y, w, L);
+      if (mine) {
+        const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)j * kPrefixRows * A.DV + c);
+        y.x = fmaf(v.x, wv, y.x);
+        y.y = fmaf(v.y, wv, y.y);
+        y.z = fmaf(v.z, wv, y.z);
+        y.w = fmaf(v.w, wv, y.w);
+      }
+    }
+    const float norm = L == 0.f ? 0.f : 1.f / L;
+    if (mine)
+      *reinterpret_cast<float4*>(out + col) =
+          make_float4(y.x * norm, y.y * norm, y.z * norm, y.w * norm);
+    if (half == 0 && lane == 0 && A.lse) A.lse[id] = (M + log2f(L)) * kLn2;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+struct PrefixPlan {
+  int dq, dv, halves, kt, RU, m, RG, teams;
+  int64_t units, slots;                // (head, row group)s, parts at most
+};
+
+static PrefixPlan prefix_plan(int seqs, int q_heads, int kv_heads, int head_dim) {
+  PrefixPlan p;
+  p.dq = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+  p.dv = std::min(p.dq, 128);
+  p.halves = p.dq / p.dv;
+  p.kt = p.dq == 256 ? 64 : 128;
+  const int64_t rows = (int64_t)std::max(seqs, 1) * (q_heads / kv_heads);
+  p.RU = (int)((rows + kPrefixRows - 1) / kPrefixRows) * p.halves;
+  p.RG = (p.RU + kTeamMost - 1) / kTeamMost;
+  p.m = (p.RU + p.RG - 1) / p.RG;
+  p.teams = std::max(1, sm_count() / p.m);
+  p.units = (int64_t)kv_heads * p.RG;
+  // a unit in (tiles - 1) / quota + 2 <= teams / units + 2 parts
+  p.slots = p.m * (p.teams + 2 * p.units);
+  return p;
+}
+
+struct PrefixSpace {
+  float* lse;
+  float2* ml;
+  float* o;
+  uint8_t* own;
+  size_t own_bytes;
+};
+
+static int prefix_workspace(const PrefixPlan& p, int seqs, int q_heads, int kv_heads, int head_dim,
+                            void* ws, PrefixSpace* out, size_t* bytes) {
+  Carve cv = {static_cast<uint8_t*>(ws), 0, 0};
+  size_t own = 0;                      // of the attention behind the prefix; it starts with the status
+  MOE_CHECK(moe_paged_attention_workspace_bytes(seqs, q_heads, kv_heads, head_dim, &own));
+  uint8_t* at = cv.take<uint8_t>(own);
+  float* lse = cv.take<float>((size_t)seqs * q_heads);
+  float2* ml = cv.take<float2>((size_t)p.slots * kPrefixRows);
+  float* o = cv.take<float>((size_t)p.slots * kPrefixRows * p.dv);
+  if (out) *out = {lse, ml, o, at, own};
+  *bytes = align_up(cv.used, 256);
+  return MOE_OK;
+}
+
+template <int DT, int DQ>
+static int launch_prefix(PrefixArgs& a, int grid, cudaStream_t s) {
+  using Cfg = PrefixCfg<DT, DQ>;
+  static std::atomic<uint64_t> ready{0};
+  auto kern = prefix_kernel<DT, DQ>;
+  int dev = 0;
+  MOE_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !((ready.load() >> dev) & 1)) {
+    MOE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+    // the warpgroups' shares come out of what the block is launched with
+    cudaFuncAttributes fa;
+    MOE_CUDA(cudaFuncGetAttributes(&fa, kern));
+    MOE_REQUIRE(fa.numRegs * (Cfg::kThreads / 128) >=
+                    2 * Cfg::kRegsSoft + Cfg::kRegsIssue + (Cfg::kE4 ? Cfg::kRegsWiden : 0),
+                MOE_ERR_CUDA, "the kernel was built with %d registers", fa.numRegs);
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  CUtensorMap kmap, vmap;
+  MOE_CHECK(make_cache_map(&kmap, a.c, a.c.k, Cfg::kKT, &a.map));
+  MOE_CHECK(make_cache_map(&vmap, a.c, a.c.v, Cfg::kKT, &a.map));
+  MOE_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(Cfg::kThreads), Cfg::kSmem, s, kmap, vmap, a));
+  return MOE_OK;
+}
+
+template <int DT>
+static int launch_prefix_dt(PrefixArgs& a, int dq, int grid, cudaStream_t s) {
+  return dq == 64    ? launch_prefix<DT, 64>(a, grid, s)
+         : dq == 128 ? launch_prefix<DT, 128>(a, grid, s)
+                     : launch_prefix<DT, 256>(a, grid, s);
+}
+
+}  // namespace moe
+
+extern "C" {
+
+int moe_prefix_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int head_dim,
+                                         size_t* bytes) {
+  MOE_REQUIRE(bytes, MOE_ERR_INVALID, "null output pointer");
+  MOE_REQUIRE(seqs >= 0 && kv_heads > 0 && head_dim > 0 && head_dim <= moe::kMaxHeadDim,
+              MOE_ERR_INVALID, "bad attention shape");
+  MOE_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0, MOE_ERR_INVALID,
+              "%d query heads for %d key heads", q_heads, kv_heads);
+  return moe::prefix_workspace(moe::prefix_plan(seqs, q_heads, kv_heads, head_dim), seqs, q_heads,
+                               kv_heads, head_dim, nullptr, nullptr, bytes);
+}
+
+int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
+  MOE_REQUIRE(r, MOE_ERR_INVALID, "null arguments");
+  const moe_paged_attention_args& t = r->attention;
+  moe::PrefixArgs a = {};
+  MOE_CHECK(moe::check_attention(t, a.c));
+  MOE_REQUIRE(r->prefix_pages >= 0 && r->prefix_pages <= a.c.table_width, MOE_ERR_INVALID,
+              "a prefix of %d pages in tables of %d", r->prefix_pages, a.c.table_width);
+  MOE_REQUIRE(t.window == 0, MOE_ERR_UNSUPPORTED, "a window does not go with a shared prefix");
+  if (a.c.seqs == 0) return MOE_OK;
+  MOE_REQUIRE(r->prefix || r->prefix_pages == 0, MOE_ERR_INVALID, "null pointer");
+  MOE_REQUIRE((uintptr_t)t.out % 16 == 0, MOE_ERR_INVALID, "out must be 16-byte aligned");
+  if (r->prefix_pages == 0) return moe::attention_from(t, 0);
+  const int S = a.c.seqs, d = a.c.head_dim, P = r->prefix_pages * a.c.page_size;
+  const moe::PrefixPlan p = moe::prefix_plan(S, t.q_heads, a.c.kv_heads, d);
+  moe::PrefixSpace ws;
+  size_t need = 0;
+  MOE_CHECK(moe::prefix_workspace(p, S, t.q_heads, a.c.kv_heads, d, t.workspace, &ws, &need));
+  MOE_REQUIRE(t.workspace_bytes >= need, MOE_ERR_WORKSPACE, "workspace %zu < %zu bytes",
+              t.workspace_bytes, need);
+  a.q = t.q;
+  a.q_ss = t.q_seq_stride;
+  a.q_hs = t.q_head_stride;
+  a.pages = r->prefix;
+  a.status = static_cast<int*>(t.workspace);
+  a.part_ml = ws.ml;
+  a.part_o = ws.o;
+  a.hq = t.q_heads;
+  a.G = t.q_heads / a.c.kv_heads;
+  a.rows = S * a.G;
+  a.keys = P;
+  a.RU = p.RU;
+  a.m = p.m;
+  a.RG = p.RG;
+  a.tiles = (P + p.kt - 1) / p.kt;
+  a.total = (long long)p.units * a.tiles;
+  const long long quota = (a.total + p.teams - 1) / p.teams;
+  MOE_REQUIRE(quota < (1ll << 30) && (int64_t)S * a.G < (1ll << 30) && p.slots < (1ll << 30),
+              MOE_ERR_UNSUPPORTED, "%d sequences behind a prefix of %d tokens are too many", S, P);
+  a.quota = (int)quota;
+  a.parts = (a.tiles - 1) / a.quota + 2;
+  MOE_REQUIRE(p.units * p.m * a.parts <= p.slots, MOE_ERR_INVALID, "parts %d", a.parts);
+  const int grid = (int)((a.total + quota - 1) / quota) * p.m;
+  a.scale = t.scale;
+  a.cap = t.softcap;
+  a.vec = (uintptr_t)t.q % 16 == 0 && (S == 1 || t.q_seq_stride % 4 == 0) &&
+          (t.q_heads == 1 || t.q_head_stride % 4 == 0);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(t.stream);
+  // the keys behind the prefix: checks q and out, and writes out
+  moe_paged_attention_args own = t;
+  own.lse = ws.lse;
+  own.workspace_bytes = ws.own_bytes;
+  {
+    ::moe::ProfScope _prof(MOE_K_PREFIX, s);
+    MOE_CHECK(a.c.dtype == MOE_CACHE_F16 ? moe::launch_prefix_dt<MOE_CACHE_F16>(a, p.dq, grid, s)
+              : a.c.dtype == MOE_CACHE_BF16
+                  ? moe::launch_prefix_dt<MOE_CACHE_BF16>(a, p.dq, grid, s)
+                  : moe::launch_prefix_dt<MOE_CACHE_E4M3>(a, p.dq, grid, s));
+  }
+  MOE_CHECK(moe::attention_from(own, P));
+  const moe::PrefixJoinArgs j = {ws.ml, ws.o, t.seq_lens, ws.lse, t.out, t.lse,
+                                 a.status, S, t.q_heads, a.G, d, p.dv, p.halves, P, a.RU, a.m, a.RG,
+                                 a.tiles, a.quota, a.parts, a.c.v_scale};
+  {
+    ::moe::ProfScope _prof(MOE_K_PREFIX, s);
+    const int64_t blocks = ((int64_t)S * t.q_heads + 7) / 8;
+    MOE_CUDA(moe::launch_pdl(moe::prefix_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, j));
+  }
+  return moe::check_launch("prefix_attention");
+}
+
+}  // extern "C"

@@ -300,9 +300,11 @@ _APPEND_ARGS = struct.Struct("@" + _CACHE + "3P6q4P2q2P4i0q")
 _ATTENTION_ARGS = struct.Struct("@" + _CACHE + "P2q4PNP3i2f0q")
 _LINEAR_ARGS = struct.Struct("@2PqPqPqP4i")
 _NORM_APPEND_ARGS = struct.Struct("@" + _CACHE + "3P6q4P2q2P4i5Pqfi0q")
+_PREFIX_ARGS = struct.Struct("@" + _CACHE + "P2q4PNP3i2f0qPi0q")
 _MASS_ARGS = struct.Struct("@" + _CACHE + "P2q4Pq2P3i2f0q")
 _EVICT_ARGS = struct.Struct("@" + _CACHE + "6P2q2P3i0q")
 assert _NORM_APPEND_ARGS.size == ctypes.sizeof(_lib.MoENormAppendArgs)
+assert _PREFIX_ARGS.size == ctypes.sizeof(_lib.MoEPrefixAttentionArgs)
 assert _MASS_ARGS.size == ctypes.sizeof(_lib.MoEAttentionMassArgs)
 assert _EVICT_ARGS.size == ctypes.sizeof(_lib.MoECacheEvictArgs)
 assert _APPEND_ARGS.size == ctypes.sizeof(_lib.MoERopeAppendArgs)
@@ -540,6 +542,57 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         *c, q.data_ptr(), qs[0], qs[1], _vector(seq_lens, _I32, "seq_lens", dev, seqs),
         out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
         _raw_stream(dev), hq, max_len, window, d ** -0.5 if scale is None else scale, softcap))
+    if status is not None and seqs:
+        status |= ws[:4].view(_I32)
+    return (out, lse) if return_lse else out
+
+
+def prefix_attention_workspace(seqs: int, q_heads: int, kv_heads: int, head_dim: int,
+                               device) -> torch.Tensor:
+    """A workspace for ``prefix_attention`` calls of these heads, with up to ``seqs``
+    sequences, that follow one another (calls that may overlap need one each)."""
+    n = _size_out("moe_prefix_attention_workspace_bytes", seqs, q_heads, kv_heads, head_dim)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     block_table: torch.Tensor, seq_lens: torch.Tensor, prefix_pages: torch.Tensor,
+                     scale: Optional[float] = None, softcap: float = 0.0, k_scale: float = 1.0,
+                     v_scale: float = 1.0, max_len: int = 0, out: Optional[torch.Tensor] = None,
+                     return_lse: bool = False, ws: Optional[torch.Tensor] = None,
+                     status: Optional[torch.Tensor] = None):
+    """``paged_attention`` of sequences that all begin with the same whole pages
+    ``prefix_pages`` (n,) int32 (a system prompt, a document): their keys are
+    read and multiplied once for all rows.  ``seq_lens`` counts the prefix; a
+    sequence is empty (0: zeros and -inf) or holds all of it (a length between
+    counts as empty, and as STATUS_BAD_PAGE).  ``block_table`` is read from the
+    first page behind the prefix on.  ``ws`` comes from
+    ``prefix_attention_workspace``; ``max_len``, ``out``, ``ws`` and ``status`` as
+    in ``paged_attention``."""
+    c, dev, seqs, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError("q must be (sequences, q_heads, head_dim)")
+    hq = shape[1]
+    qs = _rows_f32(q, "q", dev, (seqs, hq, d))
+    if out is None:
+        out = q.new_empty(seqs, hq, d)
+    elif out.dtype is not _F32 or out.get_device() != dev or out.shape != (seqs, hq, d) or \
+            not out.is_contiguous():
+        _refuse(out, "out", _F32, dev, (seqs, hq, d))
+    lse = q.new_empty(seqs, hq) if return_lse else None
+    if ws is None:
+        ws = prefix_attention_workspace(seqs, hq, hk, d, q.device)
+    elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
+        _refuse(ws, "ws", torch.uint8, dev)
+    if status is not None:
+        _vector(status, _I32, "status", dev, 1)
+    pages = prefix_pages.numel()
+    _enqueue("moe_prefix_attention_record", dev, _PREFIX_ARGS.pack(
+        *c, q.data_ptr(), qs[0], qs[1], _vector(seq_lens, _I32, "seq_lens", dev, seqs),
+        out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
+        _raw_stream(dev), hq, max_len, 0, d ** -0.5 if scale is None else scale, softcap,
+        _vector(prefix_pages, _I32, "prefix_pages", dev, pages), pages))
     if status is not None and seqs:
         status |= ws[:4].view(_I32)
     return (out, lse) if return_lse else out

@@ -1,0 +1,190 @@
+"""Attention of a batch that shares a prefix of pages, against the plain 64-bit
+attention of each sequence over all of its keys."""
+import math
+
+import pytest
+import torch
+
+from linuxnightmaresuite_b200 import kernels as K
+
+from ._attention import BF16, E4M3, F16, Cache, attend
+from .test_gpu_attention import randn
+
+pytestmark = pytest.mark.gpu
+
+
+class Shared:
+    """Sequences of `own` tokens of their own behind a prefix of `pages` pages; own 0 with
+    the prefix alone, None a padding row.  The tables do not name the prefix's pages."""
+
+    def __init__(self, own, pages, page, hkv, d, dtype, layout="nhd", seed=0):
+        P = pages * page
+        lens = [0 if n is None else P + n for n in own]
+        self.c = c = Cache(lens + [P], page, hkv, d, dtype, layout, seed)
+        self.pages = c.table_d[-1, :pages].contiguous()
+        self.table = c.table_d[:-1].contiguous()
+        self.table[:, :pages] = -9
+        self.lens, self.P = c.lens[:-1].contiguous(), P
+        for s, n in enumerate(lens):
+            if n:
+                c.kd[s], c.vd[s] = (torch.cat([x[-1], x[s][P:]]) for x in (c.kd, c.vd))
+        self.kd, self.vd, self.dtype = c.kd[:-1], c.vd[:-1], dtype
+
+    def call(self, q, **kw):
+        return K.prefix_attention(q, self.c.k, self.c.v, self.table, self.lens, self.pages,
+                                  return_lse=True, **self.c.scales, **kw)
+
+    def check(self, q, out, lse, scale, cap=0.0):
+        """The bounds of `attend` (of its own 2^-20 for the accumulators 2^-19: 16 steps of a
+        tile truncate, 2^-23 each), and for bf16 caches the probabilities' two parts: half a
+        step, 2^-9, of what the first part leaves, 2^-9 of the value."""
+        for s in range(q.shape[0]):
+            o, l, to, tl = attend(q[s].double(), self.kd[s], self.vd[s], scale, 0, cap)
+            if self.kd[s].shape[0] == 0:
+                assert (out[s] == 0).all() and torch.isneginf(lse[s]).all()
+                continue
+            vmax = self.vd[s].abs().amax((0, 2)).repeat_interleave(q.shape[1] // self.vd[s].shape[1])
+            to = to + vmax[:, None] * (2.0 ** -19 + (2.0 ** -18 if self.dtype == BF16 else 0.0))
+            err = (out[s].double() - o).abs()
+            assert (err <= to).all(), (s, err.max().item(), to.max().item())
+            assert ((lse[s].double() - l).abs() <= tl + 2.0 ** -21).all(), s
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("own,pages,page,hq,hkv,d,layout", [
+    ([1, 3], 1, 16, 4, 2, 128, "nhd"),              # less than a tile
+    ([0, None, 37, 5], 8, 16, 8, 2, 128, "nhd"),    # one whole tile; nothing of one's own; padding
+    ([2], 43, 7, 3, 1, 64, "hnd"),                  # odd pages: boxes of one row, a last tile of 45
+    ([20, 1, 9], 5, 100, 16, 2, 256, "nhd"),
+    ([0] * 35, 3, 128, 8, 2, 80, "nhd"),            # 140 rows: two row units
+    ([1, 2], 400, 16, 16, 16, 96, "hnd"),           # runs that cross from head to head
+    ([4] * 40, 21, 24, 16, 4, 192, "nhd"),          # column halves, the second one partly empty
+    ([None, None, None], 2, 16, 2, 1, 128, "nhd"),  # nobody
+    ([1, 1, 1], 300, 8, 5, 5, 16, "nhd"),
+    ([30] * 6, 150, 64, 32, 8, 128, "nhd"),         # several tiles for each CTA
+])
+def test_prefix(dtype, own, pages, page, hq, hkv, d, layout):
+    x = Shared(own, pages, page, hkv, d, dtype, layout, seed=hq + d)
+    q = 1.5 * randn(len(own), hq, d, seed=3)
+    ws = K.prefix_attention_workspace(len(own), hq, hkv, d, "cuda")
+    out, lse = x.call(q, ws=ws, max_len=int(x.lens.max()))
+    x.check(q, out, lse, d ** -0.5)
+    assert K.read_status(ws) == 0
+    again, lse2 = x.call(q, ws=ws, max_len=int(x.lens.max()))      # equal bits, and the workspace is ready
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+def test_prefix_many_rows(dtype):
+    """More row units than a team has members."""
+    own = [s % 3 for s in range(300)]
+    x = Shared(own, 20, 16, 2, 64, dtype, seed=5)
+    q = randn(300, 16, 64, seed=6)
+    x.check(q, *x.call(q), 0.125)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+def test_prefix_scales_caps_strides(dtype, d):
+    x = Shared([3, 0, None, 50], 30, 16, 2, d, dtype, seed=d)
+    wide = randn(4, 8 * d + 3, seed=2)              # rows of q off 16 bytes
+    q = wide[:, :8 * d].unflatten(1, (8, d))
+    for cap, scale, up in ((0.0, 0.3, 1.0), (5.0, 0.5, 1.0), (30.0, -0.1, 1.0), (1e-6, 0.1, 1.0),
+                           (0.0, 0.0, 1.0), (50.0, 1e-3, 1e4), (0.0, 1e30, 1e-31)):
+        z = (q * up)
+        if up == 1.0:
+            z = q
+        x.check(z, *x.call(z, scale=scale, softcap=cap), scale, cap)
+
+
+def test_prefix_out_over_q_and_no_prefix():
+    x = Shared([3, 8], 4, 16, 2, 64, F16)
+    q = randn(2, 4, 64)
+    want, lse = x.call(q)
+    z = q.clone()
+    got, lse2 = x.call(z, out=z)
+    assert got is z and torch.equal(z, want) and torch.equal(lse, lse2)
+    c = Cache([20, 7], 16, 2, 64, F16)
+    a = K.paged_attention(q, *c.args, c.lens, return_lse=True)
+    b = K.prefix_attention(q, *c.args, c.lens, x.pages[:0], return_lse=True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_prefix_reports():
+    x = Shared([3, 8, 2], 10, 16, 2, 128, F16)
+    q = randn(3, 8, 128)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x.lens[1] = 100                                 # not empty, and without the whole prefix
+    x.kd[1], x.vd[1] = x.kd[1][:0], x.vd[1][:0]
+    out, lse = x.call(q, status=status)
+    assert status.item() == K.STATUS_BAD_PAGE
+    x.check(q, out, lse, 128 ** -0.5)
+    # a prefix page that does not exist is left out
+    y = Shared([3, 8, 2], 10, 16, 2, 128, F16)
+    for bad, at in ((-1, 2), (10 ** 6, 9)):
+        y.pages[at] = bad
+        status.zero_()
+        out, lse = y.call(q, status=status)
+        assert status.item() == K.STATUS_BAD_PAGE
+    keep = torch.ones(160, dtype=torch.bool, device="cuda")
+    keep[32:48], keep[144:] = False, False
+    for s in range(3):
+        n = torch.cat([keep, torch.ones(y.kd[s].shape[0] - 160, dtype=torch.bool, device="cuda")])
+        y.kd[s], y.vd[s] = y.kd[s][n], y.vd[s][n]
+    y.check(q, out, lse, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+def test_prefix_nan_beside_and_inf_within(dtype):
+    """Slots behind the prefix's last page, or in a dropped one, may hold anything (the
+    pools of these tests are NaN); a row of q that is NaN stays alone; an infinite value
+    gives infinity or NaN in its column and nowhere else."""
+    x = Shared([3, 8], 9, 16, 2, 64, dtype)
+    q = randn(2, 4, 64)
+    want, _ = x.call(q)
+    z = q.clone()
+    z[0, 1] = math.nan
+    out, lse = x.call(z)
+    assert torch.isnan(out[0, 1]).all() and torch.isnan(lse[0, 1])
+    out[0, 1] = want[0, 1]
+    assert torch.equal(out, want)
+    if dtype != E4M3:
+        x.c.v[x.pages[1].long(), 3, 0, 5] = math.inf
+        out, _ = x.call(q)
+        assert not torch.isfinite(out[:, :2, 5]).any()
+        keep = torch.ones(64, dtype=torch.bool)
+        keep[5] = False
+        assert torch.equal(out[..., keep], want[..., keep]) and torch.equal(out[:, 2:], want[:, 2:])
+
+
+def test_prefix_captured_and_other_stream():
+    """One captured call serves other lengths and pages."""
+    x = Shared([3, 8, 60], 12, 16, 2, 128, F16)
+    y = Shared([50, None, 0], 12, 16, 2, 128, F16, seed=4)
+    q, ws = randn(3, 8, 128), K.prefix_attention_workspace(3, 8, 2, 128, "cuda")
+    pool = (max(x.c.k.shape[0], y.c.k.shape[0]),) + x.c.k.shape[1:]
+    k, v = (torch.full(pool, math.nan, dtype=F16, device="cuda") for _ in range(2))
+    table = torch.full((3, max(x.table.shape[1], y.table.shape[1])), -1, dtype=torch.int32,
+                       device="cuda")
+    lens, pages = torch.zeros_like(x.lens), x.pages.clone()
+    out = torch.empty_like(q)
+
+    def call():
+        return K.prefix_attention(q, k, v, table, lens, pages, out=out, return_lse=True, ws=ws)[1]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        lse = call()
+    for at, s in enumerate((x, y, x)):
+        k[:s.c.k.shape[0]], v[:s.c.v.shape[0]] = s.c.k, s.c.v
+        table[:, :s.table.shape[1]] = s.table
+        lens.copy_(s.lens), pages.copy_(s.pages)
+        q.copy_(randn(3, 8, 128, seed=at))
+        out.fill_(math.nan)
+        g.replay()
+        s.check(q, out, lse, 128 ** -0.5)
+    assert K.read_status(ws) == 0
