@@ -45,17 +45,16 @@ constexpr int kTeamMost = 16;
 struct PrefixArgs {
   moe_paged_cache c;                   // its block table is not used here
   CacheMap map;
-  const float* q;
-  int64_t q_ss, q_hs;
+  const uint8_t* q;                    // the rows' parts, as prefix_rows_kernel lays them out
+  const float* qscale;                 // score = product * qscale
   const int32_t* pages;
   int* status;
   float2* part_ml;                     // [slot][row] (maximum in powers of two, sum)
   float* part_o;                       // [slot][row][column of the unit]
-  int hq, G, rows, keys;               // rows of a key head, keys of the prefix
+  int rows, row_tiles, keys;           // of a key head, keys of the prefix
   int RU, m, RG, tiles, quota, parts;  // row units, team, row groups; tiles of a head; parts of a unit
   long long total;                     // tiles of all teams
-  float scale, cap;
-  int vec;                             // rows of q by 16 bytes
+  float cap;
 };
 
 template <int DT, int DQ> struct PrefixCfg {
@@ -81,9 +80,8 @@ template <int DT, int DQ> struct PrefixCfg {
   static_assert(2 * kRegsSoft + kRegsIssue + (kE4 ? kRegsWiden : 0) <=
                     65536 / kThreads / 8 * 8 * (kThreads / 128),
                 "");
-  // tensor memory: S (P over it) and O of each warpgroup, then q's third part
-  static constexpr int kSlab = kKT + kDV;
-  static constexpr int kQCol = 2 * kSlab;
+  // tensor memory: three S (P over them), O, then q's third part
+  static constexpr int kOCol = 3 * kKT, kQCol = kOCol + kDV;
   static_assert(kQCol + (kTmemQ ? DQ / 2 : 0) <= kTmemCols, "");
   static constexpr uint32_t kIdesc16 = (kBf ? (1u << 7) | (1u << 10) : 0u);
 };
@@ -91,12 +89,10 @@ template <int DT, int DQ> struct PrefixCfg {
 struct PrefixShared {
   uint64_t q_full, k_full[3], k_empty[3], v_full[3], v_empty[3];
   uint64_t rk_full[2], rk_empty[2], rv_full[2], rv_empty[2];
-  uint64_t s_full[2], p_full[2], o_full[2], drain;
+  uint64_t s_full[3], p_full[3], o_full[2], o_empty, drain;
   uint32_t tmem;
   int dead;
-  uint32_t raw_seen[2][4], seen[3][4], soft_seen[2][4];
-  float qscale[kPrefixRows];
-  int qexp[kPrefixRows];
+  uint32_t raw_seen[2][4], seen[3][4], soft_seen[3][4];
 };
 
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
@@ -137,6 +133,25 @@ __device__ __forceinline__ void tmem_ld2(uint32_t addr, float& a, float& b) {
   a = __uint_as_float(r0);
   b = __uint_as_float(r1);
 }
+// two f32 at a time
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -148,6 +163,77 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo,
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}" ::"r"(d),
       "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// q's rows as the tiles of the products: parts of [block of 64 columns][row][128 bytes],
+// swizzled, so that a CTA fetches a tile by a few bulk copies.  A warp per row; rows that
+// fill up the last tile are zero.  (Done by the CTAs of the prefix kernel themselves, at the start of
+// each piece, this took 14000 cycles of theirs.)
+// ---------------------------------------------------------------------------
+struct PrefixRowsArgs {
+  const float* q;
+  int64_t q_ss, q_hs;
+  uint8_t* tiles;
+  float* qscale;
+  int G, rows, row_tiles, heads, d, vec;
+  float scale, k_scale;
+};
+
+template <bool BF, int DQ>
+__global__ void __launch_bounds__(256) prefix_rows_kernel(const PrefixRowsArgs A) {
+  constexpr int PARTS = BF ? 3 : 2, PART = DQ / 64 * kPrefixRows * 128;
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t tile = id / kPrefixRows;                 // head, row tile
+  if (tile >= (int64_t)A.heads * A.row_tiles) return;
+  const int r = (int)(id % kPrefixRows), head = (int)(tile / A.row_tiles);
+  const int at = (int)(tile - (int64_t)head * A.row_tiles) * kPrefixRows + r, s = at / A.G;
+  const bool in = at < A.rows;
+  const float* q = A.q + s * A.q_ss + ((int64_t)head * A.G + at - (int64_t)s * A.G) * A.q_hs;
+  constexpr int PER = DQ / 32, VW = PER < 4 ? PER : 4;   // values of a lane: VW lane + 128 i ..
+  float v[PER], mx = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; i += VW) {
+    const int e = VW * lane + 32 * i;
+    if (VW == 4 && A.vec) {
+      const float4 f = in && e < A.d ? *reinterpret_cast<const float4*>(q + e)
+                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[i] = f.x;
+      v[i + 1] = f.y;
+      v[(i + 2) % PER] = f.z;
+      v[(i + 3) % PER] = f.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < VW; ++k) v[i + k] = in && e + k < A.d ? q[e + k] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mx = fmaxf(mx, fabsf(v[i]));
+  mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+  // scaled by a power of two to [2^10, 2^11), in two factors, since 2^e may lie outside the
+  // exponents of a float; a negative scale turns q, and one that vanishes stays above zero
+  const int ex = (int)(__float_as_uint(mx) >> 23);
+  const int e = mx > 0.f && ex < 255 ? 137 - max(ex, 1) : 0, e1 = e / 2, e2 = e - e1;
+  const float f1 = copysignf(__uint_as_float((uint32_t)(127 + e1) << 23), A.scale);
+  const float f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
+  if (lane == 0) A.qscale[id] = fmaxf(ldexpf(fabsf(A.scale) * A.k_scale, -e), 1e-30f);
+#pragma unroll
+  for (int i = 0; i < PER; i += VW) {
+    const int c = VW * lane + 32 * i;
+    uint8_t* to = A.tiles + tile * PARTS * PART + (c >> 6) * (kPrefixRows * 128) + r * 128 +
+                  ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2;
+    uint32_t lo[PARTS], hi[PARTS];
+    split2<BF, PARTS>(v[i] * f1 * f2, v[i + 1] * f1 * f2, lo);
+    if (VW == 4) split2<BF, PARTS>(v[(i + 2) % PER] * f1 * f2, v[(i + 3) % PER] * f1 * f2, hi);
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) {
+      if (VW == 4) *reinterpret_cast<uint2*>(to + k * PART) = make_uint2(lo[k], hi[k]);
+      else *reinterpret_cast<uint32_t*>(to + k * PART) = lo[k];
+    }
+  }
 }
 
 // A CTA's pieces: tiles t0 .. t0 + n of row unit `unit` of a head, part j of its parts.
@@ -198,7 +284,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
   uint8_t* const rv = rk + RS * Cfg::kRawK;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    mbar_init(&sh.q_full, 8);
+    mbar_init(&sh.q_full, 9);    // the copies, and every warp that is done with the piece before
     mbar_init(&sh.drain, 1);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&sh.k_full[i], E4 ? 4 : 1);
@@ -211,10 +297,14 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       mbar_init(&sh.rv_full[i], 1);
       mbar_init(&sh.rk_empty[i], 4);
       mbar_init(&sh.rv_empty[i], 4);
+    }
+    for (int i = 0; i < 3; ++i) {
       mbar_init(&sh.s_full[i], 2);
       mbar_init(&sh.p_full[i], 128);
-      mbar_init(&sh.o_full[i], 1);
     }
+    mbar_init(&sh.o_full[0], 1);
+    mbar_init(&sh.o_full[1], 1);
+    mbar_init(&sh.o_empty, 128);
     sh.dead = 0;
     fence_mbar_init();
     prefetch_map(&kmap);
@@ -235,140 +325,90 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
   };
   PrefixRun run(A);
   PrefixPiece p;
-  int n = 0;                           // tiles so far: warpgroup n & 1, its use n >> 1
+  int n = 0;                           // tiles so far: warpgroup n & 1, S n % 3
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSoft));
     const int w = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t S = tmem + lanes + (uint32_t)(w * Cfg::kSlab), O = S + KT;
-    const uint32_t other = tmem + lanes + (uint32_t)((w ^ 1) * Cfg::kSlab) + KT;
+    const uint32_t tm = tmem + lanes, O = tm + Cfg::kOCol;
     while (run.next(p)) {
-      const int r0 = p.ru / Cfg::kHalves * kPrefixRows;
-      // ---- q: a warp takes 16 rows, each scaled by a power of two to [2^10, 2^11)
-      constexpr int PER = DQ / 32;     // values of a lane: 4 lane + 128 i .. (2 lane + for 64)
-      constexpr int VW = PER < 4 ? PER : 4;
-#pragma unroll 1
-      for (int b = 0; b < 16; b += 8) {
-        float v[8][PER];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = warp * 16 + b + j, at = r0 + r, s = at / A.G;
-          const float* q = A.q + s * A.q_ss + (p.head * A.G + at - s * A.G) * A.q_hs;
-          const bool in = at < A.rows;
-#pragma unroll
-          for (int i = 0; i < PER; i += VW) {
-            const int e = VW * lane + 32 * i;
-            if (VW == 4 && A.vec) {
-              const float4 f = in && e < A.c.head_dim ? *reinterpret_cast<const float4*>(q + e)
-                                                      : make_float4(0.f, 0.f, 0.f, 0.f);
-              v[j][i] = f.x;
-              v[j][i + 1] = f.y;
-              v[j][i + 2 < PER ? i + 2 : 0] = f.z;
-              v[j][i + 3 < PER ? i + 3 : 0] = f.w;
-            } else {
-#pragma unroll
-              for (int k = 0; k < VW; ++k)
-                v[j][i + k] = in && e + k < A.c.head_dim ? q[e + k] : 0.f;
-            }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = warp * 16 + b + j;
-          float mx = 0.f;
-#pragma unroll
-          for (int i = 0; i < PER; ++i) mx = fmaxf(mx, fabsf(v[j][i]));
-          mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
-          const int ex = (int)(__float_as_uint(mx) >> 23);
-          const int e = mx > 0.f && ex < 255 ? 137 - max(ex, 1) : 0;
-          const int e1 = e / 2, e2 = e - e1;     // 2^e may lie outside the exponents of a float
-          const float f1 = copysignf(__uint_as_float((uint32_t)(127 + e1) << 23), A.scale);
-          const float f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
-          if (lane == 0) {
-            sh.qscale[r] = fmaxf(ldexpf(fabsf(A.scale) * A.c.k_scale, -e), 1e-30f);
-            sh.qexp[r] = e;
-          }
-#pragma unroll
-          for (int i = 0; i < PER; i += VW) {
-            const int c = VW * lane + 32 * i;
-            uint8_t* to = smem + (c >> 6) * (kPrefixRows * 128) + r * 128 +
-                          ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2;
-            uint32_t lo[Cfg::kParts], hi[Cfg::kParts];
-            split2<BF, Cfg::kParts>(v[j][i] * f1 * f2, v[j][i + 1] * f1 * f2, lo);
-            if (VW == 4)
-              split2<BF, Cfg::kParts>(v[j][i + 2 < PER ? i + 2 : 0] * f1 * f2,
-                                      v[j][i + 3 < PER ? i + 3 : 0] * f1 * f2, hi);
-#pragma unroll
-            for (int k = 0; k < Cfg::kSmemParts; ++k) {
-              if (VW == 4)
-                *reinterpret_cast<uint2*>(to + k * Cfg::kQPart) = make_uint2(lo[k], hi[k]);
-              else
-                *reinterpret_cast<uint32_t*>(to + k * Cfg::kQPart) = lo[k];
-            }
-          }
-        }
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");       // qscale
+      const int64_t tile = (int64_t)p.head * A.row_tiles + p.ru / Cfg::kHalves;
+      const float qscale = A.qscale[tile * kPrefixRows + row];
       if (Cfg::kTmemQ) {               // third parts: this thread's row, half of its columns
-        const int at = r0 + row, s = at / A.G;
-        const float* q = A.q + s * A.q_ss + (p.head * A.G + at - s * A.G) * A.q_hs;
-        const int e1 = sh.qexp[row] / 2, e2 = sh.qexp[row] - e1;
-        const float f1 = copysignf(__uint_as_float((uint32_t)(127 + e1) << 23), A.scale);
-        const float f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
+        const uint8_t* q = A.q + (tile * Cfg::kParts + 2) * Cfg::kQPart + row * 128;
 #pragma unroll 1
-        for (int c = 0; c < DQ / 2; c += 64) {
+        for (int c = w * (DQ / 2); c < (w + 1) * (DQ / 2); c += 64) {
           uint32_t x[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int e = w * (DQ / 2) + c + 2 * i;
-            uint32_t part[3];
-            const bool in = at < A.rows && e < A.c.head_dim;
-            split2<true, 3>(in ? q[e] * f1 * f2 : 0.f, in ? q[e + 1] * f1 * f2 : 0.f, part);
-            x[i] = part[2];
+          for (int i = 0; i < 8; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(
+                q + (c >> 6) * (kPrefixRows * 128) + ((i ^ (row & 7)) << 4));
+            x[4 * i] = v.x;
+            x[4 * i + 1] = v.y;
+            x[4 * i + 2] = v.z;
+            x[4 * i + 3] = v.w;
           }
-          tmem_st32(tmem + lanes + Cfg::kQCol + (w * (DQ / 2) + c) / 2, x);
+          tmem_st32(tm + Cfg::kQCol + c / 2, x);
         }
         tmem_wait_st();
         tc_fence_before();
       }
-      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
-
-      const float qscale = sh.qscale[row];
       const float to_cap = A.cap > 0.f ? fminf(qscale / A.cap, 3e38f) : 0.f;
       const float from_cap = A.cap * kLog2e;
       const float x2 = A.cap > 0.f ? 1.f : qscale * kLog2e;
       float o[DV], m = -INFINITY, l = 0.f;
 #pragma unroll
       for (int c = 0; c < DV; ++c) o[c] = 0.f;
-      for (int i = 0; i < p.n; ++i, ++n) {
-        if ((n & 1) != w) continue;
-        const uint32_t phase = (n >> 1) & 1;
-        wait(&sh.s_full[w], phase);
+      bool first = true;
+      auto fold = [&](int t) {         // the O of tile t, and it may be written again
+        wait(&sh.o_full[w], (t >> 1) & 1);
         tc_fence_after();
-        uint32_t seen[KT / 32], all = 0xffffffffu;
 #pragma unroll
-        for (int c = 0; c < KT / 32; ++c) {
-          seen[c] = sh.soft_seen[w][c];
-          all &= seen[c];
-        }
-        // ---- the largest score
-        float mx = -INFINITY, mn = INFINITY;
-#pragma unroll
-        for (int c = 0; c < KT / 32; ++c) {
+        for (int c = 0; c < DV; c += 32) {
           float v[32];
-          tmem_ld32(S + 32 * c, v);
-          if (all != 0xffffffffu)
+          tmem_ld32(O + c, v);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[c + k] += v[k];
+        }
+        tc_fence_before();
+        mbar_arrive(&sh.o_empty);
+      };
+      const int end = n + p.n;
+      int t = n + ((n ^ w) & 1);
+      for (; t < end; t += 2) {
+        const int b = t % 3;
+        const uint32_t S = tm + (uint32_t)(b * KT);
+        wait(&sh.s_full[b], (t / 3) & 1);
+        tc_fence_after();
+        const uint32_t* seen = sh.soft_seen[b];
+        uint32_t all = 0xffffffffu;
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) all &= seen[c];
+        auto hide = [&](float (&v)[32], int c) {
+          if (all != 0xffffffffu) {
+            const uint32_t bits = seen[c];
 #pragma unroll
             for (int k = 0; k < 32; ++k)
-              if (!((seen[c] >> k) & 1u)) v[k] = -INFINITY;
+              if (!((bits >> k) & 1u)) v[k] = -INFINITY;
+          }
+        };
+        // The loops over columns stay loops: unrolled, a tile's code is some 50 KB, and both
+        // warpgroups wait for instructions (32768 keys, 1024 rows a head, bf16 686 us instead of 440)
+        // ---- the largest score
+        float mx = -INFINITY, mn = INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < KT; c += 32) {
+          float v[32];
+          tmem_ld32(S + c, v);
+          hide(v, c / 32);
 #pragma unroll
           for (int k = 0; k < 32; ++k) mx = fmaxf(mx, v[k]);
           if (A.cap > 0.f)
 #pragma unroll
-            for (int k = 0; k < 32; ++k) mn = fminf(mn, (seen[c] >> k) & 1u ? v[k] : 0.f);
+            for (int k = 0; k < 32; ++k) mn = fminf(mn, v[k] == -INFINITY ? 0.f : v[k]);
         }
         bool steep = false;            // some score is not small against the cap
         if (A.cap > 0.f) {
@@ -377,22 +417,28 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         } else {
           mx *= x2;
         }
+        // ---- O of the tile before this one: its product had the time of the pass above
+        if (!first) fold(t - 2);
         if (__any_sync(0xffffffffu, mx > m + 8.f)) {
           const float to = mx > m + 8.f ? mx : m;
           const float f = to == -INFINITY ? 1.f : ex2(m - to);
+          if (!first) {
 #pragma unroll
-          for (int c = 0; c < DV; ++c) o[c] *= f;
+            for (int c = 0; c < DV; ++c) o[c] *= f;
+          }
           l *= f;
           m = to;
         }
+        first = false;
         const float shift = kPShift - (m == -INFINITY ? 0.f : m);
         // ---- probabilities: 32 keys' hi parts in 16 columns, then their lo parts
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < KT / 32; ++c) {
+        const uint64_t x22 = pack2(x2, x2), shift2 = pack2(shift, shift);
+        uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll 1
+        for (int c = 0; c < KT; c += 32) {
           float v[32];
           uint32_t x[32];
-          tmem_ld32(S + 32 * c, v);
+          tmem_ld32(S + c, v);
           if (A.cap > 0.f) {
             if (steep) {
 #pragma unroll
@@ -408,77 +454,70 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
               }
             }
           }
-          if (all != 0xffffffffu)
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (!((seen[c] >> k) & 1u)) v[k] = -INFINITY;
+          hide(v, c / 32);
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            const float a = ex2(fmaf(v[k], x2, shift)), b = ex2(fmaf(v[k + 1], x2, shift));
-            sum[k & 2] += a;
-            sum[(k & 2) + 1] += b;
+            float a, b;
+            unpack2(fma2(pack2(v[k], v[k + 1]), x22, shift2), a, b);
+            a = ex2(a);
+            b = ex2(b);
+            const uint64_t ab = pack2(a, b);
+            if (k & 2) sum1 = add2(sum1, ab);
+            else sum0 = add2(sum0, ab);
             uint32_t part[2];
             split2<BF, 2>(a, b, part);
             x[k / 2] = part[0];
             x[16 + k / 2] = part[1];
           }
-          tmem_st32(S + 32 * c, x);
+          tmem_st32(S + c, x);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float s0, s1;
+        unpack2(add2(sum0, sum1), s0, s1);
+        l += s0 + s1;
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&sh.p_full[w]);
-        // ---- this tile's O
-        wait(&sh.o_full[w], phase);
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < DV / 32; ++c) {
-          float v[32];
-          tmem_ld32(O + 32 * c, v);
-#pragma unroll
-          for (int k = 0; k < 32; ++k) o[32 * c + k] += v[k];
-        }
-        tc_fence_before();
+        mbar_arrive(&sh.p_full[b]);
       }
-      // ---- both warpgroups' parts: each hands over half of its columns through its O
-      constexpr int H = DV / 2;
-      tmem_st2(O + H, __float_as_uint(m), __float_as_uint(l));
+      if (!first) fold(t - 2);
+      n = end;
+      // ---- both warpgroups' parts meet in tensor memory (one in O, one in the place of
+      // S); each adds up half of the columns
+      asm volatile("bar.sync 1, 256;" ::: "memory");       // all products of the piece are done
+      const uint32_t mine = w ? tm : O, other = w ? O : tm, ml = tm + DV;
+      tmem_st2(ml + 2 * w, __float_as_uint(m), __float_as_uint(l));
 #pragma unroll
-      for (int c = 0; c < H; c += 32) {
+      for (int c = 0; c < DV; c += 32) {
         uint32_t x[32];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(w ? o[c + k] : o[H + c + k]);
-        tmem_st32(O + c, x);
+        for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(o[c + k]);
+        tmem_st32(mine + c, x);
       }
       tmem_wait_st();
       tc_fence_before();
       asm volatile("bar.sync 1, 256;" ::: "memory");
       tc_fence_after();
       float m1, l1;
-      tmem_ld2(other + H, m1, l1);
+      tmem_ld2(ml + 2 * (w ^ 1), m1, l1);
       const float M = fmaxf(m, m1), ms = M == -INFINITY ? 0.f : M;
       const float f0 = ex2(m - ms), f1 = ex2(m1 - ms);
-      const bool in = r0 + row < A.rows;
+      const bool in = p.ru / Cfg::kHalves * kPrefixRows + row < A.rows;
       if (in && w == 0)
-        A.part_ml[(int64_t)p.slot * kPrefixRows + row] =
-            make_float2(M, l * f0 + l1 * f1);
-      float* to = A.part_o + ((int64_t)p.slot * kPrefixRows + row) * DV + w * H;
+        A.part_ml[(int64_t)p.slot * kPrefixRows + row] = make_float2(M, l * f0 + l1 * f1);
+      float* to = A.part_o + ((int64_t)p.slot * kPrefixRows + row) * DV;
+#pragma unroll 1
+      for (int c = w * (DV / 2); c < (w + 1) * (DV / 2); c += 32) {
+        float v[32], u[32];
+        tmem_ld32(mine + c, v);
+        tmem_ld32(other + c, u);
 #pragma unroll
-      for (int c = 0; c < H; c += 32) {
-        float v[32];
-        tmem_ld32(other + c, v);
-#pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          float4 y;
-          y.x = (w ? o[H + c + k] : o[c + k]) * f0 + v[k] * f1;
-          y.y = (w ? o[H + c + k + 1] : o[c + k + 1]) * f0 + v[k + 1] * f1;
-          y.z = (w ? o[H + c + k + 2] : o[c + k + 2]) * f0 + v[k + 2] * f1;
-          y.w = (w ? o[H + c + k + 3] : o[c + k + 3]) * f0 + v[k + 3] * f1;
-          if (in) *reinterpret_cast<float4*>(to + c + k) = y;
-        }
+        for (int k = 0; k < 32; k += 4)
+          if (in)
+            *reinterpret_cast<float4*>(to + c + k) = make_float4(
+                v[k] * f0 + u[k] * f1, v[k + 1] * f0 + u[k + 1] * f1, v[k + 2] * f0 + u[k + 2] * f1,
+                v[k + 3] * f0 + u[k + 3] * f1);
       }
       tc_fence_before();
-      asm volatile("bar.sync 1, 256;" ::: "memory");       // O, m, l and q are free
+      asm volatile("bar.sync 1, 256;" ::: "memory");       // S and O are free
       tc_fence_after();
     }
   } else if (warp < 12) {
@@ -496,56 +535,61 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         wait(&sh.q_full, pieces & 1);
         ++pieces;
         tc_fence_after();
-        for (int i = 0; i <= p.n; ++i) {
-          if (i < p.n) {               // S of tile n + i
-            const int t = n + i, st = t % NS, w = t & 1;
+        // S runs two tiles ahead of O (one, where keys and values are widened into one stage
+        // each, in turn); S of tile t + 3 takes the place of P of tile t behind the
+        // product that reads it
+        constexpr int AHEAD = NS > 1 ? 2 : 1;
+        for (int i = -AHEAD; i < p.n; ++i) {
+          if (i + AHEAD < p.n) {       // S of tile n + i + AHEAD
+            const int t = n + i + AHEAD, st = t % NS, b = t % 3;
             wait(&sh.k_full[st], (t / NS) & 1);
-            if (lane < 4) sh.soft_seen[w][lane] = sh.seen[st][lane];
+            if (lane < 4) sh.soft_seen[b][lane] = sh.seen[st][lane];
             __syncwarp();
             if (lane == 0 && !*(volatile int*)&sh.dead) {
               tc_fence_after();
-              const uint32_t d = tmem + (uint32_t)(w * Cfg::kSlab);
+              const uint32_t d = tmem + (uint32_t)(b * KT);
               const uint32_t kb = k_lo + (uint32_t)(st * Cfg::kK >> 4);
               bool first = true;
               for (int k = Cfg::kParts - 1; k >= 0; --k) {
 #pragma unroll
                 for (int c = 0; c < DQ / 16; ++c) {
-                  const uint32_t b = kb + (uint32_t)(((c >> 2) * BLK + (c & 3) * 32) >> 4);
+                  const uint32_t kc = kb + (uint32_t)(((c >> 2) * BLK + (c & 3) * 32) >> 4);
                   if (Cfg::kTmemQ && k == 2) {
-                    tc_mma_ts(d, tmem + Cfg::kQCol + 8 * c, b, desc_hi, is, first ? 0u : 1u);
+                    tc_mma_ts(d, tmem + Cfg::kQCol + 8 * c, kc, desc_hi, is, first ? 0u : 1u);
                   } else {
                     const uint32_t a = q_lo + (uint32_t)((k * Cfg::kQPart + (c >> 2) * kPrefixRows * 128 +
                                                           (c & 3) * 32) >> 4);
-                    tc_mma_lo(d, a, b, desc_hi, is, first ? 0u : 1u);
+                    tc_mma_lo(d, a, kc, desc_hi, is, first ? 0u : 1u);
                   }
                   first = false;
                 }
               }
               tc_commit(&sh.k_empty[st]);
-              mbar_arrive(&sh.s_full[w]);
-              tc_commit(&sh.s_full[w]);
+              mbar_arrive(&sh.s_full[b]);
+              tc_commit(&sh.s_full[b]);
             }
             __syncwarp();
           }
-          if (i > 0) {                 // O of the tile before
-            const int t = n + i - 1, st = t % NS, w = t & 1;
+          if (i >= 0) {                // O of tile n + i
+            const int t = n + i, st = t % NS, b = t % 3;
             wait(&sh.v_full[st], (t / NS) & 1);
             uint32_t all = 0xffffffffu;
 #pragma unroll
-            for (int c = 0; c < KT / 32; ++c) all &= sh.soft_seen[w][c];
+            for (int c = 0; c < KT / 32; ++c) all &= sh.soft_seen[b][c];
             if (all != 0xffffffffu) {  // nothing of a row that is not seen counts
               for (int r = lane; r < KT; r += 32)
-                if (!((sh.soft_seen[w][r >> 5] >> (r & 31)) & 1u))
+                if (!((sh.soft_seen[b][r >> 5] >> (r & 31)) & 1u))
                   for (int c = 0; c < DV / 64 * 8; ++c)
                     *reinterpret_cast<uint4*>(vs + st * Cfg::kV + (c >> 3) * BLK + r * 128 +
                                               (c & 7) * 16) = make_uint4(0, 0, 0, 0);
               fence_proxy_async_smem();
             }
-            wait(&sh.p_full[w], (t >> 1) & 1);
+            wait(&sh.p_full[b], (t / 3) & 1);
+            if (t > 0) wait(&sh.o_empty, (t - 1) & 1);
             __syncwarp();
             if (lane == 0 && !*(volatile int*)&sh.dead) {
               tc_fence_after();
-              const uint32_t a = tmem + (uint32_t)(w * Cfg::kSlab), d = a + KT;
+              const uint32_t a = tmem + (uint32_t)(b * KT), d = tmem + Cfg::kOCol;
               const uint32_t vb = v_lo + (uint32_t)(st * Cfg::kV >> 4);
 #pragma unroll
               for (int k = 1; k >= 0; --k)
@@ -554,7 +598,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                   tc_mma_ts(d, a + 32 * (c >> 1) + 16 * k + 8 * (c & 1), vb + (uint32_t)(c * 2048 >> 4),
                             desc_hi, io, k == 1 && c == 0 ? 0u : 1u);
               tc_commit(&sh.v_empty[st]);
-              tc_commit(&sh.o_full[w]);
+              tc_commit(&sh.o_full[t & 1]);
             }
             __syncwarp();
           }
@@ -565,84 +609,96 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         tc_commit(&sh.drain);
         mbar_wait(&sh.drain, 0);
       }
-    } else if (warp == 9) {
-      // ---- loads
-      constexpr int EB = E4 ? 1 : 2, LINE = 128 / EB;          // elements of a line
+    } else if (warp < 11) {
+      // ---- loads: q and keys, values
+      const bool keys = warp == 9;
+      constexpr int LINE = E4 ? 128 : 64;                  // elements of a line
       constexpr int RING = E4 ? (RS ? RS : 1) : NS;
-      uint64_t* kf = E4 ? sh.rk_full : sh.k_full;
-      uint64_t* vf = E4 ? sh.rv_full : sh.v_full;
-      uint64_t* ke = E4 ? sh.rk_empty : sh.k_empty;
-      uint64_t* ve = E4 ? sh.rv_empty : sh.v_empty;
-      uint8_t* kt = E4 ? rk : ks;
-      uint8_t* vt = E4 ? rv : vs;
-      constexpr int KB = E4 ? Cfg::kRawK : Cfg::kK, VB = E4 ? Cfg::kRawV : Cfg::kV;
-      const int ps = A.c.page_size, shift = A.map.box_shift, boxes = KT >> shift;
+      uint64_t* full = E4 ? (keys ? sh.rk_full : sh.rv_full) : keys ? sh.k_full : sh.v_full;
+      uint64_t* empty = E4 ? (keys ? sh.rk_empty : sh.rv_empty) : keys ? sh.k_empty : sh.v_empty;
+      const CUtensorMap* map = keys ? &kmap : &vmap;
+      const int bytes = keys ? (E4 ? Cfg::kRawK : Cfg::kK) : E4 ? Cfg::kRawV : Cfg::kV;
+      const int lines = bytes / BLK;
+      uint8_t* const ring = keys ? (E4 ? rk : ks) : E4 ? rv : vs;
+      const uint32_t ps = A.c.page_size, shift = A.map.box_shift;
+      const int boxes = KT >> shift;
+      bool q_loads = false;
       while (run.next(p)) {
-        const int x0 = p.ru % Cfg::kHalves * 128;              // this unit's columns of V
-        for (int i = 0; i < p.n; ++i, ++n) {
-          const int st = n % RING;
-          const uint32_t round = n / RING, key0 = (uint32_t)(p.t0 + i) * KT;
-          // this lane's boxes: lane, lane + 32, ...
-          int row[4], slot[4];
-          uint32_t ok[4];
+        const int x0 = keys ? 0 : p.ru % Cfg::kHalves * 128;     // this unit's columns of V
+        // pages of this lane's boxes (lane, lane + 32, ...), fetched a tile ahead
+        int page[4];
+        uint32_t slot[4];
+        auto fetch = [&](int tile) {
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            const int box = lane + 32 * b;
-            const uint32_t key = key0 + ((uint32_t)box << shift);
-            row[b] = -1;
-            slot[b] = 0;
-            if (box < boxes && key < (uint32_t)A.keys) {
-              const uint32_t pg = key / (uint32_t)ps;
-              const int page = A.pages[pg];
-              if (page >= 0 && page < A.c.pages) {
-                row[b] = page * A.map.page_units + p.head * A.map.head_units;
-                slot[b] = (int)(key - pg * ps);
-              } else {
-                set_status(A.status, MOE_STATUS_BAD_PAGE);
-              }
+            const uint32_t key = (uint32_t)tile * KT + ((uint32_t)(lane + 32 * b) << shift);
+            page[b] = -1;
+            slot[b] = 0xffffffffu;     // no such box
+            if (lane + 32 * b < boxes && key < (uint32_t)A.keys) {
+              const uint32_t pg = key / ps;
+              page[b] = A.pages[pg];
+              slot[b] = key - pg * ps;
             }
-            ok[b] = __ballot_sync(0xffffffffu, row[b] >= 0);
           }
-          // keys of the tile that are there
-          uint32_t* seen = E4 ? sh.raw_seen[st] : sh.seen[st];
-          const uint32_t count = __popc(ok[0]) + __popc(ok[1]) + __popc(ok[2]) + __popc(ok[3]);
-          if (round > 0) wait(&ke[st], (round - 1) & 1);
-          if (lane < 4) {
-            uint32_t bits = 0;
-            for (int k = 0; k < 32; ++k) {
-              const int box = (32 * lane + k) >> shift;
-              const uint32_t word = box < 32 ? ok[0] : box < 64 ? ok[1] : box < 96 ? ok[2] : ok[3];
-              bits |= ((word >> (box & 31)) & 1u) << k;
-            }
-            seen[lane] = 32 * lane < KT ? bits : 0xffffffffu;
+        };
+        fetch(p.t0);
+        if (keys) {                    // q, once the products of the piece before are done
+          if (n > 0) wait(&sh.k_empty[(n - 1) % NS], ((n - 1) / NS) & 1);
+          if (lane == 0 && !*(volatile int*)&sh.dead) {
+            const int64_t tile = (int64_t)p.head * A.row_tiles + p.ru / Cfg::kHalves;
+            mbar_expect_tx(&sh.q_full, Cfg::kQ);
+#pragma unroll 1
+            for (int c = 0; c < Cfg::kQ; c += 16384)
+              bulk_g2s_plain(smem + c, A.q + tile * Cfg::kParts * Cfg::kQPart + c, 16384, &sh.q_full);
+            q_loads = true;
           }
           __syncwarp();
-          const bool go = !*(volatile int*)&sh.dead;
-          auto copy = [&](const CUtensorMap* map, uint8_t* to, uint64_t* bar, int bytes, int x) {
-            const int lines = bytes / BLK;
-            if (lane == 0) mbar_expect_tx(bar, (count << shift) * 128u * (uint32_t)lines);
-            __syncwarp();
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-              if (row[b] >= 0)
-                for (int c = 0; c < lines; ++c)
-                  tma_load_3d(smem_u32(to) + c * BLK + ((lane + 32 * b) << shift) * 128, map,
-                              x + c * LINE, row[b], slot[b], bar);
-          };
-          if (__any_sync(0xffffffffu, !go)) break;
-          copy(&kmap, kt + st * KB, &kf[st], KB, 0);
-          if (round > 0) wait(&ve[st], (round - 1) & 1);
+        }
+        for (int i = 0; i < p.n; ++i, ++n) {
+          const int st = n % RING;
+          const uint32_t round = n / RING;
+          if (round > 0) wait(&empty[st], (round - 1) & 1);
           if (__any_sync(0xffffffffu, *(volatile int*)&sh.dead)) break;
-          copy(&vmap, vt + st * VB, &vf[st], VB, x0);
+          uint32_t count = 0, ok[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const bool there = page[b] >= 0 && page[b] < A.c.pages;
+            if (keys && !there && slot[b] != 0xffffffffu) set_status(A.status, MOE_STATUS_BAD_PAGE);
+            ok[b] = __ballot_sync(0xffffffffu, there);
+            count += __popc(ok[b]);
+            if (!there) page[b] = -1;
+          }
+          if (keys && lane < 4) {      // keys of the tile that are there
+            uint32_t bits = 0xffffffffu;
+            if (count != (uint32_t)boxes && 32 * lane < KT)
+              for (int k = 0; k < 32; ++k) {
+                const int box = (32 * lane + k) >> shift;
+                const uint32_t word = box < 32 ? ok[0] : box < 64 ? ok[1] : box < 96 ? ok[2] : ok[3];
+                if (!((word >> (box & 31)) & 1u)) bits &= ~(1u << k);
+              }
+            (E4 ? sh.raw_seen[st] : sh.seen[st])[lane] = bits;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_expect_tx(&full[st], (count << shift) * 128u * (uint32_t)lines);
+          __syncwarp();
+          const uint32_t to = smem_u32(ring) + st * bytes;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (page[b] >= 0)
+              for (int c = 0; c < lines; ++c)
+                tma_load_3d(to + c * BLK + ((lane + 32 * b) << shift) * 128, map, x0 + c * LINE,
+                            page[b] * A.map.page_units + p.head * A.map.head_units, (int)slot[b],
+                            &full[st]);
+          __syncwarp();
+          if (i + 1 < p.n) fetch(p.t0 + i + 1);
         }
       }
       // after a timeout copies may still be under way: give them time to land
       if (*(volatile int*)&sh.dead)
-        for (int s = 0; s < RING; ++s)
-          for (int k = 0; k < 2; ++k) {
-            mbar_wait(&kf[s], k);
-            mbar_wait(&vf[s], k);
-          }
+        for (int k = 0; k < 2; ++k) {
+          for (int s = 0; s < RING; ++s) mbar_wait(&full[s], k);
+          if (q_loads) mbar_wait(&sh.q_full, k);
+        }
     }
   } else if (E4) {
     // ---- e4m3 -> fp16, rows of 128 bytes swizzled on both sides
@@ -798,27 +854,30 @@ static PrefixPlan prefix_plan(int seqs, int q_heads, int kv_heads, int head_dim)
 struct PrefixSpace {
   float* lse;
   float2* ml;
-  float* o;
-  uint8_t* own;
-  size_t own_bytes;
+  float *o, *qscale;
+  uint8_t* q;
+  size_t own_bytes;                    // of the attention behind the prefix, in front
 };
 
 static int prefix_workspace(const PrefixPlan& p, int seqs, int q_heads, int kv_heads, int head_dim,
                             void* ws, PrefixSpace* out, size_t* bytes) {
   Carve cv = {static_cast<uint8_t*>(ws), 0, 0};
-  size_t own = 0;                      // of the attention behind the prefix; it starts with the status
+  size_t own = 0;                      // starts with the status
   MOE_CHECK(moe_paged_attention_workspace_bytes(seqs, q_heads, kv_heads, head_dim, &own));
-  uint8_t* at = cv.take<uint8_t>(own);
+  cv.take<uint8_t>(own);
   float* lse = cv.take<float>((size_t)seqs * q_heads);
   float2* ml = cv.take<float2>((size_t)p.slots * kPrefixRows);
   float* o = cv.take<float>((size_t)p.slots * kPrefixRows * p.dv);
-  if (out) *out = {lse, ml, o, at, own};
+  const size_t rows = (size_t)kv_heads * (p.RU / p.halves) * kPrefixRows;
+  float* qscale = cv.take<float>(rows);
+  uint8_t* q = cv.take<uint8_t>(rows * p.dq * 3 * 2);    // three parts at most
+  if (out) *out = {lse, ml, o, qscale, q, own};
   *bytes = align_up(cv.used, 256);
   return MOE_OK;
 }
 
 template <int DT, int DQ>
-static int launch_prefix(PrefixArgs& a, int grid, cudaStream_t s) {
+static int launch_prefix(PrefixArgs& a, const PrefixRowsArgs& rows, int grid, cudaStream_t s) {
   using Cfg = PrefixCfg<DT, DQ>;
   static std::atomic<uint64_t> ready{0};
   auto kern = prefix_kernel<DT, DQ>;
@@ -837,15 +896,20 @@ static int launch_prefix(PrefixArgs& a, int grid, cudaStream_t s) {
   CUtensorMap kmap, vmap;
   MOE_CHECK(make_cache_map(&kmap, a.c, a.c.k, Cfg::kKT, &a.map));
   MOE_CHECK(make_cache_map(&vmap, a.c, a.c.v, Cfg::kKT, &a.map));
+  const int64_t blocks = (int64_t)rows.heads * rows.row_tiles * (kPrefixRows / 8);
+  MOE_REQUIRE(blocks <= 0x7fffffff, MOE_ERR_UNSUPPORTED, "%d rows are too many", rows.rows);
+  MOE_CUDA(launch_pdl(prefix_rows_kernel<Cfg::kBf, DQ>, dim3((unsigned)blocks), dim3(256), 0, s,
+                      rows));
   MOE_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(Cfg::kThreads), Cfg::kSmem, s, kmap, vmap, a));
   return MOE_OK;
 }
 
 template <int DT>
-static int launch_prefix_dt(PrefixArgs& a, int dq, int grid, cudaStream_t s) {
-  return dq == 64    ? launch_prefix<DT, 64>(a, grid, s)
-         : dq == 128 ? launch_prefix<DT, 128>(a, grid, s)
-                     : launch_prefix<DT, 256>(a, grid, s);
+static int launch_prefix_dt(PrefixArgs& a, const PrefixRowsArgs& r, int dq, int grid,
+                            cudaStream_t s) {
+  return dq == 64    ? launch_prefix<DT, 64>(a, r, grid, s)
+         : dq == 128 ? launch_prefix<DT, 128>(a, r, grid, s)
+                     : launch_prefix<DT, 256>(a, r, grid, s);
 }
 
 }  // namespace moe
@@ -882,16 +946,15 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
   MOE_CHECK(moe::prefix_workspace(p, S, t.q_heads, a.c.kv_heads, d, t.workspace, &ws, &need));
   MOE_REQUIRE(t.workspace_bytes >= need, MOE_ERR_WORKSPACE, "workspace %zu < %zu bytes",
               t.workspace_bytes, need);
-  a.q = t.q;
-  a.q_ss = t.q_seq_stride;
-  a.q_hs = t.q_head_stride;
+  const int G = t.q_heads / a.c.kv_heads;
+  a.q = ws.q;
+  a.qscale = ws.qscale;
   a.pages = r->prefix;
   a.status = static_cast<int*>(t.workspace);
   a.part_ml = ws.ml;
   a.part_o = ws.o;
-  a.hq = t.q_heads;
-  a.G = t.q_heads / a.c.kv_heads;
-  a.rows = S * a.G;
+  a.rows = S * G;
+  a.row_tiles = p.RU / p.halves;
   a.keys = P;
   a.RU = p.RU;
   a.m = p.m;
@@ -899,16 +962,17 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
   a.tiles = (P + p.kt - 1) / p.kt;
   a.total = (long long)p.units * a.tiles;
   const long long quota = (a.total + p.teams - 1) / p.teams;
-  MOE_REQUIRE(quota < (1ll << 30) && (int64_t)S * a.G < (1ll << 30) && p.slots < (1ll << 30),
+  MOE_REQUIRE(quota < (1ll << 30) && (int64_t)S * G < (1ll << 30) && p.slots < (1ll << 30),
               MOE_ERR_UNSUPPORTED, "%d sequences behind a prefix of %d tokens are too many", S, P);
   a.quota = (int)quota;
   a.parts = (a.tiles - 1) / a.quota + 2;
   MOE_REQUIRE(p.units * p.m * a.parts <= p.slots, MOE_ERR_INVALID, "parts %d", a.parts);
   const int grid = (int)((a.total + quota - 1) / quota) * p.m;
-  a.scale = t.scale;
   a.cap = t.softcap;
-  a.vec = (uintptr_t)t.q % 16 == 0 && (S == 1 || t.q_seq_stride % 4 == 0) &&
-          (t.q_heads == 1 || t.q_head_stride % 4 == 0);
+  const int vec = (uintptr_t)t.q % 16 == 0 && (S == 1 || t.q_seq_stride % 4 == 0) &&
+                  (t.q_heads == 1 || t.q_head_stride % 4 == 0);
+  const moe::PrefixRowsArgs rows = {t.q, t.q_seq_stride, t.q_head_stride, ws.q, ws.qscale, G,
+                                    a.rows, a.row_tiles, a.c.kv_heads, d, vec, t.scale, a.c.k_scale};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(t.stream);
   // the keys behind the prefix: checks q and out, and writes out
   moe_paged_attention_args own = t;
@@ -916,14 +980,14 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
   own.workspace_bytes = ws.own_bytes;
   {
     ::moe::ProfScope _prof(MOE_K_PREFIX, s);
-    MOE_CHECK(a.c.dtype == MOE_CACHE_F16 ? moe::launch_prefix_dt<MOE_CACHE_F16>(a, p.dq, grid, s)
+    MOE_CHECK(a.c.dtype == MOE_CACHE_F16 ? moe::launch_prefix_dt<MOE_CACHE_F16>(a, rows, p.dq, grid, s)
               : a.c.dtype == MOE_CACHE_BF16
-                  ? moe::launch_prefix_dt<MOE_CACHE_BF16>(a, p.dq, grid, s)
-                  : moe::launch_prefix_dt<MOE_CACHE_E4M3>(a, p.dq, grid, s));
+                  ? moe::launch_prefix_dt<MOE_CACHE_BF16>(a, rows, p.dq, grid, s)
+                  : moe::launch_prefix_dt<MOE_CACHE_E4M3>(a, rows, p.dq, grid, s));
   }
   MOE_CHECK(moe::attention_from(own, P));
   const moe::PrefixJoinArgs j = {ws.ml, ws.o, t.seq_lens, ws.lse, t.out, t.lse,
-                                 a.status, S, t.q_heads, a.G, d, p.dv, p.halves, P, a.RU, a.m, a.RG,
+                                 a.status, S, t.q_heads, G, d, p.dv, p.halves, P, a.RU, a.m, a.RG,
                                  a.tiles, a.quota, a.parts, a.c.v_scale};
   {
     ::moe::ProfScope _prof(MOE_K_PREFIX, s);
