@@ -76,7 +76,7 @@ template <int DT, int DQ> struct PrefixCfg {
   static constexpr int kSmem = 1024 + kQ + kStages * (kK + kV) + kRawStages * (kRawK + kRawV);
   static constexpr int kThreads = kE4 ? 512 : 384;
   // registers of a thread by warpgroup: what the block was launched with, dealt out again
-  static constexpr int kRegsSoft = kE4 ? 192 : 224, kRegsIssue = kE4 ? 48 : 56, kRegsWiden = 80;
+  static constexpr int kRegsSoft = kE4 ? 208 : 224, kRegsIssue = kE4 ? 48 : 56, kRegsWiden = 48;
   static_assert(2 * kRegsSoft + kRegsIssue + (kE4 ? kRegsWiden : 0) <=
                     65536 / kThreads / 8 * 8 * (kThreads / 128),
                 "");
@@ -89,24 +89,42 @@ template <int DT, int DQ> struct PrefixCfg {
 struct PrefixShared {
   uint64_t q_full, k_full[3], k_empty[3], v_full[3], v_empty[3];
   uint64_t rk_full[2], rk_empty[2], rv_full[2], rv_empty[2];
-  uint64_t s_full[3], p_full[3], o_full[2], o_empty, drain;
+  uint64_t s_full[3], p_full[3], p_read[3], o_full[2], o_empty, drain[2];
   uint32_t tmem;
   int dead;
-  uint32_t raw_seen[2][4], seen[3][4], soft_seen[3][4];
+  // keys of a tile that are there, tile t at t % 8: the loads of tile t + 8 begin when S of tile
+  // t + 5 at least has been formed, in the place of P of tile t + 2
+  uint4 seen[8];
 };
 
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 columns of this thread's row, on their way until tmem_wait_ld
+__device__ __forceinline__ void tmem_get32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
       "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// waits for all loads; r is read behind it
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  tmem_get32(addr, r);
+  tmem_wait_ld(r);
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -285,7 +303,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     mbar_init(&sh.q_full, 9);    // the copies, and every warp that is done with the piece before
-    mbar_init(&sh.drain, 1);
+    mbar_init(&sh.drain[0], 1);
+    mbar_init(&sh.drain[1], 1);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&sh.k_full[i], E4 ? 4 : 1);
       mbar_init(&sh.v_full[i], E4 ? 4 : 1);
@@ -301,6 +320,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     for (int i = 0; i < 3; ++i) {
       mbar_init(&sh.s_full[i], 2);
       mbar_init(&sh.p_full[i], 128);
+      mbar_init(&sh.p_read[i], 1);
     }
     mbar_init(&sh.o_full[0], 1);
     mbar_init(&sh.o_full[1], 1);
@@ -321,6 +341,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       *(volatile int*)&sh.dead = 1;
       set_status(A.status, MOE_STATUS_TIMEOUT);
     }
+  };
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
+    wait(bar, parity);
     __syncwarp();
   };
   PrefixRun run(A);
@@ -364,14 +387,20 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       for (int c = 0; c < DV; ++c) o[c] = 0.f;
       bool first = true;
       auto fold = [&](int t) {         // the O of tile t, and it may be written again
-        wait(&sh.o_full[w], (t >> 1) & 1);
+        warp_wait(&sh.o_full[w], (t >> 1) & 1);
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < DV; c += 32) {
-          float v[32];
-          tmem_ld32(O + c, v);
+        for (int c = 0; c < DV; c += 64) {
+          uint32_t v[32], u[32];
+          tmem_get32(O + c, v);
+          tmem_get32(O + c + 32, u);
+          tmem_wait_ld(v);
+          tmem_wait_ld(u);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[c + k] += v[k];
+          for (int k = 0; k < 32; ++k) {
+            o[c + k] += __uint_as_float(v[k]);
+            o[c + 32 + k] += __uint_as_float(u[k]);
+          }
         }
         tc_fence_before();
         mbar_arrive(&sh.o_empty);
@@ -381,42 +410,66 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       for (; t < end; t += 2) {
         const int b = t % 3;
         const uint32_t S = tm + (uint32_t)(b * KT);
-        wait(&sh.s_full[b], (t / 3) & 1);
+        warp_wait(&sh.s_full[b], (t / 3) & 1);
         tc_fence_after();
-        const uint32_t* seen = sh.soft_seen[b];
-        uint32_t all = 0xffffffffu;
-#pragma unroll
-        for (int c = 0; c < KT / 32; ++c) all &= seen[c];
-        auto hide = [&](float (&v)[32], int c) {
-          if (all != 0xffffffffu) {
-            const uint32_t bits = seen[c];
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (!((bits >> k) & 1u)) v[k] = -INFINITY;
-          }
-        };
-        // The loops over columns stay loops: unrolled, a tile's code is some 50 KB, and both
-        // warpgroups wait for instructions (32768 keys, 1024 rows a head, bf16 686 us instead of 440)
-        // ---- the largest score
-        float mx = -INFINITY, mn = INFINITY;
+        const uint32_t* seen = &sh.seen[t % 8].x;
+        const uint32_t all = seen[0] & seen[1] & seen[2] & seen[3];
+        // The loops over columns stay loops, and what few tiles need stands apart: with all of
+        // it unrolled a tile's code is some 50 KB, and both warpgroups wait for instructions
+        // (32768 keys, 1024 rows a head, bf16: 686 us instead of 440)
+        float mx = -INFINITY;
+        if (all != 0xffffffffu || A.cap > 0.f) {
+          // ---- keys that are not there become minus infinity, scores cap tanh(score / cap) log2 e
 #pragma unroll 1
-        for (int c = 0; c < KT; c += 32) {
-          float v[32];
-          tmem_ld32(S + c, v);
-          hide(v, c / 32);
+          for (int c = 0; c < KT; c += 32) {
+            uint32_t v[32];
+            tmem_get32(S + c, v);
+            tmem_wait_ld(v);
+            const uint32_t bits = seen[c / 32];
+            float big = 0.f;           // what is not there picks no form of tanh
 #pragma unroll
-          for (int k = 0; k < 32; ++k) mx = fmaxf(mx, v[k]);
-          if (A.cap > 0.f)
+            for (int k = 0; k < 32; ++k) {
+              if (!((bits >> k) & 1u)) v[k] = A.cap > 0.f ? 0u : 0xff800000u;
+              big = fmaxf(big, fabsf(__uint_as_float(v[k])));
+            }
+            if (A.cap > 0.f) {
+              if (__any_sync(0xffffffffu, !(big * to_cap < 0.5f))) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) mn = fminf(mn, v[k] == -INFINITY ? 0.f : v[k]);
+                for (int k = 0; k < 32; ++k)
+                  v[k] = __float_as_uint(from_cap * tanhf(__uint_as_float(v[k]) * to_cap));
+              } else {
+                // Lambert's continued fraction, off by less than 2^-29 of tanh y for |y| < 1/2
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                  const float y = __uint_as_float(v[k]) * to_cap, z = y * y;
+                  const float num = fmaf(z, z + 105.f, 945.f);
+                  const float den = fmaf(z, fmaf(15.f, z, 420.f), 945.f);
+                  v[k] = __float_as_uint(from_cap * __fdividef(y * num, den));
+                }
+              }
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (!((bits >> k) & 1u)) v[k] = 0xff800000u;
+            }
+            tmem_st32(S + c, v);
+          }
+          tmem_wait_st();
         }
-        bool steep = false;            // some score is not small against the cap
-        if (A.cap > 0.f) {
-          steep = __any_sync(0xffffffffu, !(fmaxf(mx, -mn) * to_cap < 0.5f));
-          mx = mx == -INFINITY ? mx : from_cap * tanhf(mx * to_cap);
-        } else {
-          mx *= x2;
+        // ---- the largest score
+#pragma unroll 1
+        for (int c = 0; c < KT; c += 64) {
+          uint32_t v[32], u[32];
+          tmem_get32(S + c, v);
+          tmem_get32(S + c + 32, u);
+          tmem_wait_ld(v);
+          tmem_wait_ld(u);
+          float top[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            top[k & 3] = fmaxf(top[k & 3], fmaxf(__uint_as_float(v[k]), __uint_as_float(u[k])));
+          mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         }
+        mx *= x2;
         // ---- O of the tile before this one: its product had the time of the pass above
         if (!first) fold(t - 2);
         if (__any_sync(0xffffffffu, mx > m + 8.f)) {
@@ -436,29 +489,13 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll 1
         for (int c = 0; c < KT; c += 32) {
-          float v[32];
-          uint32_t x[32];
-          tmem_ld32(S + c, v);
-          if (A.cap > 0.f) {
-            if (steep) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] = from_cap * tanhf(v[k] * to_cap);
-            } else {
-              // Lambert's continued fraction, off by less than 2^-29 of tanh y for |y| < 1/2
-#pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                const float y = v[k] * to_cap, z = y * y;
-                const float num = fmaf(z, z + 105.f, 945.f);
-                const float den = fmaf(z, fmaf(15.f, z, 420.f), 945.f);
-                v[k] = from_cap * __fdividef(y * num, den);
-              }
-            }
-          }
-          hide(v, c / 32);
+          uint32_t v[32], x[32];
+          tmem_get32(S + c, v);
+          tmem_wait_ld(v);
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             float a, b;
-            unpack2(fma2(pack2(v[k], v[k + 1]), x22, shift2), a, b);
+            unpack2(fma2(pack2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), x22, shift2), a, b);
             a = ex2(a);
             b = ex2(b);
             const uint64_t ab = pack2(a, b);
@@ -522,72 +559,73 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     }
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsIssue));
+    // descriptors: rows of 128 bytes, 8 of them 1024 bytes on; of V (MN-major) 64 columns in
+    // a row, the next 64 BLK on
+    const uint32_t desc_hi = (uint32_t)(sw128_desc(smem) >> 32);
     if (warp == 8) {
-      // ---- products
-      const uint64_t dk = sw128_desc(ks), dq = sw128_desc(smem);
-      const uint32_t desc_hi = (uint32_t)(dk >> 32), q_lo = (uint32_t)dq, k_lo = (uint32_t)dk;
-      // V: 64 columns in a line of 128 bytes, 8 keys 1024 bytes on, 64 columns BLK on
-      const uint32_t v_lo = ((smem_u32(vs) >> 4) & 0x3FFF) | (uint32_t)(BLK >> 4) << 16;
-      const uint32_t is = tc_idesc(128, KT) | Cfg::kIdesc16;
-      const uint32_t io = tc_idesc(128, DV) | Cfg::kIdesc16 | (1u << 16);
-      uint32_t pieces = 0;
-      while (run.next(p)) {
-        wait(&sh.q_full, pieces & 1);
-        ++pieces;
-        tc_fence_after();
-        // S runs two tiles ahead of O (one, where keys and values are widened into one stage
-        // each, in turn); S of tile t + 3 takes the place of P of tile t behind the
-        // product that reads it
-        constexpr int AHEAD = NS > 1 ? 2 : 1;
-        for (int i = -AHEAD; i < p.n; ++i) {
-          if (i + AHEAD < p.n) {       // S of tile n + i + AHEAD
-            const int t = n + i + AHEAD, st = t % NS, b = t % 3;
-            wait(&sh.k_full[st], (t / NS) & 1);
-            if (lane < 4) sh.soft_seen[b][lane] = sh.seen[st][lane];
-            __syncwarp();
-            if (lane == 0 && !*(volatile int*)&sh.dead) {
-              tc_fence_after();
-              const uint32_t d = tmem + (uint32_t)(b * KT);
-              const uint32_t kb = k_lo + (uint32_t)(st * Cfg::kK >> 4);
-              bool first = true;
-              for (int k = Cfg::kParts - 1; k >= 0; --k) {
+      // ---- S.  A thread of its own: between a tile's products the issuing thread is busy with
+      // barriers for some 700 cycles, in which the other one's products run (both in one thread
+      // 4600 cycles a tile, XXXX in two)
+      if (lane == 0) {
+        const uint32_t q_lo = (uint32_t)sw128_desc(smem), k_lo = (uint32_t)sw128_desc(ks);
+        const uint32_t is = tc_idesc(128, KT) | Cfg::kIdesc16;
+        uint32_t pieces = 0;
+        while (run.next(p)) {
+          wait(&sh.q_full, pieces++ & 1);
+          for (const int end = n + p.n; n < end; ++n) {
+            const int st = n % NS, b = n % 3;
+            wait(&sh.k_full[st], (n / NS) & 1);
+            if (n >= 3) wait(&sh.p_read[b], (n / 3 - 1) & 1);
+            if (*(volatile int*)&sh.dead) break;
+            tc_fence_after();
+            const uint32_t d = tmem + (uint32_t)(b * KT);
+            const uint32_t kb = k_lo + (uint32_t)(st * Cfg::kK >> 4);
 #pragma unroll
-                for (int c = 0; c < DQ / 16; ++c) {
-                  const uint32_t kc = kb + (uint32_t)(((c >> 2) * BLK + (c & 3) * 32) >> 4);
-                  if (Cfg::kTmemQ && k == 2) {
-                    tc_mma_ts(d, tmem + Cfg::kQCol + 8 * c, kc, desc_hi, is, first ? 0u : 1u);
-                  } else {
-                    const uint32_t a = q_lo + (uint32_t)((k * Cfg::kQPart + (c >> 2) * kPrefixRows * 128 +
-                                                          (c & 3) * 32) >> 4);
-                    tc_mma_lo(d, a, kc, desc_hi, is, first ? 0u : 1u);
-                  }
-                  first = false;
-                }
+            for (int k = Cfg::kParts - 1; k >= 0; --k)
+#pragma unroll
+              for (int c = 0; c < DQ / 16; ++c) {
+                const uint32_t kc = kb + (uint32_t)(((c >> 2) * BLK + (c & 3) * 32) >> 4);
+                const uint32_t more = k < Cfg::kParts - 1 || c > 0;
+                if (Cfg::kTmemQ && k == 2)
+                  tc_mma_ts(d, tmem + Cfg::kQCol + 8 * c, kc, desc_hi, is, more);
+                else
+                  tc_mma_lo(d, q_lo + (uint32_t)((k * Cfg::kQPart + (c >> 2) * kPrefixRows * 128 +
+                                                  (c & 3) * 32) >> 4), kc, desc_hi, is, more);
               }
-              tc_commit(&sh.k_empty[st]);
-              mbar_arrive(&sh.s_full[b]);
-              tc_commit(&sh.s_full[b]);
-            }
+            mbar_arrive(&sh.s_full[b]);
+            tc_commit(&sh.s_full[b]);
+            tc_commit(&sh.k_empty[st]);
+          }
+        }
+        tc_commit(&sh.drain[0]);       // nothing is in flight when the tensor memory goes
+        mbar_wait(&sh.drain[0], 0);
+      }
+    } else if (warp == 11) {
+      // ---- O
+      const uint32_t v_lo = ((smem_u32(vs) >> 4) & 0x3FFF) | (uint32_t)(BLK >> 4) << 16;
+      const uint32_t io = tc_idesc(128, DV) | Cfg::kIdesc16 | (1u << 16);
+      while (run.next(p)) {
+        for (const int end = n + p.n; n < end; ++n) {
+          const int st = n % NS, b = n % 3;
+          warp_wait(&sh.v_full[st], (n / NS) & 1);
+          warp_wait(&sh.p_full[b], (n / 3) & 1);
+          const uint4 seen = sh.seen[n % 8];
+          if ((seen.x & seen.y & seen.z & seen.w) != 0xffffffffu) {
+            // nothing of a row that is not seen counts
+            const uint32_t word[4] = {seen.x, seen.y, seen.z, seen.w};
+#pragma unroll
+            for (int j = 0; j < KT / 32; ++j)
+              if (!((word[j] >> lane) & 1u))
+                for (int c = 0; c < DV / 64 * 8; ++c)
+                  *reinterpret_cast<uint4*>(vs + st * Cfg::kV + (c >> 3) * BLK +
+                                            (32 * j + lane) * 128 + (c & 7) * 16) =
+                      make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
             __syncwarp();
           }
-          if (i >= 0) {                // O of tile n + i
-            const int t = n + i, st = t % NS, b = t % 3;
-            wait(&sh.v_full[st], (t / NS) & 1);
-            uint32_t all = 0xffffffffu;
-#pragma unroll
-            for (int c = 0; c < KT / 32; ++c) all &= sh.soft_seen[b][c];
-            if (all != 0xffffffffu) {  // nothing of a row that is not seen counts
-              for (int r = lane; r < KT; r += 32)
-                if (!((sh.soft_seen[b][r >> 5] >> (r & 31)) & 1u))
-                  for (int c = 0; c < DV / 64 * 8; ++c)
-                    *reinterpret_cast<uint4*>(vs + st * Cfg::kV + (c >> 3) * BLK + r * 128 +
-                                              (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-              fence_proxy_async_smem();
-            }
-            wait(&sh.p_full[b], (t / 3) & 1);
-            if (t > 0) wait(&sh.o_empty, (t - 1) & 1);
-            __syncwarp();
-            if (lane == 0 && !*(volatile int*)&sh.dead) {
+          if (lane == 0) {
+            if (n > 0) wait(&sh.o_empty, (n - 1) & 1);
+            if (!*(volatile int*)&sh.dead) {
               tc_fence_after();
               const uint32_t a = tmem + (uint32_t)(b * KT), d = tmem + Cfg::kOCol;
               const uint32_t vb = v_lo + (uint32_t)(st * Cfg::kV >> 4);
@@ -595,19 +633,19 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
               for (int k = 1; k >= 0; --k)
 #pragma unroll
                 for (int c = 0; c < KT / 16; ++c)
-                  tc_mma_ts(d, a + 32 * (c >> 1) + 16 * k + 8 * (c & 1), vb + (uint32_t)(c * 2048 >> 4),
-                            desc_hi, io, k == 1 && c == 0 ? 0u : 1u);
+                  tc_mma_ts(d, a + 32 * (c >> 1) + 16 * k + 8 * (c & 1),
+                            vb + (uint32_t)(c * 2048 >> 4), desc_hi, io, k == 0 || c > 0);
+              tc_commit(&sh.o_full[n & 1]);
+              tc_commit(&sh.p_read[b]);
               tc_commit(&sh.v_empty[st]);
-              tc_commit(&sh.o_full[t & 1]);
             }
-            __syncwarp();
           }
+          __syncwarp();
         }
-        n += p.n;
       }
-      if (lane == 0) {                 // nothing is in flight when the tensor memory goes
-        tc_commit(&sh.drain);
-        mbar_wait(&sh.drain, 0);
+      if (lane == 0) {
+        tc_commit(&sh.drain[1]);
+        mbar_wait(&sh.drain[1], 0);
       }
     } else if (warp < 11) {
       // ---- loads: q and keys, values
@@ -643,7 +681,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         };
         fetch(p.t0);
         if (keys) {                    // q, once the products of the piece before are done
-          if (n > 0) wait(&sh.k_empty[(n - 1) % NS], ((n - 1) / NS) & 1);
+          if (n > 0) warp_wait(&sh.k_empty[(n - 1) % NS], ((n - 1) / NS) & 1);
           if (lane == 0 && !*(volatile int*)&sh.dead) {
             const int64_t tile = (int64_t)p.head * A.row_tiles + p.ru / Cfg::kHalves;
             mbar_expect_tx(&sh.q_full, Cfg::kQ);
@@ -657,7 +695,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         for (int i = 0; i < p.n; ++i, ++n) {
           const int st = n % RING;
           const uint32_t round = n / RING;
-          if (round > 0) wait(&empty[st], (round - 1) & 1);
+          if (round > 0) warp_wait(&empty[st], (round - 1) & 1);
           if (__any_sync(0xffffffffu, *(volatile int*)&sh.dead)) break;
           uint32_t count = 0, ok[4];
 #pragma unroll
@@ -676,7 +714,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 const uint32_t word = box < 32 ? ok[0] : box < 64 ? ok[1] : box < 96 ? ok[2] : ok[3];
                 if (!((word >> (box & 31)) & 1u)) bits &= ~(1u << k);
               }
-            (E4 ? sh.raw_seen[st] : sh.seen[st])[lane] = bits;
+            (&sh.seen[n % 8].x)[lane] = bits;
           }
           __syncwarp();
           if (lane == 0) mbar_expect_tx(&full[st], (count << shift) * 128u * (uint32_t)lines);
@@ -728,17 +766,15 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       for (int i = 0; i < p.n; ++i, ++n) {
         const int rs = n % R, st = n % NS;
         const uint32_t rr = (n / R) & 1, round = n / NS;
-        wait(&sh.rk_full[rs], rr);
-        if (round > 0) wait(&sh.k_empty[st], (round - 1) & 1);
+        warp_wait(&sh.rk_full[rs], rr);
+        if (round > 0) warp_wait(&sh.k_empty[st], (round - 1) & 1);
         widen(rk + rs * Cfg::kRawK, ks + st * Cfg::kK, DQ);
-        if (id < 4) sh.seen[st][id] = sh.raw_seen[rs][id];
-        __syncwarp();
         if (lane == 0) {
           mbar_arrive(&sh.k_full[st]);
           mbar_arrive(&sh.rk_empty[rs]);
         }
-        wait(&sh.rv_full[rs], rr);
-        if (round > 0) wait(&sh.v_empty[st], (round - 1) & 1);
+        warp_wait(&sh.rv_full[rs], rr);
+        if (round > 0) warp_wait(&sh.v_empty[st], (round - 1) & 1);
         widen(rv + rs * Cfg::kRawV, vs + st * Cfg::kV, DV);
         if (lane == 0) {
           mbar_arrive(&sh.v_full[st]);
