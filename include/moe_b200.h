@@ -544,16 +544,15 @@ int moe_paged_attention_record(const moe_paged_attention_args* args);
 int moe_linear_record(const moe_linear_args* args);
 
 /* ---- a prefix that a batch shares -------------------------------------------------------
- * moe_paged_attention for sequences that all begin with the same `prefix_pages` whole pages
- * (a system prompt, a document): their keys are read and multiplied once, for the rows of all
- * sequences together.
+ * moe_paged_attention for sequences that begin with the same `prefix_pages` whole pages (a system
+ * prompt, a document): their keys are read and multiplied once, for the rows of all sequences
+ * together.
  *   attention: as moe_paged_attention takes them, but for window, which must be 0, and workspace,
  *          whose size is moe_prefix_attention_workspace_bytes.  out 16-byte aligned
- *   prefix (prefix_pages,) int32: the pages.  Entries of the block table for the same tokens
- *          are not read: keys and values of a sequence from prefix_pages * page_size on come
- *          from its row
- *   seq_lens: the prefix included.  0 or less gives zeros in out and -inf in lse.  So does a length
- *          between, which sets MOE_STATUS_BAD_PAGE: every other sequence holds the whole prefix
+ *   prefix (prefix_pages,) int32: the pages, which are also the first ones in the row of the block
+ *          table of each sequence that is as long as the prefix or longer.  (Either may be read.)
+ *          Shorter sequences may have any pages
+ *   seq_lens, max_len: the prefix included
  * prefix_pages 0 is moe_paged_attention.  The split over the GPU depends on sizes alone; equal
  * calls give equal bits. */
 typedef struct moe_prefix_attention_args {

@@ -69,7 +69,7 @@ struct AttArgs {
   int* arrivals;                      // one per CTA
   float2* part_ml;                    // [2 * grid][kAttHeads] (maximum, sum)
   float* part_o;                      // [2 * grid][kAttHeads][DP]
-  int hq, window, from;               // from: keys before it are not seen
+  int hq, window, from;               // sequences of `from` keys or more: without the first `from`
   float scale, cap;
 };
 
@@ -167,7 +167,9 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   // ---- this CTA's run of rounds
   auto keys_of = [&](int s, int& first) {
     const int n = min(max(A.seq_lens[s], 0), most);
-    first = A.window > 0 && n > A.window ? n - A.window : A.from;
+    first = A.window > 0 && n > A.window ? n - A.window
+            : n >= A.from                ? A.from
+                                         : 0;
     return n;
   };
   // rounds start at a multiple of KEYS, so that no box crosses a page's end;
@@ -974,7 +976,7 @@ int check_attention(const moe_paged_attention_args& r, moe_paged_cache& c) {
   return MOE_OK;
 }
 
-// The attention over the keys from `from` on.
+// The attention without the first `from` keys of each sequence that has so many.
 int attention_from(const moe_paged_attention_args& r, int from) {
   AttArgs a = {};
   MOE_CHECK(check_attention(r, a.c));

@@ -53,7 +53,7 @@ struct PrefixArgs {
   float* part_o;                       // [slot][row][column of the unit]
   int rows, row_tiles, keys;           // of a key head, keys of the prefix
   int RU, m, RG, tiles, quota, parts;  // row units, team, row groups; tiles of a head; parts of a unit
-  long long total;                     // tiles of all teams
+  uint32_t total;                      // tiles of all teams
   float cap;
 };
 
@@ -260,24 +260,24 @@ struct PrefixPiece {
 };
 struct PrefixRun {
   const PrefixArgs& A;
-  long long at, end;
+  uint32_t at, end;
   int team, member;
   __device__ explicit PrefixRun(const PrefixArgs& a) : A(a) {
     team = blockIdx.x / A.m;
     member = blockIdx.x - team * A.m;
-    at = (long long)team * A.quota;
+    at = (uint32_t)team * A.quota;
     end = min(A.total, at + A.quota);
   }
   __device__ bool next(PrefixPiece& p) {
     while (at < end) {
-      const int unit = (int)(at / A.tiles);            // head and row group
-      p.t0 = (int)(at - (long long)unit * A.tiles);
-      p.n = (int)min((long long)(A.tiles - p.t0), end - at);
+      const uint32_t unit = at / (uint32_t)A.tiles;    // head and row group
+      p.t0 = (int)(at - unit * A.tiles);
+      p.n = (int)min(A.tiles - p.t0, end - at);
+      const uint32_t first = unit * A.tiles / (uint32_t)A.quota;
       at += p.n;
-      p.head = unit / A.RG;
-      p.ru = (unit - p.head * A.RG) * A.m + member;
-      const int first = (int)((long long)unit * A.tiles / A.quota);
-      p.slot = (unit * A.m + member) * A.parts + team - first;
+      p.head = (int)unit / A.RG;
+      p.ru = ((int)unit - p.head * A.RG) * A.m + member;
+      p.slot = ((int)unit * A.m + member) * A.parts + team - (int)first;
       if (p.ru < A.RU) return true;
     }
     return false;
@@ -564,8 +564,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     const uint32_t desc_hi = (uint32_t)(sw128_desc(smem) >> 32);
     if (warp == 8) {
       // ---- S.  A thread of its own: between a tile's products the issuing thread is busy with
-      // barriers for some 700 cycles, in which the other one's products run (both in one thread
-      // 4600 cycles a tile, XXXX in two)
+      // barriers for some 700 cycles, in which the other one's products run (a tile of
+      // bf16 4600 cycles with both in one thread, 4000 in two)
       if (lane == 0) {
         const uint32_t q_lo = (uint32_t)sw128_desc(smem), k_lo = (uint32_t)sw128_desc(ks);
         const uint32_t is = tc_idesc(128, KT) | Cfg::kIdesc16;
@@ -794,9 +794,8 @@ struct PrefixJoinArgs {
   const float2* part_ml;
   const float* part_o;
   const int32_t* seq_lens;
-  const float* own_lse;                // null: no key behind any prefix
+  const float* own_lse;
   float *out, *lse;
-  int* status;
   int seqs, hq, G, d, DV, halves, keys;
   int RU, m, RG, tiles, quota, parts;
   float v_scale;
@@ -809,12 +808,9 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixJoinArgs A
   const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (id >= (int64_t)A.seqs * A.hq) return;
   const int s = (int)(id / A.hq), h = (int)(id - (int64_t)s * A.hq), head = h / A.G;
-  const int len = A.seq_lens[s];
   float* out = A.out + id * A.d;
-  if (len < A.keys) {                  // padding, or not behind this prefix
-    if (len > 0 && lane == 0) set_status(A.status, MOE_STATUS_BAD_PAGE);
-    for (int c = lane; c < A.d; c += 32) out[c] = 0.f;
-    if (lane == 0 && A.lse) A.lse[id] = -INFINITY;
+  if (A.seq_lens[s] < A.keys) {        // not behind this prefix: all of its keys are its own
+    if (lane == 0 && A.lse) A.lse[id] = A.own_lse[id];
     return;
   }
   const int r = s * A.G + h - head * A.G;
@@ -822,8 +818,8 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixJoinArgs A
   for (int half = 0; half < A.halves; ++half) {
     const int ru = r / kPrefixRows * A.halves + half, row = r % kPrefixRows;
     const int rg = ru / A.m, unit = head * A.RG + rg;
-    const int first = (int)((long long)unit * A.tiles / A.quota);
-    const int n = (int)(((long long)(unit + 1) * A.tiles - 1) / A.quota) - first + 1;
+    const int first = unit * A.tiles / A.quota;
+    const int n = ((unit + 1) * A.tiles - 1) / A.quota - first + 1;
     const int64_t slot = (int64_t)(unit * A.m + ru - rg * A.m) * A.parts;
     const float2* ml = A.part_ml + slot * kPrefixRows + row;
     const float* po = A.part_o + (slot * kPrefixRows + row) * A.DV;
@@ -996,14 +992,15 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
   a.m = p.m;
   a.RG = p.RG;
   a.tiles = (P + p.kt - 1) / p.kt;
-  a.total = (long long)p.units * a.tiles;
-  const long long quota = (a.total + p.teams - 1) / p.teams;
-  MOE_REQUIRE(quota < (1ll << 30) && (int64_t)S * G < (1ll << 30) && p.slots < (1ll << 30),
+  const int64_t total = p.units * a.tiles;
+  const int64_t quota = (total + p.teams - 1) / p.teams;
+  MOE_REQUIRE(total < (1ll << 30) && (int64_t)S * G < (1ll << 30) && p.slots < (1ll << 30),
               MOE_ERR_UNSUPPORTED, "%d sequences behind a prefix of %d tokens are too many", S, P);
+  a.total = (uint32_t)total;
   a.quota = (int)quota;
   a.parts = (a.tiles - 1) / a.quota + 2;
   MOE_REQUIRE(p.units * p.m * a.parts <= p.slots, MOE_ERR_INVALID, "parts %d", a.parts);
-  const int grid = (int)((a.total + quota - 1) / quota) * p.m;
+  const int grid = (int)((total + quota - 1) / quota) * p.m;
   a.cap = t.softcap;
   const int vec = (uintptr_t)t.q % 16 == 0 && (S == 1 || t.q_seq_stride % 4 == 0) &&
                   (t.q_heads == 1 || t.q_head_stride % 4 == 0);
@@ -1023,7 +1020,7 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
   }
   MOE_CHECK(moe::attention_from(own, P));
   const moe::PrefixJoinArgs j = {ws.ml, ws.o, t.seq_lens, ws.lse, t.out, t.lse,
-                                 a.status, S, t.q_heads, G, d, p.dv, p.halves, P, a.RU, a.m, a.RG,
+                                 S, t.q_heads, G, d, p.dv, p.halves, P, a.RU, a.m, a.RG,
                                  a.tiles, a.quota, a.parts, a.c.v_scale};
   {
     ::moe::ProfScope _prof(MOE_K_PREFIX, s);

@@ -561,14 +561,13 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      v_scale: float = 1.0, max_len: int = 0, out: Optional[torch.Tensor] = None,
                      return_lse: bool = False, ws: Optional[torch.Tensor] = None,
                      status: Optional[torch.Tensor] = None):
-    """``paged_attention`` of sequences that all begin with the same whole pages
+    """``paged_attention`` of sequences that begin with the same whole pages
     ``prefix_pages`` (n,) int32 (a system prompt, a document): their keys are
-    read and multiplied once for all rows.  ``seq_lens`` counts the prefix; a
-    sequence is empty (0: zeros and -inf) or holds all of it (a length between
-    counts as empty, and as STATUS_BAD_PAGE).  ``block_table`` is read from the
-    first page behind the prefix on.  ``ws`` comes from
-    ``prefix_attention_workspace``; ``max_len``, ``out``, ``ws`` and ``status`` as
-    in ``paged_attention``."""
+    read and multiplied once for all rows.  ``block_table`` and ``seq_lens``
+    cover whole sequences, the prefix included: the rows of those that are as
+    long as the prefix or longer begin with its pages; shorter ones (0:
+    padding) may have any.  ``ws`` comes from ``prefix_attention_workspace``; all
+    else as in ``paged_attention``, whose result it is but for the last bits."""
     c, dev, seqs, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
     shape = q.shape
     if len(shape) != 3:

@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 
 class Shared:
     """Sequences of `own` tokens of their own behind a prefix of `pages` pages; own 0 with
-    the prefix alone, None a padding row.  The tables do not name the prefix's pages."""
+    the prefix alone, None a padding row."""
 
     def __init__(self, own, pages, page, hkv, d, dtype, layout="nhd", seed=0):
         P = pages * page
@@ -23,7 +23,7 @@ class Shared:
         self.c = c = Cache(lens + [P], page, hkv, d, dtype, layout, seed)
         self.pages = c.table_d[-1, :pages].contiguous()
         self.table = c.table_d[:-1].contiguous()
-        self.table[:, :pages] = -9
+        self.table[:, :pages] = self.pages
         self.lens, self.P = c.lens[:-1].contiguous(), P
         for s, n in enumerate(lens):
             if n:
@@ -75,6 +75,21 @@ def test_prefix(dtype, own, pages, page, hq, hkv, d, layout):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+def test_prefix_longer_than_some(dtype):
+    """A sequence without the whole prefix is computed over the keys that it has."""
+    x = Shared([3, 8, None, 0, 2], 10, 16, 2, 128, dtype)
+    for s, n in ((1, 100), (3, 159), (4, 1)):
+        x.lens[s] = n
+        x.kd[s], x.vd[s] = x.kd[s][:n], x.vd[s][:n]
+    # its pages need not be the prefix's
+    x.table[1, :7] = x.c.table_d[1, :7]
+    x.kd[1], x.vd[1] = (c[x.table[1, :7].long()].flatten(0, 1)[:100].double() * f
+                        for c, f in ((x.c.k, x.c.k_scale), (x.c.v, x.c.v_scale)))
+    q = randn(5, 8, 128)
+    x.check(q, *x.call(q), 128 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
 def test_prefix_many_rows(dtype):
     """More row units than a team has members."""
     own = [s % 3 for s in range(300)]
@@ -114,11 +129,9 @@ def test_prefix_reports():
     x = Shared([3, 8, 2], 10, 16, 2, 128, F16)
     q = randn(3, 8, 128)
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
-    x.lens[1] = 100                                 # not empty, and without the whole prefix
-    x.kd[1], x.vd[1] = x.kd[1][:0], x.vd[1][:0]
-    out, lse = x.call(q, status=status)
+    x.lens[1] = 1 << 30                             # more than the table holds
+    x.call(q, status=status)
     assert status.item() == K.STATUS_BAD_PAGE
-    x.check(q, out, lse, 128 ** -0.5)
     # a prefix page that does not exist is left out
     y = Shared([3, 8, 2], 10, 16, 2, 128, F16)
     for bad, at in ((-1, 2), (10 ** 6, 9)):
