@@ -26,10 +26,13 @@ namespace moe {
 namespace cg = cooperative_groups;
 
 constexpr int kEvictThreads = 256;
+constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictCluster = 8;
 constexpr int kEvictSlots = 20480;     // of a CTA at most: 8 bytes each in shared memory
 constexpr int kDigit = 11;
 constexpr int kBins = 1 << kDigit;
+constexpr int kFew = 8;                // slots that leave one by one
+constexpr int kFewSlots = 32768;
 
 struct EvictArgs {
   moe_paged_cache c;
@@ -44,10 +47,11 @@ struct EvictArgs {
 };
 
 struct EvictShared {
-  int bins[kBins];
+  int bins[2][kBins];
   int scan[33];
   int newest, digit, above;
   int equal, movers, freed;            // of this CTA: keys equal to the limit, movers, slots given up
+  int of_warp[3][kEvictWarps];
 };
 
 // f32 -> u32 of the same order; +-0 are equal, NaN is last
@@ -57,30 +61,203 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs A) {
+// What the CTAs of a (sequence, head) need to know of it.
+struct EvictUnit {
+  const float* mass;
+  const int32_t *held, *table;
+  float* mass_out;
+  int32_t* held_out;
+  int n;                               // 0: nothing to do
+  __device__ EvictUnit(const EvictArgs& A, int unit, int rank) {
+    const int seq = unit / A.c.kv_heads, head = unit - seq * A.c.kv_heads;
+    const int told = max(A.seq_lens[seq], 0);
+    n = told > A.most ? 0 : told;
+    if (head == 0 && rank == 0 && threadIdx.x == 0) {
+      if (told > A.most) set_status(A.status, MOE_STATUS_BAD_PAGE);     // left as it is
+      if (A.apart) A.lens_out[seq] = told > A.most ? told : min(n, A.keep);
+    }
+    mass = A.mass + (int64_t)unit * A.row;
+    held = A.held + (int64_t)unit * A.row;
+    mass_out = A.mass_out + (int64_t)unit * A.row_out;
+    held_out = A.held_out + (int64_t)unit * A.row_out;
+    table = A.c.block_table + (int64_t)seq * A.c.table_stride;
+  }
+  // entries that stay where they are, where the result is another ledger
+  __device__ void copy(int i) const {
+    if (mass_out != mass) mass_out[i] = mass[i];
+    if (held_out != held) held_out[i] = held[i];
+  }
+};
+
+// The rows of up to 32 moves, (from, to) of one in each lane (-1: none), by a warp: 16 bytes a
+// lane, of keys and values, B loads under way.
+struct EvictRows {
+  uint8_t* k;
+  int64_t v_less_k;
+  int lines;                           // 16-byte lines of a row, at most 32
+  uint32_t per_line;                   // i / lines = i * per_line >> 16 for i < 2048
+  __device__ EvictRows(const EvictArgs& A, int head) {
+    const int eb = A.c.dtype == MOE_CACHE_E4M3 ? 1 : 2;
+    k = static_cast<uint8_t*>(A.c.k) + (int64_t)head * A.c.head_stride * eb;
+    v_less_k = (int64_t)((uintptr_t)A.c.v - (uintptr_t)A.c.k);
+    lines = A.c.head_dim * eb / 16;
+    per_line = 65536u / (uint32_t)lines + 1;
+  }
+  // byte offset of a slot's row, -1: its page does not exist
+  __device__ static int64_t at(const EvictArgs& A, const int32_t* table, int slot) {
+    const int p = slot / A.c.page_size, page = table[p];
+    if (page < 0 || page >= A.c.pages) return -1;
+    return ((int64_t)page * A.c.page_stride + (int64_t)(slot - p * A.c.page_size) * A.c.token_stride) *
+           (A.c.dtype == MOE_CACHE_E4M3 ? 1 : 2);
+  }
+  template <int B> __device__ void move(int64_t from, int64_t to, int count, int lane) const {
+    const int items = 2 * count * lines;
+    for (int i0 = lane; i0 - lane < items; i0 += 32 * B) {
+      uint4 v[B];
+      int64_t dst[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const int i = i0 + 32 * b, row = (int)((uint32_t)i * per_line >> 16);
+        const int64_t off = (row & 1 ? v_less_k : 0) + 16 * (i - row * lines);
+        const int64_t f = __shfl_sync(0xffffffffu, from, row / 2 & 31);
+        const int64_t d = __shfl_sync(0xffffffffu, to, row / 2 & 31);
+        dst[b] = i < items && f >= 0 ? d + off : -1;
+        if (dst[b] != -1) v[b] = *reinterpret_cast<const uint4*>(k + f + off);
+      }
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (dst[b] != -1) *reinterpret_cast<uint4*>(k + dst[b]) = v[b];
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Few slots leave (a decode step at the limit): one CTA of a (sequence, head) takes away the
+// smallest key so often.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(kEvictThreads, 6) evict_few_kernel(const EvictArgs A) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint64_t least[2][kEvictWarps];
+  __shared__ int top[kEvictWarps];
+  uint32_t* keys = reinterpret_cast<uint32_t*>(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_trigger();
+  pdl_wait();
+  const EvictUnit U(A, blockIdx.x, 0);
+  const int n = U.n, drop = n - A.keep;
+  int newest = INT32_MIN;
+#pragma unroll 4
+  for (int i = tid; i < n; i += kEvictThreads) {
+    keys[i] = order_key(U.mass[i]);
+    newest = max(newest, U.held[i]);
+  }
+  if (drop <= 0) {
+    for (int i = tid; i < n; i += kEvictThreads) U.copy(i);
+    return;
+  }
+  newest = __reduce_max_sync(0xffffffffu, newest);
+  if (lane == 0) top[warp] = newest;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kEvictWarps; ++w) newest = max(newest, top[w]);
+  const int64_t since = (int64_t)newest - A.recent;
+  // smallest key, of equals the largest slot: the smallest (key, ~slot).  Kept in any case: all
+  // ones, which only slots that are all kept so can be; taken away: never again
+  auto mine = [&]() {
+    uint64_t m = ~0ull;
+#pragma unroll 4
+    for (int i = tid; i < n; i += kEvictThreads) {
+      const uint64_t k = (uint64_t)keys[i] << 32 | (uint32_t)~i;
+      m = k < m ? k : m;
+    }
+    return m;
+  };
+  if (A.recent > 0) {
+#pragma unroll 4
+    for (int i = tid; i < n; i += kEvictThreads)
+      if (U.held[i] > since) keys[i] = 0xffffffffu;
+  }
+  uint64_t m = mine();
+  int gone[kFew];
+#pragma unroll
+  for (int r = 0; r < kFew; ++r) {
+    gone[r] = -1;
+    if (r < drop) {
+      const uint32_t hi = __reduce_min_sync(0xffffffffu, (uint32_t)(m >> 32));
+      const uint32_t lo = __reduce_min_sync(0xffffffffu, (uint32_t)(m >> 32) == hi ? (uint32_t)m : ~0u);
+      if (lane == 0) least[r & 1][warp] = (uint64_t)hi << 32 | lo;
+      __syncthreads();
+      uint64_t all = ~0ull;
+#pragma unroll
+      for (int w = 0; w < kEvictWarps; ++w) all = least[r & 1][w] < all ? least[r & 1][w] : all;
+      gone[r] = (int)~(uint32_t)all;
+      if (gone[r] % kEvictThreads == tid) {      // its thread looks for its next one
+        uint64_t next = ~0ull;
+        for (int i = tid; i < n; i += kEvictThreads) {
+          const uint64_t k = (uint64_t)keys[i] << 32 | (uint32_t)~i;
+          if (k > all && k < next) next = k;
+        }
+        m = next;
+      }
+    }
+  }
+  if (U.mass_out != U.mass || U.held_out != U.held)
+    for (int i = tid; i < A.keep; i += kEvictThreads) {
+      bool left = false;
+#pragma unroll
+      for (int r = 0; r < kFew; ++r) left |= gone[r] == i;
+      if (!left) U.copy(i);
+    }
+  if (warp != 0) return;
+  // lane j: the j-th slot from `keep` on that stays and the j-th below it that leaves
+  int from = -1, to = -1, survivors = 0;
+  for (int i = A.keep; i < n; ++i) {
+    bool left = false;
+#pragma unroll
+    for (int r = 0; r < kFew; ++r) left |= gone[r] == i;
+    if (!left && survivors++ == lane) from = i;
+  }
+#pragma unroll
+  for (int r = 0; r < kFew; ++r) {
+    int rank = 0;                      // of this slot among those that leave below `keep`
+#pragma unroll
+    for (int q = 0; q < kFew; ++q) rank += gone[q] >= 0 && gone[q] < gone[r];
+    if (gone[r] >= 0 && gone[r] < A.keep && rank == lane) to = gone[r];
+  }
+  int64_t src = -1, dst = -1;
+  if (from >= 0) {
+    U.mass_out[to] = U.mass[from];
+    U.held_out[to] = U.held[from];
+    src = EvictRows::at(A, U.table, from);
+    dst = EvictRows::at(A, U.table, to);
+    if (src < 0 || dst < 0) {
+      set_status(A.status, MOE_STATUS_BAD_PAGE);
+      src = dst = -1;
+    }
+  }
+  EvictRows(A, blockIdx.x % A.c.kv_heads).move<2>(src, dst, survivors, lane);
+}
+
+// ---------------------------------------------------------------------------
+// Any number of slots.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(const EvictArgs A) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ EvictShared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int unit = blockIdx.x / C, seq = unit / A.c.kv_heads, head = unit - seq * A.c.kv_heads;
-  const int tid = threadIdx.x, NT = kEvictThreads;
+  const int unit = blockIdx.x / C;
+  const int tid = threadIdx.x, NT = kEvictThreads, lane = tid & 31, warp = tid >> 5;
+  auto meet = [&]() {                  // a CTA alone needs no cluster's barrier
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+  };
   pdl_trigger();
   pdl_wait();
-  const int told = max(A.seq_lens[seq], 0), n = told > A.most ? 0 : told;
-  const bool first = head == 0 && rank == 0 && tid == 0;
-  if (first) {
-    if (told > A.most) set_status(A.status, MOE_STATUS_BAD_PAGE);   // left as it is
-    if (A.apart) A.lens_out[seq] = told > A.most ? told : min(n, A.keep);
-  }
-  const float* mass = A.mass + (int64_t)unit * A.row;
-  const int32_t* held = A.held + (int64_t)unit * A.row;
-  float* mass_out = A.mass_out + (int64_t)unit * A.row_out;
-  int32_t* held_out = A.held_out + (int64_t)unit * A.row_out;
+  const EvictUnit U(A, unit, rank);
+  const int n = U.n;
   if (n <= A.keep) {                   // the same for the whole cluster
-    if (mass_out != mass)
-      for (int i = rank * NT + tid; i < n; i += C * NT) mass_out[i] = mass[i];
-    if (held_out != held)
-      for (int i = rank * NT + tid; i < n; i += C * NT) held_out[i] = held[i];
+    for (int i = rank * NT + tid; i < n; i += C * NT) U.copy(i);
     return;
   }
   const int sl = (n + C - 1) / C, s0 = min(n, rank * sl), cnt = min(n, s0 + sl) - s0;
@@ -88,50 +265,57 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs A)
   int2* list = reinterpret_cast<int2*>(smem + ((4u * (uint32_t)sl + 15u) & ~15u));
 
   // ---- keys
-  if (tid == 0) sh.newest = INT32_MIN;
+  if (tid == 0) {
+    sh.newest = INT32_MIN;
+    sh.equal = sh.movers = sh.freed = 0;
+  }
+  for (int b = tid; b < 2 * kBins; b += NT) (&sh.bins[0][0])[b] = 0;
   __syncthreads();
   int newest = INT32_MIN;
+#pragma unroll 4
   for (int i = tid; i < cnt; i += NT) {
-    newest = max(newest, held[s0 + i]);
-    keys[i] = order_key(mass[s0 + i]);
+    newest = max(newest, U.held[s0 + i]);
+    keys[i] = order_key(U.mass[s0 + i]);
   }
   newest = __reduce_max_sync(0xffffffffu, newest);
-  if (tid % 32 == 0) atomicMax(&sh.newest, newest);
-  cluster.sync();
-  newest = INT32_MIN;
+  if (lane == 0) atomicMax(&sh.newest, newest);
+  meet();
   for (int r = 0; r < C; ++r) newest = max(newest, *cluster.map_shared_rank(&sh.newest, r));
   const int64_t since = (int64_t)newest - A.recent;
   if (A.recent > 0)
+#pragma unroll 4
     for (int i = tid; i < cnt; i += NT)
-      if (held[s0 + i] > since) keys[i] = 0xffffffffu;
+      if (U.held[s0 + i] > since) keys[i] = 0xffffffffu;
 
-  // ---- the keep-th largest key: digits from the top, `want` of those that match so far
+  // ---- the keep-th largest key: digits of 11, 11 and 10 bits, `want` of those that match so far
   uint32_t limit = 0, mask = 0;
   int want = A.keep;
-  for (int shift = 32 - kDigit; ; shift = max(0, shift - kDigit)) {
-    // digits of 11, 11 and 10 bits
-    const int bits = mask == 0 ? kDigit : min(kDigit, __ffs(mask) - 1);
-    const uint32_t low = (1u << bits) - 1;
-    for (int b = tid; b < kBins; b += NT) sh.bins[b] = 0;
-    __syncthreads();
+#pragma unroll 1
+  for (int d = 0; d < 3; ++d) {
+    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
+    const uint32_t low = d == 2 ? 1023u : 2047u;
+    int* bins = sh.bins[d & 1];
     for (int i = tid; i < cnt; i += NT)
-      if ((keys[i] & mask) == limit) atomicAdd(&sh.bins[(keys[i] >> shift) & low], 1);
-    cluster.sync();
+      if ((keys[i] & mask) == limit) atomicAdd(&bins[(keys[i] >> shift) & low], 1);
+    meet();
     // thread tid: 8 digits, from the largest down
     constexpr int PER = kBins / kEvictThreads;
     int sums[PER], mine = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) sums[j] = 0;
-    for (int r = 0; r < C; ++r) {
-      const int4* bins =
-          reinterpret_cast<const int4*>(cluster.map_shared_rank(&sh.bins[0], r) + kBins - PER * (tid + 1));
 #pragma unroll
-      for (int j = 0; j < PER / 4; ++j) {
-        const int4 v = bins[j];
-        sums[4 * j] += v.x;
-        sums[4 * j + 1] += v.y;
-        sums[4 * j + 2] += v.z;
-        sums[4 * j + 3] += v.w;
+    for (int r = 0; r < kEvictCluster; ++r) {
+      if (r < C) {
+        const int4* of = reinterpret_cast<const int4*>(cluster.map_shared_rank(bins, r) + kBins -
+                                                       PER * (tid + 1));
+#pragma unroll
+        for (int j = 0; j < PER / 4; ++j) {
+          const int4 v = of[j];
+          sums[4 * j] += v.x;
+          sums[4 * j + 1] += v.y;
+          sums[4 * j + 2] += v.z;
+          sums[4 * j + 3] += v.w;
+        }
       }
     }
 #pragma unroll
@@ -150,49 +334,55 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs A)
         above += sums[j];
       }
     }
-    cluster.sync();                    // the counts have been read; digit and above are there
+    __syncthreads();
     limit |= (uint32_t)sh.digit << shift;
     mask |= low << shift;
     want -= sh.above;
-    if (shift == 0) break;
+    // the third digit's counts: others read the first ones' before they came to the second
+    // barrier, which is behind us when d is 1
+    if (d == 1)
+      for (int b = tid; b < kBins; b += NT) sh.bins[0][b] = 0;
+    __syncthreads();
   }
-  // kept: keys above the limit, and the first `want` of those equal to it
-
-  // ---- equals in the slices before this one
+  // kept: keys above the limit, and the first `want` of those equal to it.  A warp takes
+  // a contiguous part of the slice, so that its counts need no barrier
   auto count = [&](bool p) { return __popc(__ballot_sync(0xffffffffu, p)); };
-  if (tid == 0) sh.equal = sh.movers = sh.freed = 0;
-  __syncthreads();
-  const int rounds = (cnt + NT - 1) / NT;
-  for (int j = 0; j < rounds; ++j) {
-    const int i = tid + j * NT;
-    const int e = count(i < cnt && keys[i] == limit);
-    if (tid % 32 == 0 && e) atomicAdd(&sh.equal, e);
+  auto before = [&](bool p) {
+    return __popc(__ballot_sync(0xffffffffu, p) & ((1u << lane) - 1));
+  };
+  const int seg = (cnt + NT - 1) / NT * 32, w0 = min(cnt, warp * seg), w1 = min(cnt, w0 + seg);
+  int equals = 0;
+  for (int i = w0 + lane; i - lane < w1; i += 32) equals += count(i < w1 && keys[i] == limit);
+  if (lane == 0) {
+    sh.of_warp[0][warp] = equals;
+    if (equals) atomicAdd(&sh.equal, equals);
   }
-  cluster.sync();
+  meet();
   int equal = 0;
   for (int r = 0; r < rank; ++r) equal += *cluster.map_shared_rank(&sh.equal, r);
+  for (int w = 0; w < warp; ++w) equal += sh.of_warp[0][w];
   // keys become what happens to a slot: 0 nothing, 1 moves away, 2 is filled
-  for (int j = 0; j < rounds; ++j) {
-    const int i = tid + j * NT;
-    const uint32_t k = i < cnt ? keys[i] : 0u;
-    const bool eq = i < cnt && k == limit;
-    int total;
-    const int before = block_excl_scan(eq ? 1 : 0, sh.scan, total);
-    const bool kept = i < cnt && (k > limit || (eq && equal + before < want));
-    equal += total;
-    const bool moves = kept && s0 + i >= A.keep, freed = i < cnt && !kept && s0 + i < A.keep;
-    if (i < cnt) keys[i] = moves ? 1u : freed ? 2u : 0u;
-    if (i < cnt && kept && !moves) {
-      if (mass_out != mass) mass_out[s0 + i] = mass[s0 + i];
-      if (held_out != held) held_out[s0 + i] = held[s0 + i];
-    }
-    const int m = count(moves), f = count(freed);
-    if (tid % 32 == 0) {
-      if (m) atomicAdd(&sh.movers, m);
-      if (f) atomicAdd(&sh.freed, f);
-    }
+  int mv = 0, fr = 0;
+  for (int i = w0 + lane; i - lane < w1; i += 32) {
+    const bool in = i < w1;
+    const uint32_t k = in ? keys[i] : 0u;
+    const bool eq = in && k == limit;
+    const int nth = equal + before(eq);          // every lane votes
+    const bool kept = in && (k > limit || (eq && nth < want));
+    equal += count(eq);
+    const bool moves = kept && s0 + i >= A.keep, freed = in && !kept && s0 + i < A.keep;
+    if (in) keys[i] = moves ? 1u : freed ? 2u : 0u;
+    if (kept && !moves) U.copy(s0 + i);
+    mv += count(moves);
+    fr += count(freed);
   }
-  cluster.sync();
+  if (lane == 0) {
+    sh.of_warp[1][warp] = mv;
+    sh.of_warp[2][warp] = fr;
+    if (mv) atomicAdd(&sh.movers, mv);
+    if (fr) atomicAdd(&sh.freed, fr);
+  }
+  meet();
   int movers = 0, freed = 0, all = 0;
   for (int r = 0; r < C; ++r) {
     const int m = *cluster.map_shared_rank(&sh.movers, r);
@@ -202,74 +392,40 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs A)
     }
     all += m;
   }
-  // ---- mover k and freed slot k meet in the list of CTA k % C
-  for (int j = 0; j < rounds; ++j) {
-    const int i = tid + j * NT;
-    const uint32_t what = i < cnt ? keys[i] : 0u;
-    int total;
-    const int k = block_excl_scan(what == 1u ? 1 : what == 2u ? 1 << 16 : 0, sh.scan, total);
-    if (what == 1u) {
-      const int at = movers + (k & 0xffff);
-      cluster.map_shared_rank(list, at % C)[at / C].x = s0 + i;
-    } else if (what == 2u) {
-      const int at = freed + (k >> 16);
-      cluster.map_shared_rank(list, at % C)[at / C].y = s0 + i;
-    }
-    movers += total & 0xffff;
-    freed += total >> 16;
+  for (int w = 0; w < warp; ++w) {
+    movers += sh.of_warp[1][w];
+    freed += sh.of_warp[2][w];
   }
-  cluster.sync();
+  // ---- mover k and freed slot k meet in the list of CTA k % C
+  for (int i = w0 + lane; i - lane < w1; i += 32) {
+    const uint32_t what = i < w1 ? keys[i] : 0u;
+    const int m = movers + before(what == 1u), f = freed + before(what == 2u);
+    if (what == 1u) cluster.map_shared_rank(list, m % C)[m / C].x = s0 + i;
+    if (what == 2u) cluster.map_shared_rank(list, f % C)[f / C].y = s0 + i;
+    movers += count(what == 1u);
+    freed += count(what == 2u);
+  }
+  meet();
+  // no CTA's shared memory is read or written by others from here on
 
-  // ---- rows: 16 bytes a lane, keys and values
-  const int eb = A.c.dtype == MOE_CACHE_E4M3 ? 1 : 2, ps = A.c.page_size;
-  const int lines = A.c.head_dim * eb / 16;                  // of a row, at most 32
-  const int32_t* table = A.c.block_table + (int64_t)seq * A.c.table_stride;
+  // ---- a warp takes 32 moves: each lane finds the rows of one, then the rows go over
+  const EvictRows rows(A, unit % A.c.kv_heads);
   const int mine = all > rank ? (all - rank + C - 1) / C : 0;
-  uint8_t* kc = static_cast<uint8_t*>(A.c.k) + (int64_t)head * A.c.head_stride * eb;
-  const int64_t v_less_k = (int64_t)((uintptr_t)A.c.v - (uintptr_t)A.c.k);
-  const uint32_t per_line = 65536u / (uint32_t)lines + 1;    // i / lines = i * per_line >> 16, i < 2048
-  auto row_of = [&](int slot) -> int64_t {
-    const int p = slot / ps, page = table[p];
-    if (page < 0 || page >= A.c.pages) return -1;
-    return ((int64_t)page * A.c.page_stride + (int64_t)(slot - p * ps) * A.c.token_stride) * eb;
-  };
-  // a warp takes 32 moves: each lane finds the rows of one, then the rows go over
-  // several at a time
-  const int lane = tid % 32, warps = NT / 32;
-  for (int m0 = tid / 32 * 32; m0 < mine; m0 += warps * 32) {
+  for (int m0 = warp * 32; m0 < mine; m0 += NT) {
     int64_t from = -1, to = -1;
     if (m0 + lane < mine) {
-      const int2 mv = list[m0 + lane];
-      mass_out[mv.y] = mass[mv.x];
-      held_out[mv.y] = held[mv.x];
-      from = row_of(mv.x);
-      to = row_of(mv.y);
+      const int2 m = list[m0 + lane];
+      U.mass_out[m.y] = U.mass[m.x];
+      U.held_out[m.y] = U.held[m.x];
+      from = EvictRows::at(A, U.table, m.x);
+      to = EvictRows::at(A, U.table, m.y);
       if (from < 0 || to < 0) {
         set_status(A.status, MOE_STATUS_BAD_PAGE);
         from = to = -1;
       }
     }
-    const int items = 2 * min(32, mine - m0) * lines;
-    constexpr int B = 8;                                     // loads under way
-    for (int i0 = lane; i0 - lane < items; i0 += 32 * B) {
-      uint4 v[B];
-      int64_t dst[B];
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-        const int i = i0 + 32 * b, row = (int)((uint32_t)i * per_line >> 16);
-        const int64_t off = (row & 1 ? v_less_k : 0) + 16 * (i - row * lines);
-        const int64_t f = __shfl_sync(0xffffffffu, from, row / 2 & 31);
-        const int64_t d = __shfl_sync(0xffffffffu, to, row / 2 & 31);
-        dst[b] = i < items && f >= 0 ? d + off : -1;
-        if (dst[b] != -1) v[b] = *reinterpret_cast<const uint4*>(kc + f + off);
-      }
-#pragma unroll
-      for (int b = 0; b < B; ++b)
-        if (dst[b] != -1) *reinterpret_cast<uint4*>(kc + dst[b]) = v[b];
-    }
+    rows.move<8>(from, to, min(32, mine - m0), lane);
   }
-  // no CTA ends while others may still read its shared memory: the last such
-  // reads and writes were before the barrier in front of the rows
 }
 
 __global__ void evict_lens_kernel(int32_t* lens, int seqs, int keep, int most) {
@@ -286,6 +442,17 @@ static bool overlap(const void* a, int64_t n, const void* b, int64_t m) {
 }
 
 static int launch_evict(EvictArgs& a, cudaStream_t s) {
+  const int64_t blocks = (int64_t)a.c.seqs * a.c.kv_heads;
+  // what sequences of max_len slots lose at most
+  if (a.most - a.keep <= kFew && a.most <= kFewSlots) {
+    MOE_REQUIRE(blocks <= 0x7fffffff, MOE_ERR_UNSUPPORTED, "%d sequences are too many", a.c.seqs);
+    const size_t bytes = (size_t)std::max(4 * a.most, 16);
+    if (bytes > 40 * 1024)
+      MOE_CUDA(cudaFuncSetAttribute(evict_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    4 * kFewSlots));
+    MOE_CUDA(launch_pdl(evict_few_kernel, dim3((unsigned)blocks), dim3(kEvictThreads), bytes, s, a));
+    return MOE_OK;
+  }
   // More CTAs for a head while the GPU is not full and a CTA would have a thousand
   // slots or more (the barriers of a cluster cost more than counting fewer)
   const int64_t units = (int64_t)a.c.seqs * a.c.kv_heads;

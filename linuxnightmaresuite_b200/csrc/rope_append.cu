@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "paged_cache.cuh"
 
@@ -225,18 +226,18 @@ struct NormArgs {
 };
 
 constexpr int kRowsAhead = 3;
+constexpr int kNormThreads = 128;
 
 template <int VEC, int M>
 struct NormRow {
   Elems<VEC> a[M], b[M];
 };
 
-template <int DT, int VEC, int GL>
-__global__ void __launch_bounds__(kRopeThreads) norm_append_kernel(const RopeArgs A, const NormArgs N) {
+// M items of a lane; PAIRS: an item of the rotation is two loads
+template <int DT, int VEC, int GL, int M, bool PAIRS>
+__global__ void __launch_bounds__(kNormThreads) norm_append_kernel(const RopeArgs A, const NormArgs N) {
   using T = typename CacheType<DT>::T;
-  constexpr int M = VEC == 4 ? 2 : 8;  // items of a lane
   __shared__ float2 cs[kMaxHeadDim / 2];
-  __shared__ float ws[2][kMaxHeadDim];
   __shared__ int64_t sh_slot;
   pdl_trigger();
   pdl_wait();
@@ -245,30 +246,23 @@ __global__ void __launch_bounds__(kRopeThreads) norm_append_kernel(const RopeArg
   const int at = N.slots ? N.slots[t] : pos;
   if (pos < 0 || at < 0) return;
   const int hk = A.c.kv_heads, d = A.c.head_dim, nr = A.nr, ni = A.ni, nv = A.nv;
-  const int h = A.rot / 2, rows = A.hq + 2 * hk;
-  const int gl = threadIdx.x % GL, groups = blockDim.x / GL;
-  const int g0 = blockIdx.y * groups + threadIdx.x / GL, step = gridDim.y * groups;
-
-  auto first_of = [&](int i) { return i < nr ? i * VEC * (VEC == 1 && A.interleaved ? 2 : 1)
-                                              : A.rot + (i - nr) * VEC; };
-  const bool pairs = !A.interleaved || VEC == 1;       // an item of the rotation is two loads
+  const int h = A.rot / 2, rows = A.hq + hk;
+  constexpr int GROUPS = kNormThreads / GL;
+  const int gl = threadIdx.x % GL;
+  const int g0 = blockIdx.y * GROUPS + threadIdx.x / GL, step = gridDim.y * GROUPS;
   const int apart = A.interleaved ? 1 : h;
+  auto first_of = [&](int i) {
+    return i < nr ? i * VEC * (VEC == 1 && A.interleaved ? 2 : 1) : A.rot + (i - nr) * VEC;
+  };
   auto fetch = [&](int row, NormRow<VEC, M>& r) {
     if (row >= rows) return;
-    const bool value = row >= A.hq + hk;
     const float* src = row < A.hq ? A.q + t * A.q_ts + row * A.q_hs
-                       : value    ? A.v + t * A.v_ts + (row - A.hq - hk) * A.v_hs
                                   : A.k + t * A.k_ts + (row - A.hq) * A.k_hs;
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      const int i = gl + m * GL;
-      if (value) {
-        if (i < nv) r.a[m] = load_elems<VEC>(src + i * VEC);
-      } else if (i < ni) {
-        const int e = first_of(i);
-        r.a[m] = load_elems<VEC>(src + e);
-        if (i < nr && pairs) r.b[m] = load_elems<VEC>(src + e + apart);
-      }
+      const int i = gl + m * GL, e = first_of(i);
+      if (i < ni) r.a[m] = load_elems<VEC>(src + e);
+      if (PAIRS && i < nr) r.b[m] = load_elems<VEC>(src + e + apart);
     }
   };
   NormRow<VEC, M> ahead[kRowsAhead];
@@ -293,19 +287,29 @@ __global__ void __launch_bounds__(kRopeThreads) norm_append_kernel(const RopeArg
         N.held[e] = pos;
       }
   }
-  for (int i = threadIdx.x; i < h; i += blockDim.x) cs[i] = rope_cos_sin(pos, A.inv_freq[i]);
-  for (int i = threadIdx.x; i < d; i += blockDim.x) {
-    if (N.q_norm) ws[0][i] = N.plus + N.q_norm[i];
-    if (N.k_norm) ws[1][i] = N.plus + N.k_norm[i];
+  for (int i = threadIdx.x; i < h; i += kNormThreads) cs[i] = rope_cos_sin(pos, A.inv_freq[i]);
+  // the weights of this lane's elements, the same for all of its rows
+  Elems<VEC> wa[2][M], wb[2][M];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const float* w = c ? N.k_norm : N.q_norm;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int i = gl + m * GL, e = first_of(i);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        wa[c][m].v[k] = w && i < ni ? N.plus + w[e + k] : 0.f;
+        wb[c][m].v[k] = w && PAIRS && i < nr ? N.plus + w[e + apart + k] : 0.f;
+      }
+    }
   }
   __syncthreads();
   const int64_t slot = sh_slot;
 
   auto finish = [&](int row, NormRow<VEC, M>& r) {
-    const bool is_q = row < A.hq, value = row >= A.hq + hk;
-    const float* w = is_q ? (N.q_norm ? ws[0] : nullptr) : (!value && N.k_norm ? ws[1] : nullptr);
+    const bool is_q = row < A.hq, normed = is_q ? N.q_norm != nullptr : N.k_norm != nullptr;
     float inv = 1.f;
-    if (w) {                                     // the same for all lanes of a group
+    if (normed) {                                // the same for all lanes of a group
       float ss = 0.f;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
@@ -313,9 +317,10 @@ __global__ void __launch_bounds__(kRopeThreads) norm_append_kernel(const RopeArg
         if (i < ni) {
 #pragma unroll
           for (int k = 0; k < VEC; ++k) ss = fmaf(r.a[m].v[k], r.a[m].v[k], ss);
-          if (i < nr && pairs)
+        }
+        if (PAIRS && i < nr) {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) ss = fmaf(r.b[m].v[k], r.b[m].v[k], ss);
+          for (int k = 0; k < VEC; ++k) ss = fmaf(r.b[m].v[k], r.b[m].v[k], ss);
         }
       }
       const uint32_t mask = GL == 32 ? 0xffffffffu
@@ -324,28 +329,23 @@ __global__ void __launch_bounds__(kRopeThreads) norm_append_kernel(const RopeArg
       for (int o = GL / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
       inv = 1.f / sqrtf(ss / (float)d + N.eps);
     }
-    const int j = is_q ? row : value ? row - A.hq - hk : row - A.hq;
-    float* qo = is_q ? A.q_out + t * A.qo_ts + j * A.qo_hs : nullptr;
-    T* co = is_q ? nullptr
-                 : static_cast<T*>(value ? A.c.v : A.c.k) + slot + (int64_t)j * A.c.head_stride;
     if (!is_q && slot < 0) return;
+    float* qo = is_q ? A.q_out + t * A.qo_ts + row * A.qo_hs : nullptr;
+    T* co = is_q ? nullptr
+                 : static_cast<T*>(A.c.k) + slot + (int64_t)(row - A.hq) * A.c.head_stride;
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       const int i = gl + m * GL;
-      if (i >= (value ? nv : ni)) continue;
-      if (value) {
-        store_cache<VEC>(co + i * VEC, r.a[m], A.c.v_scale);
-        continue;
-      }
+      if (i >= ni) continue;
       const int e0 = first_of(i);
-      const bool two = i < nr && pairs;
+      const bool two = PAIRS && i < nr;
       Elems<VEC> a = r.a[m], b = r.b[m];
-      if (w) {
+      if (normed) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) a.v[k] = a.v[k] * inv * w[e0 + k];
-        if (two)
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) b.v[k] = b.v[k] * inv * w[e0 + apart + k];
+        for (int k = 0; k < VEC; ++k) {
+          a.v[k] = a.v[k] * inv * (is_q ? wa[0][m].v[k] : wa[1][m].v[k]);
+          if (PAIRS) b.v[k] = b.v[k] * inv * (is_q ? wb[0][m].v[k] : wb[1][m].v[k]);
+        }
       }
       if (two) {
 #pragma unroll
@@ -380,6 +380,16 @@ __global__ void __launch_bounds__(kRopeThreads) norm_append_kernel(const RopeArg
       fetch(row + (k + kRowsAhead) * step, ahead[k]);
     }
   }
+  // ---- values: copied
+  if (slot < 0) return;
+  const int total = hk * nv, every = gridDim.y * kNormThreads;
+  T* to = static_cast<T*>(A.c.v) + slot;
+#pragma unroll 2
+  for (int it = blockIdx.y * kNormThreads + threadIdx.x; it < total; it += every) {
+    const int j = nv == 1 ? it : (int)__umulhi((uint32_t)it, A.mv), e = (it - j * nv) * VEC;
+    store_cache<VEC>(to + (int64_t)j * A.c.head_stride + e,
+                     load_elems<VEC>(A.v + t * A.v_ts + j * A.v_hs + e), A.c.v_scale);
+  }
 }
 
 template <int DT>
@@ -395,16 +405,22 @@ static int launch_norm_append(RopeArgs& a, const NormArgs& n, int T, cudaStream_
     a.ni = a.nr + (d - a.rot);
     a.nv = d;
   }
-  // lanes of a row: two items each at most (eight single elements)
-  const int gl = !vec || d > 128 ? 32 : d > 64 ? 16 : 8;
-  auto kern = !vec       ? norm_append_kernel<DT, 1, 32>
-              : gl == 32 ? norm_append_kernel<DT, 4, 32>
-              : gl == 16 ? norm_append_kernel<DT, 4, 16>
-                         : norm_append_kernel<DT, 4, 8>;
-  const int rows = a.hq + 2 * a.c.kv_heads;
-  const int threads = T > 8 * sm_count() ? 128 : kRopeThreads;
-  const int parts = std::max(1, std::min(sm_count() / T, rows * gl / threads));
-  MOE_CUDA(launch_pdl(kern, dim3((unsigned)T, (unsigned)parts), dim3((unsigned)threads), 0, s, a, n));
+  a.mv = 0xffffffffu / (uint32_t)a.nv + 1;
+  // lanes of a row: one item each where 32 are enough
+  const bool pairs = !a.interleaved || !vec;
+  const int gl = !vec || a.ni > 16 ? 32 : a.ni > 8 ? 16 : 8;
+  auto pick = [&](auto p) {
+    constexpr bool P = decltype(p)::value;
+    return !vec        ? norm_append_kernel<DT, 1, 32, 8, true>
+           : a.ni > 32 ? norm_append_kernel<DT, 4, 32, 2, P>
+           : gl == 32  ? norm_append_kernel<DT, 4, 32, 1, P>
+           : gl == 16  ? norm_append_kernel<DT, 4, 16, 1, P>
+                       : norm_append_kernel<DT, 4, 8, 1, P>;
+  };
+  auto kern = pairs ? pick(std::true_type{}) : pick(std::false_type{});
+  const int rows = a.hq + a.c.kv_heads;
+  const int parts = std::max(1, std::min(sm_count() / T, rows * gl / kNormThreads));
+  MOE_CUDA(launch_pdl(kern, dim3((unsigned)T, (unsigned)parts), dim3(kNormThreads), 0, s, a, n));
   return MOE_OK;
 }
 
