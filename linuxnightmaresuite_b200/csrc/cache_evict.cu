@@ -8,14 +8,13 @@
 //
 // A cluster of up to 8 CTAs owns a (sequence, head); CTA r has the slots r sl .. (r + 1) sl in
 // shared memory, as 32-bit keys whose order is that of the masses (kept in any case: all ones).
-// The keep-th largest key comes from a radix select, 11 + 11 + 10 bits: counts in
-// shared memory, added up across the cluster, and the digit found by a scan.  (The first
-// digit holds sign, exponent and two bits: masses differ by powers of two, and 8-bit digits
-// would put nearly all of them into four counters.)  Then the movers' numbers are
-// prefix sums; CTA k % C gets mover k in a list and copies its rows, 16 bytes a lane.
+// The keep-th largest key comes from a radix select of four digits: counts in
+// shared memory, added up across the cluster, and the digit found by a scan.  Then the movers'
+// numbers are prefix sums; CTA k % C gets mover k in a list and copies its rows, 16 bytes a
+// lane.  Where few slots leave, one CTA takes them one by one.
 //
-// Bound by latency where few slots leave (the digits' three rounds), by memory where long
-// prompts are cut: the rows that move, read and written once.
+// Bound by latency where few slots leave, by memory where long prompts are cut: the rows that
+// move, read and written once.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -29,8 +28,7 @@ constexpr int kEvictThreads = 256;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictCluster = 8;
 constexpr int kEvictSlots = 20480;     // of a CTA at most: 8 bytes each in shared memory
-constexpr int kDigit = 11;
-constexpr int kBins = 1 << kDigit;
+constexpr int kBins = 256;             // a thread each
 constexpr int kFew = 8;                // slots that leave one by one
 constexpr int kFewSlots = 32768;
 
@@ -47,7 +45,7 @@ struct EvictArgs {
 };
 
 struct EvictShared {
-  int bins[2][kBins];
+  int bins[4][kBins];
   int scan[33];
   int newest, digit, above;
   int equal, movers, freed;            // of this CTA: keys equal to the limit, movers, slots given up
@@ -269,7 +267,8 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(const EvictArgs
     sh.newest = INT32_MIN;
     sh.equal = sh.movers = sh.freed = 0;
   }
-  for (int b = tid; b < 2 * kBins; b += NT) (&sh.bins[0][0])[b] = 0;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) sh.bins[d][tid] = 0;
   __syncthreads();
   int newest = INT32_MIN;
 #pragma unroll 4
@@ -287,61 +286,34 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(const EvictArgs
     for (int i = tid; i < cnt; i += NT)
       if (U.held[s0 + i] > since) keys[i] = 0xffffffffu;
 
-  // ---- the keep-th largest key: digits of 11, 11 and 10 bits, `want` of those that match so far
+  // ---- the keep-th largest key: digits of 8 bits, `want` of those that match so far.  (Digits of
+  // 11 bits take one round less, but every CTA reads the others' counts, and 64 KB of those
+  // through the cluster's network took 10 us a round)
   uint32_t limit = 0, mask = 0;
   int want = A.keep;
 #pragma unroll 1
-  for (int d = 0; d < 3; ++d) {
-    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
-    const uint32_t low = d == 2 ? 1023u : 2047u;
-    int* bins = sh.bins[d & 1];
+  for (int d = 0; d < 4; ++d) {
+    const int shift = 24 - 8 * d;
+    int* bins = sh.bins[d];
+#pragma unroll 4
     for (int i = tid; i < cnt; i += NT)
-      if ((keys[i] & mask) == limit) atomicAdd(&bins[(keys[i] >> shift) & low], 1);
+      if ((keys[i] & mask) == limit) atomicAdd(&bins[(keys[i] >> shift) & 255u], 1);
     meet();
-    // thread tid: 8 digits, from the largest down
-    constexpr int PER = kBins / kEvictThreads;
-    int sums[PER], mine = 0;
+    const int digit = kBins - 1 - tid;           // thread 0: the largest
+    int mine = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) sums[j] = 0;
-#pragma unroll
-    for (int r = 0; r < kEvictCluster; ++r) {
-      if (r < C) {
-        const int4* of = reinterpret_cast<const int4*>(cluster.map_shared_rank(bins, r) + kBins -
-                                                       PER * (tid + 1));
-#pragma unroll
-        for (int j = 0; j < PER / 4; ++j) {
-          const int4 v = of[j];
-          sums[4 * j] += v.x;
-          sums[4 * j + 1] += v.y;
-          sums[4 * j + 2] += v.z;
-          sums[4 * j + 3] += v.w;
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) mine += sums[j];
+    for (int r = 0; r < kEvictCluster; ++r)
+      if (r < C) mine += *cluster.map_shared_rank(&bins[digit], r);
     int total;
-    int above = block_excl_scan(mine, sh.scan, total);
+    const int above = block_excl_scan(mine, sh.scan, total);
     if (above < want && above + mine >= want) {
-      bool found = false;
-#pragma unroll
-      for (int j = PER - 1; j >= 0; --j) {
-        if (!found && above + sums[j] >= want) {
-          found = true;
-          sh.digit = kBins - PER * (tid + 1) + j;
-          sh.above = above;
-        }
-        above += sums[j];
-      }
+      sh.digit = digit;
+      sh.above = above;
     }
     __syncthreads();
     limit |= (uint32_t)sh.digit << shift;
-    mask |= low << shift;
+    mask |= 255u << shift;
     want -= sh.above;
-    // the third digit's counts: others read the first ones' before they came to the second
-    // barrier, which is behind us when d is 1
-    if (d == 1)
-      for (int b = tid; b < kBins; b += NT) sh.bins[0][b] = 0;
     __syncthreads();
   }
   // kept: keys above the limit, and the first `want` of those equal to it.  A warp takes

@@ -228,14 +228,24 @@ struct NormArgs {
 constexpr int kRowsAhead = 3;
 constexpr int kNormThreads = 128;
 
-template <int VEC, int M>
+template <int VEC>
 struct NormRow {
-  Elems<VEC> a[M], b[M];
+  Elems<VEC> a, b;
 };
 
-// M items of a lane; PAIRS: an item of the rotation is two loads
+// The factors of a lane's item for all rows of a token: with a norm's weights w, or 1,
+//   (x0, x1) -> (x0 w0 cos - x1 w1 sin, x1 w1 cos + x0 w0 sin) / norm,
+// pair k in (k, VEC + k) of a and b, or adjacent ones of a; without a turn cos 1, sin 0.
+template <int VEC, bool PAIRS>
+struct NormFactors {
+  float c0[VEC], s1[VEC], c1[VEC], s0[VEC];      // w0 cos, w1 sin, w1 cos, w0 sin
+};
+
+// Items of a lane: one, or (M > 1, a row of 16 lanes would be too few) M; PAIRS: an item of
+// the rotation is two loads
 template <int DT, int VEC, int GL, int M, bool PAIRS>
-__global__ void __launch_bounds__(kNormThreads) norm_append_kernel(const RopeArgs A, const NormArgs N) {
+__global__ void __launch_bounds__(kNormThreads, M == 1 ? 7 : 3)
+norm_append_kernel(const RopeArgs A, const NormArgs N) {
   using T = typename CacheType<DT>::T;
   __shared__ float2 cs[kMaxHeadDim / 2];
   __shared__ int64_t sh_slot;
@@ -246,28 +256,31 @@ __global__ void __launch_bounds__(kNormThreads) norm_append_kernel(const RopeArg
   const int at = N.slots ? N.slots[t] : pos;
   if (pos < 0 || at < 0) return;
   const int hk = A.c.kv_heads, d = A.c.head_dim, nr = A.nr, ni = A.ni, nv = A.nv;
-  const int h = A.rot / 2, rows = A.hq + hk;
+  const int h = A.rot / 2;
   constexpr int GROUPS = kNormThreads / GL;
+  constexpr int HALF = VEC > 1 ? VEC / 2 : 1;    // adjacent pairs of an item
   const int gl = threadIdx.x % GL;
   const int g0 = blockIdx.y * GROUPS + threadIdx.x / GL, step = gridDim.y * GROUPS;
   const int apart = A.interleaved ? 1 : h;
   auto first_of = [&](int i) {
     return i < nr ? i * VEC * (VEC == 1 && A.interleaved ? 2 : 1) : A.rot + (i - nr) * VEC;
   };
-  auto fetch = [&](int row, NormRow<VEC, M>& r) {
+  const float* const qp = A.q + t * A.q_ts;
+  const float* const kp = A.k + t * A.k_ts;
+  // q's rows, then k's, group by group
+  auto fetch = [&](int row, const float* base, int64_t hs, int rows, NormRow<VEC> (&r)[M]) {
     if (row >= rows) return;
-    const float* src = row < A.hq ? A.q + t * A.q_ts + row * A.q_hs
-                                  : A.k + t * A.k_ts + (row - A.hq) * A.k_hs;
+    const float* src = base + row * hs;
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       const int i = gl + m * GL, e = first_of(i);
-      if (i < ni) r.a[m] = load_elems<VEC>(src + e);
-      if (PAIRS && i < nr) r.b[m] = load_elems<VEC>(src + e + apart);
+      if (i < ni) r[m].a = load_elems<VEC>(src + e);
+      if (PAIRS && i < nr) r[m].b = load_elems<VEC>(src + e + apart);
     }
   };
-  NormRow<VEC, M> ahead[kRowsAhead];
+  NormRow<VEC> ahead[kRowsAhead][M];
 #pragma unroll
-  for (int k = 0; k < kRowsAhead; ++k) fetch(g0 + k * step, ahead[k]);
+  for (int k = 0; k < kRowsAhead; ++k) fetch(g0 + k * step, qp, A.q_hs, A.hq, ahead[k]);
 
   if (threadIdx.x == blockDim.x - 1) {           // the token's slot in both caches, -1: none
     const int seq = A.seq_ids ? A.seq_ids[t] : t, n = at / A.c.page_size;
@@ -288,102 +301,132 @@ __global__ void __launch_bounds__(kNormThreads) norm_append_kernel(const RopeArg
       }
   }
   for (int i = threadIdx.x; i < h; i += kNormThreads) cs[i] = rope_cos_sin(pos, A.inv_freq[i]);
-  // the weights of this lane's elements, the same for all of its rows
-  Elems<VEC> wa[2][M], wb[2][M];
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const float* w = c ? N.k_norm : N.q_norm;
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const int i = gl + m * GL, e = first_of(i);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        wa[c][m].v[k] = w && i < ni ? N.plus + w[e + k] : 0.f;
-        wb[c][m].v[k] = w && PAIRS && i < nr ? N.plus + w[e + apart + k] : 0.f;
-      }
-    }
-  }
   __syncthreads();
   const int64_t slot = sh_slot;
 
-  auto finish = [&](int row, NormRow<VEC, M>& r) {
-    const bool is_q = row < A.hq, normed = is_q ? N.q_norm != nullptr : N.k_norm != nullptr;
+  NormFactors<VEC, PAIRS> f[M];
+  auto factors = [&](const float* w) {
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int i = gl + m * GL, e = first_of(i);
+      auto weight = [&](int x) { return w ? N.plus + w[x] : 1.f; };
+      if (PAIRS) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const float2 c = i < nr ? cs[A.interleaved ? e / 2 : e + k] : make_float2(1.f, 0.f);
+          const float w0 = i < ni ? weight(e + k) : 0.f, w1 = i < nr ? weight(e + apart + k) : 0.f;
+          f[m].c0[k] = w0 * c.x;
+          f[m].s1[k] = w1 * c.y;
+          f[m].c1[k] = w1 * c.x;
+          f[m].s0[k] = w0 * c.y;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < HALF; ++k) {
+          const float2 c = i < nr ? cs[e / 2 + k] : make_float2(1.f, 0.f);
+          const float w0 = i < ni ? weight(e + 2 * k) : 0.f;
+          const float w1 = i < ni ? weight(e + 2 * k + 1) : 0.f;
+          f[m].c0[k] = w0 * c.x;
+          f[m].s1[k] = w1 * c.y;
+          f[m].c1[k] = w1 * c.x;
+          f[m].s0[k] = w0 * c.y;
+        }
+      }
+    }
+  };
+  const float per = 1.f / (float)d;
+  // the sum of squares is the same for all lanes of a group
+  auto turn = [&](NormRow<VEC> (&r)[M], bool normed) {
     float inv = 1.f;
-    if (normed) {                                // the same for all lanes of a group
+    if (normed) {
       float ss = 0.f;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         const int i = gl + m * GL;
         if (i < ni) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) ss = fmaf(r.a[m].v[k], r.a[m].v[k], ss);
+          for (int k = 0; k < VEC; ++k) ss = fmaf(r[m].a.v[k], r[m].a.v[k], ss);
         }
         if (PAIRS && i < nr) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) ss = fmaf(r.b[m].v[k], r.b[m].v[k], ss);
+          for (int k = 0; k < VEC; ++k) ss = fmaf(r[m].b.v[k], r[m].b.v[k], ss);
         }
       }
       const uint32_t mask = GL == 32 ? 0xffffffffu
                                      : ((1u << GL % 32) - 1u) << (threadIdx.x % 32 / GL * GL);
 #pragma unroll
       for (int o = GL / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-      inv = 1.f / sqrtf(ss / (float)d + N.eps);
+      inv = 1.f / sqrtf(fmaf(ss, per, N.eps));
     }
-    if (!is_q && slot < 0) return;
-    float* qo = is_q ? A.q_out + t * A.qo_ts + row * A.qo_hs : nullptr;
-    T* co = is_q ? nullptr
-                 : static_cast<T*>(A.c.k) + slot + (int64_t)(row - A.hq) * A.c.head_stride;
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       const int i = gl + m * GL;
-      if (i >= ni) continue;
-      const int e0 = first_of(i);
-      const bool two = PAIRS && i < nr;
-      Elems<VEC> a = r.a[m], b = r.b[m];
-      if (normed) {
+      if (PAIRS) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          a.v[k] = a.v[k] * inv * (is_q ? wa[0][m].v[k] : wa[1][m].v[k]);
-          if (PAIRS) b.v[k] = b.v[k] * inv * (is_q ? wb[0][m].v[k] : wb[1][m].v[k]);
+          const float x0 = r[m].a.v[k] * inv, x1 = i < nr ? r[m].b.v[k] * inv : 0.f;
+          r[m].a.v[k] = i < nr ? fmaf(x0, f[m].c0[k], -x1 * f[m].s1[k]) : x0 * f[m].c0[k];
+          r[m].b.v[k] = fmaf(x1, f[m].c1[k], x0 * f[m].s0[k]);
         }
-      }
-      if (two) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const float2 c = cs[A.interleaved ? e0 / 2 : e0 + k];
-          const float x0 = a.v[k], x1 = b.v[k];
-          a.v[k] = fmaf(x0, c.x, -x1 * c.y);
-          b.v[k] = fmaf(x1, c.x, x0 * c.y);
-        }
-      } else if (i < nr) {
-#pragma unroll
-        for (int k = 0; k + 1 < VEC; k += 2) {
-          const float2 c = cs[(e0 + k) / 2];
-          const float x0 = a.v[k], x1 = a.v[k + 1];
-          a.v[k] = fmaf(x0, c.x, -x1 * c.y);
-          a.v[k + 1] = fmaf(x1, c.x, x0 * c.y);
-        }
-      }
-      if (is_q) {
-        store_f32<VEC>(qo + e0, a);
-        if (two) store_f32<VEC>(qo + e0 + apart, b);
       } else {
-        store_cache<VEC>(co + e0, a, A.c.k_scale);
-        if (two) store_cache<VEC>(co + e0 + apart, b, A.c.k_scale);
+#pragma unroll
+        for (int k = 0; k < HALF; ++k) {
+          const float x0 = r[m].a.v[2 * k] * inv, x1 = r[m].a.v[(2 * k + 1) % VEC] * inv;
+          r[m].a.v[2 * k] = i < nr ? fmaf(x0, f[m].c0[k], -x1 * f[m].s1[k]) : x0 * f[m].c0[k];
+          r[m].a.v[(2 * k + 1) % VEC] =
+              i < nr ? fmaf(x1, f[m].c1[k], x0 * f[m].s0[k]) : x1 * f[m].c1[k];
+        }
       }
     }
   };
-  for (int row = g0; row < rows; row += kRowsAhead * step) {
+  if (A.hq > 0) {
+    factors(N.q_norm);
+    float* const to = A.q_out + t * A.qo_ts;
+    for (int row0 = g0; row0 < A.hq; row0 += kRowsAhead * step) {
 #pragma unroll
-    for (int k = 0; k < kRowsAhead; ++k) {
-      if (row + k * step < rows) finish(row + k * step, ahead[k]);
-      fetch(row + (k + kRowsAhead) * step, ahead[k]);
+      for (int k = 0; k < kRowsAhead; ++k) {
+        const int row = row0 + k * step;
+        if (row < A.hq) {
+          turn(ahead[k], N.q_norm != nullptr);
+          float* out = to + row * A.qo_hs;
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            const int i = gl + m * GL, e = first_of(i);
+            if (i < ni) store_f32<VEC>(out + e, ahead[k][m].a);
+            if (PAIRS && i < nr) store_f32<VEC>(out + e + apart, ahead[k][m].b);
+          }
+        }
+        fetch(row + kRowsAhead * step, qp, A.q_hs, A.hq, ahead[k]);
+      }
+    }
+  }
+  if (slot < 0) return;
+#pragma unroll
+  for (int k = 0; k < kRowsAhead; ++k) fetch(g0 + k * step, kp, A.k_hs, hk, ahead[k]);
+  factors(N.k_norm);
+  {
+    T* const to = static_cast<T*>(A.c.k) + slot;
+    for (int row0 = g0; row0 < hk; row0 += kRowsAhead * step) {
+#pragma unroll
+      for (int k = 0; k < kRowsAhead; ++k) {
+        const int row = row0 + k * step;
+        if (row < hk) {
+          turn(ahead[k], N.k_norm != nullptr);
+          T* out = to + (int64_t)row * A.c.head_stride;
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            const int i = gl + m * GL, e = first_of(i);
+            if (i < ni) store_cache<VEC>(out + e, ahead[k][m].a, A.c.k_scale);
+            if (PAIRS && i < nr) store_cache<VEC>(out + e + apart, ahead[k][m].b, A.c.k_scale);
+          }
+        }
+        fetch(row + kRowsAhead * step, kp, A.k_hs, hk, ahead[k]);
+      }
     }
   }
   // ---- values: copied
-  if (slot < 0) return;
   const int total = hk * nv, every = gridDim.y * kNormThreads;
-  T* to = static_cast<T*>(A.c.v) + slot;
+  T* const to = static_cast<T*>(A.c.v) + slot;
 #pragma unroll 2
   for (int it = blockIdx.y * kNormThreads + threadIdx.x; it < total; it += every) {
     const int j = nv == 1 ? it : (int)__umulhi((uint32_t)it, A.mv), e = (it - j * nv) * VEC;
