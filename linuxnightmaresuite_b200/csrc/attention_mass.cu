@@ -8,28 +8,36 @@
 // stands by itself: no running maximum, no join, any split.
 //
 // Bound by memory: the keys are read once (again for every further 32 query heads of a
-// key head), values not at all, 8 bytes per slot for the sums.  The products go to mma.sync (m16n8k16)
-// as in the attention kernel, the heads' parts in the 16 rows of M (attention_frag.cuh);
-// on CUDA cores 4 heads would take 2 instructions per head and element and be issue-bound.  But no key
-// passes through shared memory: the order of a product's terms is free, so lane (g, t)
-// of a warp loads 16-byte chunks t, t + 4, ... of key g straight into the registers of the B
-// operand, and q's parts, in shared memory, are laid out in that order.  A warp has
-// KEYS keys' loads under way at a time and the mass of its keys behind them; that 16
-// warps of an SM alternate between loading and multiplying keeps the memory busy.
+// key head), values not at all, 8 bytes per slot for the sums.  The products go to mma.sync
+// (m16n8k16) as in the attention kernel, the heads' parts in the 16 rows of M
+// (attention_frag.cuh); on CUDA cores 4 heads would take 2 instructions per head and element and be
+// issue-bound.
+//
+// Work.  A unit is a (sequence, key head), cut into rounds of KEYS keys per warp.  All units in
+// order, each at the cost of its rounds and one more for its start (q and its parts), are dealt
+// out in equal contiguous runs to the CTAs of one resident grid, whatever the lengths.  A warp
+// takes a tile of KEYS keys of each round through a ring of its own, filled by TMA in boxes that
+// lie in one page (as in the attention kernel); the loads run on across the ends of units, page
+// ids are fetched a tile ahead of them.  (Keys loaded by the lanes themselves, straight
+// into the operands of the products, took 367 instructions for 16 keys, most of them for
+// addresses: 64 sequences of up to 4096 keys, 8 heads of 128, bf16, 89 us.)
 #include <math.h>
 
 #include <algorithm>
 #include <cmath>
 
 #include "attention_frag.cuh"
+#include "tc_common.cuh"
 
 namespace moe {
 
-constexpr int kMassWarps = 8;
-constexpr int kMassGroups = 4;         // groups of 8 query heads at one reading of the keys
+constexpr int kMassWarps = 8, kMassThreads = kMassWarps * 32;
+constexpr int kMassGroups = 4;         // groups of 8 query heads at one reading of the keys, at most
+constexpr int kMassSlots = 3;
 
 struct MassArgs {
   moe_paged_cache c;
+  CacheMap map;
   const float* q;
   int64_t q_ss, q_hs;
   const int32_t* seq_lens;
@@ -37,7 +45,7 @@ struct MassArgs {
   float* out;
   int64_t row;                         // slots of a (sequence, head) in mass and out
   int* status;
-  int hq, window, chunk, chunks;       // keys of a CTA at a time, CTAs of a (sequence, head)
+  int hq, window, pass;                // the first of the groups of heads of this launch
   float scale, cap;
 };
 
@@ -45,55 +53,224 @@ template <int DT, int DP, bool PACK> struct MassCfg {
   static constexpr bool kBf = DT == MOE_CACHE_BF16;
   using Frag = AFrag<kBf, PACK>;
   static constexpr int kElem = DT == MOE_CACHE_E4M3 ? 1 : 2;
-  static constexpr int kChunks = DP * kElem / 64;          // 16-byte chunks of a lane and key
-  static constexpr int kTiles = DP > 128 ? 2 : 4;          // 8-key tiles of a warp
-  static constexpr int kKeys = 8 * kTiles;
+  static constexpr int kRow = DP * kElem < kLine ? kLine : DP * kElem;     // bytes in the ring
+  static constexpr int kLines = kRow / kLine;
+  static constexpr int kKeys = kRow <= 128 ? 32 : 16;      // keys of a tile
+  static constexpr int kSlot = kKeys * kRow;
+  static constexpr int kRing = kMassWarps * kMassSlots * kSlot;
   static constexpr int kGroup = DP / 16 * Frag::kBytes;
+  static constexpr int kGroups = kRing + kMassGroups * kGroup <= 220 * 1024 ? kMassGroups : 2;
+  static_assert(kRing + kGroups * kGroup <= 225 * 1024, "");
+  static constexpr int kRound = kMassWarps * kKeys;
+  static constexpr int kCtas = kSlot <= 4096 ? 2 : 1;
+};
+
+// A cursor over a CTA's rounds: round r of r1 of a unit.
+struct MassCursor {
+  int seq, head, len, first, r, r1, cost;
+  long long at;                        // where the unit's cost begins
+};
+
+struct MassShared {
+  long long scan[kMassWarps], base;
+  int seq, dead;
+  uint64_t bars[kMassWarps][kMassSlots];
+  float scale[kMassGroups][kAttHeads], lse[kMassGroups][kAttHeads];
 };
 
 template <int DT, int DP, bool PACK>
-__global__ void __launch_bounds__(kMassWarps * 32, 2) mass_kernel(const MassArgs A) {
+__global__ void __launch_bounds__(kMassThreads, (MassCfg<DT, DP, PACK>::kCtas))
+mass_kernel(const __grid_constant__ CUtensorMap kmap, const MassArgs A) {
   using Cfg = MassCfg<DT, DP, PACK>;
   using Frag = typename Cfg::Frag;
-  constexpr int CH = Cfg::kChunks, NT = Cfg::kTiles, KEYS = Cfg::kKeys;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float sh_scale[kMassGroups][kAttHeads], sh_lse[kMassGroups][kAttHeads];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int D = A.c.head_dim, G = A.hq / A.c.kv_heads, ps = A.c.page_size;
-  const int unit = blockIdx.x / A.chunks, chunk0 = blockIdx.x - unit * A.chunks;
-  const int seq = unit / A.c.kv_heads, head = unit - seq * A.c.kv_heads;
+  constexpr int KEYS = Cfg::kKeys, RK = Cfg::kRound, NS = kMassSlots, LINES = Cfg::kLines;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ MassShared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int D = A.c.head_dim, hk = A.c.kv_heads, G = A.hq / hk, S = A.c.seqs;
+  const uint32_t ps = A.c.page_size;
+  const int ng = min(Cfg::kGroups, (G + kAttHeads - 1) / kAttHeads - A.pass);
+  const int most = (int)min((int64_t)A.c.table_width * A.c.page_size, A.row);
+  if (lane < NS) {
+    mbar_init(&sh.bars[warp][lane], 1);
+    fence_mbar_init();
+  }
+  if (tid == 0) {
+    sh.dead = 0;
+    prefetch_map(&kmap);
+  }
   pdl_trigger();
   pdl_wait();
-  const int64_t most = std::min<int64_t>((int64_t)A.c.table_width * ps, A.row);
-  const int told = A.seq_lens[seq], len = (int)min((int64_t)max(told, 0), most);
-  if (told > most && chunk0 == 0 && head == 0 && threadIdx.x == 0)
-    set_status(A.status, MOE_STATUS_BAD_PAGE);
-  const int first = A.window > 0 && len > A.window ? len - A.window : 0;
-  if ((int64_t)chunk0 * A.chunk >= len) return;
-  const int32_t* table = A.c.block_table + (int64_t)seq * A.c.table_stride;
-  const uint8_t* keys = static_cast<const uint8_t*>(A.c.k) +
-                        (int64_t)head * A.c.head_stride * Cfg::kElem;
-  const int row_chunks = D * Cfg::kElem / 16;
-  const int groups = (G + kAttHeads - 1) / kAttHeads;
-  const float* mass = A.mass + (int64_t)unit * A.row;
-  float* out = A.out + (int64_t)unit * A.row;
 
-  for (int pass = 0; pass < groups; pass += kMassGroups) {
-    const int ng = min(kMassGroups, groups - pass);
-    if (pass) __syncthreads();
-    // q's parts, a warp per group: scaled by a power of two to [2^10, 2^11)
+  // ---- this CTA's run
+  auto len_of = [&](int s) { return min(max(A.seq_lens[s], 0), most); };
+  auto cost_of = [&](int s) {                  // of one head of the sequence
+    const int n = len_of(s);
+    return n ? (n + RK - 1) / RK + 1 : 0;
+  };
+  const int per = (S + kMassThreads - 1) / kMassThreads, s0 = min(S, tid * per), s1 = min(S, s0 + per);
+  long long mine = 0;
+  for (int s = s0; s < s1; ++s) {
+    mine += (long long)cost_of(s) * hk;
+    if (blockIdx.x == 0 && A.seq_lens[s] > most) set_status(A.status, MOE_STATUS_BAD_PAGE);
+  }
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long n = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += n;
+  }
+  if (lane == 31) sh.scan[warp] = incl;
+  __syncthreads();
+  long long total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kMassWarps; ++w) {
+    if (w < warp) before += sh.scan[w];
+    total += sh.scan[w];
+  }
+  const long long quota = (total + gridDim.x - 1) / gridDim.x, start = blockIdx.x * quota;
+  const long long end = min(total, start + quota);
+  if (start >= end) return;
+  if (mine > 0 && before <= start && start < before + mine) {
+    int s = s0;
+    for (;;) {
+      const long long n = (long long)cost_of(s) * hk;
+      if (start < before + n) break;
+      before += n;
+      ++s;
+    }
+    sh.seq = s;
+    sh.base = before;
+  }
+  __syncthreads();
+
+  auto open = [&](MassCursor& c) {             // its rounds r .. r1 of this run; false: none
+    c.len = len_of(c.seq);
+    c.first = A.window > 0 && c.len > A.window ? c.len - A.window : 0;
+    c.r = (int)max(0ll, start - c.at - 1);
+    c.r1 = (int)min((long long)c.cost - 1, end - c.at - 1);
+    return c.r < c.r1;
+  };
+  auto next_unit = [&](MassCursor& c) {        // false: that was the last
+    do {
+      c.at += c.cost;
+      if (c.at >= end) return false;
+      if (++c.head == hk) {
+        c.head = 0;
+        do {
+          c.cost = cost_of(++c.seq);           // there is one: at < end <= total
+        } while (c.cost == 0);
+      }
+    } while (!open(c));
+    return true;
+  };
+  MassCursor C;                                // of the arithmetic
+  C.seq = sh.seq;
+  C.cost = cost_of(C.seq);
+  C.head = (int)((start - sh.base) / C.cost);
+  C.at = sh.base + (long long)C.head * C.cost;
+  bool more = open(C) || next_unit(C);
+  if (!more) return;                           // the run is the start of a unit whose rounds are not in it
+
+  // ---- loads: a cursor that runs NS - 1 tiles ahead, across the ends of units
+  MassCursor W = C;
+  bool wmore = true;
+  const uint32_t ring = smem_u32(smem) + warp * NS * Cfg::kSlot;
+  const int box = 1 << A.map.box_shift, boxes = KEYS >> A.map.box_shift;
+  int lslot = 0, page = -1;
+  uint32_t pslot = 0;
+  bool in = false;
+  auto ask = [&]() {                           // page of this lane's box of the cursor's tile
+    const int key = W.r * RK + warp * KEYS + (lane << A.map.box_shift);
+    in = wmore && lane < boxes && key < W.len && key + box > W.first;
+    if (in) {
+      const uint32_t n = (uint32_t)key / ps;
+      pslot = (uint32_t)key - n * ps;
+      page = A.c.block_table[(int64_t)W.seq * A.c.table_stride + n];
+    }
+  };
+  auto load = [&]() -> uint32_t {              // the cursor's tile; which keys are there and seen
+    if (!wmore) return 0u;
+    if (in && (page < 0 || page >= A.c.pages)) {
+      set_status(A.status, MOE_STATUS_BAD_PAGE);
+      in = false;
+    }
+    const uint32_t ok = __ballot_sync(0xffffffffu, in);
+    uint64_t* bar = &sh.bars[warp][lslot];
+    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(ok) * LINES * kLine) << A.map.box_shift);
+    __syncwarp();
+    if (in) {
+      const uint32_t to = ring + lslot * Cfg::kSlot + (lane << A.map.box_shift) * kLine;
+      const int row = page * A.map.page_units + W.head * A.map.head_units;
+#pragma unroll
+      for (int b = 0; b < LINES; ++b)
+        tma_load_3d(to + b * KEYS * kLine, &kmap, b * (kLine / Cfg::kElem), row, (int)pslot, bar);
+    }
+    lslot = lslot + 1 == NS ? 0 : lslot + 1;
+    const int key = W.r * RK + warp * KEYS + (lane & (KEYS - 1));
+    const uint32_t seen = __ballot_sync(0xffffffffu, key >= W.first && key < W.len &&
+                                                         ((ok >> ((lane & (KEYS - 1)) >> A.map.box_shift)) & 1u));
+    if (++W.r == W.r1) wmore = next_unit(W);
+    ask();
+    return seen;
+  };
+  ask();
+  uint32_t seen_of[NS - 1];
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) seen_of[i] = load();
+
+  // Bounded; after a timeout anywhere in the CTA no wait takes long any more.
+  int cslot = 0;
+  uint32_t cphase = 0;
+  auto wait_slot = [&]() {
+    uint64_t* bar = &sh.bars[warp][cslot];
+    if (!mbar_test(bar, cphase) && !*(volatile int*)&sh.dead && !mbar_wait(bar, cphase)) {
+      sh.dead = 1;
+      set_status(A.status, MOE_STATUS_TIMEOUT);
+    }
+    __syncwarp();
+    const uint32_t a = ring + cslot * Cfg::kSlot;
+    if (++cslot == NS) {
+      cslot = 0;
+      cphase ^= 1u;
+    }
+    return a;
+  };
+  uint8_t* const qs = smem + Cfg::kRing;
+
+  // fragment addresses: byte offset of 16-byte chunk c of row r, blocks of KEYS lines
+  auto slot_at = [](int r, int c) {
+    return (uint32_t)((c >> 3) * KEYS * kLine + r * kLine + (((c & 7) ^ (r & 7)) << 4));
+  };
+  const int krow = Cfg::kElem == 2 ? (lane >> 4) * 8 + (lane & 7)
+                                   : ((lane >> 3) & 1) * 8 + (lane & 7);
+  const int kch = Cfg::kElem == 2 ? (lane >> 3) & 1 : lane >> 4;
+  constexpr int PPL = kLine / 32;              // chunk pairs of a line
+  uint32_t kof[PPL];
+#pragma unroll
+  for (int j = 0; j < PPL; ++j) kof[j] = slot_at(krow, 2 * j + kch);
+  // the key whose sum this lane will hold
+  constexpr int NT = KEYS / 8;
+  const int own = NT == 4 ? 8 * (lane >> 3) + 2 * t + ((lane >> 2) & 1)
+                          : 8 * (lane >> 4) + 2 * t + ((lane >> 3) & 1);
+
+  for (bool first_unit = true;; first_unit = false) {
+    // ---- q's parts, a warp per group: scaled by a power of two to [2^10, 2^11)
+    if (!first_unit) __syncthreads();          // those before these have been read
     if (warp < ng) {
-      const int h = (pass + warp) * kAttHeads + (PACK ? g & 3 : g);
+      const int h = (A.pass + warp) * kAttHeads + (PACK ? g & 3 : g);
       const bool live = h < G && (!PACK || g < 4);
-      const float* q = A.q + (int64_t)seq * A.q_ss + ((int64_t)head * G + h) * A.q_hs;
-      // element of step i, register k: step i belongs to chunk t + 4 (i / per)
-      constexpr int PER = Cfg::kElem == 2 ? 2 : 4, ES = 16 / Cfg::kElem;
+      const float* q = A.q + (int64_t)C.seq * A.q_ss + ((int64_t)C.head * G + h) * A.q_hs;
+      // columns of a step: 2t, 2t + 1, 2t + 8, 2t + 9, of e4m3 keys 4t .. 4t + 3
+      auto column = [&](int i, int k) {
+        return 16 * i + (Cfg::kElem == 1 ? 4 * t + k : 2 * t + (k & 1) + 8 * (k >> 1));
+      };
       float v[DP / 16][4], mx = 0.f;
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int e = (t + 4 * (i / PER)) * ES + 4 * (i % PER) + k;
+          const int e = column(i, k);
           v[i][k] = h < G && e < D ? q[e] : 0.f;
           mx = fmaxf(mx, fabsf(v[i][k]));
         }
@@ -105,156 +282,154 @@ __global__ void __launch_bounds__(kMassWarps * 32, 2) mass_kernel(const MassArgs
       const float f1 = __uint_as_float((uint32_t)(127 + e1) << 23);
       const float f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
       if (t == 0) {
-        sh_scale[warp][g] = ldexpf(A.scale * A.c.k_scale, -e);
+        sh.scale[warp][g] = ldexpf(A.scale * A.c.k_scale, -e);
         // a head that is not there, or has seen no key, gives nothing
-        const float l = live ? A.lse[(int64_t)seq * A.hq + (int64_t)head * G + h] : -INFINITY;
-        sh_lse[warp][g] = l == -INFINITY ? INFINITY : l * kLog2e;
+        const float l = live ? A.lse[(int64_t)C.seq * A.hq + (int64_t)C.head * G + h] : -INFINITY;
+        sh.lse[warp][g] = l == -INFINITY ? INFINITY : l * kLog2e;
       }
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
         Frag f;
         f.set(v[i][0] * f1 * f2, v[i][1] * f1 * f2, v[i][2] * f1 * f2, v[i][3] * f1 * f2, g);
-        f.store(smem + warp * Cfg::kGroup + i * Frag::kBytes, lane);
+        f.store(qs + warp * Cfg::kGroup + i * Frag::kBytes, lane);
       }
     }
     __syncthreads();
+    const int64_t unit = ((int64_t)C.seq * hk + C.head) * A.row;
+    const float* mass = A.mass + unit;
+    float* out = A.out + unit;
 
-    for (int64_t c0 = (int64_t)chunk0 * A.chunk; c0 < len; c0 += (int64_t)A.chunks * A.chunk) {
-      const int c1 = (int)min((int64_t)len, c0 + A.chunk);
-      for (int base = (int)c0 + warp * KEYS; base < c1; base += kMassWarps * KEYS) {
-        // lane i < KEYS follows key base + i to its row, -1: not there or not seen
-        const int key = base + (lane & (KEYS - 1));
-        int64_t at = -1;
-        if (key < c1 && key >= first) {
-          const int n = key / ps, page = table[n];
-          if (page >= 0 && page < A.c.pages)
-            at = ((int64_t)page * A.c.page_stride + (int64_t)(key - n * ps) * A.c.token_stride) *
-                 Cfg::kElem;
-          else
-            set_status(A.status, MOE_STATUS_BAD_PAGE);
-        }
-        uint4 k[NT][CH];
+    for (; C.r < C.r1; ++C.r) {
+      const int key = C.r * RK + warp * KEYS + own;
+      const bool writes = key < C.len && (NT == 4 || !(lane & 4));
+      const float sum = writes ? mass[key] : 0.f;
+      const uint32_t ka = wait_slot();
+      const uint32_t seen = seen_of[0];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int64_t from = __shfl_sync(0xffffffffu, at, 8 * n + g);
-#pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            k[n][c] = make_uint4(0, 0, 0, 0);
-            if (from >= 0 && t + 4 * c < row_chunks)
-              asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                           : "=r"(k[n][c].x), "=r"(k[n][c].y), "=r"(k[n][c].z), "=r"(k[n][c].w)
-                           : "l"(keys + from + (t + 4 * c) * 16));
-          }
-        }
-        // the key whose sum this lane will hold
-        const int mine = NT == 4 ? 8 * (lane >> 3) + 2 * t + ((lane >> 2) & 1)
-                                 : 8 * (lane >> 4) + 2 * t + ((lane >> 3) & 1);
-        const bool there = __shfl_sync(0xffffffffu, at, mine) >= 0;
-        const bool writes = base + mine < c1 && (NT == 4 || !(lane & 4));
-        float sum = 0.f;
-        if (writes) sum = (pass ? out : mass)[base + mine];
+      for (int i = 0; i + 1 < NS - 1; ++i) seen_of[i] = seen_of[i + 1];
+      seen_of[NS - 2] = load();
 
-        float w[NT][2];                        // keys 8n + 2t, 8n + 2t + 1 of head g
+      float w[NT][2];                          // keys 8n + 2t, 8n + 2t + 1 of head g
 #pragma unroll
-        for (int n = 0; n < NT; ++n) w[n][0] = w[n][1] = 0.f;
-        for (int gr = 0; gr < ng; ++gr) {
-          const uint8_t* qs = smem + gr * Cfg::kGroup;
-          float x[NT][2];
+      for (int n = 0; n < NT; ++n) w[n][0] = w[n][1] = 0.f;
+#pragma unroll 1
+      for (int gr = 0; gr < ng; ++gr) {
+        const uint8_t* qg = qs + gr * Cfg::kGroup;
+        float y[NT][2];
 #pragma unroll
-          for (int k4 = 0; k4 < DP / 64; ++k4) {         // four steps in an accumulator
-            float a[NT][4];
+        for (int k4 = 0; k4 < DP / 64; ++k4) {             // four steps in an accumulator
+          float a[NT][4];
 #pragma unroll
-            for (int i = 4 * k4; i < 4 * k4 + 4; ++i) {
-              Frag f;
-              f.load(qs + i * Frag::kBytes, lane);
+          for (int kk = 4 * k4; kk < 4 * k4 + 4; kk += 3 - Cfg::kElem) {
+            Frag q0, q1;
+            q0.load(qg + kk * Frag::kBytes, lane);
+            if (Cfg::kElem == 1) q1.load(qg + (kk + 1) * Frag::kBytes, lane);
+            const int j = Cfg::kElem == 2 ? kk : kk / 2;   // chunk pair
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                uint32_t b0, b1;
-                if (Cfg::kElem == 2) {
-                  const uint4& v = k[n][i / 2 % CH];
-                  b0 = i % 2 ? v.z : v.x;
-                  b1 = i % 2 ? v.w : v.y;
+            for (int kb = 0; kb < KEYS / 16; ++kb) {
+              uint32_t b[4];
+              ldsm4(b, ka + kof[j % PPL] + (j / PPL) * KEYS * kLine + kb * 16 * kLine);
+              if (Cfg::kElem == 2) {
+                if (kk == 4 * k4) {
+                  q0.template mul<true>(a[2 * kb], b[0], b[1]);
+                  q0.template mul<true>(a[2 * kb + 1], b[2], b[3]);
                 } else {
-                  const uint4& v = k[n][i / 4 % CH];
-                  e4m3x4_f16x2(i % 4 == 0 ? v.x : i % 4 == 1 ? v.y : i % 4 == 2 ? v.z : v.w, b0,
-                               b1);
+                  q0.mul(a[2 * kb], b[0], b[1]);
+                  q0.mul(a[2 * kb + 1], b[2], b[3]);
                 }
-                if (i == 4 * k4) f.template mul<true>(a[n], b0, b1);
-                else f.mul(a[n], b0, b1);
+              } else {
+                uint32_t f[4][2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e4m3x4_f16x2(b[i], f[i][0], f[i][1]);
+                if (kk == 4 * k4) {
+                  q0.template mul<true>(a[2 * kb], f[0][0], f[0][1]);
+                  q0.template mul<true>(a[2 * kb + 1], f[1][0], f[1][1]);
+                } else {
+                  q0.mul(a[2 * kb], f[0][0], f[0][1]);
+                  q0.mul(a[2 * kb + 1], f[1][0], f[1][1]);
+                }
+                q1.mul(a[2 * kb], f[2][0], f[2][1]);
+                q1.mul(a[2 * kb + 1], f[3][0], f[3][1]);
               }
             }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              x[n][0] = (k4 ? x[n][0] : 0.f) + (a[n][0] + a[n][2]);
-              x[n][1] = (k4 ? x[n][1] : 0.f) + (a[n][1] + a[n][3]);
-            }
           }
-          const float scale = sh_scale[gr][g], lse2 = sh_lse[gr][g];
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float y = x[n][h];
-              if (PACK) y += __shfl_xor_sync(0xffffffffu, y, 16);
-              y *= scale;
-              if (A.cap > 0.f) y = A.cap * tanhf(y / A.cap);
-              const float p = ex2(fmaf(y, kLog2e, -lse2));
-              w[n][h] += lse2 == INFINITY ? 0.f : p;
-            }
+          for (int n = 0; n < NT; ++n) {
+            y[n][0] = (k4 ? y[n][0] : 0.f) + (a[n][0] + a[n][2]);
+            y[n][1] = (k4 ? y[n][1] : 0.f) + (a[n][1] + a[n][3]);
+          }
         }
-        // over the heads, which the lanes with the same t hold: halves are
-        // exchanged until one key is left
-        float r;
-        if (NT == 4) {
-          float u[4], v[2];
-          const bool hi = lane & 16, mid = lane & 8, lo = lane & 4;
+        const float scale = sh.scale[gr][g], lse2 = sh.lse[gr][g];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float keep = hi ? w[2 + i / 2][i % 2] : w[i / 2][i % 2];
-            const float give = hi ? w[i / 2][i % 2] : w[2 + i / 2][i % 2];
-            u[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
-          }
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float keep = mid ? u[2 + i] : u[i], give = mid ? u[i] : u[2 + i];
-            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+          for (int h = 0; h < 2; ++h) {
+            float z = y[n][h];
+            if (PACK) z += __shfl_xor_sync(0xffffffffu, z, 16);
+            z *= scale;
+            if (A.cap > 0.f) z = A.cap * tanhf(z / A.cap);
+            const float p = ex2(fmaf(z, kLog2e, -lse2));
+            w[n][h] += lse2 == INFINITY ? 0.f : p;
           }
-          r = (lo ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, lo ? v[0] : v[1], 4);
-        } else {
-          float u[2];
-          const bool hi = lane & 16, mid = lane & 8;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float keep = hi ? w[1][i] : w[0][i], give = hi ? w[0][i] : w[1][i];
-            u[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
-          }
-          r = (mid ? u[1] : u[0]) + __shfl_xor_sync(0xffffffffu, mid ? u[0] : u[1], 8);
-          r += __shfl_xor_sync(0xffffffffu, r, 4);
-        }
-        if (writes) out[base + mine] = there ? sum + r : sum;
       }
+      // over the heads, which the lanes with the same t hold: halves are exchanged until one
+      // key is left
+      float r;
+      const bool hi = lane & 16, mid = lane & 8, lo = lane & 4;
+      if (NT == 4) {
+        float u[4], v[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float keep = hi ? w[(2 + i / 2) % NT][i % 2] : w[i / 2][i % 2];
+          const float give = hi ? w[i / 2][i % 2] : w[(2 + i / 2) % NT][i % 2];
+          u[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float keep = mid ? u[2 + i] : u[i], give = mid ? u[i] : u[2 + i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+        }
+        r = (lo ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, lo ? v[0] : v[1], 4);
+      } else {
+        float u[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float keep = hi ? w[1][i] : w[0][i], give = hi ? w[0][i] : w[1][i];
+          u[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+        }
+        r = (mid ? u[1] : u[0]) + __shfl_xor_sync(0xffffffffu, mid ? u[0] : u[1], 8);
+        r += __shfl_xor_sync(0xffffffffu, r, 4);
+      }
+      // (what the ring holds for a key that is not there is anything)
+      if (writes) out[key] = (seen >> own) & 1u ? sum + r : sum;
     }
+    if (!next_unit(C)) break;
   }
+  // after a timeout copies may still be under way: give them time to land
+  if (*(volatile int*)&sh.dead)
+    for (int i = 0; i < NS; ++i) {
+      mbar_wait(&sh.bars[warp][i], 0);
+      mbar_wait(&sh.bars[warp][i], 1);
+    }
 }
 
 template <int DT, int DP, bool PACK>
 static int launch_mass(MassArgs& a, int64_t longest, cudaStream_t s) {
   using Cfg = MassCfg<DT, DP, PACK>;
   auto kern = mass_kernel<DT, DP, PACK>;
-  const int groups = std::min(kMassGroups, (a.hq / a.c.kv_heads + kAttHeads - 1) / kAttHeads);
-  const int smem = groups * Cfg::kGroup;
-  if (smem > 48 * 1024 - 1024)
-    MOE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  // A CTA's start (lengths, q, its parts) costs about as much as 256 keys: chunks as
-  // long as leave some six CTAs for each that is resident
-  const int64_t units = (int64_t)a.c.seqs * a.c.kv_heads, step = kMassWarps * Cfg::kKeys;
-  const int64_t even = units * longest / (12 * sm_count());
-  a.chunk = (int)(std::max<int64_t>(1, std::min<int64_t>(16, even / step)) * step);
-  a.chunks = (int)std::max<int64_t>(1, (longest + a.chunk - 1) / a.chunk);
-  MOE_REQUIRE(units * a.chunks <= 0x7fffffff, MOE_ERR_UNSUPPORTED, "%d sequences are too many",
-              a.c.seqs);
-  MOE_CUDA(launch_pdl(kern, dim3((unsigned)(units * a.chunks)), dim3(kMassWarps * 32),
-                      (size_t)smem, s, a));
+  const int all = (a.hq / a.c.kv_heads + kAttHeads - 1) / kAttHeads;
+  CUtensorMap kmap;
+  MOE_CHECK(make_cache_map(&kmap, a.c, a.c.k, Cfg::kKeys, &a.map));
+  const int64_t units = (int64_t)a.c.seqs * a.c.kv_heads;
+  const int64_t rounds = units * std::max<int64_t>(1, (longest + Cfg::kRound - 1) / Cfg::kRound);
+  const int grid = (int)std::min<int64_t>(rounds, (int64_t)Cfg::kCtas * sm_count());
+  for (a.pass = 0; a.pass < all; a.pass += Cfg::kGroups) {
+    const int smem = Cfg::kRing + std::min(Cfg::kGroups, all - a.pass) * Cfg::kGroup;
+    MOE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  Cfg::kRing + Cfg::kGroups * Cfg::kGroup));
+    MOE_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(kMassThreads), (size_t)smem, s, kmap, a));
+    a.mass = a.out;                    // further groups of heads add to the sums of the first
+  }
   return MOE_OK;
 }
 
