@@ -48,7 +48,7 @@ struct EvictShared {
   int bins[4][kBins];
   int scan[33];
   int newest, digit, above;
-  int equal, movers, freed;            // of this CTA: keys equal to the limit, movers, slots given up
+  int movers, freed;                   // of this CTA
   int of_warp[3][kEvictWarps];
 };
 
@@ -265,13 +265,13 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(const EvictArgs
   // ---- keys
   if (tid == 0) {
     sh.newest = INT32_MIN;
-    sh.equal = sh.movers = sh.freed = 0;
+    sh.movers = sh.freed = 0;
   }
 #pragma unroll
   for (int d = 0; d < 4; ++d) sh.bins[d][tid] = 0;
   __syncthreads();
   int newest = INT32_MIN;
-#pragma unroll 4
+#pragma unroll 8
   for (int i = tid; i < cnt; i += NT) {
     newest = max(newest, U.held[s0 + i]);
     keys[i] = order_key(U.mass[s0 + i]);
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(const EvictArgs
   for (int r = 0; r < C; ++r) newest = max(newest, *cluster.map_shared_rank(&sh.newest, r));
   const int64_t since = (int64_t)newest - A.recent;
   if (A.recent > 0)
-#pragma unroll 4
+#pragma unroll 8
     for (int i = tid; i < cnt; i += NT)
       if (U.held[s0 + i] > since) keys[i] = 0xffffffffu;
 
@@ -325,16 +325,14 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(const EvictArgs
   const int seg = (cnt + NT - 1) / NT * 32, w0 = min(cnt, warp * seg), w1 = min(cnt, w0 + seg);
   int equals = 0;
   for (int i = w0 + lane; i - lane < w1; i += 32) equals += count(i < w1 && keys[i] == limit);
-  if (lane == 0) {
-    sh.of_warp[0][warp] = equals;
-    if (equals) atomicAdd(&sh.equal, equals);
-  }
-  meet();
-  int equal = 0;
-  for (int r = 0; r < rank; ++r) equal += *cluster.map_shared_rank(&sh.equal, r);
+  if (lane == 0) sh.of_warp[0][warp] = equals;
+  __syncthreads();
+  int equal = 0;                       // in the slices before this one: the last digit's counts
+  for (int r = 0; r < rank; ++r) equal += *cluster.map_shared_rank(&sh.bins[3][limit & 255u], r);
   for (int w = 0; w < warp; ++w) equal += sh.of_warp[0][w];
-  // keys become what happens to a slot: 0 nothing, 1 moves away, 2 is filled
+  // keys become what happens to a slot: 0 it is given up, 1 moves away, 2 is filled, 3 stays
   int mv = 0, fr = 0;
+#pragma unroll 2
   for (int i = w0 + lane; i - lane < w1; i += 32) {
     const bool in = i < w1;
     const uint32_t k = in ? keys[i] : 0u;
@@ -343,8 +341,7 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(const EvictArgs
     const bool kept = in && (k > limit || (eq && nth < want));
     equal += count(eq);
     const bool moves = kept && s0 + i >= A.keep, freed = in && !kept && s0 + i < A.keep;
-    if (in) keys[i] = moves ? 1u : freed ? 2u : 0u;
-    if (kept && !moves) U.copy(s0 + i);
+    if (in) keys[i] = moves ? 1u : freed ? 2u : kept ? 3u : 0u;
     mv += count(moves);
     fr += count(freed);
   }
@@ -368,22 +365,28 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(const EvictArgs
     movers += sh.of_warp[1][w];
     freed += sh.of_warp[2][w];
   }
-  // ---- mover k and freed slot k meet in the list of CTA k % C
+  if (U.mass_out != U.mass || U.held_out != U.held)
+#pragma unroll 4
+    for (int i = w0 + lane; i < w1; i += 32)
+      if (keys[i] == 3u) U.copy(s0 + i);
+  // ---- mover k and freed slot k meet in the list of CTA k % C (a power of two)
+  const int shift = 31 - __clz(C);
   for (int i = w0 + lane; i - lane < w1; i += 32) {
     const uint32_t what = i < w1 ? keys[i] : 0u;
     const int m = movers + before(what == 1u), f = freed + before(what == 2u);
-    if (what == 1u) cluster.map_shared_rank(list, m % C)[m / C].x = s0 + i;
-    if (what == 2u) cluster.map_shared_rank(list, f % C)[f / C].y = s0 + i;
+    if (what == 1u) cluster.map_shared_rank(list, m & (C - 1))[m >> shift].x = s0 + i;
+    if (what == 2u) cluster.map_shared_rank(list, f & (C - 1))[f >> shift].y = s0 + i;
     movers += count(what == 1u);
     freed += count(what == 2u);
   }
   meet();
   // no CTA's shared memory is read or written by others from here on
 
-  // ---- a warp takes 32 moves: each lane finds the rows of one, then the rows go over
+  // ---- a warp takes 32 moves: a lane each finds the rows of one, then the rows go over
   const EvictRows rows(A, unit % A.c.kv_heads);
   const int mine = all > rank ? (all - rank + C - 1) / C : 0;
-  for (int m0 = warp * 32; m0 < mine; m0 += NT) {
+  constexpr int MOVES = 32;
+  for (int m0 = warp * MOVES; m0 < mine; m0 += kEvictWarps * MOVES) {
     int64_t from = -1, to = -1;
     if (m0 + lane < mine) {
       const int2 m = list[m0 + lane];
@@ -396,7 +399,7 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(const EvictArgs
         from = to = -1;
       }
     }
-    rows.move<8>(from, to, min(32, mine - m0), lane);
+    rows.move<8>(from, to, min(MOVES, mine - m0), lane);
   }
 }
 
