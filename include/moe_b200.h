@@ -553,12 +553,15 @@ int moe_linear_record(const moe_linear_args* args);
  *          table of each sequence that is as long as the prefix or longer.  (Either may be read.)
  *          Shorter sequences may have any pages
  *   seq_lens, max_len: the prefix included
+ *   form: MOE_PREFIX_AUTO lets the library choose by the sizes (short prefixes and small batches
+ *          are faster sequence by sequence); the others pin one (for tests and tuning)
  * prefix_pages 0 is moe_paged_attention.  The split over the GPU depends on sizes alone; equal
  * calls give equal bits. */
+enum { MOE_PREFIX_AUTO = 0, MOE_PREFIX_EACH = 1, MOE_PREFIX_TOGETHER = 2 };
 typedef struct moe_prefix_attention_args {
   moe_paged_attention_args attention;
   const int32_t* prefix;
-  int prefix_pages;
+  int prefix_pages, form;
 } moe_prefix_attention_args;
 int moe_prefix_attention_workspace_bytes(int seqs, int q_heads, int kv_heads, int head_dim,
                                          size_t* bytes);

@@ -39,6 +39,7 @@ MOE_STATUS_TIMEOUT = 4
 MOE_STATUS_BAD_PAGE = 8
 
 MOE_CACHE_F16, MOE_CACHE_BF16, MOE_CACHE_E4M3 = 0, 1, 2
+MOE_PREFIX_AUTO, MOE_PREFIX_EACH, MOE_PREFIX_TOGETHER = 0, 1, 2
 
 vp = ctypes.c_void_p
 ci = ctypes.c_int
@@ -108,7 +109,8 @@ class MoELinearArgs(ctypes.Structure):
 
 class MoEPrefixAttentionArgs(ctypes.Structure):
     """Mirror of ``moe_prefix_attention_args``."""
-    _fields_ = [("attention", MoEPagedAttentionArgs), ("prefix", vp), ("prefix_pages", ci)]
+    _fields_ = [("attention", MoEPagedAttentionArgs), ("prefix", vp), ("prefix_pages", ci),
+                ("form", ci)]
 
 
 class MoENormAppendArgs(ctypes.Structure):

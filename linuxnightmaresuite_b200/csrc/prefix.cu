@@ -908,6 +908,17 @@ static int prefix_workspace(const PrefixPlan& p, int seqs, int q_heads, int kv_h
   return MOE_OK;
 }
 
+// Whether the products over all rows take less time than the paged attention of each sequence over
+// the prefix, microseconds.  Fitted to both at 2 to 128 sequences behind 256 to 16384 tokens, heads of 64,
+// 128 and 256 of all types: the paged attention reads (mostly from L2) 7.5 MB a microsecond, 4.6 of e4m3; the
+// kernels here take 13 (28 at 256 columns) for their launches and starts and 3 (5) a tile.
+// 32 / 8 heads of 128, fp16: 8 x 4096 tokens 25.5 each, 28 together; 32 x 4096 73 and 30; 2 x 1024 10 and 22.
+static bool together_pays(const moe_paged_cache& c, const PrefixPlan& p, int keys, int quota) {
+  const double bytes = 2.0 * cache_elem_bytes(c.dtype) * c.seqs * c.kv_heads * c.head_dim * keys;
+  const double each = bytes / (c.dtype == MOE_CACHE_E4M3 ? 4.6e6 : 7.5e6);
+  return (p.dq == 256 ? 28.0 + 5.0 * quota : 13.0 + 3.0 * quota) < each;
+}
+
 template <int DT, int DQ>
 static int launch_prefix(PrefixArgs& a, const PrefixRowsArgs& rows, int grid, cudaStream_t s) {
   using Cfg = PrefixCfg<DT, DQ>;
@@ -970,7 +981,8 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
   if (a.c.seqs == 0) return MOE_OK;
   MOE_REQUIRE(r->prefix || r->prefix_pages == 0, MOE_ERR_INVALID, "null pointer");
   MOE_REQUIRE((uintptr_t)t.out % 16 == 0, MOE_ERR_INVALID, "out must be 16-byte aligned");
-  if (r->prefix_pages == 0) return moe::attention_from(t, 0);
+  MOE_REQUIRE(r->form >= MOE_PREFIX_AUTO && r->form <= MOE_PREFIX_TOGETHER, MOE_ERR_INVALID,
+              "form %d not known", r->form);
   const int S = a.c.seqs, d = a.c.head_dim, P = r->prefix_pages * a.c.page_size;
   const moe::PrefixPlan p = moe::prefix_plan(S, t.q_heads, a.c.kv_heads, d);
   moe::PrefixSpace ws;
@@ -993,7 +1005,7 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
   a.RG = p.RG;
   a.tiles = (P + p.kt - 1) / p.kt;
   const int64_t total = p.units * a.tiles;
-  const int64_t quota = (total + p.teams - 1) / p.teams;
+  const int64_t quota = std::max<int64_t>(1, (total + p.teams - 1) / p.teams);
   MOE_REQUIRE(total < (1ll << 30) && (int64_t)S * G < (1ll << 30) && p.slots < (1ll << 30),
               MOE_ERR_UNSUPPORTED, "%d sequences behind a prefix of %d tokens are too many", S, P);
   a.total = (uint32_t)total;
@@ -1001,6 +1013,9 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
   a.parts = (a.tiles - 1) / a.quota + 2;
   MOE_REQUIRE(p.units * p.m * a.parts <= p.slots, MOE_ERR_INVALID, "parts %d", a.parts);
   const int grid = (int)((total + quota - 1) / quota) * p.m;
+  if (P == 0 || r->form == MOE_PREFIX_EACH ||
+      (r->form == MOE_PREFIX_AUTO && !moe::together_pays(a.c, p, P, a.quota)))
+    return moe::attention_from(t, 0);
   a.cap = t.softcap;
   const int vec = (uintptr_t)t.q % 16 == 0 && (S == 1 || t.q_seq_stride % 4 == 0) &&
                   (t.q_heads == 1 || t.q_head_stride % 4 == 0);

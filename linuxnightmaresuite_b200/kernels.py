@@ -28,6 +28,9 @@ KERNELS_GEMV = _lib.MOE_KERNELS_GEMV
 KERNELS_BLOCKSCALE = _lib.MOE_KERNELS_BLOCKSCALE
 KERNELS_SPLIT_GEMM = _lib.MOE_KERNELS_SPLIT_GEMM
 STATUS_BAD_PAGE = _lib.MOE_STATUS_BAD_PAGE
+PREFIX_AUTO = _lib.MOE_PREFIX_AUTO
+PREFIX_EACH = _lib.MOE_PREFIX_EACH
+PREFIX_TOGETHER = _lib.MOE_PREFIX_TOGETHER
 # GGML type -> (weights per block, bytes per block), dequant_fast.py:723-754
 BLOCK_GEOMETRY = {QTYPE_F32: (1, 4), QTYPE_Q4_0: (32, 18), QTYPE_Q5_1: (32, 24),
                   QTYPE_Q8_0: (32, 34), QTYPE_Q4_K: (256, 144), QTYPE_Q6_K: (256, 210)}
@@ -300,7 +303,7 @@ _APPEND_ARGS = struct.Struct("@" + _CACHE + "3P6q4P2q2P4i0q")
 _ATTENTION_ARGS = struct.Struct("@" + _CACHE + "P2q4PNP3i2f0q")
 _LINEAR_ARGS = struct.Struct("@2PqPqPqP4i")
 _NORM_APPEND_ARGS = struct.Struct("@" + _CACHE + "3P6q4P2q2P4i5Pqfi0q")
-_PREFIX_ARGS = struct.Struct("@" + _CACHE + "P2q4PNP3i2f0qPi0q")
+_PREFIX_ARGS = struct.Struct("@" + _CACHE + "P2q4PNP3i2f0qP2i0q")
 _MASS_ARGS = struct.Struct("@" + _CACHE + "P2q4Pq2P3i2f0q")
 _EVICT_ARGS = struct.Struct("@" + _CACHE + "6P2q2P3i0q")
 assert _NORM_APPEND_ARGS.size == ctypes.sizeof(_lib.MoENormAppendArgs)
@@ -560,14 +563,15 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      scale: Optional[float] = None, softcap: float = 0.0, k_scale: float = 1.0,
                      v_scale: float = 1.0, max_len: int = 0, out: Optional[torch.Tensor] = None,
                      return_lse: bool = False, ws: Optional[torch.Tensor] = None,
-                     status: Optional[torch.Tensor] = None):
+                     status: Optional[torch.Tensor] = None, form: int = PREFIX_AUTO):
     """``paged_attention`` of sequences that begin with the same whole pages
     ``prefix_pages`` (n,) int32 (a system prompt, a document): their keys are
     read and multiplied once for all rows.  ``block_table`` and ``seq_lens``
     cover whole sequences, the prefix included: the rows of those that are as
     long as the prefix or longer begin with its pages; shorter ones (0:
     padding) may have any.  ``ws`` comes from ``prefix_attention_workspace``; all
-    else as in ``paged_attention``, whose result it is but for the last bits."""
+    else as in ``paged_attention``, whose result it is but for the last bits.
+    ``form`` (``PREFIX_*``) pins the kernels; the default chooses by the sizes."""
     c, dev, seqs, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
     shape = q.shape
     if len(shape) != 3:
@@ -591,7 +595,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         *c, q.data_ptr(), qs[0], qs[1], _vector(seq_lens, _I32, "seq_lens", dev, seqs),
         out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
         _raw_stream(dev), hq, max_len, 0, d ** -0.5 if scale is None else scale, softcap,
-        _vector(prefix_pages, _I32, "prefix_pages", dev, pages), pages))
+        _vector(prefix_pages, _I32, "prefix_pages", dev, pages), pages, form))
     if status is not None and seqs:
         status |= ws[:4].view(_I32)
     return (out, lse) if return_lse else out

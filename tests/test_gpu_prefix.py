@@ -30,9 +30,9 @@ class Shared:
                 c.kd[s], c.vd[s] = (torch.cat([x[-1], x[s][P:]]) for x in (c.kd, c.vd))
         self.kd, self.vd, self.dtype = c.kd[:-1], c.vd[:-1], dtype
 
-    def call(self, q, **kw):
+    def call(self, q, form=K.PREFIX_TOGETHER, **kw):
         return K.prefix_attention(q, self.c.k, self.c.v, self.table, self.lens, self.pages,
-                                  return_lse=True, **self.c.scales, **kw)
+                                  return_lse=True, form=form, **self.c.scales, **kw)
 
     def check(self, q, out, lse, scale, cap=0.0):
         """The bounds of `attend` (of its own 2^-20 for the accumulators 2^-19: 16 steps of a
@@ -72,6 +72,21 @@ def test_prefix(dtype, own, pages, page, hq, hkv, d, layout):
     assert K.read_status(ws) == 0
     again, lse2 = x.call(q, ws=ws, max_len=int(x.lens.max()))      # equal bits, and the workspace is ready
     assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("own,pages,together", [([5, 9], 4, False), ([3] * 64, 128, True)])
+def test_prefix_form_by_size(own, pages, together):
+    """Short prefixes and few sequences go one by one, the others together; equal bits of
+    the form that is chosen."""
+    x = Shared(own, pages, 16, 8, 128, F16)
+    q = randn(len(own), 32, 128)
+    got = x.call(q, K.PREFIX_AUTO)
+    same = x.call(q, K.PREFIX_TOGETHER if together else K.PREFIX_EACH)
+    assert torch.equal(got[0], same[0]) and torch.equal(got[1], same[1])
+    other = x.call(q, K.PREFIX_EACH if together else K.PREFIX_TOGETHER)
+    assert not torch.equal(got[0], other[0])
+    for out, lse in (got, other):
+        x.check(q, out, lse, 128 ** -0.5)
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
@@ -183,7 +198,8 @@ def test_prefix_captured_and_other_stream():
     out = torch.empty_like(q)
 
     def call():
-        return K.prefix_attention(q, k, v, table, lens, pages, out=out, return_lse=True, ws=ws)[1]
+        return K.prefix_attention(q, k, v, table, lens, pages, out=out, return_lse=True, ws=ws,
+                                  form=K.PREFIX_TOGETHER)[1]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
