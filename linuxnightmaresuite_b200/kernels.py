@@ -504,17 +504,28 @@ def paged_attention_workspace(seqs: int, q_heads: int, kv_heads: int, head_dim: 
     return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
+def _lse(q: torch.Tensor, lse: Optional[torch.Tensor], wanted: bool, index: int, seqs: int,
+         heads: int) -> Optional[torch.Tensor]:
+    if lse is None:
+        return q.new_empty(seqs, heads) if wanted else None
+    if lse.dtype is not _F32 or lse.get_device() != index or lse.shape != (seqs, heads) or \
+            not lse.is_contiguous():
+        _refuse(lse, "lse_out", _F32, index, (seqs, heads))
+    return lse
+
+
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                     block_table: torch.Tensor, seq_lens: torch.Tensor,
                     scale: Optional[float] = None, window: int = 0, softcap: float = 0.0,
                     k_scale: float = 1.0, v_scale: float = 1.0, max_len: int = 0,
                     out: Optional[torch.Tensor] = None, return_lse: bool = False,
-                    ws: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None):
+                    ws: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None,
+                    lse_out: Optional[torch.Tensor] = None):
     """Attention of one new token per sequence, q (seqs, q_heads, head_dim),
     over the first ``seq_lens[s]`` tokens of its pages (the last ``window`` of
     them if given): softmax(scale q.k, capped at ``softcap``) v, f32.  Returns
-    out, or (out, lse) with the natural log of the softmax sums; a sequence of
-    length 0 gives zeros and -inf.  ``out`` may be q where q is contiguous.
+    out, or (out, lse) with the natural log of the softmax sums (in ``lse_out`` if
+    given); a sequence of length 0 gives zeros and -inf.  ``out`` may be q where q is contiguous.
     ``scale`` defaults to 1 / sqrt(head_dim); ``max_len`` (no sequence is
     longer; 0 = what the table holds) sizes the launch and with it the split of
     the sequences, so equal calls give equal bits, but another ``max_len`` may
@@ -534,7 +545,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     elif out.dtype is not _F32 or out.get_device() != dev or out.shape != (seqs, hq, d) or \
             not out.is_contiguous():
         _refuse(out, "out", _F32, dev, (seqs, hq, d))
-    lse = q.new_empty(seqs, hq) if return_lse else None
+    lse = _lse(q, lse_out, return_lse, dev, seqs, hq)
     if ws is None:
         ws = paged_attention_workspace(seqs, hq, hk, d, q.device)
     elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
@@ -563,7 +574,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      scale: Optional[float] = None, softcap: float = 0.0, k_scale: float = 1.0,
                      v_scale: float = 1.0, max_len: int = 0, out: Optional[torch.Tensor] = None,
                      return_lse: bool = False, ws: Optional[torch.Tensor] = None,
-                     status: Optional[torch.Tensor] = None, form: int = PREFIX_AUTO):
+                     status: Optional[torch.Tensor] = None, form: int = PREFIX_AUTO,
+                     lse_out: Optional[torch.Tensor] = None):
     """``paged_attention`` of sequences that begin with the same whole pages
     ``prefix_pages`` (n,) int32 (a system prompt, a document): their keys are
     read and multiplied once for all rows.  ``block_table`` and ``seq_lens``
@@ -583,7 +595,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     elif out.dtype is not _F32 or out.get_device() != dev or out.shape != (seqs, hq, d) or \
             not out.is_contiguous():
         _refuse(out, "out", _F32, dev, (seqs, hq, d))
-    lse = q.new_empty(seqs, hq) if return_lse else None
+    lse = _lse(q, lse_out, return_lse, dev, seqs, hq)
     if ws is None:
         ws = prefix_attention_workspace(seqs, hq, hk, d, q.device)
     elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():

@@ -54,7 +54,9 @@ class StackedMoE:
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None,
                 caches: Optional[Sequence[PagedKVCache]] = None,
                 positions: Optional[torch.Tensor] = None,
-                seq_lens: Optional[torch.Tensor] = None, max_len: int = 0) -> torch.Tensor:
+                seq_lens: Optional[torch.Tensor] = None, max_len: int = 0,
+                prefixes: Optional[Sequence[torch.Tensor]] = None,
+                slots: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x (T, d) f32 on the device -> (T, d).  The residual stream lives in
         ``out`` (allocated if not given): the first layer adds x into it,
         later layers update it in place (the combine may write over its own
@@ -62,13 +64,16 @@ class StackedMoE:
         the first of its size.
 
         With attention layers row t is the new token of sequence t:
-        ``caches`` (one per layer), ``positions`` and ``seq_lens`` as
-        ``AttentionLayer.forward`` takes them."""
+        ``caches`` (one per layer), ``positions``, ``seq_lens`` and ``slots`` as
+        ``AttentionLayer.forward`` takes them, ``prefixes`` (one per layer) its
+        ``prefix``."""
         if self.attention is not None:
             if caches is None or positions is None or seq_lens is None:
                 raise ValueError("attention layers need caches, positions and seq_lens")
             if len(caches) != len(self.layers):
                 raise ValueError(f"{len(caches)} caches for {len(self.layers)} layers")
+            if prefixes is not None and len(prefixes) != len(self.layers):
+                raise ValueError(f"{len(prefixes)} prefixes for {len(self.layers)} layers")
         xn = self._xn.rows(*x.shape, x.device)
         res = out if out is not None else torch.empty_like(x)
         cur = x
@@ -76,7 +81,9 @@ class StackedMoE:
             if self.attention is not None:
                 K.rms_norm(cur, self.attention_norms[i], self.eps, out=xn)
                 self.attention[i].forward(xn, caches[i], positions, seq_lens, residual=cur,
-                                          out=res, max_len=max_len)
+                                          out=res, max_len=max_len,
+                                          prefix=None if prefixes is None else prefixes[i],
+                                          slots=slots)
                 cur = res
             K.rms_norm(cur, nw, self.eps, out=xn)
             layer.forward_batch(xn, residual=cur, out=res)
