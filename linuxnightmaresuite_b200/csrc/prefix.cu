@@ -70,13 +70,16 @@ template <int DT, int DQ> struct PrefixCfg {
   static constexpr int kQPart = DQ / 64 * kPrefixRows * 128;
   static constexpr int kQ = kSmemParts * kQPart;
   static constexpr int kK = kKT * DQ * 2, kV = kKT * kDV * 2;
+  // stages of keys and of values; of e4m3 the loads need two of their own more than V does
   static constexpr int kStages = kE4 && DQ == 256 ? 1 : DQ == 64 ? 3 : 2;
+  static constexpr int kStagesV = kE4 && DQ == 128 ? 1 : kStages;
   static constexpr int kRawK = kE4 ? kKT * (DQ < 128 ? 128 : DQ) : 0, kRawV = kE4 ? kKT * 128 : 0;
-  static constexpr int kRawStages = kE4 ? (DQ == 128 ? 1 : 2) : 0;
-  static constexpr int kSmem = 1024 + kQ + kStages * (kK + kV) + kRawStages * (kRawK + kRawV);
+  static constexpr int kRawStages = kE4 ? 2 : 0;
+  static constexpr int kSmem =
+      1024 + kQ + kStages * kK + kStagesV * kV + kRawStages * (kRawK + kRawV);
   static constexpr int kThreads = kE4 ? 512 : 384;
   // registers of a thread by warpgroup: what the block was launched with, dealt out again
-  static constexpr int kRegsSoft = kE4 ? 208 : 224, kRegsIssue = kE4 ? 48 : 56, kRegsWiden = 48;
+  static constexpr int kRegsSoft = kE4 ? 200 : 224, kRegsIssue = kE4 ? 48 : 56, kRegsWiden = 64;
   static_assert(2 * kRegsSoft + kRegsIssue + (kE4 ? kRegsWiden : 0) <=
                     65536 / kThreads / 8 * 8 * (kThreads / 128),
                 "");
@@ -290,7 +293,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
               const PrefixArgs A) {
   using Cfg = PrefixCfg<DT, DQ>;
   constexpr bool BF = Cfg::kBf, E4 = Cfg::kE4;
-  constexpr int KT = Cfg::kKT, DV = Cfg::kDV, NS = Cfg::kStages, RS = Cfg::kRawStages;
+  constexpr int KT = Cfg::kKT, DV = Cfg::kDV, NS = Cfg::kStages, NV = Cfg::kStagesV, RS = Cfg::kRawStages;
   constexpr int BLK = KT * 128;        // a block of 64 columns of a key or value tile
   extern __shared__ uint8_t prefix_smem[];
   __shared__ PrefixShared sh;
@@ -298,7 +301,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       (reinterpret_cast<uintptr_t>(prefix_smem) + 1023) & ~(uintptr_t)1023);
   uint8_t* const ks = smem + Cfg::kQ;
   uint8_t* const vs = ks + NS * Cfg::kK;
-  uint8_t* const rk = vs + NS * Cfg::kV;
+  uint8_t* const rk = vs + NV * Cfg::kV;
   uint8_t* const rv = rk + RS * Cfg::kRawK;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -606,8 +609,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       const uint32_t io = tc_idesc(128, DV) | Cfg::kIdesc16 | (1u << 16);
       while (run.next(p)) {
         for (const int end = n + p.n; n < end; ++n) {
-          const int st = n % NS, b = n % 3;
-          warp_wait(&sh.v_full[st], (n / NS) & 1);
+          const int st = n % NV, b = n % 3;
+          warp_wait(&sh.v_full[st], (n / NV) & 1);
           warp_wait(&sh.p_full[b], (n / 3) & 1);
           const uint4 seen = sh.seen[n % 8];
           if ((seen.x & seen.y & seen.z & seen.w) != 0xffffffffu) {
@@ -651,7 +654,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       // ---- loads: q and keys, values
       const bool keys = warp == 9;
       constexpr int LINE = E4 ? 128 : 64;                  // elements of a line
-      constexpr int RING = E4 ? (RS ? RS : 1) : NS;
+      const int RING = E4 ? RS : keys ? NS : NV;
       uint64_t* full = E4 ? (keys ? sh.rk_full : sh.rv_full) : keys ? sh.k_full : sh.v_full;
       uint64_t* empty = E4 ? (keys ? sh.rk_empty : sh.rv_empty) : keys ? sh.k_empty : sh.v_empty;
       const CUtensorMap* map = keys ? &kmap : &vmap;
@@ -746,6 +749,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     auto widen = [&](const uint8_t* from, uint8_t* to, int columns) {
       constexpr int SHARE = 128 / KT;  // threads of a row
       const int r = id % KT, c0 = id / KT;
+#pragma unroll 2
       for (int c = c0; c < columns / 16; c += SHARE) {
         const uint4 v = *reinterpret_cast<const uint4*>(from + (c >> 3) * BLK + r * 128 +
                                                         (((c & 7) ^ (r & 7)) << 4));
@@ -762,26 +766,35 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       fence_proxy_async_smem();
       __syncwarp();
     };
+    auto widen_keys = [&](int t) {
+      const int rs = t % R, st = t % NS, round = t / NS;
+      warp_wait(&sh.rk_full[rs], (t / R) & 1);
+      if (round > 0) warp_wait(&sh.k_empty[st], (round - 1) & 1);
+      widen(rk + rs * Cfg::kRawK, ks + st * Cfg::kK, DQ);
+      if (lane == 0) {
+        mbar_arrive(&sh.k_full[st]);
+        mbar_arrive(&sh.rk_empty[rs]);
+      }
+    };
+    auto widen_values = [&](int t) {
+      const int rs = t % R, st = t % NV, round = t / NV;
+      warp_wait(&sh.rv_full[rs], (t / R) & 1);
+      if (round > 0) warp_wait(&sh.v_empty[st], (round - 1) & 1);
+      widen(rv + rs * Cfg::kRawV, vs + st * Cfg::kV, DV);
+      if (lane == 0) {
+        mbar_arrive(&sh.v_full[st]);
+        mbar_arrive(&sh.rv_empty[rs]);
+      }
+    };
     while (run.next(p)) {
-      for (int i = 0; i < p.n; ++i, ++n) {
-        const int rs = n % R, st = n % NS;
-        const uint32_t rr = (n / R) & 1, round = n / NS;
-        warp_wait(&sh.rk_full[rs], rr);
-        if (round > 0) warp_wait(&sh.k_empty[st], (round - 1) & 1);
-        widen(rk + rs * Cfg::kRawK, ks + st * Cfg::kK, DQ);
-        if (lane == 0) {
-          mbar_arrive(&sh.k_full[st]);
-          mbar_arrive(&sh.rk_empty[rs]);
-        }
-        warp_wait(&sh.rv_full[rs], rr);
-        if (round > 0) warp_wait(&sh.v_empty[st], (round - 1) & 1);
-        widen(rv + rs * Cfg::kRawV, vs + st * Cfg::kV, DV);
-        if (lane == 0) {
-          mbar_arrive(&sh.v_full[st]);
-          mbar_arrive(&sh.rv_empty[rs]);
-        }
+      // keys run a tile ahead of values
+      for (int i = 0; i <= p.n; ++i) {
+        if (i < p.n && (i == 0 || NS > 1)) widen_keys(n + i);
+        if (i > 0) widen_values(n + i - 1);
+        if (i > 0 && i < p.n && NS == 1) widen_keys(n + i);
         if (*(volatile int*)&sh.dead) break;
       }
+      n += p.n;
     }
   }
   tc_dealloc_all(tmem, warp);
