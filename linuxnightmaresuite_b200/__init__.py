@@ -17,7 +17,8 @@ Modules:
   ep           expert parallelism over NVLink peer memory (IPC exchange
                windows, device-side send / serve / combine)
   attention    attention half of a decode step: paged key-value cache, rotary
-               append, single-token attention, Q4_0 / Q8_0 projections
+               append, single-token attention, Q4_0 / Q8_0 projections, shared
+               prompts, eviction by accumulated attention weight
   stacked      stacked decode step (MoE layers + shared expert + RMSNorm,
                with attention layers where given)
   synth        seeded synthetic workloads as raw GGUF block bytes
