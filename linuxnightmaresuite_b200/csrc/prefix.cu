@@ -17,17 +17,22 @@
 // core truncates where it adds, so the low parts go first, an O takes one tile of
 // keys, and sums over tiles are f32 adds in registers.
 //
-// Roles: two warpgroups take every other tile each, with a maximum, sum and O of their own
-// (they meet at the end of a piece): while one is at its exponentials the tensor cores
-// serve the other.  One thread issues the products, in the order S(i), O(i - 1), so that a
-// tile's exponentials have the time of a whole tile's products; one warp loads pages by TMA, two
-// tiles ahead.  e4m3 keys and values are widened to fp16 (exact) by four more warps.  At
-// 256 columns a CTA makes 128 columns of O: two CTAs form the same scores.
+// Roles.  Two warpgroups take every other tile's exponentials each, a row to a thread; their
+// references (maxima that move only when a score is more than 2^8 above them) go from tile to tile
+// through shared memory.  A third one adds up the tiles' O.  Two threads issue the products, one S,
+// up to three tiles ahead, and one O; two warps load pages by TMA, a tile ahead.  e4m3 keys and
+// values are widened to fp16 (exact) by four more warps.  At 256 columns a CTA makes 128
+// columns of O: two CTAs form the same scores.
 //
 // Work.  A key head has RU row units (128 rows, or half of their columns).  m of them
 // (all, up to 16) are a team: CTAs that take the same keys at the same time, so that the
 // pages come from memory once, for one CTA of a team, and from L2 for the others.  Teams get equal
 // runs of tiles, across heads; a run that crosses into the next head writes two parts.
+// Bound by the tensor pipe for large batches: 256 sequences behind 32768 tokens, 8 key heads of 128
+// with 4 query heads, bf16, 272 us, of which 255 in the prefix kernel: 343 executed GFLOP (q in three
+// parts, P in two) at 1.35 PFLOP/s, 82 % of what a library product reaches in bursts.  Bound by
+// starts for small ones (launches, the first pages, the join: 15 to 20 us), which therefore go
+// sequence by sequence.
 #include <math.h>
 
 #include <algorithm>
@@ -49,8 +54,8 @@ struct PrefixArgs {
   const float* qscale;                 // score = product * qscale
   const int32_t* pages;
   int* status;
-  float2* part_ml;                     // [slot][row] (maximum in powers of two, sum)
-  float* part_o;                       // [slot][row][column of the unit]
+  float2* part_ml;                     // [slot][warpgroup][row] (reference in powers of two, sum)
+  float* part_o;                       // [slot][row][column of the unit], for the larger reference
   int rows, row_tiles, keys;           // of a key head, keys of the prefix
   int RU, m, RG, tiles, quota, parts;  // row units, team, row groups; tiles of a head; parts of a unit
   uint32_t total;                      // tiles of all teams
@@ -76,13 +81,13 @@ template <int DT, int DQ> struct PrefixCfg {
   static constexpr int kRawK = kE4 ? kKT * (DQ < 128 ? 128 : DQ) : 0, kRawV = kE4 ? kKT * 128 : 0;
   static constexpr int kRawStages = kE4 ? 2 : 0;
   static constexpr int kSmem =
-      1024 + kQ + kStages * kK + kStagesV * kV + kRawStages * (kRawK + kRawV);
-  static constexpr int kThreads = kE4 ? 512 : 384;
+      kQ + kStages * kK + kStagesV * kV + kRawStages * (kRawK + kRawV);
+  static constexpr int kThreads = kE4 ? 640 : 512;
   // registers of a thread by warpgroup: what the block was launched with, dealt out again
-  static constexpr int kRegsSoft = kE4 ? 200 : 224, kRegsIssue = kE4 ? 48 : 56, kRegsWiden = 64;
-  static_assert(2 * kRegsSoft + kRegsIssue + (kE4 ? kRegsWiden : 0) <=
-                    65536 / kThreads / 8 * 8 * (kThreads / 128),
-                "");
+  static constexpr int kRegsSoft = kE4 ? 104 : 136, kRegsSum = kE4 ? 168 : 176;
+  static constexpr int kRegsIssue = kE4 ? 48 : 64, kRegsWiden = 56;
+  static constexpr int kRegsAll = 2 * kRegsSoft + kRegsSum + kRegsIssue + (kE4 ? kRegsWiden : 0);
+  static_assert(kRegsAll <= 65536 / kThreads / 8 * 8 * (kThreads / 128), "");
   // tensor memory: three S (P over them), O, then q's third part
   static constexpr int kOCol = 3 * kKT, kQCol = kOCol + kDV;
   static_assert(kQCol + (kTmemQ ? DQ / 2 : 0) <= kTmemCols, "");
@@ -92,12 +97,13 @@ template <int DT, int DQ> struct PrefixCfg {
 struct PrefixShared {
   uint64_t q_full, k_full[3], k_empty[3], v_full[3], v_empty[3];
   uint64_t rk_full[2], rk_empty[2], rv_full[2], rv_empty[2];
-  uint64_t s_full[3], p_full[3], p_read[3], o_full[2], o_empty, drain[2];
+  uint64_t s_full[3], p_full[3], p_read[3], m_ready[2], o_full, o_empty, drain[2];
   uint32_t tmem;
   int dead;
   // keys of a tile that are there, tile t at t % 8: the loads of tile t + 8 begin when S of tile
   // t + 5 at least has been formed, in the place of P of tile t + 2
   uint4 seen[8];
+  float m[4][kPrefixRows];             // references, tile t at t % 4
 };
 
 // 32 columns of this thread's row, on their way until tmem_wait_ld
@@ -204,8 +210,8 @@ struct PrefixRowsArgs {
 template <bool BF, int DQ>
 __global__ void __launch_bounds__(256) prefix_rows_kernel(const PrefixRowsArgs A) {
   constexpr int PARTS = BF ? 3 : 2, PART = DQ / 64 * kPrefixRows * 128;
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();                       // in this order: see the loads of the prefix kernel
   const int lane = threadIdx.x & 31;
   const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int64_t tile = id / kPrefixRows;                 // head, row tile
@@ -295,17 +301,15 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
   constexpr bool BF = Cfg::kBf, E4 = Cfg::kE4;
   constexpr int KT = Cfg::kKT, DV = Cfg::kDV, NS = Cfg::kStages, NV = Cfg::kStagesV, RS = Cfg::kRawStages;
   constexpr int BLK = KT * 128;        // a block of 64 columns of a key or value tile
-  extern __shared__ uint8_t prefix_smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ PrefixShared sh;
-  uint8_t* const smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(prefix_smem) + 1023) & ~(uintptr_t)1023);
   uint8_t* const ks = smem + Cfg::kQ;
   uint8_t* const vs = ks + NS * Cfg::kK;
   uint8_t* const rk = vs + NV * Cfg::kV;
   uint8_t* const rv = rk + RS * Cfg::kRawK;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    mbar_init(&sh.q_full, 9);    // the copies, and every warp that is done with the piece before
+    mbar_init(&sh.q_full, Cfg::kTmemQ ? 9 : 1);  // the copies, and the warps that store third parts
     mbar_init(&sh.drain[0], 1);
     mbar_init(&sh.drain[1], 1);
     for (int i = 0; i < NS; ++i) {
@@ -325,8 +329,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       mbar_init(&sh.p_full[i], 128);
       mbar_init(&sh.p_read[i], 1);
     }
-    mbar_init(&sh.o_full[0], 1);
-    mbar_init(&sh.o_full[1], 1);
+    mbar_init(&sh.m_ready[0], 128);
+    mbar_init(&sh.m_ready[1], 128);
+    mbar_init(&sh.o_full, 2);
     mbar_init(&sh.o_empty, 128);
     sh.dead = 0;
     fence_mbar_init();
@@ -335,7 +340,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
   }
   const uint32_t tmem = tc_alloc_all(&sh.tmem, warp);
   pdl_trigger();
-  pdl_wait();
+  // Keys and values need not wait for q's rows: the kernel that lays those out lets this one
+  // start when all before it is done.
+  if (warp != 13 && warp != 14) pdl_wait();
 
   // Bounded; after a timeout anywhere in the CTA no wait takes long any more, nothing more
   // is issued, and the kernel ends.
@@ -357,11 +364,12 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSoft));
     const int w = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tm = tmem + lanes, O = tm + Cfg::kOCol;
+    const uint32_t tm = tmem + lanes;
     while (run.next(p)) {
       const int64_t tile = (int64_t)p.head * A.row_tiles + p.ru / Cfg::kHalves;
       const float qscale = A.qscale[tile * kPrefixRows + row];
       if (Cfg::kTmemQ) {               // third parts: this thread's row, half of its columns
+        asm volatile("bar.sync 1, 256;" ::: "memory");     // S of the piece before has been formed
         const uint8_t* q = A.q + (tile * Cfg::kParts + 2) * Cfg::kQPart + row * 128;
 #pragma unroll 1
         for (int c = w * (DQ / 2); c < (w + 1) * (DQ / 2); c += 64) {
@@ -379,38 +387,15 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         }
         tmem_wait_st();
         tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.q_full);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.q_full);
       const float to_cap = A.cap > 0.f ? fminf(qscale / A.cap, 3e38f) : 0.f;
       const float from_cap = A.cap * kLog2e;
       const float x2 = A.cap > 0.f ? 1.f : qscale * kLog2e;
-      float o[DV], m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int c = 0; c < DV; ++c) o[c] = 0.f;
-      bool first = true;
-      auto fold = [&](int t) {         // the O of tile t, and it may be written again
-        warp_wait(&sh.o_full[w], (t >> 1) & 1);
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < DV; c += 64) {
-          uint32_t v[32], u[32];
-          tmem_get32(O + c, v);
-          tmem_get32(O + c + 32, u);
-          tmem_wait_ld(v);
-          tmem_wait_ld(u);
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            o[c + k] += __uint_as_float(v[k]);
-            o[c + 32 + k] += __uint_as_float(u[k]);
-          }
-        }
-        tc_fence_before();
-        mbar_arrive(&sh.o_empty);
-      };
-      const int end = n + p.n;
-      int t = n + ((n ^ w) & 1);
-      for (; t < end; t += 2) {
+      float m = -INFINITY, l = 0.f;    // l is a sum for the reference m
+      const int start = n, end = n + p.n;
+      for (int t = n + ((n ^ w) & 1); t < end; t += 2) {
         const int b = t % 3;
         const uint32_t S = tm + (uint32_t)(b * KT);
         warp_wait(&sh.s_full[b], (t / 3) & 1);
@@ -473,19 +458,20 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
           mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         }
         mx *= x2;
-        // ---- O of the tile before this one: its product had the time of the pass above
-        if (!first) fold(t - 2);
-        if (__any_sync(0xffffffffu, mx > m + 8.f)) {
-          const float to = mx > m + 8.f ? mx : m;
-          const float f = to == -INFINITY ? 1.f : ex2(m - to);
-          if (!first) {
-#pragma unroll
-            for (int c = 0; c < DV; ++c) o[c] *= f;
-          }
-          l *= f;
+        // ---- the reference: that of the tile before, in the other warpgroup's hands, unless a score is
+        // more than 2^8 above it
+        float to = mx;
+        if (t > start) {
+          warp_wait(&sh.m_ready[(t - 1) & 1], ((t - 1) >> 1) & 1);
+          const float before = sh.m[(t - 1) & 3][row];
+          to = mx > before + 8.f ? mx : before;
+        }
+        if (to != m) {
+          l *= ex2(m - to);
           m = to;
         }
-        first = false;
+        sh.m[t & 3][row] = m;
+        mbar_arrive(&sh.m_ready[t & 1]);
         const float shift = kPShift - (m == -INFINITY ? 0.f : m);
         // ---- probabilities: 32 keys' hi parts in 16 columns, then their lo parts
         const uint64_t x22 = pack2(x2, x2), shift2 = pack2(shift, shift);
@@ -518,54 +504,56 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         tc_fence_before();
         mbar_arrive(&sh.p_full[b]);
       }
-      if (!first) fold(t - 2);
       n = end;
-      // ---- both warpgroups' parts meet in tensor memory (one in O, one in the place of
-      // S); each adds up half of the columns
-      asm volatile("bar.sync 1, 256;" ::: "memory");       // all products of the piece are done
-      const uint32_t mine = w ? tm : O, other = w ? O : tm, ml = tm + DV;
-      tmem_st2(ml + 2 * w, __float_as_uint(m), __float_as_uint(l));
-#pragma unroll
-      for (int c = 0; c < DV; c += 32) {
-        uint32_t x[32];
-#pragma unroll
-        for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(o[c + k]);
-        tmem_st32(mine + c, x);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      tc_fence_after();
-      float m1, l1;
-      tmem_ld2(ml + 2 * (w ^ 1), m1, l1);
-      const float M = fmaxf(m, m1), ms = M == -INFINITY ? 0.f : M;
-      const float f0 = ex2(m - ms), f1 = ex2(m1 - ms);
-      const bool in = p.ru / Cfg::kHalves * kPrefixRows + row < A.rows;
-      if (in && w == 0)
-        A.part_ml[(int64_t)p.slot * kPrefixRows + row] = make_float2(M, l * f0 + l1 * f1);
-      float* to = A.part_o + ((int64_t)p.slot * kPrefixRows + row) * DV;
-#pragma unroll 1
-      for (int c = w * (DV / 2); c < (w + 1) * (DV / 2); c += 32) {
-        float v[32], u[32];
-        tmem_ld32(mine + c, v);
-        tmem_ld32(other + c, u);
-#pragma unroll
-        for (int k = 0; k < 32; k += 4)
-          if (in)
-            *reinterpret_cast<float4*>(to + c + k) = make_float4(
-                v[k] * f0 + u[k] * f1, v[k + 1] * f0 + u[k + 1] * f1, v[k + 2] * f0 + u[k + 2] * f1,
-                v[k + 3] * f0 + u[k + 3] * f1);
-      }
-      tc_fence_before();
-      asm volatile("bar.sync 1, 256;" ::: "memory");       // S and O are free
-      tc_fence_after();
+      if (p.ru / Cfg::kHalves * kPrefixRows + row < A.rows)
+        A.part_ml[((int64_t)p.slot * 2 + w) * kPrefixRows + row] = make_float2(m, l);
     }
   } else if (warp < 12) {
+    // ---- the sums of O, a row to a thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSum));
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t O = tmem + ((uint32_t)((warp & 3) * 32) << 16) + Cfg::kOCol;
+    while (run.next(p)) {
+      float o[DV], m = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < DV; ++c) o[c] = 0.f;
+      const int start = n;
+      for (const int end = n + p.n; n < end; ++n) {
+        warp_wait(&sh.o_full, n & 1);
+        tc_fence_after();
+        const float to = sh.m[n & 3][row];
+        if (n > start && __any_sync(0xffffffffu, to != m)) {
+          const float f = to != m ? ex2(m - to) : 1.f;
+#pragma unroll
+          for (int c = 0; c < DV; ++c) o[c] *= f;
+        }
+        m = to;
+#pragma unroll
+        for (int c = 0; c < DV; c += 32) {
+          uint32_t v[32];
+          tmem_get32(O + c, v);
+          tmem_wait_ld(v);
+          if (c + 32 == DV) {
+            tc_fence_before();
+            mbar_arrive(&sh.o_empty);
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[c + k] += __uint_as_float(v[k]);
+        }
+      }
+      if (p.ru / Cfg::kHalves * kPrefixRows + row < A.rows) {
+        float* to = A.part_o + ((int64_t)p.slot * kPrefixRows + row) * DV;
+#pragma unroll
+        for (int c = 0; c < DV; c += 4)
+          *reinterpret_cast<float4*>(to + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+      }
+    }
+  } else if (warp < 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsIssue));
     // descriptors: rows of 128 bytes, 8 of them 1024 bytes on; of V (MN-major) 64 columns in
     // a row, the next 64 BLK on
     const uint32_t desc_hi = (uint32_t)(sw128_desc(smem) >> 32);
-    if (warp == 8) {
+    if (warp == 12) {
       // ---- S.  A thread of its own: between a tile's products the issuing thread is busy with
       // barriers for some 700 cycles, in which the other one's products run (a tile of
       // bf16 4600 cycles with both in one thread, 4000 in two)
@@ -603,7 +591,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         tc_commit(&sh.drain[0]);       // nothing is in flight when the tensor memory goes
         mbar_wait(&sh.drain[0], 0);
       }
-    } else if (warp == 11) {
+    } else if (warp == 15) {
       // ---- O
       const uint32_t v_lo = ((smem_u32(vs) >> 4) & 0x3FFF) | (uint32_t)(BLK >> 4) << 16;
       const uint32_t io = tc_idesc(128, DV) | Cfg::kIdesc16 | (1u << 16);
@@ -638,7 +626,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 for (int c = 0; c < KT / 16; ++c)
                   tc_mma_ts(d, a + 32 * (c >> 1) + 16 * k + 8 * (c & 1),
                             vb + (uint32_t)(c * 2048 >> 4), desc_hi, io, k == 0 || c > 0);
-              tc_commit(&sh.o_full[n & 1]);
+              mbar_arrive(&sh.o_full);           // the reference is there too
+              tc_commit(&sh.o_full);
               tc_commit(&sh.p_read[b]);
               tc_commit(&sh.v_empty[st]);
             }
@@ -650,9 +639,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         tc_commit(&sh.drain[1]);
         mbar_wait(&sh.drain[1], 0);
       }
-    } else if (warp < 11) {
-      // ---- loads: q and keys, values
-      const bool keys = warp == 9;
+    } else {
+      // ---- loads: keys, values
+      const bool keys = warp == 13;
       constexpr int LINE = E4 ? 128 : 64;                  // elements of a line
       const int RING = E4 ? RS : keys ? NS : NV;
       uint64_t* full = E4 ? (keys ? sh.rk_full : sh.rv_full) : keys ? sh.k_full : sh.v_full;
@@ -663,7 +652,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       uint8_t* const ring = keys ? (E4 ? rk : ks) : E4 ? rv : vs;
       const uint32_t ps = A.c.page_size, shift = A.map.box_shift;
       const int boxes = KT >> shift;
-      bool q_loads = false;
       while (run.next(p)) {
         const int x0 = keys ? 0 : p.ru % Cfg::kHalves * 128;     // this unit's columns of V
         // pages of this lane's boxes (lane, lane + 32, ...), fetched a tile ahead
@@ -683,18 +671,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
           }
         };
         fetch(p.t0);
-        if (keys) {                    // q, once the products of the piece before are done
-          if (n > 0) warp_wait(&sh.k_empty[(n - 1) % NS], ((n - 1) / NS) & 1);
-          if (lane == 0 && !*(volatile int*)&sh.dead) {
-            const int64_t tile = (int64_t)p.head * A.row_tiles + p.ru / Cfg::kHalves;
-            mbar_expect_tx(&sh.q_full, Cfg::kQ);
-#pragma unroll 1
-            for (int c = 0; c < Cfg::kQ; c += 16384)
-              bulk_g2s_plain(smem + c, A.q + tile * Cfg::kParts * Cfg::kQPart + c, 16384, &sh.q_full);
-            q_loads = true;
-          }
-          __syncwarp();
-        }
         for (int i = 0; i < p.n; ++i, ++n) {
           const int st = n % RING;
           const uint32_t round = n / RING;
@@ -731,6 +707,18 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                             page[b] * A.map.page_units + p.head * A.map.head_units, (int)slot[b],
                             &full[st]);
           __syncwarp();
+          if (keys && i == 0) {        // q, once the products of the piece before are done
+            if (n > 0) warp_wait(&sh.k_empty[(n - 1) % NS], ((n - 1) / NS) & 1);
+            else pdl_wait();
+            if (lane == 0 && !*(volatile int*)&sh.dead) {
+              const int64_t tile = (int64_t)p.head * A.row_tiles + p.ru / Cfg::kHalves;
+              mbar_expect_tx(&sh.q_full, Cfg::kQ);
+#pragma unroll 1
+              for (int c = 0; c < Cfg::kQ; c += 16384)
+                bulk_g2s_plain(smem + c, A.q + tile * Cfg::kParts * Cfg::kQPart + c, 16384, &sh.q_full);
+            }
+            __syncwarp();
+          }
           if (i + 1 < p.n) fetch(p.t0 + i + 1);
         }
       }
@@ -738,14 +726,14 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       if (*(volatile int*)&sh.dead)
         for (int k = 0; k < 2; ++k) {
           for (int s = 0; s < RING; ++s) mbar_wait(&full[s], k);
-          if (q_loads) mbar_wait(&sh.q_full, k);
+          if (keys) mbar_wait(&sh.q_full, k);
         }
     }
   } else if (E4) {
     // ---- e4m3 -> fp16, rows of 128 bytes swizzled on both sides
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsWiden));
     constexpr int R = RS ? RS : 1;
-    const int id = tid - 384;
+    const int id = tid - 512;
     auto widen = [&](const uint8_t* from, uint8_t* to, int columns) {
       constexpr int SHARE = 128 / KT;  // threads of a row
       const int r = id % KT, c0 = id / KT;
@@ -834,10 +822,10 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixJoinArgs A
     const int first = unit * A.tiles / A.quota;
     const int n = ((unit + 1) * A.tiles - 1) / A.quota - first + 1;
     const int64_t slot = (int64_t)(unit * A.m + ru - rg * A.m) * A.parts;
-    const float2* ml = A.part_ml + slot * kPrefixRows + row;
+    const float2* ml = A.part_ml + slot * 2 * kPrefixRows + row;
     const float* po = A.part_o + (slot * kPrefixRows + row) * A.DV;
     float M = own;
-    for (int j = lane; j < n; j += 32) M = fmaxf(M, ml[(int64_t)j * kPrefixRows].x);
+    for (int j = lane; j < 2 * n; j += 32) M = fmaxf(M, ml[(int64_t)j * kPrefixRows].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float ms = M == -INFINITY ? 0.f : M;
@@ -852,9 +840,10 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixJoinArgs A
     }
 #pragma unroll 4
     for (int j = 0; j < n; ++j) {
-      const float2 p = ml[(int64_t)j * kPrefixRows];
-      const float w = ex2(p.x - ms - kPShift), wv = w * A.v_scale;
-      L = fmaf(p.y, w, L);
+      const float2 p = ml[(int64_t)(2 * j) * kPrefixRows], q = ml[(int64_t)(2 * j + 1) * kPrefixRows];
+      const float wp = ex2(p.x - ms - kPShift), wq = ex2(q.x - ms - kPShift);
+      const float wv = fmaxf(wp, wq) * A.v_scale;
+      L = fmaf(p.y, wp, fmaf(q.y, wq, L));
       if (mine) {
         const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)j * kPrefixRows * A.DV + c);
         y.x = fmaf(v.x, wv, y.x);
@@ -911,7 +900,7 @@ static int prefix_workspace(const PrefixPlan& p, int seqs, int q_heads, int kv_h
   MOE_CHECK(moe_paged_attention_workspace_bytes(seqs, q_heads, kv_heads, head_dim, &own));
   cv.take<uint8_t>(own);
   float* lse = cv.take<float>((size_t)seqs * q_heads);
-  float2* ml = cv.take<float2>((size_t)p.slots * kPrefixRows);
+  float2* ml = cv.take<float2>((size_t)p.slots * 2 * kPrefixRows);
   float* o = cv.take<float>((size_t)p.slots * kPrefixRows * p.dv);
   const size_t rows = (size_t)kv_heads * (p.RU / p.halves) * kPrefixRows;
   float* qscale = cv.take<float>(rows);
@@ -944,9 +933,8 @@ static int launch_prefix(PrefixArgs& a, const PrefixRowsArgs& rows, int grid, cu
     // the warpgroups' shares come out of what the block is launched with
     cudaFuncAttributes fa;
     MOE_CUDA(cudaFuncGetAttributes(&fa, kern));
-    MOE_REQUIRE(fa.numRegs * (Cfg::kThreads / 128) >=
-                    2 * Cfg::kRegsSoft + Cfg::kRegsIssue + (Cfg::kE4 ? Cfg::kRegsWiden : 0),
-                MOE_ERR_CUDA, "the kernel was built with %d registers", fa.numRegs);
+    MOE_REQUIRE(fa.numRegs * (Cfg::kThreads / 128) >= Cfg::kRegsAll, MOE_ERR_CUDA,
+                "the kernel was built with %d registers", fa.numRegs);
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   CUtensorMap kmap, vmap;
