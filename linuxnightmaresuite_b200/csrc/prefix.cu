@@ -95,15 +95,18 @@ template <int DT, int DQ> struct PrefixCfg {
 };
 
 struct PrefixShared {
-  uint64_t q_full, k_full[3], k_empty[3], v_full[3], v_empty[3];
+  uint64_t q_full, q_empty, k_full[3], k_empty[3], v_full[3], v_empty[3];
   uint64_t rk_full[2], rk_empty[2], rv_full[2], rv_empty[2];
-  uint64_t s_full[3], p_full[3], p_read[3], m_ready[2], o_full, o_empty, drain[2];
+  uint64_t s_full[3], p_full[3], p_read[3], m_ready[4], o_full, o_empty, drain[2];
   uint32_t tmem;
   int dead;
   // keys of a tile that are there, tile t at t % 8: the loads of tile t + 8 begin when S of tile
   // t + 5 at least has been formed, in the place of P of tile t + 2
   uint4 seen[8];
-  float m[4][kPrefixRows];             // references, tile t at t % 4
+  // references, tile t at t % 4.  Warps of a warpgroup may be two tiles apart where a piece ends
+  // between them, since its first tile waits for no reference; four are not, for O of the tile before
+  // takes the probabilities of all of them
+  float m[4][kPrefixRows];
 };
 
 // 32 columns of this thread's row, on their way until tmem_wait_ld
@@ -130,13 +133,6 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
                :
                : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
-  tmem_get32(addr, r);
-  tmem_wait_ld(r);
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
@@ -146,19 +142,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
       : "memory");
-}
-__device__ __forceinline__ void tmem_st2(uint32_t addr, uint32_t a, uint32_t b) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(a), "r"(b)
-               : "memory");
-}
-__device__ __forceinline__ void tmem_ld2(uint32_t addr, float& a, float& b) {
-  uint32_t r0, r1;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];"
-               : "=r"(r0), "=r"(r1)
-               : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  a = __uint_as_float(r0);
-  b = __uint_as_float(r1);
 }
 // two f32 at a time
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -310,6 +293,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     mbar_init(&sh.q_full, Cfg::kTmemQ ? 9 : 1);  // the copies, and the warps that store third parts
+    mbar_init(&sh.q_empty, 1);
     mbar_init(&sh.drain[0], 1);
     mbar_init(&sh.drain[1], 1);
     for (int i = 0; i < NS; ++i) {
@@ -329,8 +313,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       mbar_init(&sh.p_full[i], 128);
       mbar_init(&sh.p_read[i], 1);
     }
-    mbar_init(&sh.m_ready[0], 128);
-    mbar_init(&sh.m_ready[1], 128);
+    for (int i = 0; i < 4; ++i) mbar_init(&sh.m_ready[i], 128);
     mbar_init(&sh.o_full, 2);
     mbar_init(&sh.o_empty, 128);
     sh.dead = 0;
@@ -462,7 +445,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         // more than 2^8 above it
         float to = mx;
         if (t > start) {
-          warp_wait(&sh.m_ready[(t - 1) & 1], ((t - 1) >> 1) & 1);
+          warp_wait(&sh.m_ready[(t - 1) & 3], ((t - 1) >> 2) & 1);
           const float before = sh.m[(t - 1) & 3][row];
           to = mx > before + 8.f ? mx : before;
         }
@@ -471,7 +454,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
           m = to;
         }
         sh.m[t & 3][row] = m;
-        mbar_arrive(&sh.m_ready[t & 1]);
+        mbar_arrive(&sh.m_ready[t & 3]);
         const float shift = kPShift - (m == -INFINITY ? 0.f : m);
         // ---- probabilities: 32 keys' hi parts in 16 columns, then their lo parts
         const uint64_t x22 = pack2(x2, x2), shift2 = pack2(shift, shift);
@@ -587,6 +570,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             tc_commit(&sh.s_full[b]);
             tc_commit(&sh.k_empty[st]);
           }
+          // (Not by k_empty: a parity tells a phase from the next only, and the loads of e4m3 may be
+          // further ahead of these products than its stages)
+          tc_commit(&sh.q_empty);
         }
         tc_commit(&sh.drain[0]);       // nothing is in flight when the tensor memory goes
         mbar_wait(&sh.drain[0], 0);
@@ -652,6 +638,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       uint8_t* const ring = keys ? (E4 ? rk : ks) : E4 ? rv : vs;
       const uint32_t ps = A.c.page_size, shift = A.map.box_shift;
       const int boxes = KT >> shift;
+      uint32_t pieces = 0;
       while (run.next(p)) {
         const int x0 = keys ? 0 : p.ru % Cfg::kHalves * 128;     // this unit's columns of V
         // pages of this lane's boxes (lane, lane + 32, ...), fetched a tile ahead
@@ -708,8 +695,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                             &full[st]);
           __syncwarp();
           if (keys && i == 0) {        // q, once the products of the piece before are done
-            if (n > 0) warp_wait(&sh.k_empty[(n - 1) % NS], ((n - 1) / NS) & 1);
+            if (pieces > 0) warp_wait(&sh.q_empty, (pieces - 1) & 1);
             else pdl_wait();
+            ++pieces;
             if (lane == 0 && !*(volatile int*)&sh.dead) {
               const int64_t tile = (int64_t)p.head * A.row_tiles + p.ru / Cfg::kHalves;
               mbar_expect_tx(&sh.q_full, Cfg::kQ);
@@ -880,8 +868,9 @@ static PrefixPlan prefix_plan(int seqs, int q_heads, int kv_heads, int head_dim)
   p.m = (p.RU + p.RG - 1) / p.RG;
   p.teams = std::max(1, sm_count() / p.m);
   p.units = (int64_t)kv_heads * p.RG;
-  // a unit in (tiles - 1) / quota + 2 <= teams / units + 2 parts
-  p.slots = p.m * (p.teams + 2 * p.units);
+  // a unit in (tiles - 1) / quota + 2 <= teams / units + 2 parts.  (Of all CTAs, not of those in
+  // teams, so that a workspace for more sequences is never smaller)
+  p.slots = sm_count() + 2 * p.m * p.units;
   return p;
 }
 

@@ -129,6 +129,12 @@ def test_bad_prefix_arguments_are_refused(lib):
     small = size.value
     assert lib.moe_prefix_attention_workspace_bytes(4000, 4, 2, 64, ctypes.byref(size)) == _lib.MOE_OK
     assert size.value > small
+    for heads in ((1, 1, 64), (8, 2, 128), (16, 4, 256), (24, 1, 96)):
+        last = 0                                    # a workspace serves fewer sequences too
+        for seqs in range(1, 1500, 7):
+            assert lib.moe_prefix_attention_workspace_bytes(seqs, *heads, ctypes.byref(size)) == 0
+            assert size.value >= last, (heads, seqs)
+            last = size.value
     for bad in ((-1, 4, 2, 64), (4, 5, 2, 64), (4, 4, 0, 64), (4, 4, 2, 257)):
         assert lib.moe_prefix_attention_workspace_bytes(*bad, ctypes.byref(size)) == \
             _lib.MOE_ERR_INVALID

@@ -194,6 +194,7 @@ def check_mass(c, q, lse, mass, out, scale, window=0, cap=0.0):
     ([129], 64, 20, 2, 80, "nhd"),              # ten heads: two groups
     ([1000, 5], 24, 5, 5, 192, "hnd"),
     ([70, 2], 16, 72, 2, 128, "nhd"),           # 36 heads: the keys are read twice
+    ([50, 0, 33], 8, 34, 2, 256, "hnd"),        # 17 heads of 256: of a bf16 cache twice
 ])
 def test_attention_mass(dtype, lens, page, hq, hkv, d, layout):
     c = Cache(lens, page, hkv, d, dtype, layout, seed=hq)
@@ -382,6 +383,39 @@ def test_evict_reports():
     K.cache_evict(c.k, c.v, table, c.lens, m, t, 8, status=status)
     assert status.item() == K.STATUS_BAD_PAGE and (m[0, :, :8] == 100.0).sum() == 8
     K.cache_evict(c.k, c.v, table[:0], c.lens[:0], m[:0], t[:0], 8)      # no sequences
+
+
+def test_weights_and_evictions_at_once():
+    """Two streams, each with a batch of its own, give what each gives alone."""
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    sets = []
+    for i, dtype in enumerate((F16, BF16)):
+        c = Cache([700, 90, 1500, 3], 16, 2, 128, dtype, seed=i)
+        q, lse = randn(4, 8, 128, seed=i), None
+        lse = lse_of(c, q, 128 ** -0.5)
+        m, t = ledger(4, 2, 1500, seed=i)
+        want_m = K.attention_mass(q, c.k, c.table_d, c.lens, lse, m, out=m.clone())
+        k0 = c.k.clone()
+        alone = (torch.zeros(4, 2, 64, device="cuda"), torch.zeros(4, 2, 64, dtype=torch.int32,
+                                                                   device="cuda"))
+        K.cache_evict(*c.args, c.lens, want_m, t, 64, 8, *alone, torch.empty_like(c.lens))
+        want_k = c.k.clone()
+        sets.append((c, q, lse, m, t, want_m, k0, alone, want_k))
+    for _ in range(5):
+        got = []
+        for c, *_, k0, _, _ in sets:
+            c.k.copy_(k0)
+        torch.cuda.synchronize()
+        for side, (c, q, lse, m, t, want_m, _, alone, want_k) in zip(sides, sets):
+            with torch.cuda.stream(side):
+                x = K.attention_mass(q, c.k, c.table_d, c.lens, lse, m, out=m.clone())
+                mo, ho = (torch.zeros_like(a) for a in alone)
+                K.cache_evict(*c.args, c.lens, x, t, 64, 8, mo, ho, torch.empty_like(c.lens))
+                got.append((x, mo, ho))
+        torch.cuda.synchronize()
+        for (x, mo, ho), (c, _, _, _, _, want_m, _, alone, want_k) in zip(got, sets):
+            assert torch.equal(x, want_m) and torch.equal(mo, alone[0]) and torch.equal(ho, alone[1])
+            assert torch.equal(c.k.view(torch.int16), want_k.view(torch.int16))
 
 
 def test_evict_captured_and_other_stream():

@@ -74,6 +74,22 @@ def test_prefix(dtype, own, pages, page, hq, hkv, d, layout):
     assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("d,hkv,pages,cap", [(256, 8, 100, 0.0), (192, 4, 390, 0.0), (128, 8, 110, 0.0),
+                                             (128, 8, 110, 2.0), (64, 16, 60, 0.0), (64, 16, 60, 2.0)])
+def test_prefix_next_head(dtype, d, hkv, pages, cap):
+    """CTAs whose tiles go on with another head's rows: those are not fetched while products
+    of the head before still read theirs, and each head has references of its own.  (Six calls:
+    an order of warps that is wrong need not show in each.)"""
+    x = Shared([2, 0, 1, 3, 2, 1], pages, 32, hkv, d, dtype, seed=d)
+    q = 1.5 * randn(6, 4 * hkv, d, seed=7)
+    q[:, ::3] *= 4                                   # rows, and so warps, that differ in their forms of tanh
+    first = x.call(q, softcap=cap)
+    x.check(q, *first, d ** -0.5, cap)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(x.call(q, softcap=cap), first))
+
+
 @pytest.mark.parametrize("own,pages,together", [([5, 9], 4, False), ([3] * 64, 128, True)])
 def test_prefix_form_by_size(own, pages, together):
     """Short prefixes and few sequences go one by one, the others together; equal bits of
@@ -183,6 +199,31 @@ def test_prefix_nan_beside_and_inf_within(dtype):
         keep = torch.ones(64, dtype=torch.bool)
         keep[5] = False
         assert torch.equal(out[..., keep], want[..., keep]) and torch.equal(out[:, 2:], want[:, 2:])
+
+
+def test_prefix_at_once_and_one_workspace_for_all_sizes():
+    """Two streams with a workspace each; a workspace serves smaller batches and other heads'
+    prefixes one after the other."""
+    x, y = Shared([3] * 40, 60, 16, 2, 128, F16), Shared([9, 0, 7], 33, 16, 2, 128, BF16, seed=3)
+    qx, qy = randn(40, 8, 128, seed=1), randn(3, 8, 128, seed=2)
+    want_x, want_y = x.call(qx), y.call(qy)
+    wide = K.prefix_attention_workspace(64, 8, 2, 128, "cuda")
+    for _ in range(3):
+        for s, q, want in ((x, qx, want_x), (y, qy, want_y)):
+            got = s.call(q, ws=wide)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    spaces = [K.prefix_attention_workspace(40, 8, 2, 128, "cuda") for _ in range(2)]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (s, q) in enumerate(((x, qx), (y, qy))):
+            with torch.cuda.stream(sides[i]):
+                got[i].append(s.call(q, ws=spaces[i]))
+    torch.cuda.synchronize()
+    for i, want in enumerate((want_x, want_y)):
+        assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in got[i])
+    assert [K.read_status(w) for w in spaces + [wide]] == [0, 0, 0]
 
 
 def test_prefix_captured_and_other_stream():
