@@ -20,7 +20,8 @@
 // lie in one page (as in the attention kernel); the loads run on across the ends of units, page
 // ids are fetched a tile ahead of them.  (Keys loaded by the lanes themselves, straight
 // into the operands of the products, took 367 instructions for 16 keys, most of them for
-// addresses: 64 sequences of up to 4096 keys, 8 heads of 128, bf16, 89 us.)
+// addresses: 64 sequences of up to 4096 keys, 8 heads of 128, bf16, 89 us; now 50, 78 % of
+// the memory's rate: 254 MB at 5.1 TB/s.)
 #include <math.h>
 
 #include <algorithm>

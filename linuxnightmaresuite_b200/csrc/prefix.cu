@@ -12,8 +12,9 @@
 //   P = exp(S - m), split in two 16-bit parts, written over S
 //   O = P V     tcgen05.mma, P from tensor memory, V in shared memory as TMA left it (MN-major)
 // q's rows are f32.  They enter as hi + lo fp16 (22 bits; 24 in three bf16 parts for bf16 caches,
-// since a score's error is multiplied by its exponential), P as two parts (22 bits; 16 for bf16,
-// where V has 8, which is an error of 2^-17 of a probability whatever its size).  The tensor
+// since a score's error is multiplied by its exponential), P as two parts (22 bits; 17 for bf16,
+// where V has 8, which is an error of up to 2^-18 of a probability whatever its size; a third part would
+// need tensor memory that the three score tiles take up).  The tensor
 // core truncates where it adds, so the low parts go first, an O takes one tile of
 // keys, and sums over tiles are f32 adds in registers.
 //
