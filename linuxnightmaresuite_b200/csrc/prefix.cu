@@ -30,8 +30,8 @@
 // pages come from memory once, for one CTA of a team, and from L2 for the others.  Teams get equal
 // runs of tiles, across heads; a run that crosses into the next head writes two parts.
 // Bound by the tensor pipe for large batches: 256 sequences behind 32768 tokens, 8 key heads of 128
-// with 4 query heads, bf16, 272 us, of which 255 in the prefix kernel: 343 executed GFLOP (q in three
-// parts, P in two) at 1.35 PFLOP/s, 82 % of what a library product reaches in bursts.  Bound by
+// with 4 query heads, bf16, 279 us with the rows' parts and the join: 343 executed GFLOP (q in three
+// parts, P in two) at 1.23 PFLOP/s, 75 % of what a library product reaches in bursts.  Bound by
 // starts for small ones (launches, the first pages, the join: 15 to 20 us), which therefore go
 // sequence by sequence.
 #include <math.h>
