@@ -904,7 +904,7 @@ static int prefix_workspace(const PrefixPlan& p, int seqs, int q_heads, int kv_h
 // the prefix, microseconds.  Fitted to both at 2 to 128 sequences behind 256 to 16384 tokens, heads of 64,
 // 128 and 256 of all types: the paged attention reads (mostly from L2) 7.5 MB a microsecond, 4.6 of e4m3; the
 // kernels here take 13 (28 at 256 columns) for their launches and starts and 3 (5) a tile.
-// 32 / 8 heads of 128, fp16: 8 x 4096 tokens 25.5 each, 28 together; 32 x 4096 73 and 30; 2 x 1024 10 and 22.
+// 32 / 8 heads of 128, fp16: 8 x 4096 tokens 25.5 each, 28 together; 32 x 4096 73 and 31; 2 x 1024 10 and 22.
 static bool together_pays(const moe_paged_cache& c, const PrefixPlan& p, int keys, int quota) {
   const double bytes = 2.0 * cache_elem_bytes(c.dtype) * c.seqs * c.kv_heads * c.head_dim * keys;
   const double each = bytes / (c.dtype == MOE_CACHE_E4M3 ? 4.6e6 : 7.5e6);
