@@ -102,7 +102,9 @@ struct PrefixShared {
   uint32_t tmem;
   int dead;
   // keys of a tile that are there, tile t at t % 8: the loads of tile t + 8 begin when S of tile
-  // t + 5 at least has been formed, in the place of P of tile t + 2
+  // t + 3 at least has been formed (e4m3 heads of up to 64: two stages of loads, three of keys),
+  // in the place of P of tile t.  So its last readers are the warp that issues O of tile t, which
+  // meets between the reads and the issue
   uint4 seen[8];
   // references, tile t at t % 4.  Warps of a warpgroup may be two tiles apart where a piece ends
   // between them, since its first tile waits for no reference; four are not, for O of the tile before
@@ -599,8 +601,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                                             (32 * j + lane) * 128 + (c & 7) * 16) =
                       make_uint4(0, 0, 0, 0);
             fence_proxy_async_smem();
-            __syncwarp();
           }
+          __syncwarp();                // all lanes have read `seen`
           if (lane == 0) {
             if (n > 0) wait(&sh.o_empty, (n - 1) & 1);
             if (!*(volatile int*)&sh.dead) {

@@ -258,3 +258,24 @@ def test_prefix_captured_and_other_stream():
         g.replay()
         s.check(q, out, lse, 128 ** -0.5)
     assert K.read_status(ws) == 0
+
+
+@pytest.mark.parametrize("dtype,d", [(E4M3, 64), (E4M3, 16), (E4M3, 128), (F16, 64)])
+def test_prefix_pages_missing_along_the_way(dtype, d):
+    """Each CTA has some seventeen tiles, other keys of each are missing: which ones a tile has is
+    known for eight tiles, and e4m3 heads of up to 64 come nearest to that.  (The bounds are those
+    of the keys that are there.)"""
+    pages, page = 5200, 8
+    x = Shared([3, 0, 9], pages, page, 8, d, dtype, seed=11)
+    g = torch.Generator().manual_seed(d)
+    gone = torch.rand(pages, generator=g) < 0.03
+    x.pages[gone.cuda()] = -1
+    there = (~gone).repeat_interleave(page).cuda()
+    for s in range(3):
+        keep = torch.cat([there, torch.ones(x.kd[s].shape[0] - x.P, dtype=torch.bool, device="cuda")])
+        x.kd[s], x.vd[s] = x.kd[s][keep], x.vd[s][keep]
+    q = 1.5 * randn(3, 16, d, seed=4)
+    first = x.call(q)
+    x.check(q, *first, d ** -0.5)
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(x.call(q), first))
