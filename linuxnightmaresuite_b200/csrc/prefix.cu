@@ -9,29 +9,29 @@
 //
 // The prefix kernel.  M = 128 rows of one key head, N = KT keys:
 //   S = Q K^T   tcgen05.mma, Q and K in shared memory (K-major), S in tensor memory
-//   P = exp(S - m), split in two 16-bit parts, written over S
+//   P = exp(S - m), split in 16-bit parts, written over S
 //   O = P V     tcgen05.mma, P from tensor memory, V in shared memory as TMA left it (MN-major)
-// q's rows are f32.  They enter as hi + lo fp16 (22 bits; 24 in three bf16 parts for bf16 caches,
-// since a score's error is multiplied by its exponential), P as two parts (22 bits; 17 for bf16,
-// where V has 8, which is an error of up to 2^-18 of a probability whatever its size; a third part would
-// need tensor memory that the three score tiles take up).  The tensor
-// core truncates where it adds, so the low parts go first, an O takes one tile of
-// keys, and sums over tiles are f32 adds in registers.
+// q's rows and P are f32.  They enter as hi + lo fp16 (22 bits), for bf16 caches as three bf16 parts
+// (24): as in the paged attention, whose place this one takes by size.  (P in two bf16 parts leaves
+// room for a third score tile and is a sixth fewer products, but its error of up to 2^-16 of a
+// probability was most of the whole: 256 sequences behind 32768 tokens, 2.5e-6 of the norm, now
+// 6e-7; an f32 form has 1.4e-6.)  The tensor core truncates where it adds, so the low parts go first,
+// an O takes one tile of keys, and sums over tiles are f32 adds in registers.
 //
-// Roles.  Two warpgroups take every other tile's exponentials each, a row to a thread; their
-// references (maxima that move only when a score is more than 2^8 above them) go from tile to tile
-// through shared memory.  A third one adds up the tiles' O.  Two threads issue the products, one S,
-// up to three tiles ahead, and one O; two warps load pages by TMA, a tile ahead.  e4m3 keys and
-// values are widened to fp16 (exact) by four more warps.  At 256 columns a CTA makes 128
-// columns of O: two CTAs form the same scores.
+// Roles.  Two warpgroups take every other tile's exponentials each (bf16: half of every tile's), a
+// row to a thread; their references (maxima that move only when a score is more than 2^8 above
+// them) go from tile to tile through shared memory (bf16: both find them).  A third one adds up the
+// tiles' O.  Two threads issue the products, one S, up to three tiles ahead (bf16: two), and one O;
+// two warps load pages by TMA, a tile ahead.  e4m3 keys and values are widened to fp16 (exact) by
+// four more warps.  At 256 columns a CTA makes 128 columns of O: two CTAs form the same scores.
 //
 // Work.  A key head has RU row units (128 rows, or half of their columns).  m of them
 // (all, up to 16) are a team: CTAs that take the same keys at the same time, so that the
 // pages come from memory once, for one CTA of a team, and from L2 for the others.  Teams get equal
 // runs of tiles, across heads; a run that crosses into the next head writes two parts.
 // Bound by the tensor pipe for large batches: 256 sequences behind 32768 tokens, 8 key heads of 128
-// with 4 query heads, bf16, 279 us with the rows' parts and the join: 343 executed GFLOP (q in three
-// parts, P in two) at 1.23 PFLOP/s, 75 % of what a library product reaches in bursts.  Bound by
+// with 4 query heads, bf16, 358 us with the rows' parts and the join: 412 executed GFLOP (q and P in
+// three parts) at 1.15 PFLOP/s, 70 % of what a library product reaches in bursts.  Bound by
 // starts for small ones (launches, the first pages, the join: 15 to 20 us), which therefore go
 // sequence by sequence.
 #include <math.h>
@@ -89,8 +89,15 @@ template <int DT, int DQ> struct PrefixCfg {
   static constexpr int kRegsIssue = kE4 ? 48 : 64, kRegsWiden = 56;
   static constexpr int kRegsAll = 2 * kRegsSoft + kRegsSum + kRegsIssue + (kE4 ? kRegsWiden : 0);
   static_assert(kRegsAll <= 65536 / kThreads / 8 * 8 * (kThreads / 128), "");
-  // tensor memory: three S (P over them), O, then q's third part
-  static constexpr int kOCol = 3 * kKT, kQCol = kOCol + kDV;
+  // tensor memory: tiles of S (two parts of P over them, a third one behind them), O, then q's
+  // third part
+  static constexpr int kTiles = kBf ? 2 : 3;
+  // Whether both softmax warpgroups work on a tile, half of its keys each.  With two tiles the
+  // pipe would wait for a warpgroup that has a tile to itself (256 sequences behind 32768 tokens,
+  // 393 us; 358 shared)
+  static constexpr bool kShared = kBf;
+  static constexpr int kPCols = kKT / 2 * kParts;
+  static constexpr int kOCol = kTiles * kPCols, kQCol = kOCol + kDV;
   static_assert(kQCol + (kTmemQ ? DQ / 2 : 0) <= kTmemCols, "");
   static constexpr uint32_t kIdesc16 = (kBf ? (1u << 7) | (1u << 10) : 0u);
 };
@@ -145,6 +152,25 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st1(uint32_t addr, uint32_t r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(addr), "r"(r) : "memory");
+}
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t addr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;"
+               : "=r"(r)
+               : "r"(addr)
+               : "memory");
+  return r;
 }
 // two f32 at a time
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -289,6 +315,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
   constexpr int BLK = KT * 128;        // a block of 64 columns of a key or value tile
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ PrefixShared sh;
+  static_assert(Cfg::kSmem + (sizeof(PrefixShared) + 1023) / 1024 * 1024 <= 227 * 1024, "");
   uint8_t* const ks = smem + Cfg::kQ;
   uint8_t* const vs = ks + NS * Cfg::kK;
   uint8_t* const rk = vs + NV * Cfg::kV;
@@ -311,9 +338,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       mbar_init(&sh.rk_empty[i], 4);
       mbar_init(&sh.rv_empty[i], 4);
     }
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < Cfg::kTiles; ++i) {
       mbar_init(&sh.s_full[i], 2);
-      mbar_init(&sh.p_full[i], 128);
+      mbar_init(&sh.p_full[i], Cfg::kShared ? 256 : 128);
       mbar_init(&sh.p_read[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&sh.m_ready[i], 128);
@@ -344,7 +371,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
   };
   PrefixRun run(A);
   PrefixPiece p;
-  int n = 0;                           // tiles so far: warpgroup n & 1, S n % 3
+  constexpr int NT = Cfg::kTiles, PC = Cfg::kPCols;
+  int n = 0;                           // tiles so far: S n % NT, not shared: warpgroup n & 1
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSoft));
@@ -381,10 +409,13 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       const float x2 = A.cap > 0.f ? 1.f : qscale * kLog2e;
       float m = -INFINITY, l = 0.f;    // l is a sum for the reference m
       const int start = n, end = n + p.n;
-      for (int t = n + ((n ^ w) & 1); t < end; t += 2) {
-        const int b = t % 3;
-        const uint32_t S = tm + (uint32_t)(b * KT);
-        warp_wait(&sh.s_full[b], (t / 3) & 1);
+      // this warpgroup's columns of its tiles
+      constexpr int COLS = Cfg::kShared ? KT / 2 : KT;
+      const int c0 = Cfg::kShared ? w * COLS : 0, c1 = c0 + COLS;
+      for (int t = Cfg::kShared ? n : n + ((n ^ w) & 1); t < end; t += Cfg::kShared ? 1 : 2) {
+        const int b = t % NT;
+        const uint32_t S = tm + (uint32_t)(b * PC);
+        warp_wait(&sh.s_full[b], (t / NT) & 1);
         tc_fence_after();
         const uint32_t* seen = &sh.seen[t % 8].x;
         const uint32_t all = seen[0] & seen[1] & seen[2] & seen[3];
@@ -395,7 +426,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         if (all != 0xffffffffu || A.cap > 0.f) {
           // ---- keys that are not there become minus infinity, scores cap tanh(score / cap) log2 e
 #pragma unroll 1
-          for (int c = 0; c < KT; c += 32) {
+          for (int c = c0; c < c1; c += 32) {
             uint32_t v[32];
             tmem_get32(S + c, v);
             tmem_wait_ld(v);
@@ -431,10 +462,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         }
         // ---- the largest score
 #pragma unroll 1
-        for (int c = 0; c < KT; c += 64) {
+        for (int c = c0; c < c1; c += 64) {
           uint32_t v[32], u[32];
           tmem_get32(S + c, v);
-          tmem_get32(S + c + 32, u);
+          tmem_get32(S + (COLS < 64 ? c : c + 32), u);
           tmem_wait_ld(v);
           tmem_wait_ld(u);
           float top[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
@@ -444,10 +475,22 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
           mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         }
         mx *= x2;
-        // ---- the reference: that of the tile before, in the other warpgroup's hands, unless a score is
-        // more than 2^8 above it
+        // ---- the reference: that of the tile before unless a score is more than 2^8 above it.  Of
+        // a shared tile both warpgroups find it from both maxima, else the one before is in the other
+        // warpgroup's hands
         float to = mx;
-        if (t > start) {
+        if (Cfg::kShared) {
+          // each warpgroup leaves its maximum where the other one's third parts begin, which will
+          // overwrite it itself (shared memory is full)
+          const uint32_t third = S + KT;
+          tmem_st1(third + (w ^ 1) * (KT / 4), __float_as_uint(mx));
+          tmem_wait_st();
+          tc_fence_before();
+          asm volatile("bar.sync 2, 256;" ::: "memory");
+          tc_fence_after();
+          to = mx = fmaxf(mx, __uint_as_float(tmem_ld1(third + w * (KT / 4))));
+          if (t > start && !(mx > m + 8.f)) to = m;
+        } else if (t > start) {
           warp_wait(&sh.m_ready[(t - 1) & 3], ((t - 1) >> 2) & 1);
           const float before = sh.m[(t - 1) & 3][row];
           to = mx > before + 8.f ? mx : before;
@@ -456,15 +499,15 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
           l *= ex2(m - to);
           m = to;
         }
-        sh.m[t & 3][row] = m;
-        mbar_arrive(&sh.m_ready[t & 3]);
+        if (!Cfg::kShared || w == 0) sh.m[t & 3][row] = m;
+        if (!Cfg::kShared) mbar_arrive(&sh.m_ready[t & 3]);
         const float shift = kPShift - (m == -INFINITY ? 0.f : m);
-        // ---- probabilities: 32 keys' hi parts in 16 columns, then their lo parts
+        // ---- probabilities: 32 keys' hi parts in 16 columns, then their second parts
         const uint64_t x22 = pack2(x2, x2), shift2 = pack2(shift, shift);
         uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll 1
-        for (int c = 0; c < KT; c += 32) {
-          uint32_t v[32], x[32];
+        for (int c = c0; c < c1; c += 32) {
+          uint32_t v[32], x[32], y[16];
           tmem_get32(S + c, v);
           tmem_wait_ld(v);
 #pragma unroll
@@ -476,12 +519,14 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             const uint64_t ab = pack2(a, b);
             if (k & 2) sum1 = add2(sum1, ab);
             else sum0 = add2(sum0, ab);
-            uint32_t part[2];
-            split2<BF, 2>(a, b, part);
+            uint32_t part[Cfg::kParts];
+            split2<BF, Cfg::kParts>(a, b, part);
             x[k / 2] = part[0];
             x[16 + k / 2] = part[1];
+            y[k / 2] = part[Cfg::kParts - 1];
           }
           tmem_st32(S + c, x);
+          if (Cfg::kParts == 3) tmem_st16(S + KT + c / 2, y);
         }
         float s0, s1;
         unpack2(add2(sum0, sum1), s0, s1);
@@ -550,12 +595,12 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         while (run.next(p)) {
           wait(&sh.q_full, pieces++ & 1);
           for (const int end = n + p.n; n < end; ++n) {
-            const int st = n % NS, b = n % 3;
+            const int st = n % NS, b = n % NT;
             wait(&sh.k_full[st], (n / NS) & 1);
-            if (n >= 3) wait(&sh.p_read[b], (n / 3 - 1) & 1);
+            if (n >= NT) wait(&sh.p_read[b], (n / NT - 1) & 1);
             if (*(volatile int*)&sh.dead) break;
             tc_fence_after();
-            const uint32_t d = tmem + (uint32_t)(b * KT);
+            const uint32_t d = tmem + (uint32_t)(b * PC);
             const uint32_t kb = k_lo + (uint32_t)(st * Cfg::kK >> 4);
 #pragma unroll
             for (int k = Cfg::kParts - 1; k >= 0; --k)
@@ -586,9 +631,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
       const uint32_t io = tc_idesc(128, DV) | Cfg::kIdesc16 | (1u << 16);
       while (run.next(p)) {
         for (const int end = n + p.n; n < end; ++n) {
-          const int st = n % NV, b = n % 3;
+          const int st = n % NV, b = n % NT;
           warp_wait(&sh.v_full[st], (n / NV) & 1);
-          warp_wait(&sh.p_full[b], (n / 3) & 1);
+          warp_wait(&sh.p_full[b], (n / NT) & 1);
           const uint4 seen = sh.seen[n % 8];
           if ((seen.x & seen.y & seen.z & seen.w) != 0xffffffffu) {
             // nothing of a row that is not seen counts
@@ -607,14 +652,15 @@ prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             if (n > 0) wait(&sh.o_empty, (n - 1) & 1);
             if (!*(volatile int*)&sh.dead) {
               tc_fence_after();
-              const uint32_t a = tmem + (uint32_t)(b * KT), d = tmem + Cfg::kOCol;
+              const uint32_t a = tmem + (uint32_t)(b * PC), d = tmem + Cfg::kOCol;
               const uint32_t vb = v_lo + (uint32_t)(st * Cfg::kV >> 4);
 #pragma unroll
-              for (int k = 1; k >= 0; --k)
+              for (int k = Cfg::kParts - 1; k >= 0; --k)
 #pragma unroll
                 for (int c = 0; c < KT / 16; ++c)
-                  tc_mma_ts(d, a + 32 * (c >> 1) + 16 * k + 8 * (c & 1),
-                            vb + (uint32_t)(c * 2048 >> 4), desc_hi, io, k == 0 || c > 0);
+                  tc_mma_ts(d, a + (k < 2 ? 32 * (c >> 1) + 16 * k + 8 * (c & 1) : KT + 8 * c),
+                            vb + (uint32_t)(c * 2048 >> 4), desc_hi, io,
+                            k < Cfg::kParts - 1 || c > 0);
               mbar_arrive(&sh.o_full);           // the reference is there too
               tc_commit(&sh.o_full);
               tc_commit(&sh.p_read[b]);
@@ -907,6 +953,7 @@ static int prefix_workspace(const PrefixPlan& p, int seqs, int q_heads, int kv_h
 // 128 and 256 of all types: the paged attention reads (mostly from L2) 7.5 MB a microsecond, 4.6 of e4m3; the
 // kernels here take 13 (28 at 256 columns) for their launches and starts and 3 (5) a tile.
 // 32 / 8 heads of 128, fp16: 8 x 4096 tokens 25.5 each, 28 together; 32 x 4096 73 and 31; 2 x 1024 10 and 22.
+// bf16: 26 and 30, 74 and 33, 11 and 24.
 static bool together_pays(const moe_paged_cache& c, const PrefixPlan& p, int keys, int quota) {
   const double bytes = 2.0 * cache_elem_bytes(c.dtype) * c.seqs * c.kv_heads * c.head_dim * keys;
   const double each = bytes / (c.dtype == MOE_CACHE_E4M3 ? 4.6e6 : 7.5e6);

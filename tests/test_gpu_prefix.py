@@ -7,7 +7,7 @@ import torch
 
 from linuxnightmaresuite_b200 import kernels as K
 
-from ._attention import BF16, E4M3, F16, Cache, attend
+from ._attention import BF16, E4M3, F16, SCALES, Cache, attend
 from .test_gpu_attention import randn
 
 pytestmark = pytest.mark.gpu
@@ -279,3 +279,29 @@ def test_prefix_pages_missing_along_the_way(dtype, d):
     x.check(q, *first, d ** -0.5)
     for _ in range(4):
         assert all(torch.equal(a, b) for a, b in zip(x.call(q), first))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+def test_prefix_probabilities(dtype, d):
+    """Each probability by itself: scores that are exact, a value of one for each of 16 keys in a
+    column of its own.  Numerator and denominator are off by 2^-22 for exp2 each, the arguments
+    (below 8 in magnitude: factor, reference and sum round) by 2^-22 each; the numerator's parts by
+    2^-22, which two adds that truncate bring to 2^-21; the sum of 16 by 2^-20; quotient and scale
+    by 2^-22 together."""
+    x = Shared([0, 0, 0], 1, 16, 8, d, dtype, seed=d)
+    page = int(x.pages[0])
+    ks, vs = SCALES[dtype]
+    k, v = (torch.zeros(16, 8, d, device="cuda") for _ in range(2))
+    k[..., 0] = (4 * torch.rand(16, 8, generator=torch.Generator().manual_seed(d)) - 2).cuda() / ks
+    v[range(16), :, range(16)] = 1.0
+    x.c.k[page].copy_(k), x.c.v[page].copy_(v)
+    kd = x.c.k[page].double() * ks
+    q = torch.zeros(3, 16, d, device="cuda")
+    q[..., 0] = torch.tensor([1.0, 0.5, -0.25], device="cuda")[:, None]
+    out, _ = x.call(q, scale=1.0)
+    s = torch.einsum("shd,nhd->shn", q.double(), kd.repeat_interleave(2, 1))
+    want = torch.softmax(s, -1) * vs
+    tol = 3 * 2.0 ** -21 + 2.0 ** -20 + 2.0 ** -21
+    assert ((out[..., :16] - want).abs() <= want * tol).all(), ((out[..., :16] / want - 1).abs().max(), tol)
+    assert (out[..., 16:] == 0).all()
