@@ -65,6 +65,7 @@ struct AttArgs {
   int64_t q_ss, q_hs;
   const int32_t* seq_lens;
   float *out, *lse;
+  float2* stats;                      // (maximum, sum) in the place of lse, as a part's
   int* status;
   int* arrivals;                      // one per CTA
   float2* part_ml;                    // [2 * grid][kAttHeads] (maximum, sum)
@@ -728,7 +729,8 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         const float norm = L == 0.f ? 0.f : unit / L;
 #pragma unroll
         for (int w = 0; w < NG; ++w) f[w] *= norm;
-        if (lane == 0 && A.lse) A.lse[row0 + h] = (M + (log2f(L) - kPShift)) * kLn2;
+        if (lane == 0 && A.stats) A.stats[row0 + h] = make_float2(M, L);
+        else if (lane == 0 && A.lse) A.lse[row0 + h] = (M + (log2f(L) - kPShift)) * kLn2;
       } else if (lane == 0) {
         A.part_ml[my_slot * kAttHeads + h] = make_float2(M, L);
       }
@@ -834,7 +836,8 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       float* to = A.out + (row0 + h) * D + 4 * col;
       if (4 * col < D)
         to[0] = y[j].x * norm, to[1] = y[j].y * norm, to[2] = y[j].z * norm, to[3] = y[j].w * norm;
-      if (col == 0 && A.lse) A.lse[row0 + h] = (M[j] + (log2f(L[j]) - kPShift)) * kLn2;
+      if (col == 0 && A.stats) A.stats[row0 + h] = make_float2(M[j], L[j]);
+      else if (col == 0 && A.lse) A.lse[row0 + h] = (M[j] + (log2f(L[j]) - kPShift)) * kLn2;
     }
   }
   // after a timeout copies may still be under way: give them time to land
@@ -976,8 +979,9 @@ int check_attention(const moe_paged_attention_args& r, moe_paged_cache& c) {
   return MOE_OK;
 }
 
-// The attention without the first `from` keys of each sequence that has so many.
-int attention_from(const moe_paged_attention_args& r, int from) {
+// The attention without the first `from` keys of each sequence that has so many; with stats (seqs,
+// q_heads) the maxima (powers of two) and sums times 2^kPShift go there, and lse is not written.
+int attention_from(const moe_paged_attention_args& r, int from, float2* stats) {
   AttArgs a = {};
   MOE_CHECK(check_attention(r, a.c));
   if (a.c.seqs == 0) return MOE_OK;
@@ -987,6 +991,7 @@ int attention_from(const moe_paged_attention_args& r, int from) {
   a.seq_lens = r.seq_lens;
   a.out = r.out;
   a.lse = r.lse;
+  a.stats = stats;
   a.status = static_cast<int*>(r.workspace);
   a.hq = r.q_heads;
   a.window = r.window;

@@ -21,7 +21,7 @@ struct CacheMap {
 };
 int make_cache_map(CUtensorMap* map, const moe_paged_cache& c, void* base, int keys, CacheMap* at);
 int check_attention(const moe_paged_attention_args& r, moe_paged_cache& c);
-int attention_from(const moe_paged_attention_args& r, int from);
+int attention_from(const moe_paged_attention_args& r, int from, float2* stats = nullptr);
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"

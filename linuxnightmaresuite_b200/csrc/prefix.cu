@@ -832,7 +832,7 @@ struct PrefixJoinArgs {
   const float2* part_ml;
   const float* part_o;
   const int32_t* seq_lens;
-  const float* own_lse;
+  const float2* own;                   // (maximum, sum) of a sequence's own keys
   float *out, *lse;
   int seqs, hq, G, d, DV, halves, keys;
   int RU, m, RG, tiles, quota, parts;
@@ -847,12 +847,14 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixJoinArgs A
   if (id >= (int64_t)A.seqs * A.hq) return;
   const int s = (int)(id / A.hq), h = (int)(id - (int64_t)s * A.hq), head = h / A.G;
   float* out = A.out + id * A.d;
+  // Own keys' maximum and sum come apart, as the parts' do: one logarithm of both, rounded, would
+  // leave an error of |lse| 2^-23 in the weight of own keys against the prefix
+  const float2 own = A.own[id];
   if (A.seq_lens[s] < A.keys) {        // not behind this prefix: all of its keys are its own
-    if (lane == 0 && A.lse) A.lse[id] = A.own_lse[id];
+    if (lane == 0 && A.lse) A.lse[id] = (own.x + (log2f(own.y) - kPShift)) * kLn2;
     return;
   }
   const int r = s * A.G + h - head * A.G;
-  const float own = A.own_lse[id] * kLog2e;
   for (int half = 0; half < A.halves; ++half) {
     const int ru = r / kPrefixRows * A.halves + half, row = r % kPrefixRows;
     const int rg = ru / A.m, unit = head * A.RG + rg;
@@ -861,12 +863,12 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixJoinArgs A
     const int64_t slot = (int64_t)(unit * A.m + ru - rg * A.m) * A.parts;
     const float2* ml = A.part_ml + slot * 2 * kPrefixRows + row;
     const float* po = A.part_o + (slot * kPrefixRows + row) * A.DV;
-    float M = own;
+    float M = own.x;
     for (int j = lane; j < 2 * n; j += 32) M = fmaxf(M, ml[(int64_t)j * kPrefixRows].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float ms = M == -INFINITY ? 0.f : M;
-    const float wo = ex2(own - ms);
+    const float wo = own.y * ex2(own.x - ms - kPShift);
     const int c = 4 * lane, col = half * A.DV + c;
     const bool mine = c < A.DV && col < A.d;
     float L = wo;
@@ -924,7 +926,7 @@ static PrefixPlan prefix_plan(int seqs, int q_heads, int kv_heads, int head_dim)
 }
 
 struct PrefixSpace {
-  float* lse;
+  float2* own;
   float2* ml;
   float *o, *qscale;
   uint8_t* q;
@@ -937,13 +939,13 @@ static int prefix_workspace(const PrefixPlan& p, int seqs, int q_heads, int kv_h
   size_t own = 0;                      // starts with the status
   MOE_CHECK(moe_paged_attention_workspace_bytes(seqs, q_heads, kv_heads, head_dim, &own));
   cv.take<uint8_t>(own);
-  float* lse = cv.take<float>((size_t)seqs * q_heads);
+  float2* stats = cv.take<float2>((size_t)seqs * q_heads);
   float2* ml = cv.take<float2>((size_t)p.slots * 2 * kPrefixRows);
   float* o = cv.take<float>((size_t)p.slots * kPrefixRows * p.dv);
   const size_t rows = (size_t)kv_heads * (p.RU / p.halves) * kPrefixRows;
   float* qscale = cv.take<float>(rows);
   uint8_t* q = cv.take<uint8_t>(rows * p.dq * 3 * 2);    // three parts at most
-  if (out) *out = {lse, ml, o, qscale, q, own};
+  if (out) *out = {stats, ml, o, qscale, q, own};
   *bytes = align_up(cv.used, 256);
   return MOE_OK;
 }
@@ -1064,7 +1066,6 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(t.stream);
   // the keys behind the prefix: checks q and out, and writes out
   moe_paged_attention_args own = t;
-  own.lse = ws.lse;
   own.workspace_bytes = ws.own_bytes;
   {
     ::moe::ProfScope _prof(MOE_K_PREFIX, s);
@@ -1073,8 +1074,8 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
                   ? moe::launch_prefix_dt<MOE_CACHE_BF16>(a, rows, p.dq, grid, s)
                   : moe::launch_prefix_dt<MOE_CACHE_E4M3>(a, rows, p.dq, grid, s));
   }
-  MOE_CHECK(moe::attention_from(own, P));
-  const moe::PrefixJoinArgs j = {ws.ml, ws.o, t.seq_lens, ws.lse, t.out, t.lse,
+  MOE_CHECK(moe::attention_from(own, P, ws.own));
+  const moe::PrefixJoinArgs j = {ws.ml, ws.o, t.seq_lens, ws.own, t.out, t.lse,
                                  S, t.q_heads, G, d, p.dv, p.halves, P, a.RU, a.m, a.RG,
                                  a.tiles, a.quota, a.parts, a.c.v_scale};
   {

@@ -305,3 +305,34 @@ def test_prefix_probabilities(dtype, d):
     tol = 3 * 2.0 ** -21 + 2.0 ** -20 + 2.0 ** -21
     assert ((out[..., :16] - want).abs() <= want * tol).all(), ((out[..., :16] / want - 1).abs().max(), tol)
     assert (out[..., 16:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("d", [64, 256])
+def test_prefix_and_own_keys_of_large_scores(dtype, d):
+    """Scores that are all the same and exact, up to some thousands: the output is the share of
+    own keys, whatever the scores.  Each weight is 2^7 but for the rounding of its argument, which
+    is the same one everywhere; sums of 26 and of 160 equal terms and the join round a few
+    times, 2^-24 each, exp2 of 0 and of -7 is exact: 2^-20."""
+    x = Shared([26, 26, 0, 26, 26], 10, 16, 2, d, dtype, seed=d)
+    ks, vs = SCALES[dtype]
+    for cache in (x.c.k, x.c.v):
+        cache.copy_(torch.zeros(cache.shape, device="cuda"))
+    k = torch.zeros(16, 2, d, device="cuda")
+    k[..., 0] = 14.0 / ks                           # 448 of e4m3
+    one = torch.ones(16, 2, d, device="cuda")
+    for page in x.table.flatten().unique().tolist():
+        if page >= 0:
+            x.c.k[page].copy_(k)
+            if page not in x.pages.tolist():
+                x.c.v[page].copy_(one)
+    want = torch.tensor([n / (n + 160) for n in (26, 26, 0, 26, 26)], dtype=torch.float64).cuda() * vs
+    for a in (1.0, 3.0, 9.25, 20.125, 66.625, 71.375, 150.75, 233.0, -66.625):
+        q = torch.zeros(5, 4, d, device="cuda")
+        q[..., 0] = a * torch.tensor([1.0, 1.25, 1.0, 1.5, 1.75], device="cuda")[:, None]
+        out, lse = x.call(q, scale=1.0)
+        err = (out - want[:, None, None]).abs()
+        assert (err <= want[:, None, None] * 2.0 ** -20).all(), (a, (err / want[:, None, None]).nan_to_num().max())
+        n = torch.tensor([186.0, 186.0, 160.0, 186.0, 186.0], dtype=torch.float64).cuda()
+        s = 14.0 * q[..., 0].double()
+        assert ((lse - s - n.log()[:, None]).abs() <= s.abs() * 2.0 ** -22 + 2.0 ** -20).all(), a
