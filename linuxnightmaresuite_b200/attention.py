@@ -12,7 +12,7 @@ attention its slots receive may be cut down to those that receive most.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence
 
 import torch
 
@@ -49,6 +49,7 @@ class PagedKVCache:
         self._free: List[int] = list(range(pages - 1, -1, -1))
         self._held: List[List[int]] = [[] for _ in range(max_seqs)]
         self._users = [0] * pages                # sequences of a page
+        self._prefixes: Dict[int, torch.Tensor] = {}       # by their last page, while it is in use
         self.mass = self.held = None
         if track:
             ledger = (max_seqs, kv_heads, width * page_size)
@@ -104,6 +105,7 @@ class PagedKVCache:
             self._users[page] -= 1
             if not self._users[page]:
                 self._free.append(page)
+                self._prefixes.pop(page, None)
         self.block_table[seq, keep:] = -1
 
     def release(self, seq: int) -> None:
@@ -132,14 +134,31 @@ class PagedKVCache:
             self._list(seq, pages)
 
     def prefix(self, seq: int, tokens: int) -> torch.Tensor:
-        """The pages of the first ``tokens`` tokens (whole pages) of a sequence, for
-        ``attend``: a view of its row of the block table."""
+        """The pages of the first ``tokens`` tokens (whole pages, which it holds) of a
+        sequence, for ``attend``.  A list of its own, not part of the block table: it stays
+        right for the sequences that share these pages when this one is released or
+        trimmed, and a captured step may be replayed for them.  It is made at the first
+        call, which can not be captured; later calls return the same tensor until the last
+        sequence gives the pages back."""
         if not 0 <= seq < self.max_seqs:
             raise IndexError(f"sequence {seq} of {self.max_seqs}")
         n = tokens // self.page_size
         if tokens < 0 or tokens % self.page_size or n > self.block_table.shape[1]:
             raise ValueError(f"{tokens} tokens are not whole pages of {self.page_size} of a sequence")
-        return self.block_table[seq, :n]
+        held = self._held[seq]
+        if n > len(held):
+            raise ValueError(f"sequence {seq} holds {len(held)} pages, {n} are needed")
+        if n == 0:
+            return self.block_table[seq, :0]
+        # A page that several sequences hold came to them with all pages in front of it, and
+        # those can not change while they hold it: the last page tells the list
+        pages = self._prefixes.get(held[n - 1])
+        if pages is None:
+            if self.block_table.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("call prefix() once before a capture")
+            pages = self._prefixes[held[n - 1]] = torch.tensor(
+                held[:n], dtype=torch.int32, device=self.block_table.device)
+        return pages
 
     def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
                positions: torch.Tensor, inv_freq: Optional[torch.Tensor] = None,

@@ -213,3 +213,36 @@ def test_ledger_of_a_cache():
     with pytest.raises(ValueError, match="window"):
         plain.attend(torch.zeros(3, 2, 16), t, window=3, prefix=t)
     assert attention.evict([], t, 4) is t
+
+
+def test_a_prefix_outlives_the_sequence_that_it_came_from():
+    c = PagedKVCache(10, 4, 2, 16, max_seqs=4, max_pages_per_seq=6, device="cpu")
+    c.reserve(0, 14)
+    c.share(1, 0, 8)
+    pages = c.prefix(0, 8)
+    first = pages.tolist()
+    assert first == c.block_table[0, :2].tolist()
+    assert c.prefix(1, 8) is pages                  # the same list, made once
+    c.release(0)
+    c.reserve(0, 24)                                # another prompt in its place
+    assert pages.tolist() == first == c.block_table[1, :2].tolist()
+    assert c.prefix(0, 8).tolist() == c.block_table[0, :2].tolist() != first
+    assert c.prefix(1, 8) is pages
+    # pages that went back and came again belong to another list
+    c.release(1)
+    c.release(0)
+    c.reserve(2, 4)
+    c.share(3, 2, 4)
+    c.trim(2, 0)
+    c.reserve(2, 24)
+    for s in (2, 3):
+        for n in range(len(c._held[s]) + 1):
+            assert c.prefix(s, 4 * n).tolist() == c._held[s][:n] == c.block_table[s, :n].tolist()
+    c.trim(2, 8)
+    c.reserve(2, 16)
+    for n in range(5):
+        assert c.prefix(2, 4 * n).tolist() == c._held[2][:n]
+    with pytest.raises(ValueError, match="holds 4 pages, 5"):
+        c.prefix(2, 20)
+    c.release(2), c.release(3)
+    assert not c._prefixes

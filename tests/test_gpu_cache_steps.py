@@ -196,3 +196,57 @@ def test_cut_step_captured():
         for c, e in zip(caches, eager):
             assert torch.equal(c.mass, e.mass) and torch.equal(c.held, e.held)
     assert all(c.device_status() == 0 for c in caches)
+
+
+def test_prompt_outlives_the_sequence_that_brought_it():
+    """Sequences go on behind a prompt's pages, eager and in a captured step, when the prompt's own
+    sequence has been released and its place holds another prompt."""
+    S, tokens, hkv, d, page = 64, 8192, 2, 64, 64
+    width = tokens // page + 1
+    stack, _ = normed_decoder(F16)
+    caches = [PagedKVCache(2 * width + S, page, hkv, d, S + 1, width, F16) for _ in range(2)]
+
+    def bring(seed):
+        for li, c in enumerate(caches):
+            c.reserve(S, tokens)
+            c.append(None, randn(tokens, hkv, d, seed=seed + li), randn(tokens, hkv, d, seed=seed + 9 + li),
+                     torch.arange(tokens, dtype=torch.int32, device="cuda"),
+                     seq_ids=torch.full((tokens,), S, dtype=torch.int32, device="cuda"))
+    bring(1)
+    for c in caches:
+        for s in range(S):
+            c.share(s, S, tokens)
+            c.reserve(s, tokens + 1)
+    x, out = randn(S, 512, seed=3), torch.zeros(S, 512, device="cuda")
+    pos, lens = i32(*[tokens] * S), i32(*[tokens + 1] * S)
+    prefixes = [c.prefix(S, tokens) for c in caches]
+
+    def step(lists):
+        return stack.forward(x, out=out, caches=caches, positions=pos, seq_lens=lens, prefixes=lists,
+                             max_len=tokens + 1)
+    want = step(prefixes).clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(prefixes)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step([c.prefix(0, tokens) for c in caches])         # made above: the same lists
+    for other in (None, 20):
+        for c in caches:
+            c.release(S)
+        if other:
+            bring(other)
+        for again in (lambda: step(prefixes), lambda: step([c.prefix(5, tokens) for c in caches]),
+                      g.replay):
+            out.zero_()
+            again()
+            assert torch.equal(out, want)
+    assert all(c.device_status() == 0 for c in caches)
+    assert all(a.device_status() == 0 for a in stack.attention)
+    c = caches[0]
+    with pytest.raises(RuntimeError, match="before a capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            x.add_(0.0)
+            c.prefix(S, 2 * page)
