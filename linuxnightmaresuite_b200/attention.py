@@ -50,6 +50,7 @@ class PagedKVCache:
         self._held: List[List[int]] = [[] for _ in range(max_seqs)]
         self._users = [0] * pages                # sequences of a page
         self._prefixes: Dict[int, torch.Tensor] = {}       # by their last page, while it is in use
+        self._cut = set()                        # sequences that an eviction may have cut down
         self.mass = self.held = None
         if track:
             ledger = (max_seqs, kv_heads, width * page_size)
@@ -97,6 +98,8 @@ class PagedKVCache:
         if not 0 <= seq < self.max_seqs:
             raise IndexError(f"sequence {seq} of {self.max_seqs}")
         keep = -(-max(int(tokens), 0) // self.page_size)
+        if keep == 0:
+            self._cut.discard(seq)
         gone = self._held[seq][keep:]
         if not gone:
             return
@@ -173,6 +176,15 @@ class PagedKVCache:
                              seq_ids, interleaved, self.k_scale, self.v_scale, q_out, self.status,
                              q_norm, k_norm, eps, gemma_style, slots, self.mass, self.held)
 
+    def check_window(self, window: int, seqs: int, prefix: Optional[torch.Tensor] = None) -> None:
+        """Refuses a window over the first ``seqs`` sequences where it would not be the newest
+        tokens: behind an eviction those sit in any slots, until the sequence is released."""
+        if window and prefix is not None:
+            raise ValueError("a window does not go with a shared prefix")
+        if window and self._cut and min(self._cut) < seqs:
+            raise ValueError(f"a window does not go with an eviction: sequence {min(self._cut)} has "
+                             "been cut down, its slots are not in the order of its tokens")
+
     def attend(self, q: torch.Tensor, seq_lens: torch.Tensor, scale: Optional[float] = None,
                window: int = 0, softcap: float = 0.0, max_len: int = 0,
                out: Optional[torch.Tensor] = None, return_lse: bool = False,
@@ -183,13 +195,12 @@ class PagedKVCache:
         the call, and its status bits go where the append's do.  ``prefix``: the
         pages that all of these sequences begin with (``kernels.prefix_attention``
         and its workspace; no window)."""
+        self.check_window(window, q.shape[0], prefix)
         table, status = self.block_table[:q.shape[0]], self.status if ws is None else None
         if prefix is None:
             return K.paged_attention(q, self.k, self.v, table, seq_lens, scale, window, softcap,
                                      self.k_scale, self.v_scale, max_len, out, return_lse, ws,
                                      status, lse_out)
-        if window:
-            raise ValueError("a window does not go with a shared prefix")
         return K.prefix_attention(q, self.k, self.v, table, seq_lens, prefix, scale, softcap,
                                   self.k_scale, self.v_scale, max_len, out, return_lse, ws, status,
                                   lse_out=lse_out)
@@ -202,6 +213,7 @@ class PagedKVCache:
         if self.mass is None:
             raise ValueError("the cache keeps no ledger (track=True)")
         S = q.shape[0]
+        self.check_window(window, S)
         K.attention_mass(q, self.k, self.block_table[:S], seq_lens, lse, self.mass[:S], scale, window,
                          softcap, self.k_scale, max_len, status=self.status)
 
@@ -210,13 +222,16 @@ class PagedKVCache:
         """Cuts the first ``len(seq_lens)`` sequences down to ``keep`` slots each
         (``kernels.cache_evict``), in place; ``lens_out`` (default: seq_lens itself)
         receives the new lengths.  ``trim`` then gives their pages back.  Layers that
-        share seq_lens: see ``evict``."""
+        share seq_lens: see ``evict``.  Windows are refused from then on, until a sequence
+        is released."""
         if self.mass is None:
             raise ValueError("the cache keeps no ledger (track=True)")
         S = seq_lens.shape[0]
-        return K.cache_evict(self.k, self.v, self.block_table[:S], seq_lens, self.mass[:S],
+        lens = K.cache_evict(self.k, self.v, self.block_table[:S], seq_lens, self.mass[:S],
                              self.held[:S], keep, recent, lens_out=lens_out, max_len=max_len,
                              status=self.status)
+        self._cut.update(range(S))
+        return lens
 
     def device_status(self) -> int:
         """Reads and clears the device status bits of the appends, of the ledger
@@ -308,6 +323,14 @@ class AttentionLayer:
                 rows, self.q_heads, self.kv_heads, self.head_dim, self.device)
         return ws
 
+    def check_step(self, seqs: int, cache: PagedKVCache, prefix: Optional[torch.Tensor] = None,
+                   slots: Optional[torch.Tensor] = None) -> None:
+        """Refuses what ``forward`` can not take together, before anything is written."""
+        if self.window and slots is not None:
+            raise ValueError("a window counts slots and does not go with slots apart from the "
+                             "positions")
+        cache.check_window(self.window, seqs, prefix)
+
     def forward(self, xn: torch.Tensor, cache: PagedKVCache, positions: torch.Tensor,
                 seq_lens: torch.Tensor, residual: Optional[torch.Tensor] = None,
                 out: Optional[torch.Tensor] = None, max_len: int = 0,
@@ -320,13 +343,14 @@ class AttentionLayer:
         for the longest sequence that the table holds.
         ``prefix``: the pages that all of these sequences begin with
         (``PagedKVCache.prefix``).  ``slots`` (int32): where the new tokens go, if
-        that is not their positions (behind an eviction seq_lens - 1).  A cache with
-        a ledger receives the step's attention.
+        that is not their positions (behind an eviction seq_lens - 1).  A layer with a
+        window takes neither.  A cache with a ledger receives the step's attention.
         Returns Wo attention (+ residual); ``out`` may be ``residual``.
         Allocates nothing after the first call of a size (but ``out`` when not
         given), and the buffers stay where they are, so captured steps of
         several sizes can be replayed in any order, one after the other."""
         T = xn.shape[0]
+        self.check_step(T, cache, prefix, slots)
         hq, hk, d = self.q_heads, self.kv_heads, self.head_dim
         qkv, att, ws = self._buffers(T)
         K.linear(xn, self.w_qkv, out=qkv)

@@ -55,7 +55,7 @@ class StackedMoE:
                 caches: Optional[Sequence[PagedKVCache]] = None,
                 positions: Optional[torch.Tensor] = None,
                 seq_lens: Optional[torch.Tensor] = None, max_len: int = 0,
-                prefixes: Optional[Sequence[torch.Tensor]] = None,
+                prefixes: Optional[Sequence[Optional[torch.Tensor]]] = None,
                 slots: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x (T, d) f32 on the device -> (T, d).  The residual stream lives in
         ``out`` (allocated if not given): the first layer adds x into it,
@@ -65,8 +65,8 @@ class StackedMoE:
 
         With attention layers row t is the new token of sequence t:
         ``caches`` (one per layer), ``positions``, ``seq_lens`` and ``slots`` as
-        ``AttentionLayer.forward`` takes them, ``prefixes`` (one per layer) its
-        ``prefix``."""
+        ``AttentionLayer.forward`` takes them, ``prefixes`` (one per layer, None for
+        layers that take none: those with a window) its ``prefix``."""
         if self.attention is not None:
             if caches is None or positions is None or seq_lens is None:
                 raise ValueError("attention layers need caches, positions and seq_lens")
@@ -74,6 +74,8 @@ class StackedMoE:
                 raise ValueError(f"{len(caches)} caches for {len(self.layers)} layers")
             if prefixes is not None and len(prefixes) != len(self.layers):
                 raise ValueError(f"{len(prefixes)} prefixes for {len(self.layers)} layers")
+            for i, layer in enumerate(self.attention):
+                layer.check_step(x.shape[0], caches[i], prefixes and prefixes[i], slots)
         xn = self._xn.rows(*x.shape, x.device)
         res = out if out is not None else torch.empty_like(x)
         cur = x

@@ -8,6 +8,7 @@ import torch
 
 from linuxnightmaresuite_b200 import _lib, attention, kernels as K
 from linuxnightmaresuite_b200.attention import PagedKVCache
+from linuxnightmaresuite_b200.stacked import StackedMoE
 
 from .test_attention_cpu import BAD_CACHES, cache, lib, test_argument_record_matches_header as _match
 
@@ -246,3 +247,66 @@ def test_a_prefix_outlives_the_sequence_that_it_came_from():
         c.prefix(2, 20)
     c.release(2), c.release(3)
     assert not c._prefixes
+
+
+def _layer(window):
+    """An attention layer whose projections are never reached."""
+    layer = attention.AttentionLayer.__new__(attention.AttentionLayer)
+    layer.window, layer.q_heads, layer.kv_heads, layer.head_dim = window, 2, 2, 16
+    return layer
+
+
+def test_windows_are_refused_where_slots_are_not_in_order(monkeypatch):
+    """Before a step has written anything, in any layer."""
+    class Reached(Exception):
+        pass
+
+    def reached(*a, **k):
+        raise Reached
+
+    for name in ("rms_norm", "rope_append", "linear", "paged_attention", "prefix_attention",
+                 "attention_mass"):
+        monkeypatch.setattr(K, name, reached)
+    monkeypatch.setattr(K, "cache_evict", lambda *a, **k: a[3])
+    monkeypatch.setattr(attention.AttentionLayer, "_buffers", reached)
+    caches = [PagedKVCache(8, 4, 2, 16, max_seqs=3, device="cpu", track=True) for _ in range(2)]
+    x, t = torch.zeros(2, 64), torch.zeros(2, dtype=torch.int32)
+    pages, q = torch.zeros(1, dtype=torch.int32), torch.zeros(2, 2, 16)
+    plain, windowed = _layer(0), _layer(5)
+    stack = StackedMoE([None, None], [None, None], attention=[plain, windowed],
+                       attention_norms=[None, None])
+    step = dict(caches=caches, positions=t, seq_lens=t)
+
+    def calls(**more):
+        return (lambda: windowed.forward(x, caches[1], t, t, **more),
+                lambda: stack.forward(x, **step, slots=more.get("slots"),
+                                      prefixes=[more["prefix"]] * 2 if "prefix" in more else None))
+    for call in calls(slots=t) + calls(prefix=pages):
+        with pytest.raises(ValueError, match="window"):
+            call()
+    # these go through: no window; windows where nothing was cut; None for the layer with a window
+    for call in calls() + (lambda: plain.forward(x, caches[0], t, t, slots=t),
+                           lambda: stack.forward(x, **step, prefixes=[pages, None]),
+                           lambda: caches[1].attend(q, t, window=3),
+                           lambda: caches[1].weigh(q, t, q[..., 0], window=3)):
+        with pytest.raises(Reached):
+            call()
+    assert attention.evict(caches, t, 4) is t
+    for call in calls() + (lambda: caches[1].attend(q, t, window=3),
+                           lambda: caches[1].weigh(q, t, q[..., 0], window=3)):
+        with pytest.raises(ValueError, match="eviction: sequence 0 has been cut"):
+            call()
+    with pytest.raises(Reached):
+        caches[1].attend(q, t)                      # no window
+    caches[1].release(0)
+    with pytest.raises(ValueError, match="sequence 1 has"):
+        caches[1].attend(q, t, window=3)
+    with pytest.raises(Reached):                    # its row is not among these
+        caches[1].attend(q[:1], t[:1], window=3)
+    caches[1].trim(1, 1)
+    with pytest.raises(ValueError, match="sequence 1 has"):
+        caches[1].attend(q, t, window=3)
+    caches[1].release(1)
+    for call in calls():
+        with pytest.raises(Reached):
+            call()
