@@ -314,11 +314,14 @@ class AttentionLayer:
                 self._att.rows(T, hq * d, self.device).view(T, hq, d), self._ws)
         return parts
 
-    def _prefix_workspace(self, T: int) -> torch.Tensor:
-        """As the row buffers: one for each power of two of rows, never replaced."""
+    def _prefix_workspace(self, T: int) -> Optional[torch.Tensor]:
+        """As the row buffers: one for each power of two of rows, never replaced.  None
+        where it would have to be made in a capture: it would be cleared when the
+        graph is replayed, but not before a call that is not part of the graph (then
+        one is made for the captured call alone, with its status in the cache's)."""
         rows = 1 << max(T - 1, 0).bit_length()
         ws = self._prefix_ws.get(rows)
-        if ws is None:
+        if ws is None and not torch.cuda.is_current_stream_capturing():
             ws = self._prefix_ws[rows] = K.prefix_attention_workspace(
                 rows, self.q_heads, self.kv_heads, self.head_dim, self.device)
         return ws

@@ -250,3 +250,44 @@ def test_prompt_outlives_the_sequence_that_brought_it():
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             x.add_(0.0)
             c.prefix(S, 2 * page)
+
+
+def test_first_step_behind_a_prefix_captured():
+    """The workspace of the first call of a size is not one that only the graph's replays clear:
+    steps outside of the graph, before it is replayed and after, give the same."""
+    S, tokens, page = 33, 4096, 64
+    width = tokens // page + 1
+    stack, _ = normed_decoder(F16)
+    caches = [PagedKVCache(width + S, page, 2, 64, S + 1, width, F16) for _ in range(2)]
+    for li, c in enumerate(caches):
+        c.reserve(S, tokens)
+        c.append(None, randn(tokens, 2, 64, seed=li), randn(tokens, 2, 64, seed=5 + li),
+                 torch.arange(tokens, dtype=torch.int32, device="cuda"),
+                 seq_ids=torch.full((tokens,), S, dtype=torch.int32, device="cuda"))
+        for s in range(S):
+            c.share(s, S, tokens)
+            c.reserve(s, tokens + 1)
+    x, out = randn(S, 512, seed=3), torch.zeros(S, 512, device="cuda")
+    pos, lens = i32(*[tokens] * S), i32(*[tokens + 1] * S)
+    prefixes = [c.prefix(S, tokens) for c in caches]
+    kw = dict(out=out, caches=caches, positions=pos, seq_lens=lens, max_len=tokens + 1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                   # everything but the prefix
+        stack.forward(x, **kw)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        stack.forward(x, prefixes=prefixes, **kw)
+    assert not any(a._prefix_ws for a in stack.attention)
+    stack.forward(x, prefixes=prefixes, **kw)
+    want = out.clone()
+    for again in (g.replay, lambda: stack.forward(x, prefixes=prefixes, **kw), g.replay, g.replay):
+        out.zero_()
+        again()
+        assert torch.equal(out, want)
+    assert all(a._prefix_ws and a.device_status() == 0 for a in stack.attention)
+    assert all(c.device_status() == 0 for c in caches)
+    caches[0].block_table[3, width - 1] = -1        # reported by replays too
+    g.replay()
+    assert caches[0].device_status() == K.STATUS_BAD_PAGE and caches[1].device_status() == 0
