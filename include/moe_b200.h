@@ -548,7 +548,8 @@ int moe_linear_record(const moe_linear_args* args);
  * prompt, a document): their keys are read and multiplied once, for the rows of all sequences
  * together.
  *   attention: as moe_paged_attention takes them, but for window, which must be 0, and workspace,
- *          whose size is moe_prefix_attention_workspace_bytes.  out 16-byte aligned
+ *          whose size is moe_prefix_attention_workspace_bytes.  out 16-byte aligned, unless
+ *          prefix_pages is 0 or form is MOE_PREFIX_EACH
  *   prefix (prefix_pages,) int32: the pages, which are also the first ones in the row of the block
  *          table of each sequence that is as long as the prefix or longer.  (Either may be read.)
  *          Shorter sequences may have any pages

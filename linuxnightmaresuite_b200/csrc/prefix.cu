@@ -1022,7 +1022,9 @@ int moe_prefix_attention_record(const moe_prefix_attention_args* r) {
   MOE_REQUIRE(t.window == 0, MOE_ERR_UNSUPPORTED, "a window does not go with a shared prefix");
   if (a.c.seqs == 0) return MOE_OK;
   MOE_REQUIRE(r->prefix || r->prefix_pages == 0, MOE_ERR_INVALID, "null pointer");
-  MOE_REQUIRE((uintptr_t)t.out % 16 == 0, MOE_ERR_INVALID, "out must be 16-byte aligned");
+  // (whatever form the sizes choose; the paged attention alone takes any)
+  MOE_REQUIRE((uintptr_t)t.out % 16 == 0 || r->prefix_pages == 0 || r->form == MOE_PREFIX_EACH,
+              MOE_ERR_INVALID, "out must be 16-byte aligned");
   MOE_REQUIRE(r->form >= MOE_PREFIX_AUTO && r->form <= MOE_PREFIX_TOGETHER, MOE_ERR_INVALID,
               "form %d not known", r->form);
   const int S = a.c.seqs, d = a.c.head_dim, P = r->prefix_pages * a.c.page_size;

@@ -581,8 +581,9 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     read and multiplied once for all rows.  ``block_table`` and ``seq_lens``
     cover whole sequences, the prefix included: the rows of those that are as
     long as the prefix or longer begin with its pages; shorter ones (0:
-    padding) may have any.  ``ws`` comes from ``prefix_attention_workspace``; all
-    else as in ``paged_attention``, whose result it is but for the last bits.
+    padding) may have any.  ``ws`` comes from ``prefix_attention_workspace``,
+    ``out`` is 16-byte aligned (without prefix pages, or with ``PREFIX_EACH``, any);
+    all else as in ``paged_attention``, whose result it is but for the last bits.
     ``form`` (``PREFIX_*``) pins the kernels; the default chooses by the sizes."""
     c, dev, seqs, hk, d = _paged_cache(k_cache, v_cache, block_table, k_scale, v_scale)
     shape = q.shape

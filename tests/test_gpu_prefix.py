@@ -336,3 +336,18 @@ def test_prefix_and_own_keys_of_large_scores(dtype, d):
         n = torch.tensor([186.0, 186.0, 160.0, 186.0, 186.0], dtype=torch.float64).cuda()
         s = 14.0 * q[..., 0].double()
         assert ((lse - s - n.log()[:, None]).abs() <= s.abs() * 2.0 ** -22 + 2.0 ** -20).all(), a
+
+
+def test_prefix_out_off_16_bytes():
+    """Refused where the forms go by the sizes; where the paged attention alone runs, taken."""
+    x = Shared([3, 8], 4, 16, 2, 64, F16)
+    q = randn(2, 4, 64)
+    out = torch.empty(2 * 4 * 64 + 1, device="cuda")[1:].view(2, 4, 64)
+    for form in (K.PREFIX_AUTO, K.PREFIX_TOGETHER):
+        with pytest.raises(Exception, match="16-byte"):
+            x.call(q, form, out=out)
+    want = K.paged_attention(q, x.c.k, x.c.v, x.table, x.lens)
+    assert torch.equal(x.call(q, K.PREFIX_EACH, out=out)[0], want)
+    out.zero_()
+    K.prefix_attention(q, x.c.k, x.c.v, x.table, x.lens, x.pages[:0], out=out)
+    assert torch.equal(out, want)
