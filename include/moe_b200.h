@@ -638,7 +638,9 @@ int moe_attention_mass_record(const moe_attention_mass_args* args);
  *         be its input itself.  Otherwise the entries that stay are copied.  Entries from
  *         `keep` on, or behind a shorter sequence's length, are left as they were
  *   max_len no sequence is longer (0 = what table and ledger hold; at most 163840): it sizes the
- *         launch.  A longer one sets MOE_STATUS_BAD_PAGE and is left as it is
+ *         launch and picks the kernel, so a step that gives up one slot names keep + 1: up to 8
+ *         slots are looked for one by one (128 x 1025 slots of 8 heads 9 us, otherwise 30).  A longer
+ *         sequence sets MOE_STATUS_BAD_PAGE and is left as it is
  *   status int32 that receives MOE_STATUS_BAD_PAGE (also for a page that does not exist,
  *         whose slots' k and v are not moved), or NULL
  * A page that several sequences share is changed for all of them: give up no shared pages.

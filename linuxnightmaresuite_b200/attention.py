@@ -29,7 +29,11 @@ class PagedKVCache:
 
     With ``track`` the cache has a ledger, ``mass`` and ``held`` (max_seqs,
     kv_heads, slots): the attention that each slot has received (``weigh``) and
-    the position of the token in it, by which ``evict`` cuts sequences down."""
+    the position of the token in it, by which ``evict`` cuts sequences down.  Its
+    slots are ``max_pages_per_seq`` pages for each sequence, 8 bytes each and key
+    head: give that number, without it the ledger has room for the whole pool
+    ``max_seqs`` times.  An append sets a slot's mass to 0; what a prompt that the
+    host appends has received is the host's to write."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, max_seqs: int,
                  max_pages_per_seq: Optional[int] = None, dtype: torch.dtype = torch.float16,
@@ -221,8 +225,9 @@ class PagedKVCache:
               lens_out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Cuts the first ``len(seq_lens)`` sequences down to ``keep`` slots each
         (``kernels.cache_evict``), in place; ``lens_out`` (default: seq_lens itself)
-        receives the new lengths.  ``trim`` then gives their pages back.  Layers that
-        share seq_lens: see ``evict``.  Windows are refused from then on, until a sequence
+        receives the new lengths.  ``max_len``, which no sequence exceeds, picks the kernel:
+        ``keep + 1`` where each step gives up one slot.  ``trim`` then gives their pages
+        back.  Layers that share seq_lens: see ``evict``.  Windows are refused from then on, until a sequence
         is released."""
         if self.mass is None:
             raise ValueError("the cache keeps no ledger (track=True)")
@@ -244,7 +249,8 @@ class PagedKVCache:
 def evict(caches: Sequence[PagedKVCache], seq_lens: torch.Tensor, keep: int, recent: int = 0,
           max_len: int = 0) -> torch.Tensor:
     """``PagedKVCache.evict`` in the caches of all layers, which share seq_lens: each
-    layer keeps slots of its own choice, and the lengths change once, at the end."""
+    layer keeps slots of its own choice, and the lengths change once, at the end.
+    ``max_len``: ``keep + 1`` where each step gives up one slot."""
     others = torch.empty_like(seq_lens)
     for cache in caches[:-1]:
         cache.evict(seq_lens, keep, recent, max_len, others)

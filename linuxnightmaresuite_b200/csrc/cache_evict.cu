@@ -11,10 +11,11 @@
 // The keep-th largest key comes from a radix select of four digits: counts in
 // shared memory, added up across the cluster, and the digit found by a scan.  Then the movers'
 // numbers are prefix sums; CTA k % C gets mover k in a list and copies its rows, 16 bytes a
-// lane.  Where few slots leave, one CTA takes them one by one.
+// lane.  Where few slots leave, by the longest length that the call allows, one CTA takes them one
+// by one.
 //
-// Bound by latency where few slots leave (128 sequences, one slot of 1025 each, 8 heads: 9.7 us a
-// call, the host's time for it; by radix select 65), by memory where long prompts are cut: 6 of up to
+// Bound by latency where few slots leave (128 sequences, one slot of 1025 each, 8 heads: 9.1 us on
+// the device, about the host's time for the call; by radix select 30), by memory where long prompts are cut: 6 of up to
 // 32768 tokens to 4096, 8 heads of 128, fp16, 76 us, 40 of them the rows that move, 256 bytes
 // each at random, read and written once at 4.3 TB/s; the rest the digits' barriers across the
 // cluster.  Digits of 11 bits took 204: counts of a cluster are 64 KB a digit through its network.
@@ -32,7 +33,15 @@ constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictCluster = 8;
 constexpr int kEvictSlots = 20480;     // of a CTA at most: 8 bytes each in shared memory
 constexpr int kBins = 256;             // a thread each
-constexpr int kFew = 8;                // slots that leave one by one
+// Slots that leave one by one, of sequences of so many slots at most.  Device time in place, 8 heads,
+// one by one and by radix select, us, one slot of n + 1 (eight of 4100 in the last column):
+//                  n = 1024    4096      8192      16384     32767      4100
+//   1 sequence    4.6 / 10   6.1 / 14  8.3 / 16   12 / 17    20 / 19   9.2 / 15
+//   16 sequences  5.4 / 11   6.4 / 28  8.9 / 49   13 / 53    21 / 63   9.9 / 30
+//   64 sequences  6.1 / 20   7.9 / 43   12 / 56   25 / 78  134 / 288    14 / 45
+// With results apart one CTA of a head copies its ledger too, which costs more than the select from 8192
+// slots of up to 4 sequences on (1 x 16384 34 / 20, 1 x 32767 65 / 24).
+constexpr int kFew = 8;
 constexpr int kFewSlots = 32768;
 
 struct EvictArgs {
@@ -134,7 +143,7 @@ struct EvictRows {
 
 // ---------------------------------------------------------------------------
 // Few slots leave (a decode step at the limit): one CTA of a (sequence, head) takes away the
-// smallest key so often.
+// smallest key so often.  Registers 40, no spills; the form for any number spills 28 bytes.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(kEvictThreads, 6) evict_few_kernel(const EvictArgs A) {
   extern __shared__ __align__(16) uint8_t smem[];
