@@ -53,7 +53,10 @@ class PagedKVCache:
         self._free: List[int] = list(range(pages - 1, -1, -1))
         self._held: List[List[int]] = [[] for _ in range(max_seqs)]
         self._users = [0] * pages                # sequences of a page
-        self._prefixes: Dict[int, torch.Tensor] = {}       # by their last page, while it is in use
+        # lists of shared pages by their last page, while it is in use; then, by length, for others: a
+        # captured step may hold their addresses, so their memory is never given back
+        self._prefixes: Dict[int, torch.Tensor] = {}
+        self._spare: Dict[int, List[torch.Tensor]] = {}
         self._cut = set()                        # sequences that an eviction may have cut down
         self.mass = self.held = None
         if track:
@@ -112,7 +115,9 @@ class PagedKVCache:
             self._users[page] -= 1
             if not self._users[page]:
                 self._free.append(page)
-                self._prefixes.pop(page, None)
+                pages = self._prefixes.pop(page, None)
+                if pages is not None:
+                    self._spare.setdefault(pages.numel(), []).append(pages)
         self.block_table[seq, keep:] = -1
 
     def release(self, seq: int) -> None:
@@ -145,8 +150,8 @@ class PagedKVCache:
         sequence, for ``attend``.  A list of its own, not part of the block table: it stays
         right for the sequences that share these pages when this one is released or
         trimmed, and a captured step may be replayed for them.  It is made at the first
-        call, which can not be captured; later calls return the same tensor until the last
-        sequence gives the pages back."""
+        call, which can not be captured; later calls return the same tensor.  When the
+        last sequence has given the pages back it may become another prompt's list."""
         if not 0 <= seq < self.max_seqs:
             raise IndexError(f"sequence {seq} of {self.max_seqs}")
         n = tokens // self.page_size
@@ -163,8 +168,10 @@ class PagedKVCache:
         if pages is None:
             if self.block_table.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call prefix() once before a capture")
-            pages = self._prefixes[held[n - 1]] = torch.tensor(
-                held[:n], dtype=torch.int32, device=self.block_table.device)
+            pages = torch.tensor(held[:n], dtype=torch.int32, device=self.block_table.device)
+            if self._spare.get(n):
+                pages = self._spare[n].pop().copy_(pages)
+            self._prefixes[held[n - 1]] = pages
         return pages
 
     def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
@@ -227,8 +234,8 @@ class PagedKVCache:
         (``kernels.cache_evict``), in place; ``lens_out`` (default: seq_lens itself)
         receives the new lengths.  ``max_len``, which no sequence exceeds, picks the kernel:
         ``keep + 1`` where each step gives up one slot.  ``trim`` then gives their pages
-        back.  Layers that share seq_lens: see ``evict``.  Windows are refused from then on, until a sequence
-        is released."""
+        back.  Layers that share seq_lens: see ``evict``.  Windows over a sequence are
+        refused from then on, until it is released."""
         if self.mass is None:
             raise ValueError("the cache keeps no ledger (track=True)")
         S = seq_lens.shape[0]

@@ -310,3 +310,25 @@ def test_windows_are_refused_where_slots_are_not_in_order(monkeypatch):
     for call in calls():
         with pytest.raises(Reached):
             call()
+
+
+def test_lists_of_prefixes_keep_their_memory():
+    """A captured step may hold a list's address behind the last release: lists are used again,
+    never given back, and there are no more of a length than were in use at a time."""
+    c = PagedKVCache(12, 4, 2, 16, max_seqs=4, max_pages_per_seq=6, device="cpu")
+    seen = set()
+    for i in range(6):
+        c.reserve(i % 3, 12 + 4 * (i % 2))
+        c.share(3, i % 3, 8)
+        pages = c.prefix(3, 8)
+        assert pages.tolist() == c._held[3][:2] and c.prefix(i % 3, 8) is pages
+        assert c.prefix(i % 3, 12).tolist() == c._held[i % 3][:3]
+        seen.add(pages.data_ptr())
+        c.release(i % 3)
+        assert pages.tolist() == c._held[3]         # still in use
+        c.release(3)
+    assert len(seen) == 1 and not c._prefixes
+    assert {n: len(x) for n, x in c._spare.items()} == {2: 1, 3: 1}
+    c.reserve(0, 8), c.reserve(1, 8)
+    a, b = c.prefix(0, 8), c.prefix(1, 8)
+    assert a.data_ptr() != b.data_ptr() and a.tolist() == c._held[0] and b.tolist() == c._held[1]
