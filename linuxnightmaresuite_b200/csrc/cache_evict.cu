@@ -15,10 +15,11 @@
 // by one.
 //
 // Bound by latency where few slots leave (128 sequences, one slot of 1025 each, 8 heads: 9.1 us on
-// the device, about the host's time for the call; by radix select 30), by memory where long prompts are cut: 6 of up to
-// 32768 tokens to 4096, 8 heads of 128, fp16, 76 us, 40 of them the rows that move, 256 bytes
-// each at random, read and written once at 4.3 TB/s; the rest the digits' barriers across the
-// cluster.  Digits of 11 bits took 204: counts of a cluster are 64 KB a digit through its network.
+// the device, about the host's time for the call; by radix select 30), by memory where long prompts
+// are cut: 6 of up to 32768 tokens to 4096, 8 heads of 128, fp16, 73 us, 40 of them the rows that
+// move, 256 bytes each at random, read and written once at 4.3 TB/s; the rest the digits' barriers
+// across the cluster.  Digits of 11 bits took 204: counts of a cluster are 64 KB a digit through its
+// network.
 #include <cooperative_groups.h>
 
 #include <algorithm>
